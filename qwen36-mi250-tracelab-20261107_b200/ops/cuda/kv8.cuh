@@ -1,0 +1,44 @@
+// The 8-bit KV cache's number format: rows of D e4m3 numbers with one power of two each, held as a byte biased by 127. 255 marks
+// a row that held a NaN (its data bytes are 0).
+#pragma once
+
+#include "common.cuh"
+
+namespace b200 {
+
+constexpr int KV8_PAGE = 64;
+constexpr int KV8_E_MAX = 60;
+constexpr int KV8_E_NAN = 255;
+
+// The exponent of a row whose largest magnitude is `amax`: the smallest e with amax <= 448 * 2^e, in [-60, 60]. 448 = 1.75 * 2^8.
+__device__ __forceinline__ int kv8_exponent(float amax) {
+  const uint32_t bits = __float_as_uint(amax);
+  const int e = static_cast<int>(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return max(-KV8_E_MAX, min(KV8_E_MAX, e));  // 0 and subnormal numbers: bits >> 23 is 0, far below
+}
+__device__ __forceinline__ float kv8_two_to(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+
+// The factor that an exponent byte stands for. (A byte of 0 is written by nobody; it reads as 2^-126.)
+__device__ __forceinline__ float kv8_factor(uint32_t byte) {
+  return byte == KV8_E_NAN ? __uint_as_float(0x7fffffffu) : __uint_as_float(max(byte, 1u) << 23);
+}
+
+// Two floats to two e4m3 bytes (the first in the low one), to nearest even, and to +-448 beyond it.
+__device__ __forceinline__ uint32_t kv8_pack2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// Two e4m3 bytes to two halves, exactly.
+__device__ __forceinline__ uint32_t kv8_unpack2(uint16_t two) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(two));
+  return r;
+}
+// The four bytes of a word as two pairs of halves.
+__device__ __forceinline__ void kv8_unpack4(uint32_t word, uint32_t& lo, uint32_t& hi) {
+  lo = kv8_unpack2(static_cast<uint16_t>(word));
+  hi = kv8_unpack2(static_cast<uint16_t>(word >> 16));
+}
+
+}  // namespace b200

@@ -17,9 +17,11 @@ from ctypes import c_float, c_int, c_void_p
 
 import torch
 
+from ..config import PAGE_SIZE
 from ..obs import buildlog
 from . import torch_ops
 from .build import lib_path
+from .kv8 import Kv8Layer, check_layer
 from .spans import span_tables
 
 _lib = None
@@ -53,7 +55,7 @@ def lib() -> ctypes.PyDLL:
     return _lib
 
 
-P, I, F = c_void_p, c_int, c_float
+P, I, F, L = c_void_p, c_int, c_float, ctypes.c_longlong
 
 
 class _Sig:
@@ -84,6 +86,10 @@ class _Sig:
     b200_flash_prefill = [P, P, P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, P, P, P, P]
     b200_flash_decode = [P, P, P, P, I, I, I, I, I, I, I, I, I, P, P, P, P]
     b200_attn_combine = [P, P, P, P, I, I, I, I, P]
+    b200_kv8_write = [P, L, L, P, L, L, P, P, P, I, I, I, P, P, I, I, I, I, P, P]
+    b200_kv8_read = [P, P, P, P, P, I, I, I, P, P, I, I, I, I, P, P]
+    b200_kv8_decode_run = []
+    b200_kv8_decode = [P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, P, P, P, P, P]
 
 
 def launch_count() -> int:
@@ -720,6 +726,119 @@ def flash_decode(q: torch.Tensor, gate: torch.Tensor, kv_layer: torch.Tensor, bl
     _check(L.b200_attn_combine(_ptr(part_acc), _ptr(part_ml), _ptr(gate), _ptr(out), rows, n_q, D, n_splits, _stream()),
            "attn_combine")
     return out
+
+
+# --------------------------------------------------------------------------- the 8-bit KV cache
+def _index_tables(what: str, dev: torch.device, rows: int, positions: torch.Tensor, block_tables: torch.Tensor,
+                  seq_of_row: torch.Tensor | None = None):
+    """The row indices in the types that the kernels read: int64 positions, int32 tables and sequences."""
+    if positions.shape != (rows,) or block_tables.dim() != 2 or (seq_of_row is not None and seq_of_row.shape != (rows,)):
+        raise ValueError(f"{what}: {rows} rows, but positions {tuple(positions.shape)}, page tables {tuple(block_tables.shape)}"
+                         + ("" if seq_of_row is None else f", sequences {tuple(seq_of_row.shape)}"))
+    for t in (positions, block_tables, seq_of_row):
+        if t is not None and t.device != dev:
+            raise ValueError(f"{what}: the cache is on {dev}, an index tensor on {t.device}")
+    if positions.dtype != torch.int64 or not positions.is_contiguous():
+        positions = positions.to(torch.int64).contiguous()
+    if block_tables.dtype != torch.int32 or block_tables.stride(1) != 1:
+        block_tables = block_tables.to(torch.int32).contiguous()
+    if seq_of_row is not None and (seq_of_row.dtype != torch.int32 or not seq_of_row.is_contiguous()):
+        seq_of_row = seq_of_row.to(torch.int32).contiguous()
+    return positions, block_tables, seq_of_row
+
+
+def kv8_write(layer: Kv8Layer, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, seq_of_row: torch.Tensor,
+              block_tables: torch.Tensor) -> None:
+    """Quantise rows ``k, v [T, n_kv, D]`` (bf16, rows and heads at any stride) into the pages of their sequences: row ``t`` is the
+    token at ``positions[t]`` of sequence ``seq_of_row[t]`` (``ops/kv8.py`` has the format)."""
+    pages, n_kv, D = check_layer(layer, "kv8_write")
+    T, dev = k.shape[0], layer.data.device
+    if k.shape != (T, n_kv, D) or v.shape != (T, n_kv, D) or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
+        raise ValueError(f"kv8_write: k {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} are not bf16 [{T}, {n_kv}, {D}]")
+    if k.device != dev or v.device != dev:
+        raise ValueError(f"kv8_write: the cache is on {dev}, the rows on {k.device} and {v.device}")
+    positions, block_tables, seq_of_row = _index_tables("kv8_write", dev, T, positions, block_tables, seq_of_row)
+    if k.stride(2) != 1:
+        k = k.contiguous()
+    if v.stride(2) != 1:
+        v = v.contiguous()
+    _check(lib().b200_kv8_write(
+        k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), positions.data_ptr(), seq_of_row.data_ptr(),
+        block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1], block_tables.shape[0], layer.data.data_ptr(),
+        layer.exps.data_ptr(), T, n_kv, D, pages, _ptr(err_word(dev)), _stream()), "kv8_write")
+
+
+def kv8_read(layer: Kv8Layer, positions: torch.Tensor, seq_of_row: torch.Tensor, block_tables: torch.Tensor):
+    """``k, v [T, n_kv, D]`` (bf16, exactly what the cache stands for) of the tokens at ``positions[t]`` of sequences ``seq_of_row[t]``."""
+    pages, n_kv, D = check_layer(layer, "kv8_read")
+    T, dev = positions.shape[0], layer.data.device
+    positions, block_tables, seq_of_row = _index_tables("kv8_read", dev, T, positions, block_tables, seq_of_row)
+    k = torch.empty(T, n_kv, D, dtype=torch.bfloat16, device=dev)
+    v = torch.empty_like(k)
+    _check(lib().b200_kv8_read(
+        layer.data.data_ptr(), layer.exps.data_ptr(), positions.data_ptr(), seq_of_row.data_ptr(), block_tables.data_ptr(),
+        block_tables.stride(0), block_tables.shape[1], block_tables.shape[0], k.data_ptr(), v.data_ptr(), T, n_kv, D, pages,
+        _ptr(err_word(dev)), _stream()), "kv8_read")
+    return k, v
+
+
+def _kv8_queries(what: str, q: torch.Tensor, gate: torch.Tensor, n_kv: int, D: int, dev: torch.device):
+    if q.dim() != 3 or q.shape[2] != D or q.shape[1] % n_kv or not 1 <= q.shape[1] // n_kv <= 16 or q.dtype != torch.bfloat16:
+        raise ValueError(f"{what}: q {tuple(q.shape)} {q.dtype} is not bf16 [rows, n_q, {D}] with 1 to 16 query heads for each of {n_kv} KV heads")
+    if gate.shape != (q.shape[0], q.shape[1] * D) or gate.dtype != torch.bfloat16:
+        raise ValueError(f"{what}: gate {tuple(gate.shape)} {gate.dtype} is not bf16 {(q.shape[0], q.shape[1] * D)}")
+    if q.device != dev or gate.device != dev:
+        raise ValueError(f"{what}: the cache is on {dev}, q on {q.device}, the gate on {gate.device}")
+    q = q if q.is_contiguous() else q.contiguous()
+    if q.data_ptr() % 16:
+        q = q.clone()
+    return q, gate if gate.is_contiguous() else gate.contiguous()
+
+
+def kv8_decode(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tables: torch.Tensor, positions: torch.Tensor,
+               G: int) -> torch.Tensor:
+    """``flash_decode`` over the 8-bit cache: gated attention of ``G`` rows per sequence (decode 1, verify k + 1), each over the
+    keys ``0 .. positions[row]`` of its sequence. A row's bits depend on its own position, queries and keys only, not on the batch or ``G``. A negative
+    position is a row without keys: its output is 0. Only device tensors are touched, so the call can be captured in a CUDA graph."""
+    pages, n_kv, D = check_layer(layer, "kv8_decode")
+    dev = layer.data.device
+    q, gate = _kv8_queries("kv8_decode", q, gate, n_kv, D, dev)
+    rows, n_q, _ = q.shape
+    if G < 1 or rows % G or block_tables.shape[0] < rows // G:
+        raise ValueError(f"kv8_decode: {rows} rows are not {G} for each of at most {block_tables.shape[0]} sequences")
+    positions, block_tables, _ = _index_tables("kv8_decode", dev, rows, positions, block_tables)
+    L = lib()
+    n_splits = max(1, -(-block_tables.shape[1] * PAGE_SIZE // L.b200_kv8_decode_run()))
+    part_acc = part_ml = None
+    if n_splits > 1:
+        part_acc = torch.empty(rows, n_q, n_splits, D, dtype=torch.float32, device=dev)
+        part_ml = torch.empty(rows, n_q, n_splits, 2, dtype=torch.float32, device=dev)
+    out = torch.empty(rows, n_q * D, dtype=q.dtype, device=dev)
+    _check(L.b200_kv8_decode(
+        q.data_ptr(), gate.data_ptr(), layer.data.data_ptr(), layer.exps.data_ptr(), positions.data_ptr(), block_tables.data_ptr(),
+        block_tables.stride(0), block_tables.shape[1], pages, rows // G, G, n_q, n_kv, D, n_splits, _ptr(part_acc), _ptr(part_ml),
+        out.data_ptr(), _ptr(err_word(dev)), _stream()), "kv8_decode")
+    return out
+
+
+def kv8_prefill(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tables: torch.Tensor, seg_starts: list[int],
+                seg_pos0: list[int], meta=None) -> torch.Tensor:
+    """``flash_prefill`` over the 8-bit cache: causal gated attention of ragged spans of new tokens over what their sequences' pages
+    hold, the spans' own keys included. Span ``i`` owns rows ``seg_starts[i]:seg_starts[i + 1]`` at positions ``seg_pos0[i] ..``.
+
+    ``meta``: ``(seg_starts, seg_pos0)`` as int32 device tensors that the caller keeps, of the same numbers; without it every call uploads them."""
+    pages, n_kv, D = check_layer(layer, "kv8_prefill")
+    q, gate = _kv8_queries("kv8_prefill", q, gate, n_kv, D, layer.data.device)
+    n_seg = len(seg_pos0)
+    if (len(seg_starts) != n_seg + 1 or seg_starts[0] != 0 or seg_starts[-1] != q.shape[0] or block_tables.shape[0] < n_seg
+            or any(b < a for a, b in zip(seg_starts, seg_starts[1:]))):
+        raise ValueError(f"kv8_prefill: spans {seg_starts} with {n_seg} first positions do not make {q.shape[0]} rows of at most "
+                         f"{block_tables.shape[0]} sequences")
+    starts_t, pos0_t = meta if meta is not None else (torch.tensor(x, dtype=torch.int32).to(q.device) for x in (seg_starts, seg_pos0))
+    row = torch.arange(q.shape[0], dtype=torch.int32, device=q.device)
+    seq = torch.searchsorted(starts_t[1:n_seg + 1].contiguous(), row, right=True)
+    positions = pos0_t[seq].long() + row - starts_t[seq]
+    return kv8_decode(q, gate, layer, block_tables[seq], positions, 1)
 
 
 def argmax_rows(logits: torch.Tensor) -> torch.Tensor:

@@ -17,6 +17,7 @@ import torch
 import torch.nn.functional as F
 
 from ..config import GDN_CHUNK, PAGE_SIZE
+from .kv8 import Kv8Layer, check_layer, dequantise, quantise
 
 
 # --------------------------------------------------------------------------- norms
@@ -148,6 +149,57 @@ def paged_attention(
         p = torch.softmax(s, dim=-1)
         out[a:b] = (p @ vf).transpose(0, 1).to(q.dtype)
     return out.reshape(T, n_q * D) * torch.sigmoid(gate)
+
+
+# --------------------------------------------------------------------------- the 8-bit KV cache
+def kv8_write(layer: Kv8Layer, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, seq_of_row: torch.Tensor,
+              block_tables: torch.Tensor) -> None:
+    """Quantise rows ``k, v [T, n_kv, D]`` into the pages of their sequences (``ops/kv8.py`` has the format)."""
+    check_layer(layer, "kv8_write")
+    page, at = block_tables[seq_of_row.long(), positions // PAGE_SIZE].long(), positions % PAGE_SIZE
+    for which, x in enumerate((k, v)):
+        data, exps = quantise(x)
+        layer.data.view(torch.uint8)[page, which, :, at] = data.view(torch.uint8)
+        layer.exps[page, which, :, at] = exps
+
+
+def kv8_read(layer: Kv8Layer, positions: torch.Tensor, seq_of_row: torch.Tensor, block_tables: torch.Tensor,
+             dtype: torch.dtype = torch.bfloat16):
+    """``k, v [T, n_kv, D]`` of the tokens at ``positions[t]`` of sequences ``seq_of_row[t]``."""
+    check_layer(layer, "kv8_read")
+    page, at = block_tables[seq_of_row.long(), positions // PAGE_SIZE].long(), positions % PAGE_SIZE
+    return tuple(dequantise(layer.data.view(torch.uint8)[page, which, :, at].view(torch.float8_e4m3fn),
+                            layer.exps[page, which, :, at], dtype) for which in (0, 1))
+
+
+def _kv8_attention(q, gate, layer: Kv8Layer, tables, positions) -> torch.Tensor:
+    """One row after the other: row ``t`` sees the keys ``0 .. positions[t]`` of the pages ``tables[t]``."""
+    T, n_q, D = q.shape
+    n_kv = layer.data.shape[2]
+    out = torch.zeros(T, n_q, D, dtype=q.dtype, device=q.device)
+    for t, pos in enumerate(positions.tolist()):
+        if pos < 0:
+            continue
+        at = torch.arange(pos + 1, device=q.device)
+        k, v = (x.transpose(0, 1) for x in kv8_read(layer, at, torch.zeros_like(at), tables[t : t + 1], torch.float32))
+        s = (q[t].float().view(n_kv, n_q // n_kv, D) @ k.transpose(1, 2)) * D ** -0.5
+        out[t] = (torch.softmax(s, dim=-1) @ v).reshape(n_q, D).to(q.dtype)
+    return out.reshape(T, n_q * D) * torch.sigmoid(gate)
+
+
+def kv8_decode(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tables: torch.Tensor, positions: torch.Tensor,
+               G: int) -> torch.Tensor:
+    """Gated attention of ``G`` rows per sequence over the 8-bit cache (see ``cuda_ops.kv8_decode``)."""
+    return _kv8_attention(q, gate, layer, block_tables.repeat_interleave(G, dim=0), positions)
+
+
+def kv8_prefill(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tables: torch.Tensor, seg_starts: list[int],
+                seg_pos0: list[int], meta=None) -> torch.Tensor:
+    """Causal gated attention of ragged spans over the 8-bit cache (see ``cuda_ops.kv8_prefill``)."""
+    spans = list(zip(seg_starts, seg_starts[1:], seg_pos0))
+    seq = torch.cat([torch.full((b - a,), i) for i, (a, b, _) in enumerate(spans)]).to(q.device)
+    positions = torch.cat([torch.arange(p, p + b - a) for a, b, p in spans]).to(q.device)
+    return _kv8_attention(q, gate, layer, block_tables[seq], positions)
 
 
 # --------------------------------------------------------------------------- MoE

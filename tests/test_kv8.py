@@ -1,0 +1,152 @@
+"""The 8-bit KV cache's format and its PyTorch operators, against definitions in 64 bits, on the CPU."""
+
+import math
+
+import pytest
+import torch
+
+from b200serve.ops import torch_ops as O
+from b200serve.ops.kv8 import E_BIAS, E_MAX, E_NAN, HEAD_DIMS, Kv8Layer, Kv8Pool, check_layer, dequantise, quantise
+
+
+def _e4m3_values():
+    bits = torch.arange(256, dtype=torch.uint8)
+    x = bits.view(torch.float8_e4m3fn).double()
+    return x[x.isfinite()].unique()
+
+
+def _nearest(y: float, values) -> float:
+    """The nearest e4m3 number, ties to the one with an even last bit."""
+    d = (values - y).abs()
+    best = values[d == d.min()]
+    if len(best) == 1:
+        return best.item()
+    even = [v.item() for v in best if int(v.to(torch.float32).to(torch.float8_e4m3fn).view(torch.uint8)) % 2 == 0]
+    return even[0]
+
+
+@pytest.mark.parametrize("scale", [1.0, 2.0 ** -30, 2.0 ** 40, 3e-22, 1e21])
+def test_a_row_is_held_to_the_nearest_numbers_of_the_smallest_power(scale):
+    g = torch.Generator().manual_seed(1)
+    x = (torch.randn(6, 32, generator=g, dtype=torch.float64) * scale).bfloat16()
+    data, exps = quantise(x)
+    values = _e4m3_values()
+    for row, d, e in zip(x.double(), data.double(), exps.tolist()):
+        top = row.abs().max().item()
+        want = min(range(-E_MAX, E_MAX + 1), key=lambda c: (top > 448 * 2.0 ** c, c))
+        if top > 448 * 2.0 ** E_MAX:
+            want = E_MAX
+        assert e == want + E_BIAS
+        for a, b in zip(row.tolist(), d.tolist()):
+            y = max(-448.0, min(448.0, math.ldexp(a, -want)))
+            assert b == _nearest(y, values)
+
+
+def test_rows_at_the_edges_of_a_power():
+    x = torch.zeros(6, 32)
+    for i, top in enumerate([448.0, 449.0, 896.0, 1.75, 0.0, 2.0 ** -100]):
+        x[i, 3] = -top
+    data, exps = quantise(x)
+    assert (exps.int() - E_BIAS).tolist() == [0, 1, 1, -8, -E_MAX, -E_MAX]
+    assert data[0, 3].float() == -448 and data[1, 3].float() == -224 and data[3, 3].float() == -448
+    assert (data[4].float() == 0).all() and (data[5].float() == 0).all()
+
+
+def test_nan_marks_the_row_and_infinity_is_the_largest_number():
+    x = torch.ones(3, 64)
+    x[0, 7], x[1, 9], x[1, 10] = float("nan"), float("inf"), -float("inf")
+    data, exps = quantise(x)
+    assert exps.tolist() == [E_NAN, E_MAX + E_BIAS, 127 - 8]
+    assert (data[0].float() == 0).all()
+    back = dequantise(data, exps, torch.float32)
+    assert back[0].isnan().all() and back[1, 9] == 448 * 2.0 ** E_MAX and back[1, 10] == -448 * 2.0 ** E_MAX
+    assert (back[2] == 1).all()
+
+
+def test_a_row_comes_back_exactly_and_stays():
+    """What was held once is held again without a change: e4m3 numbers times a power of two are bf16 numbers."""
+    g = torch.Generator().manual_seed(2)
+    data, exps = quantise(torch.randn(50, 128, generator=g).bfloat16() * 3.7)
+    x = dequantise(data, exps, torch.bfloat16)
+    assert torch.equal(x.float(), dequantise(data, exps, torch.float32))
+    again = quantise(x)
+    assert torch.equal(again[0].view(torch.uint8), data.view(torch.uint8)) and torch.equal(again[1], exps)
+
+
+def _layer(pages=9, n_kv=2, D=32, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return Kv8Layer(*quantise(torch.randn(pages, 2, n_kv, 64, D, generator=g)))
+
+
+def test_write_and_read_by_page_table():
+    layer = _layer()
+    before = layer.data.clone().view(torch.uint8), layer.exps.clone()
+    tables = torch.tensor([[3, 5], [7, 1]], dtype=torch.int32)
+    seq, pos = torch.tensor([0, 0, 1, 1]), torch.tensor([63, 64, 0, 127])
+    g = torch.Generator().manual_seed(5)
+    k, v = torch.randn(4, 2, 32, generator=g), torch.randn(4, 2, 32, generator=g) * 9
+    O.kv8_write(layer, k, v, pos, seq, tables)
+    rk, rv = O.kv8_read(layer, pos, seq, tables)
+    for got, want in ((rk, k), (rv, v)):
+        assert torch.equal(got.float(), dequantise(*quantise(want), torch.float32))
+    changed = (layer.exps != before[1]) | (layer.data.view(torch.uint8) != before[0]).any(-1)
+    places = {(int(p), int(o)) for p, _, _, o in changed.nonzero()}
+    assert places == {(3, 63), (5, 0), (7, 0), (1, 63)}
+
+
+@pytest.mark.parametrize("n_q,n_kv,D,G", [(4, 1, 32, 1), (6, 3, 64, 3)])
+def test_attention_is_the_formula(n_q, n_kv, D, G):
+    layer = _layer(n_kv=n_kv, D=D)
+    tables = torch.tensor([[3, 5], [7, 1]], dtype=torch.int32)
+    last = [70, 3]
+    positions = torch.tensor([p + i - (G - 1) for p in last for i in range(G)])
+    g = torch.Generator().manual_seed(7)
+    q, gate = torch.randn(2 * G, n_q, D, generator=g), torch.randn(2 * G, n_q * D, generator=g)
+    got = O.kv8_decode(q, gate, layer, tables, positions, G).view(2 * G, n_q, D)
+    kv = dequantise(layer.data, layer.exps, torch.float32).double()
+    for r in range(2 * G):
+        pages = tables[r // G].long()
+        for h in range(n_q):
+            k, v = (kv[pages, i, h // (n_q // n_kv)].reshape(-1, D)[: positions[r] + 1] for i in (0, 1))
+            p = torch.softmax(k @ q[r, h].double() / math.sqrt(D), 0)
+            want = (p @ v) * torch.sigmoid(gate.double().view(2 * G, n_q, D)[r, h])
+            assert (got[r, h].double() - want).abs().max() < 1e-5
+
+
+def test_prefill_is_decode_row_by_row_and_a_row_without_keys_is_zero():
+    layer = _layer()
+    tables = torch.tensor([[3, 5], [7, 1]], dtype=torch.int32)
+    g = torch.Generator().manual_seed(8)
+    starts, pos0 = [0, 5, 5 + 70], [60, 0]
+    q, gate = torch.randn(75, 4, 32, generator=g), torch.randn(75, 128, generator=g)
+    got = O.kv8_prefill(q, gate, layer, tables, starts, pos0)
+    for r, (s, pos) in ((0, (0, 60)), (4, (0, 64)), (5, (1, 0)), (74, (1, 69))):
+        one = O.kv8_decode(q[r : r + 1], gate[r : r + 1], layer, tables[s : s + 1], torch.tensor([pos]), 1)
+        assert torch.equal(got[r : r + 1], one)
+    none = O.kv8_decode(q[:2], gate[:2], layer, tables, torch.tensor([-1, 5]), 1)
+    assert (none[0] == 0).all() and (none[1] != 0).any()
+
+
+def test_layers_that_do_not_fit_are_refused():
+    data, exps = _layer()
+    for bad in (Kv8Layer(data.view(torch.uint8), exps), Kv8Layer(data, exps.int()), Kv8Layer(data[:3], exps), Kv8Layer(data[..., :24], exps),
+                Kv8Layer(data[::2], exps[::2]), Kv8Layer(data[:, :1], exps[:, :1]),
+                Kv8Layer(data.transpose(2, 3).contiguous(), exps.transpose(2, 3).contiguous())):
+        with pytest.raises(ValueError, match="kv8"):
+            check_layer(bad, "kv8")
+    assert check_layer(Kv8Layer(data, exps), "kv8") == (9, 2, 32)
+    with pytest.raises(ValueError):
+        Kv8Pool(1, 4, 2, 48, "cpu")
+
+
+@pytest.mark.parametrize("D", HEAD_DIMS)
+def test_pool_pages(D):
+    pool = Kv8Pool(3, 5, 2, D, "cpu")
+    assert pool.page_bytes == sum(t[:, 0].numel() for t in (pool.data, pool.exps))
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(1, 2, D, generator=g)
+    O.kv8_write(pool[1], x, 2 * x, torch.tensor([5]), torch.tensor([0]), torch.tensor([[4]]))
+    pool.copy_page(4, 2)
+    k, v = O.kv8_read(pool[1], torch.tensor([5]), torch.tensor([0]), torch.tensor([[2]]))
+    assert torch.equal(v.float(), 2 * k.float()) and (k != 0).any()
+    assert (O.kv8_read(pool[0], torch.tensor([5]), torch.tensor([0]), torch.tensor([[2]]))[0] == 0).all()
