@@ -7,12 +7,13 @@
 // sum_j w_j 2^-b_j. So what the matrix instructions get are the stored numbers as halves (exact) and weights below 2^15.
 //
 // Bound: the cache's bytes, 2 (D + 1) per token and KV head. A context is cut into runs of RUN keys at fixed places, so what a row's
-// result is put together from depends on its own position only, never on the batch; a persistent CTA per SM takes runs in turn. In a run each
-// of the eight warps takes every eighth slab of 16 keys, brought by TMA into a ring of the warp's own that it refills itself, the
-// next runs' slabs included: no barrier stands between a warp and its data, and the finish of a run (the one place where the warps
-// meet) has the next runs' loads on their way. The products are m16n8k16 with keys (S = K Q^T) or dims (O = V^T P) as the 16 rows and query
-// columns as the 8: one token of one KV head's eight query heads fills the columns, where a tcgen05 tile would be 8 rows of 64.
-// The stored bytes become halves in registers, behind ldmatrix.
+// result is put together from depends on its own position only, never on the batch; a persistent CTA per SM takes runs in turn. Blocks of 128 keys
+// come into a ring by TMA, the next runs' blocks ahead of this one's end. On a block the eight warps first take 16 keys each
+// (S = K Q^T, maximum, weights), then D / 8 dims each over all keys (O += V^T P): a warp's part of the output is 2 tiles of 16 dims,
+// so nothing of the output is ever exchanged, only maxima and weights, 16 bytes per key. (With all dims of every eighth slab in
+// each warp, the warps' outputs were added up at each run's end, which took more instructions than the run: 74 us for 128 sequences of about 1,060.)
+// The products are m16n8k16 with keys or dims as the 16 rows and query columns as the 8: one token of one KV head's eight query heads
+// fills the columns, where a tcgen05 tile would be 8 rows of 64. The stored bytes become halves in registers, behind ldmatrix.
 #include <cuda_fp16.h>
 
 #include "kv8.cuh"
@@ -20,8 +21,9 @@
 namespace b200 {
 
 constexpr int K8D_RUN = 512;                    // keys of a run: part of the numerics
-constexpr int K8D_WARPS = 8;
-constexpr int K8D_SLAB = 16;                    // keys of a slab
+constexpr int K8D_WARPS = 8;                    // that compute
+constexpr int K8D_SLAB = 16;                    // keys of a warp's scores
+constexpr int K8D_BLOCK = K8D_WARPS * K8D_SLAB; // keys of a ring stage: two pages
 constexpr int K8D_MAX_SEQS = 1024;              // of one launch
 constexpr float K8D_LIFT = 7.0f;                // weights are 2^LIFT at the maximum: halves reach down to 2^-24
 constexpr float K8D_LAZY = 8.0f;                // the maximum moves when it grew by more: 2^(LIFT + LAZY) is below the halves' 65504
@@ -37,25 +39,24 @@ struct Kv8DecodeParams {
   float2* part_ml;           // [rows, n_q, n_splits]: maximum (log 2) and sum
   int B, G, max_pages, width, num_pages, n_q, n_kv, group, n_splits;
   int rows_per_unit, units_per_seq;  // query rows whose heads fill a unit's columns; units that cover G rows
+  int inv_group;             // column * inv_group >> 16 is column / group, for columns up to 32 of groups up to 16
   float scale_log2;
   int* err;
 };
 
-template <int D>
+template <int D, int NT>
 struct Kv8DecodeCfg {
   static constexpr int ROWB = D < 128 ? D : 128;           // bytes of a row in one swizzled block
   static constexpr int DB = D / ROWB;
-  static constexpr int TILE = K8D_SLAB * D;                // one of K or V
-  static constexpr int STAGE = 2 * TILE;
-  static constexpr int ST = D == 256 ? 3 : D == 128 ? 6 : 8;
-  static constexpr int RING = K8D_WARPS * ST * STAGE;
-  static constexpr int EXPS = K8D_WARPS * ST * 2 * K8D_SLAB;
-  static constexpr int HALF = D < 64 ? D : 64;             // dims that the finish of a run exchanges at a time
-  static constexpr int COL = HALF + 4;                     // floats between its columns: the pad spreads them over the banks
-  static constexpr int EXCH = K8D_WARPS * 8 * COL * 4;
-  static constexpr int BARS = K8D_WARPS * ST * 8;
-  static constexpr int TABLE = (2 * K8D_MAX_SEQS + 4) * 4;
-  static constexpr int SMEM = RING + EXCH + EXPS + BARS + 256;
+  static constexpr int TILE = KV8_PAGE * D;                // a page's keys or values
+  static constexpr int SLOT = 2 * TILE;                    // of the ring: the keys of a block or its values
+  static constexpr int CTAS = NT == 1 ? 2 : 1;             // per SM: one column tile's registers leave room for sixteen warps
+  static constexpr int SLOTS = (D == 256 ? 3 : D == 128 ? 6 : 8) * (D == 256 && NT > 1 ? 2 : 1);
+  static constexpr int EXPS = 4 * KV8_PAGE;                // exponents of a block's keys and values, with its keys
+  static constexpr int SMEM = SLOTS * (SLOT + EXPS);
+  static constexpr int TILES = D / 16;                     // output tiles of 16 dims
+  static constexpr int PER = TILES > K8D_WARPS ? TILES / K8D_WARPS : 1;  // of a warp
+  static constexpr int SPLIT = TILES < K8D_WARPS ? K8D_WARPS / TILES : 1;  // warps that share a tile, a part of the keys each
 };
 
 __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t* r) {
@@ -95,36 +96,35 @@ __device__ __forceinline__ int kv8_find(const int* first, int B, int x) {
   return lo;
 }
 
-// A unit is (sequence, group of its query rows, KV head, run). Walked by a warp: the slabs of the CTA's units, one after the other.
-struct Kv8Walk {
-  int id, b, rg, kh, z;
-  int slab, slabs;     // this warp's next slab of the unit, the unit's slabs
-  int page;            // lane i: the table's entry i of the run
+// A unit is (sequence, group of its query rows, KV head, run). keys: of the run, up to the last that a row of the unit sees.
+struct Kv8Unit {
+  int seq, kh, z, row0, rows, keys;
 };
 
 template <int D, int NT>
-__global__ void __launch_bounds__(32 * K8D_WARPS, 1)
+__global__ void __launch_bounds__(32 * K8D_WARPS, Kv8DecodeCfg<D, NT>::CTAS)
 kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, Kv8DecodeParams p) {
-  using C = Kv8DecodeCfg<D>;
-  constexpr int ST = C::ST, CHUNKS = D / 16, COLS = 8 * NT;
+  using C = Kv8DecodeCfg<D, NT>;
+  constexpr int SLOTS = C::SLOTS, CHUNKS = D / 16, COLS = 8 * NT, SLABS = K8D_WARPS, DI = (D + 127) / 128;
   extern __shared__ __align__(1024) uint8_t smem_k8[];
   if (smem_u32(smem_k8) & 1023u) {  // the swizzled tiles need this alignment
     if (threadIdx.x == 0) atomicCAS(p.err, 0, ERR_BAD_INDEX);
     return;
   }
-  float* exch = reinterpret_cast<float*>(smem_k8 + C::RING);
-  uint8_t* s_exps = smem_k8 + C::RING + C::EXCH;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(s_exps + C::EXPS);
-  __shared__ int s_first[K8D_MAX_SEQS + 1];   // runs of the sequences before
-  __shared__ float s_m[K8D_WARPS][COLS], s_l[K8D_WARPS][COLS];
+  uint8_t* s_exps = smem_k8 + SLOTS * C::SLOT;
+  __shared__ __align__(8) uint64_t full[SLOTS];
+  __shared__ int s_first[K8D_MAX_SEQS + 1];            // runs of the sequences before
+  __shared__ Kv8Unit s_unit[64];                       // this CTA's units, a ring in two halves
+  __shared__ __align__(16) float s_max[SLABS][COLS], s_sum[SLABS][COLS];  // read two columns at a time
+  __shared__ __align__(8) uint2 s_w[SLABS][NT][32];    // weights of a block, as the products' second operand
+  __shared__ __align__(8) uint2 s_q[NT][CHUNKS][32];   // queries, likewise
+  __shared__ float s_scale[COLS];
+  __shared__ __align__(16) float s_o[C::SPLIT > 1 ? K8D_WARPS : 1][C::SPLIT > 1 ? NT * 4 : 1][32];
   __shared__ int s_abort;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  uint8_t* ring = smem_k8 + warp * ST * C::STAGE;
-  uint8_t* ring_exps = s_exps + warp * ST * 2 * K8D_SLAB;
-  uint64_t* full = bars + warp * ST;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < K8D_WARPS * ST; ++i) mbar_init(&bars[i], 1);
+    for (int i = 0; i < SLOTS; ++i) mbar_init(&full[i], 1);
     s_abort = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tm);
@@ -132,7 +132,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, Kv8DecodeParams p) {
   pdl_wait();
   pdl_launch();
   const int most = min(p.width, p.n_splits * (K8D_RUN / KV8_PAGE)) * KV8_PAGE;  // keys that the tables can name
-  const auto length = [&](int row) { return max(0, min(static_cast<int>(min(p.positions[row], static_cast<int64_t>(most))) + 1, most)); };
+  const auto length = [&](int row) { return max(0, min(static_cast<int>(min(__ldg(p.positions + row), static_cast<int64_t>(most))) + 1, most)); };
   for (int b = threadIdx.x; b < p.B; b += blockDim.x) {
     int len = 0;
     for (int i = 0; i < p.G; ++i) len = max(len, length(b * p.G + i));
@@ -155,293 +155,360 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, Kv8DecodeParams p) {
   }
   __syncthreads();
   const int per_run = p.n_kv * p.units_per_seq, total = s_first[p.B] * per_run;
+  const int n_units = (total - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);  // of this CTA
   volatile int* abort_flag = &s_abort;
-
-  const auto enter = [&](Kv8Walk& w) {  // the unit of w.id
-    const int run = w.id / per_run, x = w.id % per_run;
-    w.rg = x % p.units_per_seq;
-    w.kh = x / p.units_per_seq;
-    w.b = kv8_find(s_first, p.B, run);
-    w.z = run - s_first[w.b];
+  const auto describe = [&](int j) {  // unit j of this CTA, by one lane
+    if (j >= n_units) return;
+    Kv8Unit u;
+    const int id = blockIdx.x + j * gridDim.x, run = id / per_run, x = id % per_run, rg = x % p.units_per_seq;
+    u.kh = x / p.units_per_seq;
+    u.seq = kv8_find(s_first, p.B, run);
+    u.z = run - s_first[u.seq];
+    u.row0 = u.seq * p.G + rg * p.rows_per_unit;
+    u.rows = min(p.rows_per_unit, (u.seq + 1) * p.G - u.row0);
     int len = 0;
-    const int r0 = w.b * p.G + w.rg * p.rows_per_unit, r1 = min(r0 + p.rows_per_unit, (w.b + 1) * p.G);
-    for (int r = r0; r < r1; ++r) len = max(len, length(r));
-    w.slabs = (max(0, min(K8D_RUN, len - w.z * K8D_RUN)) + K8D_SLAB - 1) / K8D_SLAB;
-    w.slab = warp;
+    for (int r = 0; r < u.rows; ++r) len = max(len, length(u.row0 + r));
+    u.keys = max(0, min(K8D_RUN, len - u.z * K8D_RUN));
+    s_unit[j % 64] = u;
   };
-  const auto pages = [&](Kv8Walk& w) {
-    w.page = 0;
-    const int n = (w.slabs + KV8_PAGE / K8D_SLAB - 1) / (KV8_PAGE / K8D_SLAB);
-    if (lane < n) w.page = p.tables[static_cast<size_t>(w.b) * p.max_pages + w.z * (K8D_RUN / KV8_PAGE) + lane];
-    if (w.page < 0 || w.page >= p.num_pages) { atomicCAS(p.err, 0, ERR_BAD_INDEX); w.page = 0; }
-  };
-  // The loads run ahead of the work by the ring's stages, into the next units.
-  Kv8Walk ahead;
-  ahead.id = blockIdx.x;
-  const auto seek = [&]() {  // the first unit from ahead.id on that has a slab for this warp
-    for (; ahead.id < total; ahead.id += gridDim.x) {
-      enter(ahead);
-      if (ahead.slab < ahead.slabs) { pages(ahead); return; }
-    }
-  };
-  int issued = 0;
-  const auto issue = [&]() {
-    if (ahead.id >= total) return;
-    const int page = __shfl_sync(0xffffffffu, ahead.page, ahead.slab / (KV8_PAGE / K8D_SLAB));
-    if (lane == 0) {
-      const int s = issued % ST;
-      const int row = (page * 2 * p.n_kv + ahead.kh) * KV8_PAGE + ahead.slab % (KV8_PAGE / K8D_SLAB) * K8D_SLAB;
-      const int vrow = row + p.n_kv * KV8_PAGE;
-      mbar_expect_tx(&full[s], C::STAGE + 2 * K8D_SLAB);
-      uint8_t* at = ring + s * C::STAGE;
-      tma_load_3d(at, &tm, &full[s], 0, row, 0);
-      tma_load_3d(at + C::TILE, &tm, &full[s], 0, vrow, 0);
-      bulk_load(ring_exps + s * 2 * K8D_SLAB, p.exps + row, K8D_SLAB, &full[s]);
-      bulk_load(ring_exps + s * 2 * K8D_SLAB + K8D_SLAB, p.exps + vrow, K8D_SLAB, &full[s]);
-    }
-    ++issued;
-    ahead.slab += K8D_WARPS;
-    if (ahead.slab >= ahead.slabs) { ahead.id += gridDim.x; seek(); }
-  };
-  seek();
-  for (int i = 0; i < ST; ++i) issue();
+  if (warp < 2) describe(threadIdx.x);
+  __syncthreads();
 
-  int used = 0;  // slabs consumed
-  bool ok = true;
-  // shared-memory offset of 16 bytes of a swizzled tile: row r, chunk c
+  // ---------------- loads, by the last warp. The ring takes a block's keys, then its values; by the first meeting on block k all warps have
+  // read the keys of block k and the values of block k - 1. The page numbers of a unit are read a unit ahead.
+  struct { int j, kh, pages, pg, ids; } cur = {}, nxt = {};
+  int issued = 0;  // slots asked for
+  const auto look = [&](decltype(cur)& w, int j, int limit) {  // the first unit from j on that has keys, below `limit`
+    for (; j < limit && j < n_units; ++j) {
+      const Kv8Unit& u = s_unit[j % 64];
+      if (u.keys == 0) continue;
+      w.kh = u.kh;
+      w.pg = 0;
+      w.pages = (u.keys + KV8_PAGE - 1) / KV8_PAGE;
+      w.ids = 0;
+      if (lane < w.pages) w.ids = __ldg(p.tables + static_cast<size_t>(u.seq) * p.max_pages + u.z * (K8D_RUN / KV8_PAGE) + lane);
+      break;
+    }
+    w.j = j;
+    return j < limit && j < n_units;
+  };
+  bool have = false, have_next = false;  // cur, nxt hold a unit
+  const auto issue = [&](int upto, int limit) {
+    while (issued < upto) {
+      if (!have) { have = have_next; cur = nxt; have_next = false; }
+      if (!have) { have = look(cur, cur.j, limit); nxt.j = cur.j + have; }
+      if (!have_next) have_next = look(nxt, max(nxt.j, cur.j + have), limit);
+      if (!have) { cur.j = nxt.j; return; }
+      const int s = issued % SLOTS, of = min(2, cur.pages - cur.pg), values = issued & 1;
+      int page = __shfl_sync(0xffffffffu, cur.ids, cur.pg + (lane & 1));
+      if (lane == 0) mbar_expect_tx(&full[s], of * (C::TILE + (values ? 0 : 2 * KV8_PAGE)));
+      __syncwarp();
+      if (lane < 4 && (lane & 1) < of) {  // lanes 0, 1: the tiles and their keys' exponents, 2, 3: the values' exponents
+        if (page < 0 || page >= p.num_pages) { atomicCAS(p.err, 0, ERR_BAD_INDEX); page = 0; }
+        const int row = ((page * 2 + (lane >> 1)) * p.n_kv + cur.kh) * KV8_PAGE;
+        if (lane < 2) tma_load_3d(smem_k8 + s * C::SLOT + lane * C::TILE, &tm, &full[s], 0, row + values * p.n_kv * KV8_PAGE, 0);
+        if (!values) bulk_load(s_exps + s * C::EXPS + lane * KV8_PAGE, p.exps + row, KV8_PAGE, &full[s]);
+      }
+      ++issued;
+      if (values) {
+        cur.pg += 2;
+        if (cur.pg >= cur.pages) { have = false; cur.j = nxt.j; }
+      }
+    }
+  };
+  if (warp == K8D_WARPS - 1) issue(SLOTS, 64);
+
+  // shared-memory offset of 16 bytes of a page's swizzled tile: row r, chunk c
   const auto tile_at = [&](uint32_t tile, int r, int c) {
     constexpr int PER = C::ROWB / 16;  // chunks of a block's row
     const int byte = r * C::ROWB;
-    return tile + (c / PER) * (K8D_SLAB * C::ROWB) + byte + (((c % PER) ^ ((byte >> 7) & (PER - 1))) << 4);
+    return tile + (c / PER) * (KV8_PAGE * C::ROWB) + byte + (((c % PER) ^ ((byte >> 7) & (PER - 1))) << 4);
   };
+  const int tile0 = warp % C::TILES * C::PER, part = warp / C::TILES;  // this warp's output tiles, and which part of the keys
+  bool ok = true;
+  int n = 0;  // blocks so far: their keys are in slot 2 n, their values in 2 n + 1
 
-  for (int id = blockIdx.x; id < total; id += gridDim.x) {
-    Kv8Walk u;
-    u.id = id;
-    enter(u);
-    const int row0 = u.b * p.G + u.rg * p.rows_per_unit;
-    const int n_rows = min(p.rows_per_unit, (u.b + 1) * p.G - row0), n_cols = n_rows * p.group;
-    // ---- queries: thread (g, t) holds dims 16 c + 4 t .. + 3 of column g, as halves with the column's largest number in [2^10, 2^11)
-    uint32_t qf[NT][CHUNKS][2];
-    float qscale[NT][2];   // columns 2 t, 2 t + 1: what takes the product to log-2 scores
-    int last[NT][2];       // ... position of the last visible key
+  const auto column = [&](int col, int& row, int& head) { row = col * p.inv_group >> 16; head = col - row * p.group; };
+  uint2 qnext[NT][DI];   // the next unit's queries, a warp a column
+  const auto fetch = [&](const Kv8Unit& u) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int col = n * 8 + g;
-      const bool real = col < n_cols;
-      const bf16* src = p.q + (static_cast<size_t>(row0 + (real ? col / p.group : 0)) * p.n_q + u.kh * p.group + (real ? col % p.group : 0)) * D + t * 4;
-      uint2 raw[CHUNKS];
+    for (int n8 = 0; n8 < NT; ++n8) {
+      int row, head;
+      column(n8 * 8 + warp, row, head);
+      const bf16* src = p.q + (static_cast<size_t>(u.row0 + row) * p.n_q + u.kh * p.group + head) * D + lane * 4;
 #pragma unroll
-      for (int c = 0; c < CHUNKS; ++c) raw[c] = *reinterpret_cast<const uint2*>(src + c * 16);
+      for (int i = 0; i < DI; ++i)
+        qnext[n8][i] = row < u.rows && lane * 4 + i * 128 < D ? *reinterpret_cast<const uint2*>(src + i * 128) : make_uint2(0u, 0u);
+    }
+  };
+  if (n_units > 0) fetch(s_unit[0]);
+
+  for (int j = 0; j < n_units; ++j) {
+    const Kv8Unit u = s_unit[j % 64];
+    const int n_cols = u.rows * p.group;
+    if (warp == K8D_WARPS - 1) issue(2 * n + SLOTS, j / 32 * 32 + 32);
+    // ---- queries as halves with the column's largest number in [2^10, 2^11), in the order of the products' second operand: lane
+    // (column % 8, t) holds dims 16 c + 4 t .. + 3 of chunk c
+#pragma unroll
+    for (int n8 = 0; n8 < NT; ++n8) {
+      float x[DI][4];
       float top = 0.f;
       bool bad = false;
 #pragma unroll
-      for (int c = 0; c < CHUNKS; ++c) {
-        const __nv_bfloat162* e = reinterpret_cast<const __nv_bfloat162*>(&raw[c]);
+      for (int i = 0; i < DI; ++i) {
+        const __nv_bfloat162* e = reinterpret_cast<const __nv_bfloat162*>(&qnext[n8][i]);
         const float2 a = __bfloat1622float2(e[0]), b = __bfloat1622float2(e[1]);
-        top = fmaxf(fmaxf(top, fmaxf(fabsf(a.x), fabsf(a.y))), fmaxf(fabsf(b.x), fabsf(b.y)));
-        bad |= !(fabsf(a.x) <= 3.5e38f && fabsf(a.y) <= 3.5e38f && fabsf(b.x) <= 3.5e38f && fabsf(b.y) <= 3.5e38f);
+        x[i][0] = a.x; x[i][1] = a.y; x[i][2] = b.x; x[i][3] = b.y;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) { top = fmaxf(top, fabsf(x[i][k])); bad |= !(fabsf(x[i][k]) <= 3.4e38f); }
       }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      top = warp_max(top);
       const int e = max(-110, min(110, static_cast<int>(__float_as_uint(top) >> 23) - 127 - 10));
       const float f = kv8_two_to(-e);
 #pragma unroll
-      for (int c = 0; c < CHUNKS; ++c) {
-        const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&raw[c]);
-        const float2 a = __bfloat1622float2(x[0]), b = __bfloat1622float2(x[1]);
-        const __half2 lo = __floats2half2_rn(a.x * f, a.y * f), hi = __floats2half2_rn(b.x * f, b.y * f);
-        qf[n][c][0] = *reinterpret_cast<const uint32_t*>(&lo);
-        qf[n][c][1] = *reinterpret_cast<const uint32_t*>(&hi);
+      for (int i = 0; i < DI; ++i) {
+        if (lane * 4 + i * 128 < D) {
+          const __half2 lo = __floats2half2_rn(x[i][0] * f, x[i][1] * f), hi = __floats2half2_rn(x[i][2] * f, x[i][3] * f);
+          s_q[n8][i * 8 + lane / 4][warp * 4 + lane % 4] = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+        }
       }
       // a NaN or an infinity anywhere in the column: all its scores are NaN
-      const uint32_t bads = __ballot_sync(0xffffffffu, bad);
-      const float mine = (bads >> (lane & 28)) & 15u ? __uint_as_float(0x7fffffffu) : kv8_two_to(e) * p.scale_log2;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int c = n * 8 + 2 * t + j;
-        qscale[n][j] = __shfl_sync(0xffffffffu, mine, (2 * t + j) * 4);
-        last[n][j] = c < n_cols ? length(row0 + c / p.group) - 1 : -1;
-      }
+      const bool any = __any_sync(0xffffffffu, bad);
+      if (lane == 0) s_scale[n8 * 8 + warp] = any ? __uint_as_float(0x7fffffffu) : kv8_two_to(e) * p.scale_log2;
     }
-    float o[NT][CHUNKS][4];
-    float m[NT][2], l[NT][2];
+    int len[NT][2];        // columns 2 t, 2 t + 1: keys of their rows (0: no such column)
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+    for (int n8 = 0; n8 < NT; ++n8)
 #pragma unroll
-      for (int c = 0; c < CHUNKS; ++c) o[n][c][0] = o[n][c][1] = o[n][c][2] = o[n][c][3] = 0.f;
-      m[n][0] = m[n][1] = -INFINITY;
-      l[n][0] = l[n][1] = 0.f;
+      for (int k = 0; k < 2; ++k) {
+        int row, head;
+        column(n8 * 8 + 2 * t + k, row, head);
+        len[n8][k] = row < u.rows ? length(u.row0 + row) : 0;
+      }
+    if (j + 1 < n_units) fetch(s_unit[(j + 1) % 64]);
+    __syncthreads();
+    uint2 qf[NT][CHUNKS];
+    float qscale[NT][2];   // what takes the product to log-2 scores
+    int last[NT][2];       // last visible key of the run
+    float m[NT][2], l[NT][2], o[NT][C::PER][4];
+#pragma unroll
+    for (int n8 = 0; n8 < NT; ++n8) {
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c) qf[n8][c] = s_q[n8][c][lane];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        qscale[n8][k] = s_scale[n8 * 8 + 2 * t + k];
+        last[n8][k] = len[n8][k] - 1 - u.z * K8D_RUN;
+        m[n8][k] = -INFINITY;
+        l[n8][k] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < C::PER; ++i) o[n8][i][0] = o[n8][i][1] = o[n8][i][2] = o[n8][i][3] = 0.f;
     }
 
-    for (int slab = u.slab; slab < u.slabs; slab += K8D_WARPS, ++used) {
-      const int s = used % ST;
-      ok = ok && mbar_wait_warp(&full[s], (used / ST) & 1, p.err, ERR_WAIT_FULL, abort_flag);
-      if (!ok) break;
-      const uint32_t ktile = smem_u32(ring + s * C::STAGE), vtile = ktile + C::TILE;
-      // ---- scores: S[key, column], keys g and g + 8 of the slab
-      float sc[NT][2][4];  // two chains of products
+    for (int key0 = 0; key0 < u.keys; key0 += K8D_BLOCK, ++n) {
+      const int slabs = min(SLABS, (u.keys - key0 + K8D_SLAB - 1) / K8D_SLAB);
+      const bool mine = warp < slabs;
+      const int ks = 2 * n % SLOTS, vs = (2 * n + 1) % SLOTS;
+      ok = ok && mbar_wait_warp(&full[ks], (2 * n / SLOTS) & 1, p.err, ERR_WAIT_FULL, abort_flag);
+      // ---- scores of this warp's slab: S[key, column], keys g and g + 8
+      float y[NT][2][2];  // [key][column 2 t, 2 t + 1]
+      float vi[2];
+      bool grown = false;
+      if (ok && mine) {
+        float sc[NT][2][4];  // two chains of products
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+        for (int n8 = 0; n8 < NT; ++n8)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sc[n][0][j] = sc[n][1][j] = 0.f;
+          for (int k = 0; k < 4; ++k) sc[n8][0][k] = sc[n8][1][k] = 0.f;
+        const uint32_t ktile = smem_u32(smem_k8 + ks * C::SLOT) + warp / 4 * C::TILE;
 #pragma unroll
-      for (int c = 0; c < CHUNKS; c += 2) {
-        uint32_t r[4];
-        ldmatrix4(tile_at(ktile, lane & 15, c + (lane >> 4)), r);
+        for (int c = 0; c < CHUNKS; c += 2) {
+          uint32_t r[4];
+          ldmatrix4(tile_at(ktile, warp % 4 * K8D_SLAB + (lane & 15), c + (lane >> 4)), r);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t a0, a1, a2, a3;
-          kv8_unpack4(r[2 * h], a0, a2);
-          kv8_unpack4(r[2 * h + 1], a1, a3);
+          for (int h = 0; h < 2; ++h) {
+            uint32_t a0, a1, a2, a3;
+            kv8_unpack4(r[2 * h], a0, a2);
+            kv8_unpack4(r[2 * h + 1], a1, a3);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma_f16(sc[n][h], a0, a1, a2, a3, qf[n][c + h][0], qf[n][c + h][1]);
-        }
-      }
-      const uint8_t* ex = ring_exps + s * 2 * K8D_SLAB;
-      float kf[2], vb[2], vi[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint32_t vbyte = ex[K8D_SLAB + g + 8 * i];
-        kf[i] = kv8_factor(ex[g + 8 * i]);
-        vb[i] = vbyte == KV8_E_NAN ? __uint_as_float(0x7fffffffu) : static_cast<float>(static_cast<int>(vbyte) - 127);
-        vi[i] = kv8_two_to(max(-126, 127 - static_cast<int>(vbyte)));
-      }
-      const int key = u.z * K8D_RUN + slab * K8D_SLAB + g;
-      uint32_t pw[NT][2];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float y[2][2];  // [key g, g + 8][column 2 t, 2 t + 1]
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float raw = (sc[n][0][2 * i + j] + sc[n][1][2 * i + j]) * qscale[n][j];
-            y[i][j] = key + 8 * i <= last[n][j] ? fmaf(raw, kf[i], vb[i]) : -INFINITY;
-          }
-        float w[2][2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float mx = fmaxf(y[0][j], y[1][j]);
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          float f = 1.f;
-          if (mx > m[n][j] + K8D_LAZY) {
-            f = ex2(m[n][j] - mx);  // 0 at the first key
-            m[n][j] = mx;
-            l[n][j] *= f;
-          }
-          const float base = m[n][j] == -INFINITY ? 0.f : m[n][j] - K8D_LIFT;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            w[i][j] = ex2(y[i][j] - base);
-            l[n][j] = fmaf(w[i][j], vi[i], l[n][j]);
-          }
-          if (__any_sync(0xffffffffu, f != 1.f)) {
-#pragma unroll
-            for (int c = 0; c < CHUNKS; ++c) { o[n][c][j] *= f; o[n][c][2 + j] *= f; }
+            for (int n8 = 0; n8 < NT; ++n8) mma_f16(sc[n8][h], a0, a1, a2, a3, qf[n8][c + h].x, qf[n8][c + h].y);
           }
         }
+        const uint8_t* ex = s_exps + ks * C::EXPS + warp * K8D_SLAB + g;
+        float kf[2], vb[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const __half2 two = __floats2half2_rn(w[i][0], w[i][1]);
-          pw[n][i] = movmatrix(*reinterpret_cast<const uint32_t*>(&two));  // [column g][keys 2 t, 2 t + 1]
+          const uint32_t vbyte = ex[2 * KV8_PAGE + 8 * i];
+          kf[i] = kv8_factor(ex[8 * i]);
+          vb[i] = vbyte == KV8_E_NAN ? __uint_as_float(0x7fffffffu) : static_cast<float>(static_cast<int>(vbyte) - 127);
+          vi[i] = kv8_two_to(max(-126, 127 - static_cast<int>(vbyte)));
         }
+        const int key = key0 + warp * K8D_SLAB + g;
+#pragma unroll
+        for (int n8 = 0; n8 < NT; ++n8)
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float raw = (sc[n8][0][2 * i + k] + sc[n8][1][2 * i + k]) * qscale[n8][k];
+              y[n8][i][k] = key + 8 * i <= last[n8][k] ? fmaf(raw, kf[i], vb[i]) : -INFINITY;
+              grown |= y[n8][i][k] > m[n8][k] + K8D_LAZY;
+            }
       }
-      // ---- O[dim, column] += V^T P: dims 16 c + 2 g and + 1 are the rows g and g + 8
+      // ---- a column whose maximum grew far enough takes the block's, which all warps see alike
+      const bool any = __syncthreads_or(grown);
+      if (warp == K8D_WARPS - 1) issue(2 * n + 1 + SLOTS, j / 32 * 32 + 64);
+      if (any) {
+        if (ok && mine) {
 #pragma unroll
-      for (int c = 0; c < CHUNKS; c += 2) {
-        uint32_t r[4];
-        ldmatrix4_trans(tile_at(vtile, lane & 15, c + (lane >> 4)), r);
+          for (int n8 = 0; n8 < NT; ++n8)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t a0, a1, a2, a3;
-          kv8_unpack4(__byte_perm(r[2 * h], 0, 0x3120), a0, a1);
-          kv8_unpack4(__byte_perm(r[2 * h + 1], 0, 0x3120), a2, a3);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) mma_f16(o[n][c + h], a0, a1, a2, a3, pw[n][0], pw[n][1]);
+            for (int k = 0; k < 2; ++k) {
+              float mx = fmaxf(y[n8][0][k], y[n8][1][k]);
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+              if (g == 0) s_max[warp][n8 * 8 + 2 * t + k] = mx;
+            }
         }
-      }
-      __syncwarp();  // every lane has read the stage
-      issue();
-    }
-
-    // ---- the warps' parts, in the warps' order
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float sum = l[n][j];
-        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-        if (g == 0) { s_m[warp][n * 8 + 2 * t + j] = m[n][j]; s_l[warp][n * 8 + 2 * t + j] = sum; }
-      }
-    __syncthreads();
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float f[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float top = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < K8D_WARPS; ++w) top = fmaxf(top, s_m[w][n * 8 + 2 * t + j]);
-        f[j] = m[n][j] == -INFINITY ? 0.f : ex2(m[n][j] - top);
-      }
-#pragma unroll
-      for (int h = 0; h < D / C::HALF; ++h) {
-#pragma unroll
-        for (int c = 0; c < C::HALF / 16; ++c)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float* v = o[n][h * (C::HALF / 16) + c];
-            *reinterpret_cast<float2*>(exch + (warp * 8 + 2 * t + j) * C::COL + 16 * c + 2 * g) =
-                make_float2(v[j] * f[j], v[2 + j] * f[j]);
-          }
         __syncthreads();
-        constexpr int QUADS = C::HALF / 4;  // threads per column, four numbers each
-        for (int i = threadIdx.x; i < 8 * QUADS; i += 32 * K8D_WARPS) {
-          const int col8 = i / QUADS, d = i % QUADS * 4, col = n * 8 + col8;
-          float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-          float top = -INFINITY, sum = 0.f;
 #pragma unroll
-          for (int w = 0; w < K8D_WARPS; ++w) top = fmaxf(top, s_m[w][col]);
-#pragma unroll
-          for (int w = 0; w < K8D_WARPS; ++w) {
-            const float4 v = *reinterpret_cast<const float4*>(exch + (w * 8 + col8) * C::COL + d);
-            a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
-            const float mw = s_m[w][col];
-            sum += mw == -INFINITY ? s_l[w][col] : s_l[w][col] * ex2(mw - top);  // a NaN among the scores leaves the maximum and marks the sum
+        for (int n8 = 0; n8 < NT; ++n8) {
+          float top[2] = {-INFINITY, -INFINITY};
+          for (int w = 0; w < slabs; ++w) {
+            const float2 v = *reinterpret_cast<const float2*>(&s_max[w][n8 * 8 + 2 * t]);
+            top[0] = fmaxf(top[0], v.x);
+            top[1] = fmaxf(top[1], v.y);
           }
-          if (col < n_cols) {
-            const int row = row0 + col / p.group, len = length(row);
-            const size_t head = static_cast<size_t>(row) * p.n_q + u.kh * p.group + col % p.group;
-            const int at = h * C::HALF + d;
-            if (len <= K8D_RUN) {
-              if (u.z == 0) {  // the row's only run
-                const float inv = len > 0 ? 1.0f / sum : 0.f;
-                const float* e = reinterpret_cast<const float*>(&a);
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  p.out[head * D + at + k] = __float2bfloat16(e[k] * inv * sigmoid_f(__bfloat162float(p.gate[head * D + at + k])));
-              }
-            } else if (u.z * K8D_RUN < len) {
-              const size_t slot = head * p.n_splits + u.z;
-              *reinterpret_cast<float4*>(p.part_acc + slot * D + at) = a;
-              if (at == 0) p.part_ml[slot] = make_float2(top, sum);
+          for (int k = 0; k < 2; ++k) {
+            if (top[k] > m[n8][k] + K8D_LAZY) {
+              const float f = ex2(m[n8][k] - top[k]);  // 0 at the first key
+              m[n8][k] = top[k];
+              l[n8][k] *= f;
+#pragma unroll
+              for (int i = 0; i < C::PER; ++i) { o[n8][i][k] *= f; o[n8][i][2 + k] *= f; }
             }
           }
         }
-        __syncthreads();
+      }
+      // ---- weights
+      if (ok && mine) {
+#pragma unroll
+        for (int n8 = 0; n8 < NT; ++n8) {
+          float w[2][2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float base = m[n8][k] == -INFINITY ? 0.f : m[n8][k] - K8D_LIFT;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              w[i][k] = ex2(y[n8][i][k] - base);
+              l[n8][k] = fmaf(w[i][k], vi[i], l[n8][k]);
+            }
+          }
+          uint32_t pw[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const __half2 two = __floats2half2_rn(w[i][0], w[i][1]);
+            pw[i] = movmatrix(*reinterpret_cast<const uint32_t*>(&two));  // [column g][keys 2 t, 2 t + 1]
+          }
+          s_w[warp][n8][lane] = make_uint2(pw[0], pw[1]);
+        }
+      }
+      ok = ok && mbar_wait_warp(&full[vs], ((2 * n + 1) / SLOTS) & 1, p.err, ERR_WAIT_FULL, abort_flag);
+      __syncthreads();
+      // ---- O[dim, column] += V^T P: dims 16 c + 2 g and + 1 of tile c are the rows g and g + 8
+      if (ok) {
+        // D = 256: the two tiles of a warp and one slab at a time; below: one tile and two slabs
+        const uint32_t vslot = smem_u32(smem_k8 + vs * C::SLOT);
+#pragma unroll
+        for (int k = 0; k < SLABS / C::SPLIT; k += C::PER == 2 ? 1 : 2) {
+          const int slab = part * (SLABS / C::SPLIT) + k;
+          if (slab >= slabs) break;
+          uint32_t r[4];
+          const int row = C::PER == 2 ? lane & 15 : lane;  // lanes 16 .. 31: the second tile, or the second slab
+          ldmatrix4_trans(tile_at(vslot + slab / 4 * C::TILE, slab % 4 * K8D_SLAB + row, C::PER == 2 ? tile0 + (lane >> 4) : tile0), r);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (C::PER == 1 && slab + h >= slabs) break;
+            uint32_t a0, a1, a2, a3;
+            kv8_unpack4(__byte_perm(r[2 * h], 0, 0x3120), a0, a1);
+            kv8_unpack4(__byte_perm(r[2 * h + 1], 0, 0x3120), a2, a3);
+#pragma unroll
+            for (int n8 = 0; n8 < NT; ++n8) {
+              const uint2 w = s_w[C::PER == 2 ? slab : slab + h][n8][lane];
+              mma_f16(o[n8][C::PER == 2 ? h : 0], a0, a1, a2, a3, w.x, w.y);
+            }
+          }
+        }
+      }
+    }
+
+    // ---- the sums of all keys, in the warps' order; where warps share a tile, their outputs too
+#pragma unroll
+    for (int n8 = 0; n8 < NT; ++n8)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float sum = l[n8][k];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        if (g == 0) s_sum[warp][n8 * 8 + 2 * t + k] = sum;
+      }
+    if (C::SPLIT > 1 && part > 0) {
+#pragma unroll
+      for (int n8 = 0; n8 < NT; ++n8)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s_o[warp][n8 * 4 + i][lane] = o[n8][0][i];
+    }
+    __syncthreads();
+    if (j % 32 == 31 && warp == 0) describe(j + 33 + lane);  // the half of the list that is done with
+    if (part == 0) {
+#pragma unroll
+      for (int n8 = 0; n8 < NT; ++n8) {
+        if (C::SPLIT > 1) {
+#pragma unroll
+          for (int w = 1; w < C::SPLIT; ++w)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[n8][0][i] += s_o[w * C::TILES + warp][n8 * 4 + i][lane];
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int col = n8 * 8 + 2 * t + k;
+          if (col >= n_cols) continue;
+          float sum = 0.f;
+#pragma unroll
+          for (int w = 0; w < K8D_WARPS; ++w) sum += s_sum[w][col];
+          int r, h;
+          column(col, r, h);
+          const size_t head = static_cast<size_t>(u.row0 + r) * p.n_q + u.kh * p.group + h;
+          if (len[n8][k] > K8D_RUN) {
+            if (u.z * K8D_RUN < len[n8][k]) {
+              const size_t slot = head * p.n_splits + u.z;
+              if (tile0 == 0 && g == 0) p.part_ml[slot] = make_float2(m[n8][k], sum);
+#pragma unroll
+              for (int i = 0; i < C::PER; ++i)
+                *reinterpret_cast<float2*>(p.part_acc + slot * D + (tile0 + i) * 16 + 2 * g) = make_float2(o[n8][i][k], o[n8][i][2 + k]);
+            }
+          } else if (u.z == 0) {  // the row's only run
+            const float inv = len[n8][k] > 0 ? 1.0f / sum : 0.f;
+#pragma unroll
+            for (int i = 0; i < C::PER; ++i) {
+              const size_t at = head * D + (tile0 + i) * 16 + 2 * g;
+              *reinterpret_cast<__nv_bfloat162*>(p.out + at) =
+                  __floats2bfloat162_rn(o[n8][i][k] * inv * sigmoid_f(__bfloat162float(p.gate[at])),
+                                        o[n8][i][2 + k] * inv * sigmoid_f(__bfloat162float(p.gate[at + 1])));
+            }
+          }
+        }
       }
     }
   }
-  // a wait that ran out leaves loads on their way: they end before the CTA's shared memory goes
-  if (!ok) {
-    for (; used < issued; ++used) {
+  if (warp == K8D_WARPS - 1 && *abort_flag) {  // a wait that ran out leaves loads on their way: they end before the shared memory goes
+    for (int i = max(0, issued - SLOTS); i < issued; ++i) {
       const long long t0 = clock64();
-      while (!mbar_try_wait(&full[used % ST], (used / ST) & 1) && clock64() - t0 < WAIT_CYCLES) {}
+      while (!mbar_try_wait(&full[i % SLOTS], (i / SLOTS) & 1) && clock64() - t0 < WAIT_CYCLES) {}
     }
   }
 }
@@ -504,7 +571,7 @@ int k8d_make_map(CUtensorMap* m, const void* data, int D, long long rows) {
   const int rowb = D < 128 ? D : 128;
   cuuint64_t dims[3] = {static_cast<cuuint64_t>(rowb), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(D / rowb)};
   cuuint64_t strides[2] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(rowb)};
-  cuuint32_t box[3] = {static_cast<cuuint32_t>(rowb), K8D_SLAB, static_cast<cuuint32_t>(D / rowb)}, estr[3] = {1, 1, 1};
+  cuuint32_t box[3] = {static_cast<cuuint32_t>(rowb), KV8_PAGE, static_cast<cuuint32_t>(D / rowb)}, estr[3] = {1, 1, 1};
   const CUtensorMapSwizzle sw = rowb == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : rowb == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
   return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(data), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
             CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : -2;
@@ -518,13 +585,14 @@ int k8d_launch(const CUtensorMap& tm, const Kv8DecodeParams& p, cudaStream_t st)
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -3;
   if (sms_of[dev] == 0) {
     int sms = 0;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Kv8DecodeCfg<D>::SMEM) != cudaSuccess) return -3;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Kv8DecodeCfg<D, NT>::SMEM) != cudaSuccess) return -3;
     if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return -3;
     sms_of[dev] = sms;
   }
   const long long units = static_cast<long long>(p.B) * p.units_per_seq * p.n_kv * p.n_splits;
-  const int grid = static_cast<int>(units < sms_of[dev] ? units : sms_of[dev]);
-  if (launch_pdl(kern, dim3(grid), dim3(32 * K8D_WARPS), Kv8DecodeCfg<D>::SMEM, st, tm, p) != cudaSuccess) return -4;
+  const int most_ctas = sms_of[dev] * Kv8DecodeCfg<D, NT>::CTAS;
+  const int grid = static_cast<int>(units < most_ctas ? units : most_ctas);
+  if (launch_pdl(kern, dim3(grid), dim3(32 * K8D_WARPS), Kv8DecodeCfg<D, NT>::SMEM, st, tm, p) != cudaSuccess) return -4;
   if (p.n_splits == 1) return 0;
   const int most = (p.width < p.n_splits * (K8D_RUN / KV8_PAGE) ? p.width : p.n_splits * (K8D_RUN / KV8_PAGE)) * KV8_PAGE;
   return launch_pdl(kv8_combine_kernel<D>, dim3(p.B * p.G, p.n_q), dim3(D), 0, st, p.part_acc, p.part_ml, p.gate, p.positions, p.out,
@@ -549,7 +617,7 @@ extern "C" int b200_kv8_decode(const void* q, const void* gate, const void* data
   if (reinterpret_cast<uintptr_t>(data) % 16 || reinterpret_cast<uintptr_t>(exps) % 16 || reinterpret_cast<uintptr_t>(q) % 8) return -7;
   CUtensorMap tm;
   if (k8d_make_map(&tm, data, D, rows)) return -1;
-  const int nt = G * group <= 8 ? 1 : 2, per = 8 * nt / group < G ? 8 * nt / group : G;
+  const int cols = G * group, nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4, per = 8 * nt / group < G ? 8 * nt / group : G;
   for (int b0 = 0; b0 < B; b0 += K8D_MAX_SEQS) {
     const int n = B - b0 < K8D_MAX_SEQS ? B - b0 : K8D_MAX_SEQS;
     const size_t heads = static_cast<size_t>(b0) * G * n_q;
@@ -557,10 +625,10 @@ extern "C" int b200_kv8_decode(const void* q, const void* gate, const void* data
                             static_cast<const uint8_t*>(exps), positions + static_cast<size_t>(b0) * G,
                             tables + static_cast<size_t>(b0) * max_pages, static_cast<bf16*>(out) + heads * D,
                             part_acc + heads * n_splits * D, reinterpret_cast<float2*>(part_ml) + heads * n_splits,
-                            n, G, max_pages, width, num_pages, n_q, n_kv, group, n_splits, per, (G + per - 1) / per,
+                            n, G, max_pages, width, num_pages, n_q, n_kv, group, n_splits, per, (G + per - 1) / per, (65536 + group - 1) / group,
                             1.4426950408889634f / sqrtf(static_cast<float>(D)), err};
     int rc = -7;
-#define K8D(DD) rc = nt == 1 ? k8d_launch<DD, 1>(tm, p, st) : k8d_launch<DD, 2>(tm, p, st)
+#define K8D(DD) rc = nt == 1 ? k8d_launch<DD, 1>(tm, p, st) : nt == 2 ? k8d_launch<DD, 2>(tm, p, st) : k8d_launch<DD, 4>(tm, p, st)
     if (D == 256) K8D(256);
     else if (D == 128) K8D(128);
     else if (D == 64) K8D(64);
