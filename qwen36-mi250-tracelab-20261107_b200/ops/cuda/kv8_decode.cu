@@ -7,11 +7,11 @@
 // sum_j w_j 2^-b_j. So what the matrix instructions get are the stored numbers as halves (exact) and weights below 2^15.
 //
 // Bound: the cache's bytes, 2 (D + 1) per token and KV head. A context is cut into runs of RUN keys at fixed places, so what a row's
-// result is put together from depends on its own position only, never on the batch; a persistent CTA per SM takes runs in turn. Blocks of 128 keys
-// come into a ring by TMA, the next runs' blocks ahead of this one's end. On a block the eight warps first take 16 keys each
-// (S = K Q^T, maximum, weights), then D / 8 dims each over all keys (O += V^T P): a warp's part of the output is 2 tiles of 16 dims,
-// so nothing of the output is ever exchanged, only maxima and weights, 16 bytes per key. (With all dims of every eighth slab in
-// each warp, the warps' outputs were added up at each run's end, which took more instructions than the run: 74 us for 128 sequences of about 1,060.)
+// result is put together from depends on its own position only, never on the batch; persistent CTAs take runs in turn. In a CTA
+// one warp finds the runs and brings pages of 64 keys by TMA, the next runs' pages ahead of this one's end; four warps take 16 keys
+// each (S = K Q^T, maximum, weights); four take D / 4 dims each over all 64 keys (O += V^T P), a page behind. The outputs stay where they are
+// summed: only maxima and weights are exchanged, 16 bytes per key. (With all dims of every eighth slab in each of eight warps, the
+// warps' outputs were added up at each run's end, which took more instructions than the run: 74 us for 128 sequences of about 1,060 keys.)
 // The products are m16n8k16 with keys or dims as the 16 rows and query columns as the 8: one token of one KV head's eight query heads
 // fills the columns, where a tcgen05 tile would be 8 rows of 64. The stored bytes become halves in registers, behind ldmatrix.
 #include <cuda_fp16.h>
@@ -20,11 +20,12 @@
 
 namespace b200 {
 
-constexpr int K8D_RUN = 512;                    // keys of a run: part of the numerics
-constexpr int K8D_WARPS = 8;                    // that compute
+constexpr int K8D_RUN = 256;                    // keys of a run: part of the numerics
 constexpr int K8D_SLAB = 16;                    // keys of a warp's scores
-constexpr int K8D_BLOCK = K8D_WARPS * K8D_SLAB; // keys of a ring stage: two pages
-constexpr int K8D_MAX_SEQS = 1024;              // of one launch
+constexpr int K8D_SLABS = KV8_PAGE / K8D_SLAB;  // of a page: a warp each
+constexpr int K8D_SEQS = 512;                   // of one launch
+constexpr int K8D_UNITS = 8;                    // descriptions of runs that are kept
+constexpr int K8D_PAGES = K8D_RUN / KV8_PAGE;   // of a run
 constexpr float K8D_LIFT = 7.0f;                // weights are 2^LIFT at the maximum: halves reach down to 2^-24
 constexpr float K8D_LAZY = 8.0f;                // the maximum moves when it grew by more: 2^(LIFT + LAZY) is below the halves' 65504
 
@@ -48,15 +49,19 @@ template <int D, int NT>
 struct Kv8DecodeCfg {
   static constexpr int ROWB = D < 128 ? D : 128;           // bytes of a row in one swizzled block
   static constexpr int DB = D / ROWB;
-  static constexpr int TILE = KV8_PAGE * D;                // a page's keys or values
-  static constexpr int SLOT = 2 * TILE;                    // of the ring: the keys of a block or its values
-  static constexpr int CTAS = NT == 1 ? 2 : 1;             // per SM: one column tile's registers leave room for sixteen warps
+  static constexpr int TILE = KV8_PAGE * D;                // a page's keys or values: a slot of their ring
+  static constexpr int CTAS = NT == 1 ? 2 : 1;             // per SM: one column tile's registers leave room for two
   static constexpr int SLOTS = (D == 256 ? 3 : D == 128 ? 6 : 8) * (D == 256 && NT > 1 ? 2 : 1);
-  static constexpr int EXPS = 4 * KV8_PAGE;                // exponents of a block's keys and values, with its keys
-  static constexpr int SMEM = SLOTS * (SLOT + EXPS);
+  static constexpr int EXPS = 2 * KV8_PAGE;                // exponents of a page's keys and values, with its keys
+  static constexpr int SMEM = SLOTS * (2 * TILE + EXPS);
+  static constexpr int HALVES = NT > 1 ? 2 : 1;            // groups of four warps that take scores, each of a part of the columns
+  static constexpr int NA = NT / HALVES;                   // column tiles of a group
+  static constexpr int SW = HALVES * K8D_SLABS;            // warps that take scores
+  static constexpr int OW = NT > 1 && D >= 128 ? 8 : 4;    // warps that take outputs (SPLIT is the same for all NT: part of the numerics)
+  static constexpr int THREADS = 32 * (SW + OW + 1);
   static constexpr int TILES = D / 16;                     // output tiles of 16 dims
-  static constexpr int PER = TILES > K8D_WARPS ? TILES / K8D_WARPS : 1;  // of a warp
-  static constexpr int SPLIT = TILES < K8D_WARPS ? K8D_WARPS / TILES : 1;  // warps that share a tile, a part of the keys each
+  static constexpr int PER = TILES > OW ? TILES / OW : 1;  // of a warp
+  static constexpr int SPLIT = TILES < OW ? OW / TILES : 1;  // warps that share a tile, a part of the keys each
 };
 
 __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t* r) {
@@ -76,9 +81,17 @@ __device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+// Barriers of the warps that take scores; all of them come to each one, whatever they have to do there.
+__device__ __forceinline__ void meet_scores(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(32 * K8D_SLABS) : "memory"); }
+__device__ __forceinline__ bool meet_scores_or(int id, bool mine) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %1, 0;\n\t"
+      "bar.red.or.pred q, %2, %3, p;\n\t"
+      "selp.b32 %0, 1, 0, q;\n\t}"
+      : "=r"(any) : "r"(static_cast<uint32_t>(mine)), "r"(id), "n"(32 * K8D_SLABS) : "memory");
+  return any != 0;
 }
 __device__ __forceinline__ float ex2(float x) {
   float r;
@@ -101,455 +114,638 @@ struct Kv8Unit {
   int seq, kh, z, row0, rows, keys;
 };
 
+__device__ __forceinline__ int kv8_length(const int64_t* positions, int row, int most) {
+  return max(0, min(static_cast<int>(min(__ldg(positions + row), static_cast<int64_t>(most))) + 1, most));
+}
+
 template <int D, int NT>
-__global__ void __launch_bounds__(32 * K8D_WARPS, Kv8DecodeCfg<D, NT>::CTAS)
-kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, Kv8DecodeParams p) {
+__global__ void __maxnreg__(96)  // two CTAs of 9 warps or one of 17
+kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtensorMap tm_exps, Kv8DecodeParams p) {
   using C = Kv8DecodeCfg<D, NT>;
-  constexpr int SLOTS = C::SLOTS, CHUNKS = D / 16, COLS = 8 * NT, SLABS = K8D_WARPS, DI = (D + 127) / 128;
+  constexpr int SLOTS = C::SLOTS, CHUNKS = D / 16, COLS = 8 * NT, DI = (D + 127) / 128, SLABS = K8D_SLABS, NA = C::NA;
   extern __shared__ __align__(1024) uint8_t smem_k8[];
   if (smem_u32(smem_k8) & 1023u) {  // the swizzled tiles need this alignment
     if (threadIdx.x == 0) atomicCAS(p.err, 0, ERR_BAD_INDEX);
     return;
   }
-  uint8_t* s_exps = smem_k8 + SLOTS * C::SLOT;
-  __shared__ __align__(8) uint64_t full[SLOTS];
-  __shared__ int s_first[K8D_MAX_SEQS + 1];            // runs of the sequences before
-  __shared__ Kv8Unit s_unit[64];                       // this CTA's units, a ring in two halves
-  __shared__ __align__(16) float s_max[SLABS][COLS], s_sum[SLABS][COLS];  // read two columns at a time
-  __shared__ __align__(8) uint2 s_w[SLABS][NT][32];    // weights of a block, as the products' second operand
+  uint8_t* const s_k = smem_k8;                        // [SLOTS] pages' keys
+  uint8_t* const s_v = smem_k8 + SLOTS * C::TILE;      // [SLOTS] pages' values
+  uint8_t* const s_exps = s_v + SLOTS * C::TILE;       // [SLOTS][keys' 64, values' 64]
+  __shared__ __align__(8) uint64_t k_full[SLOTS], k_empty[SLOTS], v_full[SLOTS], v_empty[SLOTS];
+  __shared__ __align__(8) uint64_t w_full[2], w_empty[2];   // weights of an even / odd page
+  __shared__ __align__(8) uint64_t u_full[K8D_UNITS], u_empty[K8D_UNITS];
+  __shared__ __align__(8) uint64_t l_full[2], l_empty[2];   // sums of an even / odd unit
+  __shared__ int s_first[K8D_SEQS + 1];                // runs behind the first of the sequences before
+  __shared__ Kv8Unit s_unit[K8D_UNITS];
+  __shared__ int s_scaled[2][C::HALVES];
+  __shared__ __align__(16) float s_max[SLABS][COLS], s_factor[2][COLS];   // read two columns at a time
+  __shared__ float s_sum[2][SLABS][COLS], s_top[2][COLS], s_scale[COLS];
+  __shared__ __align__(8) uint2 s_w[2][SLABS][NT][32]; // weights of a page, as the products' second operand
   __shared__ __align__(8) uint2 s_q[NT][CHUNKS][32];   // queries, likewise
-  __shared__ float s_scale[COLS];
-  __shared__ __align__(16) float s_o[C::SPLIT > 1 ? K8D_WARPS : 1][C::SPLIT > 1 ? NT * 4 : 1][32];
+  __shared__ float s_o[2][C::SPLIT > 1 ? C::OW : 1][C::SPLIT > 1 ? NT * 4 : 1][32];
   __shared__ int s_abort;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  volatile int* abort_flag = &s_abort;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < SLOTS; ++i) mbar_init(&full[i], 1);
+    for (int i = 0; i < SLOTS; ++i) { mbar_init(&k_full[i], 1); mbar_init(&v_full[i], 1); mbar_init(&k_empty[i], C::HALVES); mbar_init(&v_empty[i], C::OW); }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&w_full[i], C::SW); mbar_init(&w_empty[i], C::OW);
+      mbar_init(&l_full[i], C::SPLIT > 1 ? C::SW + C::OW : C::SW); mbar_init(&l_empty[i], C::OW);
+    }
+    for (int i = 0; i < K8D_UNITS; ++i) { mbar_init(&u_full[i], 1); mbar_init(&u_empty[i], C::SW + C::OW); }
     s_abort = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tm);
+    tma_prefetch_desc(&tm_exps);
   }
+  __syncthreads();
   pdl_wait();
   pdl_launch();
   const int most = min(p.width, p.n_splits * (K8D_RUN / KV8_PAGE)) * KV8_PAGE;  // keys that the tables can name
-  const auto length = [&](int row) { return max(0, min(static_cast<int>(min(__ldg(p.positions + row), static_cast<int64_t>(most))) + 1, most)); };
-  for (int b = threadIdx.x; b < p.B; b += blockDim.x) {
-    int len = 0;
-    for (int i = 0; i < p.G; ++i) len = max(len, length(b * p.G + i));
-    s_first[b + 1] = max(1, (len + K8D_RUN - 1) / K8D_RUN);  // a sequence without keys has a run, which writes its zeros
-  }
-  __syncthreads();
-  if (warp == 0) {  // inclusive sums, a lane a stretch of sequences
-    const int per = (p.B + 31) / 32, b0 = min(p.B, lane * per), b1 = min(p.B, b0 + per);
-    int sum = 0;
-    for (int b = b0; b < b1; ++b) sum += s_first[b + 1];
-    int upto = sum;
+
+  if (warp == C::SW + C::OW) {
+    // ---------------- loads. The units are the runs of all sequences; this CTA's are a grid size apart. Once the pages are on their
+    // way any other load waits behind some 30 MB of them, 4 us: what a unit needs to know is asked for two units ahead, and published one ahead.
+    const int per_seq = p.units_per_seq * p.n_kv;
+    int before = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 128) {
+      int runs[4], len[4] = {0, 0, 0, 0};
+      for (int r = 0; r < p.G; ++r)
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += u;
+        for (int i = 0; i < 4; ++i) {
+          const int b = b0 + i * 32 + lane;
+          if (b < p.B) len[i] = max(len[i], kv8_length(p.positions, b * p.G + r, most));
+        }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int b = b0 + i * 32 + lane;
+        runs[i] = b < p.B ? max(1, (len[i] + K8D_RUN - 1) / K8D_RUN) : 0;  // a sequence without keys has a run, which writes its zeros
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int u = __shfl_up_sync(0xffffffffu, runs[i], o);
+          if (lane >= o) runs[i] += u;
+        }
+        if (b < p.B) s_first[b + 1] = before + runs[i];
+        before += __shfl_sync(0xffffffffu, runs[i], 31);
+      }
     }
-    upto -= sum;
-    for (int b = b0; b < b1; ++b) { upto += s_first[b + 1]; s_first[b + 1] = upto; }
     if (lane == 0) s_first[0] = 0;
+    __syncwarp();
+    const int total = before * per_seq;
+    struct Ahead { Kv8Unit u; int len, page; };  // lane i: keys of the unit's row i, page i of its run
+    const auto ask = [&](int j) {  // unit j; rows of 0: there is none
+      Ahead a = {};
+      const int id = blockIdx.x + j * static_cast<int>(gridDim.x);
+      if (id >= total) return a;
+      const int run = id / per_seq, k = id - run * per_seq, rg = k / p.n_kv;
+      a.u.kh = k - rg * p.n_kv;
+      a.u.seq = kv8_find(s_first, p.B, run);
+      a.u.z = run - s_first[a.u.seq];
+      a.u.row0 = a.u.seq * p.G + rg * p.rows_per_unit;
+      a.u.rows = min(p.rows_per_unit, p.G - rg * p.rows_per_unit);
+      if (lane < a.u.rows) a.len = kv8_length(p.positions, a.u.row0 + lane, most);
+      if (lane < K8D_PAGES && a.u.z * K8D_PAGES + lane < p.width)
+        a.page = __ldg(p.tables + static_cast<size_t>(a.u.seq) * p.max_pages + a.u.z * K8D_PAGES + lane);
+      return a;
+    };
+    bool ok = true;
+    const auto publish = [&](Ahead& a, int j) {
+      const int us = j % K8D_UNITS;
+      a.u.keys = max(0, min(K8D_RUN, __reduce_max_sync(0xffffffffu, a.len) - a.u.z * K8D_RUN));
+      ok = ok && mbar_wait_warp(&u_empty[us], ((j / K8D_UNITS) & 1) ^ 1, p.err, ERR_WAIT_EMPTY, abort_flag);
+      if (ok && lane == 0) { s_unit[us] = a.u; mbar_arrive(&u_full[us]); }
+    };
+    Ahead now = ask(0), next = ask(1);
+    publish(now, 0);
+    publish(next, 1);
+    int n = 0;
+    for (int j = 0; now.u.rows > 0 && ok; ++j) {
+      Ahead later = ask(j + 2);
+      for (int pg = 0; pg * KV8_PAGE < now.u.keys && ok; ++pg, ++n) {
+        const int s = n % SLOTS;
+        int page = __shfl_sync(0xffffffffu, now.page, pg);
+        if (page < 0 || page >= p.num_pages) { if (lane == 0) atomicCAS(p.err, 0, ERR_BAD_INDEX); page = 0; }
+        const int row = (page * 2 * p.n_kv + now.u.kh) * KV8_PAGE;
+        ok = mbar_wait_warp(&k_empty[s], ((n / SLOTS) & 1) ^ 1, p.err, ERR_WAIT_EMPTY, abort_flag);
+        if (!ok) break;
+        if (elect_one()) {
+          mbar_expect_tx(&k_full[s], C::TILE + C::EXPS);
+          tma_load_3d(s_k + s * C::TILE, &tm, &k_full[s], 0, row, 0);
+          tma_load_3d(s_exps + s * C::EXPS, &tm_exps, &k_full[s], 0, now.u.kh, page * 2);
+        }
+        ok = mbar_wait_warp(&v_empty[s], ((n / SLOTS) & 1) ^ 1, p.err, ERR_WAIT_EMPTY, abort_flag);
+        if (!ok) { ++n; break; }
+        if (elect_one()) {
+          mbar_expect_tx(&v_full[s], C::TILE);
+          tma_load_3d(s_v + s * C::TILE, &tm, &v_full[s], 0, row + p.n_kv * KV8_PAGE, 0);
+        }
+      }
+      publish(later, j + 2);
+      now = next;
+      next = later;
+    }
+    for (int i = max(0, n - SLOTS); !ok && i < n; ++i) {  // a wait that ran out leaves loads on their way: they end before the shared memory goes
+      const long long t0 = clock64();
+      while (!(mbar_try_wait(&k_full[i % SLOTS], (i / SLOTS) & 1) && mbar_try_wait(&v_full[i % SLOTS], (i / SLOTS) & 1)) && clock64() - t0 < WAIT_CYCLES / 8) {}
+    }
+    return;
   }
-  __syncthreads();
-  const int per_run = p.n_kv * p.units_per_seq, total = s_first[p.B] * per_run;
-  const int n_units = (total - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);  // of this CTA
-  volatile int* abort_flag = &s_abort;
-  const auto describe = [&](int j) {  // unit j of this CTA, by one lane
-    if (j >= n_units) return;
-    Kv8Unit u;
-    const int id = blockIdx.x + j * gridDim.x, run = id / per_run, x = id % per_run, rg = x % p.units_per_seq;
-    u.kh = x / p.units_per_seq;
-    u.seq = kv8_find(s_first, p.B, run);
-    u.z = run - s_first[u.seq];
-    u.row0 = u.seq * p.G + rg * p.rows_per_unit;
-    u.rows = min(p.rows_per_unit, (u.seq + 1) * p.G - u.row0);
-    int len = 0;
-    for (int r = 0; r < u.rows; ++r) len = max(len, length(u.row0 + r));
-    u.keys = max(0, min(K8D_RUN, len - u.z * K8D_RUN));
-    s_unit[j % 64] = u;
-  };
-  if (warp < 2) describe(threadIdx.x);
-  __syncthreads();
-
-  // ---------------- loads, by the last warp. The ring takes a block's keys, then its values; by the first meeting on block k all warps have
-  // read the keys of block k and the values of block k - 1. The page numbers of a unit are read a unit ahead.
-  struct { int j, kh, pages, pg, ids; } cur = {}, nxt = {};
-  int issued = 0;  // slots asked for
-  const auto look = [&](decltype(cur)& w, int j, int limit) {  // the first unit from j on that has keys, below `limit`
-    for (; j < limit && j < n_units; ++j) {
-      const Kv8Unit& u = s_unit[j % 64];
-      if (u.keys == 0) continue;
-      w.kh = u.kh;
-      w.pg = 0;
-      w.pages = (u.keys + KV8_PAGE - 1) / KV8_PAGE;
-      w.ids = 0;
-      if (lane < w.pages) w.ids = __ldg(p.tables + static_cast<size_t>(u.seq) * p.max_pages + u.z * (K8D_RUN / KV8_PAGE) + lane);
-      break;
-    }
-    w.j = j;
-    return j < limit && j < n_units;
-  };
-  bool have = false, have_next = false;  // cur, nxt hold a unit
-  const auto issue = [&](int upto, int limit) {
-    while (issued < upto) {
-      if (!have) { have = have_next; cur = nxt; have_next = false; }
-      if (!have) { have = look(cur, cur.j, limit); nxt.j = cur.j + have; }
-      if (!have_next) have_next = look(nxt, max(nxt.j, cur.j + have), limit);
-      if (!have) { cur.j = nxt.j; return; }
-      const int s = issued % SLOTS, of = min(2, cur.pages - cur.pg), values = issued & 1;
-      int page = __shfl_sync(0xffffffffu, cur.ids, cur.pg + (lane & 1));
-      if (lane == 0) mbar_expect_tx(&full[s], of * (C::TILE + (values ? 0 : 2 * KV8_PAGE)));
-      __syncwarp();
-      if (lane < 4 && (lane & 1) < of) {  // lanes 0, 1: the tiles and their keys' exponents, 2, 3: the values' exponents
-        if (page < 0 || page >= p.num_pages) { atomicCAS(p.err, 0, ERR_BAD_INDEX); page = 0; }
-        const int row = ((page * 2 + (lane >> 1)) * p.n_kv + cur.kh) * KV8_PAGE;
-        if (lane < 2) tma_load_3d(smem_k8 + s * C::SLOT + lane * C::TILE, &tm, &full[s], 0, row + values * p.n_kv * KV8_PAGE, 0);
-        if (!values) bulk_load(s_exps + s * C::EXPS + lane * KV8_PAGE, p.exps + row, KV8_PAGE, &full[s]);
-      }
-      ++issued;
-      if (values) {
-        cur.pg += 2;
-        if (cur.pg >= cur.pages) { have = false; cur.j = nxt.j; }
-      }
-    }
-  };
-  if (warp == K8D_WARPS - 1) issue(SLOTS, 64);
-
   // shared-memory offset of 16 bytes of a page's swizzled tile: row r, chunk c
   const auto tile_at = [&](uint32_t tile, int r, int c) {
     constexpr int PER = C::ROWB / 16;  // chunks of a block's row
     const int byte = r * C::ROWB;
     return tile + (c / PER) * (KV8_PAGE * C::ROWB) + byte + (((c % PER) ^ ((byte >> 7) & (PER - 1))) << 4);
   };
-  const int tile0 = warp % C::TILES * C::PER, part = warp / C::TILES;  // this warp's output tiles, and which part of the keys
-  bool ok = true;
-  int n = 0;  // blocks so far: their keys are in slot 2 n, their values in 2 n + 1
-
   const auto column = [&](int col, int& row, int& head) { row = col * p.inv_group >> 16; head = col - row * p.group; };
-  uint2 qnext[NT][DI];   // the next unit's queries, a warp a column
-  const auto fetch = [&](const Kv8Unit& u) {
-#pragma unroll
-    for (int n8 = 0; n8 < NT; ++n8) {
-      int row, head;
-      column(n8 * 8 + warp, row, head);
-      const bf16* src = p.q + (static_cast<size_t>(u.row0 + row) * p.n_q + u.kh * p.group + head) * D + lane * 4;
-#pragma unroll
-      for (int i = 0; i < DI; ++i)
-        qnext[n8][i] = row < u.rows && lane * 4 + i * 128 < D ? *reinterpret_cast<const uint2*>(src + i * 128) : make_uint2(0u, 0u);
-    }
-  };
-  if (n_units > 0) fetch(s_unit[0]);
+  const auto sync_arrive = [&](uint64_t* bar) { __syncwarp(); if (lane == 0) mbar_arrive(bar); };
+  bool ok = true;
+  int n = 0;  // pages so far
 
-  for (int j = 0; j < n_units; ++j) {
-    const Kv8Unit u = s_unit[j % 64];
-    const int n_cols = u.rows * p.group;
-    if (warp == K8D_WARPS - 1) issue(2 * n + SLOTS, j / 32 * 32 + 32);
-    // ---- queries as halves with the column's largest number in [2^10, 2^11), in the order of the products' second operand: lane
-    // (column % 8, t) holds dims 16 c + 4 t .. + 3 of chunk c
+  if (warp < C::SW) {
+    // ---------------- scores, maxima and weights: slab of keys, tiles of columns
+    const int slab = warp % SLABS, tile = warp / SLABS * NA, bar = 1 + warp / SLABS;
+    constexpr int QC = 8 * NA / SLABS;  // query columns that a warp prepares
+    uint2 raw[QC][DI];
+    const auto fetch = [&](const Kv8Unit& u) {
 #pragma unroll
-    for (int n8 = 0; n8 < NT; ++n8) {
-      float x[DI][4];
-      float top = 0.f;
-      bool bad = false;
-#pragma unroll
-      for (int i = 0; i < DI; ++i) {
-        const __nv_bfloat162* e = reinterpret_cast<const __nv_bfloat162*>(&qnext[n8][i]);
-        const float2 a = __bfloat1622float2(e[0]), b = __bfloat1622float2(e[1]);
-        x[i][0] = a.x; x[i][1] = a.y; x[i][2] = b.x; x[i][3] = b.y;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) { top = fmaxf(top, fabsf(x[i][k])); bad |= !(fabsf(x[i][k]) <= 3.4e38f); }
-      }
-      top = warp_max(top);
-      const int e = max(-110, min(110, static_cast<int>(__float_as_uint(top) >> 23) - 127 - 10));
-      const float f = kv8_two_to(-e);
-#pragma unroll
-      for (int i = 0; i < DI; ++i) {
-        if (lane * 4 + i * 128 < D) {
-          const __half2 lo = __floats2half2_rn(x[i][0] * f, x[i][1] * f), hi = __floats2half2_rn(x[i][2] * f, x[i][3] * f);
-          s_q[n8][i * 8 + lane / 4][warp * 4 + lane % 4] = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-        }
-      }
-      // a NaN or an infinity anywhere in the column: all its scores are NaN
-      const bool any = __any_sync(0xffffffffu, bad);
-      if (lane == 0) s_scale[n8 * 8 + warp] = any ? __uint_as_float(0x7fffffffu) : kv8_two_to(e) * p.scale_log2;
-    }
-    int len[NT][2];        // columns 2 t, 2 t + 1: keys of their rows (0: no such column)
-#pragma unroll
-    for (int n8 = 0; n8 < NT; ++n8)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
+      for (int i = 0; i < QC; ++i) {
         int row, head;
-        column(n8 * 8 + 2 * t + k, row, head);
-        len[n8][k] = row < u.rows ? length(u.row0 + row) : 0;
+        column(tile * 8 + slab * QC + i, row, head);
+        const bf16* src = p.q + (static_cast<size_t>(u.row0 + row) * p.n_q + u.kh * p.group + head) * D + lane * 4;
+#pragma unroll
+        for (int k = 0; k < DI; ++k)
+          raw[i][k] = row < u.rows && lane * 4 + k * 128 < D ? *reinterpret_cast<const uint2*>(src + k * 128) : make_uint2(0u, 0u);
       }
-    if (j + 1 < n_units) fetch(s_unit[(j + 1) % 64]);
-    __syncthreads();
-    uint2 qf[NT][CHUNKS];
-    float qscale[NT][2];   // what takes the product to log-2 scores
-    int last[NT][2];       // last visible key of the run
-    float m[NT][2], l[NT][2], o[NT][C::PER][4];
+    };
+    // A unit's description; its queries are fetched one unit ahead. Either all these warps have it or none goes on: each stays in
+    // step with the barriers of the others.
+    bool known = false;
+    int last_next[NA][2];    // columns 2 t, 2 t + 1: last visible key of the run
+    const auto enter = [&](int j) {
+      ok = ok && mbar_wait_warp(&u_full[j % K8D_UNITS], (j / K8D_UNITS) & 1, p.err, ERR_WAIT_FULL, abort_flag);
+      known = ok = !meet_scores_or(bar, !ok);
+      if (!known) return;
+      const Kv8Unit u = s_unit[j % K8D_UNITS];
+      known = u.rows > 0;
+      if (!known) return;
+      fetch(u);
 #pragma unroll
-    for (int n8 = 0; n8 < NT; ++n8) {
+      for (int n8 = 0; n8 < NA; ++n8)
 #pragma unroll
-      for (int c = 0; c < CHUNKS; ++c) qf[n8][c] = s_q[n8][c][lane];
+        for (int k = 0; k < 2; ++k) {
+          int row, head;
+          column((tile + n8) * 8 + 2 * t + k, row, head);
+          last_next[n8][k] = (row < u.rows ? kv8_length(p.positions, u.row0 + row, most) : 0) - 1 - u.z * K8D_RUN;
+        }
+    };
+    enter(0);
+    for (int j = 0; known; ++j) {
+      const int us = j % K8D_UNITS;
+      const Kv8Unit u = s_unit[us];
+      int last[NA][2];
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        qscale[n8][k] = s_scale[n8 * 8 + 2 * t + k];
-        last[n8][k] = len[n8][k] - 1 - u.z * K8D_RUN;
-        m[n8][k] = -INFINITY;
-        l[n8][k] = 0.f;
-      }
+      for (int n8 = 0; n8 < NA; ++n8) { last[n8][0] = last_next[n8][0]; last[n8][1] = last_next[n8][1]; }
+      // queries as halves with the column's largest number in [2^10, 2^11), in the order of the products' second operand: lane
+      // (column % 8, t) holds dims 16 c + 4 t .. + 3 of chunk c
 #pragma unroll
-      for (int i = 0; i < C::PER; ++i) o[n8][i][0] = o[n8][i][1] = o[n8][i][2] = o[n8][i][3] = 0.f;
-    }
-
-    for (int key0 = 0; key0 < u.keys; key0 += K8D_BLOCK, ++n) {
-      const int slabs = min(SLABS, (u.keys - key0 + K8D_SLAB - 1) / K8D_SLAB);
-      const bool mine = warp < slabs;
-      const int ks = 2 * n % SLOTS, vs = (2 * n + 1) % SLOTS;
-      ok = ok && mbar_wait_warp(&full[ks], (2 * n / SLOTS) & 1, p.err, ERR_WAIT_FULL, abort_flag);
-      // ---- scores of this warp's slab: S[key, column], keys g and g + 8
-      float y[NT][2][2];  // [key][column 2 t, 2 t + 1]
-      float vi[2];
-      bool grown = false;
-      if (ok && mine) {
-        float sc[NT][2][4];  // two chains of products
+      for (int i = 0; i < QC; ++i) {
+        const int col = tile * 8 + slab * QC + i;
+        float x[DI][4];
+        float top = 0.f;
+        bool bad = false;
 #pragma unroll
-        for (int n8 = 0; n8 < NT; ++n8)
+        for (int k = 0; k < DI; ++k) {
+          const __nv_bfloat162* e = reinterpret_cast<const __nv_bfloat162*>(&raw[i][k]);
+          const float2 a = __bfloat1622float2(e[0]), b = __bfloat1622float2(e[1]);
+          x[k][0] = a.x; x[k][1] = a.y; x[k][2] = b.x; x[k][3] = b.y;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) sc[n8][0][k] = sc[n8][1][k] = 0.f;
-        const uint32_t ktile = smem_u32(smem_k8 + ks * C::SLOT) + warp / 4 * C::TILE;
+          for (int h = 0; h < 4; ++h) { top = fmaxf(top, fabsf(x[k][h])); bad |= !(fabsf(x[k][h]) <= 3.4e38f); }
+        }
+        top = warp_max(top);
+        const int e = max(-110, min(110, static_cast<int>(__float_as_uint(top) >> 23) - 127 - 10));
+        const float f = kv8_two_to(-e);
 #pragma unroll
-        for (int c = 0; c < CHUNKS; c += 2) {
-          uint32_t r[4];
-          ldmatrix4(tile_at(ktile, warp % 4 * K8D_SLAB + (lane & 15), c + (lane >> 4)), r);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t a0, a1, a2, a3;
-            kv8_unpack4(r[2 * h], a0, a2);
-            kv8_unpack4(r[2 * h + 1], a1, a3);
-#pragma unroll
-            for (int n8 = 0; n8 < NT; ++n8) mma_f16(sc[n8][h], a0, a1, a2, a3, qf[n8][c + h].x, qf[n8][c + h].y);
+        for (int k = 0; k < DI; ++k) {
+          if (lane * 4 + k * 128 < D) {
+            const __half2 lo = __floats2half2_rn(x[k][0] * f, x[k][1] * f), hi = __floats2half2_rn(x[k][2] * f, x[k][3] * f);
+            s_q[col / 8][k * 8 + lane / 4][col % 8 * 4 + lane % 4] = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
           }
         }
-        const uint8_t* ex = s_exps + ks * C::EXPS + warp * K8D_SLAB + g;
-        float kf[2], vb[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t vbyte = ex[2 * KV8_PAGE + 8 * i];
-          kf[i] = kv8_factor(ex[8 * i]);
-          vb[i] = vbyte == KV8_E_NAN ? __uint_as_float(0x7fffffffu) : static_cast<float>(static_cast<int>(vbyte) - 127);
-          vi[i] = kv8_two_to(max(-126, 127 - static_cast<int>(vbyte)));
-        }
-        const int key = key0 + warp * K8D_SLAB + g;
-#pragma unroll
-        for (int n8 = 0; n8 < NT; ++n8)
-#pragma unroll
-          for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const float raw = (sc[n8][0][2 * i + k] + sc[n8][1][2 * i + k]) * qscale[n8][k];
-              y[n8][i][k] = key + 8 * i <= last[n8][k] ? fmaf(raw, kf[i], vb[i]) : -INFINITY;
-              grown |= y[n8][i][k] > m[n8][k] + K8D_LAZY;
-            }
+        // a NaN or an infinity anywhere in the column: all its scores are NaN
+        const bool any = __any_sync(0xffffffffu, bad);
+        if (lane == 0) s_scale[col] = any ? __uint_as_float(0x7fffffffu) : kv8_two_to(e) * p.scale_log2;
       }
-      // ---- a column whose maximum grew far enough takes the block's, which all warps see alike
-      const bool any = __syncthreads_or(grown);
-      if (warp == K8D_WARPS - 1) issue(2 * n + 1 + SLOTS, j / 32 * 32 + 64);
-      if (any) {
-        if (ok && mine) {
+      meet_scores(bar);
+      enter(j + 1);
+      uint2 qf[CHUNKS];      // of the first column tile; a second one's are read at each use
+      float qscale[NA][2];   // what takes the product to log-2 scores
+      float m[NA][2], l[NA][2];
 #pragma unroll
-          for (int n8 = 0; n8 < NT; ++n8)
+      for (int c = 0; c < CHUNKS; ++c) qf[c] = s_q[tile][c][lane];
+#pragma unroll
+      for (int n8 = 0; n8 < NA; ++n8)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          qscale[n8][k] = s_scale[(tile + n8) * 8 + 2 * t + k];
+          m[n8][k] = -INFINITY;
+          l[n8][k] = 0.f;
+        }
+
+      for (int key0 = 0; key0 < u.keys; key0 += KV8_PAGE, ++n) {
+        const int s = n % SLOTS, half = n & 1;
+        const bool mine = key0 + slab * K8D_SLAB < u.keys;
+        ok = ok && mbar_wait_warp(&k_full[s], (n / SLOTS) & 1, p.err, ERR_WAIT_FULL, abort_flag);
+        // S[key, column], keys g and g + 8 of this warp's slab
+        float y[NA][2][2];  // [key][column 2 t, 2 t + 1]
+        float vi[2];
+        bool grown = false;
+        if (ok && mine) {
+          float sc[NA][2][4];  // two chains of products
+#pragma unroll
+          for (int n8 = 0; n8 < NA; ++n8)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sc[n8][0][k] = sc[n8][1][k] = 0.f;
+          const uint32_t ktile = smem_u32(s_k + s * C::TILE);
+#pragma unroll
+          for (int c = 0; c < CHUNKS; c += 2) {
+            uint32_t r[4];
+            ldmatrix4(tile_at(ktile, slab * K8D_SLAB + (lane & 15), c + (lane >> 4)), r);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t a0, a1, a2, a3;
+              kv8_unpack4(r[2 * h], a0, a2);
+              kv8_unpack4(r[2 * h + 1], a1, a3);
+#pragma unroll
+              for (int n8 = 0; n8 < NA; ++n8) {
+                const uint2 b = n8 == 0 ? qf[c + h] : s_q[tile + n8][c + h][lane];
+                mma_f16(sc[n8][h], a0, a1, a2, a3, b.x, b.y);
+              }
+            }
+          }
+          const uint8_t* ex = s_exps + s * C::EXPS + slab * K8D_SLAB + g;
+          float kf[2], vb[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t vbyte = ex[KV8_PAGE + 8 * i];
+            kf[i] = kv8_factor(ex[8 * i]);
+            vb[i] = vbyte == KV8_E_NAN ? __uint_as_float(0x7fffffffu) : static_cast<float>(static_cast<int>(vbyte) - 127);
+            vi[i] = kv8_two_to(max(-126, 127 - static_cast<int>(vbyte)));
+          }
+          const int key = key0 + slab * K8D_SLAB + g;
+#pragma unroll
+          for (int n8 = 0; n8 < NA; ++n8)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const float x = (sc[n8][0][2 * i + k] + sc[n8][1][2 * i + k]) * qscale[n8][k];
+                y[n8][i][k] = key + 8 * i <= last[n8][k] ? fmaf(x, kf[i], vb[i]) : -INFINITY;
+                grown |= y[n8][i][k] > m[n8][k] + K8D_LAZY;
+              }
+        }
+        // a column whose maximum grew far enough takes the page's, which all warps see alike
+        const bool any = meet_scores_or(bar, grown);
+        if (slab == 0 && lane == 0) mbar_arrive(&k_empty[s]);  // the group has read the keys
+        if (any) {
+#pragma unroll
+          for (int n8 = 0; n8 < NA; ++n8)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-              float mx = fmaxf(y[n8][0][k], y[n8][1][k]);
+              float mx = ok && mine ? fmaxf(y[n8][0][k], y[n8][1][k]) : -INFINITY;
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-              if (g == 0) s_max[warp][n8 * 8 + 2 * t + k] = mx;
+              if (g == 0) s_max[slab][(tile + n8) * 8 + 2 * t + k] = mx;
             }
+          meet_scores(bar);
         }
-        __syncthreads();
+        ok = ok && mbar_wait_warp(&w_empty[half], ((n >> 1) & 1) ^ 1, p.err, ERR_WAIT_EMPTY, abort_flag);
+        if (any) {
 #pragma unroll
-        for (int n8 = 0; n8 < NT; ++n8) {
-          float top[2] = {-INFINITY, -INFINITY};
-          for (int w = 0; w < slabs; ++w) {
-            const float2 v = *reinterpret_cast<const float2*>(&s_max[w][n8 * 8 + 2 * t]);
-            top[0] = fmaxf(top[0], v.x);
-            top[1] = fmaxf(top[1], v.y);
-          }
+          for (int n8 = 0; n8 < NA; ++n8) {
+            float2 top = make_float2(-INFINITY, -INFINITY), f = make_float2(1.f, 1.f);
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            if (top[k] > m[n8][k] + K8D_LAZY) {
-              const float f = ex2(m[n8][k] - top[k]);  // 0 at the first key
-              m[n8][k] = top[k];
-              l[n8][k] *= f;
-#pragma unroll
-              for (int i = 0; i < C::PER; ++i) { o[n8][i][k] *= f; o[n8][i][2 + k] *= f; }
+            for (int w = 0; w < SLABS; ++w) {
+              const float2 v = *reinterpret_cast<const float2*>(&s_max[w][(tile + n8) * 8 + 2 * t]);
+              top.x = fmaxf(top.x, v.x);
+              top.y = fmaxf(top.y, v.y);
             }
+            if (top.x > m[n8][0] + K8D_LAZY) { f.x = ex2(m[n8][0] - top.x); m[n8][0] = top.x; l[n8][0] *= f.x; }  // 0 at the first key
+            if (top.y > m[n8][1] + K8D_LAZY) { f.y = ex2(m[n8][1] - top.y); m[n8][1] = top.y; l[n8][1] *= f.y; }
+            if (slab == 0 && g == 0) *reinterpret_cast<float2*>(&s_factor[half][(tile + n8) * 8 + 2 * t]) = f;
           }
         }
-      }
-      // ---- weights
-      if (ok && mine) {
+        if (slab == 0 && lane == 0) s_scaled[half][warp / SLABS] = any;
+        if (ok && mine) {
 #pragma unroll
-        for (int n8 = 0; n8 < NT; ++n8) {
-          float w[2][2];
+          for (int n8 = 0; n8 < NA; ++n8) {
+            float w[2][2];
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const float base = m[n8][k] == -INFINITY ? 0.f : m[n8][k] - K8D_LIFT;
+            for (int k = 0; k < 2; ++k) {
+              const float base = m[n8][k] == -INFINITY ? 0.f : m[n8][k] - K8D_LIFT;
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                w[i][k] = ex2(y[n8][i][k] - base);
+                l[n8][k] = fmaf(w[i][k], vi[i], l[n8][k]);
+              }
+            }
+            uint32_t pw[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              w[i][k] = ex2(y[n8][i][k] - base);
-              l[n8][k] = fmaf(w[i][k], vi[i], l[n8][k]);
+              const __half2 two = __floats2half2_rn(w[i][0], w[i][1]);
+              pw[i] = movmatrix(*reinterpret_cast<const uint32_t*>(&two));  // [column g][keys 2 t, 2 t + 1]
             }
-          }
-          uint32_t pw[2];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const __half2 two = __floats2half2_rn(w[i][0], w[i][1]);
-            pw[i] = movmatrix(*reinterpret_cast<const uint32_t*>(&two));  // [column g][keys 2 t, 2 t + 1]
-          }
-          s_w[warp][n8][lane] = make_uint2(pw[0], pw[1]);
-        }
-      }
-      ok = ok && mbar_wait_warp(&full[vs], ((2 * n + 1) / SLOTS) & 1, p.err, ERR_WAIT_FULL, abort_flag);
-      __syncthreads();
-      // ---- O[dim, column] += V^T P: dims 16 c + 2 g and + 1 of tile c are the rows g and g + 8
-      if (ok) {
-        // D = 256: the two tiles of a warp and one slab at a time; below: one tile and two slabs
-        const uint32_t vslot = smem_u32(smem_k8 + vs * C::SLOT);
-#pragma unroll
-        for (int k = 0; k < SLABS / C::SPLIT; k += C::PER == 2 ? 1 : 2) {
-          const int slab = part * (SLABS / C::SPLIT) + k;
-          if (slab >= slabs) break;
-          uint32_t r[4];
-          const int row = C::PER == 2 ? lane & 15 : lane;  // lanes 16 .. 31: the second tile, or the second slab
-          ldmatrix4_trans(tile_at(vslot + slab / 4 * C::TILE, slab % 4 * K8D_SLAB + row, C::PER == 2 ? tile0 + (lane >> 4) : tile0), r);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (C::PER == 1 && slab + h >= slabs) break;
-            uint32_t a0, a1, a2, a3;
-            kv8_unpack4(__byte_perm(r[2 * h], 0, 0x3120), a0, a1);
-            kv8_unpack4(__byte_perm(r[2 * h + 1], 0, 0x3120), a2, a3);
-#pragma unroll
-            for (int n8 = 0; n8 < NT; ++n8) {
-              const uint2 w = s_w[C::PER == 2 ? slab : slab + h][n8][lane];
-              mma_f16(o[n8][C::PER == 2 ? h : 0], a0, a1, a2, a3, w.x, w.y);
-            }
+            s_w[half][slab][tile + n8][lane] = make_uint2(pw[0], pw[1]);
           }
         }
+        sync_arrive(&w_full[half]);
       }
-    }
 
-    // ---- the sums of all keys, in the warps' order; where warps share a tile, their outputs too
+      // the unit's sums
+      const int half = j & 1;
+      ok = ok && mbar_wait_warp(&l_empty[half], ((j >> 1) & 1) ^ 1, p.err, ERR_WAIT_EMPTY, abort_flag);
+#pragma unroll
+      for (int n8 = 0; n8 < NA; ++n8)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float sum = l[n8][k];
+          sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+          if (g == 0) {
+            s_sum[half][slab][(tile + n8) * 8 + 2 * t + k] = sum;
+            if (slab == 0) s_top[half][(tile + n8) * 8 + 2 * t + k] = m[n8][k];
+          }
+        }
+      __syncwarp();
+      if (lane == 0) { mbar_arrive(&l_full[half]); mbar_arrive(&u_empty[us]); }
+    }
+    return;
+  }
+
+  // ---------------- outputs: O[dim, column], dims 16 c + 2 g and + 1 of tile c are the rows g and g + 8
+  const int ow = warp - C::SW, tile0 = ow % C::TILES * C::PER, part = ow / C::TILES;  // this warp's tiles, and which part of the keys
+  for (int j = 0;; ++j) {
+    const int us = j % K8D_UNITS;
+    ok = ok && mbar_wait_warp(&u_full[us], (j / K8D_UNITS) & 1, p.err, ERR_WAIT_FULL, abort_flag);
+    if (!ok) break;
+    const Kv8Unit u = s_unit[us];
+    if (u.rows == 0) break;
+    float o[NT][C::PER][4];
+    int lens[NT][2];  // keys of the rows of columns 2 t, 2 t + 1
 #pragma unroll
     for (int n8 = 0; n8 < NT; ++n8)
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        float sum = l[n8][k];
-        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-        if (g == 0) s_sum[warp][n8 * 8 + 2 * t + k] = sum;
+        int r, h;
+        column(n8 * 8 + 2 * t + k, r, h);
+        lens[n8][k] = r < u.rows ? kv8_length(p.positions, u.row0 + r, most) : 0;
       }
-    if (C::SPLIT > 1 && part > 0) {
+    uint16_t gates[NT][2][C::PER][2];  // of rows whose only run this is
+#pragma unroll
+    for (int n8 = 0; n8 < NT; ++n8)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        int r, h;
+        column(n8 * 8 + 2 * t + k, r, h);
+        const bool direct = r < u.rows && u.z == 0 && lens[n8][k] <= K8D_RUN;
+        const uint16_t* src = reinterpret_cast<const uint16_t*>(p.gate) + (static_cast<size_t>(u.row0 + r) * p.n_q + u.kh * p.group + h) * D + tile0 * 16 + 2 * g;
+#pragma unroll
+        for (int i = 0; i < C::PER; ++i) {
+          gates[n8][k][i][0] = direct ? __ldg(src + i * 16) : uint16_t(0);
+          gates[n8][k][i][1] = direct ? __ldg(src + i * 16 + 1) : uint16_t(0);
+        }
+      }
+#pragma unroll
+    for (int n8 = 0; n8 < NT; ++n8)
+#pragma unroll
+      for (int i = 0; i < C::PER; ++i) o[n8][i][0] = o[n8][i][1] = o[n8][i][2] = o[n8][i][3] = 0.f;
+
+    for (int key0 = 0; key0 < u.keys; key0 += KV8_PAGE, ++n) {
+      const int s = n % SLOTS, half = n & 1;
+      const int slabs = min(SLABS, (u.keys - key0 + K8D_SLAB - 1) / K8D_SLAB);
+      ok = ok && mbar_wait_warp(&v_full[s], (n / SLOTS) & 1, p.err, ERR_WAIT_FULL, abort_flag)
+           && mbar_wait_warp(&w_full[half], (n >> 1) & 1, p.err, ERR_WAIT_FULL, abort_flag);
+      if (!ok) break;
+#pragma unroll
+      for (int h = 0; h < C::HALVES; ++h) {
+        if (!s_scaled[half][h]) continue;
+#pragma unroll
+        for (int n8 = h * NA; n8 < h * NA + NA; ++n8) {
+          const float2 f = *reinterpret_cast<const float2*>(&s_factor[half][n8 * 8 + 2 * t]);
+#pragma unroll
+          for (int i = 0; i < C::PER; ++i) { o[n8][i][0] *= f.x; o[n8][i][1] *= f.y; o[n8][i][2] *= f.x; o[n8][i][3] *= f.y; }
+        }
+      }
+      const uint32_t vtile = smem_u32(s_v + s * C::TILE);
+      const auto product = [&](float (*c)[4], int stride, const uint32_t* r, int slab) {  // both halves of a column tile's second operand at hand
+        uint32_t a0, a1, a2, a3;
+        kv8_unpack4(__byte_perm(r[0], 0, 0x3120), a0, a1);
+        kv8_unpack4(__byte_perm(r[1], 0, 0x3120), a2, a3);
+#pragma unroll
+        for (int n8 = 0; n8 < NT; ++n8) {
+          const uint2 w = s_w[half][slab][n8][lane];
+          mma_f16(c[n8 * stride], a0, a1, a2, a3, w.x, w.y);
+        }
+      };
+      if constexpr (C::PER >= 2) {  // two tiles and a slab per load
+#pragma unroll
+        for (int slab = 0; slab < SLABS; ++slab) {
+          if (slab >= slabs) break;
+#pragma unroll
+          for (int i = 0; i < C::PER; i += 2) {
+            uint32_t r[4];
+            ldmatrix4_trans(tile_at(vtile, slab * K8D_SLAB + (lane & 15), tile0 + i + (lane >> 4)), r);
+            product(&o[0][i], C::PER, r, slab);
+            product(&o[0][i + 1], C::PER, r + 2, slab);
+          }
+        }
+      } else {  // a tile and two slabs per load
+#pragma unroll
+        for (int k = 0; k < SLABS / C::SPLIT; k += 2) {
+          const int slab = part * (SLABS / C::SPLIT) + k;
+          if (slab >= slabs) break;
+          uint32_t r[4];
+          ldmatrix4_trans(tile_at(vtile, slab * K8D_SLAB + lane, tile0), r);
+          product(&o[0][0], 1, r, slab);
+          if (SLABS / C::SPLIT > 1 && slab + 1 < slabs) product(&o[0][0], 1, r + 2, slab + 1);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) { mbar_arrive(&v_empty[s]); mbar_arrive(&w_empty[half]); }
+    }
+
+    // where warps share a tile, their outputs meet at the barrier of the sums
+    const int half = j & 1;
+    if constexpr (C::SPLIT > 1) {
+      ok = ok && mbar_wait_warp(&l_empty[half], ((j >> 1) & 1) ^ 1, p.err, ERR_WAIT_EMPTY, abort_flag);
 #pragma unroll
       for (int n8 = 0; n8 < NT; ++n8)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s_o[warp][n8 * 4 + i][lane] = o[n8][0][i];
+        for (int i = 0; i < 4; ++i) s_o[half][ow][n8 * 4 + i][lane] = o[n8][0][i];
+      sync_arrive(&l_full[half]);
     }
-    __syncthreads();
-    if (j % 32 == 31 && warp == 0) describe(j + 33 + lane);  // the half of the list that is done with
+    ok = ok && mbar_wait_warp(&l_full[half], (j >> 1) & 1, p.err, ERR_WAIT_FULL, abort_flag);
+    if (!ok) break;
+    if constexpr (C::SPLIT > 1) {
+#pragma unroll
+      for (int n8 = 0; n8 < NT; ++n8)
+#pragma unroll
+        for (int w = 1; w < C::SPLIT; ++w)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[n8][0][i] += part == 0 ? s_o[half][w * C::TILES + ow][n8 * 4 + i][lane] : 0.f;
+    }
     if (part == 0) {
 #pragma unroll
-      for (int n8 = 0; n8 < NT; ++n8) {
-        if (C::SPLIT > 1) {
-#pragma unroll
-          for (int w = 1; w < C::SPLIT; ++w)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[n8][0][i] += s_o[w * C::TILES + warp][n8 * 4 + i][lane];
-        }
+      for (int n8 = 0; n8 < NT; ++n8)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const int col = n8 * 8 + 2 * t + k;
-          if (col >= n_cols) continue;
+          int r, h;
+          column(n8 * 8 + 2 * t + k, r, h);
+          if (r >= u.rows) continue;
           float sum = 0.f;
 #pragma unroll
-          for (int w = 0; w < K8D_WARPS; ++w) sum += s_sum[w][col];
-          int r, h;
-          column(col, r, h);
+          for (int w = 0; w < SLABS; ++w) sum += s_sum[half][w][n8 * 8 + 2 * t + k];
+          const int len = lens[n8][k];
           const size_t head = static_cast<size_t>(u.row0 + r) * p.n_q + u.kh * p.group + h;
-          if (len[n8][k] > K8D_RUN) {
-            if (u.z * K8D_RUN < len[n8][k]) {
+          if (len > K8D_RUN) {
+            if (u.z * K8D_RUN < len) {
               const size_t slot = head * p.n_splits + u.z;
-              if (tile0 == 0 && g == 0) p.part_ml[slot] = make_float2(m[n8][k], sum);
+              if (tile0 == 0 && g == 0) p.part_ml[slot] = make_float2(s_top[half][n8 * 8 + 2 * t + k], sum);
 #pragma unroll
               for (int i = 0; i < C::PER; ++i)
                 *reinterpret_cast<float2*>(p.part_acc + slot * D + (tile0 + i) * 16 + 2 * g) = make_float2(o[n8][i][k], o[n8][i][2 + k]);
             }
           } else if (u.z == 0) {  // the row's only run
-            const float inv = len[n8][k] > 0 ? 1.0f / sum : 0.f;
+            const float inv = len > 0 ? 1.0f / sum : 0.f;
 #pragma unroll
             for (int i = 0; i < C::PER; ++i) {
               const size_t at = head * D + (tile0 + i) * 16 + 2 * g;
               *reinterpret_cast<__nv_bfloat162*>(p.out + at) =
-                  __floats2bfloat162_rn(o[n8][i][k] * inv * sigmoid_f(__bfloat162float(p.gate[at])),
-                                        o[n8][i][2 + k] * inv * sigmoid_f(__bfloat162float(p.gate[at + 1])));
+                  __floats2bfloat162_rn(o[n8][i][k] * inv * sigmoid_f(__uint_as_float(static_cast<uint32_t>(gates[n8][k][i][0]) << 16)),
+                                        o[n8][i][2 + k] * inv * sigmoid_f(__uint_as_float(static_cast<uint32_t>(gates[n8][k][i][1]) << 16)));
             }
           }
         }
-      }
     }
-  }
-  if (warp == K8D_WARPS - 1 && *abort_flag) {  // a wait that ran out leaves loads on their way: they end before the shared memory goes
-    for (int i = max(0, issued - SLOTS); i < issued; ++i) {
-      const long long t0 = clock64();
-      while (!mbar_try_wait(&full[i % SLOTS], (i / SLOTS) & 1) && clock64() - t0 < WAIT_CYCLES) {}
-    }
+    __syncwarp();
+    if (lane == 0) { mbar_arrive(&l_empty[half]); mbar_arrive(&u_empty[us]); }
   }
 }
 
-// Rows of more than one run: their partials in the order of the runs, four sums of every fourth partial each.
+// Rows of more than one run. Partial z goes to sum z % 16, at the sum's own maximum, and the sums are added in order: one chain over
+// the partials where there are up to 16. What does not come from the kernel in front is read ahead of the dependency wait: that kernel has
+// waited for everything before it.
+constexpr int K8D_SUMS = 16;
+// Sums i0 .. i0 + 3 of four dims, their partials `D` floats apart.
 template <int D>
-__global__ void __launch_bounds__(D)
-kv8_combine_kernel(const float* part_acc, const float2* part_ml, const bf16* gate, const int64_t* positions, bf16* out, int n_q,
-                   int n_splits, int most) {
+__device__ __forceinline__ void k8d_sums(const float4* pa, const float2* ml, int runs, int i0, float* top, float* l, float4* acc) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { top[i] = -INFINITY; l[i] = 0.f; acc[i] = make_float4(0.f, 0.f, 0.f, 0.f); }
+#pragma unroll 4
+  for (int z0 = i0; z0 < runs; z0 += K8D_SUMS)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (z0 + i < runs) top[i] = fmaxf(top[i], ml[z0 + i].x);
+#pragma unroll 2
+  for (int z0 = i0; z0 < runs; z0 += K8D_SUMS) {
+    float2 pm[4];
+    float4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      pm[i] = z0 + i < runs ? ml[z0 + i] : make_float2(-INFINITY, 0.f);
+      v[i] = z0 + i < runs ? pa[static_cast<size_t>(z0 + i) * (D / 4)] : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float f = pm[i].x == top[i] ? 1.f : ex2(pm[i].x - top[i]);
+      l[i] = fmaf(pm[i].y, f, l[i]);  // a partial without a maximum holds no key, or scores that are all NaN, in its sum
+      acc[i].x = fmaf(v[i].x, f, acc[i].x); acc[i].y = fmaf(v[i].y, f, acc[i].y);
+      acc[i].z = fmaf(v[i].z, f, acc[i].z); acc[i].w = fmaf(v[i].w, f, acc[i].w);
+    }
+  }
+}
+__device__ __forceinline__ void k8d_add(float best, float top, float l, const float4& acc, float& sum, float4& o) {
+  const float f = top == best ? 1.f : ex2(top - best);
+  sum = fmaf(l, f, sum);
+  o.x = fmaf(acc.x, f, o.x); o.y = fmaf(acc.y, f, o.y); o.z = fmaf(acc.z, f, o.z); o.w = fmaf(acc.w, f, o.w);
+}
+__device__ __forceinline__ void k8d_store(bf16* out, const bf16* gate, const float4& o, float sum) {
+  const float inv = 1.0f / sum;
+  uint2 raw;
+  __nv_bfloat162* e = reinterpret_cast<__nv_bfloat162*>(&raw);
+  e[0] = __floats2bfloat162_rn(o.x * inv * sigmoid_f(__bfloat162float(gate[0])), o.y * inv * sigmoid_f(__bfloat162float(gate[1])));
+  e[1] = __floats2bfloat162_rn(o.z * inv * sigmoid_f(__bfloat162float(gate[2])), o.w * inv * sigmoid_f(__bfloat162float(gate[3])));
+  *reinterpret_cast<uint2*>(out) = raw;
+}
+// Tables of up to 64 runs (16,384 keys): a thread takes all sums of four dims of a head.
+template <int D>
+__global__ void __launch_bounds__(256)
+kv8_combine_few_kernel(const float* part_acc, const float2* part_ml, const bf16* gate, const int64_t* positions, bf16* out, int heads,
+                       int n_q, int n_splits, int most) {
   constexpr int QUADS = D / 4;
-  __shared__ __align__(16) float s_acc[4][D];
-  __shared__ float s_l[4];
+  const size_t head = static_cast<size_t>(blockIdx.x) * (256 / QUADS) + threadIdx.x / QUADS;
+  const int quad = threadIdx.x % QUADS;
+  const int runs = head < heads ? (kv8_length(positions, static_cast<int>(head / n_q), most) + K8D_RUN - 1) / K8D_RUN : 0;
   pdl_wait();
   pdl_launch();
-  const int row = blockIdx.x;
-  const int len = max(0, min(static_cast<int>(min(positions[row], static_cast<int64_t>(most))) + 1, most));
-  if (len <= K8D_RUN) return;
-  const int runs = (len + K8D_RUN - 1) / K8D_RUN;
-  const size_t head = static_cast<size_t>(row) * n_q + blockIdx.y;
+  if (runs <= 1) return;
   const float2* ml = part_ml + head * n_splits;
-  const int quad = threadIdx.x % QUADS, part = threadIdx.x / QUADS;
-  float top = -INFINITY;
-  for (int z = 0; z < runs; ++z) top = fmaxf(top, ml[z].x);
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float l = 0.f;
   const float4* pa = reinterpret_cast<const float4*>(part_acc + head * n_splits * D) + quad;
-#pragma unroll 4
-  for (int z = part; z < runs; z += 4) {
-    const float2 pm = ml[z];
-    const float4 v = pa[static_cast<size_t>(z) * QUADS];
-    const float f = pm.x == -INFINITY ? 1.f : ex2(pm.x - top);  // without a maximum: scores that are all NaN, in the sum
-    l = fmaf(pm.y, f, l);
-    acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y); acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
+  float best = -INFINITY, sum = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int z = 0; z < runs; ++z) best = fmaxf(best, ml[z].x);
+  for (int i = 0; i < K8D_SUMS && i < runs; i += 4) {
+    float top[4], l[4];
+    float4 acc[4];
+    k8d_sums<D>(pa, ml, runs, i, top, l, acc);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) k8d_add(best, top[k], l[k], acc[k], sum, o);
   }
-  *reinterpret_cast<float4*>(&s_acc[part][quad * 4]) = acc;
-  if (quad == 0) s_l[part] = l;
+  const size_t at = head * D + quad * 4;
+  k8d_store(out + at, gate + at, o, sum);
+}
+// More: a CTA takes up to 64 dims of a head, a thread one sum of four of them; rows of few runs as above.
+template <int D>
+__global__ void __launch_bounds__(256)
+kv8_combine_kernel(const float* part_acc, const float2* part_ml, const bf16* gate, const int64_t* positions, bf16* out, int n_q,
+                   int n_splits, int most) {
+  constexpr int DIMS = D < 64 ? D : 64, QUADS = DIMS / 4;
+  __shared__ float4 s_acc[K8D_SUMS][QUADS];
+  __shared__ float s_top[K8D_SUMS], s_l[K8D_SUMS];
+  const size_t head = blockIdx.x;
+  const int quad = threadIdx.x % QUADS, i = threadIdx.x / QUADS;
+  const int runs = (kv8_length(positions, static_cast<int>(head / n_q), most) + K8D_RUN - 1) / K8D_RUN;
+  pdl_wait();
+  pdl_launch();
+  if (runs <= 1) return;
+  const float2* ml = part_ml + head * n_splits;
+  const float4* pa = reinterpret_cast<const float4*>(part_acc + head * n_splits * D + blockIdx.y * DIMS) + quad;
+  if (i < K8D_SUMS) {
+    float top = -INFINITY, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int z = i; z < runs; z += K8D_SUMS) top = fmaxf(top, ml[z].x);
+#pragma unroll 4
+    for (int z = i; z < runs; z += K8D_SUMS) {
+      const float2 pm = ml[z];
+      const float4 v = pa[static_cast<size_t>(z) * (D / 4)];
+      k8d_add(top, pm.x, pm.y, v, l, acc);
+    }
+    s_acc[i][quad] = acc;
+    if (quad == 0) { s_top[i] = top; s_l[i] = l; }
+  }
   __syncthreads();
-  const int d = threadIdx.x;
-  const float sum = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
-  const float o = (s_acc[0][d] + s_acc[1][d]) + (s_acc[2][d] + s_acc[3][d]);
-  out[head * D + d] = __float2bfloat16(o / sum * sigmoid_f(__bfloat162float(gate[head * D + d])));
+  if (i > 0) return;
+  float best = -INFINITY, sum = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int k = 0; k < K8D_SUMS; ++k) best = fmaxf(best, s_top[k]);
+  for (int k = 0; k < K8D_SUMS; ++k) k8d_add(best, s_top[k], s_l[k], s_acc[k][quad], sum, o);
+  const size_t at = head * D + blockIdx.y * DIMS + quad * 4;
+  k8d_store(out + at, gate + at, o, sum);
 }
 
 }  // namespace b200
@@ -560,7 +756,7 @@ namespace {
 typedef CUresult (*K8dEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
                                 CUtensorMapFloatOOBfill);
-int k8d_make_map(CUtensorMap* m, const void* data, int D, long long rows) {
+int k8d_encode(CUtensorMap* m, const void* base, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle sw) {
   static K8dEncodeFn fn = nullptr;
   if (!fn) {
     void* ptr = nullptr;
@@ -568,17 +764,25 @@ int k8d_make_map(CUtensorMap* m, const void* data, int D, long long rows) {
     if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) != cudaSuccess || !ptr) return -1;
     fn = reinterpret_cast<K8dEncodeFn>(ptr);
   }
-  const int rowb = D < 128 ? D : 128;
-  cuuint64_t dims[3] = {static_cast<cuuint64_t>(rowb), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(D / rowb)};
-  cuuint64_t strides[2] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(rowb)};
-  cuuint32_t box[3] = {static_cast<cuuint32_t>(rowb), KV8_PAGE, static_cast<cuuint32_t>(D / rowb)}, estr[3] = {1, 1, 1};
-  const CUtensorMapSwizzle sw = rowb == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : rowb == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(data), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
+  const cuuint32_t estr[3] = {1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
             CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : -2;
+}
+// A page's keys or values of one head, in blocks of at most 128 bytes per row; their exponents, of keys and values together.
+int k8d_make_maps(CUtensorMap* tm, CUtensorMap* tm_exps, const void* data, const void* exps, int D, int n_kv, long long pages) {
+  const cuuint32_t rowb = D < 128 ? D : 128;
+  const cuuint64_t dims[3] = {rowb, static_cast<cuuint64_t>(pages) * 2 * n_kv * KV8_PAGE, D / rowb};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(D), rowb};
+  const cuuint32_t box[3] = {rowb, KV8_PAGE, D / rowb};
+  const cuuint64_t edims[3] = {KV8_PAGE, static_cast<cuuint64_t>(n_kv), static_cast<cuuint64_t>(pages) * 2};
+  const cuuint64_t estrides[2] = {KV8_PAGE, static_cast<cuuint64_t>(n_kv) * KV8_PAGE};
+  const cuuint32_t ebox[3] = {KV8_PAGE, 1, 2};
+  const int rc = k8d_encode(tm, data, dims, strides, box, rowb == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : rowb == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B);
+  return rc ? rc : k8d_encode(tm_exps, exps, edims, estrides, ebox, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 template <int D, int NT>
-int k8d_launch(const CUtensorMap& tm, const Kv8DecodeParams& p, cudaStream_t st) {
+int k8d_launch(const CUtensorMap& tm, const CUtensorMap& tm_exps, const Kv8DecodeParams& p, cudaStream_t st) {
   auto kern = kv8_decode_kernel<D, NT>;
   static int sms_of[64] = {};  // per device, with the function attribute set
   int dev = 0;
@@ -592,11 +796,16 @@ int k8d_launch(const CUtensorMap& tm, const Kv8DecodeParams& p, cudaStream_t st)
   const long long units = static_cast<long long>(p.B) * p.units_per_seq * p.n_kv * p.n_splits;
   const int most_ctas = sms_of[dev] * Kv8DecodeCfg<D, NT>::CTAS;
   const int grid = static_cast<int>(units < most_ctas ? units : most_ctas);
-  if (launch_pdl(kern, dim3(grid), dim3(32 * K8D_WARPS), Kv8DecodeCfg<D, NT>::SMEM, st, tm, p) != cudaSuccess) return -4;
+  if (launch_pdl(kern, dim3(grid), dim3(Kv8DecodeCfg<D, NT>::THREADS), Kv8DecodeCfg<D, NT>::SMEM, st, tm, tm_exps, p) != cudaSuccess) return -4;
   if (p.n_splits == 1) return 0;
   const int most = (p.width < p.n_splits * (K8D_RUN / KV8_PAGE) ? p.width : p.n_splits * (K8D_RUN / KV8_PAGE)) * KV8_PAGE;
-  return launch_pdl(kv8_combine_kernel<D>, dim3(p.B * p.G, p.n_q), dim3(D), 0, st, p.part_acc, p.part_ml, p.gate, p.positions, p.out,
-                    p.n_q, p.n_splits, most) == cudaSuccess ? 0 : -4;
+  const int heads = p.B * p.G * p.n_q, per = 256 / (D / 4);
+  const cudaError_t rc = p.n_splits <= 64
+      ? launch_pdl(kv8_combine_few_kernel<D>, dim3((heads + per - 1) / per), dim3(256), 0, st, p.part_acc, p.part_ml, p.gate,
+                   p.positions, p.out, heads, p.n_q, p.n_splits, most)
+      : launch_pdl(kv8_combine_kernel<D>, dim3(heads, D < 64 ? 1 : D / 64), dim3(256), 0, st, p.part_acc, p.part_ml, p.gate,
+                   p.positions, p.out, p.n_q, p.n_splits, most);
+  return rc == cudaSuccess ? 0 : -4;
 }
 }  // namespace
 
@@ -615,11 +824,14 @@ extern "C" int b200_kv8_decode(const void* q, const void* gate, const void* data
   const long long rows = static_cast<long long>(num_pages) * 2 * n_kv * KV8_PAGE;
   if (rows > 0x7fffffffLL) return -7;  // a TMA coordinate
   if (reinterpret_cast<uintptr_t>(data) % 16 || reinterpret_cast<uintptr_t>(exps) % 16 || reinterpret_cast<uintptr_t>(q) % 8) return -7;
-  CUtensorMap tm;
-  if (k8d_make_map(&tm, data, D, rows)) return -1;
+  if (D != 256 && D != 128 && D != 64 && D != 32) return -7;
+  CUtensorMap tm, tm_exps;
+  if (k8d_make_maps(&tm, &tm_exps, data, exps, D, n_kv, num_pages)) return -1;
   const int cols = G * group, nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4, per = 8 * nt / group < G ? 8 * nt / group : G;
-  for (int b0 = 0; b0 < B; b0 += K8D_MAX_SEQS) {
-    const int n = B - b0 < K8D_MAX_SEQS ? B - b0 : K8D_MAX_SEQS;
+  int rc = -7;
+  for (int b0 = 0; b0 < B; b0 += K8D_SEQS) {
+    const int n = B - b0 < K8D_SEQS ? B - b0 : K8D_SEQS;
+    if (static_cast<long long>(n) * G * n_kv * n_splits > 0x3fffffffLL) return -7;  // the units are counted in 32 bits
     const size_t heads = static_cast<size_t>(b0) * G * n_q;
     const Kv8DecodeParams p{static_cast<const bf16*>(q) + heads * D, static_cast<const bf16*>(gate) + heads * D,
                             static_cast<const uint8_t*>(exps), positions + static_cast<size_t>(b0) * G,
@@ -627,12 +839,11 @@ extern "C" int b200_kv8_decode(const void* q, const void* gate, const void* data
                             part_acc + heads * n_splits * D, reinterpret_cast<float2*>(part_ml) + heads * n_splits,
                             n, G, max_pages, width, num_pages, n_q, n_kv, group, n_splits, per, (G + per - 1) / per, (65536 + group - 1) / group,
                             1.4426950408889634f / sqrtf(static_cast<float>(D)), err};
-    int rc = -7;
-#define K8D(DD) rc = nt == 1 ? k8d_launch<DD, 1>(tm, p, st) : nt == 2 ? k8d_launch<DD, 2>(tm, p, st) : k8d_launch<DD, 4>(tm, p, st)
+#define K8D(DD) rc = nt == 1 ? k8d_launch<DD, 1>(tm, tm_exps, p, st) : nt == 2 ? k8d_launch<DD, 2>(tm, tm_exps, p, st) : k8d_launch<DD, 4>(tm, tm_exps, p, st)
     if (D == 256) K8D(256);
     else if (D == 128) K8D(128);
     else if (D == 64) K8D(64);
-    else if (D == 32) K8D(32);
+    else K8D(32);
 #undef K8D
     if (rc) return rc;
   }
