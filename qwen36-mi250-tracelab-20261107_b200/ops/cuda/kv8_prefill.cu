@@ -1,0 +1,636 @@
+// Causal gated attention of spans of new tokens over the 8-bit paged cache, on tcgen05.
+//
+//   s_ij = q_i . (k_j 2^a_j) / sqrt D,   o_i = sum_j p_ij (v_j 2^b_j) / sum_j p_ij over the keys j up to i's position,   out = o * sigmoid(gate)
+//
+// A tile is 128 MMA rows = (128 / group) consecutive positions of a span x the query heads of one KV head, as in flash_prefill.cu; a
+// page of 64 keys at a time:
+//
+//   S[128 x 64]  = Q1 K^T + Q2 K^T     the page's e4m3 bytes as TMA brought them (kind::f8f6f4, twice the rate of bf16). A bf16 query row,
+//                                      scaled by a power of two, is Q1 + Q2 in e4m3: exact but for what lies 2^-17 below its largest number
+//   y = s a_j' + b_j                   the key's power of two and, in the exponent, the value's: w = 2^(y - M + LIFT) weighs the stored
+//                                      v_j, M the running maximum of y; the softmax's own sum is sum_j w 2^-b_j
+//   O[128 x D]  += P[128 x 64] V       P and V as halves: four warps make them of the page's bytes (exact)
+//
+// Two groups of four warps take alternate pages, a thread a row; the running maximum goes from one to the other, and the output tile in
+// TMEM is rescaled where a maximum grew by more than 2^LAZY. Weights as halves reach from 2^15 to 2^-24, 2^-31 of the largest at the least.
+// A span of few tiles over a long context is cut into runs of pages for CTAs of their own, by its own length and position alone, whose partial
+// sums are added in their order: a row's bits depend on its span, never on the pass. All waits are bounded. No cluster multicast.
+#include <cuda_fp16.h>
+
+#include "kv8.cuh"
+
+namespace b200 {
+
+constexpr float K8P_LIFT = 7.0f, K8P_LAZY = 8.0f;  // weights stay below 2^15
+constexpr int K8P_THREADS = 448;                   // 8 warps softmax, MMA, loads, 4 warps values
+constexpr int K8P_CTAS = 128, K8P_MIN_PAGES = 4;   // a span is cut for about so many CTAs, into runs of no fewer pages
+
+struct Kv8PrefillParams {
+  const bf16* q;            // [T, n_q, D]
+  const bf16* gate;         // [T, n_q * D]
+  const int* starts;        // [segs + 1] first row of each span
+  const int* pos0;          // [segs] its position
+  const int* tables;        // [segs] rows of `width` pages, max_pages apart
+  bf16* out;                // [T, n_q * D]
+  float* part_acc;          // [T, n_q, max_splits, D]: of spans that are cut
+  float2* part_ml;          // [T, n_q, max_splits]
+  int segs, max_pages, width, num_pages, n_q, n_kv, group, positions, max_splits;  // positions: of a tile
+  float scale_log2;
+  int* err;
+};
+
+template <int D>
+struct Kv8PrefillCfg {
+  static constexpr int ROWB = D < 128 ? D : 128;       // bytes of a row in one swizzled block of stored numbers
+  static constexpr int DB = D / ROWB;
+  static constexpr int HB = D / 64;                    // 128-byte blocks of a row of halves
+  static constexpr int Q_TERM = 128 * D;               // [DB][128 rows][ROWB]; two terms
+  static constexpr int PAGE_BYTES = KV8_PAGE * D;      // [DB][64 rows][ROWB]: keys or values of a page
+  static constexpr int V_BYTES = KV8_PAGE * D * 2;     // [HB][64 rows][128]: values as halves
+  static constexpr int P_BYTES = 128 * 128;            // [128 rows][64 halves]
+  static constexpr int EXPS = 2 * KV8_PAGE;
+  static constexpr int SMEM = 2 * Q_TERM + 4 * PAGE_BYTES + 2 * V_BYTES + 2 * P_BYTES + 4 * EXPS + 2 * 3 * KV8_PAGE * 4 + 512 + 256;
+  static constexpr int TMEM_COLS = 128 + D <= 256 ? 256 : 512;
+};
+
+// Runs that a span of n rows whose last key is in page np - 1 is cut into, and their pages: by the span alone.
+__host__ __device__ __forceinline__ int k8p_run_pages(int n, int np, int positions, int n_kv) {
+  const int ctas = (n + positions - 1) / positions * n_kv;
+  const int cuts = K8P_CTAS / (ctas > 0 ? ctas : 1);
+  if (cuts <= 1) return np;
+  const int pages = (np + cuts - 1) / cuts;
+  return pages < K8P_MIN_PAGES ? K8P_MIN_PAGES : pages;
+}
+
+__device__ __forceinline__ void k8p_umma_f8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// K-major operand tile in rows of ROWB bytes (64 or 128) written with the swizzle of that size, groups of eight rows after each other.
+template <int ROWB>
+__device__ __forceinline__ uint64_t k8p_desc(uint32_t addr) {
+  return static_cast<uint64_t>((addr & 0x3FFFF) >> 4) | static_cast<uint64_t>(1) << 16 | static_cast<uint64_t>(8 * ROWB >> 4) << 32 |
+         static_cast<uint64_t>(1) << 46 | static_cast<uint64_t>(ROWB == 128 ? 2 : 4) << 61;
+}
+// Offset of 16 bytes of such a tile: row r, chunk c.
+template <int ROWB>
+__device__ __forceinline__ uint32_t k8p_at(int r, int c) {
+  const uint32_t byte = r * ROWB;
+  return byte + ((c ^ ((byte >> 7) & (ROWB / 16 - 1))) << 4);
+}
+__device__ __forceinline__ float k8p_ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// Two floats at a time.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(r)) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<uint64_t&>(r))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+  return r;
+}
+
+// The tile of a CTA: found among the spans' tiles by all lanes of a warp, 32 spans at a time. false: there is none.
+struct Kv8Tile { int seg, p0, row0, rows, pos0; };
+__device__ __forceinline__ bool k8p_find(const Kv8PrefillParams& p, int tile, Kv8Tile& t) {
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  for (int s0 = 0; s0 < p.segs; s0 += 32) {
+    const int s = s0 + lane;
+    const int a = s < p.segs ? p.starts[s] : 0, n = s < p.segs ? p.starts[s + 1] - a : 0;
+    const int tiles = (n + p.positions - 1) / p.positions;
+    int upto = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += u;
+    }
+    upto += before;
+    const uint32_t hit = __ballot_sync(0xffffffffu, tile < upto);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      t.seg = s0 + l;
+      t.row0 = __shfl_sync(0xffffffffu, a, l);
+      t.rows = __shfl_sync(0xffffffffu, n, l);
+      t.p0 = (tile - __shfl_sync(0xffffffffu, upto - tiles, l)) * p.positions;
+      t.pos0 = p.pos0[t.seg];
+      return true;
+    }
+    before = __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return false;
+}
+
+template <int D>
+__global__ void __launch_bounds__(K8P_THREADS, 1)
+kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtensorMap tm_exps, Kv8PrefillParams p) {
+  using C = Kv8PrefillCfg<D>;
+  extern __shared__ __align__(1024) uint8_t smem_k8p[];
+  if (smem_u32(smem_k8p) & 1023u) {  // the swizzled tiles need this alignment
+    if (threadIdx.x == 0) atomicCAS(p.err, 0, ERR_BAD_INDEX);
+    return;
+  }
+  uint8_t* const sQ = smem_k8p;                          // [2 terms]
+  uint8_t* const sK = sQ + 2 * C::Q_TERM;                // [2]
+  uint8_t* const sV8 = sK + 2 * C::PAGE_BYTES;           // [2]
+  uint8_t* const sV = sV8 + 2 * C::PAGE_BYTES;           // [2]
+  uint8_t* const sP = sV + 2 * C::V_BYTES;               // [2]: page i uses tile i & 1
+  uint8_t* const sE = sP + 2 * C::P_BYTES;               // [4][keys' 64, values' 64] exponents
+  float* const sT = reinterpret_cast<float*>(sE + 4 * C::EXPS);  // [2][2^a | b | 2^-b][64]
+  float* const s_m = sT + 2 * 3 * KV8_PAGE;              // [128] the running maximum of a row, in the hands of the page that is to see its scores next
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(s_m + 128);
+  uint64_t* const k_full = bars;                         // [2]
+  uint64_t* const k_empty = bars + 2;                    // [2]
+  uint64_t* const v8_full = bars + 4;                    // [2]
+  uint64_t* const v8_empty = bars + 6;                   // [2]
+  uint64_t* const v_full = bars + 8;                     // [2]
+  uint64_t* const v_empty = bars + 10;                   // [2]
+  uint64_t* const s_full = bars + 12;                    // [2]
+  uint64_t* const p_full = bars + 14;                    // [2]
+  uint64_t* const pv_done = bars + 16;                   // [2]
+  uint64_t* const e_full = bars + 18;                    // [4]
+  uint64_t* const t_full = bars + 22;                    // [2]
+  uint64_t* const acc_done = bars + 24;
+  uint64_t* const x_bar = bars + 25;
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 26);
+  volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  uint64_t* const m_bar = bars + 27;                     // [2]: the row maxima up to an even / odd page
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_wait();
+  Kv8Tile tile;
+  // the last tiles of the spans see the most keys and go first
+  if (!k8p_find(p, static_cast<int>(gridDim.x - 1 - blockIdx.x), tile)) return;
+  const int kh = blockIdx.y, n_pos = min(p.positions, tile.rows - tile.p0);
+  const int most = p.width;
+  const int np_all = min(most, (tile.pos0 + tile.p0 + n_pos - 1) / KV8_PAGE + 1);            // pages that the tile's rows see
+  const int run_pages = p.max_splits > 1 ? k8p_run_pages(tile.rows, min(most, (tile.pos0 + tile.rows - 1) / KV8_PAGE + 1), p.positions, p.n_kv) : most;
+  const bool cut = p.max_splits > 1 && run_pages < min(most, (tile.pos0 + tile.rows - 1) / KV8_PAGE + 1);
+  const int first = static_cast<int>(blockIdx.z) * run_pages, np = min(np_all, first + run_pages) - first;
+  if (np <= 0) return;  // nothing of this run for these rows: the sum over the runs passes over it
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); mbar_init(&v8_full[s], 1); mbar_init(&v8_empty[s], 128);
+      mbar_init(&v_full[s], 128); mbar_init(&v_empty[s], 1); mbar_init(&s_full[s], 1); mbar_init(&p_full[s], 128);
+      mbar_init(&pv_done[s], 1); mbar_init(&t_full[s], 128); mbar_init(&m_bar[s], 128);
+    }
+    for (int s = 0; s < 4; ++s) mbar_init(&e_full[s], 1);
+    mbar_init(acc_done, 1);
+    mbar_init(x_bar, 256);
+    *abort_flag = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&tm);
+    tma_prefetch_desc(&tm_exps);
+  }
+  if (warp == 8) { tmem_alloc(tmem_slot, C::TMEM_COLS); tmem_relinquish(); }
+  float* const s_qs = reinterpret_cast<float*>(sP);      // until the rows' threads have read it
+  // ---- queries: a warp a row at a time, two terms of e4m3; the largest number of a row comes to [128, 256)
+  for (int r0 = warp; r0 < 128; r0 += K8P_THREADS / 32 * 4) {
+    uint4 raw[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = r0 + i * (K8P_THREADS / 32), lp = r / p.group;
+      raw[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (r < 128 && lp < n_pos && lane * 8 < D)
+        raw[i] = *reinterpret_cast<const uint4*>(p.q + (static_cast<size_t>(tile.row0 + tile.p0 + lp) * p.n_q + kh * p.group + r % p.group) * D + lane * 8);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = r0 + i * (K8P_THREADS / 32);
+      if (r >= 128) break;
+      const __nv_bfloat162* e2 = reinterpret_cast<const __nv_bfloat162*>(&raw[i]);
+      float x[8];
+      float top = 0.f;
+      bool bad = false;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = __bfloat1622float2(e2[k]);
+        x[2 * k] = f.x;
+        x[2 * k + 1] = f.y;
+        top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+        bad |= !(fabsf(f.x) <= 3.4e38f && fabsf(f.y) <= 3.4e38f);
+      }
+      top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));  // not negative: in the order of its bits
+      const int e = max(-110, min(110, static_cast<int>(__float_as_uint(top) >> 23) - 127 - 7));
+      const float f = kv8_two_to(-e);
+      uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
+#pragma unroll
+      for (int k = 0; k < 8; k += 2) {
+        const float a = x[k] * f, b = x[k + 1] * f;
+        const uint32_t two = kv8_pack2(a, b), hh = kv8_unpack2(static_cast<uint16_t>(two));
+        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hh));
+        hi[k / 4] |= two << (8 * (k & 3));
+        lo[k / 4] |= kv8_pack2(a - back.x, b - back.y) << (8 * (k & 3));
+      }
+      if (lane * 8 < D) {
+        const int blk = lane * 8 / C::ROWB, in = lane * 8 % C::ROWB;
+        uint8_t* const at = sQ + blk * 128 * C::ROWB + k8p_at<C::ROWB>(r, in >> 4) + (in & 15);
+        *reinterpret_cast<uint2*>(at) = make_uint2(hi[0], hi[1]);
+        *reinterpret_cast<uint2*>(at + C::Q_TERM) = make_uint2(lo[0], lo[1]);
+      }
+      const bool any = __any_sync(0xffffffffu, bad);  // a NaN or an infinity: all scores of the row are NaN
+      if (lane == 0) s_qs[r] = any ? __uint_as_float(0x7fffffffu) : kv8_two_to(e) * p.scale_log2;
+    }
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const float qs = threadIdx.x < 256 ? s_qs[threadIdx.x & 127] : 0.f;
+  const uint32_t tmem = *tmem_slot;
+  __syncthreads();
+  pdl_launch();  // this CTA holds its TMEM columns
+  const uint32_t tmem_S = tmem, tmem_O = tmem + 128;     // score tile of page i at tmem_S + (i & 1) * 64
+
+  if (warp == 9) {
+    // ---------------- loads
+    if (elect_one()) {
+      const int* table = p.tables + static_cast<size_t>(tile.seg) * p.max_pages + first;
+      int next = table[0];
+      for (int i = 0; i < np; ++i) {
+        const int s = i & 1;
+        int page = next;
+        if (i + 1 < np) next = table[i + 1];
+        if (page < 0 || page >= p.num_pages) { atomicCAS(p.err, 0, ERR_BAD_INDEX); page = 0; }
+        const int row = (page * 2 * p.n_kv + kh) * KV8_PAGE;
+        // (the exponents' slot of page i was read before the scores of page i - 2 were asked for)
+        if (!mbar_wait(&k_empty[s], ((i >> 1) & 1) ^ 1, p.err, ERR_WAIT_EMPTY, abort_flag)) break;
+        mbar_expect_tx(&k_full[s], C::PAGE_BYTES);
+#pragma unroll
+        for (int b = 0; b < C::DB; ++b)
+          tma_load_2d(sK + s * C::PAGE_BYTES + b * KV8_PAGE * C::ROWB, &tm, &k_full[s], b * C::ROWB, row);
+        mbar_expect_tx(&e_full[i & 3], C::EXPS);
+        tma_load_3d(sE + (i & 3) * C::EXPS, &tm_exps, &e_full[i & 3], 0, kh, page * 2);
+        if (!mbar_wait(&v8_empty[s], ((i >> 1) & 1) ^ 1, p.err, ERR_WAIT_EMPTY, abort_flag)) break;
+        mbar_expect_tx(&v8_full[s], C::PAGE_BYTES);
+#pragma unroll
+        for (int b = 0; b < C::DB; ++b)
+          tma_load_2d(sV8 + s * C::PAGE_BYTES + b * KV8_PAGE * C::ROWB, &tm, &v8_full[s], b * C::ROWB, row + p.n_kv * KV8_PAGE);
+      }
+    }
+  } else if (warp == 8) {
+    // ---------------- MMAs
+    if (elect_one()) {
+      constexpr uint32_t idesc_s = (1u << 4) | (64u >> 3) << 17 | (128u >> 4) << 24;                                     // e4m3
+      constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | static_cast<uint32_t>(D >> 3) << 17 | (128u >> 4) << 24;     // halves, B MN-major
+      const uint32_t qa = smem_u32(sQ);
+      auto issue_qk = [&](int i) {
+        const int s = i & 1;
+        if (!mbar_wait(&k_full[s], (i >> 1) & 1, p.err, ERR_WAIT_FULL, abort_flag)) return false;
+        tc_fence_after();
+        const uint32_t ka = smem_u32(sK + s * C::PAGE_BYTES);
+#pragma unroll
+        for (int term = 0; term < 2; ++term)
+#pragma unroll
+          for (int kk = 0; kk < D / 32; ++kk) {
+            constexpr int STEPS = C::ROWB / 32;
+            const int blk = kk / STEPS, off = kk % STEPS * 32;
+            k8p_umma_f8(tmem_S + s * 64, k8p_desc<C::ROWB>(qa + term * C::Q_TERM + blk * 128 * C::ROWB + off),
+                        k8p_desc<C::ROWB>(ka + blk * KV8_PAGE * C::ROWB + off), idesc_s, (term | kk) != 0);
+          }
+        umma_commit(&s_full[s]);
+        umma_commit(&k_empty[s]);
+        return true;
+      };
+      bool ok = issue_qk(0) && (np < 2 || issue_qk(1));
+      for (int i = 0; i < np && ok; ++i) {
+        const int s = i & 1;
+        // the weights of page i are written, so its score tile has been read: the scores of page i + 2 go first
+        ok = mbar_wait(&p_full[s], (i >> 1) & 1, p.err, ERR_WAIT_FULL, abort_flag);
+        if (ok && i + 2 < np) ok = issue_qk(i + 2);
+        ok = ok && mbar_wait(&v_full[s], (i >> 1) & 1, p.err, ERR_WAIT_FULL, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t pa = smem_u32(sP + s * C::P_BYTES), va = smem_u32(sV + s * C::V_BYTES);
+#pragma unroll
+        for (int kk = 0; kk < KV8_PAGE / 16; ++kk)
+          umma_bf16(tmem_O, umma_smem_desc(pa + kk * 32), umma_smem_desc_mn(va + kk * 2048, KV8_PAGE * 128), idesc_o, (i | kk) != 0);
+        umma_commit(&pv_done[s]);
+        umma_commit(&v_empty[s]);
+      }
+      umma_commit(acc_done);
+    }
+  } else if (warp >= 10) {
+    // ---------------- values: bytes to halves; the numbers that go with a page's keys
+    const int tid = threadIdx.x - 320;
+    bool ok = true;
+    for (int i = 0; i < np; ++i) {
+      const int s = i & 1;
+      ok = mbar_wait(&e_full[i & 3], (i >> 2) & 1, p.err, ERR_WAIT_FULL, abort_flag)
+           && (i < 2 || mbar_wait(&p_full[s], ((i - 2) >> 1) & 1, p.err, ERR_WAIT_FULL, abort_flag));
+      if (!ok) break;
+      const uint32_t byte = sE[(i & 3) * C::EXPS + tid];  // threads 0 .. 63: a key's, then a value's
+      float* const t = sT + s * 3 * KV8_PAGE;
+      if (tid < KV8_PAGE) {
+        t[tid] = kv8_factor(byte);
+      } else {
+        t[tid] = byte == KV8_E_NAN ? __uint_as_float(0x7fffffffu) : static_cast<float>(static_cast<int>(byte) - 127);
+        t[KV8_PAGE + tid] = kv8_two_to(max(-126, 127 - static_cast<int>(byte)));
+      }
+      mbar_arrive(&t_full[s]);
+      ok = mbar_wait(&v8_full[s], (i >> 1) & 1, p.err, ERR_WAIT_FULL, abort_flag)
+           && (i < 2 || mbar_wait(&v_empty[s], ((i - 2) >> 1) & 1, p.err, ERR_WAIT_EMPTY, abort_flag));
+      if (!ok) break;
+      const uint8_t* src = sV8 + s * C::PAGE_BYTES;
+      uint8_t* dst = sV + s * C::V_BYTES;
+      // 16 numbers at a time: neighbouring threads take neighbouring chunks of a row. A thread's two chunks of halves go out in an
+      // order that lets eight neighbours cover all banks.
+      constexpr int PER_ROW = D / 16;
+#pragma unroll 4
+      for (int c = tid; c < KV8_PAGE * PER_ROW; c += 128) {
+        const int r = c / PER_ROW, k = c % PER_ROW;
+        const int blk = k / (C::ROWB / 16), in = k % (C::ROWB / 16);
+        const uint4 raw = *reinterpret_cast<const uint4*>(src + blk * KV8_PAGE * C::ROWB + k8p_at<C::ROWB>(r, in));
+        uint4 h[2];
+        kv8_unpack4(raw.x, h[0].x, h[0].y);
+        kv8_unpack4(raw.y, h[0].z, h[0].w);
+        kv8_unpack4(raw.z, h[1].x, h[1].y);
+        kv8_unpack4(raw.w, h[1].z, h[1].w);
+        const int swap = (k >> 2) & 1;
+        uint8_t* const to = dst + (k / 4) * KV8_PAGE * 128;
+        *reinterpret_cast<uint4*>(to + k8p_at<128>(r, (k & 3) * 2 + swap)) = swap ? h[1] : h[0];
+        *reinterpret_cast<uint4*>(to + k8p_at<128>(r, (k & 3) * 2 + 1 - swap)) = swap ? h[0] : h[1];
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      mbar_arrive(&v_full[s]);
+      mbar_arrive(&v8_empty[s]);
+    }
+  } else {
+    // ---------------- softmax + epilogue: thread (r = tid & 127, hf = tid >> 7) owns row r = one (position, head) on the pages
+    // i with i & 1 == hf, and the half hf of the output columns at the end.
+    const int r = threadIdx.x & 127, hf = threadIdx.x >> 7, rw = warp & 3;
+    const uint32_t lane_base = static_cast<uint32_t>(rw * 32) << 16;
+    const int lp = r / p.group, head = r % p.group;
+    const int qpos = tile.pos0 + tile.p0 + lp;
+    const bool row_valid = lp < n_pos;
+    constexpr int DH = D / 2;
+    float m_loc = -INFINITY;  // the maximum and the sum of this thread's own pages, at that maximum
+    float2 l2 = make_float2(0.f, 0.f);
+    const float2 qs2 = make_float2(qs, qs);
+    bool ok = true;
+    for (int i = hf; i < np && ok; i += 2) {
+      const uint32_t ph = (i >> 1) & 1;
+      ok = mbar_wait(&t_full[hf], ph, p.err, ERR_WAIT_FULL, abort_flag) && mbar_wait(&s_full[hf], ph, p.err, ERR_WAIT_TMEM, abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      float2 y[32];
+      tmem_ld64(tmem_S + hf * 64 + lane_base, reinterpret_cast<float*>(y));
+      const float* t = sT + hf * 3 * KV8_PAGE;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float4 a = *reinterpret_cast<const float4*>(t + 4 * j), b = *reinterpret_cast<const float4*>(t + KV8_PAGE + 4 * j);
+        y[2 * j] = fma2(mul2(y[2 * j], qs2), make_float2(a.x, a.y), make_float2(b.x, b.y));
+        y[2 * j + 1] = fma2(mul2(y[2 * j + 1], qs2), make_float2(a.z, a.w), make_float2(b.z, b.w));
+      }
+      const int kbase = (first + i) * KV8_PAGE;
+      if (kbase + KV8_PAGE - 1 > tile.pos0 + tile.p0) {  // only pages that end behind the tile's first query hide keys
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          y[j].x = kbase + 2 * j <= qpos ? y[j].x : -INFINITY;
+          y[j].y = kbase + 2 * j + 1 <= qpos ? y[j].y : -INFINITY;
+        }
+      }
+      float mx4[4] = {y[0].x, y[0].y, y[1].x, y[1].y};
+#pragma unroll
+      for (int j = 2; j < 32; ++j) { mx4[(2 * j) & 3] = fmaxf(mx4[(2 * j) & 3], y[j].x); mx4[(2 * j + 1) & 3] = fmaxf(mx4[(2 * j + 1) & 3], y[j].y); }
+      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+      float m_prev = -INFINITY;
+      if (i > 0) {
+        ok = mbar_wait(&m_bar[hf ^ 1], ((i - 1) >> 1) & 1, p.err, ERR_WAIT_FULL, abort_flag);
+        if (!ok) break;
+        m_prev = s_m[r];
+      }
+      const bool need = mx > m_prev + K8P_LAZY;
+      const float m = need ? mx : m_prev;
+      s_m[r] = m;
+      mbar_arrive(&m_bar[hf]);
+      // The output tile may only be rescaled once the products of page i - 1 have been added; those of this page and the later ones
+      // wait for this page's weights.
+      if (__any_sync(0xffffffffu, need) && i > 0) {  // warp-uniform: TMEM loads / stores are warp-collective
+        ok = mbar_wait(&pv_done[hf ^ 1], ((i - 1) >> 1) & 1, p.err, ERR_WAIT_EMPTY, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        const float factor = need ? k8p_ex2(m_prev - m) : 1.0f;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 16) {
+          float o[16];
+          tmem_ld16(tmem_O + lane_base + c, o);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) o[j] *= factor;
+          tmem_st16(tmem_O + lane_base + c, o);
+        }
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      }
+      if (m != m_loc) {
+        const float f = k8p_ex2(m_loc - m);  // 0 on this thread's first page
+        l2.x *= f;
+        l2.y *= f;
+        m_loc = m;
+      }
+      if (i >= 2) {  // this page's weights' tile was last read by the products of page i - 2
+        ok = mbar_wait(&pv_done[hf], ph ^ 1, p.err, ERR_WAIT_EMPTY, abort_flag);
+        if (!ok) break;
+      }
+      const float base = m == -INFINITY ? 0.f : K8P_LIFT - m;  // a row that sees no key of the run so far
+      const float2 base2 = make_float2(base, base), one2 = make_float2(1.f, 1.f);
+      uint8_t* const prow = sP + hf * C::P_BYTES + r * 128;
+      t += 2 * KV8_PAGE;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        uint4 packed;
+        __half2* pe = reinterpret_cast<__half2*>(&packed);
+        const float4 i0 = *reinterpret_cast<const float4*>(t + 8 * c), i1 = *reinterpret_cast<const float4*>(t + 8 * c + 4);
+        const float2 inv[4] = {make_float2(i0.x, i0.y), make_float2(i0.z, i0.w), make_float2(i1.x, i1.y), make_float2(i1.z, i1.w)};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 z = fma2(y[4 * c + j], one2, base2);
+          const float2 w = make_float2(k8p_ex2(z.x), k8p_ex2(z.y));
+          l2 = fma2(w, inv[j], l2);
+          pe[j] = __floats2half2_rn(w.x, w.y);
+        }
+        *reinterpret_cast<uint4*>(prow + ((c ^ (r & 7)) * 16)) = packed;  // 128-byte swizzle of the K-major tile
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      tc_fence_before();
+      mbar_arrive(&p_full[hf]);
+    }
+    float l = l2.x + l2.y;
+    ok = ok && mbar_wait(acc_done, 0, p.err, ERR_WAIT_TMEM, abort_flag) && !*abort_flag;
+    tc_fence_after();
+    float m_used = m_loc;
+    if (ok) {  // the weights' tiles are free now: even and odd pages put their sums together, even + odd
+      float* ex = reinterpret_cast<float*>(sP);
+      ex[(hf * 128 + r) * 2] = l;
+      ex[(hf * 128 + r) * 2 + 1] = m_loc;
+      mbar_arrive(x_bar);
+      ok = mbar_wait(x_bar, 0, p.err, ERR_WAIT_FULL, abort_flag);
+      const float l0 = ex[r * 2], m0 = ex[r * 2 + 1], l1 = ex[(128 + r) * 2], m1 = ex[(128 + r) * 2 + 1];
+      m_used = fmaxf(m0, m1);  // a running maximum never falls: the larger one is the last page's
+      l = m_used == -INFINITY ? l0 + l1 : l0 * k8p_ex2(m0 - m_used) + l1 * k8p_ex2(m1 - m_used);
+    }
+    const size_t row = static_cast<size_t>(tile.row0 + tile.p0 + lp);
+    const size_t at = (row * p.n_q + kh * p.group + head);
+    if (ok && cut) {
+      const size_t slot = at * p.max_splits + blockIdx.z;
+#pragma unroll 1
+      for (int c = hf * DH; c < hf * DH + DH; c += 16) {
+        float o[16];
+        tmem_ld16(tmem_O + lane_base + c, o);  // warp-collective: never predicated
+        if (row_valid) {
+          float4* dst = reinterpret_cast<float4*>(p.part_acc + slot * D + c);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) dst[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+        }
+      }
+      if (row_valid && hf == 0) p.part_ml[slot] = make_float2(m_used, l);
+    } else if (ok) {
+      const float inv = 1.0f / l;  // a row sees itself
+      const size_t base = at * D;
+#pragma unroll 1
+      for (int c = hf * DH; c < hf * DH + DH; c += 16) {
+        float o[16];
+        tmem_ld16(tmem_O + lane_base + c, o);  // warp-collective: never predicated
+        if (row_valid) {
+          uint4 g[2] = {*reinterpret_cast<const uint4*>(p.gate + base + c), *reinterpret_cast<const uint4*>(p.gate + base + c + 8)};
+          const bf16* ge = reinterpret_cast<const bf16*>(g);
+          uint4 out[2];
+          bf16* oe = reinterpret_cast<bf16*>(out);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) oe[j] = __float2bfloat16(o[j] * inv * sigmoid_f(__bfloat162float(ge[j])));
+          *reinterpret_cast<uint4*>(p.out + base + c) = out[0];
+          *reinterpret_cast<uint4*>(p.out + base + c + 8) = out[1];
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) { tc_fence_after(); tmem_dealloc(tmem, C::TMEM_COLS); }
+}
+
+// Rows of spans that were cut: their partials in the order of the runs. A CTA a tile of the kernel above, a thread four dims of a row's head at a time.
+template <int D>
+__global__ void __launch_bounds__(256)
+kv8_prefill_combine_kernel(Kv8PrefillParams p) {
+  constexpr int QUADS = D / 4;
+  pdl_wait();
+  pdl_launch();
+  Kv8Tile tile;
+  if (!k8p_find(p, blockIdx.x, tile)) return;
+  const int np = min(p.width, (tile.pos0 + tile.rows - 1) / KV8_PAGE + 1), run_pages = k8p_run_pages(tile.rows, np, p.positions, p.n_kv);
+  if (run_pages >= np) return;
+  const int n_pos = min(p.positions, tile.rows - tile.p0), heads = p.group;
+  const int np_all = min(p.width, (tile.pos0 + tile.p0 + n_pos - 1) / KV8_PAGE + 1), runs = (np_all + run_pages - 1) / run_pages;  // that wrote
+  for (int i = blockIdx.z * (256 / QUADS) + threadIdx.x / QUADS; i < n_pos * heads; i += gridDim.z * (256 / QUADS)) {
+    const size_t at = static_cast<size_t>(tile.row0 + tile.p0 + i / heads) * p.n_q + blockIdx.y * p.group + i % heads;
+    const int quad = threadIdx.x % QUADS;
+    const float2* ml = p.part_ml + at * p.max_splits;
+    const float4* pa = reinterpret_cast<const float4*>(p.part_acc + at * p.max_splits * D) + quad;
+    float top = -INFINITY, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int z = 0; z < runs; ++z) top = fmaxf(top, ml[z].x);
+#pragma unroll 4
+    for (int z = 0; z < runs; ++z) {
+      const float2 pm = ml[z];
+      const float4 v = pa[static_cast<size_t>(z) * QUADS];
+      const float f = pm.x == top ? 1.f : k8p_ex2(pm.x - top);
+      l = fmaf(pm.y, f, l);
+      o.x = fmaf(v.x, f, o.x); o.y = fmaf(v.y, f, o.y); o.z = fmaf(v.z, f, o.z); o.w = fmaf(v.w, f, o.w);
+    }
+    const float inv = 1.0f / l;
+    const bf16* g = p.gate + at * D + quad * 4;
+    uint2 raw;
+    __nv_bfloat162* e = reinterpret_cast<__nv_bfloat162*>(&raw);
+    e[0] = __floats2bfloat162_rn(o.x * inv * sigmoid_f(__bfloat162float(g[0])), o.y * inv * sigmoid_f(__bfloat162float(g[1])));
+    e[1] = __floats2bfloat162_rn(o.z * inv * sigmoid_f(__bfloat162float(g[2])), o.w * inv * sigmoid_f(__bfloat162float(g[3])));
+    *reinterpret_cast<uint2*>(p.out + at * D + quad * 4) = raw;
+  }
+}
+
+}  // namespace b200
+
+using namespace b200;
+
+namespace {
+typedef CUresult (*K8pEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                                CUtensorMapFloatOOBfill);
+int k8p_encode(CUtensorMap* m, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle sw) {
+  static K8pEncodeFn fn = nullptr;
+  if (!fn) {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) != cudaSuccess || !ptr) return -1;
+    fn = reinterpret_cast<K8pEncodeFn>(ptr);
+  }
+  const cuuint32_t estr[3] = {1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : -2;
+}
+template <int D>
+int k8p_launch(const CUtensorMap& tm, const CUtensorMap& te, const Kv8PrefillParams& p, int n_tiles, cudaStream_t st) {
+  auto kern = kv8_prefill_kernel<D>;
+  static bool configured[64] = {};  // a function attribute is set per device
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -3;
+  if (!configured[dev]) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Kv8PrefillCfg<D>::SMEM) != cudaSuccess) return -3;
+    configured[dev] = true;
+  }
+  if (launch_pdl(kern, dim3(n_tiles, p.n_kv, p.max_splits), dim3(K8P_THREADS), Kv8PrefillCfg<D>::SMEM, st, tm, te, p) != cudaSuccess) return -4;
+  if (p.max_splits == 1) return 0;
+  return launch_pdl(kv8_prefill_combine_kernel<D>, dim3(n_tiles, p.n_kv, 8), dim3(256), 0, st, p) == cudaSuccess ? 0 : -4;
+}
+}  // namespace
+
+// Positions of a tile, and the runs that a span of n rows from position pos0 on is cut into (1: it is not): the caller sizes grid and partials by them.
+extern "C" int b200_kv8_prefill_positions(int group) { return group >= 1 && group <= 16 ? 128 / group : 0; }
+extern "C" int b200_kv8_prefill_runs(int n, int pos0, int width, int group, int n_kv) {
+  if (n <= 0 || group < 1 || group > 16 || n_kv < 1) return 1;
+  const int seen = (pos0 + n - 1) / KV8_PAGE + 1, np = seen < width ? seen : width;
+  const int pages = k8p_run_pages(n, np, 128 / group, n_kv);
+  return np > 0 && pages < np ? (np + pages - 1) / pages : 1;
+}
+
+// q: [T, n_q, D] bf16 (normed and rotated), gate, out: [T, n_q * D], in 16-byte rows; data, exps: one layer of the 8-bit cache, which holds the
+// spans' own keys; starts [segs + 1], pos0 [segs] of the spans, tables [segs] rows of `width` pages. n_tiles: at least the spans' tiles.
+// max_splits: the most runs of a span (part_acc [T, n_q, max_splits, D], part_ml [.., 2] where there is more than one).
+extern "C" int b200_kv8_prefill(const void* q, const void* gate, const void* data, const void* exps, const int* starts, const int* pos0,
+                                int segs, int n_tiles, const int* tables, int max_pages, int width, int num_pages, int n_q, int n_kv,
+                                int D, int max_splits, float* part_acc, float* part_ml, void* out, int* err, cudaStream_t st) {
+  if (n_tiles <= 0 || segs <= 0) return 0;
+  const int group = n_kv > 0 ? n_q / n_kv : 0;
+  if (group < 1 || group * n_kv != n_q || group > 16 || max_splits < 1 || width < 1) return -7;
+  if (D != 256 && D != 128 && D != 64) return -7;
+  const long long rows = static_cast<long long>(num_pages) * 2 * n_kv * KV8_PAGE;
+  if (rows > 0x7fffffffLL) return -7;  // a TMA coordinate
+  for (const void* x : {q, gate, data, exps, static_cast<const void*>(out)})
+    if (reinterpret_cast<uintptr_t>(x) % 16) return -7;
+  CUtensorMap tm, te;
+  const cuuint32_t rowb = D < 128 ? D : 128;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(rows)}, strides[1] = {static_cast<cuuint64_t>(D)};
+  const cuuint32_t box[2] = {rowb, KV8_PAGE};
+  const cuuint64_t edims[3] = {KV8_PAGE, static_cast<cuuint64_t>(n_kv), static_cast<cuuint64_t>(num_pages) * 2};
+  const cuuint64_t estrides[2] = {KV8_PAGE, static_cast<cuuint64_t>(n_kv) * KV8_PAGE};
+  const cuuint32_t ebox[3] = {KV8_PAGE, 1, 2};
+  if (k8p_encode(&tm, data, 2, dims, strides, box, rowb == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B) ||
+      k8p_encode(&te, exps, 3, edims, estrides, ebox, CU_TENSOR_MAP_SWIZZLE_NONE)) return -1;
+  const Kv8PrefillParams p{static_cast<const bf16*>(q), static_cast<const bf16*>(gate), starts, pos0, tables, static_cast<bf16*>(out), part_acc,
+                           reinterpret_cast<float2*>(part_ml), segs, max_pages, width, num_pages, n_q, n_kv, group, 128 / group, max_splits,
+                           1.4426950408889634f / sqrtf(static_cast<float>(D)), err};
+  if (D == 256) return k8p_launch<256>(tm, te, p, n_tiles, st);
+  if (D == 128) return k8p_launch<128>(tm, te, p, n_tiles, st);
+  return k8p_launch<64>(tm, te, p, n_tiles, st);
+}

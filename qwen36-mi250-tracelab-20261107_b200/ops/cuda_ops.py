@@ -89,6 +89,9 @@ class _Sig:
     b200_kv8_write = [P, L, L, P, L, L, P, P, P, I, I, I, P, P, I, I, I, I, P, P]
     b200_kv8_read = [P, P, P, P, P, I, I, I, P, P, I, I, I, I, P, P]
     b200_kv8_decode_run = []
+    b200_kv8_prefill_positions = [I]
+    b200_kv8_prefill_runs = [I, I, I, I, I]
+    b200_kv8_prefill = [P, P, P, P, P, P, I, I, P, I, I, I, I, I, I, I, P, P, P, P, P]
     b200_kv8_decode = [P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, P, P, P, P, P]
 
 
@@ -782,7 +785,13 @@ def kv8_read(layer: Kv8Layer, positions: torch.Tensor, seq_of_row: torch.Tensor,
     return k, v
 
 
+KV8_HEAD_DIMS = (64, 128, 256)  # of the attention kernels over the 8-bit cache
+KV8_CUT_TILES = 64  # (tiles of a span) * (KV heads) up to which kv8_prefill.cu may cut its context
+
+
 def _kv8_queries(what: str, q: torch.Tensor, gate: torch.Tensor, n_kv: int, D: int, dev: torch.device):
+    if D not in KV8_HEAD_DIMS:
+        raise ValueError(f"{what}: head dim {D} is none of {KV8_HEAD_DIMS}")
     if q.dim() != 3 or q.shape[2] != D or q.shape[1] % n_kv or not 1 <= q.shape[1] // n_kv <= 16 or q.dtype != torch.bfloat16:
         raise ValueError(f"{what}: q {tuple(q.shape)} {q.dtype} is not bf16 [rows, n_q, {D}] with 1 to 16 query heads for each of {n_kv} KV heads")
     if gate.shape != (q.shape[0], q.shape[1] * D) or gate.dtype != torch.bfloat16:
@@ -790,9 +799,8 @@ def _kv8_queries(what: str, q: torch.Tensor, gate: torch.Tensor, n_kv: int, D: i
     if q.device != dev or gate.device != dev:
         raise ValueError(f"{what}: the cache is on {dev}, q on {q.device}, the gate on {gate.device}")
     q = q if q.is_contiguous() else q.contiguous()
-    if q.data_ptr() % 16:
-        q = q.clone()
-    return q, gate if gate.is_contiguous() else gate.contiguous()
+    gate = gate if gate.is_contiguous() else gate.contiguous()
+    return q if q.data_ptr() % 16 == 0 else q.clone(), gate if gate.data_ptr() % 16 == 0 else gate.clone()
 
 
 def kv8_decode(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tables: torch.Tensor, positions: torch.Tensor,
@@ -821,24 +829,64 @@ def kv8_decode(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_table
     return out
 
 
-def kv8_prefill(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tables: torch.Tensor, seg_starts: list[int],
-                seg_pos0: list[int], meta=None) -> torch.Tensor:
+def kv8_prefill(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tables: torch.Tensor, seg_starts: list[int] | None,
+                seg_pos0: list[int] | None, meta=None) -> torch.Tensor:
     """``flash_prefill`` over the 8-bit cache: causal gated attention of ragged spans of new tokens over what their sequences' pages
-    hold, the spans' own keys included. Span ``i`` owns rows ``seg_starts[i]:seg_starts[i + 1]`` at positions ``seg_pos0[i] ..``.
+    hold, the spans' own keys included. Span ``i`` owns rows ``seg_starts[i]:seg_starts[i + 1]`` at positions ``seg_pos0[i] ..``. The context of
+    a short span is cut into runs for CTAs of their own, by the span's own rows and position: a row's bits do not depend on the other spans.
 
-    ``meta``: ``(seg_starts, seg_pos0)`` as int32 device tensors that the caller keeps, of the same numbers; without it every call uploads them."""
+    ``meta``: ``(seg_starts, seg_pos0)`` as int32 device tensors that the caller keeps, of the same numbers; without it every call uploads
+    them. With ``meta`` the lists may be None, which lets the call be captured in a CUDA graph: no span is cut then."""
     pages, n_kv, D = check_layer(layer, "kv8_prefill")
-    q, gate = _kv8_queries("kv8_prefill", q, gate, n_kv, D, layer.data.device)
-    n_seg = len(seg_pos0)
-    if (len(seg_starts) != n_seg + 1 or seg_starts[0] != 0 or seg_starts[-1] != q.shape[0] or block_tables.shape[0] < n_seg
-            or any(b < a for a, b in zip(seg_starts, seg_starts[1:]))):
-        raise ValueError(f"kv8_prefill: spans {seg_starts} with {n_seg} first positions do not make {q.shape[0]} rows of at most "
-                         f"{block_tables.shape[0]} sequences")
-    starts_t, pos0_t = meta if meta is not None else (torch.tensor(x, dtype=torch.int32).to(q.device) for x in (seg_starts, seg_pos0))
-    row = torch.arange(q.shape[0], dtype=torch.int32, device=q.device)
-    seq = torch.searchsorted(starts_t[1:n_seg + 1].contiguous(), row, right=True)
-    positions = pos0_t[seq].long() + row - starts_t[seq]
-    return kv8_decode(q, gate, layer, block_tables[seq], positions, 1)
+    dev = layer.data.device
+    q, gate = _kv8_queries("kv8_prefill", q, gate, n_kv, D, dev)
+    T, n_q, _ = q.shape
+    L = lib()
+    group = n_q // n_kv
+    per = L.b200_kv8_prefill_positions(group)
+    if block_tables.dim() != 2 or block_tables.device != dev:
+        raise ValueError(f"kv8_prefill: page tables {tuple(block_tables.shape)} on {block_tables.device}, the cache on {dev}")
+    if block_tables.dtype != torch.int32 or block_tables.stride(1) != 1:
+        block_tables = block_tables.to(torch.int32).contiguous()
+    width = block_tables.shape[1]
+    splits = 1
+    if seg_starts is not None:
+        n_seg = len(seg_pos0)
+        lens = [b - a for a, b in zip(seg_starts, seg_starts[1:])]
+        if len(lens) != n_seg or seg_starts[0] != 0 or seg_starts[-1] != T or block_tables.shape[0] < n_seg or min(lens, default=0) < 0:
+            raise ValueError(f"kv8_prefill: spans {seg_starts} with {n_seg} first positions do not make {T} rows of at most "
+                             f"{block_tables.shape[0]} sequences")
+        n_tiles = sum([(n + per - 1) // per for n in lens])
+        for n, pos in zip(lens, seg_pos0):
+            if pos < 0 or pos + n > width * PAGE_SIZE:
+                raise ValueError(f"kv8_prefill: rows at positions {pos} .. {pos + n - 1}, page tables of {width} pages")
+            if 0 < n * n_kv <= per * KV8_CUT_TILES:  # short enough to be cut
+                splits = max(splits, L.b200_kv8_prefill_runs(n, pos, width, group, n_kv))
+    elif meta is None:
+        raise ValueError("kv8_prefill: neither the spans' lists nor their device tensors")
+    else:
+        n_seg = meta[1].shape[0]
+        n_tiles = T // per + n_seg
+    if meta is not None:
+        starts_t, pos0_t = meta
+        if (starts_t.dtype, pos0_t.dtype) != (torch.int32, torch.int32) or starts_t.numel() <= n_seg - (n_seg == 0) or pos0_t.numel() < n_seg \
+                or starts_t.device != dev or pos0_t.device != dev:
+            raise ValueError(f"kv8_prefill: meta of {starts_t.numel()} and {pos0_t.numel()} numbers ({starts_t.dtype}, {starts_t.device}) for {n_seg} spans")
+    elif T:
+        both = torch.tensor([*seg_starts, *seg_pos0], dtype=torch.int32).to(dev)
+        starts_t, pos0_t = both[: n_seg + 1], both[n_seg + 1 :]
+    out = torch.empty(T, n_q * D, dtype=q.dtype, device=dev)
+    if T == 0:
+        return out
+    part_acc = part_ml = None
+    if splits > 1:
+        part_acc = torch.empty(T, n_q, splits, D, dtype=torch.float32, device=dev)
+        part_ml = torch.empty(T, n_q, splits, 2, dtype=torch.float32, device=dev)
+    _check(L.b200_kv8_prefill(
+        q.data_ptr(), gate.data_ptr(), layer.data.data_ptr(), layer.exps.data_ptr(), starts_t.data_ptr(), pos0_t.data_ptr(), n_seg, n_tiles,
+        block_tables.data_ptr(), block_tables.stride(0), width, pages, n_q, n_kv, D, splits, _ptr(part_acc), _ptr(part_ml),
+        out.data_ptr(), _ptr(err_word(dev)), _stream()), "kv8_prefill")
+    return out
 
 
 def argmax_rows(logits: torch.Tensor) -> torch.Tensor:
