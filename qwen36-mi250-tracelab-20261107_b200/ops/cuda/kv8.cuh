@@ -35,6 +35,9 @@ __device__ __forceinline__ uint32_t kv8_unpack2(uint16_t two) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(two));
   return r;
 }
+// For outputs that are rounded to bf16 next: the reciprocal unit's quotient, off by 2 units in the last place, and not the exact one,
+// whose subroutine took most of a prefill tile's last phase (32,000 cycles for 128 rows of 256).
+__device__ __forceinline__ float kv8_sigmoid(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
 // The four bytes of a word as two pairs of halves.
 __device__ __forceinline__ void kv8_unpack4(uint32_t word, uint32_t& lo, uint32_t& hi) {
   lo = kv8_unpack2(static_cast<uint16_t>(word));

@@ -623,8 +623,8 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
             for (int i = 0; i < C::PER; ++i) {
               const size_t at = head * D + (tile0 + i) * 16 + 2 * g;
               *reinterpret_cast<__nv_bfloat162*>(p.out + at) =
-                  __floats2bfloat162_rn(o[n8][i][k] * inv * sigmoid_f(__uint_as_float(static_cast<uint32_t>(gates[n8][k][i][0]) << 16)),
-                                        o[n8][i][2 + k] * inv * sigmoid_f(__uint_as_float(static_cast<uint32_t>(gates[n8][k][i][1]) << 16)));
+                  __floats2bfloat162_rn(o[n8][i][k] * inv * kv8_sigmoid(__uint_as_float(static_cast<uint32_t>(gates[n8][k][i][0]) << 16)),
+                                        o[n8][i][2 + k] * inv * kv8_sigmoid(__uint_as_float(static_cast<uint32_t>(gates[n8][k][i][1]) << 16)));
             }
           }
         }
@@ -675,8 +675,8 @@ __device__ __forceinline__ void k8d_store(bf16* out, const bf16* gate, const flo
   const float inv = 1.0f / sum;
   uint2 raw;
   __nv_bfloat162* e = reinterpret_cast<__nv_bfloat162*>(&raw);
-  e[0] = __floats2bfloat162_rn(o.x * inv * sigmoid_f(__bfloat162float(gate[0])), o.y * inv * sigmoid_f(__bfloat162float(gate[1])));
-  e[1] = __floats2bfloat162_rn(o.z * inv * sigmoid_f(__bfloat162float(gate[2])), o.w * inv * sigmoid_f(__bfloat162float(gate[3])));
+  e[0] = __floats2bfloat162_rn(o.x * inv * kv8_sigmoid(__bfloat162float(gate[0])), o.y * inv * kv8_sigmoid(__bfloat162float(gate[1])));
+  e[1] = __floats2bfloat162_rn(o.z * inv * kv8_sigmoid(__bfloat162float(gate[2])), o.w * inv * kv8_sigmoid(__bfloat162float(gate[3])));
   *reinterpret_cast<uint2*>(out) = raw;
 }
 // Tables of up to 64 runs (16,384 keys): a thread takes all sums of four dims of a head.

@@ -6,7 +6,8 @@
 // page of 64 keys at a time:
 //
 //   S[128 x 64]  = Q1 K^T + Q2 K^T     the page's e4m3 bytes as TMA brought them (kind::f8f6f4, twice the rate of bf16). A bf16 query row,
-//                                      scaled by a power of two, is Q1 + Q2 in e4m3: exact but for what lies 2^-17 below its largest number
+//                                      scaled by a power of two, is Q1 + Q2 in e4m3: exact but for what lies 2^-17 below its largest number.
+//                                      The terms lie in TMEM
 //   y = s a_j' + b_j                   the key's power of two and, in the exponent, the value's: w = 2^(y - M + LIFT) weighs the stored
 //                                      v_j, M the running maximum of y; the softmax's own sum is sum_j w 2^-b_j
 //   O[128 x D]  += P[128 x 64] V       P and V as halves: four warps make them of the page's bytes (exact)
@@ -35,6 +36,7 @@ struct Kv8PrefillParams {
   float* part_acc;          // [T, n_q, max_splits, D]: of spans that are cut
   float2* part_ml;          // [T, n_q, max_splits]
   int segs, max_pages, width, num_pages, n_q, n_kv, group, positions, max_splits;  // positions: of a tile
+  int inv_group;            // r * inv_group >> 16 is r / group, for rows below 128 of groups up to 16
   float scale_log2;
   int* err;
 };
@@ -44,13 +46,13 @@ struct Kv8PrefillCfg {
   static constexpr int ROWB = D < 128 ? D : 128;       // bytes of a row in one swizzled block of stored numbers
   static constexpr int DB = D / ROWB;
   static constexpr int HB = D / 64;                    // 128-byte blocks of a row of halves
-  static constexpr int Q_TERM = 128 * D;               // [DB][128 rows][ROWB]; two terms
+  static constexpr int Q_TERM = 128 * D;               // a term of the queries on its way to TMEM: [128 rows][D], chunks of 16 bytes XOR row
   static constexpr int PAGE_BYTES = KV8_PAGE * D;      // [DB][64 rows][ROWB]: keys or values of a page
   static constexpr int V_BYTES = KV8_PAGE * D * 2;     // [HB][64 rows][128]: values as halves
   static constexpr int P_BYTES = 128 * 128;            // [128 rows][64 halves]
   static constexpr int EXPS = 2 * KV8_PAGE;
   static constexpr int SMEM = 2 * Q_TERM + 4 * PAGE_BYTES + 2 * V_BYTES + 2 * P_BYTES + 4 * EXPS + 2 * 3 * KV8_PAGE * 4 + 512 + 256;
-  static constexpr int TMEM_COLS = 128 + D <= 256 ? 256 : 512;
+  static constexpr int TMEM_COLS = 128 + D + D / 2 <= 256 ? 256 : 512;  // two score tiles of 64, the output, two terms of the queries
 };
 
 // Runs that a span of n rows whose last key is in page np - 1 is cut into, and their pages: by the span alone.
@@ -62,12 +64,13 @@ __host__ __device__ __forceinline__ int k8p_run_pages(int n, int np, int positio
   return pages < K8P_MIN_PAGES ? K8P_MIN_PAGES : pages;
 }
 
-__device__ __forceinline__ void k8p_umma_f8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+// D[tmem] (+)= A[tmem] * B[smem]^T: a lane of A is a row, a column four of its bytes.
+__device__ __forceinline__ void k8p_umma_f8(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 // K-major operand tile in rows of ROWB bytes (64 or 128) written with the swizzle of that size, groups of eight rows after each other.
@@ -107,7 +110,7 @@ __device__ __forceinline__ bool k8p_find(const Kv8PrefillParams& p, int tile, Kv
   int before = 0;
   for (int s0 = 0; s0 < p.segs; s0 += 32) {
     const int s = s0 + lane;
-    const int a = s < p.segs ? p.starts[s] : 0, n = s < p.segs ? p.starts[s + 1] - a : 0;
+    const int a = s < p.segs ? p.starts[s] : 0, n = s < p.segs ? p.starts[s + 1] - a : 0, pos = s < p.segs ? p.pos0[s] : 0;
     const int tiles = (n + p.positions - 1) / p.positions;
     int upto = tiles;
 #pragma unroll
@@ -123,7 +126,7 @@ __device__ __forceinline__ bool k8p_find(const Kv8PrefillParams& p, int tile, Kv
       t.row0 = __shfl_sync(0xffffffffu, a, l);
       t.rows = __shfl_sync(0xffffffffu, n, l);
       t.p0 = (tile - __shfl_sync(0xffffffffu, upto - tiles, l)) * p.positions;
-      t.pos0 = p.pos0[t.seg];
+      t.pos0 = __shfl_sync(0xffffffffu, pos, l);
       return true;
     }
     before = __shfl_sync(0xffffffffu, upto, 31);
@@ -164,6 +167,8 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
   uint64_t* const x_bar = bars + 25;
   uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 26);
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  uint64_t* const q_full = bars + 29;
+  uint64_t* const q_ready = bars + 30;
   uint64_t* const m_bar = bars + 27;                     // [2]: the row maxima up to an even / odd page
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -188,70 +193,62 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
     for (int s = 0; s < 4; ++s) mbar_init(&e_full[s], 1);
     mbar_init(acc_done, 1);
     mbar_init(x_bar, 256);
+    mbar_init(q_ready, K8P_THREADS - 64);
+    mbar_init(q_full, 256);
     *abort_flag = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tm);
     tma_prefetch_desc(&tm_exps);
   }
   if (warp == 8) { tmem_alloc(tmem_slot, C::TMEM_COLS); tmem_relinquish(); }
-  float* const s_qs = reinterpret_cast<float*>(sP);      // until the rows' threads have read it
-  // ---- queries: a warp a row at a time, two terms of e4m3; the largest number of a row comes to [128, 256)
-  for (int r0 = warp; r0 < 128; r0 += K8P_THREADS / 32 * 4) {
-    uint4 raw[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = r0 + i * (K8P_THREADS / 32), lp = r / p.group;
-      raw[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (r < 128 && lp < n_pos && lane * 8 < D)
-        raw[i] = *reinterpret_cast<const uint4*>(p.q + (static_cast<size_t>(tile.row0 + tile.p0 + lp) * p.n_q + kh * p.group + r % p.group) * D + lane * 8);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = r0 + i * (K8P_THREADS / 32);
-      if (r >= 128) break;
-      const __nv_bfloat162* e2 = reinterpret_cast<const __nv_bfloat162*>(&raw[i]);
-      float x[8];
-      float top = 0.f;
-      bool bad = false;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float2 f = __bfloat1622float2(e2[k]);
-        x[2 * k] = f.x;
-        x[2 * k + 1] = f.y;
-        top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
-        bad |= !(fabsf(f.x) <= 3.4e38f && fabsf(f.y) <= 3.4e38f);
-      }
-      top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));  // not negative: in the order of its bits
-      const int e = max(-110, min(110, static_cast<int>(__float_as_uint(top) >> 23) - 127 - 7));
-      const float f = kv8_two_to(-e);
-      uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
-#pragma unroll
-      for (int k = 0; k < 8; k += 2) {
-        const float a = x[k] * f, b = x[k + 1] * f;
-        const uint32_t two = kv8_pack2(a, b), hh = kv8_unpack2(static_cast<uint16_t>(two));
-        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hh));
-        hi[k / 4] |= two << (8 * (k & 3));
-        lo[k / 4] |= kv8_pack2(a - back.x, b - back.y) << (8 * (k & 3));
-      }
-      if (lane * 8 < D) {
-        const int blk = lane * 8 / C::ROWB, in = lane * 8 % C::ROWB;
-        uint8_t* const at = sQ + blk * 128 * C::ROWB + k8p_at<C::ROWB>(r, in >> 4) + (in & 15);
-        *reinterpret_cast<uint2*>(at) = make_uint2(hi[0], hi[1]);
-        *reinterpret_cast<uint2*>(at + C::Q_TERM) = make_uint2(lo[0], lo[1]);
-      }
-      const bool any = __any_sync(0xffffffffu, bad);  // a NaN or an infinity: all scores of the row are NaN
-      if (lane == 0) s_qs[r] = any ? __uint_as_float(0x7fffffffu) : kv8_two_to(e) * p.scale_log2;
-    }
-  }
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const float qs = threadIdx.x < 256 ? s_qs[threadIdx.x & 127] : 0.f;
   const uint32_t tmem = *tmem_slot;
-  __syncthreads();
   pdl_launch();  // this CTA holds its TMEM columns
-  const uint32_t tmem_S = tmem, tmem_O = tmem + 128;     // score tile of page i at tmem_S + (i & 1) * 64
+  const uint32_t tmem_S = tmem, tmem_O = tmem + 128, tmem_Q = tmem_O + D;  // score tile of page i at tmem_S + (i & 1) * 64
+  float* const s_qs = reinterpret_cast<float*>(sP);      // until the rows' threads have read it
+  if (warp != 8 && warp != 9) {
+    // ---- queries: a warp a row at a time, two terms of e4m3; the largest number of a row comes to [128, 256)
+    constexpr int WARPS = K8P_THREADS / 32 - 2, PER = (128 + WARPS - 1) / WARPS;
+    const int w = warp < 8 ? warp : warp - 2;
+    uint4 raw[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int r = w + i * WARPS, lp = r * p.inv_group >> 16;
+      raw[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (r < 128 && lp < n_pos && lane * 8 < D)
+        raw[i] = *reinterpret_cast<const uint4*>(p.q + (static_cast<size_t>(tile.row0 + tile.p0 + lp) * p.n_q + kh * p.group + (r - lp * p.group)) * D + lane * 8);
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int r = w + i * WARPS;
+      if (r >= 128) break;
+      const uint32_t* word = reinterpret_cast<const uint32_t*>(&raw[i]);
+      // magnitudes of bf16 numbers are in the order of their bits
+      uint32_t top = __vmaxu2(__vmaxu2(word[0] & 0x7fff7fffu, word[1] & 0x7fff7fffu), __vmaxu2(word[2] & 0x7fff7fffu, word[3] & 0x7fff7fffu));
+      top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
+      const int e = max(-110, min(110, static_cast<int>(top >> 7) - 127 - 7));
+      const float f = kv8_two_to(-e);
+      uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float a = __uint_as_float(word[k] << 16) * f, b = __uint_as_float(word[k] & 0xffff0000u) * f;
+        const uint32_t two = kv8_pack2(a, b), hh = kv8_unpack2(static_cast<uint16_t>(two));
+        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hh));
+        hi[k / 2] |= two << (16 * (k & 1));
+        lo[k / 2] |= kv8_pack2(a - back.x, b - back.y) << (16 * (k & 1));
+      }
+      if (lane * 8 < D) {
+        uint8_t* const at = sQ + r * D + (((lane >> 1) ^ (r & (D / 16 - 1))) << 4) + (lane & 1) * 8;
+        *reinterpret_cast<uint2*>(at) = make_uint2(hi[0], hi[1]);
+        *reinterpret_cast<uint2*>(at + C::Q_TERM) = make_uint2(lo[0], lo[1]);
+      }
+      // a NaN or an infinity: all scores of the row are NaN
+      if (lane == 0) s_qs[r] = top >= 0x7f80u ? __uint_as_float(0x7fffffffu) : kv8_two_to(e) * p.scale_log2;
+    }
+    mbar_arrive(q_ready);
+  }
 
   if (warp == 9) {
     // ---------------- loads
@@ -284,7 +281,6 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
     if (elect_one()) {
       constexpr uint32_t idesc_s = (1u << 4) | (64u >> 3) << 17 | (128u >> 4) << 24;                                     // e4m3
       constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | static_cast<uint32_t>(D >> 3) << 17 | (128u >> 4) << 24;     // halves, B MN-major
-      const uint32_t qa = smem_u32(sQ);
       auto issue_qk = [&](int i) {
         const int s = i & 1;
         if (!mbar_wait(&k_full[s], (i >> 1) & 1, p.err, ERR_WAIT_FULL, abort_flag)) return false;
@@ -296,14 +292,14 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
           for (int kk = 0; kk < D / 32; ++kk) {
             constexpr int STEPS = C::ROWB / 32;
             const int blk = kk / STEPS, off = kk % STEPS * 32;
-            k8p_umma_f8(tmem_S + s * 64, k8p_desc<C::ROWB>(qa + term * C::Q_TERM + blk * 128 * C::ROWB + off),
+            k8p_umma_f8(tmem_S + s * 64, tmem_Q + term * (D / 4) + kk * 8,
                         k8p_desc<C::ROWB>(ka + blk * KV8_PAGE * C::ROWB + off), idesc_s, (term | kk) != 0);
           }
         umma_commit(&s_full[s]);
         umma_commit(&k_empty[s]);
         return true;
       };
-      bool ok = issue_qk(0) && (np < 2 || issue_qk(1));
+      bool ok = mbar_wait(q_full, 0, p.err, ERR_WAIT_FULL, abort_flag) && issue_qk(0) && (np < 2 || issue_qk(1));
       for (int i = 0; i < np && ok; ++i) {
         const int s = i & 1;
         // the weights of page i are written, so its score tile has been read: the scores of page i + 2 go first
@@ -324,6 +320,15 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
   } else if (warp >= 10) {
     // ---------------- values: bytes to halves; the numbers that go with a page's keys
     const int tid = threadIdx.x - 320;
+    // A thread has 16 numbers of every ROWS-th row, neighbours have neighbouring chunks of a row. Its two chunks of halves go out in an
+    // order that lets eight neighbours cover all banks. ROWS is a multiple of eight: the swizzle of a thread's rows is the same.
+    constexpr int PER_ROW = D / 16, ROWS = 128 / PER_ROW;
+    static_assert(ROWS % 8 == 0, "rows of a step");
+    const int r = tid / PER_ROW, k = tid % PER_ROW;
+    const bool swap = (k >> 2) & 1;
+    const uint32_t from = k / (C::ROWB / 16) * KV8_PAGE * C::ROWB + k8p_at<C::ROWB>(r, k % (C::ROWB / 16));
+    const uint32_t to0 = k / 4 * KV8_PAGE * 128 + k8p_at<128>(r, (k & 3) * 2 + swap);
+    const uint32_t to1 = k / 4 * KV8_PAGE * 128 + k8p_at<128>(r, (k & 3) * 2 + 1 - swap);
     bool ok = true;
     for (int i = 0; i < np; ++i) {
       const int s = i & 1;
@@ -342,25 +347,18 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
       ok = mbar_wait(&v8_full[s], (i >> 1) & 1, p.err, ERR_WAIT_FULL, abort_flag)
            && (i < 2 || mbar_wait(&v_empty[s], ((i - 2) >> 1) & 1, p.err, ERR_WAIT_EMPTY, abort_flag));
       if (!ok) break;
-      const uint8_t* src = sV8 + s * C::PAGE_BYTES;
-      uint8_t* dst = sV + s * C::V_BYTES;
-      // 16 numbers at a time: neighbouring threads take neighbouring chunks of a row. A thread's two chunks of halves go out in an
-      // order that lets eight neighbours cover all banks.
-      constexpr int PER_ROW = D / 16;
-#pragma unroll 4
-      for (int c = tid; c < KV8_PAGE * PER_ROW; c += 128) {
-        const int r = c / PER_ROW, k = c % PER_ROW;
-        const int blk = k / (C::ROWB / 16), in = k % (C::ROWB / 16);
-        const uint4 raw = *reinterpret_cast<const uint4*>(src + blk * KV8_PAGE * C::ROWB + k8p_at<C::ROWB>(r, in));
+      const uint8_t* const src = sV8 + s * C::PAGE_BYTES + from;
+      uint8_t* const dst = sV + s * C::V_BYTES;
+#pragma unroll
+      for (int c = 0; c < KV8_PAGE / ROWS; ++c) {
+        const uint4 raw = *reinterpret_cast<const uint4*>(src + c * ROWS * C::ROWB);
         uint4 h[2];
         kv8_unpack4(raw.x, h[0].x, h[0].y);
         kv8_unpack4(raw.y, h[0].z, h[0].w);
         kv8_unpack4(raw.z, h[1].x, h[1].y);
         kv8_unpack4(raw.w, h[1].z, h[1].w);
-        const int swap = (k >> 2) & 1;
-        uint8_t* const to = dst + (k / 4) * KV8_PAGE * 128;
-        *reinterpret_cast<uint4*>(to + k8p_at<128>(r, (k & 3) * 2 + swap)) = swap ? h[1] : h[0];
-        *reinterpret_cast<uint4*>(to + k8p_at<128>(r, (k & 3) * 2 + 1 - swap)) = swap ? h[0] : h[1];
+        *reinterpret_cast<uint4*>(dst + to0 + c * ROWS * 128) = swap ? h[1] : h[0];
+        *reinterpret_cast<uint4*>(dst + to1 + c * ROWS * 128) = swap ? h[0] : h[1];
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(&v_full[s]);
@@ -371,14 +369,28 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
     // i with i & 1 == hf, and the half hf of the output columns at the end.
     const int r = threadIdx.x & 127, hf = threadIdx.x >> 7, rw = warp & 3;
     const uint32_t lane_base = static_cast<uint32_t>(rw * 32) << 16;
-    const int lp = r / p.group, head = r % p.group;
+    const int lp = r * p.inv_group >> 16, head = r - lp * p.group;
     const int qpos = tile.pos0 + tile.p0 + lp;
     const bool row_valid = lp < n_pos;
     constexpr int DH = D / 2;
     float m_loc = -INFINITY;  // the maximum and the sum of this thread's own pages, at that maximum
     float2 l2 = make_float2(0.f, 0.f);
-    const float2 qs2 = make_float2(qs, qs);
-    bool ok = true;
+    bool ok = mbar_wait(q_ready, 0, p.err, ERR_WAIT_FULL, abort_flag);
+    {  // the queries' terms to TMEM, one by either group: as an operand there they take no bandwidth of shared memory, which bounds a page
+      const uint8_t* const src = sQ + hf * C::Q_TERM + r * D;
+#pragma unroll
+      for (int c = 0; c < D / 16; c += 4) {
+        uint4 w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const uint4*>(src + (((c + j) ^ (r & (D / 16 - 1))) << 4));
+        tmem_st16(tmem_Q + lane_base + hf * (D / 4) + c * 4, reinterpret_cast<const float*>(w));
+      }
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      tc_fence_before();
+      mbar_arrive(q_full);
+    }
+    const float2 qs2 = make_float2(s_qs[r], s_qs[r]);
+    asm volatile("bar.sync 1, 256;" ::: "memory");  // all have read it: the weights' tiles may be written. Nobody has left before
     for (int i = hf; i < np && ok; i += 2) {
       const uint32_t ph = (i >> 1) & 1;
       ok = mbar_wait(&t_full[hf], ph, p.err, ERR_WAIT_FULL, abort_flag) && mbar_wait(&s_full[hf], ph, p.err, ERR_WAIT_TMEM, abort_flag);
@@ -479,37 +491,48 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
       m_used = fmaxf(m0, m1);  // a running maximum never falls: the larger one is the last page's
       l = m_used == -INFINITY ? l0 + l1 : l0 * k8p_ex2(m0 - m_used) + l1 * k8p_ex2(m1 - m_used);
     }
-    const size_t row = static_cast<size_t>(tile.row0 + tile.p0 + lp);
-    const size_t at = (row * p.n_q + kh * p.group + head);
-    if (ok && cut) {
-      const size_t slot = at * p.max_splits + blockIdx.z;
+    // The outputs go through shared memory, 16 bytes of a row in the place of their number XOR the row, so that a warp reads gates and
+    // writes outputs of a whole row at a time (with a thread a row from TMEM to the output, the end of a tile took 13 us).
+    float* const so = reinterpret_cast<float*>(sQ);        // [128][D], in the place of Q and the pages' bytes
+    if (ok) {
+      const float inv = cut ? 1.0f : 1.0f / l;             // (a row sees itself)
 #pragma unroll 1
       for (int c = hf * DH; c < hf * DH + DH; c += 16) {
         float o[16];
-        tmem_ld16(tmem_O + lane_base + c, o);  // warp-collective: never predicated
-        if (row_valid) {
-          float4* dst = reinterpret_cast<float4*>(p.part_acc + slot * D + c);
+        tmem_ld16(tmem_O + lane_base + c, o);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) dst[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
-        }
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<float4*>(so + r * D + (((c >> 2) + j) ^ (r & 7)) * 4) =
+              make_float4(o[4 * j] * inv, o[4 * j + 1] * inv, o[4 * j + 2] * inv, o[4 * j + 3] * inv);
       }
-      if (row_valid && hf == 0) p.part_ml[slot] = make_float2(m_used, l);
-    } else if (ok) {
-      const float inv = 1.0f / l;  // a row sees itself
-      const size_t base = at * D;
-#pragma unroll 1
-      for (int c = hf * DH; c < hf * DH + DH; c += 16) {
-        float o[16];
-        tmem_ld16(tmem_O + lane_base + c, o);  // warp-collective: never predicated
-        if (row_valid) {
-          uint4 g[2] = {*reinterpret_cast<const uint4*>(p.gate + base + c), *reinterpret_cast<const uint4*>(p.gate + base + c + 8)};
-          const bf16* ge = reinterpret_cast<const bf16*>(g);
-          uint4 out[2];
-          bf16* oe = reinterpret_cast<bf16*>(out);
+      if (cut && row_valid && hf == 0)
+        p.part_ml[((static_cast<size_t>(tile.row0 + tile.p0 + lp) * p.n_q + kh * p.group + head)) * p.max_splits + blockIdx.z] = make_float2(m_used, l);
+      mbar_arrive(x_bar);
+      ok = mbar_wait(x_bar, 1, p.err, ERR_WAIT_FULL, abort_flag);
+    }
+    if (ok) {
+      constexpr int LANES = D / 8, ROWS = 32 / LANES;      // 8 numbers a lane, rows a warp takes at once
+      const int sub = lane / LANES, d = lane % LANES * 8, n_rows = n_pos * p.group;
+#pragma unroll 4
+      for (int row = warp * ROWS + sub; row < n_rows; row += 8 * ROWS) {
+        const float* const src = so + row * D;
+        const float4 a = *reinterpret_cast<const float4*>(src + ((d >> 2) ^ (row & 7)) * 4), b = *reinterpret_cast<const float4*>(src + (((d >> 2) + 1) ^ (row & 7)) * 4);
+        const int pos = row * p.inv_group >> 16;
+        const size_t at = static_cast<size_t>(tile.row0 + tile.p0 + pos) * p.n_q + kh * p.group + (row - pos * p.group);
+        if (cut) {
+          float* const dst = p.part_acc + (at * p.max_splits + blockIdx.z) * D + d;
+          *reinterpret_cast<float4*>(dst) = a;
+          *reinterpret_cast<float4*>(dst + 4) = b;
+        } else {
+          const uint4 g = *reinterpret_cast<const uint4*>(p.gate + at * D + d);
+          const uint32_t* gw = reinterpret_cast<const uint32_t*>(&g);
+          const float o[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+          uint4 out;
+          __nv_bfloat162* oe = reinterpret_cast<__nv_bfloat162*>(&out);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) oe[j] = __float2bfloat16(o[j] * inv * sigmoid_f(__bfloat162float(ge[j])));
-          *reinterpret_cast<uint4*>(p.out + base + c) = out[0];
-          *reinterpret_cast<uint4*>(p.out + base + c + 8) = out[1];
+          for (int j = 0; j < 4; ++j)
+            oe[j] = __floats2bfloat162_rn(o[2 * j] * kv8_sigmoid(__uint_as_float(gw[j] << 16)), o[2 * j + 1] * kv8_sigmoid(__uint_as_float(gw[j] & 0xffff0000u)));
+          *reinterpret_cast<uint4*>(p.out + at * D + d) = out;
         }
       }
     }
@@ -553,8 +576,8 @@ kv8_prefill_combine_kernel(Kv8PrefillParams p) {
     const bf16* g = p.gate + at * D + quad * 4;
     uint2 raw;
     __nv_bfloat162* e = reinterpret_cast<__nv_bfloat162*>(&raw);
-    e[0] = __floats2bfloat162_rn(o.x * inv * sigmoid_f(__bfloat162float(g[0])), o.y * inv * sigmoid_f(__bfloat162float(g[1])));
-    e[1] = __floats2bfloat162_rn(o.z * inv * sigmoid_f(__bfloat162float(g[2])), o.w * inv * sigmoid_f(__bfloat162float(g[3])));
+    e[0] = __floats2bfloat162_rn(o.x * inv * kv8_sigmoid(__bfloat162float(g[0])), o.y * inv * kv8_sigmoid(__bfloat162float(g[1])));
+    e[1] = __floats2bfloat162_rn(o.z * inv * kv8_sigmoid(__bfloat162float(g[2])), o.w * inv * kv8_sigmoid(__bfloat162float(g[3])));
     *reinterpret_cast<uint2*>(p.out + at * D + quad * 4) = raw;
   }
 }
@@ -591,7 +614,7 @@ int k8p_launch(const CUtensorMap& tm, const CUtensorMap& te, const Kv8PrefillPar
   }
   if (launch_pdl(kern, dim3(n_tiles, p.n_kv, p.max_splits), dim3(K8P_THREADS), Kv8PrefillCfg<D>::SMEM, st, tm, te, p) != cudaSuccess) return -4;
   if (p.max_splits == 1) return 0;
-  return launch_pdl(kv8_prefill_combine_kernel<D>, dim3(n_tiles, p.n_kv, 8), dim3(256), 0, st, p) == cudaSuccess ? 0 : -4;
+  return launch_pdl(kv8_prefill_combine_kernel<D>, dim3(n_tiles, p.n_kv, (128 + 256 / (D / 4) - 1) / (256 / (D / 4))), dim3(256), 0, st, p) == cudaSuccess ? 0 : -4;
 }
 }  // namespace
 
@@ -629,7 +652,7 @@ extern "C" int b200_kv8_prefill(const void* q, const void* gate, const void* dat
       k8p_encode(&te, exps, 3, edims, estrides, ebox, CU_TENSOR_MAP_SWIZZLE_NONE)) return -1;
   const Kv8PrefillParams p{static_cast<const bf16*>(q), static_cast<const bf16*>(gate), starts, pos0, tables, static_cast<bf16*>(out), part_acc,
                            reinterpret_cast<float2*>(part_ml), segs, max_pages, width, num_pages, n_q, n_kv, group, 128 / group, max_splits,
-                           1.4426950408889634f / sqrtf(static_cast<float>(D)), err};
+                           (65536 + group - 1) / group, 1.4426950408889634f / sqrtf(static_cast<float>(D)), err};
   if (D == 256) return k8p_launch<256>(tm, te, p, n_tiles, st);
   if (D == 128) return k8p_launch<128>(tm, te, p, n_tiles, st);
   return k8p_launch<64>(tm, te, p, n_tiles, st);
