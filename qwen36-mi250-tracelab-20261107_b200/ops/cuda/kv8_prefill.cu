@@ -233,11 +233,11 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
       uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
+        // the first four significant bits, and the other four
         const float a = __uint_as_float(word[k] << 16) * f, b = __uint_as_float(word[k] & 0xffff0000u) * f;
-        const uint32_t two = kv8_pack2(a, b), hh = kv8_unpack2(static_cast<uint16_t>(two));
-        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hh));
-        hi[k / 2] |= two << (16 * (k & 1));
-        lo[k / 2] |= kv8_pack2(a - back.x, b - back.y) << (16 * (k & 1));
+        const float ah = __uint_as_float(__float_as_uint(a) & 0xfff00000u), bh = __uint_as_float(__float_as_uint(b) & 0xfff00000u);
+        hi[k / 2] |= kv8_pack2(ah, bh) << (16 * (k & 1));
+        lo[k / 2] |= kv8_pack2(a - ah, b - bh) << (16 * (k & 1));
       }
       if (lane * 8 < D) {
         uint8_t* const at = sQ + r * D + (((lane >> 1) ^ (r & (D / 16 - 1))) << 4) + (lane & 1) * 8;
@@ -478,6 +478,21 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
       mbar_arrive(&p_full[hf]);
     }
     float l = l2.x + l2.y;
+    // the gates of the rows that this warp will write are asked for ahead of the last products
+    constexpr int LANES = D / 8, ROWS = 32 / LANES, STEPS = 16 / ROWS;  // 8 numbers a lane, rows a warp takes at once
+    const int sub = lane / LANES, d = lane % LANES * 8, n_rows = n_pos * p.group;
+    const size_t head0 = static_cast<size_t>(tile.row0 + tile.p0) * p.n_q + kh * p.group;
+    const auto head_of = [&](int row) {
+      const int pos = row * p.inv_group >> 16;
+      return head0 + static_cast<size_t>(pos) * p.n_q + (row - pos * p.group);
+    };
+    uint4 gate[STEPS];
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      const int row = (i * 8 + warp) * ROWS + sub;
+      gate[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (!cut && row < n_rows) gate[i] = __ldg(reinterpret_cast<const uint4*>(p.gate + head_of(row) * D + d));
+    }
     ok = ok && mbar_wait(acc_done, 0, p.err, ERR_WAIT_TMEM, abort_flag) && !*abort_flag;
     tc_fence_after();
     float m_used = m_loc;
@@ -511,21 +526,19 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
       ok = mbar_wait(x_bar, 1, p.err, ERR_WAIT_FULL, abort_flag);
     }
     if (ok) {
-      constexpr int LANES = D / 8, ROWS = 32 / LANES;      // 8 numbers a lane, rows a warp takes at once
-      const int sub = lane / LANES, d = lane % LANES * 8, n_rows = n_pos * p.group;
-#pragma unroll 4
-      for (int row = warp * ROWS + sub; row < n_rows; row += 8 * ROWS) {
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        const int row = (i * 8 + warp) * ROWS + sub;
+        if (row >= n_rows) break;
         const float* const src = so + row * D;
         const float4 a = *reinterpret_cast<const float4*>(src + ((d >> 2) ^ (row & 7)) * 4), b = *reinterpret_cast<const float4*>(src + (((d >> 2) + 1) ^ (row & 7)) * 4);
-        const int pos = row * p.inv_group >> 16;
-        const size_t at = static_cast<size_t>(tile.row0 + tile.p0 + pos) * p.n_q + kh * p.group + (row - pos * p.group);
+        const size_t at = head_of(row);
         if (cut) {
           float* const dst = p.part_acc + (at * p.max_splits + blockIdx.z) * D + d;
           *reinterpret_cast<float4*>(dst) = a;
           *reinterpret_cast<float4*>(dst + 4) = b;
         } else {
-          const uint4 g = *reinterpret_cast<const uint4*>(p.gate + at * D + d);
-          const uint32_t* gw = reinterpret_cast<const uint32_t*>(&g);
+          const uint32_t* gw = reinterpret_cast<const uint32_t*>(&gate[i]);
           const float o[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
           uint4 out;
           __nv_bfloat162* oe = reinterpret_cast<__nv_bfloat162*>(&out);
