@@ -51,7 +51,7 @@ struct Kv8PrefillCfg {
   static constexpr int V_BYTES = KV8_PAGE * D * 2;     // [HB][64 rows][128]: values as halves
   static constexpr int P_BYTES = 128 * 128;            // [128 rows][64 halves]
   static constexpr int EXPS = 2 * KV8_PAGE;
-  static constexpr int SMEM = 2 * Q_TERM + 4 * PAGE_BYTES + 2 * V_BYTES + 2 * P_BYTES + 4 * EXPS + 2 * 3 * KV8_PAGE * 4 + 512 + 256;
+  static constexpr int SMEM = 2 * Q_TERM + 4 * PAGE_BYTES + 2 * V_BYTES + 2 * P_BYTES + 4 * EXPS + 2 * 3 * KV8_PAGE * 4 + 512 + 46 * 8;
   static constexpr int TMEM_COLS = 128 + D + D / 2 <= 256 ? 256 : 512;  // two score tiles of 64, the output, two terms of the queries
 };
 
@@ -144,32 +144,37 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
     return;
   }
   uint8_t* const sQ = smem_k8p;                          // [2 terms]
-  uint8_t* const sK = sQ + 2 * C::Q_TERM;                // [2]
-  uint8_t* const sV8 = sK + 2 * C::PAGE_BYTES;           // [2]
-  uint8_t* const sV = sV8 + 2 * C::PAGE_BYTES;           // [2]
+  // Pages' keys and values, four of each: two of each in the place of the queries, once those are in TMEM. (With two of each, a
+  // load had to come and its products to end within two pages: 1.71 ms for 4 x 2048 rows of long prompts.)
+  const auto k_slot = [&](int s) { return sQ + (s < 2 ? 4 + s : s - 2) * C::PAGE_BYTES; };
+  const auto v_slot = [&](int s) { return sQ + (s < 2 ? 6 + s : s) * C::PAGE_BYTES; };
+  static_assert(2 * C::Q_TERM == 4 * C::PAGE_BYTES, "slots in the place of the queries");
+  uint8_t* const sV = sQ + 8 * C::PAGE_BYTES;            // [2]
   uint8_t* const sP = sV + 2 * C::V_BYTES;               // [2]: page i uses tile i & 1
   uint8_t* const sE = sP + 2 * C::P_BYTES;               // [4][keys' 64, values' 64] exponents
   float* const sT = reinterpret_cast<float*>(sE + 4 * C::EXPS);  // [2][2^a | b | 2^-b][64]
   float* const s_m = sT + 2 * 3 * KV8_PAGE;              // [128] the running maximum of a row, in the hands of the page that is to see its scores next
   uint64_t* const bars = reinterpret_cast<uint64_t*>(s_m + 128);
-  uint64_t* const k_full = bars;                         // [2]
-  uint64_t* const k_empty = bars + 2;                    // [2]
-  uint64_t* const v8_full = bars + 4;                    // [2]
-  uint64_t* const v8_empty = bars + 6;                   // [2]
-  uint64_t* const v_full = bars + 8;                     // [2]
-  uint64_t* const v_empty = bars + 10;                   // [2]
-  uint64_t* const s_full = bars + 12;                    // [2]
-  uint64_t* const p_full = bars + 14;                    // [2]
-  uint64_t* const pv_done = bars + 16;                   // [2]
-  uint64_t* const e_full = bars + 18;                    // [4]
-  uint64_t* const t_full = bars + 22;                    // [2]
-  uint64_t* const acc_done = bars + 24;
-  uint64_t* const x_bar = bars + 25;
-  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 26);
+  uint64_t* const k_full = bars;                         // [4]
+  uint64_t* const k_empty = bars + 4;                    // [4]
+  uint64_t* const v8_full = bars + 8;                    // [4]
+  uint64_t* const v8_empty = bars + 12;                  // [4]
+  uint64_t* const e_full = bars + 16;                    // [4]
+  uint64_t* const e_empty = bars + 20;                   // [4]
+  uint64_t* const v_full = bars + 24;                    // [2]
+  uint64_t* const v_empty = bars + 26;                   // [2]
+  uint64_t* const s_full = bars + 28;                    // [2]
+  uint64_t* const p_full = bars + 30;                    // [2]
+  uint64_t* const pv_done = bars + 32;                   // [2]
+  uint64_t* const t_full = bars + 34;                    // [2]
+  uint64_t* const m_bar = bars + 36;                     // [2]: the row maxima up to an even / odd page
+  uint64_t* const acc_done = bars + 38;
+  uint64_t* const x_bar = bars + 39;
+  uint64_t* const q_ready = bars + 40;                   // the queries' terms are in shared memory, in TMEM
+  uint64_t* const q_full = bars + 41;
+  uint64_t* const s_empty = bars + 42;                   // [2]: the scores are in their threads' registers
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 44);
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  uint64_t* const q_full = bars + 29;
-  uint64_t* const q_ready = bars + 30;
-  uint64_t* const m_bar = bars + 27;                     // [2]: the row maxima up to an even / odd page
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
@@ -186,11 +191,13 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); mbar_init(&v8_full[s], 1); mbar_init(&v8_empty[s], 128);
       mbar_init(&v_full[s], 128); mbar_init(&v_empty[s], 1); mbar_init(&s_full[s], 1); mbar_init(&p_full[s], 128);
-      mbar_init(&pv_done[s], 1); mbar_init(&t_full[s], 128); mbar_init(&m_bar[s], 128);
+      mbar_init(&pv_done[s], 1); mbar_init(&t_full[s], 128); mbar_init(&s_empty[s], 128); mbar_init(&m_bar[s], 128);
     }
-    for (int s = 0; s < 4; ++s) mbar_init(&e_full[s], 1);
+    for (int s = 0; s < 4; ++s) {
+      mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); mbar_init(&v8_full[s], 1); mbar_init(&v8_empty[s], 128);
+      mbar_init(&e_full[s], 1); mbar_init(&e_empty[s], 128);
+    }
     mbar_init(acc_done, 1);
     mbar_init(x_bar, 256);
     mbar_init(q_ready, K8P_THREADS - 64);
@@ -256,24 +263,26 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
       const int* table = p.tables + static_cast<size_t>(tile.seg) * p.max_pages + first;
       int next = table[0];
       for (int i = 0; i < np; ++i) {
-        const int s = i & 1;
+        const int s = i & 3;
+        const uint32_t again = ((i >> 2) & 1) ^ 1;
         int page = next;
         if (i + 1 < np) next = table[i + 1];
         if (page < 0 || page >= p.num_pages) { atomicCAS(p.err, 0, ERR_BAD_INDEX); page = 0; }
         const int row = (page * 2 * p.n_kv + kh) * KV8_PAGE;
-        // (the exponents' slot of page i was read before the scores of page i - 2 were asked for)
-        if (!mbar_wait(&k_empty[s], ((i >> 1) & 1) ^ 1, p.err, ERR_WAIT_EMPTY, abort_flag)) break;
+        if (i == 2 && !mbar_wait(q_full, 0, p.err, ERR_WAIT_FULL, abort_flag)) break;  // the queries' place is free
+        if (!mbar_wait(&k_empty[s], again, p.err, ERR_WAIT_EMPTY, abort_flag)) break;
         mbar_expect_tx(&k_full[s], C::PAGE_BYTES);
 #pragma unroll
         for (int b = 0; b < C::DB; ++b)
-          tma_load_2d(sK + s * C::PAGE_BYTES + b * KV8_PAGE * C::ROWB, &tm, &k_full[s], b * C::ROWB, row);
-        mbar_expect_tx(&e_full[i & 3], C::EXPS);
-        tma_load_3d(sE + (i & 3) * C::EXPS, &tm_exps, &e_full[i & 3], 0, kh, page * 2);
-        if (!mbar_wait(&v8_empty[s], ((i >> 1) & 1) ^ 1, p.err, ERR_WAIT_EMPTY, abort_flag)) break;
+          tma_load_2d(k_slot(s) + b * KV8_PAGE * C::ROWB, &tm, &k_full[s], b * C::ROWB, row);
+        if (!mbar_wait(&e_empty[s], again, p.err, ERR_WAIT_EMPTY, abort_flag)) break;
+        mbar_expect_tx(&e_full[s], C::EXPS);
+        tma_load_3d(sE + s * C::EXPS, &tm_exps, &e_full[s], 0, kh, page * 2);
+        if (!mbar_wait(&v8_empty[s], again, p.err, ERR_WAIT_EMPTY, abort_flag)) break;
         mbar_expect_tx(&v8_full[s], C::PAGE_BYTES);
 #pragma unroll
         for (int b = 0; b < C::DB; ++b)
-          tma_load_2d(sV8 + s * C::PAGE_BYTES + b * KV8_PAGE * C::ROWB, &tm, &v8_full[s], b * C::ROWB, row + p.n_kv * KV8_PAGE);
+          tma_load_2d(v_slot(s) + b * KV8_PAGE * C::ROWB, &tm, &v8_full[s], b * C::ROWB, row + p.n_kv * KV8_PAGE);
       }
     }
   } else if (warp == 8) {
@@ -282,10 +291,10 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
       constexpr uint32_t idesc_s = (1u << 4) | (64u >> 3) << 17 | (128u >> 4) << 24;                                     // e4m3
       constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | static_cast<uint32_t>(D >> 3) << 17 | (128u >> 4) << 24;     // halves, B MN-major
       auto issue_qk = [&](int i) {
-        const int s = i & 1;
-        if (!mbar_wait(&k_full[s], (i >> 1) & 1, p.err, ERR_WAIT_FULL, abort_flag)) return false;
+        const int s = i & 1, ks = i & 3;
+        if (!mbar_wait(&k_full[ks], (i >> 2) & 1, p.err, ERR_WAIT_FULL, abort_flag)) return false;
         tc_fence_after();
-        const uint32_t ka = smem_u32(sK + s * C::PAGE_BYTES);
+        const uint32_t ka = smem_u32(k_slot(ks));
 #pragma unroll
         for (int term = 0; term < 2; ++term)
 #pragma unroll
@@ -296,16 +305,16 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
                         k8p_desc<C::ROWB>(ka + blk * KV8_PAGE * C::ROWB + off), idesc_s, (term | kk) != 0);
           }
         umma_commit(&s_full[s]);
-        umma_commit(&k_empty[s]);
+        umma_commit(&k_empty[ks]);
         return true;
       };
       bool ok = mbar_wait(q_full, 0, p.err, ERR_WAIT_FULL, abort_flag) && issue_qk(0) && (np < 2 || issue_qk(1));
       for (int i = 0; i < np && ok; ++i) {
         const int s = i & 1;
-        // the weights of page i are written, so its score tile has been read: the scores of page i + 2 go first
-        ok = mbar_wait(&p_full[s], (i >> 1) & 1, p.err, ERR_WAIT_FULL, abort_flag);
-        if (ok && i + 2 < np) ok = issue_qk(i + 2);
-        ok = ok && mbar_wait(&v_full[s], (i >> 1) & 1, p.err, ERR_WAIT_FULL, abort_flag);
+        // the scores of page i + 2 as soon as those of page i have been read, while their weights are made
+        if (i + 2 < np) ok = mbar_wait(&s_empty[s], (i >> 1) & 1, p.err, ERR_WAIT_TMEM, abort_flag) && issue_qk(i + 2);
+        ok = ok && mbar_wait(&p_full[s], (i >> 1) & 1, p.err, ERR_WAIT_FULL, abort_flag)
+             && mbar_wait(&v_full[s], (i >> 1) & 1, p.err, ERR_WAIT_FULL, abort_flag);
         if (!ok) break;
         tc_fence_after();
         const uint32_t pa = smem_u32(sP + s * C::P_BYTES), va = smem_u32(sV + s * C::V_BYTES);
@@ -332,10 +341,11 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
     bool ok = true;
     for (int i = 0; i < np; ++i) {
       const int s = i & 1;
-      ok = mbar_wait(&e_full[i & 3], (i >> 2) & 1, p.err, ERR_WAIT_FULL, abort_flag)
+      const int vs = i & 3;
+      ok = mbar_wait(&e_full[vs], (i >> 2) & 1, p.err, ERR_WAIT_FULL, abort_flag)
            && (i < 2 || mbar_wait(&p_full[s], ((i - 2) >> 1) & 1, p.err, ERR_WAIT_FULL, abort_flag));
       if (!ok) break;
-      const uint32_t byte = sE[(i & 3) * C::EXPS + tid];  // threads 0 .. 63: a key's, then a value's
+      const uint32_t byte = sE[vs * C::EXPS + tid];  // threads 0 .. 63: a key's, then a value's
       float* const t = sT + s * 3 * KV8_PAGE;
       if (tid < KV8_PAGE) {
         t[tid] = kv8_factor(byte);
@@ -344,10 +354,11 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
         t[KV8_PAGE + tid] = kv8_two_to(max(-126, 127 - static_cast<int>(byte)));
       }
       mbar_arrive(&t_full[s]);
-      ok = mbar_wait(&v8_full[s], (i >> 1) & 1, p.err, ERR_WAIT_FULL, abort_flag)
+      mbar_arrive(&e_empty[vs]);
+      ok = mbar_wait(&v8_full[vs], (i >> 2) & 1, p.err, ERR_WAIT_FULL, abort_flag)
            && (i < 2 || mbar_wait(&v_empty[s], ((i - 2) >> 1) & 1, p.err, ERR_WAIT_EMPTY, abort_flag));
       if (!ok) break;
-      const uint8_t* const src = sV8 + s * C::PAGE_BYTES + from;
+      const uint8_t* const src = v_slot(vs) + from;
       uint8_t* const dst = sV + s * C::V_BYTES;
 #pragma unroll
       for (int c = 0; c < KV8_PAGE / ROWS; ++c) {
@@ -362,7 +373,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(&v_full[s]);
-      mbar_arrive(&v8_empty[s]);
+      mbar_arrive(&v8_empty[vs]);
     }
   } else {
     // ---------------- softmax + epilogue: thread (r = tid & 127, hf = tid >> 7) owns row r = one (position, head) on the pages
@@ -398,6 +409,8 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
       tc_fence_after();
       float2 y[32];
       tmem_ld64(tmem_S + hf * 64 + lane_base, reinterpret_cast<float*>(y));
+      tc_fence_before();
+      mbar_arrive(&s_empty[hf]);
       const float* t = sT + hf * 3 * KV8_PAGE;
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
