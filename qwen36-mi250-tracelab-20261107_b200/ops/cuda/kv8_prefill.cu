@@ -51,7 +51,7 @@ struct Kv8PrefillCfg {
   static constexpr int V_BYTES = KV8_PAGE * D * 2;     // [HB][64 rows][128]: values as halves
   static constexpr int P_BYTES = 128 * 128;            // [128 rows][64 halves]
   static constexpr int EXPS = 2 * KV8_PAGE;
-  static constexpr int SMEM = 2 * Q_TERM + 4 * PAGE_BYTES + 2 * V_BYTES + 2 * P_BYTES + 4 * EXPS + 2 * 3 * KV8_PAGE * 4 + 512 + 46 * 8;
+  static constexpr int SMEM = 7 * PAGE_BYTES + 2 * V_BYTES + 2 * P_BYTES + 4 * EXPS + 4 * 3 * KV8_PAGE * 4 + 512 + 53 * 8;
   static constexpr int TMEM_COLS = 128 + D + D / 2 <= 256 ? 256 : 512;  // two score tiles of 64, the output, two terms of the queries
 };
 
@@ -144,19 +144,19 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
     return;
   }
   uint8_t* const sQ = smem_k8p;                          // [2 terms]
-  // Pages' keys and values, four of each: two of each in the place of the queries, once those are in TMEM. (With two of each, a
-  // load had to come and its products to end within two pages: 1.71 ms for 4 x 2048 rows of long prompts.)
-  const auto k_slot = [&](int s) { return sQ + (s < 2 ? 4 + s : s - 2) * C::PAGE_BYTES; };
-  const auto v_slot = [&](int s) { return sQ + (s < 2 ? 6 + s : s) * C::PAGE_BYTES; };
+  // Keys of three pages and values of four, stored: of one and three in the place of the queries, once those are in TMEM. (With two
+  // of each, a load had to come and its products to end within two pages.)
+  const auto k_slot = [&](int s) { return sQ + (s < 2 ? 4 + s : 0) * C::PAGE_BYTES; };
+  const auto v_slot = [&](int s) { return sQ + (s == 0 ? 6 : s) * C::PAGE_BYTES; };
   static_assert(2 * C::Q_TERM == 4 * C::PAGE_BYTES, "slots in the place of the queries");
-  uint8_t* const sV = sQ + 8 * C::PAGE_BYTES;            // [2]
+  uint8_t* const sV = sQ + 7 * C::PAGE_BYTES;            // [2]
   uint8_t* const sP = sV + 2 * C::V_BYTES;               // [2]: page i uses tile i & 1
   uint8_t* const sE = sP + 2 * C::P_BYTES;               // [4][keys' 64, values' 64] exponents
-  float* const sT = reinterpret_cast<float*>(sE + 4 * C::EXPS);  // [2][2^a | b | 2^-b][64]
-  float* const s_m = sT + 2 * 3 * KV8_PAGE;              // [128] the running maximum of a row, in the hands of the page that is to see its scores next
+  float* const sT = reinterpret_cast<float*>(sE + 4 * C::EXPS);  // [4][2^a | b | 2^-b][64]
+  float* const s_m = sT + 4 * 3 * KV8_PAGE;              // [128] the running maximum of a row, in the hands of the page that is to see its scores next
   uint64_t* const bars = reinterpret_cast<uint64_t*>(s_m + 128);
-  uint64_t* const k_full = bars;                         // [4]
-  uint64_t* const k_empty = bars + 4;                    // [4]
+  uint64_t* const k_full = bars;                         // [3]
+  uint64_t* const k_empty = bars + 4;                    // [3]
   uint64_t* const v8_full = bars + 8;                    // [4]
   uint64_t* const v8_empty = bars + 12;                  // [4]
   uint64_t* const e_full = bars + 16;                    // [4]
@@ -166,14 +166,15 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
   uint64_t* const s_full = bars + 28;                    // [2]
   uint64_t* const p_full = bars + 30;                    // [2]
   uint64_t* const pv_done = bars + 32;                   // [2]
-  uint64_t* const t_full = bars + 34;                    // [2]
+  uint64_t* const t_full = bars + 44;                    // [4]
   uint64_t* const m_bar = bars + 36;                     // [2]: the row maxima up to an even / odd page
   uint64_t* const acc_done = bars + 38;
   uint64_t* const x_bar = bars + 39;
   uint64_t* const q_ready = bars + 40;                   // the queries' terms are in shared memory, in TMEM
   uint64_t* const q_full = bars + 41;
   uint64_t* const s_empty = bars + 42;                   // [2]: the scores are in their threads' registers
-  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 44);
+  uint64_t* const t_empty = bars + 48;                   // [4]
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 52);
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -192,11 +193,11 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) {
       mbar_init(&v_full[s], 128); mbar_init(&v_empty[s], 1); mbar_init(&s_full[s], 1); mbar_init(&p_full[s], 128);
-      mbar_init(&pv_done[s], 1); mbar_init(&t_full[s], 128); mbar_init(&s_empty[s], 128); mbar_init(&m_bar[s], 128);
+      mbar_init(&pv_done[s], 1); mbar_init(&s_empty[s], 128); mbar_init(&m_bar[s], 128);
     }
     for (int s = 0; s < 4; ++s) {
       mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); mbar_init(&v8_full[s], 1); mbar_init(&v8_empty[s], 128);
-      mbar_init(&e_full[s], 1); mbar_init(&e_empty[s], 128);
+      mbar_init(&e_full[s], 1); mbar_init(&e_empty[s], 128); mbar_init(&t_full[s], 128); mbar_init(&t_empty[s], 128);
     }
     mbar_init(acc_done, 1);
     mbar_init(x_bar, 256);
@@ -263,21 +264,21 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
       const int* table = p.tables + static_cast<size_t>(tile.seg) * p.max_pages + first;
       int next = table[0];
       for (int i = 0; i < np; ++i) {
-        const int s = i & 3;
+        const int s = i & 3, ks = i % 3;
         const uint32_t again = ((i >> 2) & 1) ^ 1;
         int page = next;
         if (i + 1 < np) next = table[i + 1];
         if (page < 0 || page >= p.num_pages) { atomicCAS(p.err, 0, ERR_BAD_INDEX); page = 0; }
         const int row = (page * 2 * p.n_kv + kh) * KV8_PAGE;
-        if (i == 2 && !mbar_wait(q_full, 0, p.err, ERR_WAIT_FULL, abort_flag)) break;  // the queries' place is free
-        if (!mbar_wait(&k_empty[s], again, p.err, ERR_WAIT_EMPTY, abort_flag)) break;
-        mbar_expect_tx(&k_full[s], C::PAGE_BYTES);
+        if (!mbar_wait(&k_empty[ks], ((i / 3) & 1) ^ 1, p.err, ERR_WAIT_EMPTY, abort_flag)) break;
+        mbar_expect_tx(&k_full[ks], C::PAGE_BYTES);
 #pragma unroll
         for (int b = 0; b < C::DB; ++b)
-          tma_load_2d(k_slot(s) + b * KV8_PAGE * C::ROWB, &tm, &k_full[s], b * C::ROWB, row);
+          tma_load_2d(k_slot(ks) + b * KV8_PAGE * C::ROWB, &tm, &k_full[ks], b * C::ROWB, row);
         if (!mbar_wait(&e_empty[s], again, p.err, ERR_WAIT_EMPTY, abort_flag)) break;
         mbar_expect_tx(&e_full[s], C::EXPS);
         tma_load_3d(sE + s * C::EXPS, &tm_exps, &e_full[s], 0, kh, page * 2);
+        if (i == 1 && !mbar_wait(q_full, 0, p.err, ERR_WAIT_FULL, abort_flag)) break;  // from here on in the queries' place
         if (!mbar_wait(&v8_empty[s], again, p.err, ERR_WAIT_EMPTY, abort_flag)) break;
         mbar_expect_tx(&v8_full[s], C::PAGE_BYTES);
 #pragma unroll
@@ -291,8 +292,8 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
       constexpr uint32_t idesc_s = (1u << 4) | (64u >> 3) << 17 | (128u >> 4) << 24;                                     // e4m3
       constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | static_cast<uint32_t>(D >> 3) << 17 | (128u >> 4) << 24;     // halves, B MN-major
       auto issue_qk = [&](int i) {
-        const int s = i & 1, ks = i & 3;
-        if (!mbar_wait(&k_full[ks], (i >> 2) & 1, p.err, ERR_WAIT_FULL, abort_flag)) return false;
+        const int s = i & 1, ks = i % 3;
+        if (!mbar_wait(&k_full[ks], (i / 3) & 1, p.err, ERR_WAIT_FULL, abort_flag)) return false;
         tc_fence_after();
         const uint32_t ka = smem_u32(k_slot(ks));
 #pragma unroll
@@ -338,24 +339,29 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
     const uint32_t from = k / (C::ROWB / 16) * KV8_PAGE * C::ROWB + k8p_at<C::ROWB>(r, k % (C::ROWB / 16));
     const uint32_t to0 = k / 4 * KV8_PAGE * 128 + k8p_at<128>(r, (k & 3) * 2 + swap);
     const uint32_t to1 = k / 4 * KV8_PAGE * 128 + k8p_at<128>(r, (k & 3) * 2 + 1 - swap);
-    bool ok = true;
-    for (int i = 0; i < np; ++i) {
-      const int s = i & 1;
-      const int vs = i & 3;
-      ok = mbar_wait(&e_full[vs], (i >> 2) & 1, p.err, ERR_WAIT_FULL, abort_flag)
-           && (i < 2 || mbar_wait(&p_full[s], ((i - 2) >> 1) & 1, p.err, ERR_WAIT_FULL, abort_flag));
-      if (!ok) break;
-      const uint32_t byte = sE[vs * C::EXPS + tid];  // threads 0 .. 63: a key's, then a value's
-      float* const t = sT + s * 3 * KV8_PAGE;
+    // What goes with a page's keys and values, two pages ahead of the conversion: the scores wait for it
+    const auto numbers = [&](int i) {
+      const int es = i & 3;
+      const bool ok = mbar_wait(&e_full[es], (i >> 2) & 1, p.err, ERR_WAIT_FULL, abort_flag)
+                      && mbar_wait(&t_empty[es], ((i >> 2) & 1) ^ 1, p.err, ERR_WAIT_EMPTY, abort_flag);
+      if (!ok) return false;
+      const uint32_t byte = sE[es * C::EXPS + tid];  // threads 0 .. 63: a key's, then a value's
+      float* const t = sT + es * 3 * KV8_PAGE;
       if (tid < KV8_PAGE) {
         t[tid] = kv8_factor(byte);
       } else {
         t[tid] = byte == KV8_E_NAN ? __uint_as_float(0x7fffffffu) : static_cast<float>(static_cast<int>(byte) - 127);
         t[KV8_PAGE + tid] = kv8_two_to(max(-126, 127 - static_cast<int>(byte)));
       }
-      mbar_arrive(&t_full[s]);
-      mbar_arrive(&e_empty[vs]);
-      ok = mbar_wait(&v8_full[vs], (i >> 2) & 1, p.err, ERR_WAIT_FULL, abort_flag)
+      mbar_arrive(&t_full[es]);
+      mbar_arrive(&e_empty[es]);
+      return true;
+    };
+    bool ok = numbers(0) && (np < 2 || numbers(1));
+    for (int i = 0; i < np && ok; ++i) {
+      const int s = i & 1, vs = i & 3;
+      ok = (i + 2 >= np || numbers(i + 2))
+           && mbar_wait(&v8_full[vs], (i >> 2) & 1, p.err, ERR_WAIT_FULL, abort_flag)
            && (i < 2 || mbar_wait(&v_empty[s], ((i - 2) >> 1) & 1, p.err, ERR_WAIT_EMPTY, abort_flag));
       if (!ok) break;
       const uint8_t* const src = v_slot(vs) + from;
@@ -404,14 +410,14 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
     asm volatile("bar.sync 1, 256;" ::: "memory");  // all have read it: the weights' tiles may be written. Nobody has left before
     for (int i = hf; i < np && ok; i += 2) {
       const uint32_t ph = (i >> 1) & 1;
-      ok = mbar_wait(&t_full[hf], ph, p.err, ERR_WAIT_FULL, abort_flag) && mbar_wait(&s_full[hf], ph, p.err, ERR_WAIT_TMEM, abort_flag);
+      ok = mbar_wait(&t_full[i & 3], (i >> 2) & 1, p.err, ERR_WAIT_FULL, abort_flag) && mbar_wait(&s_full[hf], ph, p.err, ERR_WAIT_TMEM, abort_flag);
       if (!ok) break;
       tc_fence_after();
       float2 y[32];
       tmem_ld64(tmem_S + hf * 64 + lane_base, reinterpret_cast<float*>(y));
       tc_fence_before();
       mbar_arrive(&s_empty[hf]);
-      const float* t = sT + hf * 3 * KV8_PAGE;
+      const float* t = sT + (i & 3) * 3 * KV8_PAGE;
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         const float4 a = *reinterpret_cast<const float4*>(t + 4 * j), b = *reinterpret_cast<const float4*>(t + KV8_PAGE + 4 * j);
@@ -489,6 +495,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       tc_fence_before();
       mbar_arrive(&p_full[hf]);
+      mbar_arrive(&t_empty[i & 3]);
     }
     float l = l2.x + l2.y;
     // the gates of the rows that this warp will write are asked for ahead of the last products
