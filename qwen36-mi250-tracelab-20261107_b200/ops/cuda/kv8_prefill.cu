@@ -13,7 +13,7 @@
 //   O[128 x D]  += P[128 x 64] V       P and V as halves: four warps make them of the page's bytes (exact)
 //
 // Two groups of four warps take alternate pages, a thread a row; the running maximum goes from one to the other, and the output tile in
-// TMEM is rescaled where a maximum grew by more than 2^LAZY. Weights as halves reach from 2^15 to 2^-24, 2^-31 of the largest at the least.
+// TMEM is rescaled where a maximum grew by more than 2^LAZY. Weights as halves reach from 2^15 to 2^-24, 2^-28 of the largest at the least.
 // A span of few tiles over a long context is cut into runs of pages for CTAs of their own, by its own length and position alone, whose partial
 // sums are added in their order: a row's bits depend on its span, never on the pass. All waits are bounded. No cluster multicast.
 #include <cuda_fp16.h>
@@ -22,7 +22,7 @@
 
 namespace b200 {
 
-constexpr float K8P_LIFT = 7.0f, K8P_LAZY = 8.0f;  // weights stay below 2^15
+constexpr float K8P_LIFT = 4.0f, K8P_LAZY = 11.0f;  // weights stay below 2^15
 constexpr int K8P_THREADS = 448;                   // 8 warps softmax, MMA, loads, 4 warps values
 constexpr int K8P_CTAS = 128, K8P_MIN_PAGES = 4;   // a span is cut for about so many CTAs, into runs of no fewer pages
 
