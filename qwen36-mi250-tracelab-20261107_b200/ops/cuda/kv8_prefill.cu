@@ -85,6 +85,16 @@ __device__ __forceinline__ uint32_t k8p_at(int r, int c) {
   const uint32_t byte = r * ROWB;
   return byte + ((c ^ ((byte >> 7) & (ROWB / 16 - 1))) << 4);
 }
+// Whether a barrier's phase is complete, without a wait.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred P;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 P, [%1], %2;\n\t"
+      "selp.b32 %0, 1, 0, P;\n\t}"
+      : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return done != 0;
+}
 __device__ __forceinline__ float k8p_ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -291,39 +301,44 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
     if (elect_one()) {
       constexpr uint32_t idesc_s = (1u << 4) | (64u >> 3) << 17 | (128u >> 4) << 24;                                     // e4m3
       constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | static_cast<uint32_t>(D >> 3) << 17 | (128u >> 4) << 24;     // halves, B MN-major
-      auto issue_qk = [&](int i) {
-        const int s = i & 1, ks = i % 3;
-        if (!mbar_wait(&k_full[ks], (i / 3) & 1, p.err, ERR_WAIT_FULL, abort_flag)) return false;
-        tc_fence_after();
-        const uint32_t ka = smem_u32(k_slot(ks));
+      // Scores of page q once page q - 2's have been read and the keys are there, products of page v once its weights and values are: whichever
+      // comes first. (In a fixed order one waited behind the other: 1.54 ms for 4 x 2048 rows of long prompts.)
+      if (!mbar_wait(q_full, 0, p.err, ERR_WAIT_FULL, abort_flag)) *abort_flag = 1;
+      int q = 0, v = 0;
+      long long t0 = clock64();
+      while (v < np && !*abort_flag) {
+        if (v < q && mbar_test(&p_full[v & 1], (v >> 1) & 1) && mbar_test(&v_full[v & 1], (v >> 1) & 1)) {
+          tc_fence_after();
+          const int s = v & 1;
+          const uint32_t pa = smem_u32(sP + s * C::P_BYTES), va = smem_u32(sV + s * C::V_BYTES);
 #pragma unroll
-        for (int term = 0; term < 2; ++term)
+          for (int kk = 0; kk < KV8_PAGE / 16; ++kk)
+            umma_bf16(tmem_O, umma_smem_desc(pa + kk * 32), umma_smem_desc_mn(va + kk * 2048, KV8_PAGE * 128), idesc_o, (v | kk) != 0);
+          umma_commit(&pv_done[s]);
+          umma_commit(&v_empty[s]);
+          ++v;
+          t0 = clock64();
+        } else if (q < np && (q < 2 || mbar_test(&s_empty[q & 1], ((q - 2) >> 1) & 1)) && mbar_test(&k_full[q % 3], (q / 3) & 1)) {
+          tc_fence_after();
+          const int s = q & 1, ks = q % 3;
+          const uint32_t ka = smem_u32(k_slot(ks));
 #pragma unroll
-          for (int kk = 0; kk < D / 32; ++kk) {
-            constexpr int STEPS = C::ROWB / 32;
-            const int blk = kk / STEPS, off = kk % STEPS * 32;
-            k8p_umma_f8(tmem_S + s * 64, tmem_Q + term * (D / 4) + kk * 8,
-                        k8p_desc<C::ROWB>(ka + blk * KV8_PAGE * C::ROWB + off), idesc_s, (term | kk) != 0);
-          }
-        umma_commit(&s_full[s]);
-        umma_commit(&k_empty[ks]);
-        return true;
-      };
-      bool ok = mbar_wait(q_full, 0, p.err, ERR_WAIT_FULL, abort_flag) && issue_qk(0) && (np < 2 || issue_qk(1));
-      for (int i = 0; i < np && ok; ++i) {
-        const int s = i & 1;
-        // the scores of page i + 2 as soon as those of page i have been read, while their weights are made
-        if (i + 2 < np) ok = mbar_wait(&s_empty[s], (i >> 1) & 1, p.err, ERR_WAIT_TMEM, abort_flag) && issue_qk(i + 2);
-        ok = ok && mbar_wait(&p_full[s], (i >> 1) & 1, p.err, ERR_WAIT_FULL, abort_flag)
-             && mbar_wait(&v_full[s], (i >> 1) & 1, p.err, ERR_WAIT_FULL, abort_flag);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t pa = smem_u32(sP + s * C::P_BYTES), va = smem_u32(sV + s * C::V_BYTES);
+          for (int term = 0; term < 2; ++term)
 #pragma unroll
-        for (int kk = 0; kk < KV8_PAGE / 16; ++kk)
-          umma_bf16(tmem_O, umma_smem_desc(pa + kk * 32), umma_smem_desc_mn(va + kk * 2048, KV8_PAGE * 128), idesc_o, (i | kk) != 0);
-        umma_commit(&pv_done[s]);
-        umma_commit(&v_empty[s]);
+            for (int kk = 0; kk < D / 32; ++kk) {
+              constexpr int STEPS = C::ROWB / 32;
+              const int blk = kk / STEPS, off = kk % STEPS * 32;
+              k8p_umma_f8(tmem_S + s * 64, tmem_Q + term * (D / 4) + kk * 8, k8p_desc<C::ROWB>(ka + blk * KV8_PAGE * C::ROWB + off),
+                          idesc_s, (term | kk) != 0);
+            }
+          umma_commit(&s_full[s]);
+          umma_commit(&k_empty[ks]);
+          ++q;
+          t0 = clock64();
+        } else if (clock64() - t0 > WAIT_CYCLES) {
+          *abort_flag = 1;
+          atomicCAS(p.err, 0, ERR_WAIT_FULL);
+        }
       }
       umma_commit(acc_done);
     }
