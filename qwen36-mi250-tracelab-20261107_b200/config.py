@@ -241,6 +241,7 @@ class EngineConfig:
     max_seqs: int = 128  # concurrent running sequences (state slots in use by requests)
     state_slots: int = 0  # 0: max_seqs + room for prefix-cache snapshots
     kv_pages: int = 0  # 0: size from free device memory
+    kv_dtype: str = "auto"  # of the KV pool: "auto" (the activations') | "e4m3" (8 bits and a power of two per row, ops/kv8.py)
     kv_fraction: float = 0.85
     reserve_gb: float = 6.0
     prefill_pack_tokens: int = 8192
@@ -298,6 +299,7 @@ class EngineConfig:
             "req_stamps": "ENGINE_REQ_STAMPS",
             "device": "ENGINE_DEVICE",
             "kv_pages": "ENGINE_KV_PAGES",
+            "kv_dtype": "ENGINE_KV_DTYPE",
             "state_slots": "ENGINE_STATE_SLOTS",
         }
         for attr, env in env_map.items():

@@ -26,6 +26,7 @@ import torch
 
 from ..config import PAGE_SIZE, ModelConfig
 from ..ops import spans, torch_ops
+from ..ops.kv8 import Kv8Layer, Kv8Pool
 from ..utils.upload import to_device
 from .checkpoint import LayerWeights, Weights
 
@@ -108,7 +109,8 @@ class Model:
         its share of the routed experts (``parallel.ep.shard_experts``) and exchanges rows with the other ranks inside
         every MoE block, so all ranks must run their forward passes in step. ``pp`` (a ``parallel.pp.PPContext``) marks
         ``weights`` as one rank's run of layers (``parallel.pp.split_layers``): the pass receives its input rows from the
-        rank before and hands its output to the rank after."""
+        rank before and hands its output to the rank after. ``kv_dtype``: the type of the paged KV pool, the activations' by default;
+        ``torch.float8_e4m3fn`` selects the 8-bit pool (``ops/kv8.py``), whose pages take half the memory and half the time to read."""
         self.tp = tp
         self.ep = ep
         self.pp = pp
@@ -120,10 +122,13 @@ class Model:
         self.device, self.dtype = dev, dt
         self.num_pages, self.state_slots = num_pages, state_slots
         # page 0 and slot 0 are scratch targets for the padding rows of fixed-size graph buckets
-        self.kv = torch.zeros(
-            cfg.num_kv_layers, num_pages, 2, cfg.num_key_value_heads, PAGE_SIZE, cfg.head_dim,
-            dtype=kv_dtype or dt, device=dev,
-        )
+        if kv_dtype == torch.float8_e4m3fn:
+            self.kv = Kv8Pool(cfg.num_kv_layers, num_pages, cfg.num_key_value_heads, cfg.head_dim, dev)
+        else:
+            self.kv = torch.zeros(
+                cfg.num_kv_layers, num_pages, 2, cfg.num_key_value_heads, PAGE_SIZE, cfg.head_dim,
+                dtype=kv_dtype or dt, device=dev,
+            )
         n_gdn = len(cfg.gdn_layers)
         self.conv_state = torch.zeros(
             n_gdn, state_slots, cfg.gdn_conv_dim, cfg.linear_conv_kernel_dim - 1, dtype=dt, device=dev
@@ -149,7 +154,34 @@ class Model:
         self.rec_state[:, dst].copy_(self.rec_state[:, src])
 
     def copy_page(self, src: int, dst: int) -> None:
+        if isinstance(self.kv, Kv8Pool):
+            self.kv.copy_page(src, dst)
+            return
         self.kv[:, dst].copy_(self.kv[:, src])
+
+    @property
+    def page_bytes(self) -> int:
+        """Bytes of one page over all layers."""
+        return self.kv.page_bytes if isinstance(self.kv, Kv8Pool) else self.kv[:, 0].numel() * self.kv.element_size()
+
+    def read_kv(self, layer: int, table: torch.Tensor, length: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """Keys and values ``[length, n_kv, D]`` of a sequence in KV layer ``layer`` from its page table ``[pages]``: what another
+        replica takes over with ``write_kv``, whatever the type of either's pool."""
+        pos = torch.arange(length, device=self.device)
+        kv = self.kv[layer]
+        if isinstance(kv, Kv8Layer):
+            return self.ops.kv8_read(kv, pos, torch.zeros_like(pos, dtype=torch.int32), table[None, :])
+        page, at = table[pos // PAGE_SIZE].long(), pos % PAGE_SIZE
+        return kv[page, 0, :, at], kv[page, 1, :, at]
+
+    def write_kv(self, layer: int, table: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pos0: int = 0) -> None:
+        """Rows ``[n, n_kv, D]`` of keys and values into the pages of a sequence, from position ``pos0`` on."""
+        pos = torch.arange(pos0, pos0 + k.shape[0], device=self.device)
+        kv = self.kv[layer]
+        if isinstance(kv, Kv8Layer):
+            self.ops.kv8_write(kv, k, v, pos, torch.zeros_like(pos, dtype=torch.int32), table[None, :])
+        else:
+            torch_ops.kv_write(kv, k.to(kv.dtype), v.to(kv.dtype), table[pos // PAGE_SIZE].long(), pos % PAGE_SIZE)
 
     def new_ring(self, B: int, G: int):
         """Per-layer state-after-row buffers of one verify pass."""
@@ -200,14 +232,27 @@ class Model:
             batch.tables = spans.span_tables(batch.seg_starts, batch.seg_slots, batch.seg_pos0, tile_rows, self.device)
         return {"meta": getattr(batch.tables, kind)}
 
+    def _attention_spans(self, batch: PackedBatch) -> dict:
+        """The arguments of ``ops.attention`` that describe a ragged pass: the spans' lists, and their device tables. Over the 8-bit pool those
+        are the spans' first rows and positions, which the other kernels' tables hold; a captured pass has no lists."""
+        meta = self._span_meta(batch, "flash")
+        if not isinstance(self.kv, Kv8Pool):
+            return {"seg_starts": batch.seg_starts, "seg_pos0": batch.seg_pos0, **meta}
+        if not meta:
+            return {"seg_starts": batch.seg_starts, "seg_pos0": batch.seg_pos0}
+        tables = batch.meta or batch.tables
+        meta = {"meta": (tables.gdn[5], tables.flash[3])} if tables.flash is not None else {}
+        if batch.meta is not None:
+            return {"seg_starts": None, "seg_pos0": None, **meta}
+        return {"seg_starts": batch.seg_starts, "seg_pos0": batch.seg_pos0, **meta}
+
     def _attention(self, lw, kv_layer, h, batch: PackedBatch) -> torch.Tensor:
         cfg, ops = self.cfg, self.ops
         qkv = ops.linear(h, lw.in_proj)
         core = ops.attention(
             qkv, batch.positions, batch.seq_of_row, batch.block_tables, kv_layer, lw.q_norm, lw.k_norm,
             cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim, cfg.rotary_dim, cfg.rope_theta,
-            cfg.rms_norm_eps, batch.G, batch.seg_starts, batch.seg_pos0,
-            **self._span_meta(batch, "flash"),
+            cfg.rms_norm_eps, batch.G, **self._attention_spans(batch),
         )
         return self._out_proj(core, lw.out_proj)
 
@@ -320,7 +365,7 @@ class Model:
                 core = ops.attention(mixed[:T], batch.positions, batch.seq_of_row, batch.block_tables,
                                      self.kv[self._kv_index[i]], lw.q_norm, lw.k_norm, cfg.num_attention_heads,
                                      cfg.num_key_value_heads, cfg.head_dim, cfg.rotary_dim, cfg.rope_theta, eps, 0,
-                                     batch.seg_starts, batch.seg_pos0, **self._span_meta(batch, "flash"))
+                                     **self._attention_spans(batch))
             sp.gemm_reduce_scatter(pad(core), lw.out_proj)
             res, full = sp.reduce_norm_allgather(rpr, res, lw.post_norm, eps)
             logits = sp.gemm_gathered(full, lw.router, out_dtype=torch.float32)

@@ -13,7 +13,7 @@
 //                (reference: engine/fast/fused.py:530-551).
 //
 // KV layout: kv[page][2][n_kv][PAGE][D] bf16; page tables int32 [B, max_pages]; page 0 is scratch.
-#include "common.cuh"
+#include "kv8.cuh"
 
 namespace b200 {
 
@@ -66,11 +66,12 @@ __device__ __forceinline__ void copy_bf16_vec(bf16* dst, const bf16* src) {
 // are on their way: a power and a sine per head and frequency bounded the kernel before (121 us at 8192 rows of 20
 // heads, 302 MB; 94 us now, 23 instead of 30 us at 2048). A lane owns D / 32 consecutive dims, one vector load / store per tensor.
 constexpr int PREP_WARPS = 20;
-template <int D>
+// KV8: keys and values go into the 8-bit cache (`kv` its data, `exps` its powers of two), rounded to bf16 first as for the other.
+template <int D, bool KV8>
 __global__ void __launch_bounds__(32 * PREP_WARPS)
 attn_prep_kernel(const bf16* qkv, int ld, const int64_t* positions, const int* tables, int max_pages,
                  const int* seq_of_row, const bf16* q_norm, const bf16* k_norm, bf16* q_out,
-                 bf16* gate_out, bf16* kv, int n_q, int n_kv, int rot, float theta, float eps,
+                 bf16* gate_out, void* kv, uint8_t* exps, int n_q, int n_kv, int rot, float theta, float eps,
                  int num_pages, int* err) {
   constexpr int PER = D / 32;
   __shared__ float s_cos[D / 2], s_sin[D / 2];
@@ -134,8 +135,31 @@ attn_prep_kernel(const bf16* qkv, int ld, const int64_t* positions, const int* t
       if (page < 0 || page >= num_pages) { if (lane == 0) atomicCAS(err, 0, ERR_BAD_INDEX); continue; }
       const int which = head < n_q + n_kv ? 0 : 1;
       const int kh = which ? head - n_q - n_kv : head - n_q;
-      bf16* dst = kv + ((((static_cast<size_t>(page) * 2 + which) * n_kv + kh) * PAGE) + pos % PAGE) * D;
-      store_bf16_vec<PER>(dst + d0, v);
+      const size_t at = ((static_cast<size_t>(page) * 2 + which) * n_kv + kh) * PAGE + pos % PAGE;
+      if constexpr (KV8) {
+        float amax = 0.f;
+        bool nan = false;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          v[i] = __bfloat162float(__float2bfloat16(v[i]));
+          amax = fmaxf(amax, fabsf(v[i]));
+          nan |= v[i] != v[i];
+        }
+        nan = __any_sync(0xffffffffu, nan);
+        const int e = kv8_exponent(warp_max(amax));
+        const float f = nan ? 0.f : kv8_two_to(-e);
+        uint8_t* dst = static_cast<uint8_t*>(kv) + at * D + d0;
+        if constexpr (PER == 1) {
+          dst[0] = static_cast<uint8_t>(nan ? 0u : kv8_pack2(v[0] * f, 0.f));
+        } else {
+#pragma unroll
+          for (int i = 0; i < PER; i += 2)
+            *reinterpret_cast<uint16_t*>(dst + i) = static_cast<uint16_t>(nan ? 0u : kv8_pack2(v[i] * f, v[i + 1] * f));
+        }
+        if (lane == 0) exps[at] = static_cast<uint8_t>(nan ? KV8_E_NAN : e + 127);
+      } else {
+        store_bf16_vec<PER>(static_cast<bf16*>(kv) + at * D + d0, v);
+      }
     }
   }
 }
@@ -406,18 +430,19 @@ static cudaError_t launch_combine(const float* part_acc, const float* part_ml, c
 
 using namespace b200;
 
-extern "C" int b200_attn_prep(const void* qkv, int ld, const int64_t* positions, const int* tables, int max_pages,
-                              const int* seq_of_row, const void* q_norm, const void* k_norm, void* q_out, void* gate_out,
-                              void* kv, int rows, int n_q, int n_kv, int D, int rot, float theta, float eps,
-                              int num_pages, int* err, cudaStream_t st) {
+namespace {
+template <bool KV8>
+int prep(const void* qkv, int ld, const int64_t* positions, const int* tables, int max_pages, const int* seq_of_row, const void* q_norm,
+         const void* k_norm, void* q_out, void* gate_out, void* kv, void* exps, int rows, int n_q, int n_kv, int D, int rot, float theta,
+         float eps, int num_pages, int* err, cudaStream_t st) {
   if (rows <= 0) return 0;
   if (rot > D) return -7;
   const int heads = n_q + 2 * n_kv;
   const dim3 grid(rows), block(32 * (heads < PREP_WARPS ? heads : PREP_WARPS));
-#define PREP(DD)                                                                                                      \
-  launch_pdl(attn_prep_kernel<DD>, grid, block, 0, st, static_cast<const bf16*>(qkv), ld, positions, tables,    \
-             max_pages, seq_of_row, static_cast<const bf16*>(q_norm), static_cast<const bf16*>(k_norm),              \
-             static_cast<bf16*>(q_out), static_cast<bf16*>(gate_out), static_cast<bf16*>(kv), n_q, n_kv, rot, theta, \
+#define PREP(DD)                                                                                                            \
+  launch_pdl(attn_prep_kernel<DD, KV8>, grid, block, 0, st, static_cast<const bf16*>(qkv), ld, positions, tables,           \
+             max_pages, seq_of_row, static_cast<const bf16*>(q_norm), static_cast<const bf16*>(k_norm),                    \
+             static_cast<bf16*>(q_out), static_cast<bf16*>(gate_out), kv, static_cast<uint8_t*>(exps), n_q, n_kv, rot, theta, \
              eps, num_pages, err)
   if (D == 256) PREP(256);
   else if (D == 128) PREP(128);
@@ -426,6 +451,24 @@ extern "C" int b200_attn_prep(const void* qkv, int ld, const int64_t* positions,
   else return -7;
 #undef PREP
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
+}
+}  // namespace
+
+extern "C" int b200_attn_prep(const void* qkv, int ld, const int64_t* positions, const int* tables, int max_pages,
+                              const int* seq_of_row, const void* q_norm, const void* k_norm, void* q_out, void* gate_out,
+                              void* kv, int rows, int n_q, int n_kv, int D, int rot, float theta, float eps,
+                              int num_pages, int* err, cudaStream_t st) {
+  return prep<false>(qkv, ld, positions, tables, max_pages, seq_of_row, q_norm, k_norm, q_out, gate_out, kv, nullptr, rows, n_q, n_kv, D, rot,
+                     theta, eps, num_pages, err, st);
+}
+
+// The same into one layer of the 8-bit cache: data, exps.
+extern "C" int b200_attn_prep_kv8(const void* qkv, int ld, const int64_t* positions, const int* tables, int max_pages,
+                                  const int* seq_of_row, const void* q_norm, const void* k_norm, void* q_out, void* gate_out,
+                                  void* data, void* exps, int rows, int n_q, int n_kv, int D, int rot, float theta, float eps,
+                                  int num_pages, int* err, cudaStream_t st) {
+  return prep<true>(qkv, ld, positions, tables, max_pages, seq_of_row, q_norm, k_norm, q_out, gate_out, data, exps, rows, n_q, n_kv, D, rot,
+                    theta, eps, num_pages, err, st);
 }
 
 extern "C" int b200_paged_attn(const void* q, const void* gate, const void* kv, const int* tables, int max_pages,

@@ -78,6 +78,7 @@ class _Sig:
     b200_gdn_decode = [P, I, P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, P, P]
     b200_gdn_decode_behind_projection = b200_gdn_decode
     b200_attn_prep = [P, I, P, P, I, P, P, P, P, P, P, I, I, I, I, I, F, F, I, P, P]
+    b200_attn_prep_kv8 = [P, I, P, P, I, P, P, P, P, P, P, P, I, I, I, I, I, F, F, I, P, P]
     b200_paged_attn = [P, P, P, P, I, P, P, P, P, I, I, I, I, I, I, I, P]
     b200_gdn_prefill = [P, I, P, P, P, P, P, P, P, P, P, P, P, I, P, I, P, P, P, I, I, I, I, I, F, I, P, P]
     b200_gdn_prefill_work_stride = [I]
@@ -624,9 +625,15 @@ def attention(qkv, positions, seq_of_row, block_tables, kv_layer, q_norm, k_norm
     ``G > 0``: every sequence has exactly ``G`` rows (decode ``G = 1``, verify ``G = k + 1``) and the
     flash-decoding kernel runs. ``G = 0``: ragged prefill spans; the page gather + softmax
     runs in PyTorch per sequence after the fused prep kernel.
+
+    ``kv_layer`` may be a ``Kv8Layer``: keys and values are then quantised as they are written, and ``kv8_decode`` or ``kv8_prefill``
+    (``meta``: its device tensors) reads them.
     """
     rows = qkv.shape[0]
     dev = qkv.device
+    if isinstance(kv_layer, Kv8Layer):
+        return _kv8_attention(qkv, positions, seq_of_row, block_tables, kv_layer, q_norm, k_norm, n_q, n_kv, head_dim, rotary_dim,
+                              theta, eps, G, seg_starts, seg_pos0, meta)
     q = torch.empty(rows, n_q, head_dim, dtype=qkv.dtype, device=dev)
     gate = torch.empty(rows, n_q * head_dim, dtype=qkv.dtype, device=dev)
     num_pages = kv_layer.shape[0]
@@ -887,6 +894,25 @@ def kv8_prefill(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tabl
         block_tables.data_ptr(), block_tables.stride(0), width, pages, n_q, n_kv, D, splits, _ptr(part_acc), _ptr(part_ml),
         out.data_ptr(), _ptr(err_word(dev)), _stream()), "kv8_prefill")
     return out
+
+
+def _kv8_attention(qkv, positions, seq_of_row, block_tables, layer, q_norm, k_norm, n_q, n_kv, head_dim, rotary_dim, theta, eps, G,
+                   seg_starts, seg_pos0, meta) -> torch.Tensor:
+    """``attention`` over a layer of the 8-bit cache. Head dims without a kernel take the PyTorch operators, as the bf16 prefill does."""
+    if head_dim not in KV8_HEAD_DIMS or not 1 <= n_q // n_kv <= 16:
+        return torch_ops.attention(qkv, positions, seq_of_row, block_tables, layer, q_norm, k_norm, n_q, n_kv, head_dim, rotary_dim,
+                                   theta, eps, G, seg_starts, seg_pos0)
+    pages, _, _ = check_layer(layer, "attention")
+    rows, dev = qkv.shape[0], qkv.device
+    q = torch.empty(rows, n_q, head_dim, dtype=qkv.dtype, device=dev)
+    gate = torch.empty(rows, n_q * head_dim, dtype=qkv.dtype, device=dev)
+    _check(lib().b200_attn_prep_kv8(
+        _ptr(qkv), qkv.stride(0), _ptr(positions), _ptr(block_tables), block_tables.stride(0), _ptr(seq_of_row),
+        _ptr(q_norm), _ptr(k_norm), _ptr(q), _ptr(gate), _ptr(layer.data), _ptr(layer.exps), rows, n_q, n_kv, head_dim, rotary_dim,
+        theta, eps, pages, _ptr(err_word(dev)), _stream()), "attn_prep_kv8")
+    if G == 0:
+        return kv8_prefill(q, gate, layer, block_tables, seg_starts, seg_pos0, meta=meta)
+    return kv8_decode(q, gate, layer, block_tables, positions, G)
 
 
 def argmax_rows(logits: torch.Tensor) -> torch.Tensor:

@@ -172,34 +172,37 @@ def kv8_read(layer: Kv8Layer, positions: torch.Tensor, seq_of_row: torch.Tensor,
                             layer.exps[page, which, :, at], dtype) for which in (0, 1))
 
 
-def _kv8_attention(q, gate, layer: Kv8Layer, tables, positions) -> torch.Tensor:
-    """One row after the other: row ``t`` sees the keys ``0 .. positions[t]`` of the pages ``tables[t]``."""
+def _kv8_attention(q, gate, layer: Kv8Layer, block_tables, seg_starts, positions) -> torch.Tensor:
+    """Sequence ``i`` owns rows ``seg_starts[i]:seg_starts[i + 1]``; a row sees the keys ``0 .. positions[row]`` (none: its output is 0)."""
     T, n_q, D = q.shape
     n_kv = layer.data.shape[2]
     out = torch.zeros(T, n_q, D, dtype=q.dtype, device=q.device)
-    for t, pos in enumerate(positions.tolist()):
-        if pos < 0:
+    for i, (a, b) in enumerate(zip(seg_starts, seg_starts[1:])):
+        pos = positions[a:b].long()
+        total = int(pos.max()) + 1 if b > a else 0
+        if total <= 0:
             continue
-        at = torch.arange(pos + 1, device=q.device)
-        k, v = (x.transpose(0, 1) for x in kv8_read(layer, at, torch.zeros_like(at), tables[t : t + 1], torch.float32))
-        s = (q[t].float().view(n_kv, n_q // n_kv, D) @ k.transpose(1, 2)) * D ** -0.5
-        out[t] = (torch.softmax(s, dim=-1) @ v).reshape(n_q, D).to(q.dtype)
+        at = torch.arange(total, device=q.device)
+        k, v = (x.transpose(0, 1).repeat_interleave(n_q // n_kv, dim=0)
+                for x in kv8_read(layer, at, torch.zeros_like(at), block_tables[i : i + 1], torch.float32))  # [n_q, total, D]
+        s = (q[a:b].transpose(0, 1).float() @ k.transpose(1, 2)) * D ** -0.5
+        s = s.masked_fill(at[None, :] > pos[:, None], float("-inf"))
+        o = (torch.softmax(s, dim=-1) @ v).transpose(0, 1)
+        out[a:b] = torch.where(pos[:, None, None] >= 0, o, torch.zeros_like(o)).to(q.dtype)
     return out.reshape(T, n_q * D) * torch.sigmoid(gate)
 
 
 def kv8_decode(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tables: torch.Tensor, positions: torch.Tensor,
                G: int) -> torch.Tensor:
     """Gated attention of ``G`` rows per sequence over the 8-bit cache (see ``cuda_ops.kv8_decode``)."""
-    return _kv8_attention(q, gate, layer, block_tables.repeat_interleave(G, dim=0), positions)
+    return _kv8_attention(q, gate, layer, block_tables, list(range(0, q.shape[0] + 1, G)), positions)
 
 
 def kv8_prefill(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tables: torch.Tensor, seg_starts: list[int],
                 seg_pos0: list[int], meta=None) -> torch.Tensor:
     """Causal gated attention of ragged spans over the 8-bit cache (see ``cuda_ops.kv8_prefill``)."""
-    spans = list(zip(seg_starts, seg_starts[1:], seg_pos0))
-    seq = torch.cat([torch.full((b - a,), i) for i, (a, b, _) in enumerate(spans)]).to(q.device)
-    positions = torch.cat([torch.arange(p, p + b - a) for a, b, p in spans]).to(q.device)
-    return _kv8_attention(q, gate, layer, block_tables[seq], positions)
+    positions = torch.cat([torch.arange(p, p + b - a) for a, b, p in zip(seg_starts, seg_starts[1:], seg_pos0)]).to(q.device)
+    return _kv8_attention(q, gate, layer, block_tables, seg_starts, positions)
 
 
 # --------------------------------------------------------------------------- MoE
@@ -549,6 +552,11 @@ def attention(qkv, positions, seq_of_row, block_tables, kv_layer, q_norm, k_norm
               theta, eps, G: int, seg_starts=None, seg_pos0=None) -> torch.Tensor:
     """q/k norm, RoPE, KV page write and causal gated attention over the paged cache (see ``cuda_ops.attention``)."""
     q, gate, k, v = attn_prep(qkv, positions, q_norm, k_norm, n_q, n_kv, head_dim, rotary_dim, theta, eps)
+    if isinstance(kv_layer, Kv8Layer):
+        kv8_write(kv_layer, k, v, positions, seq_of_row, block_tables)
+        if G > 0:
+            return kv8_decode(q, gate, kv_layer, block_tables, positions, G)
+        return kv8_prefill(q, gate, kv_layer, block_tables, seg_starts, seg_pos0)
     page_ids = block_tables[seq_of_row.long(), positions // PAGE_SIZE].long()
     kv_write(kv_layer, k, v, page_ids, positions % PAGE_SIZE)
     if G > 0:

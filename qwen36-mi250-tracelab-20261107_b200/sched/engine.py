@@ -29,9 +29,13 @@ from ..config import PAGE_SIZE, EngineConfig, ModelConfig
 from ..models.checkpoint import Weights
 from ..models.qwen36 import Model, PackedBatch
 from ..ops import torch_ops
+from ..ops.kv8 import Kv8Pool
 from ..obs import looptimers
 from .request import EngineError, Generation, Sampling, TokenEvent
 from .sampling import pick_tokens
+
+
+KV_DTYPES = {"auto": None, "e4m3": torch.float8_e4m3fn}  # of EngineConfig.kv_dtype
 
 
 def _select_ops(device: torch.device):
@@ -64,6 +68,8 @@ class Engine:
         self.device = weights.device
         self.ops = ops or _select_ops(self.device)
         c = self.cfg
+        if c.kv_dtype not in KV_DTYPES:
+            raise ValueError(f"kv_dtype {c.kv_dtype!r} is none of {', '.join(KV_DTYPES)}")
         self.chunk = max(PAGE_SIZE, (c.prefill_chunk_tokens + PAGE_SIZE - 1) // PAGE_SIZE * PAGE_SIZE)
         self.max_model_len = c.max_model_len
         self.max_pages_per_seq = (self.max_model_len + PAGE_SIZE - 1) // PAGE_SIZE + 1
@@ -79,11 +85,11 @@ class Engine:
             self.ops.pack_weights(weights)  # before the KV pool is sized: padded copies replace a few tensors
         n_slots = c.state_slots or (c.max_seqs * 2 + 2)
         n_pages = c.kv_pages or self._agree_min(self._auto_pages(weights, n_slots), tp if tp is not None else pp)
-        self.model = Model(weights, n_pages, n_slots, ops=self.ops, tp=tp, ep=ep, pp=pp)
+        self.model = Model(weights, n_pages, n_slots, ops=self.ops, tp=tp, ep=ep, pp=pp, kv_dtype=KV_DTYPES[c.kv_dtype])
         self.model.draft_index = draft_index
         self.pages = PagePool(n_pages)
         self.slots = SlotPool(n_slots)
-        page_bytes = self.model.kv[:, 0].numel() * self.model.kv.element_size()
+        page_bytes = self.model.page_bytes
         slot_bytes = self.mcfg.gdn_state_bytes()
         self.cache = PrefixCache(
             self.pages, self.slots, page_bytes, slot_bytes, c.prefix_cache_entries, c.prefix_cache_tokens,
@@ -136,7 +142,10 @@ class Engine:
     # ------------------------------------------------------------------ sizing
     def _auto_pages(self, weights: Weights, n_slots: int) -> int:
         c, m = self.cfg, self.mcfg
-        per_page = m.kv_bytes_per_token(2 if weights.dtype != torch.float32 else 4) * PAGE_SIZE
+        if KV_DTYPES[c.kv_dtype] is not None:
+            per_page = Kv8Pool.page_bytes_of(m.num_kv_layers, m.num_key_value_heads, m.head_dim)
+        else:
+            per_page = m.kv_bytes_per_token(2 if weights.dtype != torch.float32 else 4) * PAGE_SIZE
         if self.device.type != "cuda":
             return min(4096, c.max_seqs * (min(self.max_model_len, 8192) // PAGE_SIZE + 2) + 64)
         free, _total = torch.cuda.mem_get_info(self.device)

@@ -479,3 +479,104 @@ def test_arguments_that_do_not_fit_are_refused(C):
     assert C.kv8_decode(q[:0], gate[:0], layer, tables, pos[:0], 1).shape == (0, n_q * D)
     assert C.kv8_prefill(q[:0], gate[:0], layer, tables, [0, 0], [0]).shape == (0, n_q * D)
     C.check_errors(q.device)
+
+
+# ------------------------------------------------------------------ in the model and the engine
+@pytest.mark.parametrize("n_q,n_kv,D,G", [(16, 2, 256, 1), (16, 2, 256, 4), (4, 1, 64, 2), (16, 2, 256, 0), (6, 3, 128, 0), (4, 1, 32, 1), (4, 1, 32, 0)])
+def test_attention_writes_what_the_quantiser_makes_of_the_bf16_rows(C, n_q, n_kv, D, G):
+    """The block over the 8-bit pool against the block over the bf16 pool: the same rows, quantised; and its output against the formula."""
+    from b200serve.ops import torch_ops as O
+
+    B, rot = 3, D // 4
+    per = [G] * B if G else [70, 1, 130]
+    pos0 = [5, 64, 300]
+    starts = [0]
+    for n in per:
+        starts.append(starts[-1] + n)
+    T = starts[-1]
+    g = _gen(D + G)
+    layer = _layer(30, n_kv, D, seed=2)
+    kv = torch.zeros(30, 2, n_kv, 64, D, dtype=torch.bfloat16, device=DEV)
+    tables = _tables([a + b for a, b in zip(per, pos0)], 8, 30)
+    tables[tables > 29] = 0  # the fallback for other head dims gathers whole tables
+    qkv = torch.randn(T, n_q * 2 * D + 2 * n_kv * D, device=DEV, generator=g).bfloat16()
+    positions = torch.cat([torch.arange(p, p + n) for p, n in zip(pos0, per)]).to(DEV)
+    seq = torch.cat([torch.full((n,), i) for i, n in enumerate(per)]).int().to(DEV)
+    qn, kn = ((torch.randn(D, device=DEV, generator=g) * 0.1).bfloat16() for _ in range(2))
+    args = (qn, kn, n_q, n_kv, D, rot, 1e7, 1e-6, G, starts, pos0)
+    before = Kv8Layer(layer.data.clone(), layer.exps.clone())
+    got = C.attention(qkv, positions, seq, tables, layer, *args)
+    C.check_errors(qkv.device)
+    if D != 32:
+        C.attention(qkv, positions, seq, tables, kv, *args)
+        page, at = tables[seq.long(), positions // 64].long(), positions % 64
+        for i in (0, 1):
+            data, exps = quantise(kv[page, i, :, at])
+            before.data.view(torch.uint8)[page, i, :, at] = data.view(torch.uint8)
+            before.exps[page, i, :, at] = exps
+        assert torch.equal(layer.data.view(torch.uint8), before.data.view(torch.uint8)) and torch.equal(layer.exps, before.exps)
+    q, gate, _, _ = O.attn_prep(qkv.float(), positions, qn.float(), kn.float(), n_q, n_kv, D, rot, 1e7, 1e-6)
+    want, tol = _attention(q, gate, layer, tables[seq.long()], positions)
+    # beyond what the operators may be off by: q, rounded to bf16 where the reference's is not (its norm in fp32 and its rotation: 3 roundings of
+    # 2^-9 each in a score of up to a few times sqrt D), moves weights by 2^-7 of their parts
+    kv32 = dequantise(layer.data, layer.exps, torch.float32)
+    assert ((got.double() - want).abs() <= tol + 0.05 * kv32.abs().max()).all()
+    assert torch.nn.functional.cosine_similarity(got.double(), want, dim=-1).min() > 0.999
+
+
+def test_captured_prefill_takes_device_tables_alone(C):
+    n_q, n_kv, D = 16, 2, 256
+    layer = _layer(30, n_kv, D)
+    lens, pos0 = [40, 0, 70], [100, 0, 200]
+    tables = _tables([a + b for a, b in zip(lens, pos0)], 8, 30)
+    starts = [0, 40, 40, 110]
+    q, gate = _rows(110, n_q, D, 1)
+    meta = tuple(torch.tensor(x, dtype=torch.int32, device=DEV) for x in (starts, pos0))
+    graph = torch.cuda.CUDAGraph()
+    C.kv8_prefill(q, gate, layer, tables, None, None, meta=meta)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out = C.kv8_prefill(q, gate, layer, tables, None, None, meta=meta)
+    graph.replay()
+    C.check_errors(q.device)
+    seq = torch.tensor([0] * 40 + [2] * 70, device=DEV)
+    pos = torch.cat([torch.arange(p, p + n) for n, p in zip(lens, pos0)]).to(DEV)
+    _check(out, _attention(q, gate, layer, tables[seq], pos))
+    meta[1].copy_(torch.tensor([20, 0, 150], dtype=torch.int32))  # other positions in the same tables
+    graph.replay()
+    C.check_errors(q.device)
+    pos = torch.cat([torch.arange(p, p + n) for n, p in zip(lens, [20, 0, 150])]).to(DEV)
+    _check(out, _attention(q, gate, layer, tables[seq], pos))
+    with pytest.raises(ValueError, match="kv8_prefill"):
+        C.kv8_prefill(q, gate, layer, tables, None, None)
+
+
+def test_engine_with_the_8_bit_pool(C):
+    """Greedy tokens are the same alone, in a batch, with and without graphs, and with draft chains verified."""
+    from b200serve.config import EngineConfig, ModelConfig
+    from b200serve.models.checkpoint import random_weights
+    from b200serve.ops.kv8 import Kv8Pool
+    from b200serve.sched.engine import Engine
+    from b200serve.sched.request import Sampling
+
+    cfg = ModelConfig.tiny(head_dim=64, num_attention_heads=4, num_key_value_heads=1)
+    w = random_weights(cfg, seed=0, device=DEV, dtype=torch.bfloat16, std=0.05, lm_head_std=0.5)
+    g = torch.Generator().manual_seed(3)
+    prompts = [torch.randint(3, 1024, (int(n),), generator=g).tolist() for n in (17, 190, 64, 600, 130)]
+    s = Sampling(max_tokens=24, ignore_eos=True)
+
+    def run(prompts, **kw):
+        ecfg = EngineConfig(max_model_len=1024, prefill_chunk_tokens=64, max_seqs=8, kv_pages=256, decode_buckets=(1, 4, 8), kv_dtype="e4m3", **kw)
+        eng = Engine(w, ecfg)
+        return eng, [x.output for x in eng.generate(prompts, s)]
+
+    eng, batched = run(prompts, mtp=False)
+    assert isinstance(eng.model.kv, Kv8Pool) and eng._graphs is not None and not eng._graphs.errors
+    for p, want in zip(prompts[:3], batched):
+        assert run([p], mtp=False)[1] == [want]
+    assert run(prompts, mtp=False, cuda_graphs=False)[1] == batched
+    spec, out = run(prompts, mtp=True, spec_k=2)
+    assert out == batched and spec.stats["mtp_verify_steps"] > 0
+    graphs, out = run(prompts[:1], mtp=False, prefill_graphs=True)
+    assert out == batched[:1]
+    C.check_errors(torch.device(DEV))
