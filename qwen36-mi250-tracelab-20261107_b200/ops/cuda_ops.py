@@ -739,22 +739,31 @@ def flash_decode(q: torch.Tensor, gate: torch.Tensor, kv_layer: torch.Tensor, bl
 
 
 # --------------------------------------------------------------------------- the 8-bit KV cache
+# The smallest of these calls take a few microseconds on the GPU, less than their way there: each attribute of a tensor is asked for
+# once, and the stream by its number (current_stream() builds an object, 3 us).
+def _raw_stream(dev: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
 def _index_tables(what: str, dev: torch.device, rows: int, positions: torch.Tensor, block_tables: torch.Tensor,
                   seq_of_row: torch.Tensor | None = None):
-    """The row indices in the types that the kernels read: int64 positions, int32 tables and sequences."""
-    if positions.shape != (rows,) or block_tables.dim() != 2 or (seq_of_row is not None and seq_of_row.shape != (rows,)):
-        raise ValueError(f"{what}: {rows} rows, but positions {tuple(positions.shape)}, page tables {tuple(block_tables.shape)}"
+    """The row indices in the types that the kernels read (int64 positions, int32 tables and sequences), the tables' shape and row distance."""
+    shape = block_tables.shape
+    if positions.shape != (rows,) or len(shape) != 2 or (seq_of_row is not None and seq_of_row.shape != (rows,)):
+        raise ValueError(f"{what}: {rows} rows, but positions {tuple(positions.shape)}, page tables {tuple(shape)}"
                          + ("" if seq_of_row is None else f", sequences {tuple(seq_of_row.shape)}"))
-    for t in (positions, block_tables, seq_of_row):
-        if t is not None and t.device != dev:
-            raise ValueError(f"{what}: the cache is on {dev}, an index tensor on {t.device}")
+    if positions.device != dev or block_tables.device != dev or (seq_of_row is not None and seq_of_row.device != dev):
+        raise ValueError(f"{what}: the cache is on {dev}, positions on {positions.device}, page tables on {block_tables.device}"
+                         + ("" if seq_of_row is None else f", sequences on {seq_of_row.device}"))
     if positions.dtype != torch.int64 or not positions.is_contiguous():
         positions = positions.to(torch.int64).contiguous()
-    if block_tables.dtype != torch.int32 or block_tables.stride(1) != 1:
+    step, one = block_tables.stride()
+    if block_tables.dtype != torch.int32 or one != 1:
         block_tables = block_tables.to(torch.int32).contiguous()
+        step = shape[1]
     if seq_of_row is not None and (seq_of_row.dtype != torch.int32 or not seq_of_row.is_contiguous()):
         seq_of_row = seq_of_row.to(torch.int32).contiguous()
-    return positions, block_tables, seq_of_row
+    return positions, block_tables, seq_of_row, step, shape[1], shape[0]
 
 
 def kv8_write(layer: Kv8Layer, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, seq_of_row: torch.Tensor,
@@ -762,33 +771,37 @@ def kv8_write(layer: Kv8Layer, k: torch.Tensor, v: torch.Tensor, positions: torc
     """Quantise rows ``k, v [T, n_kv, D]`` (bf16, rows and heads at any stride) into the pages of their sequences: row ``t`` is the
     token at ``positions[t]`` of sequence ``seq_of_row[t]`` (``ops/kv8.py`` has the format)."""
     pages, n_kv, D = check_layer(layer, "kv8_write")
-    T, dev = k.shape[0], layer.data.device
-    if k.shape != (T, n_kv, D) or v.shape != (T, n_kv, D) or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
-        raise ValueError(f"kv8_write: k {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} are not bf16 [{T}, {n_kv}, {D}]")
+    data, exps = layer
+    dev, shape = data.device, k.shape
+    T = shape[0] if len(shape) else 0
+    if shape != (T, n_kv, D) or v.shape != shape or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
+        raise ValueError(f"kv8_write: k {tuple(shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} are not bf16 [{T}, {n_kv}, {D}]")
     if k.device != dev or v.device != dev:
         raise ValueError(f"kv8_write: the cache is on {dev}, the rows on {k.device} and {v.device}")
-    positions, block_tables, seq_of_row = _index_tables("kv8_write", dev, T, positions, block_tables, seq_of_row)
-    if k.stride(2) != 1:
+    positions, block_tables, seq_of_row, step, width, seqs = _index_tables("kv8_write", dev, T, positions, block_tables, seq_of_row)
+    ks, vs = k.stride(), v.stride()
+    if ks[2] != 1:
         k = k.contiguous()
-    if v.stride(2) != 1:
+        ks = k.stride()
+    if vs[2] != 1:
         v = v.contiguous()
+        vs = v.stride()
     _check(lib().b200_kv8_write(
-        k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), positions.data_ptr(), seq_of_row.data_ptr(),
-        block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1], block_tables.shape[0], layer.data.data_ptr(),
-        layer.exps.data_ptr(), T, n_kv, D, pages, _ptr(err_word(dev)), _stream()), "kv8_write")
+        k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], positions.data_ptr(), seq_of_row.data_ptr(), block_tables.data_ptr(),
+        step, width, seqs, data.data_ptr(), exps.data_ptr(), T, n_kv, D, pages, err_word(dev).data_ptr(), _raw_stream(dev)), "kv8_write")
 
 
 def kv8_read(layer: Kv8Layer, positions: torch.Tensor, seq_of_row: torch.Tensor, block_tables: torch.Tensor):
     """``k, v [T, n_kv, D]`` (bf16, exactly what the cache stands for) of the tokens at ``positions[t]`` of sequences ``seq_of_row[t]``."""
     pages, n_kv, D = check_layer(layer, "kv8_read")
-    T, dev = positions.shape[0], layer.data.device
-    positions, block_tables, seq_of_row = _index_tables("kv8_read", dev, T, positions, block_tables, seq_of_row)
+    data, exps = layer
+    dev, T = data.device, positions.numel()
+    positions, block_tables, seq_of_row, step, width, seqs = _index_tables("kv8_read", dev, T, positions, block_tables, seq_of_row)
     k = torch.empty(T, n_kv, D, dtype=torch.bfloat16, device=dev)
     v = torch.empty_like(k)
     _check(lib().b200_kv8_read(
-        layer.data.data_ptr(), layer.exps.data_ptr(), positions.data_ptr(), seq_of_row.data_ptr(), block_tables.data_ptr(),
-        block_tables.stride(0), block_tables.shape[1], block_tables.shape[0], k.data_ptr(), v.data_ptr(), T, n_kv, D, pages,
-        _ptr(err_word(dev)), _stream()), "kv8_read")
+        data.data_ptr(), exps.data_ptr(), positions.data_ptr(), seq_of_row.data_ptr(), block_tables.data_ptr(), step, width, seqs,
+        k.data_ptr(), v.data_ptr(), T, n_kv, D, pages, err_word(dev).data_ptr(), _raw_stream(dev)), "kv8_read")
     return k, v
 
 
@@ -797,17 +810,19 @@ KV8_CUT_TILES = 64  # (tiles of a span) * (KV heads) up to which kv8_prefill.cu 
 
 
 def _kv8_queries(what: str, q: torch.Tensor, gate: torch.Tensor, n_kv: int, D: int, dev: torch.device):
+    """Queries and gates, contiguous in 16-byte rows; their number and the query heads."""
     if D not in KV8_HEAD_DIMS:
         raise ValueError(f"{what}: head dim {D} is none of {KV8_HEAD_DIMS}")
-    if q.dim() != 3 or q.shape[2] != D or q.shape[1] % n_kv or not 1 <= q.shape[1] // n_kv <= 16 or q.dtype != torch.bfloat16:
-        raise ValueError(f"{what}: q {tuple(q.shape)} {q.dtype} is not bf16 [rows, n_q, {D}] with 1 to 16 query heads for each of {n_kv} KV heads")
-    if gate.shape != (q.shape[0], q.shape[1] * D) or gate.dtype != torch.bfloat16:
-        raise ValueError(f"{what}: gate {tuple(gate.shape)} {gate.dtype} is not bf16 {(q.shape[0], q.shape[1] * D)}")
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != D or shape[1] % n_kv or not 1 <= shape[1] // n_kv <= 16 or q.dtype != torch.bfloat16:
+        raise ValueError(f"{what}: q {tuple(shape)} {q.dtype} is not bf16 [rows, n_q, {D}] with 1 to 16 query heads for each of {n_kv} KV heads")
+    rows, n_q, _ = shape
+    if gate.shape != (rows, n_q * D) or gate.dtype != torch.bfloat16:
+        raise ValueError(f"{what}: gate {tuple(gate.shape)} {gate.dtype} is not bf16 {(rows, n_q * D)}")
     if q.device != dev or gate.device != dev:
         raise ValueError(f"{what}: the cache is on {dev}, q on {q.device}, the gate on {gate.device}")
-    q = q if q.is_contiguous() else q.contiguous()
-    gate = gate if gate.is_contiguous() else gate.contiguous()
-    return q if q.data_ptr() % 16 == 0 else q.clone(), gate if gate.data_ptr() % 16 == 0 else gate.clone()
+    q, gate = (t if t.is_contiguous() else t.contiguous() for t in (q, gate))
+    return q if q.data_ptr() % 16 == 0 else q.clone(), gate if gate.data_ptr() % 16 == 0 else gate.clone(), rows, n_q
 
 
 def kv8_decode(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tables: torch.Tensor, positions: torch.Tensor,
@@ -816,23 +831,23 @@ def kv8_decode(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_table
     keys ``0 .. positions[row]`` of its sequence. A row's bits depend on its own position, queries and keys only, not on the batch or ``G``. A negative
     position is a row without keys: its output is 0. Only device tensors are touched, so the call can be captured in a CUDA graph."""
     pages, n_kv, D = check_layer(layer, "kv8_decode")
-    dev = layer.data.device
-    q, gate = _kv8_queries("kv8_decode", q, gate, n_kv, D, dev)
-    rows, n_q, _ = q.shape
-    if G < 1 or rows % G or block_tables.shape[0] < rows // G:
-        raise ValueError(f"kv8_decode: {rows} rows are not {G} for each of at most {block_tables.shape[0]} sequences")
-    positions, block_tables, _ = _index_tables("kv8_decode", dev, rows, positions, block_tables)
+    data, exps = layer
+    dev = data.device
+    q, gate, rows, n_q = _kv8_queries("kv8_decode", q, gate, n_kv, D, dev)
+    positions, block_tables, _, step, width, seqs = _index_tables("kv8_decode", dev, rows, positions, block_tables)
+    if G < 1 or rows % G or seqs < rows // G:
+        raise ValueError(f"kv8_decode: {rows} rows are not {G} for each of at most {seqs} sequences")
     L = lib()
-    n_splits = max(1, -(-block_tables.shape[1] * PAGE_SIZE // L.b200_kv8_decode_run()))
-    part_acc = part_ml = None
-    if n_splits > 1:
-        part_acc = torch.empty(rows, n_q, n_splits, D, dtype=torch.float32, device=dev)
-        part_ml = torch.empty(rows, n_q, n_splits, 2, dtype=torch.float32, device=dev)
-    out = torch.empty(rows, n_q * D, dtype=q.dtype, device=dev)
+    n_splits = max(1, -(-width * PAGE_SIZE // L.b200_kv8_decode_run()))
+    acc = ml = None
+    if n_splits > 1:  # partials: sums, then maxima and sums of weights
+        part = torch.empty(rows * n_q * n_splits * (D + 2), dtype=torch.float32, device=dev)
+        acc = part.data_ptr()
+        ml = acc + rows * n_q * n_splits * D * 4
+    out = torch.empty_like(gate)
     _check(L.b200_kv8_decode(
-        q.data_ptr(), gate.data_ptr(), layer.data.data_ptr(), layer.exps.data_ptr(), positions.data_ptr(), block_tables.data_ptr(),
-        block_tables.stride(0), block_tables.shape[1], pages, rows // G, G, n_q, n_kv, D, n_splits, _ptr(part_acc), _ptr(part_ml),
-        out.data_ptr(), _ptr(err_word(dev)), _stream()), "kv8_decode")
+        q.data_ptr(), gate.data_ptr(), data.data_ptr(), exps.data_ptr(), positions.data_ptr(), block_tables.data_ptr(), step, width, pages,
+        rows // G, G, n_q, n_kv, D, n_splits, acc, ml, out.data_ptr(), err_word(dev).data_ptr(), _raw_stream(dev)), "kv8_decode")
     return out
 
 
@@ -845,28 +860,30 @@ def kv8_prefill(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tabl
     ``meta``: ``(seg_starts, seg_pos0)`` as int32 device tensors that the caller keeps, of the same numbers; without it every call uploads
     them. With ``meta`` the lists may be None, which lets the call be captured in a CUDA graph: no span is cut then."""
     pages, n_kv, D = check_layer(layer, "kv8_prefill")
-    dev = layer.data.device
-    q, gate = _kv8_queries("kv8_prefill", q, gate, n_kv, D, dev)
-    T, n_q, _ = q.shape
+    data, exps = layer
+    dev = data.device
+    q, gate, T, n_q = _kv8_queries("kv8_prefill", q, gate, n_kv, D, dev)
     L = lib()
     group = n_q // n_kv
     per = L.b200_kv8_prefill_positions(group)
     if block_tables.dim() != 2 or block_tables.device != dev:
         raise ValueError(f"kv8_prefill: page tables {tuple(block_tables.shape)} on {block_tables.device}, the cache on {dev}")
-    if block_tables.dtype != torch.int32 or block_tables.stride(1) != 1:
+    seqs, width = block_tables.shape
+    step, one = block_tables.stride()
+    if block_tables.dtype != torch.int32 or one != 1:
         block_tables = block_tables.to(torch.int32).contiguous()
-    width = block_tables.shape[1]
+        step = width
     splits = 1
     if seg_starts is not None:
         n_seg = len(seg_pos0)
         lens = [b - a for a, b in zip(seg_starts, seg_starts[1:])]
-        if len(lens) != n_seg or seg_starts[0] != 0 or seg_starts[-1] != T or block_tables.shape[0] < n_seg or min(lens, default=0) < 0:
-            raise ValueError(f"kv8_prefill: spans {seg_starts} with {n_seg} first positions do not make {T} rows of at most "
-                             f"{block_tables.shape[0]} sequences")
-        n_tiles = sum([(n + per - 1) // per for n in lens])
+        if len(lens) != n_seg or seg_starts[0] != 0 or seg_starts[-1] != T or seqs < n_seg or min(lens, default=0) < 0:
+            raise ValueError(f"kv8_prefill: spans {seg_starts} with {n_seg} first positions do not make {T} rows of at most {seqs} sequences")
+        n_tiles = 0
         for n, pos in zip(lens, seg_pos0):
             if pos < 0 or pos + n > width * PAGE_SIZE:
                 raise ValueError(f"kv8_prefill: rows at positions {pos} .. {pos + n - 1}, page tables of {width} pages")
+            n_tiles += (n + per - 1) // per
             if 0 < n * n_kv <= per * KV8_CUT_TILES:  # short enough to be cut
                 splits = max(splits, L.b200_kv8_prefill_runs(n, pos, width, group, n_kv))
     elif meta is None:
@@ -876,23 +893,24 @@ def kv8_prefill(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tabl
         n_tiles = T // per + n_seg
     if meta is not None:
         starts_t, pos0_t = meta
-        if (starts_t.dtype, pos0_t.dtype) != (torch.int32, torch.int32) or starts_t.numel() <= n_seg - (n_seg == 0) or pos0_t.numel() < n_seg \
+        if starts_t.dtype != torch.int32 or pos0_t.dtype != torch.int32 or starts_t.numel() < n_seg + 1 or pos0_t.numel() < n_seg \
                 or starts_t.device != dev or pos0_t.device != dev:
             raise ValueError(f"kv8_prefill: meta of {starts_t.numel()} and {pos0_t.numel()} numbers ({starts_t.dtype}, {starts_t.device}) for {n_seg} spans")
     elif T:
         both = torch.tensor([*seg_starts, *seg_pos0], dtype=torch.int32).to(dev)
         starts_t, pos0_t = both[: n_seg + 1], both[n_seg + 1 :]
-    out = torch.empty(T, n_q * D, dtype=q.dtype, device=dev)
+    out = torch.empty_like(gate)
     if T == 0:
         return out
-    part_acc = part_ml = None
-    if splits > 1:
-        part_acc = torch.empty(T, n_q, splits, D, dtype=torch.float32, device=dev)
-        part_ml = torch.empty(T, n_q, splits, 2, dtype=torch.float32, device=dev)
+    acc = ml = None
+    if splits > 1:  # partials: sums, then maxima and sums of weights
+        part = torch.empty(T * n_q * splits * (D + 2), dtype=torch.float32, device=dev)
+        acc = part.data_ptr()
+        ml = acc + T * n_q * splits * D * 4
     _check(L.b200_kv8_prefill(
-        q.data_ptr(), gate.data_ptr(), layer.data.data_ptr(), layer.exps.data_ptr(), starts_t.data_ptr(), pos0_t.data_ptr(), n_seg, n_tiles,
-        block_tables.data_ptr(), block_tables.stride(0), width, pages, n_q, n_kv, D, splits, _ptr(part_acc), _ptr(part_ml),
-        out.data_ptr(), _ptr(err_word(dev)), _stream()), "kv8_prefill")
+        q.data_ptr(), gate.data_ptr(), data.data_ptr(), exps.data_ptr(), starts_t.data_ptr(), pos0_t.data_ptr(), n_seg, n_tiles,
+        block_tables.data_ptr(), step, width, pages, n_q, n_kv, D, splits, acc, ml, out.data_ptr(), err_word(dev).data_ptr(),
+        _raw_stream(dev)), "kv8_prefill")
     return out
 
 

@@ -65,17 +65,18 @@ class Kv8Pool:
 def check_layer(layer: Kv8Layer, what: str) -> tuple[int, int, int]:
     """``(pages, n_kv, D)`` of a layer whose parts fit each other; ``ValueError`` otherwise."""
     data, exps = layer
+    shape = data.shape
     if data.dtype != torch.float8_e4m3fn or exps.dtype != torch.uint8:
         raise ValueError(f"{what}: an 8-bit KV layer holds float8_e4m3fn data and uint8 exponents, not {data.dtype} and {exps.dtype}")
-    if data.dim() != 5 or data.shape[1] != 2 or data.shape[3] != PAGE_SIZE or data.shape[:4] != exps.shape:
-        raise ValueError(f"{what}: data {tuple(data.shape)} and exponents {tuple(exps.shape)} are not [pages, 2, n_kv, {PAGE_SIZE}, D] and the same without D")
+    if len(shape) != 5 or shape[1] != 2 or shape[3] != PAGE_SIZE or shape[:4] != exps.shape:
+        raise ValueError(f"{what}: data {tuple(shape)} and exponents {tuple(exps.shape)} are not [pages, 2, n_kv, {PAGE_SIZE}, D] and the same without D")
     if not (data.is_contiguous() and exps.is_contiguous()):
         raise ValueError(f"{what}: the parts of an 8-bit KV layer are contiguous")
     if data.device != exps.device:
         raise ValueError(f"{what}: data on {data.device}, exponents on {exps.device}")
-    if data.shape[4] not in HEAD_DIMS:
-        raise ValueError(f"{what}: head dim {data.shape[4]} is none of {HEAD_DIMS}")
-    return data.shape[0], data.shape[2], data.shape[4]
+    if shape[4] not in HEAD_DIMS:
+        raise ValueError(f"{what}: head dim {shape[4]} is none of {HEAD_DIMS}")
+    return shape[0], shape[2], shape[4]
 
 
 def two_to(e: torch.Tensor) -> torch.Tensor:
