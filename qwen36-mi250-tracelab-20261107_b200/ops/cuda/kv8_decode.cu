@@ -99,7 +99,7 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
-// Sequence whose runs [first[b], first[b + 1]) hold run x.
+// Sequence b whose part [first[b], first[b + 1]) holds x.
 __device__ __forceinline__ int kv8_find(const int* first, int B, int x) {
   int lo = 0, hi = B;
   while (hi - lo > 1) {
@@ -115,11 +115,11 @@ struct Kv8Unit {
 };
 
 __device__ __forceinline__ int kv8_length(const int64_t* positions, int row, int most) {
-  return max(0, min(static_cast<int>(min(__ldg(positions + row), static_cast<int64_t>(most))) + 1, most));
+  return static_cast<int>(max(int64_t(-1), min(__ldg(positions + row), static_cast<int64_t>(most) - 1))) + 1;
 }
 
 template <int D, int NT>
-__global__ void __maxnreg__(96)  // two CTAs of 9 warps or one of 17
+__global__ void __maxnreg__(96)  // two CTAs of 9 warps or one of 17: five warps of a quarter SM
 kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtensorMap tm_exps, Kv8DecodeParams p) {
   using C = Kv8DecodeCfg<D, NT>;
   constexpr int SLOTS = C::SLOTS, CHUNKS = D / 16, COLS = 8 * NT, DI = (D + 127) / 128, SLABS = K8D_SLABS, NA = C::NA;
@@ -135,8 +135,9 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
   __shared__ __align__(8) uint64_t w_full[2], w_empty[2];   // weights of an even / odd page
   __shared__ __align__(8) uint64_t u_full[K8D_UNITS], u_empty[K8D_UNITS];
   __shared__ __align__(8) uint64_t l_full[2], l_empty[2];   // sums of an even / odd unit
-  __shared__ int s_first[K8D_SEQS + 1];                // runs behind the first of the sequences before
+  __shared__ int s_first[K8D_SEQS + 1], s_tail[K8D_SEQS + 1];  // full runs of the sequences before; last runs that are not full, likewise
   __shared__ Kv8Unit s_unit[K8D_UNITS];
+  __shared__ int s_len[K8D_UNITS][32];                 // keys of the unit's rows
   __shared__ int s_scaled[2][C::HALVES];
   __shared__ __align__(16) float s_max[SLABS][COLS], s_factor[2][COLS];   // read two columns at a time
   __shared__ float s_sum[2][SLABS][COLS], s_top[2][COLS], s_scale[COLS];
@@ -165,12 +166,14 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
   const int most = min(p.width, p.n_splits * (K8D_RUN / KV8_PAGE)) * KV8_PAGE;  // keys that the tables can name
 
   if (warp == C::SW + C::OW) {
-    // ---------------- loads. The units are the runs of all sequences; this CTA's are a grid size apart. Once the pages are on their
-    // way any other load waits behind some 30 MB of them, 4 us: what a unit needs to know is asked for two units ahead, and published one ahead.
+    // ---------------- loads. The units are the runs of all sequences, those of RUN keys first and what is left of each sequence last, so that
+    // the CTAs, which take units a grid size apart, get as many pages each. Once the pages are on their way any other load waits behind
+    // some 30 MB of them, 4 us: what a unit needs to know is asked for two units ahead, and published one ahead.
     const int per_seq = p.units_per_seq * p.n_kv;
-    int before = 0;
+    int full_before = 0, tails_before = 0;
     for (int b0 = 0; b0 < p.B; b0 += 128) {
-      int runs[4], len[4] = {0, 0, 0, 0};
+      int len[4] = {0, 0, 0, 0};
+#pragma unroll 4
       for (int r = 0; r < p.G; ++r)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -180,19 +183,21 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int b = b0 + i * 32 + lane;
-        runs[i] = b < p.B ? max(1, (len[i] + K8D_RUN - 1) / K8D_RUN) : 0;  // a sequence without keys has a run, which writes its zeros
+        int full = len[i] / K8D_RUN;
+        const uint32_t tails = __ballot_sync(0xffffffffu, b < p.B && (len[i] % K8D_RUN || len[i] == 0));  // one without keys has a run, which writes its zeros
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-          const int u = __shfl_up_sync(0xffffffffu, runs[i], o);
-          if (lane >= o) runs[i] += u;
+          const int u = __shfl_up_sync(0xffffffffu, full, o);
+          if (lane >= o) full += u;
         }
-        if (b < p.B) s_first[b + 1] = before + runs[i];
-        before += __shfl_sync(0xffffffffu, runs[i], 31);
+        if (b < p.B) { s_first[b + 1] = full_before + full; s_tail[b + 1] = tails_before + __popc(tails & (2u << lane) - 1u); }
+        full_before += __shfl_sync(0xffffffffu, full, 31);
+        tails_before += __popc(tails);
       }
     }
-    if (lane == 0) s_first[0] = 0;
+    if (lane == 0) s_first[0] = s_tail[0] = 0;
     __syncwarp();
-    const int total = before * per_seq;
+    const int total = (full_before + tails_before) * per_seq;
     struct Ahead { Kv8Unit u; int len, page; };  // lane i: keys of the unit's row i, page i of its run
     const auto ask = [&](int j) {  // unit j; rows of 0: there is none
       Ahead a = {};
@@ -200,8 +205,8 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
       if (id >= total) return a;
       const int run = id / per_seq, k = id - run * per_seq, rg = k / p.n_kv;
       a.u.kh = k - rg * p.n_kv;
-      a.u.seq = kv8_find(s_first, p.B, run);
-      a.u.z = run - s_first[a.u.seq];
+      a.u.seq = run < full_before ? kv8_find(s_first, p.B, run) : kv8_find(s_tail, p.B, run - full_before);
+      a.u.z = (run < full_before ? run : s_first[a.u.seq + 1]) - s_first[a.u.seq];
       a.u.row0 = a.u.seq * p.G + rg * p.rows_per_unit;
       a.u.rows = min(p.rows_per_unit, p.G - rg * p.rows_per_unit);
       if (lane < a.u.rows) a.len = kv8_length(p.positions, a.u.row0 + lane, most);
@@ -214,6 +219,8 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
       const int us = j % K8D_UNITS;
       a.u.keys = max(0, min(K8D_RUN, __reduce_max_sync(0xffffffffu, a.len) - a.u.z * K8D_RUN));
       ok = ok && mbar_wait_warp(&u_empty[us], ((j / K8D_UNITS) & 1) ^ 1, p.err, ERR_WAIT_EMPTY, abort_flag);
+      if (ok) s_len[us][lane] = a.len;
+      __syncwarp();
       if (ok && lane == 0) { s_unit[us] = a.u; mbar_arrive(&u_full[us]); }
     };
     Ahead now = ask(0), next = ask(1);
@@ -281,7 +288,6 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
     // A unit's description; its queries are fetched one unit ahead. Either all these warps have it or none goes on: each stays in
     // step with the barriers of the others.
     bool known = false;
-    int last_next[NA][2];    // columns 2 t, 2 t + 1: last visible key of the run
     const auto enter = [&](int j) {
       ok = ok && mbar_wait_warp(&u_full[j % K8D_UNITS], (j / K8D_UNITS) & 1, p.err, ERR_WAIT_FULL, abort_flag);
       known = ok = !meet_scores_or(bar, !ok);
@@ -290,22 +296,20 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
       known = u.rows > 0;
       if (!known) return;
       fetch(u);
+    };
+    enter(0);
+    for (int j = 0; known; ++j) {
+      const int us = j % K8D_UNITS;
+      const Kv8Unit u = s_unit[us];
+      int last[NA][2];  // columns 2 t, 2 t + 1: last visible key of the run
 #pragma unroll
       for (int n8 = 0; n8 < NA; ++n8)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           int row, head;
           column((tile + n8) * 8 + 2 * t + k, row, head);
-          last_next[n8][k] = (row < u.rows ? kv8_length(p.positions, u.row0 + row, most) : 0) - 1 - u.z * K8D_RUN;
+          last[n8][k] = s_len[us][row] - 1 - u.z * K8D_RUN;
         }
-    };
-    enter(0);
-    for (int j = 0; known; ++j) {
-      const int us = j % K8D_UNITS;
-      const Kv8Unit u = s_unit[us];
-      int last[NA][2];
-#pragma unroll
-      for (int n8 = 0; n8 < NA; ++n8) { last[n8][0] = last_next[n8][0]; last[n8][1] = last_next[n8][1]; }
       // queries as halves with the column's largest number in [2^10, 2^11), in the order of the products' second operand: lane
       // (column % 8, t) holds dims 16 c + 4 t .. + 3 of chunk c
 #pragma unroll
@@ -493,29 +497,17 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
     const Kv8Unit u = s_unit[us];
     if (u.rows == 0) break;
     float o[NT][C::PER][4];
-    int lens[NT][2];  // keys of the rows of columns 2 t, 2 t + 1
+    uint32_t gates[NT][2][C::PER];  // of rows whose only run this is, two dims each
 #pragma unroll
     for (int n8 = 0; n8 < NT; ++n8)
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         int r, h;
         column(n8 * 8 + 2 * t + k, r, h);
-        lens[n8][k] = r < u.rows ? kv8_length(p.positions, u.row0 + r, most) : 0;
-      }
-    uint16_t gates[NT][2][C::PER][2];  // of rows whose only run this is
+        const bool direct = r < u.rows && u.z == 0 && s_len[us][r] <= K8D_RUN;
+        const bf16* src = p.gate + (static_cast<size_t>(u.row0 + r) * p.n_q + u.kh * p.group + h) * D + tile0 * 16 + 2 * g;
 #pragma unroll
-    for (int n8 = 0; n8 < NT; ++n8)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        int r, h;
-        column(n8 * 8 + 2 * t + k, r, h);
-        const bool direct = r < u.rows && u.z == 0 && lens[n8][k] <= K8D_RUN;
-        const uint16_t* src = reinterpret_cast<const uint16_t*>(p.gate) + (static_cast<size_t>(u.row0 + r) * p.n_q + u.kh * p.group + h) * D + tile0 * 16 + 2 * g;
-#pragma unroll
-        for (int i = 0; i < C::PER; ++i) {
-          gates[n8][k][i][0] = direct ? __ldg(src + i * 16) : uint16_t(0);
-          gates[n8][k][i][1] = direct ? __ldg(src + i * 16 + 1) : uint16_t(0);
-        }
+        for (int i = 0; i < C::PER; ++i) gates[n8][k][i] = direct ? __ldg(reinterpret_cast<const uint32_t*>(src + i * 16)) : 0u;
       }
 #pragma unroll
     for (int n8 = 0; n8 < NT; ++n8)
@@ -607,7 +599,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
           float sum = 0.f;
 #pragma unroll
           for (int w = 0; w < SLABS; ++w) sum += s_sum[half][w][n8 * 8 + 2 * t + k];
-          const int len = lens[n8][k];
+          const int len = s_len[us][r];
           const size_t head = static_cast<size_t>(u.row0 + r) * p.n_q + u.kh * p.group + h;
           if (len > K8D_RUN) {
             if (u.z * K8D_RUN < len) {
@@ -623,8 +615,8 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
             for (int i = 0; i < C::PER; ++i) {
               const size_t at = head * D + (tile0 + i) * 16 + 2 * g;
               *reinterpret_cast<__nv_bfloat162*>(p.out + at) =
-                  __floats2bfloat162_rn(o[n8][i][k] * inv * kv8_sigmoid(__uint_as_float(static_cast<uint32_t>(gates[n8][k][i][0]) << 16)),
-                                        o[n8][i][2 + k] * inv * kv8_sigmoid(__uint_as_float(static_cast<uint32_t>(gates[n8][k][i][1]) << 16)));
+                  __floats2bfloat162_rn(o[n8][i][k] * inv * kv8_sigmoid(__uint_as_float(gates[n8][k][i] << 16)),
+                                        o[n8][i][2 + k] * inv * kv8_sigmoid(__uint_as_float(gates[n8][k][i] & 0xffff0000u)));
             }
           }
         }
@@ -671,23 +663,27 @@ __device__ __forceinline__ void k8d_add(float best, float top, float l, const fl
   sum = fmaf(l, f, sum);
   o.x = fmaf(acc.x, f, o.x); o.y = fmaf(acc.y, f, o.y); o.z = fmaf(acc.z, f, o.z); o.w = fmaf(acc.w, f, o.w);
 }
-__device__ __forceinline__ void k8d_store(bf16* out, const bf16* gate, const float4& o, float sum) {
+__device__ __forceinline__ void k8d_store(bf16* out, uint2 gate, const float4& o, float sum) {
   const float inv = 1.0f / sum;
+  const auto sig = [](uint32_t bits) { return kv8_sigmoid(__uint_as_float(bits)); };
   uint2 raw;
   __nv_bfloat162* e = reinterpret_cast<__nv_bfloat162*>(&raw);
-  e[0] = __floats2bfloat162_rn(o.x * inv * kv8_sigmoid(__bfloat162float(gate[0])), o.y * inv * kv8_sigmoid(__bfloat162float(gate[1])));
-  e[1] = __floats2bfloat162_rn(o.z * inv * kv8_sigmoid(__bfloat162float(gate[2])), o.w * inv * kv8_sigmoid(__bfloat162float(gate[3])));
+  e[0] = __floats2bfloat162_rn(o.x * inv * sig(gate.x << 16), o.y * inv * sig(gate.x & 0xffff0000u));
+  e[1] = __floats2bfloat162_rn(o.z * inv * sig(gate.y << 16), o.w * inv * sig(gate.y & 0xffff0000u));
   *reinterpret_cast<uint2*>(out) = raw;
 }
-// Tables of up to 64 runs (16,384 keys): a thread takes all sums of four dims of a head.
+// Tables of up to 64 runs (16,384 keys): a thread takes all sums of four dims of a head. Its CTAs are small enough to wait beside the
+// kernel in front.
 template <int D>
-__global__ void __launch_bounds__(256)
+__global__ void __maxnreg__(72)
 kv8_combine_few_kernel(const float* part_acc, const float2* part_ml, const bf16* gate, const int64_t* positions, bf16* out, int heads,
                        int n_q, int n_splits, int most) {
   constexpr int QUADS = D / 4;
-  const size_t head = static_cast<size_t>(blockIdx.x) * (256 / QUADS) + threadIdx.x / QUADS;
+  const size_t head = static_cast<size_t>(blockIdx.x) * (128 / QUADS) + threadIdx.x / QUADS;
   const int quad = threadIdx.x % QUADS;
   const int runs = head < heads ? (kv8_length(positions, static_cast<int>(head / n_q), most) + K8D_RUN - 1) / K8D_RUN : 0;
+  const size_t at = head * D + quad * 4;
+  const uint2 g = runs > 1 ? __ldg(reinterpret_cast<const uint2*>(gate + at)) : make_uint2(0u, 0u);
   pdl_wait();
   pdl_launch();
   if (runs <= 1) return;
@@ -695,29 +691,54 @@ kv8_combine_few_kernel(const float* part_acc, const float2* part_ml, const bf16*
   const float4* pa = reinterpret_cast<const float4*>(part_acc + head * n_splits * D) + quad;
   float best = -INFINITY, sum = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-  for (int z = 0; z < runs; ++z) best = fmaxf(best, ml[z].x);
-  for (int i = 0; i < K8D_SUMS && i < runs; i += 4) {
-    float top[4], l[4];
-    float4 acc[4];
-    k8d_sums<D>(pa, ml, runs, i, top, l, acc);
+  if (runs <= K8D_SUMS) {  // a sum has one partial: it is that one, and all are asked for at once
+    constexpr int AT_ONCE = 6;
+    float2 pm[AT_ONCE];
+    float4 v[AT_ONCE];
+    const auto ask = [&](int z0) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) k8d_add(best, top[k], l[k], acc[k], sum, o);
+      for (int i = 0; i < AT_ONCE; ++i) {
+        pm[i] = z0 + i < runs ? ml[z0 + i] : make_float2(-INFINITY, 0.f);
+        v[i] = z0 + i < runs ? pa[static_cast<size_t>(z0 + i) * QUADS] : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    };
+    ask(0);
+    for (int z = AT_ONCE; z < runs; ++z) best = fmaxf(best, ml[z].x);
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) best = fmaxf(best, pm[i].x);
+    for (int z0 = 0;;) {
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) k8d_add(best, pm[i].x, pm[i].y, v[i], sum, o);
+      z0 += AT_ONCE;
+      if (z0 >= runs) break;
+      ask(z0);
+    }
+  } else {
+#pragma unroll 8
+    for (int z = 0; z < runs; ++z) best = fmaxf(best, ml[z].x);
+    for (int i = 0; i < K8D_SUMS; i += 4) {
+      float top[4], l[4];
+      float4 acc[4];
+      k8d_sums<D>(pa, ml, runs, i, top, l, acc);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) k8d_add(best, top[k], l[k], acc[k], sum, o);
+    }
   }
-  const size_t at = head * D + quad * 4;
-  k8d_store(out + at, gate + at, o, sum);
+  k8d_store(out + at, g, o, sum);
 }
-// More: a CTA takes up to 64 dims of a head, a thread one sum of four of them; rows of few runs as above.
+// More: a CTA takes 64 dims of a head, a thread one sum of four of them, eight of its partials under way; rows of few runs as above.
 template <int D>
 __global__ void __launch_bounds__(256)
 kv8_combine_kernel(const float* part_acc, const float2* part_ml, const bf16* gate, const int64_t* positions, bf16* out, int n_q,
                    int n_splits, int most) {
-  constexpr int DIMS = D < 64 ? D : 64, QUADS = DIMS / 4;
+  constexpr int DIMS = 64, QUADS = DIMS / 4;
   __shared__ float4 s_acc[K8D_SUMS][QUADS];
   __shared__ float s_top[K8D_SUMS], s_l[K8D_SUMS];
   const size_t head = blockIdx.x;
   const int quad = threadIdx.x % QUADS, i = threadIdx.x / QUADS;
   const int runs = (kv8_length(positions, static_cast<int>(head / n_q), most) + K8D_RUN - 1) / K8D_RUN;
+  const size_t at = head * D + blockIdx.y * DIMS + quad * 4;
+  const uint2 g = __ldg(reinterpret_cast<const uint2*>(gate + at));
   pdl_wait();
   pdl_launch();
   if (runs <= 1) return;
@@ -726,13 +747,24 @@ kv8_combine_kernel(const float* part_acc, const float2* part_ml, const bf16* gat
   if (i < K8D_SUMS) {
     float top = -INFINITY, l = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int z = i; z < runs; z += K8D_SUMS) top = fmaxf(top, ml[z].x);
-#pragma unroll 4
-    for (int z = i; z < runs; z += K8D_SUMS) {
-      const float2 pm = ml[z];
-      const float4 v = pa[static_cast<size_t>(z) * (D / 4)];
-      k8d_add(top, pm.x, pm.y, v, l, acc);
+    constexpr int AT_ONCE = 8;
+    for (int z0 = i; z0 < runs; z0 += AT_ONCE * K8D_SUMS) {
+      float2 pm[AT_ONCE];
+      float4 v[AT_ONCE];
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; ++k) {
+        const int z = z0 + k * K8D_SUMS;
+        pm[k] = z < runs ? ml[z] : make_float2(-INFINITY, 0.f);
+        v[k] = z < runs ? pa[static_cast<size_t>(z) * (D / 4)] : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      float next = top;
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; ++k) next = fmaxf(next, pm[k].x);
+      const float f = next == top ? 1.f : ex2(top - next);
+      top = next;
+      l *= f; acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; ++k) k8d_add(top, pm[k].x, pm[k].y, v[k], l, acc);
     }
     s_acc[i][quad] = acc;
     if (quad == 0) { s_top[i] = top; s_l[i] = l; }
@@ -744,8 +776,7 @@ kv8_combine_kernel(const float* part_acc, const float2* part_ml, const bf16* gat
 #pragma unroll
   for (int k = 0; k < K8D_SUMS; ++k) best = fmaxf(best, s_top[k]);
   for (int k = 0; k < K8D_SUMS; ++k) k8d_add(best, s_top[k], s_l[k], s_acc[k][quad], sum, o);
-  const size_t at = head * D + blockIdx.y * DIMS + quad * 4;
-  k8d_store(out + at, gate + at, o, sum);
+  k8d_store(out + at, g, o, sum);
 }
 
 }  // namespace b200
@@ -777,7 +808,7 @@ int k8d_make_maps(CUtensorMap* tm, CUtensorMap* tm_exps, const void* data, const
   const cuuint64_t edims[3] = {KV8_PAGE, static_cast<cuuint64_t>(n_kv), static_cast<cuuint64_t>(pages) * 2};
   const cuuint64_t estrides[2] = {KV8_PAGE, static_cast<cuuint64_t>(n_kv) * KV8_PAGE};
   const cuuint32_t ebox[3] = {KV8_PAGE, 1, 2};
-  const int rc = k8d_encode(tm, data, dims, strides, box, rowb == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : rowb == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B);
+  const int rc = k8d_encode(tm, data, dims, strides, box, rowb == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
   return rc ? rc : k8d_encode(tm_exps, exps, edims, estrides, ebox, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
@@ -799,11 +830,11 @@ int k8d_launch(const CUtensorMap& tm, const CUtensorMap& tm_exps, const Kv8Decod
   if (launch_pdl(kern, dim3(grid), dim3(Kv8DecodeCfg<D, NT>::THREADS), Kv8DecodeCfg<D, NT>::SMEM, st, tm, tm_exps, p) != cudaSuccess) return -4;
   if (p.n_splits == 1) return 0;
   const int most = (p.width < p.n_splits * (K8D_RUN / KV8_PAGE) ? p.width : p.n_splits * (K8D_RUN / KV8_PAGE)) * KV8_PAGE;
-  const int heads = p.B * p.G * p.n_q, per = 256 / (D / 4);
+  const int heads = p.B * p.G * p.n_q, per = 128 / (D / 4);
   const cudaError_t rc = p.n_splits <= 64
-      ? launch_pdl(kv8_combine_few_kernel<D>, dim3((heads + per - 1) / per), dim3(256), 0, st, p.part_acc, p.part_ml, p.gate,
+      ? launch_pdl(kv8_combine_few_kernel<D>, dim3((heads + per - 1) / per), dim3(128), 0, st, p.part_acc, p.part_ml, p.gate,
                    p.positions, p.out, heads, p.n_q, p.n_splits, most)
-      : launch_pdl(kv8_combine_kernel<D>, dim3(heads, D < 64 ? 1 : D / 64), dim3(256), 0, st, p.part_acc, p.part_ml, p.gate,
+      : launch_pdl(kv8_combine_kernel<D>, dim3(heads, D / 64), dim3(256), 0, st, p.part_acc, p.part_ml, p.gate,
                    p.positions, p.out, p.n_q, p.n_splits, most);
   return rc == cudaSuccess ? 0 : -4;
 }
@@ -824,7 +855,7 @@ extern "C" int b200_kv8_decode(const void* q, const void* gate, const void* data
   const long long rows = static_cast<long long>(num_pages) * 2 * n_kv * KV8_PAGE;
   if (rows > 0x7fffffffLL) return -7;  // a TMA coordinate
   if (reinterpret_cast<uintptr_t>(data) % 16 || reinterpret_cast<uintptr_t>(exps) % 16 || reinterpret_cast<uintptr_t>(q) % 8) return -7;
-  if (D != 256 && D != 128 && D != 64 && D != 32) return -7;
+  if (D != 256 && D != 128 && D != 64) return -7;
   CUtensorMap tm, tm_exps;
   if (k8d_make_maps(&tm, &tm_exps, data, exps, D, n_kv, num_pages)) return -1;
   const int cols = G * group, nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4, per = 8 * nt / group < G ? 8 * nt / group : G;
@@ -842,8 +873,7 @@ extern "C" int b200_kv8_decode(const void* q, const void* gate, const void* data
 #define K8D(DD) rc = nt == 1 ? k8d_launch<DD, 1>(tm, tm_exps, p, st) : nt == 2 ? k8d_launch<DD, 2>(tm, tm_exps, p, st) : k8d_launch<DD, 4>(tm, tm_exps, p, st)
     if (D == 256) K8D(256);
     else if (D == 128) K8D(128);
-    else if (D == 64) K8D(64);
-    else K8D(32);
+    else K8D(64);
 #undef K8D
     if (rc) return rc;
   }
