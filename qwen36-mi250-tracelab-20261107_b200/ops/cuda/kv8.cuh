@@ -44,4 +44,15 @@ __device__ __forceinline__ void kv8_unpack4(uint32_t word, uint32_t& lo, uint32_
   hi = kv8_unpack2(static_cast<uint16_t>(word >> 16));
 }
 
+// Whether a barrier's phase is complete, without a wait.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred P;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 P, [%1], %2;\n\t"
+      "selp.b32 %0, 1, 0, P;\n\t}"
+      : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return done != 0;
+}
+
 }  // namespace b200

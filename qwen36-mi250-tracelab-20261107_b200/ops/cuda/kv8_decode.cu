@@ -99,6 +99,11 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
+// A wait for a barrier that was looked at before.
+__device__ __forceinline__ bool wait_seen(bool seen, uint64_t* bar, uint32_t parity, int* err, int code, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, seen) || mbar_wait_warp(bar, parity, err, code, abort_flag);
+}
+
 // Sequence b whose part [first[b], first[b + 1]) holds x.
 __device__ __forceinline__ int kv8_find(const int* first, int B, int x) {
   int lo = 0, hi = B;
@@ -109,13 +114,24 @@ __device__ __forceinline__ int kv8_find(const int* first, int B, int x) {
   return lo;
 }
 
-// A unit is (sequence, group of its query rows, KV head, run). keys: of the run, up to the last that a row of the unit sees.
+// A unit is (sequence, group of its query rows, KV head, run). keys: of the run, up to the last that a row of the unit sees. same: the CTA's
+// unit before has the same queries.
 struct Kv8Unit {
-  int seq, kh, z, row0, rows, keys;
+  int seq, kh, z, row0, rows, keys, same;
 };
 
+// Loads that nothing waits for before their value is used; without the condition the value stays.
+__device__ __forceinline__ void ask_64(int64_t& x, const int64_t* p, bool yes) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q ld.global.nc.s64 %0, [%1];\n\t}" : "+l"(x) : "l"(p), "r"(static_cast<int>(yes)));
+}
+__device__ __forceinline__ void ask_32(uint32_t& x, const void* p, bool yes) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q ld.global.nc.u32 %0, [%1];\n\t}" : "+r"(x) : "l"(p), "r"(static_cast<int>(yes)));
+}
+__device__ __forceinline__ int kv8_length(int64_t position, int most) {
+  return static_cast<int>(max(int64_t(-1), min(position, static_cast<int64_t>(most) - 1))) + 1;
+}
 __device__ __forceinline__ int kv8_length(const int64_t* positions, int row, int most) {
-  return static_cast<int>(max(int64_t(-1), min(__ldg(positions + row), static_cast<int64_t>(most) - 1))) + 1;
+  return kv8_length(__ldg(positions + row), most);
 }
 
 template <int D, int NT>
@@ -166,9 +182,9 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
   const int most = min(p.width, p.n_splits * (K8D_RUN / KV8_PAGE)) * KV8_PAGE;  // keys that the tables can name
 
   if (warp == C::SW + C::OW) {
-    // ---------------- loads. The units are the runs of all sequences, those of RUN keys first and what is left of each sequence last, so that
-    // the CTAs, which take units a grid size apart, get as many pages each. Once the pages are on their way any other load waits behind
-    // some 30 MB of them, 4 us: what a unit needs to know is asked for two units ahead, and published one ahead.
+    // ---------------- loads. The units are the runs of all sequences. Those of RUN keys are dealt out first, in one piece to each CTA, so that most follow
+    // one of the same queries; what is left of each sequence goes round, beginning with the CTAs that got a unit less. Once the pages are on
+    // their way any other load waits behind some 30 MB of them, 4 us: what a unit needs to know is asked for two units ahead, and published one ahead.
     const int per_seq = p.units_per_seq * p.n_kv;
     int full_before = 0, tails_before = 0;
     for (int b0 = 0; b0 < p.B; b0 += 128) {
@@ -197,57 +213,80 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
     }
     if (lane == 0) s_first[0] = s_tail[0] = 0;
     __syncwarp();
-    const int total = (full_before + tails_before) * per_seq;
-    struct Ahead { Kv8Unit u; int len, page; };  // lane i: keys of the unit's row i, page i of its run
+    const int grid = gridDim.x, cta = blockIdx.x;
+    const int full = full_before * per_seq, tails = tails_before * per_seq, extra = full % grid;
+    const int mine = full / grid + (cta < extra), first_full = cta * (full / grid) + min(cta, extra), first_tail = (cta + grid - extra) % grid;
+    int seq_before = -1, k_before = 0;
+    struct Ahead { Kv8Unit u; int64_t position; uint32_t page; };  // lane i: position of the unit's row i, page i of its run
     const auto ask = [&](int j) {  // unit j; rows of 0: there is none
       Ahead a = {};
-      const int id = blockIdx.x + j * static_cast<int>(gridDim.x);
-      if (id >= total) return a;
-      const int run = id / per_seq, k = id - run * per_seq, rg = k / p.n_kv;
+      a.position = -1;
+      int k;
+      if (j < mine) {
+        const int id = first_full + j;
+        a.u.seq = kv8_find(s_first, p.B, id / per_seq);
+        const int runs = s_first[a.u.seq + 1] - s_first[a.u.seq], at = id - s_first[a.u.seq] * per_seq;
+        k = at / runs;
+        a.u.z = at - k * runs;
+      } else {
+        const int id = first_tail + (j - mine) * grid, tail = id / per_seq;
+        if (id >= tails) return a;
+        a.u.seq = kv8_find(s_tail, p.B, tail);
+        k = id - tail * per_seq;
+        a.u.z = s_first[a.u.seq + 1] - s_first[a.u.seq];
+      }
+      a.u.same = a.u.seq == seq_before && k == k_before;
+      seq_before = a.u.seq;
+      k_before = k;
+      const int rg = k / p.n_kv;
       a.u.kh = k - rg * p.n_kv;
-      a.u.seq = run < full_before ? kv8_find(s_first, p.B, run) : kv8_find(s_tail, p.B, run - full_before);
-      a.u.z = (run < full_before ? run : s_first[a.u.seq + 1]) - s_first[a.u.seq];
       a.u.row0 = a.u.seq * p.G + rg * p.rows_per_unit;
       a.u.rows = min(p.rows_per_unit, p.G - rg * p.rows_per_unit);
-      if (lane < a.u.rows) a.len = kv8_length(p.positions, a.u.row0 + lane, most);
-      if (lane < K8D_PAGES && a.u.z * K8D_PAGES + lane < p.width)
-        a.page = __ldg(p.tables + static_cast<size_t>(a.u.seq) * p.max_pages + a.u.z * K8D_PAGES + lane);
+      ask_64(a.position, p.positions + a.u.row0 + lane, lane < a.u.rows);
+      ask_32(a.page, p.tables + static_cast<size_t>(a.u.seq) * p.max_pages + a.u.z * K8D_PAGES + lane,
+             lane < K8D_PAGES && a.u.z * K8D_PAGES + lane < p.width);
       return a;
     };
     bool ok = true;
     const auto publish = [&](Ahead& a, int j) {
       const int us = j % K8D_UNITS;
-      a.u.keys = max(0, min(K8D_RUN, __reduce_max_sync(0xffffffffu, a.len) - a.u.z * K8D_RUN));
+      const int len = kv8_length(a.position, most);
+      a.u.keys = max(0, min(K8D_RUN, __reduce_max_sync(0xffffffffu, len) - a.u.z * K8D_RUN));
       ok = ok && mbar_wait_warp(&u_empty[us], ((j / K8D_UNITS) & 1) ^ 1, p.err, ERR_WAIT_EMPTY, abort_flag);
-      if (ok) s_len[us][lane] = a.len;
+      if (ok) s_len[us][lane] = len;
       __syncwarp();
       if (ok && lane == 0) { s_unit[us] = a.u; mbar_arrive(&u_full[us]); }
     };
     Ahead now = ask(0), next = ask(1);
     publish(now, 0);
-    publish(next, 1);
     int n = 0;
     for (int j = 0; now.u.rows > 0 && ok; ++j) {
-      Ahead later = ask(j + 2);
-      for (int pg = 0; pg * KV8_PAGE < now.u.keys && ok; ++pg, ++n) {
+      Ahead later = {};
+      int pg = 0;
+      const auto load = [&] {
         const int s = n % SLOTS;
-        int page = __shfl_sync(0xffffffffu, now.page, pg);
+        int page = static_cast<int>(__shfl_sync(0xffffffffu, now.page, pg));
         if (page < 0 || page >= p.num_pages) { if (lane == 0) atomicCAS(p.err, 0, ERR_BAD_INDEX); page = 0; }
         const int row = (page * 2 * p.n_kv + now.u.kh) * KV8_PAGE;
         ok = mbar_wait_warp(&k_empty[s], ((n / SLOTS) & 1) ^ 1, p.err, ERR_WAIT_EMPTY, abort_flag);
-        if (!ok) break;
+        if (!ok) return;
         if (elect_one()) {
           mbar_expect_tx(&k_full[s], C::TILE + C::EXPS);
           tma_load_3d(s_k + s * C::TILE, &tm, &k_full[s], 0, row, 0);
           tma_load_3d(s_exps + s * C::EXPS, &tm_exps, &k_full[s], 0, now.u.kh, page * 2);
         }
         ok = mbar_wait_warp(&v_empty[s], ((n / SLOTS) & 1) ^ 1, p.err, ERR_WAIT_EMPTY, abort_flag);
-        if (!ok) { ++n; break; }
-        if (elect_one()) {
+        if (ok && elect_one()) {
           mbar_expect_tx(&v_full[s], C::TILE);
           tma_load_3d(s_v + s * C::TILE, &tm, &v_full[s], 0, row + p.n_kv * KV8_PAGE, 0);
         }
-      }
+        ++n;
+        ++pg;
+      };
+      if (now.u.keys > 0) load();
+      later = ask(j + 2);
+      if (j == 0) publish(next, 1);  // the warps of scores want it before they give a slot back
+      while (pg * KV8_PAGE < now.u.keys && ok) load();
       publish(later, j + 2);
       now = next;
       next = later;
@@ -279,10 +318,11 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
       for (int i = 0; i < QC; ++i) {
         int row, head;
         column(tile * 8 + slab * QC + i, row, head);
-        const bf16* src = p.q + (static_cast<size_t>(u.row0 + row) * p.n_q + u.kh * p.group + head) * D + lane * 4;
+        // a column without a row takes the last one's: nothing reads what comes of it. No condition on the load, so that nothing waits for it here.
+        const bf16* src = p.q + (static_cast<size_t>(u.row0 + min(row, u.rows - 1)) * p.n_q + u.kh * p.group + head) * D + lane * 4 % D;
 #pragma unroll
         for (int k = 0; k < DI; ++k)
-          raw[i][k] = row < u.rows && lane * 4 + k * 128 < D ? *reinterpret_cast<const uint2*>(src + k * 128) : make_uint2(0u, 0u);
+          asm volatile("ld.global.nc.v2.u32 {%0, %1}, [%2];" : "=r"(raw[i][k].x), "=r"(raw[i][k].y) : "l"(src + k * 128));
       }
     };
     // A unit's description; its queries are fetched one unit ahead. Either all these warps have it or none goes on: each stays in
@@ -294,10 +334,12 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
       if (!known) return;
       const Kv8Unit u = s_unit[j % K8D_UNITS];
       known = u.rows > 0;
-      if (!known) return;
-      fetch(u);
+      if (known && !u.same) fetch(u);
     };
+    uint2 qf[CHUNKS];      // queries of the first column tile; a second one's are read at each use
+    float qscale[NA][2];   // what takes the product to log-2 scores
     enter(0);
+    const auto keys_here = [&](int i) { return mbar_test(&k_full[i % SLOTS], (i / SLOTS) & 1); };
     for (int j = 0; known; ++j) {
       const int us = j % K8D_UNITS;
       const Kv8Unit u = s_unit[us];
@@ -310,56 +352,59 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
           column((tile + n8) * 8 + 2 * t + k, row, head);
           last[n8][k] = s_len[us][row] - 1 - u.z * K8D_RUN;
         }
-      // queries as halves with the column's largest number in [2^10, 2^11), in the order of the products' second operand: lane
-      // (column % 8, t) holds dims 16 c + 4 t .. + 3 of chunk c
+      if (!u.same) {
+        // queries as halves with the column's largest number in [2^10, 2^11), in the order of the products' second operand: lane
+        // (column % 8, t) holds dims 16 c + 4 t .. + 3 of chunk c
 #pragma unroll
-      for (int i = 0; i < QC; ++i) {
-        const int col = tile * 8 + slab * QC + i;
-        float x[DI][4];
-        float top = 0.f;
-        bool bad = false;
+        for (int i = 0; i < QC; ++i) {
+          const int col = tile * 8 + slab * QC + i;
+          float x[DI][4];
+          float top = 0.f;
+          bool bad = false;
 #pragma unroll
-        for (int k = 0; k < DI; ++k) {
-          const __nv_bfloat162* e = reinterpret_cast<const __nv_bfloat162*>(&raw[i][k]);
-          const float2 a = __bfloat1622float2(e[0]), b = __bfloat1622float2(e[1]);
-          x[k][0] = a.x; x[k][1] = a.y; x[k][2] = b.x; x[k][3] = b.y;
+          for (int k = 0; k < DI; ++k) {
+            const __nv_bfloat162* e = reinterpret_cast<const __nv_bfloat162*>(&raw[i][k]);
+            const float2 a = __bfloat1622float2(e[0]), b = __bfloat1622float2(e[1]);
+            x[k][0] = a.x; x[k][1] = a.y; x[k][2] = b.x; x[k][3] = b.y;
 #pragma unroll
-          for (int h = 0; h < 4; ++h) { top = fmaxf(top, fabsf(x[k][h])); bad |= !(fabsf(x[k][h]) <= 3.4e38f); }
-        }
-        top = warp_max(top);
-        const int e = max(-110, min(110, static_cast<int>(__float_as_uint(top) >> 23) - 127 - 10));
-        const float f = kv8_two_to(-e);
-#pragma unroll
-        for (int k = 0; k < DI; ++k) {
-          if (lane * 4 + k * 128 < D) {
-            const __half2 lo = __floats2half2_rn(x[k][0] * f, x[k][1] * f), hi = __floats2half2_rn(x[k][2] * f, x[k][3] * f);
-            s_q[col / 8][k * 8 + lane / 4][col % 8 * 4 + lane % 4] = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+            for (int h = 0; h < 4; ++h) { top = fmaxf(top, fabsf(x[k][h])); bad |= !(fabsf(x[k][h]) <= 3.4e38f); }
           }
+          top = warp_max(top);
+          const int e = max(-110, min(110, static_cast<int>(__float_as_uint(top) >> 23) - 127 - 10));
+          const float f = kv8_two_to(-e);
+#pragma unroll
+          for (int k = 0; k < DI; ++k) {
+            if (lane * 4 + k * 128 < D) {
+              const __half2 lo = __floats2half2_rn(x[k][0] * f, x[k][1] * f), hi = __floats2half2_rn(x[k][2] * f, x[k][3] * f);
+              s_q[col / 8][k * 8 + lane / 4][col % 8 * 4 + lane % 4] = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+            }
+          }
+          // a NaN or an infinity anywhere in the column: all its scores are NaN
+          const bool any = __any_sync(0xffffffffu, bad);
+          if (lane == 0) s_scale[col] = any ? __uint_as_float(0x7fffffffu) : kv8_two_to(e) * p.scale_log2;
         }
-        // a NaN or an infinity anywhere in the column: all its scores are NaN
-        const bool any = __any_sync(0xffffffffu, bad);
-        if (lane == 0) s_scale[col] = any ? __uint_as_float(0x7fffffffu) : kv8_two_to(e) * p.scale_log2;
+        meet_scores(bar);
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) qf[c] = s_q[tile][c][lane];
+#pragma unroll
+        for (int n8 = 0; n8 < NA; ++n8)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) qscale[n8][k] = s_scale[(tile + n8) * 8 + 2 * t + k];
       }
-      meet_scores(bar);
       enter(j + 1);
-      uint2 qf[CHUNKS];      // of the first column tile; a second one's are read at each use
-      float qscale[NA][2];   // what takes the product to log-2 scores
+      bool k_seen = keys_here(n);  // barriers are looked at ahead of their wait, which takes its time even where there is none
       float m[NA][2], l[NA][2];
 #pragma unroll
-      for (int c = 0; c < CHUNKS; ++c) qf[c] = s_q[tile][c][lane];
-#pragma unroll
-      for (int n8 = 0; n8 < NA; ++n8)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          qscale[n8][k] = s_scale[(tile + n8) * 8 + 2 * t + k];
-          m[n8][k] = -INFINITY;
-          l[n8][k] = 0.f;
-        }
+      for (int n8 = 0; n8 < NA; ++n8) {
+        m[n8][0] = m[n8][1] = -INFINITY;
+        l[n8][0] = l[n8][1] = 0.f;
+      }
 
       for (int key0 = 0; key0 < u.keys; key0 += KV8_PAGE, ++n) {
         const int s = n % SLOTS, half = n & 1;
         const bool mine = key0 + slab * K8D_SLAB < u.keys;
-        ok = ok && mbar_wait_warp(&k_full[s], (n / SLOTS) & 1, p.err, ERR_WAIT_FULL, abort_flag);
+        const bool w_seen = mbar_test(&w_empty[half], ((n >> 1) & 1) ^ 1);
+        ok = ok && wait_seen(k_seen, &k_full[s], (n / SLOTS) & 1, p.err, ERR_WAIT_FULL, abort_flag);
         // S[key, column], keys g and g + 8 of this warp's slab
         float y[NA][2][2];  // [key][column 2 t, 2 t + 1]
         float vi[2];
@@ -424,7 +469,8 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
             }
           meet_scores(bar);
         }
-        ok = ok && mbar_wait_warp(&w_empty[half], ((n >> 1) & 1) ^ 1, p.err, ERR_WAIT_EMPTY, abort_flag);
+        k_seen = keys_here(n + 1);
+        ok = ok && wait_seen(w_seen, &w_empty[half], ((n >> 1) & 1) ^ 1, p.err, ERR_WAIT_EMPTY, abort_flag);
         if (any) {
 #pragma unroll
           for (int n8 = 0; n8 < NA; ++n8) {
@@ -497,17 +543,20 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
     const Kv8Unit u = s_unit[us];
     if (u.rows == 0) break;
     float o[NT][C::PER][4];
-    uint32_t gates[NT][2][C::PER];  // of rows whose only run this is, two dims each
+    uint32_t gates[NT][2][C::PER];  // where a run is all there is, two dims each
 #pragma unroll
     for (int n8 = 0; n8 < NT; ++n8)
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         int r, h;
         column(n8 * 8 + 2 * t + k, r, h);
-        const bool direct = r < u.rows && u.z == 0 && s_len[us][r] <= K8D_RUN;
+        const bool direct = p.n_splits == 1 && r < u.rows;
         const bf16* src = p.gate + (static_cast<size_t>(u.row0 + r) * p.n_q + u.kh * p.group + h) * D + tile0 * 16 + 2 * g;
 #pragma unroll
-        for (int i = 0; i < C::PER; ++i) gates[n8][k][i] = direct ? __ldg(reinterpret_cast<const uint32_t*>(src + i * 16)) : 0u;
+        for (int i = 0; i < C::PER; ++i) {
+          gates[n8][k][i] = 0u;
+          ask_32(gates[n8][k][i], src + i * 16, direct);
+        }
       }
 #pragma unroll
     for (int n8 = 0; n8 < NT; ++n8)
@@ -596,21 +645,24 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
           int r, h;
           column(n8 * 8 + 2 * t + k, r, h);
           if (r >= u.rows) continue;
-          float sum = 0.f;
-#pragma unroll
-          for (int w = 0; w < SLABS; ++w) sum += s_sum[half][w][n8 * 8 + 2 * t + k];
           const int len = s_len[us][r];
           const size_t head = static_cast<size_t>(u.row0 + r) * p.n_q + u.kh * p.group + h;
-          if (len > K8D_RUN) {
+          const auto sum = [&] {
+            float x = 0.f;
+#pragma unroll
+            for (int w = 0; w < SLABS; ++w) x += s_sum[half][w][n8 * 8 + 2 * t + k];
+            return x;
+          };
+          if (p.n_splits > 1) {
             if (u.z * K8D_RUN < len) {
               const size_t slot = head * p.n_splits + u.z;
-              if (tile0 == 0 && g == 0) p.part_ml[slot] = make_float2(s_top[half][n8 * 8 + 2 * t + k], sum);
+              if (tile0 == 0 && g == 0) p.part_ml[slot] = make_float2(s_top[half][n8 * 8 + 2 * t + k], sum());
 #pragma unroll
               for (int i = 0; i < C::PER; ++i)
                 *reinterpret_cast<float2*>(p.part_acc + slot * D + (tile0 + i) * 16 + 2 * g) = make_float2(o[n8][i][k], o[n8][i][2 + k]);
             }
-          } else if (u.z == 0) {  // the row's only run
-            const float inv = len > 0 ? 1.0f / sum : 0.f;
+          } else {
+            const float inv = len > 0 ? 1.0f / sum() : 0.f;
 #pragma unroll
             for (int i = 0; i < C::PER; ++i) {
               const size_t at = head * D + (tile0 + i) * 16 + 2 * g;
@@ -626,7 +678,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
   }
 }
 
-// Rows of more than one run. Partial z goes to sum z % 16, at the sum's own maximum, and the sums are added in order: one chain over
+// What the runs of a row come to. Partial z goes to sum z % 16, at the sum's own maximum, and the sums are added in order: one chain over
 // the partials where there are up to 16. What does not come from the kernel in front is read ahead of the dependency wait: that kernel has
 // waited for everything before it.
 constexpr int K8D_SUMS = 16;
@@ -663,8 +715,8 @@ __device__ __forceinline__ void k8d_add(float best, float top, float l, const fl
   sum = fmaf(l, f, sum);
   o.x = fmaf(acc.x, f, o.x); o.y = fmaf(acc.y, f, o.y); o.z = fmaf(acc.z, f, o.z); o.w = fmaf(acc.w, f, o.w);
 }
-__device__ __forceinline__ void k8d_store(bf16* out, uint2 gate, const float4& o, float sum) {
-  const float inv = 1.0f / sum;
+__device__ __forceinline__ void k8d_store(bf16* out, uint2 gate, const float4& o, float sum, bool any) {
+  const float inv = any ? 1.0f / sum : 0.f;  // a row without keys
   const auto sig = [](uint32_t bits) { return kv8_sigmoid(__uint_as_float(bits)); };
   uint2 raw;
   __nv_bfloat162* e = reinterpret_cast<__nv_bfloat162*>(&raw);
@@ -683,10 +735,10 @@ kv8_combine_few_kernel(const float* part_acc, const float2* part_ml, const bf16*
   const int quad = threadIdx.x % QUADS;
   const int runs = head < heads ? (kv8_length(positions, static_cast<int>(head / n_q), most) + K8D_RUN - 1) / K8D_RUN : 0;
   const size_t at = head * D + quad * 4;
-  const uint2 g = runs > 1 ? __ldg(reinterpret_cast<const uint2*>(gate + at)) : make_uint2(0u, 0u);
+  const uint2 g = head < heads ? __ldg(reinterpret_cast<const uint2*>(gate + at)) : make_uint2(0u, 0u);
   pdl_wait();
   pdl_launch();
-  if (runs <= 1) return;
+  if (head >= heads) return;
   const float2* ml = part_ml + head * n_splits;
   const float4* pa = reinterpret_cast<const float4*>(part_acc + head * n_splits * D) + quad;
   float best = -INFINITY, sum = 0.f;
@@ -724,7 +776,7 @@ kv8_combine_few_kernel(const float* part_acc, const float2* part_ml, const bf16*
       for (int k = 0; k < 4; ++k) k8d_add(best, top[k], l[k], acc[k], sum, o);
     }
   }
-  k8d_store(out + at, g, o, sum);
+  k8d_store(out + at, g, o, sum, runs > 0);
 }
 // More: a CTA takes 64 dims of a head, a thread one sum of four of them, eight of its partials under way; rows of few runs as above.
 template <int D>
@@ -741,7 +793,6 @@ kv8_combine_kernel(const float* part_acc, const float2* part_ml, const bf16* gat
   const uint2 g = __ldg(reinterpret_cast<const uint2*>(gate + at));
   pdl_wait();
   pdl_launch();
-  if (runs <= 1) return;
   const float2* ml = part_ml + head * n_splits;
   const float4* pa = reinterpret_cast<const float4*>(part_acc + head * n_splits * D + blockIdx.y * DIMS) + quad;
   if (i < K8D_SUMS) {
@@ -776,7 +827,7 @@ kv8_combine_kernel(const float* part_acc, const float2* part_ml, const bf16* gat
 #pragma unroll
   for (int k = 0; k < K8D_SUMS; ++k) best = fmaxf(best, s_top[k]);
   for (int k = 0; k < K8D_SUMS; ++k) k8d_add(best, s_top[k], s_l[k], s_acc[k][quad], sum, o);
-  k8d_store(out + at, g, o, sum);
+  k8d_store(out + at, g, o, sum, runs > 0);
 }
 
 }  // namespace b200

@@ -85,16 +85,6 @@ __device__ __forceinline__ uint32_t k8p_at(int r, int c) {
   const uint32_t byte = r * ROWB;
   return byte + ((c ^ ((byte >> 7) & (ROWB / 16 - 1))) << 4);
 }
-// Whether a barrier's phase is complete, without a wait.
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n\t.reg .pred P;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 P, [%1], %2;\n\t"
-      "selp.b32 %0, 1, 0, P;\n\t}"
-      : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-  return done != 0;
-}
 __device__ __forceinline__ float k8p_ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
