@@ -35,9 +35,22 @@ __device__ __forceinline__ uint32_t kv8_unpack2(uint16_t two) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(two));
   return r;
 }
-// For outputs that are rounded to bf16 next: the reciprocal unit's quotient, off by 2 units in the last place, and not the exact one,
-// whose subroutine took most of a prefill tile's last phase (32,000 cycles for 128 rows of 256).
-__device__ __forceinline__ float kv8_sigmoid(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
+// Two sigmoids, of the halves of a word of bf16 gates, for outputs that are rounded to bf16 next: 1 / (1 + 2^-t) with t = x log2(e), both from one
+// reciprocal, 1 / a = b / (a b). The special functions bound the end of a prefill tile (128 rows of 256: 4,096 cycles with a reciprocal
+// each, 3,072 so; an exact division took 32,000). Below t = -62 a sigmoid stays at 2^-62, so that a b is finite; a NaN stays one.
+__device__ __forceinline__ float2 kv8_sigmoid2(uint32_t gates) {
+  float a[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float x = __uint_as_float(i ? gates & 0xffff0000u : gates << 16);
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(a[i]) : "f"(x * -1.4426950408889634f), "f"(62.0f));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a[i]));
+    a[i] += 1.0f;
+  }
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a[0] * a[1]));
+  return make_float2(r * a[1], r * a[0]);
+}
 // The four bytes of a word as two pairs of halves.
 __device__ __forceinline__ void kv8_unpack4(uint32_t word, uint32_t& lo, uint32_t& hi) {
   lo = kv8_unpack2(static_cast<uint16_t>(word));
@@ -53,6 +66,19 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
       "selp.b32 %0, 1, 0, P;\n\t}"
       : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
   return done != 0;
+}
+
+// Loads under a condition that nothing waits for before their value is used (after one in a branch the compiler waits at the branch's end);
+// without it the value stays.
+__device__ __forceinline__ void ask_64(int64_t& x, const int64_t* p, bool yes) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q ld.global.nc.s64 %0, [%1];\n\t}" : "+l"(x) : "l"(p), "r"(static_cast<int>(yes)));
+}
+__device__ __forceinline__ void ask_32(uint32_t& x, const void* p, bool yes) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q ld.global.nc.u32 %0, [%1];\n\t}" : "+r"(x) : "l"(p), "r"(static_cast<int>(yes)));
+}
+__device__ __forceinline__ void ask_128(uint4& x, const void* p, bool yes) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t@q ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+               : "+r"(x.x), "+r"(x.y), "+r"(x.z), "+r"(x.w) : "l"(p), "r"(static_cast<int>(yes)));
 }
 
 }  // namespace b200

@@ -120,13 +120,6 @@ struct Kv8Unit {
   int seq, kh, z, row0, rows, keys, same;
 };
 
-// Loads that nothing waits for before their value is used; without the condition the value stays.
-__device__ __forceinline__ void ask_64(int64_t& x, const int64_t* p, bool yes) {
-  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q ld.global.nc.s64 %0, [%1];\n\t}" : "+l"(x) : "l"(p), "r"(static_cast<int>(yes)));
-}
-__device__ __forceinline__ void ask_32(uint32_t& x, const void* p, bool yes) {
-  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q ld.global.nc.u32 %0, [%1];\n\t}" : "+r"(x) : "l"(p), "r"(static_cast<int>(yes)));
-}
 __device__ __forceinline__ int kv8_length(int64_t position, int most) {
   return static_cast<int>(max(int64_t(-1), min(position, static_cast<int64_t>(most) - 1))) + 1;
 }
@@ -666,9 +659,9 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
 #pragma unroll
             for (int i = 0; i < C::PER; ++i) {
               const size_t at = head * D + (tile0 + i) * 16 + 2 * g;
+              const float2 gate = kv8_sigmoid2(gates[n8][k][i]);
               *reinterpret_cast<__nv_bfloat162*>(p.out + at) =
-                  __floats2bfloat162_rn(o[n8][i][k] * inv * kv8_sigmoid(__uint_as_float(gates[n8][k][i] << 16)),
-                                        o[n8][i][2 + k] * inv * kv8_sigmoid(__uint_as_float(gates[n8][k][i] & 0xffff0000u)));
+                  __floats2bfloat162_rn(o[n8][i][k] * inv * gate.x, o[n8][i][2 + k] * inv * gate.y);
             }
           }
         }
@@ -717,11 +710,11 @@ __device__ __forceinline__ void k8d_add(float best, float top, float l, const fl
 }
 __device__ __forceinline__ void k8d_store(bf16* out, uint2 gate, const float4& o, float sum, bool any) {
   const float inv = any ? 1.0f / sum : 0.f;  // a row without keys
-  const auto sig = [](uint32_t bits) { return kv8_sigmoid(__uint_as_float(bits)); };
+  const float2 g0 = kv8_sigmoid2(gate.x), g1 = kv8_sigmoid2(gate.y);
   uint2 raw;
   __nv_bfloat162* e = reinterpret_cast<__nv_bfloat162*>(&raw);
-  e[0] = __floats2bfloat162_rn(o.x * inv * sig(gate.x << 16), o.y * inv * sig(gate.x & 0xffff0000u));
-  e[1] = __floats2bfloat162_rn(o.z * inv * sig(gate.y << 16), o.w * inv * sig(gate.y & 0xffff0000u));
+  e[0] = __floats2bfloat162_rn(o.x * inv * g0.x, o.y * inv * g0.y);
+  e[1] = __floats2bfloat162_rn(o.z * inv * g1.x, o.w * inv * g1.y);
   *reinterpret_cast<uint2*>(out) = raw;
 }
 // Tables of up to 64 runs (16,384 keys): a thread takes all sums of four dims of a head. Its CTAs are small enough to wait beside the

@@ -170,6 +170,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
   uint64_t* const m_bar = bars + 36;                     // [2]: the row maxima up to an even / odd page
   uint64_t* const acc_done = bars + 38;
   uint64_t* const x_bar = bars + 39;
+  uint64_t* const o_full = bars + 34;                    // the outputs are in shared memory
   uint64_t* const q_ready = bars + 40;                   // the queries' terms are in shared memory, in TMEM
   uint64_t* const q_full = bars + 41;
   uint64_t* const s_empty = bars + 42;                   // [2]: the scores are in their threads' registers
@@ -201,6 +202,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
     }
     mbar_init(acc_done, 1);
     mbar_init(x_bar, 256);
+    mbar_init(o_full, 256);
     mbar_init(q_ready, K8P_THREADS - 64);
     mbar_init(q_full, 256);
     *abort_flag = 0;
@@ -216,17 +218,18 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
   pdl_launch();  // this CTA holds its TMEM columns
   const uint32_t tmem_S = tmem, tmem_O = tmem + 128, tmem_Q = tmem_O + D;  // score tile of page i at tmem_S + (i & 1) * 64
   float* const s_qs = reinterpret_cast<float*>(sP);      // until the rows' threads have read it
+  constexpr int WARPS = K8P_THREADS / 32 - 2;            // of the warps that convert queries and write outputs
+  const int w = warp < 8 ? warp : warp - 2;              // its number among them
   if (warp != 8 && warp != 9) {
     // ---- queries: a warp a row at a time, two terms of e4m3; the largest number of a row comes to [128, 256)
-    constexpr int WARPS = K8P_THREADS / 32 - 2, PER = (128 + WARPS - 1) / WARPS;
-    const int w = warp < 8 ? warp : warp - 2;
+    constexpr int PER = (128 + WARPS - 1) / WARPS;
     uint4 raw[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int r = w + i * WARPS, lp = r * p.inv_group >> 16;
       raw[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (r < 128 && lp < n_pos && lane * 8 < D)
-        raw[i] = *reinterpret_cast<const uint4*>(p.q + (static_cast<size_t>(tile.row0 + tile.p0 + lp) * p.n_q + kh * p.group + (r - lp * p.group)) * D + lane * 8);
+      ask_128(raw[i], p.q + (static_cast<size_t>(tile.row0 + tile.p0 + lp) * p.n_q + kh * p.group + (r - lp * p.group)) * D + lane * 8,
+              r < 128 && lp < n_pos && lane * 8 < D);
     }
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
@@ -259,7 +262,10 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
   }
 
   if (warp == 9) {
-    // ---------------- loads
+    // ---------------- loads. The gates are needed at the end, when other loads of this SM's neighbours are under way: they are brought to L2 now.
+    for (int i = lane; !cut && i < n_pos; i += 32)
+      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;"
+                     ::"l"(p.gate + (static_cast<size_t>(tile.row0 + tile.p0 + i) * p.n_q + kh * p.group) * D), "r"(p.group * D * 2) : "memory");
     if (elect_one()) {
       const int* table = p.tables + static_cast<size_t>(tile.seg) * p.max_pages + first;
       int next = table[0];
@@ -503,21 +509,6 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
       mbar_arrive(&t_empty[i & 3]);
     }
     float l = l2.x + l2.y;
-    // the gates of the rows that this warp will write are asked for ahead of the last products
-    constexpr int LANES = D / 8, ROWS = 32 / LANES, STEPS = 16 / ROWS;  // 8 numbers a lane, rows a warp takes at once
-    const int sub = lane / LANES, d = lane % LANES * 8, n_rows = n_pos * p.group;
-    const size_t head0 = static_cast<size_t>(tile.row0 + tile.p0) * p.n_q + kh * p.group;
-    const auto head_of = [&](int row) {
-      const int pos = row * p.inv_group >> 16;
-      return head0 + static_cast<size_t>(pos) * p.n_q + (row - pos * p.group);
-    };
-    uint4 gate[STEPS];
-#pragma unroll
-    for (int i = 0; i < STEPS; ++i) {
-      const int row = (i * 8 + warp) * ROWS + sub;
-      gate[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (!cut && row < n_rows) gate[i] = __ldg(reinterpret_cast<const uint4*>(p.gate + head_of(row) * D + d));
-    }
     ok = ok && mbar_wait(acc_done, 0, p.err, ERR_WAIT_TMEM, abort_flag) && !*abort_flag;
     tc_fence_after();
     float m_used = m_loc;
@@ -547,13 +538,30 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
       }
       if (cut && row_valid && hf == 0)
         p.part_ml[((static_cast<size_t>(tile.row0 + tile.p0 + lp) * p.n_q + kh * p.group + head)) * p.max_splits + blockIdx.z] = make_float2(m_used, l);
-      mbar_arrive(x_bar);
-      ok = mbar_wait(x_bar, 1, p.err, ERR_WAIT_FULL, abort_flag);
+      mbar_arrive(o_full);
     }
-    if (ok) {
+  }
+  if (warp != 8 && warp != 9) {
+    // ---------------- outputs, a warp whole rows at a time, their gates ahead of the last products
+    constexpr int LANES = D / 8, ROWS = 32 / LANES, STEPS = (128 + WARPS * ROWS - 1) / (WARPS * ROWS);  // 8 numbers a lane, rows a warp takes at once
+    const int sub = lane / LANES, d = lane % LANES * 8, n_rows = n_pos * p.group;
+    const size_t head0 = static_cast<size_t>(tile.row0 + tile.p0) * p.n_q + kh * p.group;
+    const auto head_of = [&](int row) {
+      const int pos = row * p.inv_group >> 16;
+      return head0 + static_cast<size_t>(pos) * p.n_q + (row - pos * p.group);
+    };
+    uint4 gate[STEPS];
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      const int row = (i * WARPS + w) * ROWS + sub;
+      gate[i] = make_uint4(0u, 0u, 0u, 0u);
+      ask_128(gate[i], p.gate + head_of(row) * D + d, !cut && row < n_rows);
+    }
+    const float* const so = reinterpret_cast<const float*>(sQ);
+    if (mbar_wait(o_full, 0, p.err, ERR_WAIT_FULL, abort_flag)) {
 #pragma unroll
       for (int i = 0; i < STEPS; ++i) {
-        const int row = (i * 8 + warp) * ROWS + sub;
+        const int row = (i * WARPS + w) * ROWS + sub;
         if (row >= n_rows) break;
         const float* const src = so + row * D;
         const float4 a = *reinterpret_cast<const float4*>(src + ((d >> 2) ^ (row & 7)) * 4), b = *reinterpret_cast<const float4*>(src + (((d >> 2) + 1) ^ (row & 7)) * 4);
@@ -563,13 +571,15 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
           *reinterpret_cast<float4*>(dst) = a;
           *reinterpret_cast<float4*>(dst + 4) = b;
         } else {
-          const uint32_t* gw = reinterpret_cast<const uint32_t*>(&gate[i]);
+          const uint32_t gw[4] = {gate[i].x, gate[i].y, gate[i].z, gate[i].w};
           const float o[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
           uint4 out;
           __nv_bfloat162* oe = reinterpret_cast<__nv_bfloat162*>(&out);
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            oe[j] = __floats2bfloat162_rn(o[2 * j] * kv8_sigmoid(__uint_as_float(gw[j] << 16)), o[2 * j + 1] * kv8_sigmoid(__uint_as_float(gw[j] & 0xffff0000u)));
+          for (int j = 0; j < 4; ++j) {
+            const float2 g = kv8_sigmoid2(gw[j]);
+            oe[j] = __floats2bfloat162_rn(o[2 * j] * g.x, o[2 * j + 1] * g.y);
+          }
           *reinterpret_cast<uint4*>(p.out + at * D + d) = out;
         }
       }
@@ -611,11 +621,12 @@ kv8_prefill_combine_kernel(Kv8PrefillParams p) {
       o.x = fmaf(v.x, f, o.x); o.y = fmaf(v.y, f, o.y); o.z = fmaf(v.z, f, o.z); o.w = fmaf(v.w, f, o.w);
     }
     const float inv = 1.0f / l;
-    const bf16* g = p.gate + at * D + quad * 4;
+    const uint2 gw = __ldg(reinterpret_cast<const uint2*>(p.gate + at * D + quad * 4));
+    const float2 g0 = kv8_sigmoid2(gw.x), g1 = kv8_sigmoid2(gw.y);
     uint2 raw;
     __nv_bfloat162* e = reinterpret_cast<__nv_bfloat162*>(&raw);
-    e[0] = __floats2bfloat162_rn(o.x * inv * kv8_sigmoid(__bfloat162float(g[0])), o.y * inv * kv8_sigmoid(__bfloat162float(g[1])));
-    e[1] = __floats2bfloat162_rn(o.z * inv * kv8_sigmoid(__bfloat162float(g[2])), o.w * inv * kv8_sigmoid(__bfloat162float(g[3])));
+    e[0] = __floats2bfloat162_rn(o.x * inv * g0.x, o.y * inv * g0.y);
+    e[1] = __floats2bfloat162_rn(o.z * inv * g1.x, o.w * inv * g1.y);
     *reinterpret_cast<uint2*>(p.out + at * D + quad * 4) = raw;
   }
 }
