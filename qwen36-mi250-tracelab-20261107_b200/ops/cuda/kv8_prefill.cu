@@ -590,45 +590,60 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
   if (warp == 8) { tc_fence_after(); tmem_dealloc(tmem, C::TMEM_COLS); }
 }
 
-// Rows of spans that were cut: their partials in the order of the runs. A CTA a tile of the kernel above, a thread four dims of a row's head at a time.
+// Rows of spans that were cut: their partials in the order of the runs, eight under way. A thread takes four dims of a row's head. What does not
+// come from the kernel in front is read ahead of the dependency wait: that kernel has waited for everything before it.
 template <int D>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(128)
 kv8_prefill_combine_kernel(Kv8PrefillParams p) {
-  constexpr int QUADS = D / 4;
-  pdl_wait();
-  pdl_launch();
-  Kv8Tile tile;
-  if (!k8p_find(p, blockIdx.x, tile)) return;
+  constexpr int QUADS = D / 4, AT_ONCE = 8;
+  Kv8Tile tile = {};
+  const bool found = k8p_find(p, blockIdx.x, tile);
   const int np = min(p.width, (tile.pos0 + tile.rows - 1) / KV8_PAGE + 1), run_pages = k8p_run_pages(tile.rows, np, p.positions, p.n_kv);
-  if (run_pages >= np) return;
-  const int n_pos = min(p.positions, tile.rows - tile.p0), heads = p.group;
+  const int n_pos = min(p.positions, tile.rows - tile.p0), i = blockIdx.z * (128 / QUADS) + threadIdx.x / QUADS;
+  const bool work = found && run_pages < np && i < n_pos * p.group;
   const int np_all = min(p.width, (tile.pos0 + tile.p0 + n_pos - 1) / KV8_PAGE + 1), runs = (np_all + run_pages - 1) / run_pages;  // that wrote
-  for (int i = blockIdx.z * (256 / QUADS) + threadIdx.x / QUADS; i < n_pos * heads; i += gridDim.z * (256 / QUADS)) {
-    const size_t at = static_cast<size_t>(tile.row0 + tile.p0 + i / heads) * p.n_q + blockIdx.y * p.group + i % heads;
-    const int quad = threadIdx.x % QUADS;
-    const float2* ml = p.part_ml + at * p.max_splits;
-    const float4* pa = reinterpret_cast<const float4*>(p.part_acc + at * p.max_splits * D) + quad;
-    float top = -INFINITY, l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-    for (int z = 0; z < runs; ++z) top = fmaxf(top, ml[z].x);
-#pragma unroll 4
-    for (int z = 0; z < runs; ++z) {
-      const float2 pm = ml[z];
-      const float4 v = pa[static_cast<size_t>(z) * QUADS];
-      const float f = pm.x == top ? 1.f : k8p_ex2(pm.x - top);
-      l = fmaf(pm.y, f, l);
-      o.x = fmaf(v.x, f, o.x); o.y = fmaf(v.y, f, o.y); o.z = fmaf(v.z, f, o.z); o.w = fmaf(v.w, f, o.w);
+  const int pos = i * p.inv_group >> 16, quad = threadIdx.x % QUADS;
+  const size_t at = static_cast<size_t>(tile.row0 + tile.p0 + pos) * p.n_q + blockIdx.y * p.group + (i - pos * p.group);
+  const uint2 gate = work ? __ldg(reinterpret_cast<const uint2*>(p.gate + at * D + quad * 4)) : make_uint2(0u, 0u);
+  pdl_wait();  // in all threads: what comes next takes this kernel's end for the end of the one in front, too
+  pdl_launch();
+  if (!work) return;
+  const float2* ml = p.part_ml + at * p.max_splits;
+  const float4* pa = reinterpret_cast<const float4*>(p.part_acc + at * p.max_splits * D) + quad;
+  float2 pm[AT_ONCE];
+  float4 v[AT_ONCE];
+  const auto ask = [&](int z0) {
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; ++k) {
+      pm[k] = z0 + k < runs ? ml[z0 + k] : make_float2(-INFINITY, 0.f);
+      v[k] = z0 + k < runs ? pa[static_cast<size_t>(z0 + k) * QUADS] : make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    const float inv = 1.0f / l;
-    const uint2 gw = __ldg(reinterpret_cast<const uint2*>(p.gate + at * D + quad * 4));
-    const float2 g0 = kv8_sigmoid2(gw.x), g1 = kv8_sigmoid2(gw.y);
-    uint2 raw;
-    __nv_bfloat162* e = reinterpret_cast<__nv_bfloat162*>(&raw);
-    e[0] = __floats2bfloat162_rn(o.x * inv * g0.x, o.y * inv * g0.y);
-    e[1] = __floats2bfloat162_rn(o.z * inv * g1.x, o.w * inv * g1.y);
-    *reinterpret_cast<uint2*>(p.out + at * D + quad * 4) = raw;
+  };
+  ask(0);
+  float top = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int z = AT_ONCE; z < runs; ++z) top = fmaxf(top, ml[z].x);
+#pragma unroll
+  for (int k = 0; k < AT_ONCE; ++k) top = fmaxf(top, pm[k].x);
+  for (int z0 = 0;;) {
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; ++k) {
+      const float f = pm[k].x == top ? 1.f : k8p_ex2(pm[k].x - top);
+      l = fmaf(pm[k].y, f, l);
+      o.x = fmaf(v[k].x, f, o.x); o.y = fmaf(v[k].y, f, o.y); o.z = fmaf(v[k].z, f, o.z); o.w = fmaf(v[k].w, f, o.w);
+    }
+    z0 += AT_ONCE;
+    if (z0 >= runs) break;
+    ask(z0);
   }
+  const float inv = 1.0f / l;
+  const float2 g0 = kv8_sigmoid2(gate.x), g1 = kv8_sigmoid2(gate.y);
+  uint2 raw;
+  __nv_bfloat162* e = reinterpret_cast<__nv_bfloat162*>(&raw);
+  e[0] = __floats2bfloat162_rn(o.x * inv * g0.x, o.y * inv * g0.y);
+  e[1] = __floats2bfloat162_rn(o.z * inv * g1.x, o.w * inv * g1.y);
+  *reinterpret_cast<uint2*>(p.out + at * D + quad * 4) = raw;
 }
 
 }  // namespace b200
@@ -663,7 +678,7 @@ int k8p_launch(const CUtensorMap& tm, const CUtensorMap& te, const Kv8PrefillPar
   }
   if (launch_pdl(kern, dim3(n_tiles, p.n_kv, p.max_splits), dim3(K8P_THREADS), Kv8PrefillCfg<D>::SMEM, st, tm, te, p) != cudaSuccess) return -4;
   if (p.max_splits == 1) return 0;
-  return launch_pdl(kv8_prefill_combine_kernel<D>, dim3(n_tiles, p.n_kv, (128 + 256 / (D / 4) - 1) / (256 / (D / 4))), dim3(256), 0, st, p) == cudaSuccess ? 0 : -4;
+  return launch_pdl(kv8_prefill_combine_kernel<D>, dim3(n_tiles, p.n_kv, 128 / (128 / (D / 4))), dim3(128), 0, st, p) == cudaSuccess ? 0 : -4;
 }
 }  // namespace
 
