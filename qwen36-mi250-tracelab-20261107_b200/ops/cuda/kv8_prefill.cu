@@ -604,8 +604,11 @@ kv8_prefill_combine_kernel(Kv8PrefillParams p) {
   const int np_all = min(p.width, (tile.pos0 + tile.p0 + n_pos - 1) / KV8_PAGE + 1), runs = (np_all + run_pages - 1) / run_pages;  // that wrote
   const int pos = i * p.inv_group >> 16, quad = threadIdx.x % QUADS;
   const size_t at = static_cast<size_t>(tile.row0 + tile.p0 + pos) * p.n_q + blockIdx.y * p.group + (i - pos * p.group);
+  // Threads without work leave before the wait, so that the grid does not come in waves behind it; those of the first CTA stay: this kernel must
+  // not end before the one in front, for whose end what comes next takes it.
+  if (!work && (blockIdx.x | blockIdx.y | blockIdx.z) != 0) return;
   const uint2 gate = work ? __ldg(reinterpret_cast<const uint2*>(p.gate + at * D + quad * 4)) : make_uint2(0u, 0u);
-  pdl_wait();  // in all threads: what comes next takes this kernel's end for the end of the one in front, too
+  pdl_wait();
   pdl_launch();
   if (!work) return;
   const float2* ml = p.part_ml + at * p.max_splits;
