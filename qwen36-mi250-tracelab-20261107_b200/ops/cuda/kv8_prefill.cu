@@ -457,6 +457,12 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
       const float m = need ? mx : m_prev;
       s_m[r] = m;
       mbar_arrive(&m_bar[hf]);
+      // This page's weights' tile was last read by the products of page i - 2. They are also the ones behind those of page i - 3, without
+      // whose end a wait for page i - 1's would take that barrier's phase before for its own and go on at once.
+      if (i >= 2) {
+        ok = mbar_wait(&pv_done[hf], ph ^ 1, p.err, ERR_WAIT_EMPTY, abort_flag);
+        if (!ok) break;
+      }
       // The output tile may only be rescaled once the products of page i - 1 have been added; those of this page and the later ones
       // wait for this page's weights.
       if (__any_sync(0xffffffffu, need) && i > 0) {  // warp-uniform: TMEM loads / stores are warp-collective
@@ -479,10 +485,6 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
         l2.x *= f;
         l2.y *= f;
         m_loc = m;
-      }
-      if (i >= 2) {  // this page's weights' tile was last read by the products of page i - 2
-        ok = mbar_wait(&pv_done[hf], ph ^ 1, p.err, ERR_WAIT_EMPTY, abort_flag);
-        if (!ok) break;
       }
       const float base = m == -INFINITY ? 0.f : K8P_LIFT - m;  // a row that sees no key of the run so far
       const float2 base2 = make_float2(base, base), one2 = make_float2(1.f, 1.f);

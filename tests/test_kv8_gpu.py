@@ -359,6 +359,22 @@ def test_prefill_rows_have_the_same_bits_beside_other_spans(C):
     C.check_errors(q.device)
 
 
+def test_prefill_of_a_full_pass(C):
+    """As many tiles as the GPU holds at a time and more, and maxima that grow page by page: outputs are rescaled while products are under way."""
+    n_q, n_kv, D, spans, n = 16, 2, 256, 8, 1024
+    layer = _layer(spans * n // 64, n_kv, D)
+    tables = torch.arange(spans * n // 64, device=DEV, dtype=torch.int32).view(spans, -1)
+    q, gate = _rows(spans * n, n_q, D, 9, scale=6.0)
+    starts = [i * n for i in range(spans + 1)]
+    got = C.kv8_prefill(q, gate, layer, tables, starts, [0] * spans)
+    for _ in range(4):
+        assert torch.equal(C.kv8_prefill(q, gate, layer, tables, starts, [0] * spans), got)
+    for i in range(spans):  # every other one of the rows in the last eight tiles
+        rows = torch.arange(i * n + n - 128, i * n + n, 2, device=DEV)
+        _check(got[rows], _attention(q[rows], gate[rows], layer, tables[i].expand(len(rows), -1), rows - i * n), i)
+    C.check_errors(q.device)
+
+
 # ------------------------------------------------------------------ how they are called
 @pytest.mark.parametrize("kind", ["decode", "prefill"])
 def test_another_stream_views_and_index_types(C, kind):
