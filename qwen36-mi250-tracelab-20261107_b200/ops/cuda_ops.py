@@ -745,6 +745,11 @@ def _raw_stream(dev: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
+def _err_ptr(dev: torch.device) -> int:
+    word = _err.get(dev.index)
+    return (word if word is not None and dev.index == torch._C._cuda_getDevice() else err_word(dev)).data_ptr()
+
+
 def _index_tables(what: str, dev: torch.device, rows: int, positions: torch.Tensor, block_tables: torch.Tensor,
                   seq_of_row: torch.Tensor | None = None):
     """The row indices in the types that the kernels read (int64 positions, int32 tables and sequences), the tables' shape and row distance."""
@@ -788,7 +793,7 @@ def kv8_write(layer: Kv8Layer, k: torch.Tensor, v: torch.Tensor, positions: torc
         vs = v.stride()
     _check(lib().b200_kv8_write(
         k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], positions.data_ptr(), seq_of_row.data_ptr(), block_tables.data_ptr(),
-        step, width, seqs, data.data_ptr(), exps.data_ptr(), T, n_kv, D, pages, err_word(dev).data_ptr(), _raw_stream(dev)), "kv8_write")
+        step, width, seqs, data.data_ptr(), exps.data_ptr(), T, n_kv, D, pages, _err_ptr(dev), _raw_stream(dev)), "kv8_write")
 
 
 def kv8_read(layer: Kv8Layer, positions: torch.Tensor, seq_of_row: torch.Tensor, block_tables: torch.Tensor):
@@ -801,7 +806,7 @@ def kv8_read(layer: Kv8Layer, positions: torch.Tensor, seq_of_row: torch.Tensor,
     v = torch.empty_like(k)
     _check(lib().b200_kv8_read(
         data.data_ptr(), exps.data_ptr(), positions.data_ptr(), seq_of_row.data_ptr(), block_tables.data_ptr(), step, width, seqs,
-        k.data_ptr(), v.data_ptr(), T, n_kv, D, pages, err_word(dev).data_ptr(), _raw_stream(dev)), "kv8_read")
+        k.data_ptr(), v.data_ptr(), T, n_kv, D, pages, _err_ptr(dev), _raw_stream(dev)), "kv8_read")
     return k, v
 
 
@@ -821,8 +826,11 @@ def _kv8_queries(what: str, q: torch.Tensor, gate: torch.Tensor, n_kv: int, D: i
         raise ValueError(f"{what}: gate {tuple(gate.shape)} {gate.dtype} is not bf16 {(rows, n_q * D)}")
     if q.device != dev or gate.device != dev:
         raise ValueError(f"{what}: the cache is on {dev}, q on {q.device}, the gate on {gate.device}")
-    q, gate = (t if t.is_contiguous() else t.contiguous() for t in (q, gate))
-    return q if q.data_ptr() % 16 == 0 else q.clone(), gate if gate.data_ptr() % 16 == 0 else gate.clone(), rows, n_q
+    if not q.is_contiguous() or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+    if not gate.is_contiguous() or gate.data_ptr() % 16:
+        gate = gate.clone(memory_format=torch.contiguous_format)
+    return q, gate, rows, n_q
 
 
 def kv8_decode(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tables: torch.Tensor, positions: torch.Tensor,
@@ -841,13 +849,14 @@ def kv8_decode(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_table
     n_splits = max(1, -(-width * PAGE_SIZE // L.b200_kv8_decode_run()))
     acc = ml = None
     if n_splits > 1:  # partials: sums, then maxima and sums of weights
-        part = torch.empty(rows * n_q * n_splits * (D + 2), dtype=torch.float32, device=dev)
-        acc = part.data_ptr()
-        ml = acc + rows * n_q * n_splits * D * 4
+        part = rows * n_q * n_splits * 4
+        scratch = data.new_empty(part * (D + 2))  # bytes: an allocation like another's takes half the time of one that names type and device
+        acc = scratch.data_ptr()
+        ml = acc + part * D
     out = torch.empty_like(gate)
     _check(L.b200_kv8_decode(
         q.data_ptr(), gate.data_ptr(), data.data_ptr(), exps.data_ptr(), positions.data_ptr(), block_tables.data_ptr(), step, width, pages,
-        rows // G, G, n_q, n_kv, D, n_splits, acc, ml, out.data_ptr(), err_word(dev).data_ptr(), _raw_stream(dev)), "kv8_decode")
+        rows // G, G, n_q, n_kv, D, n_splits, acc, ml, out.data_ptr(), _err_ptr(dev), _raw_stream(dev)), "kv8_decode")
     return out
 
 
@@ -904,12 +913,13 @@ def kv8_prefill(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tabl
         return out
     acc = ml = None
     if splits > 1:  # partials: sums, then maxima and sums of weights
-        part = torch.empty(T * n_q * splits * (D + 2), dtype=torch.float32, device=dev)
-        acc = part.data_ptr()
-        ml = acc + T * n_q * splits * D * 4
+        part = T * n_q * splits * 4
+        scratch = data.new_empty(part * (D + 2))  # bytes, as above
+        acc = scratch.data_ptr()
+        ml = acc + part * D
     _check(L.b200_kv8_prefill(
         q.data_ptr(), gate.data_ptr(), data.data_ptr(), exps.data_ptr(), starts_t.data_ptr(), pos0_t.data_ptr(), n_seg, n_tiles,
-        block_tables.data_ptr(), step, width, pages, n_q, n_kv, D, splits, acc, ml, out.data_ptr(), err_word(dev).data_ptr(),
+        block_tables.data_ptr(), step, width, pages, n_q, n_kv, D, splits, acc, ml, out.data_ptr(), _err_ptr(dev),
         _raw_stream(dev)), "kv8_prefill")
     return out
 

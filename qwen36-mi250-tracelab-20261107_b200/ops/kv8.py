@@ -65,11 +65,11 @@ class Kv8Pool:
 def check_layer(layer: Kv8Layer, what: str) -> tuple[int, int, int]:
     """``(pages, n_kv, D)`` of a layer whose parts fit each other; ``ValueError`` otherwise."""
     data, exps = layer
-    shape = data.shape
+    shape, parts = data.shape, exps.shape
     if data.dtype != torch.float8_e4m3fn or exps.dtype != torch.uint8:
         raise ValueError(f"{what}: an 8-bit KV layer holds float8_e4m3fn data and uint8 exponents, not {data.dtype} and {exps.dtype}")
-    if len(shape) != 5 or shape[1] != 2 or shape[3] != PAGE_SIZE or shape[:4] != exps.shape:
-        raise ValueError(f"{what}: data {tuple(shape)} and exponents {tuple(exps.shape)} are not [pages, 2, n_kv, {PAGE_SIZE}, D] and the same without D")
+    if len(shape) != 5 or shape[1] != 2 or shape[3] != PAGE_SIZE or parts + shape[4:] != shape:
+        raise ValueError(f"{what}: data {tuple(shape)} and exponents {tuple(parts)} are not [pages, 2, n_kv, {PAGE_SIZE}, D] and the same without D")
     if not (data.is_contiguous() and exps.is_contiguous()):
         raise ValueError(f"{what}: the parts of an 8-bit KV layer are contiguous")
     if data.device != exps.device:
