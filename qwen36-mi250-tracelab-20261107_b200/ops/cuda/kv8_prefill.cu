@@ -268,8 +268,8 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
                      ::"l"(p.gate + (static_cast<size_t>(tile.row0 + tile.p0 + i) * p.n_q + kh * p.group) * D), "r"(p.group * D * 2) : "memory");
     if (elect_one()) {
       const int* table = p.tables + static_cast<size_t>(tile.seg) * p.max_pages + first;
-      int next = table[0];
-      for (int i = 0; i < np; ++i) {
+      int next = table[0], i = 0;
+      for (; i < np; ++i) {
         const int s = i & 3, ks = i % 3;
         const uint32_t again = ((i >> 2) & 1) ^ 1;
         int page = next;
@@ -290,6 +290,18 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
 #pragma unroll
         for (int b = 0; b < C::DB; ++b)
           tma_load_2d(v_slot(s) + b * KV8_PAGE * C::ROWB, &tm, &v8_full[s], b * C::ROWB, row + p.n_kv * KV8_PAGE);
+      }
+      // after a wait that ran out: loads on their way end before the shared memory goes (a page that was begun may lack some: the limit ends that)
+      const auto land = [&](uint64_t* bar, uint32_t parity) {
+        const long long t0 = clock64();
+        while (!mbar_test(bar, parity) && clock64() - t0 < WAIT_CYCLES / 8) {}
+      };
+      if (i < np || *abort_flag) {
+        for (int k = max(0, i - 3); k <= min(i, np - 1); ++k) {
+          land(&k_full[k % 3], (k / 3) & 1);
+          land(&e_full[k & 3], (k >> 2) & 1);
+          land(&v8_full[k & 3], (k >> 2) & 1);
+        }
       }
     }
   } else if (warp == 8) {
