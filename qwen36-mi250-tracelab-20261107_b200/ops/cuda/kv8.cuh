@@ -71,13 +71,16 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
 // Loads under a condition that nothing waits for before their value is used (after one in a branch the compiler waits at the branch's end);
 // without it the value stays.
 __device__ __forceinline__ void ask_64(int64_t& x, const int64_t* p, bool yes) {
-  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q ld.global.nc.s64 %0, [%1];\n\t}" : "+l"(x) : "l"(p), "r"(static_cast<int>(yes)));
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q ld.global.s64 %0, [%1];\n\t}" : "+l"(x) : "l"(p), "r"(static_cast<int>(yes)));
 }
 __device__ __forceinline__ void ask_32(uint32_t& x, const void* p, bool yes) {
-  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q ld.global.nc.u32 %0, [%1];\n\t}" : "+r"(x) : "l"(p), "r"(static_cast<int>(yes)));
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q ld.global.u32 %0, [%1];\n\t}" : "+r"(x) : "l"(p), "r"(static_cast<int>(yes)));
+}
+__device__ __forceinline__ void ask_8(uint16_t& x, const void* p, bool yes) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q ld.global.u8 %0, [%1];\n\t}" : "+h"(x) : "l"(p), "r"(static_cast<int>(yes)));
 }
 __device__ __forceinline__ void ask_128(uint4& x, const void* p, bool yes) {
-  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t@q ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t@q ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
                : "+r"(x.x), "+r"(x.y), "+r"(x.z), "+r"(x.w) : "l"(p), "r"(static_cast<int>(yes)));
 }
 

@@ -12,27 +12,27 @@
 
 namespace b200 {
 
-// Index of a token's row in the cache (of its key; the value's is n_kv * 64 further), or -1.
-__device__ __forceinline__ long long kv8_row(int64_t pos, int seq, int kh, const int* tables, int max_pages, int width, int n_seqs,
-                                             int num_pages, int n_kv) {
-  if (pos < 0 || pos >= static_cast<int64_t>(width) * KV8_PAGE || seq < 0 || seq >= n_seqs) return -1;
-  const int page = tables[static_cast<size_t>(seq) * max_pages + pos / KV8_PAGE];
-  if (page < 0 || page >= num_pages) return -1;
-  return (static_cast<long long>(page) * 2 * n_kv + kh) * KV8_PAGE + pos % KV8_PAGE;
-}
+// Where a token's row is: its page, asked for where the indices name one (nothing waits for it here), and from it the row in the
+// cache (of the key; the value's is n_kv * 64 further).
+struct Kv8Where {
+  uint32_t page;
+  int at, kh;
+  __device__ __forceinline__ Kv8Where(int64_t pos, int seq, int kh_, const int* tables, int max_pages, int width, int n_seqs, bool real)
+      : page(0xffffffffu), at(static_cast<int>(pos & (KV8_PAGE - 1))), kh(kh_) {
+    ask_32(page, tables + static_cast<size_t>(seq) * max_pages + pos / KV8_PAGE,
+           real && pos >= 0 && pos < static_cast<int64_t>(width) * KV8_PAGE && seq >= 0 && seq < n_seqs);
+  }
+  __device__ __forceinline__ bool there(int num_pages) const { return static_cast<int>(page) >= 0 && static_cast<int>(page) < num_pages; }
+  __device__ __forceinline__ size_t row(int n_kv) const { return (static_cast<size_t>(page) * 2 * n_kv + kh) * KV8_PAGE + at; }
+};
 
 // Eight numbers of a row; ALIGNED: with one 16-byte load.
 template <bool ALIGNED>
-__device__ __forceinline__ void load8(const bf16* p, float* v) {
-  if constexpr (ALIGNED) {
-    const uint4 raw = *reinterpret_cast<const uint4*>(p);
-    const __nv_bfloat162* e = reinterpret_cast<const __nv_bfloat162*>(&raw);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { const float2 f = __bfloat1622float2(e[i]); v[2 * i] = f.x; v[2 * i + 1] = f.y; }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __bfloat162float(p[i]);
-  }
+__device__ __forceinline__ uint4 load8(const bf16* p) {
+  if constexpr (ALIGNED) return *reinterpret_cast<const uint4*>(p);
+  const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+  const auto word = [&](int i) { return static_cast<uint32_t>(h[i]) | static_cast<uint32_t>(h[i + 1]) << 16; };
+  return make_uint4(word(0), word(2), word(4), word(6));
 }
 
 template <int D, bool ALIGNED>
@@ -46,35 +46,37 @@ kv8_write_kernel(const bf16* k, long long k_row, long long k_head, const bf16* v
   const long long item = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) / LANES;  // (token, head)
   const int part = threadIdx.x % LANES;
   const bool real = item < static_cast<long long>(T) * n_kv;
-  const int row = real ? static_cast<int>(item / n_kv) : 0, kh = static_cast<int>(item % n_kv);
-  float x[2][8];
-  load8<ALIGNED>(k + row * k_row + (real ? kh : 0) * k_head + part * 8, x[0]);
-  load8<ALIGNED>(v + row * v_row + (real ? kh : 0) * v_head + part * 8, x[1]);
-  const long long at = real ? kv8_row(positions[row], seq_of_row[row], kh, tables, max_pages, width, n_seqs, num_pages, n_kv) : -1;
+  const int row = real ? static_cast<int>(item / n_kv) : 0, kh = real ? static_cast<int>(item - static_cast<long long>(row) * n_kv) : 0;
+  const int64_t pos = positions[row];
+  const int seq = seq_of_row[row];
+  const uint4 raw[2] = {load8<ALIGNED>(k + row * k_row + kh * k_head + part * 8), load8<ALIGNED>(v + row * v_row + kh * v_head + part * 8)};
+  const Kv8Where where(pos, seq, kh, tables, max_pages, width, n_seqs, real);
+  const bool there = where.there(num_pages);
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
-    float amax = 0.f, nan = 0.f;  // fmaxf passes over a NaN; a sum of zeros and NaNs keeps it
+    const uint32_t w[4] = {raw[which].x, raw[which].y, raw[which].z, raw[which].w};
+    // magnitudes of bf16 numbers are in the order of their bits, those of NaNs above all others
+    uint32_t top = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+    top = max(top & 0xffffu, top >> 16);
+    if constexpr (LANES == 32) {
+      top = __reduce_max_sync(0xffffffffu, top);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) { amax = fmaxf(amax, fabsf(x[which][i])); nan = x[which][i] != x[which][i] ? 1.f : nan; }
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) {
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-      nan = fmaxf(nan, __shfl_xor_sync(0xffffffffu, nan, o));
+      for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
     }
-    const int e = kv8_exponent(amax);
+    const bool nan = top > 0x7f80u;
+    const int e = kv8_exponent(__uint_as_float(top << 16));
     const float f = kv8_two_to(-e);
-    uint2 packed = make_uint2(0u, 0u);
-    if (nan == 0.f) {
-      packed.x = kv8_pack2(x[which][0] * f, x[which][1] * f) | kv8_pack2(x[which][2] * f, x[which][3] * f) << 16;
-      packed.y = kv8_pack2(x[which][4] * f, x[which][5] * f) | kv8_pack2(x[which][6] * f, x[which][7] * f) << 16;
-    }
-    if (at >= 0) {
-      const size_t r = static_cast<size_t>(at) + static_cast<size_t>(which) * n_kv * KV8_PAGE;
-      *reinterpret_cast<uint2*>(data + r * D + part * 8) = packed;
-      if (part == 0) exps[r] = static_cast<uint8_t>(nan == 0.f ? e + 127 : KV8_E_NAN);
+    uint32_t two[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) two[j] = kv8_pack2(__uint_as_float(w[j] << 16) * f, __uint_as_float(w[j] & 0xffff0000u) * f);
+    if (there) {
+      const size_t r = where.row(n_kv) + static_cast<size_t>(which) * n_kv * KV8_PAGE;
+      *reinterpret_cast<uint2*>(data + r * D + part * 8) = nan ? make_uint2(0u, 0u) : make_uint2(two[0] | two[1] << 16, two[2] | two[3] << 16);
+      if (part == 0) exps[r] = static_cast<uint8_t>(nan ? KV8_E_NAN : e + 127);
     }
   }
-  if (real && at < 0 && part == 0) atomicCAS(err, 0, ERR_BAD_INDEX);
+  if (real && !there && part == 0) atomicCAS(err, 0, ERR_BAD_INDEX);
 }
 
 template <int D>
@@ -87,24 +89,22 @@ kv8_read_kernel(const uint8_t* data, const uint8_t* exps, const int64_t* positio
   const long long item = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) / LANES;
   const int part = threadIdx.x % LANES;
   if (item >= static_cast<long long>(T) * n_kv) return;
-  const int row = static_cast<int>(item / n_kv), kh = static_cast<int>(item % n_kv);
-  const long long at = kv8_row(positions[row], seq_of_row[row], kh, tables, max_pages, width, n_seqs, num_pages, n_kv);
+  const int row = static_cast<int>(item / n_kv), kh = static_cast<int>(item - static_cast<long long>(row) * n_kv);
+  const Kv8Where where(positions[row], seq_of_row[row], kh, tables, max_pages, width, n_seqs, true);
+  const bool there = where.there(num_pages);
   uint4 raw[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
-  uint32_t byte[2] = {127u, 127u};
-  if (at >= 0) {
+  uint16_t byte[2] = {127, 127};
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      const size_t r = static_cast<size_t>(at) + static_cast<size_t>(which) * n_kv * KV8_PAGE;
-      raw[which] = *reinterpret_cast<const uint4*>(data + r * D + part * 16);
-      byte[which] = exps[r];
-    }
-  } else if (part == 0) {
-    atomicCAS(err, 0, ERR_BAD_INDEX);
+  for (int which = 0; which < 2; ++which) {
+    const size_t r = where.row(n_kv) + static_cast<size_t>(which) * n_kv * KV8_PAGE;
+    ask_128(raw[which], data + r * D + part * 16, there);
+    ask_8(byte[which], exps + r, there);
   }
+  if (!there && part == 0) atomicCAS(err, 0, ERR_BAD_INDEX);
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     const float f = kv8_factor(byte[which]);
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[which]);
+    const uint32_t w[4] = {raw[which].x, raw[which].y, raw[which].z, raw[which].w};
     uint4 out[2];
     __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(out);
 #pragma unroll

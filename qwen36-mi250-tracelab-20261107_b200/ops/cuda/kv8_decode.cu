@@ -124,7 +124,7 @@ __device__ __forceinline__ int kv8_length(int64_t position, int most) {
   return static_cast<int>(max(int64_t(-1), min(position, static_cast<int64_t>(most) - 1))) + 1;
 }
 __device__ __forceinline__ int kv8_length(const int64_t* positions, int row, int most) {
-  return kv8_length(__ldg(positions + row), most);
+  return kv8_length(positions[row], most);
 }
 
 template <int D, int NT>
@@ -315,7 +315,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
         const bf16* src = p.q + (static_cast<size_t>(u.row0 + min(row, u.rows - 1)) * p.n_q + u.kh * p.group + head) * D + lane * 4 % D;
 #pragma unroll
         for (int k = 0; k < DI; ++k)
-          asm volatile("ld.global.nc.v2.u32 {%0, %1}, [%2];" : "=r"(raw[i][k].x), "=r"(raw[i][k].y) : "l"(src + k * 128));
+          asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(raw[i][k].x), "=r"(raw[i][k].y) : "l"(src + k * 128));
       }
     };
     // A unit's description; its queries are fetched one unit ahead. Either all these warps have it or none goes on: each stays in
@@ -728,7 +728,7 @@ kv8_combine_few_kernel(const float* part_acc, const float2* part_ml, const bf16*
   const int quad = threadIdx.x % QUADS;
   const int runs = head < heads ? (kv8_length(positions, static_cast<int>(head / n_q), most) + K8D_RUN - 1) / K8D_RUN : 0;
   const size_t at = head * D + quad * 4;
-  const uint2 g = head < heads ? __ldg(reinterpret_cast<const uint2*>(gate + at)) : make_uint2(0u, 0u);
+  const uint2 g = head < heads ? *reinterpret_cast<const uint2*>(gate + at) : make_uint2(0u, 0u);
   pdl_wait();
   pdl_launch();
   if (head >= heads) return;
@@ -783,7 +783,7 @@ kv8_combine_kernel(const float* part_acc, const float2* part_ml, const bf16* gat
   const int quad = threadIdx.x % QUADS, i = threadIdx.x / QUADS;
   const int runs = (kv8_length(positions, static_cast<int>(head / n_q), most) + K8D_RUN - 1) / K8D_RUN;
   const size_t at = head * D + blockIdx.y * DIMS + quad * 4;
-  const uint2 g = __ldg(reinterpret_cast<const uint2*>(gate + at));
+  const uint2 g = *reinterpret_cast<const uint2*>(gate + at);
   pdl_wait();
   pdl_launch();
   const float2* ml = part_ml + head * n_splits;

@@ -621,7 +621,7 @@ kv8_prefill_combine_kernel(Kv8PrefillParams p) {
   // Threads without work leave before the wait, so that the grid does not come in waves behind it; those of the first CTA stay: this kernel must
   // not end before the one in front, for whose end what comes next takes it.
   if (!work && (blockIdx.x | blockIdx.y | blockIdx.z) != 0) return;
-  const uint2 gate = work ? __ldg(reinterpret_cast<const uint2*>(p.gate + at * D + quad * 4)) : make_uint2(0u, 0u);
+  const uint2 gate = work ? *reinterpret_cast<const uint2*>(p.gate + at * D + quad * 4) : make_uint2(0u, 0u);
   pdl_wait();
   pdl_launch();
   if (!work) return;
