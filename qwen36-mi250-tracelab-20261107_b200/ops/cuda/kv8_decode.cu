@@ -23,7 +23,10 @@ namespace b200 {
 constexpr int K8D_RUN = 256;                    // keys of a run: part of the numerics
 constexpr int K8D_SLAB = 16;                    // keys of a warp's scores
 constexpr int K8D_SLABS = KV8_PAGE / K8D_SLAB;  // of a page: a warp each
-constexpr int K8D_SEQS = 512;                   // of one launch
+constexpr int K8D_OUT = 4;                      // warps that take outputs
+constexpr int K8D_THREADS = 32 * (K8D_SLABS + K8D_OUT + 1);
+constexpr int K8D_CTAS = 2;                     // per SM
+constexpr int K8D_SEQS = 256;                   // of one launch
 constexpr int K8D_UNITS = 8;                    // descriptions of runs that are kept
 constexpr int K8D_PAGES = K8D_RUN / KV8_PAGE;   // of a run
 constexpr float K8D_LIFT = 7.0f;                // weights are 2^LIFT at the maximum: halves reach down to 2^-24
@@ -40,7 +43,7 @@ struct Kv8DecodeParams {
   float2* part_ml;           // [rows, n_q, n_splits]: maximum (log 2) and sum
   int B, G, max_pages, width, num_pages, n_q, n_kv, group, n_splits;
   int rows_per_unit, units_per_seq;  // query rows whose heads fill a unit's columns; units that cover G rows
-  int inv_group;             // column * inv_group >> 16 is column / group, for columns up to 32 of groups up to 16
+  int inv_group;             // column * inv_group >> 16 is column / group, for columns up to 16 of groups up to 16
   float scale_log2;
   int* err;
 };
@@ -50,18 +53,10 @@ struct Kv8DecodeCfg {
   static constexpr int ROWB = D < 128 ? D : 128;           // bytes of a row in one swizzled block
   static constexpr int DB = D / ROWB;
   static constexpr int TILE = KV8_PAGE * D;                // a page's keys or values: a slot of their ring
-  static constexpr int CTAS = NT == 1 ? 2 : 1;             // per SM: one column tile's registers leave room for two
-  static constexpr int SLOTS = (D == 256 ? 3 : D == 128 ? 6 : 8) * (D == 256 && NT > 1 ? 2 : 1);
+  static constexpr int SLOTS = D == 256 ? 3 : D == 128 ? 6 : 8;
   static constexpr int EXPS = 2 * KV8_PAGE;                // exponents of a page's keys and values, with its keys
   static constexpr int SMEM = SLOTS * (2 * TILE + EXPS);
-  static constexpr int HALVES = NT > 1 ? 2 : 1;            // groups of four warps that take scores, each of a part of the columns
-  static constexpr int NA = NT / HALVES;                   // column tiles of a group
-  static constexpr int SW = HALVES * K8D_SLABS;            // warps that take scores
-  static constexpr int OW = NT > 1 && D >= 128 ? 8 : 4;    // warps that take outputs (SPLIT is the same for all NT: part of the numerics)
-  static constexpr int THREADS = 32 * (SW + OW + 1);
-  static constexpr int TILES = D / 16;                     // output tiles of 16 dims
-  static constexpr int PER = TILES > OW ? TILES / OW : 1;  // of a warp
-  static constexpr int SPLIT = TILES < OW ? OW / TILES : 1;  // warps that share a tile, a part of the keys each
+  static constexpr int PER = D / 16 / K8D_OUT;             // output tiles of 16 dims of a warp
 };
 
 __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t* r) {
@@ -82,15 +77,15 @@ __device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // Barriers of the warps that take scores; all of them come to each one, whatever they have to do there.
-__device__ __forceinline__ void meet_scores(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(32 * K8D_SLABS) : "memory"); }
-__device__ __forceinline__ bool meet_scores_or(int id, bool mine) {
+__device__ __forceinline__ void meet_scores() { asm volatile("bar.sync 1, %0;" ::"n"(32 * K8D_SLABS) : "memory"); }
+__device__ __forceinline__ bool meet_scores_or(bool mine) {
   uint32_t any;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %1, 0;\n\t"
-      "bar.red.or.pred q, %2, %3, p;\n\t"
+      "bar.red.or.pred q, 1, %2, p;\n\t"
       "selp.b32 %0, 1, 0, q;\n\t}"
-      : "=r"(any) : "r"(static_cast<uint32_t>(mine)), "r"(id), "n"(32 * K8D_SLABS) : "memory");
+      : "=r"(any) : "r"(static_cast<uint32_t>(mine)), "n"(32 * K8D_SLABS) : "memory");
   return any != 0;
 }
 __device__ __forceinline__ float ex2(float x) {
@@ -105,7 +100,8 @@ __device__ __forceinline__ bool wait_seen(bool seen, uint64_t* bar, uint32_t par
 }
 
 // Sequence b whose part [first[b], first[b + 1]) holds x.
-__device__ __forceinline__ int kv8_find(const int* first, int B, int x) {
+template <class T>
+__device__ __forceinline__ int kv8_find(const T* first, int B, int x) {
   int lo = 0, hi = B;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -128,10 +124,10 @@ __device__ __forceinline__ int kv8_length(const int64_t* positions, int row, int
 }
 
 template <int D, int NT>
-__global__ void __maxnreg__(96)  // two CTAs of 9 warps or one of 17: five warps of a quarter SM
+__global__ void __maxnreg__(96)  // two CTAs of 9 warps: five of a quarter SM at the most
 kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtensorMap tm_exps, Kv8DecodeParams p) {
   using C = Kv8DecodeCfg<D, NT>;
-  constexpr int SLOTS = C::SLOTS, CHUNKS = D / 16, COLS = 8 * NT, DI = (D + 127) / 128, SLABS = K8D_SLABS, NA = C::NA;
+  constexpr int SLOTS = C::SLOTS, CHUNKS = D / 16, COLS = 8 * NT, DI = (D + 127) / 128, SLABS = K8D_SLABS;
   extern __shared__ __align__(1024) uint8_t smem_k8[];
   if (smem_u32(smem_k8) & 1023u) {  // the swizzled tiles need this alignment
     if (threadIdx.x == 0) atomicCAS(p.err, 0, ERR_BAD_INDEX);
@@ -144,26 +140,26 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
   __shared__ __align__(8) uint64_t w_full[2], w_empty[2];   // weights of an even / odd page
   __shared__ __align__(8) uint64_t u_full[K8D_UNITS], u_empty[K8D_UNITS];
   __shared__ __align__(8) uint64_t l_full[2], l_empty[2];   // sums of an even / odd unit
-  __shared__ int s_first[K8D_SEQS + 1], s_tail[K8D_SEQS + 1];  // full runs of the sequences before; last runs that are not full, likewise
+  __shared__ int s_first[K8D_SEQS + 1];                // full runs of the sequences before
+  __shared__ uint16_t s_tail[K8D_SEQS + 1];            // last runs that are not full, likewise
   __shared__ Kv8Unit s_unit[K8D_UNITS];
-  __shared__ int s_len[K8D_UNITS][32];                 // keys of the unit's rows
-  __shared__ int s_scaled[2][C::HALVES];
+  __shared__ int s_len[K8D_UNITS][COLS];               // keys of the unit's rows
+  __shared__ int s_scaled[2];
   __shared__ __align__(16) float s_max[SLABS][COLS], s_factor[2][COLS];   // read two columns at a time
   __shared__ float s_sum[2][SLABS][COLS], s_top[2][COLS], s_scale[COLS];
   __shared__ __align__(8) uint2 s_w[2][SLABS][NT][32]; // weights of a page, as the products' second operand
   __shared__ __align__(8) uint2 s_q[NT][CHUNKS][32];   // queries, likewise
-  __shared__ float s_o[2][C::SPLIT > 1 ? C::OW : 1][C::SPLIT > 1 ? NT * 4 : 1][32];
   __shared__ int s_abort;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   volatile int* abort_flag = &s_abort;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < SLOTS; ++i) { mbar_init(&k_full[i], 1); mbar_init(&v_full[i], 1); mbar_init(&k_empty[i], C::HALVES); mbar_init(&v_empty[i], C::OW); }
+    for (int i = 0; i < SLOTS; ++i) { mbar_init(&k_full[i], 1); mbar_init(&v_full[i], 1); mbar_init(&k_empty[i], 1); mbar_init(&v_empty[i], K8D_OUT); }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&w_full[i], C::SW); mbar_init(&w_empty[i], C::OW);
-      mbar_init(&l_full[i], C::SPLIT > 1 ? C::SW + C::OW : C::SW); mbar_init(&l_empty[i], C::OW);
+      mbar_init(&w_full[i], SLABS); mbar_init(&w_empty[i], K8D_OUT);
+      mbar_init(&l_full[i], SLABS); mbar_init(&l_empty[i], K8D_OUT);
     }
-    for (int i = 0; i < K8D_UNITS; ++i) { mbar_init(&u_full[i], 1); mbar_init(&u_empty[i], C::SW + C::OW); }
+    for (int i = 0; i < K8D_UNITS; ++i) { mbar_init(&u_full[i], 1); mbar_init(&u_empty[i], SLABS + K8D_OUT); }
     s_abort = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tm);
@@ -174,7 +170,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
   pdl_launch();
   const int most = min(p.width, p.n_splits * (K8D_RUN / KV8_PAGE)) * KV8_PAGE;  // keys that the tables can name
 
-  if (warp == C::SW + C::OW) {
+  if (warp == SLABS + K8D_OUT) {
     // ---------------- loads. The units are the runs of all sequences. Those of RUN keys are dealt out first, in one piece to each CTA, so that most follow
     // one of the same queries; what is left of each sequence goes round, beginning with the CTAs that got a unit less. Once the pages are on
     // their way any other load waits behind some 30 MB of them, 4 us: what a unit needs to know is asked for two units ahead, and published one ahead.
@@ -246,7 +242,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
       const int len = kv8_length(a.position, most);
       a.u.keys = max(0, min(K8D_RUN, __reduce_max_sync(0xffffffffu, len) - a.u.z * K8D_RUN));
       ok = ok && mbar_wait_warp(&u_empty[us], ((j / K8D_UNITS) & 1) ^ 1, p.err, ERR_WAIT_EMPTY, abort_flag);
-      if (ok) s_len[us][lane] = len;
+      if (ok && lane < COLS) s_len[us][lane] = len;
       __syncwarp();
       if (ok && lane == 0) { s_unit[us] = a.u; mbar_arrive(&u_full[us]); }
     };
@@ -301,16 +297,16 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
   bool ok = true;
   int n = 0;  // pages so far
 
-  if (warp < C::SW) {
+  if (warp < SLABS) {
     // ---------------- scores, maxima and weights: slab of keys, tiles of columns
-    const int slab = warp % SLABS, tile = warp / SLABS * NA, bar = 1 + warp / SLABS;
-    constexpr int QC = 8 * NA / SLABS;  // query columns that a warp prepares
+    const int slab = warp;
+    constexpr int QC = COLS / SLABS;  // query columns that a warp prepares
     uint2 raw[QC][DI];
     const auto fetch = [&](const Kv8Unit& u) {
 #pragma unroll
       for (int i = 0; i < QC; ++i) {
         int row, head;
-        column(tile * 8 + slab * QC + i, row, head);
+        column(slab * QC + i, row, head);
         // a column without a row takes the last one's: nothing reads what comes of it. No condition on the load, so that nothing waits for it here.
         const bf16* src = p.q + (static_cast<size_t>(u.row0 + min(row, u.rows - 1)) * p.n_q + u.kh * p.group + head) * D + lane * 4 % D;
 #pragma unroll
@@ -323,26 +319,26 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
     bool known = false;
     const auto enter = [&](int j) {
       ok = ok && mbar_wait_warp(&u_full[j % K8D_UNITS], (j / K8D_UNITS) & 1, p.err, ERR_WAIT_FULL, abort_flag);
-      known = ok = !meet_scores_or(bar, !ok);
+      known = ok = !meet_scores_or(!ok);
       if (!known) return;
       const Kv8Unit u = s_unit[j % K8D_UNITS];
       known = u.rows > 0;
       if (known && !u.same) fetch(u);
     };
-    uint2 qf[CHUNKS];      // queries of the first column tile; a second one's are read at each use
-    float qscale[NA][2];   // what takes the product to log-2 scores
+    uint2 qf[NT == 1 ? CHUNKS : 1];  // queries of the column tile; those of two are read at each use
+    float qscale[NT][2];   // what takes the product to log-2 scores
     enter(0);
     const auto keys_here = [&](int i) { return mbar_test(&k_full[i % SLOTS], (i / SLOTS) & 1); };
     for (int j = 0; known; ++j) {
       const int us = j % K8D_UNITS;
       const Kv8Unit u = s_unit[us];
-      int last[NA][2];  // columns 2 t, 2 t + 1: last visible key of the run
+      int last[NT][2];  // columns 2 t, 2 t + 1: last visible key of the run
 #pragma unroll
-      for (int n8 = 0; n8 < NA; ++n8)
+      for (int n8 = 0; n8 < NT; ++n8)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           int row, head;
-          column((tile + n8) * 8 + 2 * t + k, row, head);
+          column(n8 * 8 + 2 * t + k, row, head);
           last[n8][k] = s_len[us][row] - 1 - u.z * K8D_RUN;
         }
       if (!u.same) {
@@ -350,7 +346,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
         // (column % 8, t) holds dims 16 c + 4 t .. + 3 of chunk c
 #pragma unroll
         for (int i = 0; i < QC; ++i) {
-          const int col = tile * 8 + slab * QC + i;
+          const int col = slab * QC + i;
           float x[DI][4];
           float top = 0.f;
           bool bad = false;
@@ -376,19 +372,19 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
           const bool any = __any_sync(0xffffffffu, bad);
           if (lane == 0) s_scale[col] = any ? __uint_as_float(0x7fffffffu) : kv8_two_to(e) * p.scale_log2;
         }
-        meet_scores(bar);
+        meet_scores();
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) qf[c] = s_q[tile][c][lane];
+        for (int c = 0; c < (NT == 1 ? CHUNKS : 0); ++c) qf[c] = s_q[0][c][lane];
 #pragma unroll
-        for (int n8 = 0; n8 < NA; ++n8)
+        for (int n8 = 0; n8 < NT; ++n8)
 #pragma unroll
-          for (int k = 0; k < 2; ++k) qscale[n8][k] = s_scale[(tile + n8) * 8 + 2 * t + k];
+          for (int k = 0; k < 2; ++k) qscale[n8][k] = s_scale[n8 * 8 + 2 * t + k];
       }
       enter(j + 1);
       bool k_seen = keys_here(n);  // barriers are looked at ahead of their wait, which takes its time even where there is none
-      float m[NA][2], l[NA][2];
+      float m[NT][2], l[NT][2];
 #pragma unroll
-      for (int n8 = 0; n8 < NA; ++n8) {
+      for (int n8 = 0; n8 < NT; ++n8) {
         m[n8][0] = m[n8][1] = -INFINITY;
         l[n8][0] = l[n8][1] = 0.f;
       }
@@ -399,13 +395,13 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
         const bool w_seen = mbar_test(&w_empty[half], ((n >> 1) & 1) ^ 1);
         ok = ok && wait_seen(k_seen, &k_full[s], (n / SLOTS) & 1, p.err, ERR_WAIT_FULL, abort_flag);
         // S[key, column], keys g and g + 8 of this warp's slab
-        float y[NA][2][2];  // [key][column 2 t, 2 t + 1]
+        float y[NT][2][2];  // [key][column 2 t, 2 t + 1]
         float vi[2];
         bool grown = false;
         if (ok && mine) {
-          float sc[NA][2][4];  // two chains of products
+          float sc[NT][2][4];  // two chains of products
 #pragma unroll
-          for (int n8 = 0; n8 < NA; ++n8)
+          for (int n8 = 0; n8 < NT; ++n8)
 #pragma unroll
             for (int k = 0; k < 4; ++k) sc[n8][0][k] = sc[n8][1][k] = 0.f;
           const uint32_t ktile = smem_u32(s_k + s * C::TILE);
@@ -419,8 +415,8 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
               kv8_unpack4(r[2 * h], a0, a2);
               kv8_unpack4(r[2 * h + 1], a1, a3);
 #pragma unroll
-              for (int n8 = 0; n8 < NA; ++n8) {
-                const uint2 b = n8 == 0 ? qf[c + h] : s_q[tile + n8][c + h][lane];
+              for (int n8 = 0; n8 < NT; ++n8) {
+                const uint2 b = NT == 1 ? qf[NT == 1 ? c + h : 0] : s_q[n8][c + h][lane];
                 mma_f16(sc[n8][h], a0, a1, a2, a3, b.x, b.y);
               }
             }
@@ -436,7 +432,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
           }
           const int key = key0 + slab * K8D_SLAB + g;
 #pragma unroll
-          for (int n8 = 0; n8 < NA; ++n8)
+          for (int n8 = 0; n8 < NT; ++n8)
 #pragma unroll
             for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -447,42 +443,42 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
               }
         }
         // a column whose maximum grew far enough takes the page's, which all warps see alike
-        const bool any = meet_scores_or(bar, grown);
+        const bool any = meet_scores_or(grown);
         if (slab == 0 && lane == 0) mbar_arrive(&k_empty[s]);  // the group has read the keys
         if (any) {
 #pragma unroll
-          for (int n8 = 0; n8 < NA; ++n8)
+          for (int n8 = 0; n8 < NT; ++n8)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
               float mx = ok && mine ? fmaxf(y[n8][0][k], y[n8][1][k]) : -INFINITY;
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-              if (g == 0) s_max[slab][(tile + n8) * 8 + 2 * t + k] = mx;
+              if (g == 0) s_max[slab][n8 * 8 + 2 * t + k] = mx;
             }
-          meet_scores(bar);
+          meet_scores();
         }
         k_seen = keys_here(n + 1);
         ok = ok && wait_seen(w_seen, &w_empty[half], ((n >> 1) & 1) ^ 1, p.err, ERR_WAIT_EMPTY, abort_flag);
         if (any) {
 #pragma unroll
-          for (int n8 = 0; n8 < NA; ++n8) {
+          for (int n8 = 0; n8 < NT; ++n8) {
             float2 top = make_float2(-INFINITY, -INFINITY), f = make_float2(1.f, 1.f);
 #pragma unroll
             for (int w = 0; w < SLABS; ++w) {
-              const float2 v = *reinterpret_cast<const float2*>(&s_max[w][(tile + n8) * 8 + 2 * t]);
+              const float2 v = *reinterpret_cast<const float2*>(&s_max[w][n8 * 8 + 2 * t]);
               top.x = fmaxf(top.x, v.x);
               top.y = fmaxf(top.y, v.y);
             }
             if (top.x > m[n8][0] + K8D_LAZY) { f.x = ex2(m[n8][0] - top.x); m[n8][0] = top.x; l[n8][0] *= f.x; }  // 0 at the first key
             if (top.y > m[n8][1] + K8D_LAZY) { f.y = ex2(m[n8][1] - top.y); m[n8][1] = top.y; l[n8][1] *= f.y; }
-            if (slab == 0 && g == 0) *reinterpret_cast<float2*>(&s_factor[half][(tile + n8) * 8 + 2 * t]) = f;
+            if (slab == 0 && g == 0) *reinterpret_cast<float2*>(&s_factor[half][n8 * 8 + 2 * t]) = f;
           }
         }
-        if (slab == 0 && lane == 0) s_scaled[half][warp / SLABS] = any;
+        if (slab == 0 && lane == 0) s_scaled[half] = any;
         if (ok && mine) {
 #pragma unroll
-          for (int n8 = 0; n8 < NA; ++n8) {
+          for (int n8 = 0; n8 < NT; ++n8) {
             float w[2][2];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
@@ -499,7 +495,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
               const __half2 two = __floats2half2_rn(w[i][0], w[i][1]);
               pw[i] = movmatrix(*reinterpret_cast<const uint32_t*>(&two));  // [column g][keys 2 t, 2 t + 1]
             }
-            s_w[half][slab][tile + n8][lane] = make_uint2(pw[0], pw[1]);
+            s_w[half][slab][n8][lane] = make_uint2(pw[0], pw[1]);
           }
         }
         sync_arrive(&w_full[half]);
@@ -509,7 +505,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
       const int half = j & 1;
       ok = ok && mbar_wait_warp(&l_empty[half], ((j >> 1) & 1) ^ 1, p.err, ERR_WAIT_EMPTY, abort_flag);
 #pragma unroll
-      for (int n8 = 0; n8 < NA; ++n8)
+      for (int n8 = 0; n8 < NT; ++n8)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           float sum = l[n8][k];
@@ -517,8 +513,8 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
           sum += __shfl_xor_sync(0xffffffffu, sum, 8);
           sum += __shfl_xor_sync(0xffffffffu, sum, 16);
           if (g == 0) {
-            s_sum[half][slab][(tile + n8) * 8 + 2 * t + k] = sum;
-            if (slab == 0) s_top[half][(tile + n8) * 8 + 2 * t + k] = m[n8][k];
+            s_sum[half][slab][n8 * 8 + 2 * t + k] = sum;
+            if (slab == 0) s_top[half][n8 * 8 + 2 * t + k] = m[n8][k];
           }
         }
       __syncwarp();
@@ -528,7 +524,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
   }
 
   // ---------------- outputs: O[dim, column], dims 16 c + 2 g and + 1 of tile c are the rows g and g + 8
-  const int ow = warp - C::SW, tile0 = ow % C::TILES * C::PER, part = ow / C::TILES;  // this warp's tiles, and which part of the keys
+  const int tile0 = (warp - SLABS) * C::PER;  // this warp's tiles
   for (int j = 0;; ++j) {
     const int us = j % K8D_UNITS;
     ok = ok && mbar_wait_warp(&u_full[us], (j / K8D_UNITS) & 1, p.err, ERR_WAIT_FULL, abort_flag);
@@ -562,11 +558,9 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
       ok = ok && mbar_wait_warp(&v_full[s], (n / SLOTS) & 1, p.err, ERR_WAIT_FULL, abort_flag)
            && mbar_wait_warp(&w_full[half], (n >> 1) & 1, p.err, ERR_WAIT_FULL, abort_flag);
       if (!ok) break;
+      if (s_scaled[half]) {
 #pragma unroll
-      for (int h = 0; h < C::HALVES; ++h) {
-        if (!s_scaled[half][h]) continue;
-#pragma unroll
-        for (int n8 = h * NA; n8 < h * NA + NA; ++n8) {
+        for (int n8 = 0; n8 < NT; ++n8) {
           const float2 f = *reinterpret_cast<const float2*>(&s_factor[half][n8 * 8 + 2 * t]);
 #pragma unroll
           for (int i = 0; i < C::PER; ++i) { o[n8][i][0] *= f.x; o[n8][i][1] *= f.y; o[n8][i][2] *= f.x; o[n8][i][3] *= f.y; }
@@ -597,75 +591,55 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
         }
       } else {  // a tile and two slabs per load
 #pragma unroll
-        for (int k = 0; k < SLABS / C::SPLIT; k += 2) {
-          const int slab = part * (SLABS / C::SPLIT) + k;
+        for (int slab = 0; slab < SLABS; slab += 2) {
           if (slab >= slabs) break;
           uint32_t r[4];
           ldmatrix4_trans(tile_at(vtile, slab * K8D_SLAB + lane, tile0), r);
           product(&o[0][0], 1, r, slab);
-          if (SLABS / C::SPLIT > 1 && slab + 1 < slabs) product(&o[0][0], 1, r + 2, slab + 1);
+          if (slab + 1 < slabs) product(&o[0][0], 1, r + 2, slab + 1);
         }
       }
       __syncwarp();
       if (lane == 0) { mbar_arrive(&v_empty[s]); mbar_arrive(&w_empty[half]); }
     }
 
-    // where warps share a tile, their outputs meet at the barrier of the sums
     const int half = j & 1;
-    if constexpr (C::SPLIT > 1) {
-      ok = ok && mbar_wait_warp(&l_empty[half], ((j >> 1) & 1) ^ 1, p.err, ERR_WAIT_EMPTY, abort_flag);
-#pragma unroll
-      for (int n8 = 0; n8 < NT; ++n8)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s_o[half][ow][n8 * 4 + i][lane] = o[n8][0][i];
-      sync_arrive(&l_full[half]);
-    }
     ok = ok && mbar_wait_warp(&l_full[half], (j >> 1) & 1, p.err, ERR_WAIT_FULL, abort_flag);
     if (!ok) break;
-    if constexpr (C::SPLIT > 1) {
 #pragma unroll
-      for (int n8 = 0; n8 < NT; ++n8)
+    for (int n8 = 0; n8 < NT; ++n8)
 #pragma unroll
-        for (int w = 1; w < C::SPLIT; ++w)
+      for (int k = 0; k < 2; ++k) {
+        int r, h;
+        column(n8 * 8 + 2 * t + k, r, h);
+        if (r >= u.rows) continue;
+        const int len = s_len[us][r];
+        const size_t head = static_cast<size_t>(u.row0 + r) * p.n_q + u.kh * p.group + h;
+        const auto sum = [&] {
+          float x = 0.f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[n8][0][i] += part == 0 ? s_o[half][w * C::TILES + ow][n8 * 4 + i][lane] : 0.f;
-    }
-    if (part == 0) {
+          for (int w = 0; w < SLABS; ++w) x += s_sum[half][w][n8 * 8 + 2 * t + k];
+          return x;
+        };
+        if (p.n_splits > 1) {
+          if (u.z * K8D_RUN < len) {
+            const size_t slot = head * p.n_splits + u.z;
+            if (tile0 == 0 && g == 0) p.part_ml[slot] = make_float2(s_top[half][n8 * 8 + 2 * t + k], sum());
 #pragma unroll
-      for (int n8 = 0; n8 < NT; ++n8)
+            for (int i = 0; i < C::PER; ++i)
+              *reinterpret_cast<float2*>(p.part_acc + slot * D + (tile0 + i) * 16 + 2 * g) = make_float2(o[n8][i][k], o[n8][i][2 + k]);
+          }
+        } else {
+          const float inv = len > 0 ? 1.0f / sum() : 0.f;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          int r, h;
-          column(n8 * 8 + 2 * t + k, r, h);
-          if (r >= u.rows) continue;
-          const int len = s_len[us][r];
-          const size_t head = static_cast<size_t>(u.row0 + r) * p.n_q + u.kh * p.group + h;
-          const auto sum = [&] {
-            float x = 0.f;
-#pragma unroll
-            for (int w = 0; w < SLABS; ++w) x += s_sum[half][w][n8 * 8 + 2 * t + k];
-            return x;
-          };
-          if (p.n_splits > 1) {
-            if (u.z * K8D_RUN < len) {
-              const size_t slot = head * p.n_splits + u.z;
-              if (tile0 == 0 && g == 0) p.part_ml[slot] = make_float2(s_top[half][n8 * 8 + 2 * t + k], sum());
-#pragma unroll
-              for (int i = 0; i < C::PER; ++i)
-                *reinterpret_cast<float2*>(p.part_acc + slot * D + (tile0 + i) * 16 + 2 * g) = make_float2(o[n8][i][k], o[n8][i][2 + k]);
-            }
-          } else {
-            const float inv = len > 0 ? 1.0f / sum() : 0.f;
-#pragma unroll
-            for (int i = 0; i < C::PER; ++i) {
-              const size_t at = head * D + (tile0 + i) * 16 + 2 * g;
-              const float2 gate = kv8_sigmoid2(gates[n8][k][i]);
-              *reinterpret_cast<__nv_bfloat162*>(p.out + at) =
-                  __floats2bfloat162_rn(o[n8][i][k] * inv * gate.x, o[n8][i][2 + k] * inv * gate.y);
-            }
+          for (int i = 0; i < C::PER; ++i) {
+            const size_t at = head * D + (tile0 + i) * 16 + 2 * g;
+            const float2 gate = kv8_sigmoid2(gates[n8][k][i]);
+            *reinterpret_cast<__nv_bfloat162*>(p.out + at) =
+                __floats2bfloat162_rn(o[n8][i][k] * inv * gate.x, o[n8][i][2 + k] * inv * gate.y);
           }
         }
-    }
+      }
     __syncwarp();
     if (lane == 0) { mbar_arrive(&l_empty[half]); mbar_arrive(&u_empty[us]); }
   }
@@ -869,9 +843,9 @@ int k8d_launch(const CUtensorMap& tm, const CUtensorMap& tm_exps, const Kv8Decod
     sms_of[dev] = sms;
   }
   const long long units = static_cast<long long>(p.B) * p.units_per_seq * p.n_kv * p.n_splits;
-  const int most_ctas = sms_of[dev] * Kv8DecodeCfg<D, NT>::CTAS;
+  const int most_ctas = sms_of[dev] * K8D_CTAS;
   const int grid = static_cast<int>(units < most_ctas ? units : most_ctas);
-  if (launch_pdl(kern, dim3(grid), dim3(Kv8DecodeCfg<D, NT>::THREADS), Kv8DecodeCfg<D, NT>::SMEM, st, tm, tm_exps, p) != cudaSuccess) return -4;
+  if (launch_pdl(kern, dim3(grid), dim3(K8D_THREADS), Kv8DecodeCfg<D, NT>::SMEM, st, tm, tm_exps, p) != cudaSuccess) return -4;
   if (p.n_splits == 1) return 0;
   const int most = (p.width < p.n_splits * (K8D_RUN / KV8_PAGE) ? p.width : p.n_splits * (K8D_RUN / KV8_PAGE)) * KV8_PAGE;
   const int heads = p.B * p.G * p.n_q, per = 128 / (D / 4);
@@ -902,7 +876,7 @@ extern "C" int b200_kv8_decode(const void* q, const void* gate, const void* data
   if (D != 256 && D != 128 && D != 64) return -7;
   CUtensorMap tm, tm_exps;
   if (k8d_make_maps(&tm, &tm_exps, data, exps, D, n_kv, num_pages)) return -1;
-  const int cols = G * group, nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4, per = 8 * nt / group < G ? 8 * nt / group : G;
+  const int cols = G * group, nt = cols <= 8 ? 1 : 2, per = 8 * nt / group < G ? 8 * nt / group : G;
   int rc = -7;
   for (int b0 = 0; b0 < B; b0 += K8D_SEQS) {
     const int n = B - b0 < K8D_SEQS ? B - b0 : K8D_SEQS;
@@ -914,7 +888,7 @@ extern "C" int b200_kv8_decode(const void* q, const void* gate, const void* data
                             part_acc + heads * n_splits * D, reinterpret_cast<float2*>(part_ml) + heads * n_splits,
                             n, G, max_pages, width, num_pages, n_q, n_kv, group, n_splits, per, (G + per - 1) / per, (65536 + group - 1) / group,
                             1.4426950408889634f / sqrtf(static_cast<float>(D)), err};
-#define K8D(DD) rc = nt == 1 ? k8d_launch<DD, 1>(tm, tm_exps, p, st) : nt == 2 ? k8d_launch<DD, 2>(tm, tm_exps, p, st) : k8d_launch<DD, 4>(tm, tm_exps, p, st)
+#define K8D(DD) rc = nt == 1 ? k8d_launch<DD, 1>(tm, tm_exps, p, st) : k8d_launch<DD, 2>(tm, tm_exps, p, st)
     if (D == 256) K8D(256);
     else if (D == 128) K8D(128);
     else K8D(64);
