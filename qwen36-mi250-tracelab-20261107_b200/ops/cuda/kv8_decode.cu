@@ -20,7 +20,9 @@
 
 namespace b200 {
 
-constexpr int K8D_RUN = 256;                    // keys of a run: part of the numerics
+// Keys of a run: part of the numerics. Of 256: one context of 900 keys 9.6 us and not 12.4, but 128 of about 1,088 in 37.0 and not 35.2, four of about
+// 90,000 in 57.7 and not 54.2, 40 passes of four rows over about 4,096 keys in 59.7 and not 51.2: each run's end costs about a page's time.
+constexpr int K8D_RUN = 512;
 constexpr int K8D_SLAB = 16;                    // keys of a warp's scores
 constexpr int K8D_SLABS = KV8_PAGE / K8D_SLAB;  // of a page: a warp each
 constexpr int K8D_OUT = 4;                      // warps that take outputs
@@ -691,7 +693,7 @@ __device__ __forceinline__ void k8d_store(bf16* out, uint2 gate, const float4& o
   e[1] = __floats2bfloat162_rn(o.z * inv * g1.x, o.w * inv * g1.y);
   *reinterpret_cast<uint2*>(out) = raw;
 }
-// Tables of up to 64 runs (16,384 keys): a thread takes all sums of four dims of a head. Its CTAs are small enough to wait beside the
+// Tables of up to 64 runs (32,768 keys): a thread takes all sums of four dims of a head. Its CTAs are small enough to wait beside the
 // kernel in front.
 template <int D>
 __global__ void __maxnreg__(72)
