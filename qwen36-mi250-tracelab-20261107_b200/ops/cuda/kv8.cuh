@@ -35,21 +35,19 @@ __device__ __forceinline__ uint32_t kv8_unpack2(uint16_t two) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(two));
   return r;
 }
-// Two sigmoids, of the halves of a word of bf16 gates, for outputs that are rounded to bf16 next: 1 / (1 + 2^-t) with t = x log2(e), both from one
-// reciprocal, 1 / a = b / (a b). The special functions bound the end of a prefill tile (128 rows of 256: 4,096 cycles with a reciprocal
-// each, 3,072 so; an exact division took 32,000). Below t = -62 a sigmoid stays at 2^-62, so that a b is finite; a NaN stays one.
+// The sigmoids of the halves of a word of bf16 gates, for outputs that are rounded to bf16 next: 1 / (1 + 2^-t) with t = x log2(e) on the unit of
+// special functions. An exact division is a subroutine: the loop at the end of a prefill tile (128 rows of 256) took 32,500 cycles with it, and 20,000
+// so. (Two sigmoids from one reciprocal, 1 / a = b / (a b), need a case of their own where the product overflows or one is NaN: no faster.)
 __device__ __forceinline__ float2 kv8_sigmoid2(uint32_t gates) {
   float a[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const float x = __uint_as_float(i ? gates & 0xffff0000u : gates << 16);
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(a[i]) : "f"(x * -1.4426950408889634f), "f"(62.0f));
-    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a[i]));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a[i]) : "f"(x * -1.4426950408889634f));
     a[i] += 1.0f;
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(a[i]));
   }
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a[0] * a[1]));
-  return make_float2(r * a[1], r * a[0]);
+  return make_float2(a[0], a[1]);
 }
 // The four bytes of a word as two pairs of halves.
 __device__ __forceinline__ void kv8_unpack4(uint32_t word, uint32_t& lo, uint32_t& hi) {

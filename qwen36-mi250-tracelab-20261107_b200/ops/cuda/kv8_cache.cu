@@ -5,7 +5,11 @@
 //
 // Bound: memory, 4 D bytes of bf16 and 2 (D + 1) of the cache per token and KV head. D / 8 (write) or D / 16 (read) neighbouring
 // lanes own a row, 16 bytes of input each, and take the key and the value of a (token, head) together: two loads in flight per thread and one
-// look-up of the page. The row maximum is a shuffle among its lanes.
+// look-up of the page. The row maximum is one of its lanes' bits. Two rows a thread, all loads under way at once, were no faster (write, 6.9 us and
+// 6.7) or slower (read, 58.2 and 55.6).
+//
+// Measured, 2 heads of 256: 128 rows written in 2.0 us, which is a launch and two look-ups; 8,192 rows in 6.8 us (25 MB at 3.7 TB/s, of which 2 us
+// as before); 98,304 rows read in 55.6 us (303 MB at 5.5 TB/s: 83 % of the copy rate), 6,001 rows in 6.2 us.
 #include <cuda_fp16.h>
 
 #include "kv8.cuh"

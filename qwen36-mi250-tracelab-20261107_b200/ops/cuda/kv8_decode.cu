@@ -7,13 +7,20 @@
 // sum_j w_j 2^-b_j. So what the matrix instructions get are the stored numbers as halves (exact) and weights below 2^15.
 //
 // Bound: the cache's bytes, 2 (D + 1) per token and KV head. A context is cut into runs of RUN keys at fixed places, so what a row's
-// result is put together from depends on its own position only, never on the batch; persistent CTAs take runs in turn. In a CTA
-// one warp finds the runs and brings pages of 64 keys by TMA, the next runs' pages ahead of this one's end; four warps take 16 keys
-// each (S = K Q^T, maximum, weights); four take D / 4 dims each over all 64 keys (O += V^T P), a page behind. The outputs stay where they are
-// summed: only maxima and weights are exchanged, 16 bytes per key. (With all dims of every eighth slab in each of eight warps, the
-// warps' outputs were added up at each run's end, which took more instructions than the run: 74 us for 128 sequences of about 1,060 keys.)
+// result is put together from depends on its own position only, never on the batch; persistent CTAs, two per SM, take runs in turn. In a
+// CTA one warp finds the runs and brings pages of 64 keys by TMA, three pages ahead; four warps take 16 keys each (S = K Q^T, maximum,
+// weights); four take D / 4 dims each over all 64 keys (O += V^T P), a page behind. The outputs stay where they are summed: only maxima and
+// weights are exchanged, 16 bytes per key. (With all dims of every eighth slab in each of eight warps, the warps' outputs were added up at
+// each run's end, which took more instructions than the run: 74 us for 128 sequences of about 1,088 keys, and 35 now.)
 // The products are m16n8k16 with keys or dims as the 16 rows and query columns as the 8: one token of one KV head's eight query heads
-// fills the columns, where a tcgen05 tile would be 8 rows of 64. The stored bytes become halves in registers, behind ldmatrix.
+// fills the columns, where a tcgen05 tile would be 8 rows of 64. (The tcgen05 form, S^T and O^T on tiles of 128 keys with two e4m3 terms of queries and
+// weights, took 68 us there: V^T as an operand from rows of values costs 1,300 cycles per 128 keys.) The stored bytes become halves in
+// registers, behind ldmatrix. More than 16 columns (verify passes) are units of their own, which find the pages in L2: as 32 columns of
+// one CTA of 17 warps they took 65 us, and 50 so, for 40 passes of four rows over about 4,096 keys.
+//
+// Measured, heads of 256, 16 over 2: 128 sequences of about 1,088 keys 35 us, 142 MB at 4.1 TB/s; four of about 90,000 54 us, 241 MB at 4.4 TB/s;
+// 40 passes of four rows over about 4,096 keys 50 us. What is left is a page's chain of steps (1,900 cycles for a CTA, 740 of them the scores'
+// products, which wait on each other), about 2,000 cycles at a run's end, 4 us before the first page is there and the joining of the runs.
 #include <cuda_fp16.h>
 
 #include "kv8.cuh"
@@ -651,7 +658,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
 // the partials where there are up to 16. What does not come from the kernel in front is read ahead of the dependency wait: that kernel has
 // waited for everything before it.
 constexpr int K8D_SUMS = 16;
-// Sums i0 .. i0 + 3 of four dims, their partials `D` floats apart.
+// Sums i0 .. i0 + 3 of four dims, their partials `D` floats apart. (Where a row has up to 16 runs, each is its sum: no step is lost on maxima of one.)
 template <int D>
 __device__ __forceinline__ void k8d_sums(const float4* pa, const float2* ml, int runs, int i0, float* top, float* l, float4* acc) {
 #pragma unroll

@@ -16,6 +16,13 @@
 // TMEM is rescaled where a maximum grew by more than 2^LAZY. Weights as halves reach from 2^15 to 2^-24, 2^-28 of the largest at the least.
 // A span of few tiles over a long context is cut into runs of pages for CTAs of their own, by its own length and position alone, whose partial
 // sums are added in their order: a row's bits depend on its span, never on the pass. All waits are bounded. No cluster multicast.
+//
+// Bound: the tensor pipe would take 1,024 cycles for a page of 256-wide heads, shared memory 1,600 (keys twice and P once as operands, V once, the
+// conversion of V, weights and tables); a page takes 1,830 to 1,950. A tile's first scores come about 10,000 cycles after its start (queries to two terms,
+// to TMEM), and its end takes 7,000 to 8,000: most of a short context's time.
+// Measured, 16 heads of 256 over 2: 4 x 2,048 rows of prompts of about 28,672 tokens 1,540 to 1,600 us (1.55 TFLOP: 0.97 to 1.0 PFLOP/s; the bf16
+// cache's kernel 1,940), 8 x 1,024 rows of fresh prompts 149 us (206), 61 rows over 3,584 tokens 22.6 us, seven spans of 1,531 rows of
+// heads of 128, 6 over 3, 16.5 us.
 #include <cuda_fp16.h>
 
 #include "kv8.cuh"
@@ -310,7 +317,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
       constexpr uint32_t idesc_s = (1u << 4) | (64u >> 3) << 17 | (128u >> 4) << 24;                                     // e4m3
       constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | static_cast<uint32_t>(D >> 3) << 17 | (128u >> 4) << 24;     // halves, B MN-major
       // Scores of page q once page q - 2's have been read and the keys are there, products of page v once its weights and values are: whichever
-      // comes first. (In a fixed order one waited behind the other: 1.54 ms for 4 x 2048 rows of long prompts.)
+      // comes first: in a fixed order one waited behind the other.
       if (!mbar_wait(q_full, 0, p.err, ERR_WAIT_FULL, abort_flag)) *abort_flag = 1;
       int q = 0, v = 0;
       long long t0 = clock64();

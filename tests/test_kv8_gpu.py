@@ -375,6 +375,29 @@ def test_prefill_of_a_full_pass(C):
     C.check_errors(q.device)
 
 
+@pytest.mark.parametrize("n", [300, 1500])  # a run of keys, several
+def test_gates_of_all_sizes(C, n):
+    """Far below and above where a sigmoid is 0 and 1 in bf16, infinite and NaN: a number's gate is its own alone."""
+    n_q, n_kv, D = 16, 2, 128
+    layer = _layer(n // 64 + 3, n_kv, D)
+    tables = _tables([n], n // 64 + 1, n // 64 + 3)
+    q, gate = _rows(80, n_q, D, 4)
+    odd = torch.tensor([float("nan"), float("inf"), float("-inf"), -1000.0, -100.0, -60.0, -44.0, 60.0, 1000.0], device=DEV).bfloat16()
+    at = torch.arange(0, gate.numel(), 3, device=DEV)
+    gate.view(-1)[at] = odd[torch.arange(len(at), device=DEV) % len(odd)]
+    pos = torch.arange(n - 80, n, device=DEV)
+    sig = torch.sigmoid(gate.double())
+    clean = gate.clone()
+    clean.view(-1)[at] = 0
+    out, tol = _attention(q, clean, layer, tables.expand(80, -1), pos)
+    of_one = 1 / torch.sigmoid(clean.double())
+    want, tol = out * of_one * sig, tol * of_one * sig + 1e-30  # an output below a bf16 number's least is one there
+    for got in (C.kv8_prefill(q, gate, layer, tables, [0, 80], [n - 80]), C.kv8_decode(q, gate, layer, tables, pos, 80)):
+        assert torch.equal(got.isnan(), gate.isnan())
+        ok = ~gate.isnan()
+        assert ((got.double() - want).abs() <= tol)[ok].all()
+
+
 # ------------------------------------------------------------------ how they are called
 @pytest.mark.parametrize("kind", ["decode", "prefill"])
 def test_another_stream_views_and_index_types(C, kind):
