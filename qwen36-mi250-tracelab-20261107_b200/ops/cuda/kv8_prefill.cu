@@ -706,14 +706,9 @@ int k8p_launch(const CUtensorMap& tm, const CUtensorMap& te, const Kv8PrefillPar
 }
 }  // namespace
 
-// Positions of a tile, and the runs that a span of n rows from position pos0 on is cut into (1: it is not): the caller sizes grid and partials by them.
+// Positions of a tile, and what a span is cut by (k8p_run_pages): 0, the CTAs, 1, a run's least pages. The caller sizes grid and partials by them.
 extern "C" int b200_kv8_prefill_positions(int group) { return group >= 1 && group <= 16 ? 128 / group : 0; }
-extern "C" int b200_kv8_prefill_runs(int n, int pos0, int width, int group, int n_kv) {
-  if (n <= 0 || group < 1 || group > 16 || n_kv < 1) return 1;
-  const int seen = (pos0 + n - 1) / KV8_PAGE + 1, np = seen < width ? seen : width;
-  const int pages = k8p_run_pages(n, np, 128 / group, n_kv);
-  return np > 0 && pages < np ? (np + pages - 1) / pages : 1;
-}
+extern "C" int b200_kv8_prefill_cut(int which) { return which ? K8P_MIN_PAGES : K8P_CTAS; }
 
 // q: [T, n_q, D] bf16 (normed and rotated), gate, out: [T, n_q * D], in 16-byte rows; data, exps: one layer of the 8-bit cache, which holds the
 // spans' own keys; starts [segs + 1], pos0 [segs] of the spans, tables [segs] rows of `width` pages. n_tiles: at least the spans' tiles.

@@ -91,7 +91,7 @@ class _Sig:
     b200_kv8_read = [P, P, P, P, P, I, I, I, P, P, I, I, I, I, P, P]
     b200_kv8_decode_run = []
     b200_kv8_prefill_positions = [I]
-    b200_kv8_prefill_runs = [I, I, I, I, I]
+    b200_kv8_prefill_cut = [I]
     b200_kv8_prefill = [P, P, P, P, P, P, I, I, P, I, I, I, I, I, I, I, P, P, P, P, P]
     b200_kv8_decode = [P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, P, P, P, P, P]
 
@@ -811,7 +811,6 @@ def kv8_read(layer: Kv8Layer, positions: torch.Tensor, seq_of_row: torch.Tensor,
 
 
 KV8_HEAD_DIMS = (64, 128, 256)  # of the attention kernels over the 8-bit cache
-KV8_CUT_TILES = 64  # (tiles of a span) * (KV heads) up to which kv8_prefill.cu may cut its context
 
 
 def _kv8_queries(what: str, q: torch.Tensor, gate: torch.Tensor, n_kv: int, D: int, dev: torch.device):
@@ -889,12 +888,15 @@ def kv8_prefill(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tabl
         if len(lens) != n_seg or seg_starts[0] != 0 or seg_starts[-1] != T or seqs < n_seg or min(lens, default=0) < 0:
             raise ValueError(f"kv8_prefill: spans {seg_starts} with {n_seg} first positions do not make {T} rows of at most {seqs} sequences")
         n_tiles = 0
+        ctas, least = L.b200_kv8_prefill_cut(0), L.b200_kv8_prefill_cut(1)
         for n, pos in zip(lens, seg_pos0):
             if pos < 0 or pos + n > width * PAGE_SIZE:
                 raise ValueError(f"kv8_prefill: rows at positions {pos} .. {pos + n - 1}, page tables of {width} pages")
-            n_tiles += (n + per - 1) // per
-            if 0 < n * n_kv <= per * KV8_CUT_TILES:  # short enough to be cut
-                splits = max(splits, L.b200_kv8_prefill_runs(n, pos, width, group, n_kv))
+            tiles = -(-n // per)
+            n_tiles += tiles
+            if 0 < 2 * tiles * n_kv <= ctas:  # into so many runs is the span cut (kv8_prefill.cu, k8p_run_pages)
+                seen = (pos + n - 1) // PAGE_SIZE + 1
+                splits = max(splits, -(-seen // max(least, -(-seen // (ctas // (tiles * n_kv))))))
     elif meta is None:
         raise ValueError("kv8_prefill: neither the spans' lists nor their device tensors")
     else:
