@@ -8,8 +8,8 @@
 // look-up of the page. The row maximum is one of its lanes' bits. Two rows a thread, all loads under way at once, were no faster (write, 6.9 us and
 // 6.7) or slower (read, 58.2 and 55.6).
 //
-// Measured, 2 heads of 256: 128 rows written in 2.0 us, which is a launch and two look-ups; 8,192 rows in 6.8 us (25 MB at 3.7 TB/s, of which 2 us
-// as before); 98,304 rows read in 55.6 us (303 MB at 5.5 TB/s: 83 % of the copy rate), 6,001 rows in 6.2 us.
+// Measured, 2 heads of 256: 128 rows written in 1.8 us, which is a launch and two look-ups; 8,192 rows in 6.3 us (25 MB at 4.0 TB/s, of which 1.8 us
+// as before); 98,304 rows read in 54.3 us (304 MB at 5.6 TB/s: 85 % of the copy rate), 6,001 rows in 5.9 us.
 #include <cuda_fp16.h>
 
 #include "kv8.cuh"
@@ -47,10 +47,10 @@ kv8_write_kernel(const bf16* k, long long k_row, long long k_head, const bf16* v
   constexpr int LANES = D / 8;
   pdl_wait();
   pdl_launch();
-  const long long item = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) / LANES;  // (token, head)
+  const uint32_t item = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;  // (token, head), in 32 bits: a division of 64 takes as long as the rest
   const int part = threadIdx.x % LANES;
-  const bool real = item < static_cast<long long>(T) * n_kv;
-  const int row = real ? static_cast<int>(item / n_kv) : 0, kh = real ? static_cast<int>(item - static_cast<long long>(row) * n_kv) : 0;
+  const bool real = item < static_cast<uint32_t>(T) * n_kv;
+  const int row = real ? static_cast<int>(item / static_cast<uint32_t>(n_kv)) : 0, kh = real ? static_cast<int>(item) - row * n_kv : 0;
   const int64_t pos = positions[row];
   const int seq = seq_of_row[row];
   const uint4 raw[2] = {load8<ALIGNED>(k + row * k_row + kh * k_head + part * 8), load8<ALIGNED>(v + row * v_row + kh * v_head + part * 8)};
@@ -90,10 +90,10 @@ kv8_read_kernel(const uint8_t* data, const uint8_t* exps, const int64_t* positio
   constexpr int LANES = D / 16;
   pdl_wait();
   pdl_launch();
-  const long long item = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) / LANES;
+  const uint32_t item = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
   const int part = threadIdx.x % LANES;
-  if (item >= static_cast<long long>(T) * n_kv) return;
-  const int row = static_cast<int>(item / n_kv), kh = static_cast<int>(item - static_cast<long long>(row) * n_kv);
+  if (item >= static_cast<uint32_t>(T) * n_kv) return;
+  const int row = static_cast<int>(item / static_cast<uint32_t>(n_kv)), kh = static_cast<int>(item) - row * n_kv;
   const Kv8Where where(positions[row], seq_of_row[row], kh, tables, max_pages, width, n_seqs, true);
   const bool there = where.there(num_pages);
   uint4 raw[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
@@ -121,7 +121,7 @@ kv8_read_kernel(const uint8_t* data, const uint8_t* exps, const int64_t* positio
         o[2 * i + j] = __floats2bfloat162_rn(x.x * f, x.y * f);
       }
     }
-    uint4* dst = reinterpret_cast<uint4*>((which ? v : k) + item * D + part * 16);
+    uint4* dst = reinterpret_cast<uint4*>((which ? v : k) + static_cast<size_t>(item) * D + part * 16);
     dst[0] = out[0];
     dst[1] = out[1];
   }
@@ -136,6 +136,7 @@ extern "C" int b200_kv8_write(const void* k, long long k_row, long long k_head, 
                               const int64_t* positions, const int* seq_of_row, const int* tables, int max_pages, int width,
                               int n_seqs, void* data, void* exps, int T, int n_kv, int D, int num_pages, int* err, cudaStream_t st) {
   if (T <= 0) return 0;
+  if (static_cast<long long>(T) * n_kv > 0x7fffffffLL) return -7;  // rows are counted in 32 bits
   const auto rows_of_16 = [](const void* p, long long row, long long head) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && row % 8 == 0 && head % 8 == 0;
   };
@@ -162,6 +163,7 @@ extern "C" int b200_kv8_read(const void* data, const void* exps, const int64_t* 
                              int max_pages, int width, int n_seqs, void* k, void* v, int T, int n_kv, int D, int num_pages, int* err,
                              cudaStream_t st) {
   if (T <= 0) return 0;
+  if (static_cast<long long>(T) * n_kv > 0x7fffffffLL) return -7;  // rows are counted in 32 bits
   const long long threads = static_cast<long long>(T) * n_kv * (D / 16);
   const dim3 grid(static_cast<unsigned>((threads + 255) / 256));
   cudaError_t rc;
