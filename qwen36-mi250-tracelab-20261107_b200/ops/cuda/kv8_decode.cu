@@ -19,8 +19,9 @@
 // one CTA of 17 warps they took 65 us, and 50 so, for 40 passes of four rows over about 4,096 keys.
 //
 // Measured, heads of 256, 16 over 2: 128 sequences of about 1,088 keys 35 us, 142 MB at 4.1 TB/s; four of about 90,000 54 us, 241 MB at 4.4 TB/s;
-// 40 passes of four rows over about 4,096 keys 50 us. What is left is a page's chain of steps (1,900 cycles for a CTA, 740 of them the scores'
-// products, which wait on each other), about 2,000 cycles at a run's end, 4 us before the first page is there and the joining of the runs.
+// 40 passes of four rows over about 4,096 keys 50 us. With one column tile the pages come at the memory's rate once they come; what is left is 5 us
+// before the first is asked for, CTAs that wait for the last whole runs, and 4 to 6 us for joining the runs. With two it is a page's chain of steps (2,330
+// cycles for a CTA, 1,200 of them the scores' products).
 #include <cuda_fp16.h>
 
 #include "kv8.cuh"
