@@ -42,7 +42,7 @@ struct Kv8PrefillParams {
   bf16* out;                // [T, n_q * D]
   float* part_acc;          // [T, n_q, max_splits, D]: of spans that are cut
   float2* part_ml;          // [T, n_q, max_splits]
-  int segs, max_pages, width, num_pages, n_q, n_kv, group, positions, max_splits;  // positions: of a tile
+  int T, segs, max_pages, width, num_pages, n_q, n_kv, group, positions, max_splits;  // positions: of a tile
   int inv_group;            // r * inv_group >> 16 is r / group, for rows below 128 of groups up to 16
   float scale_log2;
   int* err;
@@ -58,7 +58,7 @@ struct Kv8PrefillCfg {
   static constexpr int V_BYTES = KV8_PAGE * D * 2;     // [HB][64 rows][128]: values as halves
   static constexpr int P_BYTES = 128 * 128;            // [128 rows][64 halves]
   static constexpr int EXPS = 2 * KV8_PAGE;
-  static constexpr int SMEM = 7 * PAGE_BYTES + 2 * V_BYTES + 2 * P_BYTES + 4 * EXPS + 4 * 3 * KV8_PAGE * 4 + 512 + 53 * 8;
+  static constexpr int SMEM = 7 * PAGE_BYTES + 2 * V_BYTES + 2 * P_BYTES + 4 * EXPS + 4 * 3 * KV8_PAGE * 4 + 512 + 54 * 8;
   static constexpr int TMEM_COLS = 128 + D + D / 2 <= 256 ? 256 : 512;  // two score tiles of 64, the output, two terms of the queries
 };
 
@@ -110,14 +110,28 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   return r;
 }
 
-// The tile of a CTA: found among the spans' tiles by all lanes of a warp, 32 spans at a time. false: there is none.
-struct Kv8Tile { int seg, p0, row0, rows, pos0; };
+// The tile of a CTA: found among the spans' tiles by all lanes of a warp, 32 spans at a time. false: there is none. The spans come from device memory
+// that the host may not have seen: one that is not within the T rows and its page table, or that was given too few runs, has no tiles, and leaves an error.
+struct Kv8Tile { int seg, p0, row0, rows, pos0, run_pages; };
 __device__ __forceinline__ bool k8p_find(const Kv8PrefillParams& p, int tile, Kv8Tile& t) {
   const int lane = threadIdx.x & 31;
   int before = 0;
   for (int s0 = 0; s0 < p.segs; s0 += 32) {
     const int s = s0 + lane;
-    const int a = s < p.segs ? p.starts[s] : 0, n = s < p.segs ? p.starts[s + 1] - a : 0, pos = s < p.segs ? p.pos0[s] : 0;
+    uint32_t word[3] = {0, 0, 0};  // all three under way at once: each of them is a wait for memory
+    ask_32(word[0], p.starts + s, s < p.segs);
+    ask_32(word[1], p.starts + s + 1, s < p.segs);
+    ask_32(word[2], p.pos0 + s, s < p.segs);
+    const int a = word[0], b = word[1], pos = word[2];
+    int n = (0 <= a) & (a <= b) & (b <= p.T) ? b - a : -1;
+    if ((n > 0) & ((pos < 0) | (pos > p.width * KV8_PAGE - n))) n = -1;
+    int run_pages = p.width;
+    if (p.max_splits > 1) {
+      const int np = (pos + n - 1) / KV8_PAGE + 1;
+      run_pages = k8p_run_pages(n, np, p.positions, p.n_kv);
+      if ((n > 0) & (run_pages * p.max_splits < np)) n = -1;
+    }
+    if (n < 0) { atomicCAS(p.err, 0, ERR_BAD_INDEX); n = 0; }
     const int tiles = (n + p.positions - 1) / p.positions;
     int upto = tiles;
 #pragma unroll
@@ -134,6 +148,7 @@ __device__ __forceinline__ bool k8p_find(const Kv8PrefillParams& p, int tile, Kv
       t.rows = __shfl_sync(0xffffffffu, n, l);
       t.p0 = (tile - __shfl_sync(0xffffffffu, upto - tiles, l)) * p.positions;
       t.pos0 = __shfl_sync(0xffffffffu, pos, l);
+      t.run_pages = __shfl_sync(0xffffffffu, run_pages, l);
       return true;
     }
     before = __shfl_sync(0xffffffffu, upto, 31);
@@ -184,6 +199,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
   uint64_t* const t_empty = bars + 48;                   // [4]
   uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 52);
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* const s_cut = abort_flag + 1;            // whether the span is cut: needed at the end, and a register less until then
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
@@ -191,11 +207,8 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
   // the last tiles of the spans see the most keys and go first
   if (!k8p_find(p, static_cast<int>(gridDim.x - 1 - blockIdx.x), tile)) return;
   const int kh = blockIdx.y, n_pos = min(p.positions, tile.rows - tile.p0);
-  const int most = p.width;
-  const int np_all = min(most, (tile.pos0 + tile.p0 + n_pos - 1) / KV8_PAGE + 1);            // pages that the tile's rows see
-  const int run_pages = p.max_splits > 1 ? k8p_run_pages(tile.rows, min(most, (tile.pos0 + tile.rows - 1) / KV8_PAGE + 1), p.positions, p.n_kv) : most;
-  const bool cut = p.max_splits > 1 && run_pages < min(most, (tile.pos0 + tile.rows - 1) / KV8_PAGE + 1);
-  const int first = static_cast<int>(blockIdx.z) * run_pages, np = min(np_all, first + run_pages) - first;
+  const int np_all = (tile.pos0 + tile.p0 + n_pos - 1) / KV8_PAGE + 1, np_span = (tile.pos0 + tile.rows - 1) / KV8_PAGE + 1;  // pages that the tile's, the span's rows see
+  const int first = static_cast<int>(blockIdx.z) * tile.run_pages, np = min(np_all, first + tile.run_pages) - first;
   if (np <= 0) return;  // nothing of this run for these rows: the sum over the runs passes over it
 
   if (threadIdx.x == 0) {
@@ -213,6 +226,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
     mbar_init(q_ready, K8P_THREADS - 64);
     mbar_init(q_full, 256);
     *abort_flag = 0;
+    *s_cut = tile.run_pages < np_span;
     mbar_fence_init();
     tma_prefetch_desc(&tm);
     tma_prefetch_desc(&tm_exps);
@@ -270,7 +284,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
 
   if (warp == 9) {
     // ---------------- loads. The gates are needed at the end, when other loads of this SM's neighbours are under way: they are brought to L2 now.
-    for (int i = lane; !cut && i < n_pos; i += 32)
+    for (int i = *s_cut ? n_pos : lane; i < n_pos; i += 32)
       asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;"
                      ::"l"(p.gate + (static_cast<size_t>(tile.row0 + tile.p0 + i) * p.n_q + kh * p.group) * D), "r"(p.group * D * 2) : "memory");
     if (elect_one()) {
@@ -547,6 +561,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
     // writes outputs of a whole row at a time (with a thread a row from TMEM to the output, the end of a tile took 13 us).
     float* const so = reinterpret_cast<float*>(sQ);        // [128][D], in the place of Q and the pages' bytes
     if (ok) {
+      const bool cut = *s_cut;
       const float inv = cut ? 1.0f : 1.0f / l;             // (a row sees itself)
 #pragma unroll 1
       for (int c = hf * DH; c < hf * DH + DH; c += 16) {
@@ -571,6 +586,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
       const int pos = row * p.inv_group >> 16;
       return head0 + static_cast<size_t>(pos) * p.n_q + (row - pos * p.group);
     };
+    const bool cut = *s_cut;
     uint4 gate[STEPS];
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
@@ -619,10 +635,10 @@ kv8_prefill_combine_kernel(Kv8PrefillParams p) {
   constexpr int QUADS = D / 4, AT_ONCE = 8;
   Kv8Tile tile = {};
   const bool found = k8p_find(p, blockIdx.x, tile);
-  const int np = min(p.width, (tile.pos0 + tile.rows - 1) / KV8_PAGE + 1), run_pages = k8p_run_pages(tile.rows, np, p.positions, p.n_kv);
+  const int np = (tile.pos0 + tile.rows - 1) / KV8_PAGE + 1, run_pages = tile.run_pages;
   const int n_pos = min(p.positions, tile.rows - tile.p0), i = blockIdx.z * (128 / QUADS) + threadIdx.x / QUADS;
   const bool work = found && run_pages < np && i < n_pos * p.group;
-  const int np_all = min(p.width, (tile.pos0 + tile.p0 + n_pos - 1) / KV8_PAGE + 1), runs = (np_all + run_pages - 1) / run_pages;  // that wrote
+  const int np_all = (tile.pos0 + tile.p0 + n_pos - 1) / KV8_PAGE + 1, runs = (np_all + run_pages - 1) / run_pages;  // that wrote
   const int pos = i * p.inv_group >> 16, quad = threadIdx.x % QUADS;
   const size_t at = static_cast<size_t>(tile.row0 + tile.p0 + pos) * p.n_q + blockIdx.y * p.group + (i - pos * p.group);
   // Threads without work leave before the wait, so that the grid does not come in waves behind it; those of the first CTA stay: this kernel must
@@ -711,14 +727,14 @@ extern "C" int b200_kv8_prefill_positions(int group) { return group >= 1 && grou
 extern "C" int b200_kv8_prefill_cut(int which) { return which ? K8P_MIN_PAGES : K8P_CTAS; }
 
 // q: [T, n_q, D] bf16 (normed and rotated), gate, out: [T, n_q * D], in 16-byte rows; data, exps: one layer of the 8-bit cache, which holds the
-// spans' own keys; starts [segs + 1], pos0 [segs] of the spans, tables [segs] rows of `width` pages. n_tiles: at least the spans' tiles.
+// spans' own keys; starts [segs + 1], pos0 [segs] of the spans, within T rows, tables [segs] rows of `width` pages. n_tiles: at least the spans' tiles.
 // max_splits: the most runs of a span (part_acc [T, n_q, max_splits, D], part_ml [.., 2] where there is more than one).
 extern "C" int b200_kv8_prefill(const void* q, const void* gate, const void* data, const void* exps, const int* starts, const int* pos0,
-                                int segs, int n_tiles, const int* tables, int max_pages, int width, int num_pages, int n_q, int n_kv,
+                                int T, int segs, int n_tiles, const int* tables, int max_pages, int width, int num_pages, int n_q, int n_kv,
                                 int D, int max_splits, float* part_acc, float* part_ml, void* out, int* err, cudaStream_t st) {
   if (n_tiles <= 0 || segs <= 0) return 0;
   const int group = n_kv > 0 ? n_q / n_kv : 0;
-  if (group < 1 || group * n_kv != n_q || group > 16 || max_splits < 1 || width < 1) return -7;
+  if (group < 1 || group * n_kv != n_q || group > 16 || max_splits < 1 || width < 1 || width > 0x7fffffff / KV8_PAGE) return -7;
   if (D != 256 && D != 128 && D != 64) return -7;
   const long long rows = static_cast<long long>(num_pages) * 2 * n_kv * KV8_PAGE;
   if (rows > 0x7fffffffLL) return -7;  // a TMA coordinate
@@ -734,7 +750,7 @@ extern "C" int b200_kv8_prefill(const void* q, const void* gate, const void* dat
   if (k8p_encode(&tm, data, 2, dims, strides, box, rowb == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B) ||
       k8p_encode(&te, exps, 3, edims, estrides, ebox, CU_TENSOR_MAP_SWIZZLE_NONE)) return -1;
   const Kv8PrefillParams p{static_cast<const bf16*>(q), static_cast<const bf16*>(gate), starts, pos0, tables, static_cast<bf16*>(out), part_acc,
-                           reinterpret_cast<float2*>(part_ml), segs, max_pages, width, num_pages, n_q, n_kv, group, 128 / group, max_splits,
+                           reinterpret_cast<float2*>(part_ml), T, segs, max_pages, width, num_pages, n_q, n_kv, group, 128 / group, max_splits,
                            (65536 + group - 1) / group, 1.4426950408889634f / sqrtf(static_cast<float>(D)), err};
   if (D == 256) return k8p_launch<256>(tm, te, p, n_tiles, st);
   if (D == 128) return k8p_launch<128>(tm, te, p, n_tiles, st);

@@ -92,7 +92,7 @@ class _Sig:
     b200_kv8_decode_run = []
     b200_kv8_prefill_positions = [I]
     b200_kv8_prefill_cut = [I]
-    b200_kv8_prefill = [P, P, P, P, P, P, I, I, P, I, I, I, I, I, I, I, P, P, P, P, P]
+    b200_kv8_prefill = [P, P, P, P, P, P, I, I, I, P, I, I, I, I, I, I, I, P, P, P, P, P]
     b200_kv8_decode = [P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, P, P, P, P, P]
 
 
@@ -866,7 +866,8 @@ def kv8_prefill(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tabl
     a short span is cut into runs for CTAs of their own, by the span's own rows and position: a row's bits do not depend on the other spans.
 
     ``meta``: ``(seg_starts, seg_pos0)`` as int32 device tensors that the caller keeps, of the same numbers; without it every call uploads
-    them. With ``meta`` the lists may be None, which lets the call be captured in a CUDA graph: no span is cut then."""
+    them. With ``meta`` the lists may be None, which lets the call be captured in a CUDA graph: no span is cut then. A span in ``meta`` that is not
+    within the rows and its page table is left out, and reported by ``check_errors``."""
     pages, n_kv, D = check_layer(layer, "kv8_prefill")
     data, exps = layer
     dev = data.device
@@ -881,6 +882,11 @@ def kv8_prefill(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tabl
     if block_tables.dtype != torch.int32 or one != 1:
         block_tables = block_tables.to(torch.int32).contiguous()
         step = width
+    if meta is not None:
+        starts_t, pos0_t = meta
+        for t in meta:
+            if t.dtype != torch.int32 or t.device != dev or t.dim() != 1 or t.stride(0) != 1:
+                raise ValueError(f"kv8_prefill: meta holds contiguous int32 vectors on {dev}, not {t.dtype} {tuple(t.shape)} with strides {t.stride()} on {t.device}")
     splits = 1
     if seg_starts is not None:
         n_seg = len(seg_pos0)
@@ -900,13 +906,13 @@ def kv8_prefill(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tabl
     elif meta is None:
         raise ValueError("kv8_prefill: neither the spans' lists nor their device tensors")
     else:
-        n_seg = meta[1].shape[0]
+        n_seg = pos0_t.shape[0]
         n_tiles = T // per + n_seg
+        if seqs < n_seg:
+            raise ValueError(f"kv8_prefill: meta of {n_seg} spans, page tables of {seqs} sequences")
     if meta is not None:
-        starts_t, pos0_t = meta
-        if starts_t.dtype != torch.int32 or pos0_t.dtype != torch.int32 or starts_t.numel() < n_seg + 1 or pos0_t.numel() < n_seg \
-                or starts_t.device != dev or pos0_t.device != dev:
-            raise ValueError(f"kv8_prefill: meta of {starts_t.numel()} and {pos0_t.numel()} numbers ({starts_t.dtype}, {starts_t.device}) for {n_seg} spans")
+        if starts_t.shape[0] < n_seg + 1 or pos0_t.shape[0] < n_seg:
+            raise ValueError(f"kv8_prefill: meta of {starts_t.shape[0]} and {pos0_t.shape[0]} numbers for {n_seg} spans")
     elif T:
         both = torch.tensor([*seg_starts, *seg_pos0], dtype=torch.int32).to(dev)
         starts_t, pos0_t = both[: n_seg + 1], both[n_seg + 1 :]
@@ -920,7 +926,7 @@ def kv8_prefill(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tabl
         acc = scratch.data_ptr()
         ml = acc + part * D
     _check(L.b200_kv8_prefill(
-        q.data_ptr(), gate.data_ptr(), data.data_ptr(), exps.data_ptr(), starts_t.data_ptr(), pos0_t.data_ptr(), n_seg, n_tiles,
+        q.data_ptr(), gate.data_ptr(), data.data_ptr(), exps.data_ptr(), starts_t.data_ptr(), pos0_t.data_ptr(), T, n_seg, n_tiles,
         block_tables.data_ptr(), step, width, pages, n_q, n_kv, D, splits, acc, ml, out.data_ptr(), _err_ptr(dev),
         _raw_stream(dev)), "kv8_prefill")
     return out

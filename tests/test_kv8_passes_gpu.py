@@ -1,0 +1,85 @@
+"""Passes over the 8-bit KV cache as the engine makes them: unlike spans packed together, captured passes, spans from device memory."""
+
+import pytest
+import torch
+from test_kv8_gpu import _attention, _check, _layer, _rows, _tables
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.fixture(scope="module")
+def C():
+    from b200serve.ops import cuda_ops
+
+    cuda_ops.lib()
+    return cuda_ops
+
+
+class _Pass:
+    """Spans of ``lens`` new rows on ``pos0`` cached tokens each, with the call over all of them and over one alone."""
+
+    def __init__(self, C, lens, pos0, heads=(16, 2, 256), width=None, seed=9):
+        n_q, n_kv, D = heads
+        total = [a + b for a, b in zip(lens, pos0)]
+        pages = sum((n + 63) // 64 for n in total) + 2
+        self.C, self.lens, self.pos0 = C, lens, pos0
+        self.layer = _layer(pages, n_kv, D)
+        self.tables = _tables(total, width or max(total) // 64 + 1, pages)
+        self.starts = [0]
+        for n in lens:
+            self.starts.append(self.starts[-1] + n)
+        self.q, self.gate = _rows(self.starts[-1], n_q, D, seed)
+        self.meta = tuple(torch.tensor(x, dtype=torch.int32, device=DEV) for x in (self.starts, pos0))
+
+    def packed(self, meta=True):
+        return self.C.kv8_prefill(self.q, self.gate, self.layer, self.tables, self.starts, self.pos0, meta=self.meta if meta else None)
+
+    def from_device(self, starts=None, pos0=None, tables=None):
+        """The call of a captured pass: no lists."""
+        meta = tuple(m if x is None else torch.tensor(x, dtype=torch.int32, device=DEV) for m, x in zip(self.meta, (starts, pos0)))
+        return self.C.kv8_prefill(self.q, self.gate, self.layer, self.tables if tables is None else tables, None, None, meta=meta)
+
+    def alone(self, i):
+        a, b = self.starts[i], self.starts[i + 1]
+        return self.C.kv8_prefill(self.q[a:b], self.gate[a:b], self.layer, self.tables[i : i + 1], [0, b - a], [self.pos0[i]])
+
+    def check(self, got, spans=None):
+        for i in range(len(self.lens)) if spans is None else spans:
+            a, b = self.starts[i], self.starts[i + 1]
+            pos = torch.arange(self.pos0[i], self.pos0[i] + b - a, device=DEV)
+            _check(got[a:b], _attention(self.q[a:b], self.gate[a:b], self.layer, self.tables[i].expand(b - a, -1), pos), f"span {i}")
+
+
+def test_device_spans_that_do_not_fit_are_refused(C):
+    p = _Pass(C, [40, 70], [100, 200])
+    starts, pos0 = p.meta
+    for meta in ((torch.stack([starts, starts], 1)[:, 0], pos0), (starts, torch.stack([pos0, pos0], 1)[:, 0]), (starts.long(), pos0),
+                 (starts, pos0.view(1, -1)), (starts.cpu(), pos0), (starts[:2], pos0)):
+        for lists in ((p.starts, p.pos0), (None, None)):
+            with pytest.raises(ValueError, match="kv8_prefill: meta"):
+                C.kv8_prefill(p.q, p.gate, p.layer, p.tables, *lists, meta=meta)
+    with pytest.raises(ValueError, match="kv8_prefill"):
+        p.from_device(tables=p.tables[:1])
+    C.check_errors(p.q.device)
+
+
+@pytest.mark.parametrize("starts,pos0", [([0, 40, 111], None), ([0, 40, 39], None), ([0, 40, 1 << 30], None), (None, [100, -1]),
+                                         (None, [100, 251]), (None, [100, 2**31 - 1])])
+def test_a_device_span_outside_its_rows_or_pages_is_left_out_and_reported(C, starts, pos0):
+    p = _Pass(C, [40, 70], [100, 200], width=5)
+    got = p.from_device(starts, pos0)
+    with pytest.raises(C.KernelError, match="index"):
+        C.check_errors(p.q.device)
+    p.check(got, [0])
+    p.check(p.from_device())
+    C.check_errors(p.q.device)
+
+
+def test_device_spans_with_more_runs_than_the_lists_say_are_reported(C):
+    p = _Pass(C, [40, 70], [5000, 600])
+    small = C.kv8_prefill  # the lists name short contexts, the tensors a long one
+    meta = (p.meta[0], p.meta[1])
+    small(p.q, p.gate, p.layer, p.tables, p.starts, [500, 600], meta=meta)
+    with pytest.raises(C.KernelError, match="index"):
+        C.check_errors(p.q.device)
