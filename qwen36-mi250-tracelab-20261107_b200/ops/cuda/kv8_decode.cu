@@ -186,6 +186,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
     // their way any other load waits behind some 30 MB of them, 4 us: what a unit needs to know is asked for two units ahead, and published one ahead.
     const int per_seq = p.units_per_seq * p.n_kv;
     int full_before = 0, tails_before = 0;
+    bool past = false;  // a row that stands behind its page table
     for (int b0 = 0; b0 < p.B; b0 += 128) {
       int len[4] = {0, 0, 0, 0};
 #pragma unroll 4
@@ -193,7 +194,11 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int b = b0 + i * 32 + lane;
-          if (b < p.B) len[i] = max(len[i], kv8_length(p.positions, b * p.G + r, most));
+          if (b < p.B) {
+            const int64_t position = p.positions[b * p.G + r];
+            len[i] = max(len[i], kv8_length(position, most));
+            past |= position >= most;
+          }
         }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -210,6 +215,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
         tails_before += __popc(tails);
       }
     }
+    if (past) atomicCAS(p.err, 0, ERR_BAD_INDEX);
     if (lane == 0) s_first[0] = s_tail[0] = 0;
     __syncwarp();
     const int grid = gridDim.x, cta = blockIdx.x;
@@ -872,7 +878,7 @@ int k8d_launch(const CUtensorMap& tm, const CUtensorMap& tm_exps, const Kv8Decod
 extern "C" int b200_kv8_decode_run(void) { return K8D_RUN; }
 
 // q: [B * G, n_q, D] bf16 (normed and rotated), G rows per sequence; gate, out: [B * G, n_q * D]; data, exps: one layer of the 8-bit cache, which
-// holds the rows' own keys; positions [B * G] (negative: a row without keys, whose output is 0); tables [B] rows of `width` pages.
+// holds the rows' own keys; positions [B * G] (negative: a row without keys, whose output is 0; behind the page table: an error, and the table's keys); tables [B] rows of `width` pages.
 // n_splits runs cover a row of the tables; part_acc [B * G, n_q, n_splits, D] and part_ml [.., 2] where n_splits > 1.
 extern "C" int b200_kv8_decode(const void* q, const void* gate, const void* data, const void* exps, const int64_t* positions,
                                const int* tables, int max_pages, int width, int num_pages, int B, int G, int n_q, int n_kv, int D,

@@ -836,7 +836,7 @@ def kv8_decode(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_table
                G: int) -> torch.Tensor:
     """``flash_decode`` over the 8-bit cache: gated attention of ``G`` rows per sequence (decode 1, verify k + 1), each over the
     keys ``0 .. positions[row]`` of its sequence. A row's bits depend on its own position, queries and keys only, not on the batch or ``G``. A negative
-    position is a row without keys: its output is 0. Only device tensors are touched, so the call can be captured in a CUDA graph."""
+    position is a row without keys: its output is 0; one behind its page table is reported by ``check_errors``. Only device tensors are touched, so the call can be captured in a CUDA graph."""
     pages, n_kv, D = check_layer(layer, "kv8_decode")
     data, exps = layer
     dev = data.device

@@ -83,3 +83,15 @@ def test_device_spans_with_more_runs_than_the_lists_say_are_reported(C):
     small(p.q, p.gate, p.layer, p.tables, p.starts, [500, 600], meta=meta)
     with pytest.raises(C.KernelError, match="index"):
         C.check_errors(p.q.device)
+
+
+@pytest.mark.parametrize("G", [1, 4])
+def test_decode_behind_the_page_table_is_reported(C, G):
+    p = _Pass(C, [G], [128 - G], width=2)
+    last = torch.arange(128 - G, 128, device=DEV)
+    C.kv8_decode(p.q, p.gate, p.layer, p.tables, last, G)
+    C.check_errors(p.q.device)
+    for beyond in (1, 64, 1 << 40):
+        C.kv8_decode(p.q, p.gate, p.layer, p.tables, last + beyond, G)
+        with pytest.raises(C.KernelError, match="index"):
+            C.check_errors(p.q.device)
