@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(32 * PREP_WARPS)
 attn_prep_kernel(const bf16* qkv, int ld, const int64_t* positions, const int* tables, int max_pages,
                  const int* seq_of_row, const bf16* q_norm, const bf16* k_norm, bf16* q_out,
                  bf16* gate_out, void* kv, uint8_t* exps, int n_q, int n_kv, int rot, float theta, float eps,
-                 int num_pages, int* err) {
+                 int num_pages, int width, int n_seqs, int* err) {
   constexpr int PER = D / 32;
   __shared__ float s_cos[D / 2], s_sin[D / 2];
   __shared__ __align__(16) bf16 s_rot[PREP_WARPS][D];  // a head's normed vector: the rotary partner is another lane's
@@ -131,7 +131,8 @@ attn_prep_kernel(const bf16* qkv, int ld, const int64_t* positions, const int* t
       copy_bf16_vec<PER>(gate_out + (static_cast<size_t>(row) * n_q + head) * D + d0, src + D + d0);
     } else {
       const int seq = seq_of_row[row];
-      const int page = tables[static_cast<size_t>(seq) * max_pages + pos / PAGE];
+      const bool named = !KV8 || (pos >= 0 && pos < static_cast<int64_t>(width) * PAGE && seq >= 0 && seq < n_seqs);  // by the tables
+      const int page = named ? tables[static_cast<size_t>(seq) * max_pages + pos / PAGE] : -1;
       if (page < 0 || page >= num_pages) { if (lane == 0) atomicCAS(err, 0, ERR_BAD_INDEX); continue; }
       const int which = head < n_q + n_kv ? 0 : 1;
       const int kh = which ? head - n_q - n_kv : head - n_q;
@@ -434,7 +435,7 @@ namespace {
 template <bool KV8>
 int prep(const void* qkv, int ld, const int64_t* positions, const int* tables, int max_pages, const int* seq_of_row, const void* q_norm,
          const void* k_norm, void* q_out, void* gate_out, void* kv, void* exps, int rows, int n_q, int n_kv, int D, int rot, float theta,
-         float eps, int num_pages, int* err, cudaStream_t st) {
+         float eps, int num_pages, int width, int n_seqs, int* err, cudaStream_t st) {
   if (rows <= 0) return 0;
   if (rot > D) return -7;
   const int heads = n_q + 2 * n_kv;
@@ -443,7 +444,7 @@ int prep(const void* qkv, int ld, const int64_t* positions, const int* tables, i
   launch_pdl(attn_prep_kernel<DD, KV8>, grid, block, 0, st, static_cast<const bf16*>(qkv), ld, positions, tables,           \
              max_pages, seq_of_row, static_cast<const bf16*>(q_norm), static_cast<const bf16*>(k_norm),                    \
              static_cast<bf16*>(q_out), static_cast<bf16*>(gate_out), kv, static_cast<uint8_t*>(exps), n_q, n_kv, rot, theta, \
-             eps, num_pages, err)
+             eps, num_pages, width, n_seqs, err)
   if (D == 256) PREP(256);
   else if (D == 128) PREP(128);
   else if (D == 64) PREP(64);
@@ -459,16 +460,16 @@ extern "C" int b200_attn_prep(const void* qkv, int ld, const int64_t* positions,
                               void* kv, int rows, int n_q, int n_kv, int D, int rot, float theta, float eps,
                               int num_pages, int* err, cudaStream_t st) {
   return prep<false>(qkv, ld, positions, tables, max_pages, seq_of_row, q_norm, k_norm, q_out, gate_out, kv, nullptr, rows, n_q, n_kv, D, rot,
-                     theta, eps, num_pages, err, st);
+                     theta, eps, num_pages, 0, 0, err, st);
 }
 
-// The same into one layer of the 8-bit cache: data, exps.
+// The same into one layer of the 8-bit cache: data, exps. tables: n_seqs rows of `width` pages, max_pages apart.
 extern "C" int b200_attn_prep_kv8(const void* qkv, int ld, const int64_t* positions, const int* tables, int max_pages,
-                                  const int* seq_of_row, const void* q_norm, const void* k_norm, void* q_out, void* gate_out,
+                                  int width, int n_seqs, const int* seq_of_row, const void* q_norm, const void* k_norm, void* q_out, void* gate_out,
                                   void* data, void* exps, int rows, int n_q, int n_kv, int D, int rot, float theta, float eps,
                                   int num_pages, int* err, cudaStream_t st) {
   return prep<true>(qkv, ld, positions, tables, max_pages, seq_of_row, q_norm, k_norm, q_out, gate_out, data, exps, rows, n_q, n_kv, D, rot,
-                    theta, eps, num_pages, err, st);
+                    theta, eps, num_pages, width, n_seqs, err, st);
 }
 
 extern "C" int b200_paged_attn(const void* q, const void* gate, const void* kv, const int* tables, int max_pages,

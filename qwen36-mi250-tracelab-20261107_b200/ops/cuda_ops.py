@@ -78,7 +78,7 @@ class _Sig:
     b200_gdn_decode = [P, I, P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, P, P]
     b200_gdn_decode_behind_projection = b200_gdn_decode
     b200_attn_prep = [P, I, P, P, I, P, P, P, P, P, P, I, I, I, I, I, F, F, I, P, P]
-    b200_attn_prep_kv8 = [P, I, P, P, I, P, P, P, P, P, P, P, I, I, I, I, I, F, F, I, P, P]
+    b200_attn_prep_kv8 = [P, I, P, P, I, I, I, P, P, P, P, P, P, P, I, I, I, I, I, F, F, I, P, P]
     b200_paged_attn = [P, P, P, P, I, P, P, P, P, I, I, I, I, I, I, I, P]
     b200_gdn_prefill = [P, I, P, P, P, P, P, P, P, P, P, P, P, I, P, I, P, P, P, I, I, I, I, I, F, I, P, P]
     b200_gdn_prefill_work_stride = [I]
@@ -938,12 +938,17 @@ def _kv8_attention(qkv, positions, seq_of_row, block_tables, layer, q_norm, k_no
     if head_dim not in KV8_HEAD_DIMS or not 1 <= n_q // n_kv <= 16:
         return torch_ops.attention(qkv, positions, seq_of_row, block_tables, layer, q_norm, k_norm, n_q, n_kv, head_dim, rotary_dim,
                                    theta, eps, G, seg_starts, seg_pos0)
-    pages, _, _ = check_layer(layer, "attention")
-    rows, dev = qkv.shape[0], qkv.device
+    pages, layer_heads, layer_dim = check_layer(layer, "attention")
+    rows, dev = qkv.shape[0], layer.data.device
+    if (layer_heads, layer_dim) != (n_kv, head_dim) or n_q % n_kv:
+        raise ValueError(f"attention: {n_q} over {n_kv} heads of {head_dim}, an 8-bit KV layer of {layer_heads} heads of {layer_dim}")
+    if qkv.dim() != 2 or qkv.shape[1] < 2 * (n_q + n_kv) * head_dim or qkv.dtype != torch.bfloat16 or qkv.stride(1) != 1 or qkv.device != dev:
+        raise ValueError(f"attention: projected rows {tuple(qkv.shape)} {qkv.dtype} on {qkv.device} are not bf16 [rows, {2 * (n_q + n_kv) * head_dim}] on {dev}")
+    positions, block_tables, seq_of_row, step, width, seqs = _index_tables("attention", dev, rows, positions, block_tables, seq_of_row)
     q = torch.empty(rows, n_q, head_dim, dtype=qkv.dtype, device=dev)
     gate = torch.empty(rows, n_q * head_dim, dtype=qkv.dtype, device=dev)
     _check(lib().b200_attn_prep_kv8(
-        _ptr(qkv), qkv.stride(0), _ptr(positions), _ptr(block_tables), block_tables.stride(0), _ptr(seq_of_row),
+        _ptr(qkv), qkv.stride(0), _ptr(positions), _ptr(block_tables), step, width, seqs, _ptr(seq_of_row),
         _ptr(q_norm), _ptr(k_norm), _ptr(q), _ptr(gate), _ptr(layer.data), _ptr(layer.exps), rows, n_q, n_kv, head_dim, rotary_dim,
         theta, eps, pages, _ptr(err_word(dev)), _stream()), "attn_prep_kv8")
     if G == 0:

@@ -95,3 +95,31 @@ def test_decode_behind_the_page_table_is_reported(C, G):
         C.kv8_decode(p.q, p.gate, p.layer, p.tables, last + beyond, G)
         with pytest.raises(C.KernelError, match="index"):
             C.check_errors(p.q.device)
+
+
+@pytest.mark.parametrize("G", [0, 1])
+def test_the_block_writes_nothing_behind_the_page_table(C, G):
+    """A position that no entry of the row's own table names, a sequence that the tables lack: reported, and no page changes."""
+    n_q, n_kv, D, rows = 16, 2, 256, 3
+    layer = _layer(8, n_kv, D)
+    tables = _tables([128, 128, 100], 2, 8)
+    before = layer.data.view(torch.uint8).clone(), layer.exps.clone()
+    qkv = torch.randn(rows, 2 * (n_q + n_kv) * D, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)).bfloat16()
+    norm = torch.zeros(D, device=DEV).bfloat16()
+    seq = torch.arange(rows, dtype=torch.int32, device=DEV)
+    good = torch.tensor([5, 6, 7], device=DEV)
+
+    def call(positions, seq, layer=layer, qkv=qkv, n_q=n_q, n_kv=n_kv, D=D):
+        return C.attention(qkv, positions, seq, tables, layer, norm, norm, n_q, n_kv, D, D // 4, 1e7, 1e-6, G, [0, 1, 2, 3], [5, 6, 7])
+
+    for positions, of in ((torch.tensor([128, 200, 1 << 33], device=DEV), seq), (good, seq + 3), (good, seq - 3), (torch.tensor([-1, -64, -70], device=DEV), seq)):
+        call(positions, of)
+        with pytest.raises(C.KernelError, match="index"):
+            C.check_errors(qkv.device)
+        assert torch.equal(layer.data.view(torch.uint8), before[0]) and torch.equal(layer.exps, before[1])
+    for wrong in ({"n_kv": 4}, {"D": 128}, {"n_q": 15}, {"qkv": qkv[:, :-1]}, {"qkv": qkv.float()}, {"positions": good[:2]}, {"seq": seq[:2]},
+                  {"layer": _layer(8, 1, D)}):
+        with pytest.raises(ValueError, match="attention"):
+            call(**{"positions": good, "seq": seq, **wrong})
+    call(good.int(), seq.long())  # other index types are taken as for the operators
+    C.check_errors(qkv.device)
