@@ -40,13 +40,20 @@ struct Kv8PrefillParams {
   const int* pos0;          // [segs] its position
   const int* tables;        // [segs] rows of `width` pages, max_pages apart
   bf16* out;                // [T, n_q * D]
-  float* part_acc;          // [T, n_q, max_splits, D]: of spans that are cut
-  float2* part_ml;          // [T, n_q, max_splits]
-  int T, segs, max_pages, width, num_pages, n_q, n_kv, group, positions, max_splits;  // positions: of a tile
+  float* part_acc;          // [part_rows, D]: per span that is cut [rows, n_q, its runs]
+  float2* part_ml;          // [part_rows]
+  long long part_rows;      // 0: no span is cut
+  int T, segs, max_pages, width, num_pages, n_q, n_kv, group, positions;  // positions: of a tile
   int inv_group;            // r * inv_group >> 16 is r / group, for rows below 128 of groups up to 16
   float scale_log2;
   int* err;
 };
+
+// A tile of a span, and its run of pages. part: the span's first partial.
+struct Kv8Tile { int seg, p0, row0, rows, pos0, run_pages, runs, run; long long part; };
+// What a CTA makes of it: rows from `row` on, of n_pos positions from `pos` on, np pages (0: nothing to do) from page `first` of the span's; of a
+// cut span (else runs is 1) the partial of its first row's head 0, the heads' `runs` apart.
+struct Kv8Work { int seg, row, n_pos, pos, first, np, runs; long long part; };
 
 template <int D>
 struct Kv8PrefillCfg {
@@ -58,7 +65,7 @@ struct Kv8PrefillCfg {
   static constexpr int V_BYTES = KV8_PAGE * D * 2;     // [HB][64 rows][128]: values as halves
   static constexpr int P_BYTES = 128 * 128;            // [128 rows][64 halves]
   static constexpr int EXPS = 2 * KV8_PAGE;
-  static constexpr int SMEM = 7 * PAGE_BYTES + 2 * V_BYTES + 2 * P_BYTES + 4 * EXPS + 4 * 3 * KV8_PAGE * 4 + 512 + 54 * 8;
+  static constexpr int SMEM = 7 * PAGE_BYTES + 2 * V_BYTES + 2 * P_BYTES + 4 * EXPS + 4 * 3 * KV8_PAGE * 4 + 512 + 53 * 8 + static_cast<int>(sizeof(Kv8Work));
   static constexpr int TMEM_COLS = 128 + D + D / 2 <= 256 ? 256 : 512;  // two score tiles of 64, the output, two terms of the queries
 };
 
@@ -110,13 +117,15 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   return r;
 }
 
-// The tile of a CTA: found among the spans' tiles by all lanes of a warp, 32 spans at a time. false: there is none. The spans come from device memory
-// that the host may not have seen: one that is not within the T rows and its page table, or that was given too few runs, has no tiles, and leaves an error.
-struct Kv8Tile { int seg, p0, row0, rows, pos0, run_pages; };
-__device__ __forceinline__ bool k8p_find(const Kv8PrefillParams& p, int tile, Kv8Tile& t) {
+// The tile of a CTA, and its run of pages: number `at` of the spans' (run, tile) pairs, found by all lanes of a warp, 32 spans at a time. CUT: number `at`
+// of the tiles of spans that are cut. PARTS: spans may be cut. false: there is none. The spans come from device memory that the host may not have seen: one that is not within the T
+// rows and its page table, or has no room among the partials, has no tiles, and leaves an error, as do more pairs or tiles than the grid has (all: look for them).
+template <bool PARTS, bool CUT>
+__device__ __forceinline__ bool k8p_find(const Kv8PrefillParams& p, int at, bool all, Kv8Tile& t) {
   const int lane = threadIdx.x & 31;
-  int before = 0;
-  for (int s0 = 0; s0 < p.segs; s0 += 32) {
+  int before = 0, parts_before = 0;
+  bool found = false;
+  for (int s0 = 0; s0 < p.segs && (all || !found); s0 += 32) {
     const int s = s0 + lane;
     uint32_t word[3] = {0, 0, 0};  // all three under way at once: each of them is a wait for memory
     ask_32(word[0], p.starts + s, s < p.segs);
@@ -125,38 +134,54 @@ __device__ __forceinline__ bool k8p_find(const Kv8PrefillParams& p, int tile, Kv
     const int a = word[0], b = word[1], pos = word[2];
     int n = (0 <= a) & (a <= b) & (b <= p.T) ? b - a : -1;
     if ((n > 0) & ((pos < 0) | (pos > p.width * KV8_PAGE - n))) n = -1;
-    int run_pages = p.width;
-    if (p.max_splits > 1) {
-      const int np = (pos + n - 1) / KV8_PAGE + 1;
-      run_pages = k8p_run_pages(n, np, p.positions, p.n_kv);
-      if ((n > 0) & (run_pages * p.max_splits < np)) n = -1;
-    }
     if (n < 0) { atomicCAS(p.err, 0, ERR_BAD_INDEX); n = 0; }
     const int tiles = (n + p.positions - 1) / p.positions;
-    int upto = tiles;
+    int run_pages = p.width, runs = 1;
+    if (PARTS && n > 0) {
+      const int np = (pos + n - 1) / KV8_PAGE + 1;
+      run_pages = k8p_run_pages(n, np, p.positions, p.n_kv);
+      runs = (np + run_pages - 1) / run_pages;
+    }
+    const int work = CUT ? (runs > 1 ? tiles : 0) : tiles * runs, parts = runs > 1 ? n * runs : 0;
+    int upto = work;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int u = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += u;
     }
     upto += before;
-    const uint32_t hit = __ballot_sync(0xffffffffu, tile < upto);
-    if (hit) {
-      const int l = __ffs(hit) - 1;
+    const uint32_t hit = __ballot_sync(0xffffffffu, at < upto);
+    if (hit && !found) {
+      found = true;
+      const int l = __ffs(hit) - 1, n_tiles = __shfl_sync(0xffffffffu, tiles, l);
       t.seg = s0 + l;
       t.row0 = __shfl_sync(0xffffffffu, a, l);
       t.rows = __shfl_sync(0xffffffffu, n, l);
-      t.p0 = (tile - __shfl_sync(0xffffffffu, upto - tiles, l)) * p.positions;
       t.pos0 = __shfl_sync(0xffffffffu, pos, l);
       t.run_pages = __shfl_sync(0xffffffffu, run_pages, l);
-      return true;
+      t.runs = __shfl_sync(0xffffffffu, runs, l);
+      const int i = at - __shfl_sync(0xffffffffu, upto - work, l);
+      t.run = CUT || !PARTS || t.runs == 1 ? 0 : i / n_tiles;
+      t.p0 = (i - t.run * n_tiles) * p.positions;
+      t.part = 0;
+      if (PARTS && t.runs > 1) {
+        const int first = parts_before + __reduce_add_sync(0xffffffffu, lane < l ? parts : 0);
+        t.part = static_cast<long long>(first) * p.n_q;
+        if (t.part + static_cast<long long>(t.rows) * t.runs * p.n_q > p.part_rows) {
+          if (lane == 0) atomicCAS(p.err, 0, ERR_BAD_INDEX);
+          return false;
+        }
+      }
     }
     before = __shfl_sync(0xffffffffu, upto, 31);
+    if (PARTS) parts_before += __reduce_add_sync(0xffffffffu, parts);
   }
-  return false;
+  if (all && before > static_cast<int>(gridDim.x) && lane == 0) atomicCAS(p.err, 0, ERR_BAD_INDEX);  // the host counted other spans
+  return found;
 }
 
-template <int D>
+// PARTS: a pass in which a span is cut. (In one form for all, passes without took 1 % longer.)
+template <int D, bool PARTS>
 __global__ void __launch_bounds__(K8P_THREADS, 1)
 kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtensorMap tm_exps, Kv8PrefillParams p) {
   using C = Kv8PrefillCfg<D>;
@@ -199,19 +224,28 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
   uint64_t* const t_empty = bars + 48;                   // [4]
   uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 52);
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile int* const s_cut = abort_flag + 1;            // whether the span is cut: needed at the end, and a register less until then
+  volatile Kv8Work* const s_work = reinterpret_cast<volatile Kv8Work*>(bars + 53);  // what is needed at the end alone stays here until then
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
-  Kv8Tile tile;
-  // the last tiles of the spans see the most keys and go first
-  if (!k8p_find(p, static_cast<int>(gridDim.x - 1 - blockIdx.x), tile)) return;
-  const int kh = blockIdx.y, n_pos = min(p.positions, tile.rows - tile.p0);
-  const int np_all = (tile.pos0 + tile.p0 + n_pos - 1) / KV8_PAGE + 1, np_span = (tile.pos0 + tile.rows - 1) / KV8_PAGE + 1;  // pages that the tile's, the span's rows see
-  const int first = static_cast<int>(blockIdx.z) * tile.run_pages, np = min(np_all, first + tile.run_pages) - first;
-  if (np <= 0) return;  // nothing of this run for these rows: the sum over the runs passes over it
-
-  if (threadIdx.x == 0) {
+  // One warp looks its tile up (all of them would take turns at the same instructions), while others make things ready. The last tiles of the
+  // spans see the most keys and go first.
+  if (warp == 0) {
+    Kv8Tile t = {};
+    const bool found = k8p_find<PARTS, false>(p, static_cast<int>(gridDim.x - 1 - blockIdx.x), (blockIdx.x | blockIdx.y) == 0, t);
+    if (lane == 0) {
+      const int n_pos = min(p.positions, t.rows - t.p0), first = t.run * t.run_pages;
+      s_work->seg = t.seg;
+      s_work->row = t.row0 + t.p0;
+      s_work->n_pos = n_pos;
+      s_work->pos = t.pos0 + t.p0;
+      s_work->first = first;
+      s_work->np = found ? min((t.pos0 + t.p0 + n_pos - 1) / KV8_PAGE + 1, first + t.run_pages) - first : 0;  // up to the last that the tile's rows see
+      s_work->runs = t.runs;
+      s_work->part = t.part + static_cast<long long>(t.p0) * p.n_q * t.runs + t.run;
+    }
+  }
+  if (threadIdx.x == 32) {
     for (int s = 0; s < 2; ++s) {
       mbar_init(&v_full[s], 128); mbar_init(&v_empty[s], 1); mbar_init(&s_full[s], 1); mbar_init(&p_full[s], 128);
       mbar_init(&pv_done[s], 1); mbar_init(&s_empty[s], 128); mbar_init(&m_bar[s], 128);
@@ -226,7 +260,6 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
     mbar_init(q_ready, K8P_THREADS - 64);
     mbar_init(q_full, 256);
     *abort_flag = 0;
-    *s_cut = tile.run_pages < np_span;
     mbar_fence_init();
     tma_prefetch_desc(&tm);
     tma_prefetch_desc(&tm_exps);
@@ -237,6 +270,11 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_launch();  // this CTA holds its TMEM columns
+  const int kh = blockIdx.y, row0 = s_work->row, n_pos = s_work->n_pos, pos0 = s_work->pos, np = s_work->np;
+  if (np <= 0) {  // no tile, or nothing of this run for its rows: the sum over the runs passes over it
+    if (warp == 8) tmem_dealloc(tmem, C::TMEM_COLS);
+    return;
+  }
   const uint32_t tmem_S = tmem, tmem_O = tmem + 128, tmem_Q = tmem_O + D;  // score tile of page i at tmem_S + (i & 1) * 64
   float* const s_qs = reinterpret_cast<float*>(sP);      // until the rows' threads have read it
   constexpr int WARPS = K8P_THREADS / 32 - 2;            // of the warps that convert queries and write outputs
@@ -249,7 +287,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
     for (int i = 0; i < PER; ++i) {
       const int r = w + i * WARPS, lp = r * p.inv_group >> 16;
       raw[i] = make_uint4(0u, 0u, 0u, 0u);
-      ask_128(raw[i], p.q + (static_cast<size_t>(tile.row0 + tile.p0 + lp) * p.n_q + kh * p.group + (r - lp * p.group)) * D + lane * 8,
+      ask_128(raw[i], p.q + (static_cast<size_t>(row0 + lp) * p.n_q + kh * p.group + (r - lp * p.group)) * D + lane * 8,
               r < 128 && lp < n_pos && lane * 8 < D);
     }
 #pragma unroll
@@ -284,11 +322,11 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
 
   if (warp == 9) {
     // ---------------- loads. The gates are needed at the end, when other loads of this SM's neighbours are under way: they are brought to L2 now.
-    for (int i = *s_cut ? n_pos : lane; i < n_pos; i += 32)
+    for (int i = PARTS && s_work->runs > 1 ? n_pos : lane; i < n_pos; i += 32)
       asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;"
-                     ::"l"(p.gate + (static_cast<size_t>(tile.row0 + tile.p0 + i) * p.n_q + kh * p.group) * D), "r"(p.group * D * 2) : "memory");
+                     ::"l"(p.gate + (static_cast<size_t>(row0 + i) * p.n_q + kh * p.group) * D), "r"(p.group * D * 2) : "memory");
     if (elect_one()) {
-      const int* table = p.tables + static_cast<size_t>(tile.seg) * p.max_pages + first;
+      const int* table = p.tables + static_cast<size_t>(s_work->seg) * p.max_pages + s_work->first;
       int next = table[0], i = 0;
       for (; i < np; ++i) {
         const int s = i & 3, ks = i % 3;
@@ -431,8 +469,9 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
     const int r = threadIdx.x & 127, hf = threadIdx.x >> 7, rw = warp & 3;
     const uint32_t lane_base = static_cast<uint32_t>(rw * 32) << 16;
     const int lp = r * p.inv_group >> 16, head = r - lp * p.group;
-    const int qpos = tile.pos0 + tile.p0 + lp;
+    const int qpos = pos0 + lp;
     const bool row_valid = lp < n_pos;
+    const int key0 = s_work->first * KV8_PAGE;
     constexpr int DH = D / 2;
     float m_loc = -INFINITY;  // the maximum and the sum of this thread's own pages, at that maximum
     float2 l2 = make_float2(0.f, 0.f);
@@ -468,8 +507,8 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
         y[2 * j] = fma2(mul2(y[2 * j], qs2), make_float2(a.x, a.y), make_float2(b.x, b.y));
         y[2 * j + 1] = fma2(mul2(y[2 * j + 1], qs2), make_float2(a.z, a.w), make_float2(b.z, b.w));
       }
-      const int kbase = (first + i) * KV8_PAGE;
-      if (kbase + KV8_PAGE - 1 > tile.pos0 + tile.p0) {  // only pages that end behind the tile's first query hide keys
+      const int kbase = key0 + i * KV8_PAGE;
+      if (kbase + KV8_PAGE - 1 > pos0) {  // only pages that end behind the tile's first query hide keys
 #pragma unroll
         for (int j = 0; j < 32; ++j) {
           y[j].x = kbase + 2 * j <= qpos ? y[j].x : -INFINITY;
@@ -555,13 +594,14 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
       ok = mbar_wait(x_bar, 0, p.err, ERR_WAIT_FULL, abort_flag);
       const float l0 = ex[r * 2], m0 = ex[r * 2 + 1], l1 = ex[(128 + r) * 2], m1 = ex[(128 + r) * 2 + 1];
       m_used = fmaxf(m0, m1);  // a running maximum never falls: the larger one is the last page's
-      l = m_used == -INFINITY ? l0 + l1 : l0 * k8p_ex2(m0 - m_used) + l1 * k8p_ex2(m1 - m_used);
+      l = m_used == -INFINITY ? l0 + l1 : fmaf(l0, k8p_ex2(m0 - m_used), l1 * k8p_ex2(m1 - m_used));
     }
     // The outputs go through shared memory, 16 bytes of a row in the place of their number XOR the row, so that a warp reads gates and
     // writes outputs of a whole row at a time (with a thread a row from TMEM to the output, the end of a tile took 13 us).
     float* const so = reinterpret_cast<float*>(sQ);        // [128][D], in the place of Q and the pages' bytes
     if (ok) {
-      const bool cut = *s_cut;
+      const int runs = PARTS ? s_work->runs : 1;
+      const bool cut = runs > 1;
       const float inv = cut ? 1.0f : 1.0f / l;             // (a row sees itself)
 #pragma unroll 1
       for (int c = hf * DH; c < hf * DH + DH; c += 16) {
@@ -573,7 +613,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
               make_float4(o[4 * j] * inv, o[4 * j + 1] * inv, o[4 * j + 2] * inv, o[4 * j + 3] * inv);
       }
       if (cut && row_valid && hf == 0)
-        p.part_ml[((static_cast<size_t>(tile.row0 + tile.p0 + lp) * p.n_q + kh * p.group + head)) * p.max_splits + blockIdx.z] = make_float2(m_used, l);
+        p.part_ml[s_work->part + (lp * p.n_q + kh * p.group + head) * runs] = make_float2(m_used, l);
       mbar_arrive(o_full);
     }
   }
@@ -581,12 +621,14 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
     // ---------------- outputs, a warp whole rows at a time, their gates ahead of the last products
     constexpr int LANES = D / 8, ROWS = 32 / LANES, STEPS = (128 + WARPS * ROWS - 1) / (WARPS * ROWS);  // 8 numbers a lane, rows a warp takes at once
     const int sub = lane / LANES, d = lane % LANES * 8, n_rows = n_pos * p.group;
-    const size_t head0 = static_cast<size_t>(tile.row0 + tile.p0) * p.n_q + kh * p.group;
+    const size_t head0 = static_cast<size_t>(row0) * p.n_q + kh * p.group;
     const auto head_of = [&](int row) {
       const int pos = row * p.inv_group >> 16;
       return head0 + static_cast<size_t>(pos) * p.n_q + (row - pos * p.group);
     };
-    const bool cut = *s_cut;
+    const int runs = PARTS ? s_work->runs : 1;
+    const bool cut = runs > 1;
+    float* const dst0 = p.part_acc + (cut ? s_work->part + kh * p.group * runs : 0) * D + d;
     uint4 gate[STEPS];
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
@@ -604,7 +646,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
         const float4 a = *reinterpret_cast<const float4*>(src + ((d >> 2) ^ (row & 7)) * 4), b = *reinterpret_cast<const float4*>(src + (((d >> 2) + 1) ^ (row & 7)) * 4);
         const size_t at = head_of(row);
         if (cut) {
-          float* const dst = p.part_acc + (at * p.max_splits + blockIdx.z) * D + d;
+          float* const dst = dst0 + static_cast<int>(at - head0) * runs * D;
           *reinterpret_cast<float4*>(dst) = a;
           *reinterpret_cast<float4*>(dst + 4) = b;
         } else {
@@ -634,13 +676,12 @@ __global__ void __launch_bounds__(128)
 kv8_prefill_combine_kernel(Kv8PrefillParams p) {
   constexpr int QUADS = D / 4, AT_ONCE = 8;
   Kv8Tile tile = {};
-  const bool found = k8p_find(p, blockIdx.x, tile);
-  const int np = (tile.pos0 + tile.rows - 1) / KV8_PAGE + 1, run_pages = tile.run_pages;
+  const bool found = k8p_find<true, true>(p, blockIdx.x, (blockIdx.x | blockIdx.y | blockIdx.z) == 0, tile);
   const int n_pos = min(p.positions, tile.rows - tile.p0), i = blockIdx.z * (128 / QUADS) + threadIdx.x / QUADS;
-  const bool work = found && run_pages < np && i < n_pos * p.group;
-  const int np_all = (tile.pos0 + tile.p0 + n_pos - 1) / KV8_PAGE + 1, runs = (np_all + run_pages - 1) / run_pages;  // that wrote
-  const int pos = i * p.inv_group >> 16, quad = threadIdx.x % QUADS;
-  const size_t at = static_cast<size_t>(tile.row0 + tile.p0 + pos) * p.n_q + blockIdx.y * p.group + (i - pos * p.group);
+  const bool work = found && i < n_pos * p.group;
+  const int np_all = (tile.pos0 + tile.p0 + n_pos - 1) / KV8_PAGE + 1, runs = found ? (np_all + tile.run_pages - 1) / tile.run_pages : 0;  // that wrote
+  const int pos = i * p.inv_group >> 16, quad = threadIdx.x % QUADS, head = blockIdx.y * p.group + (i - pos * p.group);
+  const size_t at = static_cast<size_t>(tile.row0 + tile.p0 + pos) * p.n_q + head;
   // Threads without work leave before the wait, so that the grid does not come in waves behind it; those of the first CTA stay: this kernel must
   // not end before the one in front, for whose end what comes next takes it.
   if (!work && (blockIdx.x | blockIdx.y | blockIdx.z) != 0) return;
@@ -648,8 +689,9 @@ kv8_prefill_combine_kernel(Kv8PrefillParams p) {
   pdl_wait();
   pdl_launch();
   if (!work) return;
-  const float2* ml = p.part_ml + at * p.max_splits;
-  const float4* pa = reinterpret_cast<const float4*>(p.part_acc + at * p.max_splits * D) + quad;
+  const size_t part = tile.part + (static_cast<size_t>(tile.p0 + pos) * p.n_q + head) * tile.runs;
+  const float2* ml = p.part_ml + part;
+  const float4* pa = reinterpret_cast<const float4*>(p.part_acc + part * D) + quad;
   float2 pm[AT_ONCE];
   float4 v[AT_ONCE];
   const auto ask = [&](int z0) {
@@ -707,18 +749,18 @@ int k8p_encode(CUtensorMap* m, const void* base, int rank, const cuuint64_t* dim
             CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : -2;
 }
 template <int D>
-int k8p_launch(const CUtensorMap& tm, const CUtensorMap& te, const Kv8PrefillParams& p, int n_tiles, cudaStream_t st) {
-  auto kern = kv8_prefill_kernel<D>;
-  static bool configured[64] = {};  // a function attribute is set per device
+int k8p_launch(const CUtensorMap& tm, const CUtensorMap& te, const Kv8PrefillParams& p, int pairs, int cut_tiles, cudaStream_t st) {
+  auto kern = cut_tiles > 0 ? kv8_prefill_kernel<D, true> : kv8_prefill_kernel<D, false>;
+  static bool configured[2][64] = {};  // a function attribute is set per device
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -3;
-  if (!configured[dev]) {
+  if (!configured[cut_tiles > 0][dev]) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Kv8PrefillCfg<D>::SMEM) != cudaSuccess) return -3;
-    configured[dev] = true;
+    configured[cut_tiles > 0][dev] = true;
   }
-  if (launch_pdl(kern, dim3(n_tiles, p.n_kv, p.max_splits), dim3(K8P_THREADS), Kv8PrefillCfg<D>::SMEM, st, tm, te, p) != cudaSuccess) return -4;
-  if (p.max_splits == 1) return 0;
-  return launch_pdl(kv8_prefill_combine_kernel<D>, dim3(n_tiles, p.n_kv, 128 / (128 / (D / 4))), dim3(128), 0, st, p) == cudaSuccess ? 0 : -4;
+  if (launch_pdl(kern, dim3(pairs, p.n_kv), dim3(K8P_THREADS), Kv8PrefillCfg<D>::SMEM, st, tm, te, p) != cudaSuccess) return -4;
+  if (cut_tiles == 0) return 0;
+  return launch_pdl(kv8_prefill_combine_kernel<D>, dim3(cut_tiles, p.n_kv, 128 / (128 / (D / 4))), dim3(128), 0, st, p) == cudaSuccess ? 0 : -4;
 }
 }  // namespace
 
@@ -727,14 +769,15 @@ extern "C" int b200_kv8_prefill_positions(int group) { return group >= 1 && grou
 extern "C" int b200_kv8_prefill_cut(int which) { return which ? K8P_MIN_PAGES : K8P_CTAS; }
 
 // q: [T, n_q, D] bf16 (normed and rotated), gate, out: [T, n_q * D], in 16-byte rows; data, exps: one layer of the 8-bit cache, which holds the
-// spans' own keys; starts [segs + 1], pos0 [segs] of the spans, within T rows, tables [segs] rows of `width` pages. n_tiles: at least the spans' tiles.
-// max_splits: the most runs of a span (part_acc [T, n_q, max_splits, D], part_ml [.., 2] where there is more than one).
+// spans' own keys; starts [segs + 1], pos0 [segs] of the spans, within T rows, tables [segs] rows of `width` pages. pairs: at least the spans' tiles, each
+// times its span's runs; cut_tiles: at least those of spans that are cut; part_rows: their rows' heads, times their runs (part_acc [part_rows, D],
+// part_ml [part_rows, 2]); of the last two either both or none.
 extern "C" int b200_kv8_prefill(const void* q, const void* gate, const void* data, const void* exps, const int* starts, const int* pos0,
-                                int T, int segs, int n_tiles, const int* tables, int max_pages, int width, int num_pages, int n_q, int n_kv,
-                                int D, int max_splits, float* part_acc, float* part_ml, void* out, int* err, cudaStream_t st) {
-  if (n_tiles <= 0 || segs <= 0) return 0;
+                                int T, int segs, int pairs, int cut_tiles, long long part_rows, const int* tables, int max_pages, int width,
+                                int num_pages, int n_q, int n_kv, int D, float* part_acc, float* part_ml, void* out, int* err, cudaStream_t st) {
+  if (pairs <= 0 || segs <= 0) return 0;
   const int group = n_kv > 0 ? n_q / n_kv : 0;
-  if (group < 1 || group * n_kv != n_q || group > 16 || max_splits < 1 || width < 1 || width > 0x7fffffff / KV8_PAGE) return -7;
+  if (group < 1 || group * n_kv != n_q || group > 16 || cut_tiles < 0 || (cut_tiles > 0) != (part_rows > 0) || width < 1 || width > 0x7fffffff / KV8_PAGE) return -7;
   if (D != 256 && D != 128 && D != 64) return -7;
   const long long rows = static_cast<long long>(num_pages) * 2 * n_kv * KV8_PAGE;
   if (rows > 0x7fffffffLL) return -7;  // a TMA coordinate
@@ -750,9 +793,9 @@ extern "C" int b200_kv8_prefill(const void* q, const void* gate, const void* dat
   if (k8p_encode(&tm, data, 2, dims, strides, box, rowb == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B) ||
       k8p_encode(&te, exps, 3, edims, estrides, ebox, CU_TENSOR_MAP_SWIZZLE_NONE)) return -1;
   const Kv8PrefillParams p{static_cast<const bf16*>(q), static_cast<const bf16*>(gate), starts, pos0, tables, static_cast<bf16*>(out), part_acc,
-                           reinterpret_cast<float2*>(part_ml), T, segs, max_pages, width, num_pages, n_q, n_kv, group, 128 / group, max_splits,
+                           reinterpret_cast<float2*>(part_ml), part_rows, T, segs, max_pages, width, num_pages, n_q, n_kv, group, 128 / group,
                            (65536 + group - 1) / group, 1.4426950408889634f / sqrtf(static_cast<float>(D)), err};
-  if (D == 256) return k8p_launch<256>(tm, te, p, n_tiles, st);
-  if (D == 128) return k8p_launch<128>(tm, te, p, n_tiles, st);
-  return k8p_launch<64>(tm, te, p, n_tiles, st);
+  if (D == 256) return k8p_launch<256>(tm, te, p, pairs, cut_tiles, st);
+  if (D == 128) return k8p_launch<128>(tm, te, p, pairs, cut_tiles, st);
+  return k8p_launch<64>(tm, te, p, pairs, cut_tiles, st);
 }

@@ -92,7 +92,7 @@ class _Sig:
     b200_kv8_decode_run = []
     b200_kv8_prefill_positions = [I]
     b200_kv8_prefill_cut = [I]
-    b200_kv8_prefill = [P, P, P, P, P, P, I, I, I, P, I, I, I, I, I, I, I, P, P, P, P, P]
+    b200_kv8_prefill = [P, P, P, P, P, P, I, I, I, I, L, P, I, I, I, I, I, I, P, P, P, P, P]
     b200_kv8_decode = [P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, P, P, P, P, P]
 
 
@@ -811,6 +811,9 @@ def kv8_read(layer: Kv8Layer, positions: torch.Tensor, seq_of_row: torch.Tensor,
 
 
 KV8_HEAD_DIMS = (64, 128, 256)  # of the attention kernels over the 8-bit cache
+# Bytes of partials that one launch of kv8_prefill may take. A span that is cut takes up to 17 MB of them (heads of 256): a pass of more cut spans than
+# fit goes out in several launches, each of 15 such spans and twelve waves of CTAs at the least.
+KV8_PREFILL_PARTS = 256 << 20
 
 
 def _kv8_queries(what: str, q: torch.Tensor, gate: torch.Tensor, n_kv: int, D: int, dev: torch.device):
@@ -887,27 +890,35 @@ def kv8_prefill(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tabl
         for t in meta:
             if t.dtype != torch.int32 or t.device != dev or t.dim() != 1 or t.stride(0) != 1:
                 raise ValueError(f"kv8_prefill: meta holds contiguous int32 vectors on {dev}, not {t.dtype} {tuple(t.shape)} with strides {t.stride()} on {t.device}")
-    splits = 1
+    # Launches: spans s0 .. s1, the (tile, run) pairs, the tiles of cut spans, their rows times their runs.
+    launches, s0, pairs, cut_tiles, part = [], 0, 0, 0, 0
     if seg_starts is not None:
         n_seg = len(seg_pos0)
         lens = [b - a for a, b in zip(seg_starts, seg_starts[1:])]
         if len(lens) != n_seg or seg_starts[0] != 0 or seg_starts[-1] != T or seqs < n_seg or min(lens, default=0) < 0:
             raise ValueError(f"kv8_prefill: spans {seg_starts} with {n_seg} first positions do not make {T} rows of at most {seqs} sequences")
-        n_tiles = 0
         ctas, least = L.b200_kv8_prefill_cut(0), L.b200_kv8_prefill_cut(1)
-        for n, pos in zip(lens, seg_pos0):
+        most = KV8_PREFILL_PARTS // (n_q * (D + 2) * 4)
+        for i, (n, pos) in enumerate(zip(lens, seg_pos0)):
             if pos < 0 or pos + n > width * PAGE_SIZE:
                 raise ValueError(f"kv8_prefill: rows at positions {pos} .. {pos + n - 1}, page tables of {width} pages")
             tiles = -(-n // per)
-            n_tiles += tiles
             if 0 < 2 * tiles * n_kv <= ctas:  # into so many runs is the span cut (kv8_prefill.cu, k8p_run_pages)
                 seen = (pos + n - 1) // PAGE_SIZE + 1
-                splits = max(splits, -(-seen // max(least, -(-seen // (ctas // (tiles * n_kv))))))
+                runs = -(-seen // max(least, -(-seen // (ctas // (tiles * n_kv)))))
+                if runs > 1:
+                    if part and part + n * runs > most:
+                        launches.append((s0, i, pairs, cut_tiles, part))
+                        s0, pairs, cut_tiles, part = i, 0, 0, 0
+                    cut_tiles += tiles
+                    part += n * runs
+                    tiles *= runs
+            pairs += tiles
     elif meta is None:
         raise ValueError("kv8_prefill: neither the spans' lists nor their device tensors")
     else:
         n_seg = pos0_t.shape[0]
-        n_tiles = T // per + n_seg
+        pairs = T // per + n_seg
         if seqs < n_seg:
             raise ValueError(f"kv8_prefill: meta of {n_seg} spans, page tables of {seqs} sequences")
     if meta is not None:
@@ -919,16 +930,19 @@ def kv8_prefill(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tabl
     out = torch.empty_like(gate)
     if T == 0:
         return out
+    launches.append((s0, n_seg, pairs, cut_tiles, part))
     acc = ml = None
-    if splits > 1:  # partials: sums, then maxima and sums of weights
-        part = T * n_q * splits * 4
-        scratch = data.new_empty(part * (D + 2))  # bytes, as above
+    if part or len(launches) > 1:  # partials of the cut spans' rows: sums, then maxima and sums of weights
+        rows = max(x[4] for x in launches) * n_q * 4
+        scratch = data.new_empty(rows * (D + 2))  # bytes, as above
         acc = scratch.data_ptr()
-        ml = acc + part * D
-    _check(L.b200_kv8_prefill(
-        q.data_ptr(), gate.data_ptr(), data.data_ptr(), exps.data_ptr(), starts_t.data_ptr(), pos0_t.data_ptr(), T, n_seg, n_tiles,
-        block_tables.data_ptr(), step, width, pages, n_q, n_kv, D, splits, acc, ml, out.data_ptr(), _err_ptr(dev),
-        _raw_stream(dev)), "kv8_prefill")
+        ml = acc + rows * D
+    starts_p, pos0_p, tables_p = starts_t.data_ptr(), pos0_t.data_ptr(), block_tables.data_ptr()
+    err, st = _err_ptr(dev), _raw_stream(dev)
+    for a, b, pairs, cut_tiles, part in launches:
+        _check(L.b200_kv8_prefill(
+            q.data_ptr(), gate.data_ptr(), data.data_ptr(), exps.data_ptr(), starts_p + 4 * a, pos0_p + 4 * a, T, b - a, pairs, cut_tiles,
+            part * n_q, tables_p + 4 * a * step, step, width, pages, n_q, n_kv, D, acc, ml, out.data_ptr(), err, st), "kv8_prefill")
     return out
 
 

@@ -123,3 +123,57 @@ def test_the_block_writes_nothing_behind_the_page_table(C, G):
             call(**{"positions": good, "seq": seq, **wrong})
     call(good.int(), seq.long())  # other index types are taken as for the operators
     C.check_errors(qkv.device)
+
+
+# ------------------------------------------------------------------ unlike spans in one pass
+def test_partials_go_by_the_cut_rows_alone(C):
+    """Sixteen rows on a long context are cut into 57 runs; the 6,144 rows beside them are not, and take no partials."""
+    p = _Pass(C, [16, 2048, 2048, 2048], [32768, 0, 0, 0])
+    alone = [p.alone(i) for i in range(4)]
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = p.packed()
+    torch.cuda.synchronize()
+    taken = torch.cuda.max_memory_allocated() - before - got.numel() * got.element_size()
+    C.check_errors(got.device)
+    assert taken <= 17 << 20  # 128 CTAs of 128 rows of 258 numbers
+    for i in range(4):
+        assert torch.equal(got[p.starts[i] : p.starts[i + 1]], alone[i]), i
+    p.check(got, [0])
+
+
+MANY = ([(i * 37) % 50 + (i % 5 == 0) * 150 for i in range(75)], [(i * 977) % 4000 for i in range(75)])  # 75 spans, one of them empty
+
+
+@pytest.mark.parametrize("heads", [(16, 2, 256), (6, 3, 128), (8, 1, 64)])
+def test_more_spans_than_a_warp_looks_at_once(C, heads):
+    p = _Pass(C, *MANY, heads=heads)
+    got = p.packed()
+    assert torch.equal(p.packed(meta=False), got)
+    for i in range(0, 75, 7):
+        assert torch.equal(got[p.starts[i] : p.starts[i + 1]], p.alone(i)), i
+    C.check_errors(got.device)
+    p.check(got, [0, 1, 31, 32, 33, 63, 64, 74])
+
+
+def test_a_pass_of_more_partials_than_a_launch_takes(C, monkeypatch):
+    p = _Pass(C, *MANY)
+    want, n0 = p.packed(), C.launch_count()
+    p.packed()
+    one = C.launch_count() - n0
+    monkeypatch.setattr(C, "KV8_PREFILL_PARTS", 40 << 20)
+    n0 = C.launch_count()
+    got = p.packed()
+    assert C.launch_count() - n0 > 2 * one
+    assert torch.equal(got, want)
+    C.check_errors(got.device)
+
+
+def test_lists_that_are_not_the_tensors_numbers_are_reported(C):
+    """Fewer tiles, less room for partials, fewer tiles that are cut than the tensors' spans make."""
+    p = _Pass(C, [40, 70], [700, 600], width=13)
+    for starts, pos0 in (([0, 110, 110], [0, 0]), ([0, 5, 110], [700, 0]), ([0, 110, 110], [700, 0])):
+        p.C.kv8_prefill(p.q, p.gate, p.layer, p.tables, starts, pos0, meta=p.meta)
+        with pytest.raises(C.KernelError, match="index"):
+            C.check_errors(p.q.device)
