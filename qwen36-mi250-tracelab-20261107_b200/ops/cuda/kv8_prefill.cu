@@ -44,6 +44,7 @@ struct Kv8PrefillParams {
   float2* part_ml;          // [part_rows]
   long long part_rows;      // 0: no span is cut
   int T, segs, max_pages, width, num_pages, n_q, n_kv, group, positions;  // positions: of a tile
+  int exact;                // the grid has as many pairs as the spans
   int inv_group;            // r * inv_group >> 16 is r / group, for rows below 128 of groups up to 16
   float scale_log2;
   int* err;
@@ -229,10 +230,10 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   // One warp looks its tile up (all of them would take turns at the same instructions), while others make things ready. The last tiles of the
-  // spans see the most keys and go first.
+  // spans see the most keys and go first, where no CTA without a pair goes ahead of them.
   if (warp == 0) {
     Kv8Tile t = {};
-    const bool found = k8p_find<PARTS, false>(p, static_cast<int>(gridDim.x - 1 - blockIdx.x), (blockIdx.x | blockIdx.y) == 0, t);
+    const bool found = k8p_find<PARTS, false>(p, static_cast<int>(p.exact ? gridDim.x - 1 - blockIdx.x : blockIdx.x), (blockIdx.x | blockIdx.y) == 0, t);
     if (lane == 0) {
       const int n_pos = min(p.positions, t.rows - t.p0), first = t.run * t.run_pages;
       s_work->seg = t.seg;
@@ -770,10 +771,10 @@ extern "C" int b200_kv8_prefill_cut(int which) { return which ? K8P_MIN_PAGES : 
 
 // q: [T, n_q, D] bf16 (normed and rotated), gate, out: [T, n_q * D], in 16-byte rows; data, exps: one layer of the 8-bit cache, which holds the
 // spans' own keys; starts [segs + 1], pos0 [segs] of the spans, within T rows, tables [segs] rows of `width` pages. pairs: at least the spans' tiles, each
-// times its span's runs; cut_tiles: at least those of spans that are cut; part_rows: their rows' heads, times their runs (part_acc [part_rows, D],
+// times its span's runs (exact: no more than those); cut_tiles: at least those of spans that are cut; part_rows: their rows' heads, times their runs (part_acc [part_rows, D],
 // part_ml [part_rows, 2]); of the last two either both or none.
 extern "C" int b200_kv8_prefill(const void* q, const void* gate, const void* data, const void* exps, const int* starts, const int* pos0,
-                                int T, int segs, int pairs, int cut_tiles, long long part_rows, const int* tables, int max_pages, int width,
+                                int T, int segs, int pairs, int exact, int cut_tiles, long long part_rows, const int* tables, int max_pages, int width,
                                 int num_pages, int n_q, int n_kv, int D, float* part_acc, float* part_ml, void* out, int* err, cudaStream_t st) {
   if (pairs <= 0 || segs <= 0) return 0;
   const int group = n_kv > 0 ? n_q / n_kv : 0;
@@ -793,7 +794,7 @@ extern "C" int b200_kv8_prefill(const void* q, const void* gate, const void* dat
   if (k8p_encode(&tm, data, 2, dims, strides, box, rowb == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B) ||
       k8p_encode(&te, exps, 3, edims, estrides, ebox, CU_TENSOR_MAP_SWIZZLE_NONE)) return -1;
   const Kv8PrefillParams p{static_cast<const bf16*>(q), static_cast<const bf16*>(gate), starts, pos0, tables, static_cast<bf16*>(out), part_acc,
-                           reinterpret_cast<float2*>(part_ml), part_rows, T, segs, max_pages, width, num_pages, n_q, n_kv, group, 128 / group,
+                           reinterpret_cast<float2*>(part_ml), part_rows, T, segs, max_pages, width, num_pages, n_q, n_kv, group, 128 / group, exact,
                            (65536 + group - 1) / group, 1.4426950408889634f / sqrtf(static_cast<float>(D)), err};
   if (D == 256) return k8p_launch<256>(tm, te, p, pairs, cut_tiles, st);
   if (D == 128) return k8p_launch<128>(tm, te, p, pairs, cut_tiles, st);

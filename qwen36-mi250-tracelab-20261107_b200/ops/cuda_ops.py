@@ -92,7 +92,7 @@ class _Sig:
     b200_kv8_decode_run = []
     b200_kv8_prefill_positions = [I]
     b200_kv8_prefill_cut = [I]
-    b200_kv8_prefill = [P, P, P, P, P, P, I, I, I, I, L, P, I, I, I, I, I, I, P, P, P, P, P]
+    b200_kv8_prefill = [P, P, P, P, P, P, I, I, I, I, I, L, P, I, I, I, I, I, I, P, P, P, P, P]
     b200_kv8_decode = [P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, P, P, P, P, P]
 
 
@@ -869,8 +869,8 @@ def kv8_prefill(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tabl
     a short span is cut into runs for CTAs of their own, by the span's own rows and position: a row's bits do not depend on the other spans.
 
     ``meta``: ``(seg_starts, seg_pos0)`` as int32 device tensors that the caller keeps, of the same numbers; without it every call uploads
-    them. With ``meta`` the lists may be None, which lets the call be captured in a CUDA graph: no span is cut then. A span in ``meta`` that is not
-    within the rows and its page table is left out, and reported by ``check_errors``."""
+    them. With ``meta`` the lists may be None, which lets the call be captured in a CUDA graph: spans are cut as they would be with them, and the bits
+    are the same. A span in ``meta`` that is not within the rows and its page table is left out, and reported by ``check_errors``."""
     pages, n_kv, D = check_layer(layer, "kv8_prefill")
     data, exps = layer
     dev = data.device
@@ -891,14 +891,15 @@ def kv8_prefill(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tabl
             if t.dtype != torch.int32 or t.device != dev or t.dim() != 1 or t.stride(0) != 1:
                 raise ValueError(f"kv8_prefill: meta holds contiguous int32 vectors on {dev}, not {t.dtype} {tuple(t.shape)} with strides {t.stride()} on {t.device}")
     # Launches: spans s0 .. s1, the (tile, run) pairs, the tiles of cut spans, their rows times their runs.
-    launches, s0, pairs, cut_tiles, part = [], 0, 0, 0, 0
+    launches = []
+    ctas, least = L.b200_kv8_prefill_cut(0), L.b200_kv8_prefill_cut(1)
+    most = KV8_PREFILL_PARTS // (n_q * (D + 2) * 4)
     if seg_starts is not None:
         n_seg = len(seg_pos0)
         lens = [b - a for a, b in zip(seg_starts, seg_starts[1:])]
-        if len(lens) != n_seg or seg_starts[0] != 0 or seg_starts[-1] != T or seqs < n_seg or min(lens, default=0) < 0:
+        if not seg_starts or len(lens) != n_seg or seg_starts[0] != 0 or seg_starts[-1] != T or seqs < n_seg or min(lens, default=0) < 0:
             raise ValueError(f"kv8_prefill: spans {seg_starts} with {n_seg} first positions do not make {T} rows of at most {seqs} sequences")
-        ctas, least = L.b200_kv8_prefill_cut(0), L.b200_kv8_prefill_cut(1)
-        most = KV8_PREFILL_PARTS // (n_q * (D + 2) * 4)
+        s0 = pairs = cut_tiles = part = 0
         for i, (n, pos) in enumerate(zip(lens, seg_pos0)):
             if pos < 0 or pos + n > width * PAGE_SIZE:
                 raise ValueError(f"kv8_prefill: rows at positions {pos} .. {pos + n - 1}, page tables of {width} pages")
@@ -914,13 +915,24 @@ def kv8_prefill(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tabl
                     part += n * runs
                     tiles *= runs
             pairs += tiles
+        launches.append((s0, n_seg, pairs, cut_tiles, part))
     elif meta is None:
         raise ValueError("kv8_prefill: neither the spans' lists nor their device tensors")
     else:
         n_seg = pos0_t.shape[0]
-        pairs = T // per + n_seg
         if seqs < n_seg:
             raise ValueError(f"kv8_prefill: meta of {n_seg} spans, page tables of {seqs} sequences")
+        # The spans are not known here, and are cut as they would be by their lists: room for the most that they can come to. A span that is cut
+        # has at most ctas / n_kv pairs, of half as many tiles, and at least one.
+        each, runs = ctas // n_kv, -(-width // least)
+        if each < 2 or runs < 2:
+            launches.append((0, n_seg, T // per + n_seg, 0, 0))
+        else:
+            at_once = max(1, most // (per * each))
+            for a in range(0, n_seg, at_once):
+                n = min(at_once, n_seg - a)
+                tiles = T // per + n
+                launches.append((a, a + n, min(tiles * runs, tiles + n * each), min(tiles, n * (each // 2)), min(n * per * each, T * runs)))
     if meta is not None:
         if starts_t.shape[0] < n_seg + 1 or pos0_t.shape[0] < n_seg:
             raise ValueError(f"kv8_prefill: meta of {starts_t.shape[0]} and {pos0_t.shape[0]} numbers for {n_seg} spans")
@@ -930,10 +942,10 @@ def kv8_prefill(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tabl
     out = torch.empty_like(gate)
     if T == 0:
         return out
-    launches.append((s0, n_seg, pairs, cut_tiles, part))
     acc = ml = None
-    if part or len(launches) > 1:  # partials of the cut spans' rows: sums, then maxima and sums of weights
-        rows = max(x[4] for x in launches) * n_q * 4
+    part = max((x[4] for x in launches), default=0)
+    if part:  # of the cut spans' rows: sums, then maxima and sums of weights
+        rows = part * n_q * 4
         scratch = data.new_empty(rows * (D + 2))  # bytes, as above
         acc = scratch.data_ptr()
         ml = acc + rows * D
@@ -941,8 +953,9 @@ def kv8_prefill(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tabl
     err, st = _err_ptr(dev), _raw_stream(dev)
     for a, b, pairs, cut_tiles, part in launches:
         _check(L.b200_kv8_prefill(
-            q.data_ptr(), gate.data_ptr(), data.data_ptr(), exps.data_ptr(), starts_p + 4 * a, pos0_p + 4 * a, T, b - a, pairs, cut_tiles,
-            part * n_q, tables_p + 4 * a * step, step, width, pages, n_q, n_kv, D, acc, ml, out.data_ptr(), err, st), "kv8_prefill")
+            q.data_ptr(), gate.data_ptr(), data.data_ptr(), exps.data_ptr(), starts_p + 4 * a, pos0_p + 4 * a, T, b - a, pairs,
+            seg_starts is not None, cut_tiles, part * n_q, tables_p + 4 * a * step, step, width, pages, n_q, n_kv, D, acc, ml,
+            out.data_ptr(), err, st), "kv8_prefill")
     return out
 
 

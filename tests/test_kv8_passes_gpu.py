@@ -177,3 +177,72 @@ def test_lists_that_are_not_the_tensors_numbers_are_reported(C):
         p.C.kv8_prefill(p.q, p.gate, p.layer, p.tables, starts, pos0, meta=p.meta)
         with pytest.raises(C.KernelError, match="index"):
             C.check_errors(p.q.device)
+
+
+# ------------------------------------------------------------------ captured passes
+@pytest.mark.parametrize("heads", [(16, 2, 256), (8, 8, 64), (6, 3, 128)])
+@pytest.mark.parametrize("lens,pos0", [([61], [3584]), ([600], [0]), ([64], [704]), ([1, 17, 300], [5000, 900, 40]), ([2000, 30], [100, 4000]), ([5], [100])])
+@pytest.mark.parametrize("width", [None, 600])
+def test_spans_from_device_memory_are_cut_as_from_the_lists(C, heads, lens, pos0, width):
+    p = _Pass(C, lens, pos0, heads, width=width)
+    want = p.packed()
+    assert torch.equal(p.from_device(), want)
+    for i in range(len(lens)):
+        assert torch.equal(p.alone(i), want[p.starts[i] : p.starts[i + 1]]), i
+    C.check_errors(want.device)
+    p.check(want, [i for i, n in enumerate(lens) if n <= 64])
+
+
+def test_many_spans_from_device_memory(C, monkeypatch):
+    p = _Pass(C, *MANY)
+    want = p.packed()
+    assert torch.equal(p.from_device(), want)
+    monkeypatch.setattr(C, "KV8_PREFILL_PARTS", 40 << 20)
+    assert torch.equal(p.from_device(), want)
+    C.check_errors(want.device)
+
+
+def test_a_captured_pass_has_the_eager_bits_at_each_replay(C):
+    """One graph, whose spans and positions change between replays: cut, not cut, cut otherwise."""
+    p = _Pass(C, [90, 20, 18], [3000, 0, 0], width=80)
+    p.tables[1:] = p.tables[:1]  # the fillers' keys are whatever lies there
+    graph = torch.cuda.CUDAGraph()
+    p.from_device()
+    torch.cuda.synchronize()
+    meta = tuple(m.clone() for m in p.meta)
+    with torch.cuda.graph(graph):
+        out = C.kv8_prefill(p.q, p.gate, p.layer, p.tables, None, None, meta=meta)
+    for starts, pos0 in (([0, 90, 110, 128], [3000, 0, 0]), ([0, 1, 64, 128], [2999, 0, 0]), ([0, 90, 110, 128], [17, 0, 0]), ([0, 128, 128, 128], [2900, 0, 0])):
+        meta[0].copy_(torch.tensor(starts, dtype=torch.int32))
+        meta[1].copy_(torch.tensor(pos0, dtype=torch.int32))
+        graph.replay()
+        want = C.kv8_prefill(p.q, p.gate, p.layer, p.tables, starts, pos0)
+        assert torch.equal(out, want), (starts, pos0)
+    C.check_errors(out.device)
+
+
+def test_engine_with_captured_prefill_of_cut_spans(C):
+    """Prompts whose later chunks are cut, and a session's next turn: alone with captured passes, alone without, and packed."""
+    from b200serve.config import EngineConfig, ModelConfig
+    from b200serve.models.checkpoint import random_weights
+    from b200serve.sched.engine import Engine
+    from b200serve.sched.request import Sampling
+
+    cfg = ModelConfig.tiny(head_dim=64, num_attention_heads=4, num_key_value_heads=1)
+    w = random_weights(cfg, seed=0, device=DEV, dtype=torch.bfloat16, std=0.05, lm_head_std=0.5)
+    g = torch.Generator().manual_seed(3)
+    prompts = [torch.randint(3, 1024, (n,), generator=g).tolist() for n in (600, 333, 850)]
+    s = Sampling(max_tokens=24, ignore_eos=True)
+
+    def engine(**kw):
+        return Engine(w, EngineConfig(max_model_len=1024, prefill_chunk_tokens=64, max_seqs=8, kv_pages=256, decode_buckets=(1, 4), kv_dtype="e4m3", mtp=False, **kw))
+
+    packed = engine()
+    want = [x.output for x in packed.generate(prompts, s)]
+    graphs, plain = engine(prefill_graphs=True), engine()
+    for p, out in zip(prompts, want):
+        assert graphs.generate([p], s)[0].output == plain.generate([p], s)[0].output == out
+        turn = p + out + [9, 8, 7, 6, 5]
+        assert graphs.generate([turn], s)[0].output == plain.generate([turn], s)[0].output
+    assert graphs.stats["prefill_graph_passes"] >= sum(len(p) // 64 for p in prompts) and not graphs._pgraphs.errors
+    C.check_errors(torch.device(DEV))
