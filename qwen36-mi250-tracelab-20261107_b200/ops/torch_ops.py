@@ -186,8 +186,12 @@ def _kv8_attention(q, gate, layer: Kv8Layer, block_tables, seg_starts, positions
         k, v = (x.transpose(0, 1).repeat_interleave(n_q // n_kv, dim=0)
                 for x in kv8_read(layer, at, torch.zeros_like(at), block_tables[i : i + 1], torch.float32))  # [n_q, total, D]
         s = (q[a:b].transpose(0, 1).float() @ k.transpose(1, 2)) * D ** -0.5
-        s = s.masked_fill(at[None, :] > pos[:, None], float("-inf"))
-        o = (torch.softmax(s, dim=-1) @ v).transpose(0, 1)
+        hidden = at[None, :] > pos[:, None]
+        s = s.masked_fill(hidden, float("-inf"))
+        # a value that is marked as NaN must not meet the weight of 0 of a row that does not see it
+        bad = v.isnan().any(-1)
+        o = torch.softmax(s, dim=-1) @ v.masked_fill(bad[..., None], 0.0)
+        o = o.masked_fill((bad[:, None, :] & ~hidden).any(-1, keepdim=True), float("nan")).transpose(0, 1)
         out[a:b] = torch.where(pos[:, None, None] >= 0, o, torch.zeros_like(o)).to(q.dtype)
     return out.reshape(T, n_q * D) * torch.sigmoid(gate)
 

@@ -199,3 +199,21 @@ def test_a_prefix_moves_between_pools_of_either_type():
     for x, y, z, src in zip(a, b, c, (k, v)):
         assert torch.equal(x, y) and torch.equal(x.float(), z.float())
         assert torch.equal(x.float(), dequantise(*quantise(src), torch.float32))
+
+
+@pytest.mark.parametrize("kind", ["decode", "prefill"])
+@pytest.mark.parametrize("which", [0, 1])
+def test_a_nan_row_reaches_the_rows_that_see_it_alone(kind, which):
+    """A key or value that is marked as NaN is masked for the rows before it: their weights of 0 must not meet it."""
+    layer = _layer(n_kv=2, D=32)
+    tables = torch.tensor([[3, 5]], dtype=torch.int32)
+    layer.data.view(torch.uint8)[5, which, 1, 4], layer.exps[5, which, 1, 4] = 0, E_NAN  # position 68, KV head 1
+    g = torch.Generator().manual_seed(3)
+    q, gate = torch.randn(8, 4, 32, generator=g), torch.randn(8, 128, generator=g)
+    if kind == "decode":
+        got = O.kv8_decode(q, gate, layer, tables, torch.arange(64, 72), 8)
+    else:
+        got = O.kv8_prefill(q, gate, layer, tables, [0, 8], [64])
+    got = got.view(8, 4, 32)
+    assert got[4:, 2:].isnan().all()
+    assert got[:4].isfinite().all() and got[:, :2].isfinite().all()
