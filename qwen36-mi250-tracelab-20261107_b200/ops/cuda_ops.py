@@ -750,6 +750,13 @@ def _err_ptr(dev: torch.device) -> int:
     return (word if word is not None and dev.index == torch._C._cuda_getDevice() else err_word(dev)).data_ptr()
 
 
+def _kv8_layer(layer: Kv8Layer, what: str) -> tuple[int, int, int]:
+    """``(pages, n_kv, D)`` of a layer on a GPU."""
+    if not layer.data.is_cuda:
+        raise ValueError(f"{what}: the cache is on {layer.data.device}: torch_ops has the operators for it")
+    return check_layer(layer, what)
+
+
 def _index_tables(what: str, dev: torch.device, rows: int, positions: torch.Tensor, block_tables: torch.Tensor,
                   seq_of_row: torch.Tensor | None = None):
     """The row indices in the types that the kernels read (int64 positions, int32 tables and sequences), the tables' shape and row distance."""
@@ -775,7 +782,7 @@ def kv8_write(layer: Kv8Layer, k: torch.Tensor, v: torch.Tensor, positions: torc
               block_tables: torch.Tensor) -> None:
     """Quantise rows ``k, v [T, n_kv, D]`` (bf16, rows and heads at any stride) into the pages of their sequences: row ``t`` is the
     token at ``positions[t]`` of sequence ``seq_of_row[t]`` (``ops/kv8.py`` has the format)."""
-    pages, n_kv, D = check_layer(layer, "kv8_write")
+    pages, n_kv, D = _kv8_layer(layer, "kv8_write")
     data, exps = layer
     dev, shape = data.device, k.shape
     T = shape[0] if len(shape) else 0
@@ -798,7 +805,7 @@ def kv8_write(layer: Kv8Layer, k: torch.Tensor, v: torch.Tensor, positions: torc
 
 def kv8_read(layer: Kv8Layer, positions: torch.Tensor, seq_of_row: torch.Tensor, block_tables: torch.Tensor):
     """``k, v [T, n_kv, D]`` (bf16, exactly what the cache stands for) of the tokens at ``positions[t]`` of sequences ``seq_of_row[t]``."""
-    pages, n_kv, D = check_layer(layer, "kv8_read")
+    pages, n_kv, D = _kv8_layer(layer, "kv8_read")
     data, exps = layer
     dev, T = data.device, positions.numel()
     positions, block_tables, seq_of_row, step, width, seqs = _index_tables("kv8_read", dev, T, positions, block_tables, seq_of_row)
@@ -840,7 +847,7 @@ def kv8_decode(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_table
     """``flash_decode`` over the 8-bit cache: gated attention of ``G`` rows per sequence (decode 1, verify k + 1), each over the
     keys ``0 .. positions[row]`` of its sequence. A row's bits depend on its own position, queries and keys only, not on the batch or ``G``. A negative
     position is a row without keys: its output is 0; one behind its page table is reported by ``check_errors``. Only device tensors are touched, so the call can be captured in a CUDA graph."""
-    pages, n_kv, D = check_layer(layer, "kv8_decode")
+    pages, n_kv, D = _kv8_layer(layer, "kv8_decode")
     data, exps = layer
     dev = data.device
     q, gate, rows, n_q = _kv8_queries("kv8_decode", q, gate, n_kv, D, dev)
@@ -871,7 +878,7 @@ def kv8_prefill(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tabl
     ``meta``: ``(seg_starts, seg_pos0)`` as int32 device tensors that the caller keeps, of the same numbers; without it every call uploads
     them. With ``meta`` the lists may be None, which lets the call be captured in a CUDA graph: spans are cut as they would be with them, and the bits
     are the same. A span in ``meta`` that is not within the rows and its page table is left out, and reported by ``check_errors``."""
-    pages, n_kv, D = check_layer(layer, "kv8_prefill")
+    pages, n_kv, D = _kv8_layer(layer, "kv8_prefill")
     data, exps = layer
     dev = data.device
     q, gate, T, n_q = _kv8_queries("kv8_prefill", q, gate, n_kv, D, dev)
@@ -965,7 +972,7 @@ def _kv8_attention(qkv, positions, seq_of_row, block_tables, layer, q_norm, k_no
     if head_dim not in KV8_HEAD_DIMS or not 1 <= n_q // n_kv <= 16:
         return torch_ops.attention(qkv, positions, seq_of_row, block_tables, layer, q_norm, k_norm, n_q, n_kv, head_dim, rotary_dim,
                                    theta, eps, G, seg_starts, seg_pos0)
-    pages, layer_heads, layer_dim = check_layer(layer, "attention")
+    pages, layer_heads, layer_dim = _kv8_layer(layer, "attention")
     rows, dev = qkv.shape[0], layer.data.device
     if (layer_heads, layer_dim) != (n_kv, head_dim) or n_q % n_kv:
         raise ValueError(f"attention: {n_q} over {n_kv} heads of {head_dim}, an 8-bit KV layer of {layer_heads} heads of {layer_dim}")

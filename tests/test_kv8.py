@@ -217,3 +217,19 @@ def test_a_nan_row_reaches_the_rows_that_see_it_alone(kind, which):
     got = got.view(8, 4, 32)
     assert got[4:, 2:].isnan().all()
     assert got[:4].isfinite().all() and got[:, :2].isfinite().all()
+
+
+def test_the_kernels_calls_refuse_tensors_that_are_not_on_a_gpu():
+    from b200serve.ops import cuda_ops as C
+
+    layer = _layer(n_kv=2, D=64)
+    tables, pos, seq = torch.tensor([[3, 5]], dtype=torch.int32), torch.arange(4), torch.zeros(4, dtype=torch.int32)
+    k, q, gate = torch.zeros(4, 2, 64).bfloat16(), torch.zeros(4, 4, 64).bfloat16(), torch.zeros(4, 256).bfloat16()
+    words = dict(C._err)
+    norm = torch.zeros(64).bfloat16()
+    for call in (lambda: C.kv8_write(layer, k, k, pos, seq, tables), lambda: C.kv8_read(layer, pos, seq, tables),
+                 lambda: C.kv8_decode(q, gate, layer, tables, pos, 4), lambda: C.kv8_prefill(q, gate, layer, tables, [0, 4], [0]),
+                 lambda: C.attention(torch.zeros(4, 768).bfloat16(), pos, seq, tables, layer, norm, norm, 4, 2, 64, 16, 1e7, 1e-6, 4)):
+        with pytest.raises(ValueError, match="(kv8_|attention).* cpu"):
+            call()
+    assert C._err == words
