@@ -175,11 +175,12 @@ class Model:
         return kv[page, 0, :, at], kv[page, 1, :, at]
 
     def write_kv(self, layer: int, table: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pos0: int = 0) -> None:
-        """Rows ``[n, n_kv, D]`` of keys and values into the pages of a sequence, from position ``pos0`` on."""
+        """Rows ``[n, n_kv, D]`` of keys and values (of any floating type) into the pages of a sequence, from position ``pos0`` on. The 8-bit pool
+        quantises them in the activations' type, as it does the model's own."""
         pos = torch.arange(pos0, pos0 + k.shape[0], device=self.device)
         kv = self.kv[layer]
         if isinstance(kv, Kv8Layer):
-            self.ops.kv8_write(kv, k, v, pos, torch.zeros_like(pos, dtype=torch.int32), table[None, :])
+            self.ops.kv8_write(kv, k.to(self.dtype), v.to(self.dtype), pos, torch.zeros_like(pos, dtype=torch.int32), table[None, :])
         else:
             torch_ops.kv_write(kv, k.to(kv.dtype), v.to(kv.dtype), table[pos // PAGE_SIZE].long(), pos % PAGE_SIZE)
 

@@ -246,3 +246,27 @@ def test_engine_with_captured_prefill_of_cut_spans(C):
         assert graphs.generate([turn], s)[0].output == plain.generate([turn], s)[0].output
     assert graphs.stats["prefill_graph_passes"] >= sum(len(p) // 64 for p in prompts) and not graphs._pgraphs.errors
     C.check_errors(torch.device(DEV))
+
+
+# ------------------------------------------------------------------ the model's pool
+def _tiny(C, head_dim=64, n_q=4, n_kv=1):
+    from b200serve.config import ModelConfig
+    from b200serve.models.checkpoint import random_weights
+
+    cfg = ModelConfig.tiny(head_dim=head_dim, num_attention_heads=n_q, num_key_value_heads=n_kv)
+    return cfg, random_weights(cfg, seed=0, device=DEV, dtype=torch.bfloat16, std=0.05, lm_head_std=0.5)
+
+
+def test_rows_of_other_types_go_into_the_8_bit_pool(C):
+    from b200serve.models.qwen36 import Model
+    from b200serve.ops.kv8 import dequantise, quantise
+
+    cfg, w = _tiny(C)
+    model = Model(w, 8, 2, ops=C, kv_dtype=torch.float8_e4m3fn)
+    table = torch.tensor([3, 5], dtype=torch.int32, device=DEV)
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        k, v = (torch.randn(100, 1, 64, device=DEV, generator=torch.Generator(device=DEV).manual_seed(i)).to(dtype) for i in (0, 1))
+        model.write_kv(0, table, k, v)
+        for got, src in zip(model.read_kv(0, table, 100), (k, v)):
+            assert torch.equal(got, dequantise(*quantise(src.bfloat16()), torch.bfloat16))
+    C.check_errors(k.device)
