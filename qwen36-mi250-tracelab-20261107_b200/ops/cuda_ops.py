@@ -823,6 +823,12 @@ KV8_HEAD_DIMS = (64, 128, 256)  # of the attention kernels over the 8-bit cache
 KV8_PREFILL_PARTS = 256 << 20
 
 
+def kv8_kernels(n_q: int, n_kv: int, head_dim: int) -> bool:
+    """Whether the attention kernels over the 8-bit cache take these heads. ``attention`` runs others in PyTorch, sequence by sequence, with the host
+    waiting for their lengths: slow, and not to be captured in a CUDA graph."""
+    return head_dim in KV8_HEAD_DIMS and n_q % n_kv == 0 and n_q // n_kv <= 16
+
+
 def _kv8_queries(what: str, q: torch.Tensor, gate: torch.Tensor, n_kv: int, D: int, dev: torch.device):
     """Queries and gates, contiguous in 16-byte rows; their number and the query heads."""
     if D not in KV8_HEAD_DIMS:
@@ -969,13 +975,13 @@ def kv8_prefill(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tabl
 def _kv8_attention(qkv, positions, seq_of_row, block_tables, layer, q_norm, k_norm, n_q, n_kv, head_dim, rotary_dim, theta, eps, G,
                    seg_starts, seg_pos0, meta) -> torch.Tensor:
     """``attention`` over a layer of the 8-bit cache. Head dims without a kernel take the PyTorch operators, as the bf16 prefill does."""
-    if head_dim not in KV8_HEAD_DIMS or not 1 <= n_q // n_kv <= 16:
-        return torch_ops.attention(qkv, positions, seq_of_row, block_tables, layer, q_norm, k_norm, n_q, n_kv, head_dim, rotary_dim,
-                                   theta, eps, G, seg_starts, seg_pos0)
     pages, layer_heads, layer_dim = _kv8_layer(layer, "attention")
     rows, dev = qkv.shape[0], layer.data.device
     if (layer_heads, layer_dim) != (n_kv, head_dim) or n_q % n_kv:
         raise ValueError(f"attention: {n_q} over {n_kv} heads of {head_dim}, an 8-bit KV layer of {layer_heads} heads of {layer_dim}")
+    if not kv8_kernels(n_q, n_kv, head_dim):
+        return torch_ops.attention(qkv, positions, seq_of_row, block_tables, layer, q_norm, k_norm, n_q, n_kv, head_dim, rotary_dim,
+                                   theta, eps, G, seg_starts, seg_pos0)
     if qkv.dim() != 2 or qkv.shape[1] < 2 * (n_q + n_kv) * head_dim or qkv.dtype != torch.bfloat16 or qkv.stride(1) != 1 or qkv.device != dev:
         raise ValueError(f"attention: projected rows {tuple(qkv.shape)} {qkv.dtype} on {qkv.device} are not bf16 [rows, {2 * (n_q + n_kv) * head_dim}] on {dev}")
     positions, block_tables, seq_of_row, step, width, seqs = _index_tables("attention", dev, rows, positions, block_tables, seq_of_row)

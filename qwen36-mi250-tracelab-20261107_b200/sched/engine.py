@@ -122,7 +122,8 @@ class Engine:
         self._graphs = None
         # library collectives (the NCCL baseline path) stay out of CUDA graphs; the fused NVLink kernels go in
         emulate = c.cuda_graphs and c.graphs_on_cpu and self.device.type != "cuda"
-        if (self.device.type == "cuda" or emulate) and c.cuda_graphs and (tp is None or getattr(tp.comm, "fused", False) or emulate):
+        native = self.device.type == "cuda" and (KV_DTYPES[c.kv_dtype] is None or self._kv8_kernels())
+        if (native or emulate) and c.cuda_graphs and (tp is None or getattr(tp.comm, "fused", False) or emulate):
             from .graphs import DecodeGraphs
 
             self._graphs = DecodeGraphs(self)
@@ -138,6 +139,11 @@ class Engine:
 
             if PrefillGraphs.supported(self):
                 self._pgraphs = PrefillGraphs(self)
+
+    def _kv8_kernels(self) -> bool:
+        """Whether attention over the 8-bit pool runs in kernels alone; a pass that does not cannot be captured."""
+        m, known = self.mcfg, getattr(self.ops, "kv8_kernels", None)
+        return known is not None and known(m.num_attention_heads, m.num_key_value_heads, m.head_dim)
 
     # ------------------------------------------------------------------ sizing
     def _auto_pages(self, weights: Weights, n_slots: int) -> int:

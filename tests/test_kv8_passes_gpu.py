@@ -270,3 +270,28 @@ def test_rows_of_other_types_go_into_the_8_bit_pool(C):
         for got, src in zip(model.read_kv(0, table, 100), (k, v)):
             assert torch.equal(got, dequantise(*quantise(src.bfloat16()), torch.bfloat16))
     C.check_errors(k.device)
+
+
+@pytest.mark.parametrize("head_dim,n_q,n_kv,native", [(32, 4, 1, False), (64, 6, 2, True), (64, 4, 4, True)])
+def test_engine_captures_what_can_be_captured(C, head_dim, n_q, n_kv, native):
+    """Heads without an attention kernel over the 8-bit pool run without graphs, and none is tried."""
+    from b200serve.config import EngineConfig
+    from b200serve.sched.engine import Engine
+    from b200serve.sched.request import Sampling
+
+    cfg, w = _tiny(C, head_dim, n_q, n_kv)
+    assert C.kv8_kernels(n_q, n_kv, head_dim) == native
+    g = torch.Generator().manual_seed(3)
+    prompts = [torch.randint(3, 1024, (n,), generator=g).tolist() for n in (17, 190)]
+    s = Sampling(max_tokens=8, ignore_eos=True)
+
+    def run(prompts, **kw):
+        eng = Engine(w, EngineConfig(max_model_len=512, prefill_chunk_tokens=64, max_seqs=4, kv_pages=64, decode_buckets=(1, 4), kv_dtype="e4m3", **kw))
+        eng.warmup()
+        return eng, [x.output for x in eng.generate(prompts, s)]
+
+    eng, outs = run(prompts, mtp=False)
+    assert (eng._graphs is not None) == native and not (native and eng._graphs.errors)
+    assert run(prompts[1:], mtp=False)[1] == outs[1:] and all(len(o) == 8 for o in outs)
+    assert run(prompts, mtp=True, spec_k=2)[1] == outs
+    C.check_errors(torch.device(DEV))
