@@ -241,11 +241,9 @@ class Model:
             return {"seg_starts": batch.seg_starts, "seg_pos0": batch.seg_pos0, **meta}
         if not meta:
             return {"seg_starts": batch.seg_starts, "seg_pos0": batch.seg_pos0}
-        tables = batch.meta or batch.tables
-        meta = {"meta": (tables.gdn[5], tables.flash[3])} if tables.flash is not None else {}
         if batch.meta is not None:
-            return {"seg_starts": None, "seg_pos0": None, **meta}
-        return {"seg_starts": batch.seg_starts, "seg_pos0": batch.seg_pos0, **meta}
+            return {"seg_starts": None, "seg_pos0": None, "meta": batch.meta.spans}
+        return {"seg_starts": batch.seg_starts, "seg_pos0": batch.seg_pos0, "meta": batch.tables.spans}
 
     def _attention(self, lw, kv_layer, h, batch: PackedBatch) -> torch.Tensor:
         cfg, ops = self.cfg, self.ops

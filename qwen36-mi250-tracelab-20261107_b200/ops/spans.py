@@ -66,6 +66,12 @@ class SpanTables:
     pos0: list[int]
     gdn: tuple
     flash: tuple | None
+    pos0_t: torch.Tensor
+
+    @property
+    def spans(self) -> tuple:
+        """The spans' first rows and positions, what ``cuda_ops.kv8_prefill`` takes as ``meta``: no tile table goes with them."""
+        return self.gdn[5], self.pos0_t
 
     def of(self, starts, slots, pos0, tile_rows: int | None) -> bool:
         return (self.starts == starts and self.slots == slots and self.pos0 == pos0
@@ -89,7 +95,7 @@ def tables(parts, seq: torch.Tensor, starts, slots, pos0, tile_rows: int | None)
     """``parts``: the words on the device; ``seq``: the span of every row."""
     chunks, tiles, per_span, st, sl, p0 = parts
     return SpanTables(list(starts), list(slots), list(pos0), (len(slots), len(chunks) // 4, chunks, per_span, seq, st, sl),
-                      (tile_rows, len(tiles) // 4, tiles, p0) if tile_rows else None)
+                      (tile_rows, len(tiles) // 4, tiles, p0) if tile_rows else None, p0)
 
 
 def span_tables(starts, slots, pos0, tile_rows: int | None, device: torch.device) -> SpanTables:

@@ -432,6 +432,10 @@ class PrefillTables:
     def __init__(self, gdn, flash) -> None:
         self.gdn, self.flash = gdn, flash
 
+    @property
+    def spans(self) -> tuple:
+        return self.gdn[5], self.flash[3]
+
 
 class _PrefillBucket:
     """One captured prefill pass of ``rows`` packed rows: ONE request's span of up to ``rows - 64`` tokens plus filler

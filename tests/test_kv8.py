@@ -233,3 +233,24 @@ def test_the_kernels_calls_refuse_tensors_that_are_not_on_a_gpu():
         with pytest.raises(ValueError, match="(kv8_|attention).* cpu"):
             call()
     assert C._err == words
+
+
+@pytest.mark.parametrize("n_q,n_kv", [(4, 1), (6, 2), (5, 1)])
+def test_the_layers_of_a_pass_share_the_spans_device_tensors(n_q, n_kv):
+    """Whatever the heads: a group that has no table of query tiles has its spans' rows and positions on the device all the same."""
+    import types
+
+    from b200serve.config import ModelConfig
+    from b200serve.models.checkpoint import random_weights
+    from b200serve.models.qwen36 import Model, PackedBatch
+
+    cfg = ModelConfig.tiny(num_attention_heads=n_q, num_key_value_heads=n_kv)
+    w = random_weights(cfg, seed=0, device="cpu", dtype=torch.float32)
+    ops = types.SimpleNamespace(**{k: getattr(O, k) for k in dir(O) if not k.startswith("__")}, SPAN_TABLES=True)
+    model = Model(w, 8, 4, ops=ops, kv_dtype=torch.float8_e4m3fn)
+    batch = PackedBatch.prefill([[1] * 5, [2] * 70], [1, 2], [3, 0], torch.tensor([[1, 2], [3, 4]], dtype=torch.int32), "cpu")
+    args = model._attention_spans(batch)
+    assert (args["seg_starts"], args["seg_pos0"]) == ([0, 5, 75], [3, 0])
+    assert [t.tolist() for t in args["meta"]] == [[0, 5, 75], [3, 0]] and all(t.dtype == torch.int32 for t in args["meta"])
+    again = model._attention_spans(batch)["meta"]
+    assert all(a.data_ptr() == b.data_ptr() for a, b in zip(args["meta"], again))
