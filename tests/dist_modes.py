@@ -126,3 +126,38 @@ def mode_dp_ep_served(rank, world, dev):
     if cuda:
         dist.barrier()
         ep.close()
+
+
+def mode_kv8_ranks(rank, world, dev):
+    """Tensor-parallel and layer-split engines over the 8-bit pool: each rank has the pool of its own heads or layers, all give
+    the same tokens, and those of the layer split (the same operations, elsewhere) are the unsplit engine's."""
+    from b200serve.config import EngineConfig, ModelConfig
+    from b200serve.models.checkpoint import random_weights
+    from b200serve.ops.kv8 import Kv8Pool
+    from b200serve.parallel.pp import PPContext, split_layers
+    from b200serve.parallel.tp import DistComm, TPContext, shard_weights
+    from b200serve.sched.engine import Engine
+    from b200serve.sched.request import Sampling
+
+    cfg = ModelConfig.tiny(num_hidden_layers=8, num_key_value_heads=2, mtp_num_hidden_layers=0)
+    full = random_weights(cfg, seed=0, device="cpu", dtype=torch.float32, std=0.05, lm_head_std=0.5)
+    g = torch.Generator().manual_seed(5)
+    prompts = [torch.randint(3, 1024, (n,), generator=g).tolist() for n in (20, 70, 150)]
+    s = Sampling(max_tokens=8, ignore_eos=True)
+    ecfg = EngineConfig(max_model_len=1024, prefill_chunk_tokens=64, max_seqs=4, mtp=False, kv_pages=128, kv_dtype="e4m3", device="cpu")
+
+    def outputs(eng):
+        assert isinstance(eng.model.kv, Kv8Pool)
+        got = [x.output for x in eng.generate(prompts, s)]
+        mine = torch.tensor(got)
+        every = [torch.empty_like(mine) for _ in range(world)]
+        dist.all_gather(every, mine)
+        assert all(torch.equal(mine, x) for x in every)
+        return got, eng.model.page_bytes
+
+    want, page = outputs(Engine(full, ecfg))
+    got, part = outputs(Engine(split_layers(full, rank, world), ecfg, pp=PPContext(rank, world)))
+    assert got == want and part * world == page
+    got, part = outputs(Engine(shard_weights(full, rank, world), ecfg, tp=TPContext(rank, world, DistComm(dist.group.WORLD))))
+    # sums over the ranks come in another order, and a key's rounding may flip: first tokens, which lead by far, stay
+    assert [x[0] for x in got] == [x[0] for x in want] and part * world == page

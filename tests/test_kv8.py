@@ -254,3 +254,46 @@ def test_the_layers_of_a_pass_share_the_spans_device_tensors(n_q, n_kv):
     assert [t.tolist() for t in args["meta"]] == [[0, 5, 75], [3, 0]] and all(t.dtype == torch.int32 for t in args["meta"])
     again = model._attention_spans(batch)["meta"]
     assert all(a.data_ptr() == b.data_ptr() for a, b in zip(args["meta"], again))
+
+
+def test_two_ranks_over_the_8_bit_pool():
+    from test_tp import _launch
+
+    r = _launch("kv8_ranks", 2, 29661, env={"CUDA_VISIBLE_DEVICES": ""})
+    assert r.returncode == 0 and "OK kv8_ranks" in r.stdout, r.stdout[-3000:] + r.stderr[-3000:]
+
+
+def hand_over(ops, device, dtype, kv_dtypes, head_dim):
+    """A prefix's keys, values and recurrent states go from one model to another, into other pages and another slot; the next
+    tokens' hidden states over either, and what was handed over."""
+    from b200serve.config import ModelConfig
+    from b200serve.models.checkpoint import random_weights
+    from b200serve.models.qwen36 import Model, PackedBatch
+
+    cfg = ModelConfig.tiny(num_hidden_layers=8, head_dim=head_dim, mtp_num_hidden_layers=0)
+    w = random_weights(cfg, seed=0, device=device, dtype=dtype, std=0.05)
+    a, b = (Model(w, 8, 4, ops=ops, kv_dtype=t) for t in kv_dtypes)
+    n = 100
+    g = torch.Generator().manual_seed(1)
+    tokens = torch.randint(3, 1024, (n + 3,), generator=g).tolist()
+    ta, tb = torch.tensor([3, 5], dtype=torch.int32), torch.tensor([6, 2], dtype=torch.int32)
+    a.forward(PackedBatch.prefill([tokens[:n]], [1], [0], ta[None], device))
+    rows = []
+    for layer in range(cfg.num_kv_layers):
+        rows.append(a.read_kv(layer, ta.to(device), n))
+        b.write_kv(layer, tb.to(device), *rows[-1])
+    b.conv_state[:, 2].copy_(a.conv_state[:, 1])
+    b.rec_state[:, 2].copy_(a.rec_state[:, 1])
+    outs = [[], []]
+    for i in range(n, n + 3):
+        for out, model, slot, table in zip(outs, (a, b), (1, 2), (ta, tb)):
+            out.append(model.forward(PackedBatch.uniform([tokens[i]], [i], [slot], table[None], 1, device)).clone())
+    return outs, rows
+
+
+@pytest.mark.parametrize("to", [torch.float8_e4m3fn, None])
+def test_a_generation_goes_on_over_a_prefix_that_was_handed_over(to):
+    (here, there), rows = hand_over(O, "cpu", torch.float32, (torch.float8_e4m3fn, to), 32)
+    assert all(k.abs().max() > 0 and k.shape == (100, 1, 32) for k, _ in rows)
+    for x, y in zip(here, there):  # into a pool of full width: what is new there is not rounded to 8 bits
+        assert torch.equal(x, y) if to is not None else torch.nn.functional.cosine_similarity(x, y).min() > 0.99

@@ -295,3 +295,74 @@ def test_engine_captures_what_can_be_captured(C, head_dim, n_q, n_kv, native):
     assert run(prompts[1:], mtp=False)[1] == outs[1:] and all(len(o) == 8 for o in outs)
     assert run(prompts, mtp=True, spec_k=2)[1] == outs
     C.check_errors(torch.device(DEV))
+
+
+def test_a_generation_goes_on_over_a_prefix_that_was_handed_over(C):
+    from test_kv8 import hand_over
+
+    (here, there), rows = hand_over(C, DEV, torch.bfloat16, (torch.float8_e4m3fn,) * 2, 64)
+    C.check_errors(torch.device(DEV))
+    assert all(torch.equal(x, y) and x.isfinite().all() for x, y in zip(here, there))
+    assert all(k.abs().max() > 0 and k.shape == (100, 1, 64) for k, _ in rows)
+
+
+# ------------------------------------------------------------------ more than a launch, and the block
+@pytest.mark.parametrize("heads", [(16, 2, 256), (8, 1, 64), (6, 3, 128)])
+@pytest.mark.parametrize("G", [1, 3])
+def test_decode_of_more_sequences_than_a_launch_takes_with_partials(C, heads, G):
+    """Two launches, each with the join of its own rows; lengths around the ends of runs, and rows without keys."""
+    B = 300
+    lens = [(0, 1, 511, 512, 513, 700, 1024, 1025, 64, 1300)[i % 10] for i in range(B)]
+    n_q, n_kv, D = heads
+    pages = sum((n + 63) // 64 for n in lens) + 2
+    layer = _layer(pages, n_kv, D)
+    tables = _tables(lens, 22, pages)
+    positions = torch.tensor([n - G + i for n in lens for i in range(G)], device=DEV)
+    q, gate = _rows(B * G, n_q, D, 1)
+    got = C.kv8_decode(q, gate, layer, tables, positions, G)
+    C.check_errors(q.device)
+    for a, b in ((0, 20), (250, 262), (290, 300)):
+        rows = slice(a * G, b * G)
+        _check(got[rows], _attention(q[rows], gate[rows], layer, tables[a:b].repeat_interleave(G, 0), positions[rows]), (a, b))
+        one = C.kv8_decode(q[rows], gate[rows], layer, tables[a:b], positions[rows], G)
+        assert torch.equal(one, got[rows])
+
+
+@pytest.mark.parametrize("n_q,n_kv,D,G", [(16, 2, 256, 1), (16, 2, 256, 4), (16, 2, 256, 0), (6, 3, 128, 0), (4, 1, 64, 2)])
+def test_the_block_is_the_fused_write_and_the_operator(C, n_q, n_kv, D, G):
+    """The block's output has the bits of the operator on the queries and gates that the fused write leaves, and keeps the operator's
+    bound; the queries are the formula's, rounded to bf16 at each of the kernel's steps."""
+    from b200serve.ops import torch_ops as O
+    from b200serve.ops.kv8 import Kv8Layer
+
+    rot, theta, eps = D // 4, 1e7, 1e-6
+    per, pos0 = ([G] * 3 if G else [70, 1, 130]), [5, 64, 600]
+    starts = [0]
+    for n in per:
+        starts.append(starts[-1] + n)
+    T = starts[-1]
+    g = torch.Generator(device=DEV).manual_seed(D + G)
+    layer = _layer(30, n_kv, D, seed=2)
+    tables = _tables([a + b for a, b in zip(per, pos0)], 12, 30)
+    qkv = torch.randn(T, n_q * 2 * D + 2 * n_kv * D, device=DEV, generator=g).bfloat16()
+    positions = torch.cat([torch.arange(p, p + n) for p, n in zip(pos0, per)]).to(DEV)
+    seq = torch.cat([torch.full((n,), i) for i, n in enumerate(per)]).int().to(DEV)
+    qn, kn = ((torch.randn(D, device=DEV, generator=g) * 0.1).bfloat16() for _ in range(2))
+    q = torch.empty(T, n_q, D, dtype=torch.bfloat16, device=DEV)
+    gate = torch.empty(T, n_q * D, dtype=torch.bfloat16, device=DEV)
+    other = Kv8Layer(layer.data.clone(), layer.exps.clone())
+    rc = C.lib().b200_attn_prep_kv8(
+        qkv.data_ptr(), qkv.stride(0), positions.data_ptr(), tables.data_ptr(), 12, 12, 3, seq.data_ptr(), qn.data_ptr(), kn.data_ptr(), q.data_ptr(),
+        gate.data_ptr(), other.data.data_ptr(), other.exps.data_ptr(), T, n_q, n_kv, D, rot, theta, eps, 30,
+        C.err_word(qkv.device).data_ptr(), torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    got = C.attention(qkv, positions, seq, tables, layer, qn, kn, n_q, n_kv, D, rot, theta, eps, G, starts, pos0)
+    C.check_errors(qkv.device)
+    assert torch.equal(layer.data.view(torch.uint8), other.data.view(torch.uint8)) and torch.equal(layer.exps, other.exps)
+    want = C.kv8_decode(q, gate, layer, tables, positions, G) if G else C.kv8_prefill(q, gate, layer, tables, starts, pos0)
+    assert torch.equal(got, want)
+    _check(got, _attention(q, gate, layer, tables[seq.long()], positions))
+    rq, rgate, _, _ = O.attn_prep(qkv.float(), positions, qn.float(), kn.float(), n_q, n_kv, D, rot, theta, eps)
+    assert torch.equal(gate.float(), rgate)
+    # three roundings to bf16 (the norm, cosine and sine, their products) of numbers no larger than the head's largest rotated ones, and the last one
+    assert ((q.float() - rq).abs() <= 5 * 2.0 ** -8 * rq.abs().amax(-1, keepdim=True)).all()
