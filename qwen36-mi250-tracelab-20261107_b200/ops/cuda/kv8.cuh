@@ -35,6 +35,11 @@ __device__ __forceinline__ uint32_t kv8_unpack2(uint16_t two) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(two));
   return r;
 }
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 // The sigmoids of the halves of a word of bf16 gates, for outputs that are rounded to bf16 next: 1 / (1 + 2^-t) with t = x log2(e) on the unit of
 // special functions. An exact division is a subroutine: the loop at the end of a prefill tile (128 rows of 256) took 32,500 cycles with it, and 20,000
 // so. (Two sigmoids from one reciprocal, 1 / a = b / (a b), need a case of their own where the product overflows or one is NaN: no faster.)
@@ -43,8 +48,7 @@ __device__ __forceinline__ float2 kv8_sigmoid2(uint32_t gates) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const float x = __uint_as_float(i ? gates & 0xffff0000u : gates << 16);
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a[i]) : "f"(x * -1.4426950408889634f));
-    a[i] += 1.0f;
+    a[i] = ex2(x * -1.4426950408889634f) + 1.0f;
     asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(a[i]));
   }
   return make_float2(a[0], a[1]);
@@ -80,6 +84,30 @@ __device__ __forceinline__ void ask_8(uint16_t& x, const void* p, bool yes) {
 __device__ __forceinline__ void ask_128(uint4& x, const void* p, bool yes) {
   asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t@q ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
                : "+r"(x.x), "+r"(x.y), "+r"(x.z), "+r"(x.w) : "l"(p), "r"(static_cast<int>(yes)));
+}
+
+// The tensor map of bytes of `rank` dims (2 or 3), the strides of all but the first in bytes. Not 0: it cannot be made.
+inline int kv8_encode(CUtensorMap* m, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box,
+                      CUtensorMapSwizzle sw) {
+  typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                               const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static EncodeFn fn = nullptr;
+  if (!fn) {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) != cudaSuccess || !ptr) return -1;
+    fn = reinterpret_cast<EncodeFn>(ptr);
+  }
+  const cuuint32_t estr[3] = {1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : -2;
+}
+// That of a layer's exponents [pages, 2, n_kv, 64]: a box has those of a page's keys and values of one head.
+inline int kv8_encode_exps(CUtensorMap* m, const void* exps, int n_kv, long long pages) {
+  const cuuint64_t dims[3] = {KV8_PAGE, static_cast<cuuint64_t>(n_kv), static_cast<cuuint64_t>(pages) * 2};
+  const cuuint64_t strides[2] = {KV8_PAGE, static_cast<cuuint64_t>(n_kv) * KV8_PAGE};
+  const cuuint32_t box[3] = {KV8_PAGE, 1, 2};
+  return kv8_encode(m, exps, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 }  // namespace b200

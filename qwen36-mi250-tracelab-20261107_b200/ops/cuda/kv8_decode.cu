@@ -45,7 +45,6 @@ constexpr float K8D_LAZY = 8.0f;                // the maximum moves when it gre
 struct Kv8DecodeParams {
   const bf16* q;             // [rows, n_q, D]
   const bf16* gate;          // [rows, n_q * D]
-  const uint8_t* exps;       // [pages, 2, n_kv, 64]
   const int64_t* positions;  // [rows]
   const int* tables;         // [B] rows of `width` pages, max_pages apart
   bf16* out;                 // [rows, n_q * D]
@@ -61,7 +60,6 @@ struct Kv8DecodeParams {
 template <int D, int NT>
 struct Kv8DecodeCfg {
   static constexpr int ROWB = D < 128 ? D : 128;           // bytes of a row in one swizzled block
-  static constexpr int DB = D / ROWB;
   static constexpr int TILE = KV8_PAGE * D;                // a page's keys or values: a slot of their ring
   static constexpr int SLOTS = D == 256 ? 3 : D == 128 ? 6 : 8;
   static constexpr int EXPS = 2 * KV8_PAGE;                // exponents of a page's keys and values, with its keys
@@ -97,11 +95,6 @@ __device__ __forceinline__ bool meet_scores_or(bool mine) {
       "selp.b32 %0, 1, 0, q;\n\t}"
       : "=r"(any) : "r"(static_cast<uint32_t>(mine)), "n"(32 * K8D_SLABS) : "memory");
   return any != 0;
-}
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
 }
 
 // A wait for a barrier that was looked at before.
@@ -818,32 +811,14 @@ kv8_combine_kernel(const float* part_acc, const float2* part_ml, const bf16* gat
 using namespace b200;
 
 namespace {
-typedef CUresult (*K8dEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
-                                CUtensorMapFloatOOBfill);
-int k8d_encode(CUtensorMap* m, const void* base, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle sw) {
-  static K8dEncodeFn fn = nullptr;
-  if (!fn) {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) != cudaSuccess || !ptr) return -1;
-    fn = reinterpret_cast<K8dEncodeFn>(ptr);
-  }
-  const cuuint32_t estr[3] = {1, 1, 1};
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : -2;
-}
 // A page's keys or values of one head, in blocks of at most 128 bytes per row; their exponents, of keys and values together.
 int k8d_make_maps(CUtensorMap* tm, CUtensorMap* tm_exps, const void* data, const void* exps, int D, int n_kv, long long pages) {
   const cuuint32_t rowb = D < 128 ? D : 128;
   const cuuint64_t dims[3] = {rowb, static_cast<cuuint64_t>(pages) * 2 * n_kv * KV8_PAGE, D / rowb};
   const cuuint64_t strides[2] = {static_cast<cuuint64_t>(D), rowb};
   const cuuint32_t box[3] = {rowb, KV8_PAGE, D / rowb};
-  const cuuint64_t edims[3] = {KV8_PAGE, static_cast<cuuint64_t>(n_kv), static_cast<cuuint64_t>(pages) * 2};
-  const cuuint64_t estrides[2] = {KV8_PAGE, static_cast<cuuint64_t>(n_kv) * KV8_PAGE};
-  const cuuint32_t ebox[3] = {KV8_PAGE, 1, 2};
-  const int rc = k8d_encode(tm, data, dims, strides, box, rowb == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
-  return rc ? rc : k8d_encode(tm_exps, exps, edims, estrides, ebox, CU_TENSOR_MAP_SWIZZLE_NONE);
+  const int rc = kv8_encode(tm, data, 3, dims, strides, box, rowb == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+  return rc ? rc : kv8_encode_exps(tm_exps, exps, n_kv, pages);
 }
 
 template <int D, int NT>
@@ -899,7 +874,7 @@ extern "C" int b200_kv8_decode(const void* q, const void* gate, const void* data
     if (static_cast<long long>(n) * G * n_kv * n_splits > 0x3fffffffLL) return -7;  // the units are counted in 32 bits
     const size_t heads = static_cast<size_t>(b0) * G * n_q;
     const Kv8DecodeParams p{static_cast<const bf16*>(q) + heads * D, static_cast<const bf16*>(gate) + heads * D,
-                            static_cast<const uint8_t*>(exps), positions + static_cast<size_t>(b0) * G,
+                            positions + static_cast<size_t>(b0) * G,
                             tables + static_cast<size_t>(b0) * max_pages, static_cast<bf16*>(out) + heads * D,
                             part_acc + heads * n_splits * D, reinterpret_cast<float2*>(part_ml) + heads * n_splits,
                             n, G, max_pages, width, num_pages, n_q, n_kv, group, n_splits, per, (G + per - 1) / per, (65536 + group - 1) / group,

@@ -100,11 +100,6 @@ __device__ __forceinline__ uint32_t k8p_at(int r, int c) {
   const uint32_t byte = r * ROWB;
   return byte + ((c ^ ((byte >> 7) & (ROWB / 16 - 1))) << 4);
 }
-__device__ __forceinline__ float k8p_ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
 // Two floats at a time.
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   float2 r;
@@ -542,7 +537,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
         ok = mbar_wait(&pv_done[hf ^ 1], ((i - 1) >> 1) & 1, p.err, ERR_WAIT_EMPTY, abort_flag);
         if (!ok) break;
         tc_fence_after();
-        const float factor = need ? k8p_ex2(m_prev - m) : 1.0f;
+        const float factor = need ? ex2(m_prev - m) : 1.0f;
 #pragma unroll 1
         for (int c = 0; c < D; c += 16) {
           float o[16];
@@ -554,7 +549,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       }
       if (m != m_loc) {
-        const float f = k8p_ex2(m_loc - m);  // 0 on this thread's first page
+        const float f = ex2(m_loc - m);  // 0 on this thread's first page
         l2.x *= f;
         l2.y *= f;
         m_loc = m;
@@ -572,7 +567,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float2 z = fma2(y[4 * c + j], one2, base2);
-          const float2 w = make_float2(k8p_ex2(z.x), k8p_ex2(z.y));
+          const float2 w = make_float2(ex2(z.x), ex2(z.y));
           l2 = fma2(w, inv[j], l2);
           pe[j] = __floats2half2_rn(w.x, w.y);
         }
@@ -595,7 +590,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
       ok = mbar_wait(x_bar, 0, p.err, ERR_WAIT_FULL, abort_flag);
       const float l0 = ex[r * 2], m0 = ex[r * 2 + 1], l1 = ex[(128 + r) * 2], m1 = ex[(128 + r) * 2 + 1];
       m_used = fmaxf(m0, m1);  // a running maximum never falls: the larger one is the last page's
-      l = m_used == -INFINITY ? l0 + l1 : fmaf(l0, k8p_ex2(m0 - m_used), l1 * k8p_ex2(m1 - m_used));
+      l = m_used == -INFINITY ? l0 + l1 : fmaf(l0, ex2(m0 - m_used), l1 * ex2(m1 - m_used));
     }
     // The outputs go through shared memory, 16 bytes of a row in the place of their number XOR the row, so that a warp reads gates and
     // writes outputs of a whole row at a time (with a thread a row from TMEM to the output, the end of a tile took 13 us).
@@ -712,7 +707,7 @@ kv8_prefill_combine_kernel(Kv8PrefillParams p) {
   for (int z0 = 0;;) {
 #pragma unroll
     for (int k = 0; k < AT_ONCE; ++k) {
-      const float f = pm[k].x == top ? 1.f : k8p_ex2(pm[k].x - top);
+      const float f = pm[k].x == top ? 1.f : ex2(pm[k].x - top);
       l = fmaf(pm[k].y, f, l);
       o.x = fmaf(v[k].x, f, o.x); o.y = fmaf(v[k].y, f, o.y); o.z = fmaf(v[k].z, f, o.z); o.w = fmaf(v[k].w, f, o.w);
     }
@@ -734,21 +729,6 @@ kv8_prefill_combine_kernel(Kv8PrefillParams p) {
 using namespace b200;
 
 namespace {
-typedef CUresult (*K8pEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
-                                CUtensorMapFloatOOBfill);
-int k8p_encode(CUtensorMap* m, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle sw) {
-  static K8pEncodeFn fn = nullptr;
-  if (!fn) {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) != cudaSuccess || !ptr) return -1;
-    fn = reinterpret_cast<K8pEncodeFn>(ptr);
-  }
-  const cuuint32_t estr[3] = {1, 1, 1};
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : -2;
-}
 template <int D>
 int k8p_launch(const CUtensorMap& tm, const CUtensorMap& te, const Kv8PrefillParams& p, int pairs, int cut_tiles, cudaStream_t st) {
   auto kern = cut_tiles > 0 ? kv8_prefill_kernel<D, true> : kv8_prefill_kernel<D, false>;
@@ -788,11 +768,8 @@ extern "C" int b200_kv8_prefill(const void* q, const void* gate, const void* dat
   const cuuint32_t rowb = D < 128 ? D : 128;
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(rows)}, strides[1] = {static_cast<cuuint64_t>(D)};
   const cuuint32_t box[2] = {rowb, KV8_PAGE};
-  const cuuint64_t edims[3] = {KV8_PAGE, static_cast<cuuint64_t>(n_kv), static_cast<cuuint64_t>(num_pages) * 2};
-  const cuuint64_t estrides[2] = {KV8_PAGE, static_cast<cuuint64_t>(n_kv) * KV8_PAGE};
-  const cuuint32_t ebox[3] = {KV8_PAGE, 1, 2};
-  if (k8p_encode(&tm, data, 2, dims, strides, box, rowb == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B) ||
-      k8p_encode(&te, exps, 3, edims, estrides, ebox, CU_TENSOR_MAP_SWIZZLE_NONE)) return -1;
+  if (kv8_encode(&tm, data, 2, dims, strides, box, rowb == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B) ||
+      kv8_encode_exps(&te, exps, n_kv, num_pages)) return -1;
   const Kv8PrefillParams p{static_cast<const bf16*>(q), static_cast<const bf16*>(gate), starts, pos0, tables, static_cast<bf16*>(out), part_acc,
                            reinterpret_cast<float2*>(part_ml), part_rows, T, segs, max_pages, width, num_pages, n_q, n_kv, group, 128 / group, exact,
                            (65536 + group - 1) / group, 1.4426950408889634f / sqrtf(static_cast<float>(D)), err};
