@@ -662,7 +662,14 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) { tc_fence_after(); tmem_dealloc(tmem, C::TMEM_COLS); }
+  if (warp == 8) {
+    tc_fence_after();
+    if (*abort_flag) {  // after a wait that ran out: products on their way end before their TMEM and shared memory go
+      const long long t0 = clock64();
+      while (!mbar_test(acc_done, 0) && clock64() - t0 < WAIT_CYCLES / 8) {}
+    }
+    tmem_dealloc(tmem, C::TMEM_COLS);
+  }
 }
 
 // Rows of spans that were cut: their partials in the order of the runs, eight under way. A thread takes four dims of a row's head. What does not
