@@ -1,5 +1,7 @@
 """Passes over the 8-bit KV cache as the engine makes them: unlike spans packed together, captured passes, spans from device memory."""
 
+import gc
+
 import pytest
 import torch
 from test_kv8_gpu import _attention, _check, _layer, _rows, _tables
@@ -14,6 +16,12 @@ def C():
 
     cuda_ops.lib()
     return cuda_ops
+
+
+@pytest.fixture(autouse=True)
+def collected():
+    """No engine of a test before is collected, and its graphs freed, while one of this test captures."""
+    gc.collect()
 
 
 class _Pass:
@@ -286,6 +294,7 @@ def test_engine_captures_what_can_be_captured(C, head_dim, n_q, n_kv, native):
     s = Sampling(max_tokens=8, ignore_eos=True)
 
     def run(prompts, **kw):
+        gc.collect()
         eng = Engine(w, EngineConfig(max_model_len=512, prefill_chunk_tokens=64, max_seqs=4, kv_pages=64, decode_buckets=(1, 4), kv_dtype="e4m3", **kw))
         eng.warmup()
         return eng, [x.output for x in eng.generate(prompts, s)]
