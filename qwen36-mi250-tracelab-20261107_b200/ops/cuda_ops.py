@@ -12,6 +12,7 @@ current stream, ``engine/fast/hipmega_rtc.py:150-215``).
 from __future__ import annotations
 
 import ctypes
+import functools
 import time
 from ctypes import c_float, c_int, c_void_p
 
@@ -875,6 +876,12 @@ def kv8_decode(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_table
     return out
 
 
+@functools.cache
+def _kv8_prefill_cut() -> tuple[int, int]:
+    """By what the kernel cuts spans (kv8_prefill.cu, k8p_run_pages): CTAs, the fewest pages of a run."""
+    return lib().b200_kv8_prefill_cut(0), lib().b200_kv8_prefill_cut(1)
+
+
 def kv8_prefill(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tables: torch.Tensor, seg_starts: list[int] | None,
                 seg_pos0: list[int] | None, meta=None) -> torch.Tensor:
     """``flash_prefill`` over the 8-bit cache: causal gated attention of ragged spans of new tokens over what their sequences' pages
@@ -900,12 +907,13 @@ def kv8_prefill(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tabl
         step = width
     if meta is not None:
         starts_t, pos0_t = meta
-        for t in meta:
-            if t.dtype != torch.int32 or t.device != dev or t.dim() != 1 or t.stride(0) != 1:
-                raise ValueError(f"kv8_prefill: meta holds contiguous int32 vectors on {dev}, not {t.dtype} {tuple(t.shape)} with strides {t.stride()} on {t.device}")
+        if starts_t.dtype is not torch.int32 or pos0_t.dtype is not torch.int32 or starts_t.stride() != (1,) or pos0_t.stride() != (1,) \
+                or starts_t.device != dev or pos0_t.device != dev:
+            raise ValueError(f"kv8_prefill: meta holds contiguous int32 vectors on {dev}, not " + " and ".join(
+                f"{t.dtype} {tuple(t.shape)} with strides {t.stride()} on {t.device}" for t in meta))
     # Launches: spans s0 .. s1, the (tile, run) pairs, the tiles of cut spans, their rows times their runs.
     launches = []
-    ctas, least = L.b200_kv8_prefill_cut(0), L.b200_kv8_prefill_cut(1)
+    ctas, least = _kv8_prefill_cut()
     most = KV8_PREFILL_PARTS // (n_q * (D + 2) * 4)
     if seg_starts is not None:
         n_seg = len(seg_pos0)
@@ -956,7 +964,7 @@ def kv8_prefill(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tabl
     if T == 0:
         return out
     acc = ml = None
-    part = max((x[4] for x in launches), default=0)
+    part = launches[0][4] if len(launches) == 1 else max((x[4] for x in launches), default=0)
     if part:  # of the cut spans' rows: sums, then maxima and sums of weights
         rows = part * n_q * 4
         scratch = data.new_empty(rows * (D + 2))  # bytes, as above
