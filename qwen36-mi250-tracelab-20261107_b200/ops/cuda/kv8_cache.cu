@@ -6,7 +6,7 @@
 // Bound: memory, 4 D bytes of bf16 and 2 (D + 1) of the cache per token and KV head. D / 8 (write) or D / 16 (read) neighbouring
 // lanes own a row, 16 bytes of input each, and take the key and the value of a (token, head) together: two loads in flight per thread and one
 // look-up of the page. The row maximum is one of its lanes' bits. Two rows a thread, all loads under way at once, were no faster (write, 6.9 us and
-// 6.7) or slower (read, 58.2 and 55.6).
+// 6.8) or slower (read, 58.2 and 55.6; all four before rows were counted in 32 bits).
 //
 // Measured, 2 heads of 256: 128 rows written in 1.8 us, which is a launch and two look-ups; 8,192 rows in 6.3 us (25 MB at 4.0 TB/s, of which 1.8 us
 // as before); 98,304 rows read in 54.3 us (304 MB at 5.6 TB/s: 85 % of the copy rate), 6,001 rows in 5.9 us.

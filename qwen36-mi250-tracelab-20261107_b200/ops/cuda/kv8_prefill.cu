@@ -15,14 +15,16 @@
 // Two groups of four warps take alternate pages, a thread a row; the running maximum goes from one to the other, and the output tile in
 // TMEM is rescaled where a maximum grew by more than 2^LAZY. Weights as halves reach from 2^15 to 2^-24, 2^-28 of the largest at the least.
 // A span of few tiles over a long context is cut into runs of pages for CTAs of their own, by its own length and position alone, whose partial
-// sums are added in their order: a row's bits depend on its span, never on the pass. All waits are bounded. No cluster multicast.
+// sums are added in their order: a row's bits depend on its span, never on the pass. There is a CTA for each (tile, run) that there is, found by a scan of the
+// spans, and partials for the rows of cut spans: 16 rows on 32,768 tokens beside three fresh spans of 2,048 take 238 us, where tiles times the most runs of
+// any span took 568. A captured pass has as many CTAs as its spans can come to. All waits are bounded. No cluster multicast.
 //
 // Bound: the tensor pipe would take 1,024 cycles for a page of 256-wide heads, shared memory 1,600 (keys twice and P once as operands, V once, the
 // conversion of V, weights and tables); a page takes 1,830 to 1,950. A tile's first scores come about 10,000 cycles after its start (queries to two terms,
 // to TMEM), and its end takes 7,000 to 8,000: most of a short context's time.
-// Measured, 16 heads of 256 over 2: 4 x 2,048 rows of prompts of about 28,672 tokens 1,540 to 1,600 us (1.55 TFLOP: 0.97 to 1.0 PFLOP/s; the bf16
-// cache's kernel 1,940), 8 x 1,024 rows of fresh prompts 149 us (206), 61 rows over 3,584 tokens 22.6 us, seven spans of 1,531 rows of
-// heads of 128, 6 over 3, 16.5 us.
+// Measured, 16 heads of 256 over 2: 4 x 2,048 rows of prompts of about 28,672 tokens 1,565 to 1,645 us (1.55 TFLOP: 0.94 to 0.99 PFLOP/s; the bf16
+// cache's kernel 1,940), 8 x 1,024 rows of fresh prompts 150 us (206), 61 rows over 3,584 tokens 23.0 us, seven spans of 1,531 rows of
+// heads of 128, 6 over 3, 15.2 us.
 #include <cuda_fp16.h>
 
 #include "kv8.cuh"
