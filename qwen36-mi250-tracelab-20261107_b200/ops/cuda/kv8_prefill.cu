@@ -227,10 +227,12 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   // One warp looks its tile up (all of them would take turns at the same instructions), while others make things ready. The last tiles of the
-  // spans see the most keys and go first, where no CTA without a pair goes ahead of them.
+  // spans see the most keys and go first; where the grid may have more CTAs than pairs, those with one do, of all heads.
+  const uint32_t cta = blockIdx.y * gridDim.x + blockIdx.x;
+  const int kh = PARTS && !p.exact ? cta % p.n_kv : blockIdx.y;
   if (warp == 0) {
     Kv8Tile t = {};
-    const bool found = k8p_find<PARTS, false>(p, static_cast<int>(p.exact ? gridDim.x - 1 - blockIdx.x : blockIdx.x), (blockIdx.x | blockIdx.y) == 0, t);
+    const bool found = k8p_find<PARTS, false>(p, static_cast<int>(!PARTS || p.exact ? gridDim.x - 1 - blockIdx.x : cta / p.n_kv), cta == 0, t);
     if (lane == 0) {
       const int n_pos = min(p.positions, t.rows - t.p0), first = t.run * t.run_pages;
       s_work->seg = t.seg;
@@ -242,6 +244,10 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
       s_work->runs = t.runs;
       s_work->part = t.part + static_cast<long long>(t.p0) * p.n_q * t.runs + t.run;
     }
+  }
+  if (PARTS && !p.exact) {  // many CTAs have no pair, and leave at once
+    __syncthreads();
+    if (s_work->np <= 0) return;
   }
   if (threadIdx.x == 32) {
     for (int s = 0; s < 2; ++s) {
@@ -268,7 +274,7 @@ kv8_prefill_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_launch();  // this CTA holds its TMEM columns
-  const int kh = blockIdx.y, row0 = s_work->row, n_pos = s_work->n_pos, pos0 = s_work->pos, np = s_work->np;
+  const int row0 = s_work->row, n_pos = s_work->n_pos, pos0 = s_work->pos, np = s_work->np;
   if (np <= 0) {  // no tile, or nothing of this run for its rows: the sum over the runs passes over it
     if (warp == 8) tmem_dealloc(tmem, C::TMEM_COLS);
     return;

@@ -944,7 +944,7 @@ def kv8_prefill(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tabl
         if seqs < n_seg:
             raise ValueError(f"kv8_prefill: meta of {n_seg} spans, page tables of {seqs} sequences")
         # The spans are not known here, and are cut as they would be by their lists: room for the most that they can come to. A span that is cut
-        # has at most ctas / n_kv pairs, of half as many tiles, and at least one.
+        # has at most ctas / n_kv pairs, of half as many tiles, and at least one; most pairs come of one span that is not, and all the others.
         each, runs = ctas // n_kv, -(-width // least)
         if each < 2 or runs < 2:
             launches.append((0, n_seg, T // per + n_seg, 0, 0))
@@ -953,7 +953,8 @@ def kv8_prefill(q: torch.Tensor, gate: torch.Tensor, layer: Kv8Layer, block_tabl
             for a in range(0, n_seg, at_once):
                 n = min(at_once, n_seg - a)
                 tiles = T // per + n
-                launches.append((a, a + n, min(tiles * runs, tiles + n * each), min(tiles, n * (each // 2)), min(n * per * each, T * runs)))
+                launches.append((a, a + n, min(tiles * runs, (n - 1) * each + max(each, T // per + 1)), min(tiles, n * (each // 2)),
+                                 min(n * per * each, T * runs)))
     if meta is not None:
         if starts_t.shape[0] < n_seg + 1 or pos0_t.shape[0] < n_seg:
             raise ValueError(f"kv8_prefill: meta of {starts_t.shape[0]} and {pos0_t.shape[0]} numbers for {n_seg} spans")
