@@ -94,6 +94,8 @@ class _Sig:
     b200_kv8_prefill_positions = [I]
     b200_kv8_prefill_cut = [I]
     b200_kv8_prefill = [P, P, P, P, P, P, I, I, I, I, I, L, P, I, I, I, I, I, I, P, P, P, P, P]
+    b200_sample_max_exclude = []
+    b200_sample = [P, I, L, I, I, P, P, P, P, P, P, I, P, P]
     b200_kv8_decode = [P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, P, P, P, P, P]
 
 
@@ -1003,6 +1005,50 @@ def _kv8_attention(qkv, positions, seq_of_row, block_tables, layer, q_norm, k_no
     if G == 0:
         return kv8_prefill(q, gate, layer, block_tables, seg_starts, seg_pos0, meta=meta)
     return kv8_decode(q, gate, layer, block_tables, positions, G)
+
+
+# --------------------------------------------------------------------------- sampling
+LOGIT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def sample(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor, top_p: torch.Tensor, min_p: torch.Tensor, u: torch.Tensor,
+           exclude: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Next token of each row of ``logits [n, V]`` (fp32, bf16 or fp16, rows at any stride): int64 ``[n]``, ``torch_ops.sample`` has the
+    rules. A row's own settings: ``temperature``, ``top_p``, ``min_p``, ``u`` fp32 ``[n]`` and ``top_k`` int32 ``[n]``; ``exclude [n, m]`` int32, at
+    most 64 ids per row. A row's pick depends on its own logits and settings only. ``out`` (int64 ``[n]``, contiguous) receives the picks in place of
+    a new tensor. Only device tensors are touched, so the call can be captured in a CUDA graph."""
+    shape = logits.shape
+    kind = LOGIT_TYPES.get(logits.dtype)
+    if not logits.is_cuda:
+        raise ValueError(f"sample: the logits are on {logits.device}: torch_ops has the operator for them")
+    if len(shape) != 2 or kind is None or shape[1] < 1 or shape[1] > 1 << 30:
+        raise ValueError(f"sample: logits {tuple(shape)} {logits.dtype} are not fp32, bf16 or fp16 [rows, vocabulary]")
+    n, V = shape
+    dev = logits.device
+    for name, t, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
+                           ("min_p", min_p, torch.float32), ("u", u, torch.float32)):
+        if t.shape != (n,) or t.dtype is not dtype or t.device != dev or not t.is_contiguous():
+            raise ValueError(f"sample: {name} {tuple(t.shape)} {t.dtype} with strides {t.stride()} on {t.device} is not a contiguous {dtype} [{n}] on {dev}")
+    m = 0
+    if exclude is not None:
+        m = exclude.shape[1] if exclude.dim() == 2 else -1
+        if exclude.shape != (n, m) or exclude.dtype is not torch.int32 or exclude.device != dev or not exclude.is_contiguous():
+            raise ValueError(f"sample: exclude {tuple(exclude.shape)} {exclude.dtype} on {exclude.device} is not a contiguous int32 [{n}, ids] on {dev}")
+        if m > lib().b200_sample_max_exclude():
+            raise ValueError(f"sample: {m} excluded ids per row, at most {lib().b200_sample_max_exclude()}")
+    if out is None:
+        out = torch.empty(n, dtype=torch.int64, device=dev)
+    elif out.shape != (n,) or out.dtype is not torch.int64 or out.device != dev or not out.is_contiguous():
+        raise ValueError(f"sample: out {tuple(out.shape)} {out.dtype} on {out.device} is not a contiguous int64 [{n}] on {dev}")
+    if n == 0:
+        return out
+    _err_ptr(dev)  # refuses tensors of another device than the current one
+    if logits.stride(1) != 1:
+        logits = logits.contiguous()
+    _check(lib().b200_sample(
+        logits.data_ptr(), kind, logits.stride(0), n, V, temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(), min_p.data_ptr(),
+        u.data_ptr(), exclude.data_ptr() if m else None, m, out.data_ptr(), _raw_stream(dev)), "sample")
+    return out
 
 
 def argmax_rows(logits: torch.Tensor) -> torch.Tensor:

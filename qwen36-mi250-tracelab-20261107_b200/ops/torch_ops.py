@@ -571,6 +571,38 @@ def attention(qkv, positions, seq_of_row, block_tables, kv_layer, q_norm, k_norm
 
 
 # --------------------------------------------------------------------------- head
+def sample(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor, top_p: torch.Tensor, min_p: torch.Tensor, u: torch.Tensor,
+           exclude: torch.Tensor | None = None) -> torch.Tensor:
+    """Next token of each row of ``logits [n, V]`` (fp32, bf16 or fp16): int64 ``[n]``.
+
+    With ``w_i = exp((x_i - max) / temperature)``, tokens stand in descending order of ``x``, the lower id first among equals. Kept are the
+    first ``top_k`` (0: all), of those the ones before which at most ``top_p`` of their weight stands, of those the ones of weight ``min_p``
+    at least; the pick is the first kept token up to which more than ``u`` (in ``[0, 1)``) of the kept weight stands. A row of temperature 0 picks
+    the first token of the order. ``exclude [n, m]`` int32 names tokens that count as minus infinity (entries outside ``[0, V)`` name none), as
+    do NaNs; a row with nothing but those gives -1. All in 64 bits: with a large vocabulary a draw decides between numbers 1e-9 apart."""
+    n, V = logits.shape
+    dev = logits.device
+    x = logits.double()
+    x = torch.where(x.isnan(), float("-inf"), x)
+    if exclude is not None and exclude.shape[1]:
+        ids = exclude.long()
+        x = torch.cat([x, x.new_zeros(n, 1)], 1).scatter_(1, ids.where((ids >= 0) & (ids < V), V), float("-inf"))[:, :V]
+    x, ids = torch.sort(x, dim=-1, descending=True, stable=True)
+    top, greedy = x[:, :1], ~(temperature > 0)
+    y = (x - top) / torch.where(greedy, 1.0, temperature.double())[:, None]
+    w = torch.where(x == top, 1.0, torch.where(y <= 0, torch.exp(y), 0.0)).masked_fill_(x == float("-inf"), 0.0)
+    rank = torch.arange(V, device=dev)[None, :]
+    k = top_k.long()[:, None]
+    w.masked_fill_((k > 0) & (rank >= k), 0.0)
+    cum = torch.cumsum(w, -1)
+    p = top_p.double()[:, None]
+    keep = ((cum - w <= p * cum[:, -1:]) | (p >= 1)) & (w >= min_p.double()[:, None]) & (w > 0)
+    last = (keep.sum(-1, keepdim=True) - 1).clamp_(min=0)  # the kept tokens are the first ones
+    at = (cum <= u.double()[:, None] * cum.gather(1, last)).sum(-1, keepdim=True)
+    at = torch.minimum(at, last).masked_fill_(greedy[:, None], 0)
+    return ids.gather(1, at)[:, 0].masked_fill_(top[:, 0] == float("-inf"), -1)
+
+
 def argmax_rows(logits: torch.Tensor) -> torch.Tensor:
     """First index of the row maximum (ties to the lower id)."""
     return torch.argmax(logits.float(), dim=-1)
