@@ -12,6 +12,7 @@
 // 400 to a neighbouring token, and a request's tokens would depend on how the sums were cut.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
+#include <float.h>
 
 #include "common.cuh"
 
@@ -30,6 +31,20 @@ struct SampleArgs {
   const int* exclude;  // [n, n_exclude], entries outside [0, V) name no token
   int n_exclude;
   int64_t* out;
+};
+
+// What a row's launches tell each other.
+struct SamplePlan {
+  float reach, least, ref;  // threshold of the list; below `least` a token has no weight; what the tail's weights are relative to
+  int skip;                 // the list cannot decide this row
+  uint32_t listed, done;    // tokens in the list, CTAs that have finished their part of the row
+};
+struct SampleWork {
+  int* left;         // rows left to the wide kernel, and which
+  int* left_rows;
+  SamplePlan* plan;  // [n]
+  uint64_t* list;    // [n, LIST]
+  double* tail;      // [n, tasks]
 };
 
 enum LogitType : int { LOGIT_F32 = 0, LOGIT_BF16 = 1, LOGIT_F16 = 2 };
@@ -63,6 +78,21 @@ __device__ __forceinline__ double weight_of(float x, float m, double inv_t) {
   if (x == m) return 1.0;
   const double y = (static_cast<double>(x) - static_cast<double>(m)) * inv_t;
   return y <= 0.0 ? exp(y) : 0.0;  // (a NaN: an infinite m and an infinite T)
+}
+
+// Descending; n a power of two.
+template <int THREADS>
+__device__ __forceinline__ void sort_down(uint64_t* a, int n) {
+  for (int k = 2; k <= n; k <<= 1)
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < n / 2; i += THREADS) {
+        const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
+        const uint64_t x = a[lo], y = a[hi];
+        if ((x < y) == ((lo & k) == 0)) { a[lo] = y; a[hi] = x; }
+      }
+    }
+  __syncthreads();
 }
 
 constexpr int WIDE_CTAS = 8;       // of a row: one cluster
@@ -261,21 +291,6 @@ struct WideRow {
     cluster.sync();
   }
 
-  // Descending by comp; n a power of two.
-  __device__ void sort_list(int n) {
-    uint64_t* a = s.list.item;
-    for (int k = 2; k <= n; k <<= 1)
-      for (int j = k >> 1; j > 0; j >>= 1) {
-        __syncthreads();
-        for (int i = tid; i < n / 2; i += WIDE_THREADS) {
-          const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
-          const uint64_t x = a[lo], y = a[hi];
-          if ((x < y) == ((lo & k) == 0)) { a[lo] = y; a[hi] = x; }
-        }
-      }
-    __syncthreads();
-  }
-
   // The place in the row's order: by count the token of rank `rank_target` (from 1), by weight the first one up to which more than
   // `target` stands (target: the first CTA's). Leaves comp in s.cut of every CTA, the weight up to and with it in s.cut_mass of the first.
   __device__ void search(bool by_count, uint32_t rank_target, double target) {
@@ -314,7 +329,7 @@ struct WideRow {
       int size = 2;
       while (size < n) size <<= 1;
       for (int i = n + tid; i < size; i += WIDE_THREADS) s.list.item[i] = 0;
-      sort_list(size);
+      sort_down<WIDE_THREADS>(s.list.item, size);
       constexpr int PER = WIDE_LIST / WIDE_THREADS;
       double v[PER];
       for (int j = 0; j < PER; ++j) {
@@ -348,13 +363,8 @@ struct WideRow {
 };
 
 template <typename T>
-__global__ void __cluster_dims__(WIDE_CTAS, 1, 1) __launch_bounds__(WIDE_THREADS)
-sample_wide_kernel(SampleArgs a) {
-  extern __shared__ __align__(16) uint8_t smem_raw[];
-  WideShared& s = *reinterpret_cast<WideShared*>(smem_raw);
-  pdl_wait();
-  pdl_launch();
-  const int at = blockIdx.x / WIDE_CTAS, tid = threadIdx.x;
+__device__ void sample_wide_row(const SampleArgs& a, int at, WideShared& s) {
+  const int tid = threadIdx.x;
   const int per = (a.V + WIDE_CTAS * 8 - 1) / (WIDE_CTAS * 8) * 8;
   WideRow<T> r(s, static_cast<const T*>(a.logits) + at * a.stride, a.V, per);
   const float temperature = a.temperature[at];
@@ -414,16 +424,462 @@ sample_wide_kernel(SampleArgs a) {
   if (first) a.out[at] = comp_id(s.cut > cut ? s.cut : cut);
 }
 
+// The rows that the stream left to this kernel: a cluster takes one after the other.
 template <typename T>
-static int launch_wide(const SampleArgs& a, cudaStream_t st) {
-  static bool configured[64] = {};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -3;
-  if (!configured[dev]) {
-    if (cudaFuncSetAttribute(sample_wide_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(WideShared)) != cudaSuccess) return -3;
-    configured[dev] = true;
+__global__ void __cluster_dims__(WIDE_CTAS, 1, 1) __launch_bounds__(WIDE_THREADS)
+sample_wide_kernel(SampleArgs a, SampleWork w) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  WideShared& s = *reinterpret_cast<WideShared*>(smem_raw);
+  pdl_wait();
+  pdl_launch();
+  const int rows = *w.left;
+  for (int i = blockIdx.x / WIDE_CTAS; i < rows; i += gridDim.x / WIDE_CTAS) {
+    sample_wide_row<T>(a, w.left_rows[i], s);
+    cg::this_cluster().sync();  // everyone has read what the next row writes over
   }
-  return launch_pdl(sample_wide_kernel<T>, dim3(a.n * WIDE_CTAS), dim3(WIDE_THREADS), sizeof(WideShared), st, a) == cudaSuccess ? 0 : -4;
+}
+
+// ------------------------------------------------------------------ the stream
+// Most rows are decided by their largest tokens. Three launches:
+//  plan    a CTA per row looks at 16,384 of its logits and guesses a threshold that about `want` tokens reach;
+//  stream  reads every logit once: tokens that reach the threshold go into the row's list, the weights of the others into the row's tail.
+//          The CTA that finishes a row last puts the list in order and searches it; a row whose place lies in the tail (or whose
+//          list has run over) is left to
+//  wide    the kernel above.
+// A guess that is off costs time, never a result: what the list and the tail say is exact.
+//
+// Sums are added up in an order that goes by V alone: the weights of a lane's tokens of a task, the lanes of a warp, the tasks of a row.
+constexpr int PLAN_THREADS = 512, PLAN_PER = 32, PLAN_SAMPLE = PLAN_THREADS * PLAN_PER, PLAN_BLOCK = 256, PLAN_BINS = 1024;
+constexpr int STREAM_THREADS = 256, STREAM_WARPS = STREAM_THREADS / 32;
+constexpr int TASK = 512;           // tokens that a warp takes at a time
+constexpr int LIST = 2048;          // most tokens of a list
+constexpr int LIST_PER = LIST / STREAM_THREADS;
+constexpr int LIST_K = 1024;        // top-k up to which a list is expected to hold the k tokens
+
+// What a list is made to hold: all of the k, with room for the guess's error (one part in sqrt(want * 16384 / V)), or as many as leave room above.
+__device__ __forceinline__ int list_want(bool greedy, int k) {
+  if (greedy) return 48;
+  if (k <= 0) return 1400;
+  return k <= 700 ? 2 * k + 64 : 1500;
+}
+
+// The settings of a row in a form that all CTAs agree on.
+struct RowAsk {
+  bool greedy, cut_k;  // cut_k: top-k leaves something out
+  int k;
+  double p, least, u, inv_t;
+  __device__ RowAsk(const SampleArgs& a, int at) {
+    const float t = a.temperature[at];
+    greedy = !(t > 0.f);
+    k = a.top_k[at];
+    cut_k = k > 0 && k < a.V;
+    p = a.top_p[at];
+    least = a.min_p[at];
+    u = a.u[at];
+    inv_t = greedy ? 1.0 : 1.0 / static_cast<double>(t);
+  }
+};
+
+// Sums over the threads before this one, in a fixed order; `warp_sum` holds one number per warp. All threads of the CTA.
+template <int THREADS>
+__device__ __forceinline__ double sum_before(double v, double* warp_sum) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  double up = v;
+  for (int o = 1; o < 32; o <<= 1) {
+    const double t = __shfl_up_sync(0xffffffffu, up, o);
+    if (lane >= o) up += t;
+  }
+  __syncthreads();
+  if (lane == 31) warp_sum[warp] = up;
+  __syncthreads();
+  double before = 0.0;
+  for (int w = 0; w < warp; ++w) before += warp_sum[w];
+  const double mine = __shfl_up_sync(0xffffffffu, up, 1);
+  return before + (lane ? mine : 0.0);
+}
+
+struct ListShared {
+  uint64_t item[LIST];
+  double warp_sum[STREAM_WARPS];
+  double total, cut;
+  int place, last;
+};
+
+// The pick of a row from its `c` largest tokens in s.item (unsorted) and the weight `tail` of all others, relative to `ref`; all: there
+// are no others of any weight. -2 where the tokens do not decide it. All threads of a CTA of STREAM_THREADS.
+__device__ int pick_from_list(ListShared& s, int c, const RowAsk& r, double tail, float ref, bool all) {
+  const int tid = threadIdx.x;
+  if (c == 0) return ref == -INFINITY && all ? -1 : -2;
+  int size = 2;
+  while (size < c) size <<= 1;
+  for (int i = c + tid; i < size; i += STREAM_THREADS) s.item[i] = 0;
+  sort_down<STREAM_THREADS>(s.item, size);
+  if (r.greedy) return comp_id(s.item[0]);
+  const float m = comp_value(s.item[0]);
+  // what weighs nothing beside `ref` weighs nothing beside m as well, unless m lies far below (an excluded token is the largest)
+  if ((static_cast<double>(ref) - static_cast<double>(m)) * r.inv_t > WIDE_RANGE / 4) return -2;
+  if (tail > 0.0) tail *= ref == m ? 1.0 : exp((static_cast<double>(ref) - static_cast<double>(m)) * r.inv_t);
+  else all = all || !r.cut_k;  // (a row with a top-k has no tail summed up)
+  if (!(tail < 1e300)) return -2;
+  if (r.cut_k && c < r.k && !all) return -2;
+  const int nk = r.cut_k ? min(r.k, c) : c;
+  const bool closed = r.cut_k || all;  // no token outside the list is in play
+
+  double cum[LIST_PER];
+  int positive = 0, enough = 0;
+#pragma unroll
+  for (int j = 0; j < LIST_PER; ++j) {
+    const int i = tid * LIST_PER + j;
+    const double w = i < nk ? weight_of(comp_value(s.item[i]), m, r.inv_t) : 0.0;
+    positive += w > 0.0;
+    enough += w >= r.least && i < nk;
+    cum[j] = w + (j ? cum[j - 1] : 0.0);
+  }
+  const double before = sum_before<STREAM_THREADS>(cum[LIST_PER - 1], s.warp_sum);
+#pragma unroll
+  for (int j = 0; j < LIST_PER; ++j) cum[j] += before;
+  if (tid == 0) { s.place = s.last = 0; }
+  if (tid == STREAM_THREADS - 1) s.total = cum[LIST_PER - 1] + (closed ? 0.0 : tail);
+  __syncthreads();
+  for (int o = 16; o; o >>= 1) { positive += __shfl_xor_sync(0xffffffffu, positive, o); enough += __shfl_xor_sync(0xffffffffu, enough, o); }
+  if ((tid & 31) == 0) { atomicAdd(&s.place, positive); atomicAdd(&s.last, enough); }
+  __syncthreads();
+  positive = s.place; enough = max(1, s.last);
+  const double sum = s.total;
+  constexpr int OPEN = 1 << 30;
+  int limit = closed ? nk : OPEN;
+  // the first place with more than `target` up to it, OPEN if there is none
+  const auto find = [&](double target) {
+    __syncthreads();
+    if (tid == 0) s.place = OPEN;
+    __syncthreads();
+    int at = OPEN;
+#pragma unroll
+    for (int j = LIST_PER - 1; j >= 0; --j)
+      if (cum[j] > target && tid * LIST_PER + j < nk) at = tid * LIST_PER + j;
+    if (at != OPEN) atomicMin(&s.place, at);
+    __syncthreads();
+    return s.place;
+  };
+  if (r.p < 1.0) {
+    const int at = find(r.p * sum);
+    if (at != OPEN) limit = at + 1;
+    else if (!closed) return -2;
+  }
+  if (r.least > 0.0) {
+    if (enough < nk || closed) limit = min(limit, enough);
+    else if (limit == OPEN) return -2;
+  }
+  double total = sum;
+  if (limit != OPEN) {
+    __syncthreads();
+    const int j = limit - 1 - tid * LIST_PER;
+#pragma unroll
+    for (int i = 0; i < LIST_PER; ++i)
+      if (i == j) s.cut = cum[i];
+    __syncthreads();
+    total = s.cut;
+  }
+  const int at = find(r.u * total);
+  if (at < limit && at != OPEN) return comp_id(s.item[at]);
+  if (limit == OPEN) return -2;
+  return comp_id(s.item[max(0, min(limit, positive) - 1)]);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(PLAN_THREADS) sample_plan_kernel(SampleArgs a, SampleWork w) {
+  __shared__ uint32_t bins[PLAN_BINS];
+  __shared__ float warp_top[PLAN_THREADS / 32], warp_low[PLAN_THREADS / 32];
+  __shared__ uint32_t warp_count[PLAN_THREADS / 32];
+  __shared__ int found;
+  pdl_wait();
+  pdl_launch();
+  const int at = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.V;
+  const T* row = static_cast<const T*>(a.logits) + at * a.stride;
+  const RowAsk ask(a, at);
+  if (at == 0 && tid == 0) *w.left = 0;
+  for (int b = tid; b < PLAN_BINS; b += PLAN_THREADS) bins[b] = 0;
+  if (tid == 0) found = -1;
+  float x[PLAN_PER];
+  float top = -INFINITY, low = INFINITY;
+  const bool whole = V <= PLAN_SAMPLE;
+#pragma unroll
+  for (int i = 0; i < PLAN_PER; ++i) {
+    int id = i * PLAN_THREADS + tid;
+    if (!whole) {
+      const long long block = i * (PLAN_THREADS / PLAN_BLOCK) + tid / PLAN_BLOCK;
+      id = static_cast<int>(block * (V - PLAN_BLOCK) / (PLAN_SAMPLE / PLAN_BLOCK - 1)) + tid % PLAN_BLOCK;
+    }
+    x[i] = id < V ? logit_value(row[id]) : -INFINITY;
+    top = fmaxf(top, x[i]);
+    if (x[i] != -INFINITY) low = fminf(low, x[i]);
+  }
+  for (int o = 16; o; o >>= 1) {
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+  }
+  if (lane == 0) { warp_top[warp] = top; warp_low[warp] = low; }
+  __syncthreads();
+  for (int i = 0; i < PLAN_THREADS / 32; ++i) { top = fmaxf(top, warp_top[i]); low = fminf(low, warp_low[i]); }
+  const float t = ask.greedy ? 1.f : a.temperature[at];
+  const float least = fmaxf(top - WIDE_RANGE * t, -FLT_MAX);  // below it nothing has any weight
+  const float range = fminf(fminf(WIDE_RANGE * t, top - low), 1e38f);
+  const float scale = range > 0.f ? fminf(PLAN_BINS / range, 1e38f) : 0.f;
+#pragma unroll
+  for (int i = 0; i < PLAN_PER; ++i)
+    if (x[i] >= least) atomicAdd(&bins[min(PLAN_BINS - 1, static_cast<int>((top - x[i]) * scale))], 1u);
+  __syncthreads();
+  // the bin in which the sample has its share of `want`
+  const int want = list_want(ask.greedy, ask.cut_k ? ask.k : 0);
+  const uint32_t share = max(1u, static_cast<uint32_t>(static_cast<long long>(want) * min(V, PLAN_SAMPLE) / V));
+  const uint32_t c0 = bins[2 * tid], c1 = bins[2 * tid + 1];
+  uint32_t up = c0 + c1;
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t v = __shfl_up_sync(0xffffffffu, up, o);
+    if (lane >= o) up += v;
+  }
+  if (lane == 31) warp_count[warp] = up;
+  __syncthreads();
+  for (int i = 0; i < warp; ++i) up += warp_count[i];
+  if (up >= share && up - c1 < share) found = 2 * tid + 1;
+  if (up - c1 >= share && up - c1 - c0 < share) found = 2 * tid;
+  __syncthreads();
+  if (tid == 0) {
+    float reach = found < 0 || scale == 0.f ? least : fmaxf(top - (found + 1) / scale, least);
+    const bool number = reach == reach;  // (infinite logits at an infinite temperature)
+    SamplePlan plan;
+    plan.reach = number ? reach : -FLT_MAX;
+    plan.least = number ? least : -FLT_MAX;
+    plan.ref = top;
+    plan.listed = 0;
+    plan.done = 0;
+    plan.skip = ask.cut_k && ask.k > LIST_K && reach > least;
+    w.plan[at] = plan;
+  }
+}
+
+// exp(d * inv_t) for d * inv_t in [-100, 0]: 2^(z / 256) by a table of the 256 fractions and a polynomial for what is left of the
+// argument, at most ln 2 / 512 of it either way, whose fifth power is below one part in 2^57. Eleven 64-bit operations for each token.
+struct ExpTable {
+  double two[256];
+  __device__ void fill() {
+    for (int i = threadIdx.x; i < 256; i += blockDim.x) two[i] = exp2(i / 256.0);
+  }
+  __device__ __forceinline__ double weight(double d, double inv_t, double inv_step) const {
+    const double z = fma(d, inv_step, 0x1.8p52);  // the nearest whole number stands in the low word
+    const int n = __double2loint(z);
+    const double r = fma(z - 0x1.8p52, -0.0027076061740622863, d * inv_t);  // ln 2 / 256
+    double q = fma(r, 1.0 / 24.0, 1.0 / 6.0);
+    q = fma(q, r, 0.5);
+    q = fma(q, r, 1.0);
+    const double t = two[n & 255];
+    const double scaled = __hiloint2double(__double2hiint(t) + ((n >> 8) << 20), __double2loint(t));
+    return fma(scaled, q * r, scaled);
+  }
+};
+// An fp32 number as fp64 by its bits (the conversion instruction takes four times as long as an addition); 0 and numbers below 2^-126 become some
+// that are as small, which nothing is lost by in a difference of logits.
+__device__ __forceinline__ double wide_of(float x) {
+  const uint32_t b = __float_as_uint(x);
+  return __hiloint2double(static_cast<int>((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + 0x38000000u)), static_cast<int>(b << 29));
+}
+
+// The sixteen logits of a lane in a task, from `row` on: piece i of 16 bytes holds tokens first + i * 32 * VE ..
+template <typename T>
+struct TaskLogits {
+  static constexpr int VE = 16 / sizeof(T), PIECES = TASK / (32 * VE);
+  static __device__ __forceinline__ int id(int first, int i, int j) { return first + i * 32 * VE + j; }
+  uint4 raw[PIECES];
+  __device__ __forceinline__ void load(const T* row, int first, int V, bool aligned) {
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const int at = id(first, i, 0);
+      if (aligned && at + VE <= V) {
+        raw[i] = __ldg(reinterpret_cast<const uint4*>(row + at));
+      } else {
+        T one[VE];
+#pragma unroll
+        for (int j = 0; j < VE; ++j) one[j] = at + j < V ? row[at + j] : static_cast<T>(-INFINITY);
+        memcpy(&raw[i], one, 16);
+      }
+    }
+  }
+  __device__ __forceinline__ float value(int i, int j) const {
+    T one[VE];
+    memcpy(one, &raw[i], 16);
+    return logit_value(one[j]);
+  }
+};
+
+// CTA x of a row takes `tasks_per_warp` tasks for each warp, from task x * STREAM_WARPS * tasks_per_warp on.
+template <typename T>
+__global__ void __launch_bounds__(STREAM_THREADS, 4) sample_stream_kernel(SampleArgs a, SampleWork w, int tasks, int tasks_per_warp) {
+  using Task = TaskLogits<T>;
+  __shared__ ListShared s;
+  __shared__ ExpTable table;
+  __shared__ int banned[SAMPLE_MAX_EXCLUDE];
+  __shared__ int n_banned;
+  const int at = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.V;
+  table.fill();
+  if (tid == 0) n_banned = 0;
+  __syncthreads();
+  pdl_wait();
+  pdl_launch();
+  const RowAsk ask(a, at);
+  SamplePlan& plan = w.plan[at];
+  if (plan.skip) {
+    if (blockIdx.x == 0 && tid == 0) w.left_rows[atomicAdd(w.left, 1)] = at;
+    return;
+  }
+  const float reach = plan.reach, least = plan.least, ref = plan.ref;
+  const T* row = static_cast<const T*>(a.logits) + at * a.stride;
+  const bool aligned = (reinterpret_cast<uintptr_t>(row) & 15) == 0;
+  const int task0 = blockIdx.x * STREAM_WARPS * tasks_per_warp;
+  for (int j = tid; j < a.n_exclude; j += STREAM_THREADS) {
+    const int id = a.exclude[static_cast<long long>(at) * a.n_exclude + j];
+    if (id >= task0 * TASK && id < min(V, (task0 + STREAM_WARPS * tasks_per_warp) * TASK)) banned[atomicAdd(&n_banned, 1)] = id;
+  }
+  if (a.n_exclude) __syncthreads();
+  const int bans = n_banned;
+  const bool with_tail = !ask.greedy && !ask.cut_k && reach > least;
+  const double ref_wide = wide_of(ref), inv_step = ask.inv_t * 369.32993046757463;  // 256 / ln 2
+  uint64_t* list = w.list + static_cast<size_t>(at) * LIST;
+
+  for (int i = 0; i < tasks_per_warp; ++i) {
+    const int task = task0 + i * STREAM_WARPS + warp;
+    if (task >= tasks) break;
+    const int first = task * TASK + lane * Task::VE;
+    Task x;
+    x.load(row, first, V, aligned);
+    uint32_t hits = 0;
+    double tail = 0.0;
+#pragma unroll
+    for (int p = 0; p < Task::PIECES; ++p)
+#pragma unroll
+      for (int j = 0; j < Task::VE; ++j) {
+        float v = x.value(p, j);
+        if (bans)
+          for (int e = 0; e < bans; ++e)
+            if (banned[e] == Task::id(first, p, j)) v = -INFINITY;
+        const bool hit = v >= reach;
+        hits |= static_cast<uint32_t>(hit) << (p * Task::VE + j);
+        if (with_tail && __any_sync(0xffffffffu, v >= least && !hit)) {
+          const double e = table.weight(wide_of(v) - ref_wide, ask.inv_t, inv_step);
+          tail += v >= least && !hit ? e : 0.0;
+        }
+      }
+    if (with_tail) {
+      for (int o = 16; o; o >>= 1) tail += __shfl_xor_sync(0xffffffffu, tail, o);
+      if (lane == 0) w.tail[static_cast<size_t>(at) * tasks + task] = tail;
+    }
+    if (__any_sync(0xffffffffu, hits)) {
+      const uint32_t mine = __popc(hits);
+      uint32_t up = mine;
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, up, o);
+        if (lane >= o) up += v;
+      }
+      uint32_t to = lane == 31 ? atomicAdd(&plan.listed, up) : 0;
+      to = __shfl_sync(0xffffffffu, to, 31) + up - mine;
+#pragma unroll
+      for (int p = 0; p < Task::PIECES; ++p)
+#pragma unroll
+        for (int j = 0; j < Task::VE; ++j)
+          if (hits >> (p * Task::VE + j) & 1) {
+            if (to < LIST) list[to] = comp_of(x.value(p, j), Task::id(first, p, j));
+            ++to;
+          }
+    }
+  }
+  __threadfence();
+  __syncthreads();
+  if (tid == 0) s.last = atomicAdd(&plan.done, 1u) == gridDim.x - 1;
+  __syncthreads();
+  if (!s.last) return;
+  __threadfence();
+  const uint32_t listed = __ldcg(&plan.listed);
+  int pick = -2;
+  if (listed <= LIST) {
+    double tail = 0.0;
+    if (with_tail) {
+      for (int i = tid; i < tasks; i += STREAM_THREADS) tail += __ldcg(w.tail + static_cast<size_t>(at) * tasks + i);
+      const double before = sum_before<STREAM_THREADS>(tail, s.warp_sum);
+      if (tid == STREAM_THREADS - 1) s.total = before + tail;
+      __syncthreads();
+      tail = s.total;
+    }
+    for (int i = tid; i < static_cast<int>(listed); i += STREAM_THREADS) s.item[i] = __ldcg(list + i);
+    __syncthreads();
+    pick = pick_from_list(s, static_cast<int>(listed), ask, tail, ref, reach <= least);
+  }
+  if (tid == 0) {
+    if (pick == -2) w.left_rows[atomicAdd(w.left, 1)] = at;
+    else a.out[at] = pick;
+  }
+}
+
+// A vocabulary that fits a list: one launch, a CTA per row.
+template <typename T>
+__global__ void __launch_bounds__(STREAM_THREADS) sample_short_kernel(SampleArgs a) {
+  __shared__ ListShared s;
+  __shared__ int listed;
+  const int at = blockIdx.x, tid = threadIdx.x;
+  if (tid == 0) listed = 0;
+  pdl_wait();
+  pdl_launch();
+  __syncthreads();
+  const T* row = static_cast<const T*>(a.logits) + at * a.stride;
+  for (int i = tid; i < a.V; i += STREAM_THREADS) {
+    const uint64_t c = comp_of(logit_value(row[i]), i);
+    bool out = c == 0;
+    for (int j = 0; j < a.n_exclude; ++j) out |= a.exclude[static_cast<long long>(at) * a.n_exclude + j] == i;
+    if (!out) s.item[atomicAdd(&listed, 1)] = c;
+  }
+  __syncthreads();
+  const int pick = pick_from_list(s, listed, RowAsk(a, at), 0.0, -INFINITY, true);
+  if (tid == 0) a.out[at] = pick;
+}
+
+constexpr int MAX_DEVICES = 64;
+
+static size_t align_up(size_t v) { return (v + 255) / 256 * 256; }
+static int task_count(int V) { return (V + TASK - 1) / TASK; }
+
+// Bytes of a call's workspace: [left][left rows][plans][lists][tails]
+static size_t sample_work(int n, int V, void* base, SampleWork* w) {
+  size_t at = 0;
+  uint8_t* p = static_cast<uint8_t*>(base);
+  const auto take = [&](size_t bytes) { uint8_t* r = p + at; at += align_up(bytes); return r; };
+  w->left = reinterpret_cast<int*>(take(4));
+  w->left_rows = reinterpret_cast<int*>(take(static_cast<size_t>(n) * 4));
+  w->plan = reinterpret_cast<SamplePlan*>(take(static_cast<size_t>(n) * sizeof(SamplePlan)));
+  w->list = reinterpret_cast<uint64_t*>(take(static_cast<size_t>(n) * LIST * 8));
+  w->tail = reinterpret_cast<double*>(take(static_cast<size_t>(n) * task_count(V) * 8));
+  return at;
+}
+
+template <typename T>
+static int launch_sample(const SampleArgs& a, void* work, cudaStream_t st) {
+  if (a.V <= LIST)
+    return launch_pdl(sample_short_kernel<T>, dim3(a.n), dim3(STREAM_THREADS), 0, st, a) == cudaSuccess ? 0 : -4;
+  static int sms[MAX_DEVICES] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= MAX_DEVICES) return -3;
+  if (!sms[dev]) {
+    if (cudaFuncSetAttribute(sample_wide_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(WideShared)) != cudaSuccess) return -3;
+    if (cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return -3;
+  }
+  SampleWork w;
+  sample_work(a.n, a.V, work, &w);
+  const int tasks = task_count(a.V);
+  // tasks for a warp: as many as leave every SM a few CTAs
+  const long long all = static_cast<long long>(tasks) * a.n / STREAM_WARPS, most = 16LL * sms[dev];
+  const int per = static_cast<int>(all / most < 1 ? 1 : all / most > 16 ? 16 : all / most);
+  const int ctas = (tasks + STREAM_WARPS * per - 1) / (STREAM_WARPS * per);
+  const int clusters = a.n < sms[dev] / WIDE_CTAS ? a.n : sms[dev] / WIDE_CTAS;
+  if (launch_pdl(sample_plan_kernel<T>, dim3(a.n), dim3(PLAN_THREADS), 0, st, a, w) != cudaSuccess) return -4;
+  if (launch_pdl(sample_stream_kernel<T>, dim3(ctas, a.n), dim3(STREAM_THREADS), 0, st, a, w, tasks, per) != cudaSuccess) return -4;
+  return launch_pdl(sample_wide_kernel<T>, dim3(clusters * WIDE_CTAS), dim3(WIDE_THREADS), sizeof(WideShared), st, a, w) == cudaSuccess ? 0 : -4;
 }
 
 }  // namespace b200
@@ -431,17 +887,23 @@ static int launch_wide(const SampleArgs& a, cudaStream_t st) {
 using namespace b200;
 
 extern "C" int b200_sample_max_exclude() { return SAMPLE_MAX_EXCLUDE; }
+extern "C" int b200_sample_max_rows() { return 65535; }
+
+extern "C" long long b200_sample_work_bytes(int n, int V) {
+  SampleWork w;
+  return V <= LIST ? 0 : static_cast<long long>(sample_work(n, V, nullptr, &w));
+}
 
 extern "C" int b200_sample(const void* logits, int type, long long stride, int n, int V, const float* temperature, const int* top_k,
                            const float* top_p, const float* min_p, const float* u, const int* exclude, int n_exclude, int64_t* out,
-                           cudaStream_t st) {
+                           void* work, cudaStream_t st) {
   if (n <= 0) return 0;
-  if (V <= 0 || n_exclude < 0 || n_exclude > SAMPLE_MAX_EXCLUDE || V > (1 << 30) || n > (1 << 27)) return -7;
+  if (V <= 0 || n_exclude < 0 || n_exclude > SAMPLE_MAX_EXCLUDE || V > (1 << 30) || n > b200_sample_max_rows()) return -7;
   const SampleArgs a{logits, stride, n, V, temperature, top_k, top_p, min_p, u, exclude, n_exclude, out};
   switch (type) {
-    case LOGIT_F32: return launch_wide<float>(a, st);
-    case LOGIT_BF16: return launch_wide<bf16>(a, st);
-    case LOGIT_F16: return launch_wide<__half>(a, st);
+    case LOGIT_F32: return launch_sample<float>(a, work, st);
+    case LOGIT_BF16: return launch_sample<bf16>(a, work, st);
+    case LOGIT_F16: return launch_sample<__half>(a, work, st);
   }
   return -7;
 }

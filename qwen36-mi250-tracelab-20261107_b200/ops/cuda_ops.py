@@ -95,7 +95,9 @@ class _Sig:
     b200_kv8_prefill_cut = [I]
     b200_kv8_prefill = [P, P, P, P, P, P, I, I, I, I, I, L, P, I, I, I, I, I, I, P, P, P, P, P]
     b200_sample_max_exclude = []
-    b200_sample = [P, I, L, I, I, P, P, P, P, P, P, I, P, P]
+    b200_sample_max_rows = []
+    b200_sample_work_bytes = [I, I]
+    b200_sample = [P, I, L, I, I, P, P, P, P, P, P, I, P, P, P]
     b200_kv8_decode = [P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, P, P, P, P, P]
 
 
@@ -1008,6 +1010,16 @@ def _kv8_attention(qkv, positions, seq_of_row, block_tables, layer, q_norm, k_no
 
 
 # --------------------------------------------------------------------------- sampling
+SAMPLE_ROWS = 4096  # of one launch
+
+
+@functools.cache
+def _sample_work(n: int, V: int) -> int:
+    fn = lib().b200_sample_work_bytes
+    fn.restype = ctypes.c_longlong
+    return fn(n, V)
+
+
 LOGIT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -1045,9 +1057,16 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor,
     _err_ptr(dev)  # refuses tensors of another device than the current one
     if logits.stride(1) != 1:
         logits = logits.contiguous()
+    if n > SAMPLE_ROWS:  # parts of the rows, each with a workspace of its own
+        for i in range(0, n, SAMPLE_ROWS):
+            j = slice(i, i + SAMPLE_ROWS)
+            sample(logits[j], temperature[j], top_k[j], top_p[j], min_p[j], u[j], None if exclude is None else exclude[j], out[j])
+        return out
+    size = _sample_work(n, V)
+    work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     _check(lib().b200_sample(
         logits.data_ptr(), kind, logits.stride(0), n, V, temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(), min_p.data_ptr(),
-        u.data_ptr(), exclude.data_ptr() if m else None, m, out.data_ptr(), _raw_stream(dev)), "sample")
+        u.data_ptr(), exclude.data_ptr() if m else None, m, out.data_ptr(), _ptr(work), _raw_stream(dev)), "sample")
     return out
 
 
