@@ -96,7 +96,8 @@ __device__ __forceinline__ void sort_down(uint64_t* a, int n) {
 }
 
 constexpr int WIDE_CTAS = 8;       // of a row: one cluster
-constexpr int WIDE_THREADS = 512;
+constexpr int WIDE_THREADS = 1024;
+constexpr int WIDE_BATCH = 8;      // logits that a thread asks for at a time
 constexpr int WIDE_BINS = 2048;
 constexpr int WIDE_LIST = 2048;    // candidates that are put in order one by one
 constexpr float WIDE_RANGE = 80.f; // e^-80 of the largest weight, 2^18 times, is nothing in 64 bits
@@ -150,10 +151,17 @@ struct WideRow {
   // f(x, comp) for every token of this CTA's part that counts
   template <typename F>
   __device__ void each(F f) const {
-    for (int i = begin + tid; i < end; i += WIDE_THREADS) {
-      const float x = logit_value(row[i]);
-      const uint64_t c = comp_of(x, i);
-      if (c != 0 && !(s.n_banned && banned(i))) f(x, c);
+    for (int i0 = begin + tid; i0 < end; i0 += WIDE_THREADS * WIDE_BATCH) {
+      T raw[WIDE_BATCH];
+#pragma unroll
+      for (int j = 0; j < WIDE_BATCH; ++j) raw[j] = i0 + j * WIDE_THREADS < end ? row[i0 + j * WIDE_THREADS] : static_cast<T>(-INFINITY);
+#pragma unroll
+      for (int j = 0; j < WIDE_BATCH; ++j) {
+        const int i = i0 + j * WIDE_THREADS;
+        const float x = logit_value(raw[j]);
+        const uint64_t c = comp_of(x, i);
+        if (c != 0 && !(s.n_banned && banned(i))) f(x, c);
+      }
     }
   }
   __device__ int bin_of(float x) const { return min(WIDE_BINS - 1, static_cast<int>((m - x) * scale)); }
@@ -450,7 +458,7 @@ sample_wide_kernel(SampleArgs a, SampleWork w) {
 //
 // Sums are added up in an order that goes by V alone: the weights of a lane's tokens of a task, the lanes of a warp, the tasks of a row.
 constexpr int PLAN_THREADS = 512, PLAN_PER = 32, PLAN_SAMPLE = PLAN_THREADS * PLAN_PER, PLAN_BLOCK = 256, PLAN_BINS = 1024;
-constexpr int STREAM_THREADS = 256, STREAM_WARPS = STREAM_THREADS / 32;
+constexpr int STREAM_THREADS = 512, STREAM_WARPS = STREAM_THREADS / 32;
 constexpr int TASK = 512;           // tokens that a warp takes at a time
 constexpr int LIST = 2048;          // most tokens of a list
 constexpr int LIST_PER = LIST / STREAM_THREADS;
@@ -498,22 +506,77 @@ __device__ __forceinline__ double sum_before(double v, double* warp_sum) {
   return before + (lane ? mine : 0.0);
 }
 
+constexpr int LIST_BINS = 1024;
+constexpr int LIST_BIN_MOST = 96;  // tokens of a bin that are compared each with each
+
 struct ListShared {
-  uint64_t item[LIST];
+  uint64_t item[LIST], other[LIST];
+  uint32_t bins[LIST_BINS];
+  uint32_t warp_count[STREAM_WARPS];
   double warp_sum[STREAM_WARPS];
   double total, cut;
   int place, last;
 };
 
+// Puts s.item[0 .. c) into descending order: bins by value, in a bin by comparing each with each. `hi` and `lo`: about where the values lie.
+// Rows of many equal values are sorted by exchanges instead. (1,400 tokens by exchanges alone: TODO us of a row's 22.)
+__device__ void order_list(ListShared& s, int c, float hi, float lo) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  static_assert(LIST_BINS == 2 * STREAM_THREADS, "two bins per thread");
+  const float scale = hi > lo ? fminf(LIST_BINS / (hi - lo), 1e30f) : 0.f;
+  s.bins[2 * tid] = s.bins[2 * tid + 1] = 0;
+  __syncthreads();
+  uint64_t mine[LIST_PER];
+  uint32_t bin[LIST_PER], at[LIST_PER];
+#pragma unroll
+  for (int j = 0; j < LIST_PER; ++j) {
+    const int i = tid + j * STREAM_THREADS;
+    if (i < c) {
+      mine[j] = s.item[i];
+      bin[j] = min(LIST_BINS - 1, max(0, static_cast<int>((hi - comp_value(mine[j])) * scale)));
+      at[j] = atomicAdd(&s.bins[bin[j]], 1u);
+    }
+  }
+  __syncthreads();
+  const uint32_t c0 = s.bins[2 * tid], c1 = s.bins[2 * tid + 1];
+  uint32_t up = c0 + c1;
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t v = __shfl_up_sync(0xffffffffu, up, o);
+    if (lane >= o) up += v;
+  }
+  if (lane == 31) s.warp_count[warp] = up;
+  if (__syncthreads_or(max(c0, c1) > LIST_BIN_MOST)) {
+    int size = 2;
+    while (size < c) size <<= 1;
+    for (int i = c + tid; i < size; i += STREAM_THREADS) s.item[i] = 0;
+    sort_down<STREAM_THREADS>(s.item, size);
+    return;
+  }
+  for (int w = 0; w < warp; ++w) up += s.warp_count[w];
+  s.bins[2 * tid] = up - c1 - c0;  // where a bin starts
+  s.bins[2 * tid + 1] = up - c1;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < LIST_PER; ++j)
+    if (tid + j * STREAM_THREADS < c) s.other[s.bins[bin[j]] + at[j]] = mine[j];
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < LIST_PER; ++j)
+    if (tid + j * STREAM_THREADS < c) {
+      const uint32_t from = s.bins[bin[j]], to = bin[j] + 1 < LIST_BINS ? s.bins[bin[j] + 1] : static_cast<uint32_t>(c);
+      uint32_t above = from;
+      for (uint32_t i = from; i < to; ++i) above += s.other[i] > mine[j];
+      s.item[above] = mine[j];
+    }
+  __syncthreads();
+}
+
 // The pick of a row from its `c` largest tokens in s.item (unsorted) and the weight `tail` of all others, relative to `ref`; all: there
 // are no others of any weight. -2 where the tokens do not decide it. All threads of a CTA of STREAM_THREADS.
-__device__ int pick_from_list(ListShared& s, int c, const RowAsk& r, double tail, float ref, bool all) {
+__device__ int pick_from_list(ListShared& s, int c, const RowAsk& r, double tail, float ref, bool all, float hi, float lo) {
   const int tid = threadIdx.x;
   if (c == 0) return ref == -INFINITY && all ? -1 : -2;
-  int size = 2;
-  while (size < c) size <<= 1;
-  for (int i = c + tid; i < size; i += STREAM_THREADS) s.item[i] = 0;
-  sort_down<STREAM_THREADS>(s.item, size);
+  order_list(s, c, hi, lo);
   if (r.greedy) return comp_id(s.item[0]);
   const float m = comp_value(s.item[0]);
   // what weighs nothing beside `ref` weighs nothing beside m as well, unless m lies far below (an excluded token is the largest)
@@ -653,28 +716,32 @@ __global__ void __launch_bounds__(PLAN_THREADS) sample_plan_kernel(SampleArgs a,
     plan.ref = top;
     plan.listed = 0;
     plan.done = 0;
-    plan.skip = ask.cut_k && ask.k > LIST_K && reach > least;
+    plan.skip = (ask.cut_k && ask.k > LIST_K && reach > least) || t > 1e30f;  // (at such a temperature even a token of `least` weighs something)
     w.plan[at] = plan;
   }
 }
 
-// exp(d * inv_t) for d * inv_t in [-100, 0]: 2^(z / 256) by a table of the 256 fractions and a polynomial for what is left of the
-// argument, at most ln 2 / 512 of it either way, whose fifth power is below one part in 2^57. Eleven 64-bit operations for each token.
-struct ExpTable {
-  double two[256];
-  __device__ void fill() {
-    for (int i = threadIdx.x; i < 256; i += blockDim.x) two[i] = exp2(i / 256.0);
+// 2^(s / 32) for s in [-4000, 0] and a little more: the fraction's 32 values are held by a warp's lanes, and what is left of s, at most half either
+// way, goes through a polynomial: with f ln 2 / 32 = g, at most 0.011, the powers of g over their factorials up to the fifth (the sixth is one part
+// in 2^49). All lanes of the warp take part. Ten 64-bit operations for each token, the multiplication into the caller's sum included.
+struct ExpLanes {
+  int lo, hi;
+  __device__ __forceinline__ ExpLanes() {
+    const double t = exp2((threadIdx.x & 31) / 32.0);
+    lo = __double2loint(t);
+    hi = __double2hiint(t);
   }
-  __device__ __forceinline__ double weight(double d, double inv_t, double inv_step) const {
-    const double z = fma(d, inv_step, 0x1.8p52);  // the nearest whole number stands in the low word
+  static constexpr double G = 0.69314718055994531 / 32;
+  __device__ __forceinline__ double add(double sum, double s) const {
+    const double z = s + 0x1.8p52;  // the nearest whole number stands in the low word
     const int n = __double2loint(z);
-    const double r = fma(z - 0x1.8p52, -0.0027076061740622863, d * inv_t);  // ln 2 / 256
-    double q = fma(r, 1.0 / 24.0, 1.0 / 6.0);
-    q = fma(q, r, 0.5);
-    q = fma(q, r, 1.0);
-    const double t = two[n & 255];
-    const double scaled = __hiloint2double(__double2hiint(t) + ((n >> 8) << 20), __double2loint(t));
-    return fma(scaled, q * r, scaled);
+    const double f = s - (z - 0x1.8p52);
+    double q = fma(f, G * G * G * G * G / 120, G * G * G * G / 24);
+    q = fma(f, q, G * G * G / 6);
+    q = fma(f, q, G * G / 2);
+    q = fma(f, q, G);
+    const double t = __hiloint2double(__shfl_sync(0xffffffffu, hi, n) + ((n & ~31) << 15), __shfl_sync(0xffffffffu, lo, n));
+    return fma(t, fma(f, q, 1.0), sum);
   }
 };
 // An fp32 number as fp64 by its bits (the conversion instruction takes four times as long as an addition); 0 and numbers below 2^-126 become some
@@ -704,23 +771,22 @@ struct TaskLogits {
       }
     }
   }
-  __device__ __forceinline__ float value(int i, int j) const {
+  __device__ __forceinline__ T value(int i, int j) const {
     T one[VE];
     memcpy(one, &raw[i], 16);
-    return logit_value(one[j]);
+    return one[j];
   }
 };
 
 // CTA x of a row takes `tasks_per_warp` tasks for each warp, from task x * STREAM_WARPS * tasks_per_warp on.
 template <typename T>
-__global__ void __launch_bounds__(STREAM_THREADS, 4) sample_stream_kernel(SampleArgs a, SampleWork w, int tasks, int tasks_per_warp) {
+__global__ void __launch_bounds__(STREAM_THREADS, 2) sample_stream_kernel(SampleArgs a, SampleWork w, int tasks, int tasks_per_warp) {
   using Task = TaskLogits<T>;
   __shared__ ListShared s;
-  __shared__ ExpTable table;
   __shared__ int banned[SAMPLE_MAX_EXCLUDE];
   __shared__ int n_banned;
   const int at = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.V;
-  table.fill();
+  const ExpLanes exps;
   if (tid == 0) n_banned = 0;
   __syncthreads();
   pdl_wait();
@@ -742,7 +808,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, 4) sample_stream_kernel(Sample
   if (a.n_exclude) __syncthreads();
   const int bans = n_banned;
   const bool with_tail = !ask.greedy && !ask.cut_k && reach > least;
-  const double ref_wide = wide_of(ref), inv_step = ask.inv_t * 369.32993046757463;  // 256 / ln 2
+  const double step = ask.inv_t * 46.166241308446828, start = -static_cast<double>(ref) * step;  // 32 / ln 2
   uint64_t* list = w.list + static_cast<size_t>(at) * LIST;
 
   for (int i = 0; i < tasks_per_warp; ++i) {
@@ -757,16 +823,14 @@ __global__ void __launch_bounds__(STREAM_THREADS, 4) sample_stream_kernel(Sample
     for (int p = 0; p < Task::PIECES; ++p)
 #pragma unroll
       for (int j = 0; j < Task::VE; ++j) {
-        float v = x.value(p, j);
+        float v = static_cast<float>(x.value(p, j));  // (a NaN is in neither the list nor the tail)
         if (bans)
           for (int e = 0; e < bans; ++e)
             if (banned[e] == Task::id(first, p, j)) v = -INFINITY;
         const bool hit = v >= reach;
         hits |= static_cast<uint32_t>(hit) << (p * Task::VE + j);
-        if (with_tail && __any_sync(0xffffffffu, v >= least && !hit)) {
-          const double e = table.weight(wide_of(v) - ref_wide, ask.inv_t, inv_step);
-          tail += v >= least && !hit ? e : 0.0;
-        }
+        // (tokens that are not the tail's add e^-80 each: nothing)
+        if (with_tail) tail = exps.add(tail, fma(wide_of(hit ? least : fmaxf(v, least)), step, start));
       }
     if (with_tail) {
       for (int o = 16; o; o >>= 1) tail += __shfl_xor_sync(0xffffffffu, tail, o);
@@ -786,7 +850,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, 4) sample_stream_kernel(Sample
 #pragma unroll
         for (int j = 0; j < Task::VE; ++j)
           if (hits >> (p * Task::VE + j) & 1) {
-            if (to < LIST) list[to] = comp_of(x.value(p, j), Task::id(first, p, j));
+            if (to < LIST) list[to] = comp_of(logit_value(x.value(p, j)), Task::id(first, p, j));
             ++to;
           }
     }
@@ -810,7 +874,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, 4) sample_stream_kernel(Sample
     }
     for (int i = tid; i < static_cast<int>(listed); i += STREAM_THREADS) s.item[i] = __ldcg(list + i);
     __syncthreads();
-    pick = pick_from_list(s, static_cast<int>(listed), ask, tail, ref, reach <= least);
+    pick = pick_from_list(s, static_cast<int>(listed), ask, tail, ref, reach <= least, ref, reach);
   }
   if (tid == 0) {
     if (pick == -2) w.left_rows[atomicAdd(w.left, 1)] = at;
@@ -823,8 +887,9 @@ template <typename T>
 __global__ void __launch_bounds__(STREAM_THREADS) sample_short_kernel(SampleArgs a) {
   __shared__ ListShared s;
   __shared__ int listed;
+  __shared__ uint32_t top, low;  // as order keys
   const int at = blockIdx.x, tid = threadIdx.x;
-  if (tid == 0) listed = 0;
+  if (tid == 0) { listed = 0; top = 0; low = ~0u; }
   pdl_wait();
   pdl_launch();
   __syncthreads();
@@ -833,10 +898,13 @@ __global__ void __launch_bounds__(STREAM_THREADS) sample_short_kernel(SampleArgs
     const uint64_t c = comp_of(logit_value(row[i]), i);
     bool out = c == 0;
     for (int j = 0; j < a.n_exclude; ++j) out |= a.exclude[static_cast<long long>(at) * a.n_exclude + j] == i;
-    if (!out) s.item[atomicAdd(&listed, 1)] = c;
+    if (out) continue;
+    s.item[atomicAdd(&listed, 1)] = c;
+    atomicMax(&top, static_cast<uint32_t>(c >> 32));
+    atomicMin(&low, static_cast<uint32_t>(c >> 32));
   }
   __syncthreads();
-  const int pick = pick_from_list(s, listed, RowAsk(a, at), 0.0, -INFINITY, true);
+  const int pick = pick_from_list(s, listed, RowAsk(a, at), 0.0, -INFINITY, true, key_value(top), key_value(low));
   if (tid == 0) a.out[at] = pick;
 }
 
