@@ -670,8 +670,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) sample_plan_kernel(SampleArgs a,
   for (int i = 0; i < PLAN_PER; ++i) {
     int id = i * PLAN_THREADS + tid;
     if (!whole) {
-      const long long block = i * (PLAN_THREADS / PLAN_BLOCK) + tid / PLAN_BLOCK;
-      id = static_cast<int>(block * (V - PLAN_BLOCK) / (PLAN_SAMPLE / PLAN_BLOCK - 1)) + tid % PLAN_BLOCK;
+      const int block = i * (PLAN_THREADS / PLAN_BLOCK) + tid / PLAN_BLOCK;
+      id = block * ((V - PLAN_BLOCK) / (PLAN_SAMPLE / PLAN_BLOCK - 1)) + tid % PLAN_BLOCK;
     }
     x[i] = id < V ? logit_value(row[id]) : -INFINITY;
     top = fmaxf(top, x[i]);
@@ -744,23 +744,16 @@ struct ExpLanes {
     return fma(t, fma(f, q, 1.0), sum);
   }
 };
-// An fp32 number as fp64 by its bits (the conversion instruction takes four times as long as an addition); 0 and numbers below 2^-126 become some
-// that are as small, which nothing is lost by in a difference of logits.
-__device__ __forceinline__ double wide_of(float x) {
-  const uint32_t b = __float_as_uint(x);
-  return __hiloint2double(static_cast<int>((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + 0x38000000u)), static_cast<int>(b << 29));
-}
-
 // The sixteen logits of a lane in a task, from `row` on: piece i of 16 bytes holds tokens first + i * 32 * VE ..
 template <typename T>
 struct TaskLogits {
   static constexpr int VE = 16 / sizeof(T), PIECES = TASK / (32 * VE);
-  static __device__ __forceinline__ int id(int first, int i, int j) { return first + i * 32 * VE + j; }
+  static __device__ __forceinline__ int id(int first, int e) { return first + e / VE * (32 * VE) + e % VE; }
   uint4 raw[PIECES];
   __device__ __forceinline__ void load(const T* row, int first, int V, bool aligned) {
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
-      const int at = id(first, i, 0);
+      const int at = id(first, i * VE);
       if (aligned && at + VE <= V) {
         raw[i] = __ldg(reinterpret_cast<const uint4*>(row + at));
       } else {
@@ -771,10 +764,23 @@ struct TaskLogits {
       }
     }
   }
-  __device__ __forceinline__ T value(int i, int j) const {
+  __device__ __forceinline__ float value(int e) const {
     T one[VE];
-    memcpy(one, &raw[i], 16);
-    return one[j];
+    memcpy(one, &raw[e / VE], 16);
+    return static_cast<float>(one[e % VE]);
+  }
+  // minus infinity in the place of the tokens named
+  __device__ __forceinline__ void strike(int first, const int* ids, int n) {
+    for (int b = 0; b < n; ++b)
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        T one[VE];
+        memcpy(one, &raw[i], 16);
+#pragma unroll
+        for (int j = 0; j < VE; ++j)
+          if (id(first, i * VE + j) == ids[b]) one[j] = static_cast<T>(-INFINITY);
+        memcpy(&raw[i], one, 16);
+      }
   }
 };
 
@@ -817,24 +823,23 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) sample_stream_kernel(Sample
     const int first = task * TASK + lane * Task::VE;
     Task x;
     x.load(row, first, V, aligned);
+    if (bans) x.strike(first, banned, bans);
     uint32_t hits = 0;
-    double tail = 0.0;
-#pragma unroll
-    for (int p = 0; p < Task::PIECES; ++p)
-#pragma unroll
-      for (int j = 0; j < Task::VE; ++j) {
-        float v = static_cast<float>(x.value(p, j));  // (a NaN is in neither the list nor the tail)
-        if (bans)
-          for (int e = 0; e < bans; ++e)
-            if (banned[e] == Task::id(first, p, j)) v = -INFINITY;
-        const bool hit = v >= reach;
-        hits |= static_cast<uint32_t>(hit) << (p * Task::VE + j);
-        // (tokens that are not the tail's add e^-80 each: nothing)
-        if (with_tail) tail = exps.add(tail, fma(wide_of(hit ? least : fmaxf(v, least)), step, start));
-      }
     if (with_tail) {
+      double tail = 0.0;
+#pragma unroll
+      for (int e = 0; e < TASK / 32; ++e) {
+        const float v = x.value(e);
+        const bool hit = v >= reach;  // (a NaN is in neither the list nor the tail)
+        hits |= hit ? 1u << e : 0u;
+        // tokens that are not the tail's add e^-80 each: nothing
+        tail = exps.add(tail, fma(static_cast<double>(hit ? least : fmaxf(v, least)), step, start));
+      }
       for (int o = 16; o; o >>= 1) tail += __shfl_xor_sync(0xffffffffu, tail, o);
       if (lane == 0) w.tail[static_cast<size_t>(at) * tasks + task] = tail;
+    } else {
+#pragma unroll
+      for (int e = 0; e < TASK / 32; ++e) hits |= x.value(e) >= reach ? 1u << e : 0u;
     }
     if (__any_sync(0xffffffffu, hits)) {
       const uint32_t mine = __popc(hits);
@@ -845,14 +850,10 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) sample_stream_kernel(Sample
       }
       uint32_t to = lane == 31 ? atomicAdd(&plan.listed, up) : 0;
       to = __shfl_sync(0xffffffffu, to, 31) + up - mine;
-#pragma unroll
-      for (int p = 0; p < Task::PIECES; ++p)
-#pragma unroll
-        for (int j = 0; j < Task::VE; ++j)
-          if (hits >> (p * Task::VE + j) & 1) {
-            if (to < LIST) list[to] = comp_of(logit_value(x.value(p, j)), Task::id(first, p, j));
-            ++to;
-          }
+      for (; hits; hits &= hits - 1, ++to) {
+        const int id = Task::id(first, __ffs(hits) - 1);
+        if (to < LIST) list[to] = comp_of(logit_value(row[id]), id);
+      }
     }
   }
   __threadfence();
