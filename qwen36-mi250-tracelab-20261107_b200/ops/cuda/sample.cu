@@ -35,8 +35,11 @@ struct SampleArgs {
 
 // What a row's launches tell each other.
 struct SamplePlan {
+  double step;              // 32 log2 of a logit's weight beside `ref` is (logit - ref) * step
   float reach, least, ref;  // threshold of the list; below `least` a token has no weight; what the tail's weights are relative to
-  int skip;                 // the list cannot decide this row
+  float low;                // the sample's smallest
+  int skip, with_tail;      // the list cannot decide this row; the others' weights are summed up
+  uint64_t top;             // of a row that is left with a whole list: its first token
   uint32_t listed, done;    // tokens in the list, CTAs that have finished their part of the row
 };
 struct SampleWork {
@@ -45,6 +48,7 @@ struct SampleWork {
   SamplePlan* plan;  // [n]
   uint64_t* list;    // [n, LIST]
   double* tail;      // [n, tasks]
+  double* powers;    // 2^(i / 32)
 };
 
 enum LogitType : int { LOGIT_F32 = 0, LOGIT_BF16 = 1, LOGIT_F16 = 2 };
@@ -95,25 +99,119 @@ __device__ __forceinline__ void sort_down(uint64_t* a, int n) {
   __syncthreads();
 }
 
-constexpr int WIDE_CTAS = 8;       // of a row: one cluster
+constexpr int LIST = 2048;         // most tokens that are put in order one by one
+constexpr int LIST_BINS = 1024;
+constexpr int LIST_BIN_MOST = 96;  // tokens of a bin that are compared each with each
+
+struct Order {
+  uint64_t item[LIST], other[LIST];
+  uint32_t bins[LIST_BINS], warp_count[32];
+};
+
+// Puts s.item[0 .. c) into descending order: bins by value, in a bin each is compared with each. `hi` and `lo`: about where the values lie.
+// Many equal values are sorted by exchanges instead, which take 66 rounds for a full list. All threads of the CTA.
+template <int THREADS>
+__device__ void order_list(Order& s, int c, float hi, float lo) {
+  constexpr int PER = LIST / THREADS, BINS = LIST_BINS / THREADS;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const float scale = hi > lo ? fminf(LIST_BINS / (hi - lo), 1e30f) : 0.f;
+#pragma unroll
+  for (int j = 0; j < BINS; ++j) s.bins[tid * BINS + j] = 0;
+  __syncthreads();
+  uint64_t mine[PER];
+  uint32_t bin[PER], at[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int i = tid + j * THREADS;
+    if (i < c) {
+      mine[j] = s.item[i];
+      bin[j] = min(LIST_BINS - 1, max(0, static_cast<int>((hi - comp_value(mine[j])) * scale)));
+      at[j] = atomicAdd(&s.bins[bin[j]], 1u);
+    }
+  }
+  __syncthreads();
+  uint32_t own[BINS], most = 0, up = 0;
+#pragma unroll
+  for (int j = 0; j < BINS; ++j) { own[j] = s.bins[tid * BINS + j]; most = max(most, own[j]); up += own[j]; }
+  const uint32_t sum = up;
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t v = __shfl_up_sync(0xffffffffu, up, o);
+    if (lane >= o) up += v;
+  }
+  if (lane == 31) s.warp_count[warp] = up;
+  if (__syncthreads_or(most > LIST_BIN_MOST)) {
+    int size = 2;
+    while (size < c) size <<= 1;
+    for (int i = c + tid; i < size; i += THREADS) s.item[i] = 0;
+    sort_down<THREADS>(s.item, size);
+    return;
+  }
+  for (int w = 0; w < warp; ++w) up += s.warp_count[w];
+  up -= sum;
+#pragma unroll
+  for (int j = 0; j < BINS; ++j) { s.bins[tid * BINS + j] = up; up += own[j]; }  // where a bin starts
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < PER; ++j)
+    if (tid + j * THREADS < c) s.other[s.bins[bin[j]] + at[j]] = mine[j];
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < PER; ++j)
+    if (tid + j * THREADS < c) {
+      const uint32_t from = s.bins[bin[j]], to = bin[j] + 1 < LIST_BINS ? s.bins[bin[j] + 1] : static_cast<uint32_t>(c);
+      uint32_t above = from;
+      for (uint32_t i = from; i < to; ++i) above += s.other[i] > mine[j];
+      s.item[above] = mine[j];
+    }
+  __syncthreads();
+}
+
+// 2^(s / 32) for s in [-4000, 0] and a little more: the fraction's 32 values are held by a warp's lanes, and what is left of s, at most half either
+// way, goes through a polynomial: with f ln 2 / 32 = g, at most 0.011, the powers of g over their factorials up to the fifth (the sixth is one part
+// in 2^49). All lanes of the warp take part. Nine 64-bit operations, the multiplication into the caller's sum included.
+struct ExpLanes {
+  int lo, hi;
+  __device__ __forceinline__ explicit ExpLanes(double power_of_lane) {
+    lo = __double2loint(power_of_lane);
+    hi = __double2hiint(power_of_lane);
+  }
+  static constexpr double G = 0.69314718055994531 / 32;
+  __device__ __forceinline__ double add(double sum, double s) const {
+    const double z = s + 0x1.8p52;  // the nearest whole number stands in the low word
+    const int n = __double2loint(z);
+    const double f = s - (z - 0x1.8p52);
+    double q = fma(f, G * G * G * G * G / 120, G * G * G * G / 24);
+    q = fma(f, q, G * G * G / 6);
+    q = fma(f, q, G * G / 2);
+    q = fma(f, q, G);
+    const double t = __hiloint2double(__shfl_sync(0xffffffffu, hi, n) + ((n & ~31) << 15), __shfl_sync(0xffffffffu, lo, n));
+    return fma(t, fma(f, q, 1.0), sum);
+  }
+};
+constexpr double STEPS = 46.166241308446828;  // 32 / ln 2
+
+constexpr int WIDE_CTAS = 16;       // of a row: one cluster
 constexpr int WIDE_THREADS = 1024;
-constexpr int WIDE_BATCH = 8;      // logits that a thread asks for at a time
+constexpr int WIDE_HELD = 16384;    // logits that a CTA holds; its part of a larger vocabulary is read again in every pass
 constexpr int WIDE_BINS = 2048;
-constexpr int WIDE_LIST = 2048;    // candidates that are put in order one by one
-constexpr float WIDE_RANGE = 80.f; // e^-80 of the largest weight, 2^18 times, is nothing in 64 bits
+constexpr int WIDE_LIMBS = 4;
+constexpr float WIDE_RANGE = 80.f;  // e^-80 of the largest weight, 2^22 times, is nothing in 64 bits
+constexpr int SAMPLE_MAX_VOCAB = 1 << 22;
 
 struct WideTable {  // sums up to and with each bin, of the whole row
   uint32_t count[WIDE_BINS];
   double mass[WIDE_BINS];
 };
 struct WideShared {
+  float held[WIDE_HELD];
   union {
-    struct { uint32_t count[WIDE_BINS], m0[WIDE_BINS], m1[WIDE_BINS], m2[WIDE_BINS]; } bins;  // this CTA's part; a mass in 96 bits
-    struct { uint64_t item[WIDE_LIST]; double mass[WIDE_LIST]; } list;                       // (of the first CTA)
+    struct { uint32_t count[WIDE_BINS], mass[WIDE_LIMBS][WIDE_BINS]; } bins;  // this CTA's part
+    Order list;                                                             // (of the first CTA)
   };
   WideTable first, finer;  // of the first CTA
   uint64_t top[WIDE_CTAS], low[WIDE_CTAS];  // every CTA's
   double part[WIDE_CTAS];
+  unsigned long long sums[1 + WIDE_LIMBS][WIDE_BINS / WIDE_CTAS];
   double warp_sum[WIDE_THREADS / 32];
   uint64_t warp_top[WIDE_THREADS / 32], warp_low[WIDE_THREADS / 32];
   uint32_t warp_count[WIDE_THREADS / 32];
@@ -125,324 +223,408 @@ struct WideShared {
   uint32_t members;
   uint64_t cut;
   // the first CTA's
+  int place;
   uint32_t base_count;
   double base_mass, cut_mass;
 };
 
-// One row, one cluster. `T` is the type of the logits.
+// One row, one cluster. This is one-off code: what it takes is the latency of its steps and of fetching their instructions, so what is used
+// twice is there once. Arguments go by value, into registers.
 template <typename T>
-struct WideRow {
-  cg::cluster_group cluster = cg::this_cluster();
+struct WidePart {  // a CTA's part of the row
   WideShared& s;
   const T* row;
-  const int rank, tid, V, begin, end;
-  float m, scale;  // maximum; bins per unit of m - x
-  double inv_t;
-  uint64_t range_lo, range_hi;  // the members of the bin that a search is in
+  int begin, end;
+  bool held;
 
-  __device__ WideRow(WideShared& sh, const T* r, int v, int per)
-      : s(sh), row(r), rank(cluster_rank()), tid(threadIdx.x), V(v), begin(min(v, rank * per)), end(min(v, rank * per + per)) {}
-
-  __device__ bool banned(int id) const {
+  // The logit of token i, minus infinity for one that does not count and behind the end.
+  __device__ __forceinline__ float value(int i) const {
+    if (i >= end) return -INFINITY;
+    if (held) return s.held[i - begin];
     for (int j = 0; j < s.n_banned; ++j)
-      if (s.banned[j] == id) return true;
-    return false;
+      if (s.banned[j] == i) return -INFINITY;
+    return logit_value(row[i]);
   }
-  // f(x, comp) for every token of this CTA's part that counts
+  // f(x, id) for every token, by whole warps
   template <typename F>
-  __device__ void each(F f) const {
-    for (int i0 = begin + tid; i0 < end; i0 += WIDE_THREADS * WIDE_BATCH) {
-      T raw[WIDE_BATCH];
-#pragma unroll
-      for (int j = 0; j < WIDE_BATCH; ++j) raw[j] = i0 + j * WIDE_THREADS < end ? row[i0 + j * WIDE_THREADS] : static_cast<T>(-INFINITY);
-#pragma unroll
-      for (int j = 0; j < WIDE_BATCH; ++j) {
-        const int i = i0 + j * WIDE_THREADS;
-        const float x = logit_value(raw[j]);
-        const uint64_t c = comp_of(x, i);
-        if (c != 0 && !(s.n_banned && banned(i))) f(x, c);
-      }
+  __device__ __forceinline__ void each(F f) const {
+    const int stop = begin + (end - begin + WIDE_THREADS - 1) / WIDE_THREADS * WIDE_THREADS;
+    if (held) {
+#pragma unroll 4
+      for (int i = begin + static_cast<int>(threadIdx.x); i < stop; i += WIDE_THREADS) f(i < end ? s.held[i - begin] : -INFINITY, i);
+    } else {
+#pragma unroll 1
+      for (int i = begin + static_cast<int>(threadIdx.x); i < stop; i += WIDE_THREADS) f(value(i), i);
     }
   }
-  __device__ int bin_of(float x) const { return min(WIDE_BINS - 1, static_cast<int>((m - x) * scale)); }
+};
+struct WideScale {
+  float m, floor, scale;  // maximum; below it no weight; bins per unit of m - x
+  double inv_t, step;
+  __device__ __forceinline__ int bin(float x) const { return min(WIDE_BINS - 1, static_cast<int>((m - x) * scale)); }
+};
 
-  // largest and smallest comp over the cluster, in every CTA (0 where there is none)
-  __device__ void extremes(uint64_t& top, uint64_t& low) {
+// Largest and smallest over the cluster, in every CTA.
+__device__ __noinline__ void wide_extremes(WideShared& s, uint64_t* top_of, uint64_t* low_of) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int tid = threadIdx.x;
+  uint64_t top = *top_of, low = *low_of;
+  for (int o = 16; o; o >>= 1) {
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    low = min(low, __shfl_xor_sync(0xffffffffu, low, o));
+  }
+  if ((tid & 31) == 0) { s.warp_top[tid >> 5] = top; s.warp_low[tid >> 5] = low; }
+  __syncthreads();
+  if (tid < 32) {
+    top = s.warp_top[tid]; low = s.warp_low[tid];
     for (int o = 16; o; o >>= 1) {
       top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
       low = min(low, __shfl_xor_sync(0xffffffffu, low, o));
     }
-    if ((tid & 31) == 0) { s.warp_top[tid >> 5] = top; s.warp_low[tid >> 5] = low; }
-    __syncthreads();
     if (tid < WIDE_CTAS) {
-      for (int w = 0; w < WIDE_THREADS / 32; ++w) { top = max(top, s.warp_top[w]); low = min(low, s.warp_low[w]); }
-      *cluster.map_shared_rank(&s.top[rank], tid) = top;
-      *cluster.map_shared_rank(&s.low[rank], tid) = low;
+      *cluster.map_shared_rank(&s.top[cluster_rank()], tid) = top;
+      *cluster.map_shared_rank(&s.low[cluster_rank()], tid) = low;
     }
-    cluster.sync();
-    top = 0; low = ~0ull;
-    for (int r = 0; r < WIDE_CTAS; ++r) { top = max(top, s.top[r]); low = min(low, s.low[r]); }
   }
-  // sum over the cluster in a fixed order, in every CTA
-  __device__ double sum(double v) {
+  cluster.sync();
+  top = 0; low = ~0ull;
+#pragma unroll
+  for (int r = 0; r < WIDE_CTAS; ++r) { top = max(top, s.top[r]); low = min(low, s.low[r]); }
+  *top_of = top; *low_of = low;
+}
+// Sum over the cluster in a fixed order, in every CTA.
+__device__ double wide_sum(WideShared& s, double v) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int tid = threadIdx.x;
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if ((tid & 31) == 0) s.warp_sum[tid >> 5] = v;
+  __syncthreads();
+  if (tid < 32) {
+    v = s.warp_sum[tid];
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if ((tid & 31) == 0) s.warp_sum[tid >> 5] = v;
-    __syncthreads();
-    if (tid < WIDE_CTAS) {
-      v = 0.0;
-      for (int w = 0; w < WIDE_THREADS / 32; ++w) v += s.warp_sum[w];
-      *cluster.map_shared_rank(&s.part[rank], tid) = v;
-    }
-    cluster.sync();
-    v = 0.0;
-    for (int r = 0; r < WIDE_CTAS; ++r) v += s.part[r];
-    cluster.sync();
-    return v;
+    if (tid < WIDE_CTAS) *cluster.map_shared_rank(&s.part[cluster_rank()], tid) = v;
   }
+  cluster.sync();
+  v = 0.0;
+#pragma unroll
+  for (int r = 0; r < WIDE_CTAS; ++r) v += s.part[r];
+  cluster.sync();
+  return v;
+}
 
-  __device__ void clear() {
-    for (int b = tid; b < WIDE_BINS; b += WIDE_THREADS) s.bins.count[b] = s.bins.m0[b] = s.bins.m1[b] = s.bins.m2[b] = 0;
-    __syncthreads();
+// The sums of the threads before this one; all threads of the CTA.
+__device__ __forceinline__ double wide_before(WideShared& s, double v, uint32_t c, uint32_t* count) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  double up = v;
+  uint32_t cup = c;
+  for (int o = 1; o < 32; o <<= 1) {
+    const double t = __shfl_up_sync(0xffffffffu, up, o);
+    const uint32_t tc = __shfl_up_sync(0xffffffffu, cup, o);
+    if (lane >= o) { up += t; cup += tc; }
   }
-  // a weight as a whole number of 2^-62: integers add up to the same sum in any order
-  __device__ void add(int b, double w) {
-    atomicAdd(&s.bins.count[b], 1u);
-    const unsigned long long f = __double2ull_rn(w * 0x1p62);
-    const uint32_t lo = static_cast<uint32_t>(f);
-    uint32_t hi = static_cast<uint32_t>(f >> 32);
-    if (lo) hi += atomicAdd(&s.bins.m0[b], lo) > 0xffffffffu - lo;
-    if (hi && atomicAdd(&s.bins.m1[b], hi) > 0xffffffffu - hi) atomicAdd(&s.bins.m2[b], 1u);
+  __syncthreads();
+  if (lane == 31) { s.warp_sum[warp] = up; s.warp_count[warp] = cup; }
+  __syncthreads();
+  double of = s.warp_sum[lane];
+  uint32_t cof = s.warp_count[lane];
+  for (int o = 1; o < 32; o <<= 1) {
+    const double t = __shfl_up_sync(0xffffffffu, of, o);
+    const uint32_t tc = __shfl_up_sync(0xffffffffu, cof, o);
+    if (lane >= o) { of += t; cof += tc; }
   }
-  // the CTAs' bins to sums up to each bin, in the first CTA
-  __device__ void tabulate(WideTable WideShared::*which) {
-    cluster.sync();
-    constexpr int OWN = WIDE_BINS / WIDE_CTAS;
-    WideTable* table = cluster.map_shared_rank(&(s.*which), 0);
-    if (tid < OWN) {
-      const int b = rank * OWN + tid;
-      unsigned long long count = 0, m0 = 0, m1 = 0, m2 = 0;
-      for (int r = 0; r < WIDE_CTAS; ++r) {
-        const auto* from = cluster.map_shared_rank(&s.bins, r);
-        count += from->count[b]; m0 += from->m0[b]; m1 += from->m1[b]; m2 += from->m2[b];
-      }
-      table->count[b] = static_cast<uint32_t>(count);
-      table->mass[b] = static_cast<double>(m2) * 4.0 + static_cast<double>(m1) * 0x1p-30 + static_cast<double>(m0) * 0x1p-62;
-    }
-    cluster.sync();
-    if (rank != 0) return;
-    constexpr int PER = WIDE_BINS / WIDE_THREADS;
-    WideTable& t = s.*which;
-    uint32_t c[PER];
-    double v[PER];
-    for (int j = 0; j < PER; ++j) {
-      c[j] = t.count[tid * PER + j] + (j ? c[j - 1] : 0u);
-      v[j] = t.mass[tid * PER + j] + (j ? v[j - 1] : 0.0);
-    }
-    uint32_t before_c = 0;
-    const double before = scan_before(v[PER - 1], c[PER - 1], &before_c);
-    for (int j = 0; j < PER; ++j) { t.count[tid * PER + j] = before_c + c[j]; t.mass[tid * PER + j] = before + v[j]; }
-    __syncthreads();
-  }
-  // sums of the threads before this one; all threads of the CTA
-  __device__ double scan_before(double v, uint32_t c, uint32_t* count) {
-    const int lane = tid & 31, warp = tid >> 5;
-    double up = v;
-    uint32_t cup = c;
-    for (int o = 1; o < 32; o <<= 1) {
-      const double t = __shfl_up_sync(0xffffffffu, up, o);
-      const uint32_t tc = __shfl_up_sync(0xffffffffu, cup, o);
-      if (lane >= o) { up += t; cup += tc; }
-    }
-    __syncthreads();
-    if (lane == 31) { s.warp_sum[warp] = up; s.warp_count[warp] = cup; }
-    __syncthreads();
-    double before = 0.0;
-    uint32_t cbefore = 0;
-    for (int w = 0; w < warp; ++w) { before += s.warp_sum[w]; cbefore += s.warp_count[w]; }
-    const double mine = __shfl_up_sync(0xffffffffu, up, 1);
-    const uint32_t cmine = __shfl_up_sync(0xffffffffu, cup, 1);
-    *count = cbefore + (lane ? cmine : 0u);
-    return before + (lane ? mine : 0.0);
-  }
+  const double before = __shfl_sync(0xffffffffu, of, warp - 1);
+  const uint32_t cbefore = __shfl_sync(0xffffffffu, cof, warp - 1);
+  const double mine = __shfl_up_sync(0xffffffffu, up, 1);
+  const uint32_t cmine = __shfl_up_sync(0xffffffffu, cup, 1);
+  *count = (warp ? cbefore : 0u) + (lane ? cmine : 0u);
+  return (warp ? before : 0.0) + (lane ? mine : 0.0);
+}
 
-  // The first CTA looks for the bin with the place: the first one up to which more than `target` of the weight stands, or (by_count)
-  // at least `rank_target` tokens; the last one with any, if there is none. Behind the barrier all CTAs know the bin.
-  __device__ void find_bin(const WideTable& t, bool by_count, uint32_t rank_target, double target, uint32_t base_count, double base_mass) {
-    if (rank == 0) {
-      if (tid == 0) s.bin = -1;
+// The tokens that `place` gives a bin (none: -1) into this CTA's bins. A weight goes in as a whole number, in limbs of as many bits as no sum of this
+// CTA's tokens runs over with: whole numbers add up to the same sum in any order.
+template <typename T, typename F>
+__device__ __forceinline__ void wide_tally(const WidePart<T>& part, const WideScale& c, double power, bool counts, F place) {
+  WideShared& s = part.s;
+  for (int b = threadIdx.x; b < WIDE_BINS * (1 + WIDE_LIMBS); b += WIDE_THREADS) s.bins.count[b] = 0;  // (and the masses behind the counts)
+  __syncthreads();
+  const ExpLanes exps(power);
+  const double one = part.held ? 0x1p54 : 0x1p56, m = c.m;
+  const int limb = part.held ? 18 : 14;
+  const uint32_t mask = (1u << limb) - 1;
+  part.each([&](float x, int i) {
+    double w = exps.add(0.0, (static_cast<double>(x) - m) * c.step);
+    if (x < c.floor) w = 0.0;
+    if (c.m == INFINITY) w = x == c.m ? 1.0 : 0.0;
+    const int b = x == -INFINITY ? -1 : place(x, i);
+    if (b < 0) return;
+    if (counts) atomicAdd(&s.bins.count[b], 1u);
+    unsigned long long f = __double2ull_rn(w * one);
+#pragma unroll
+    for (int l = 0; l < WIDE_LIMBS; ++l) {
+      const uint32_t v = static_cast<uint32_t>(f) & (l == WIDE_LIMBS - 1 ? ~0u : mask);
+      if (v) atomicAdd(&s.bins.mass[l][b], v);
+      f >>= limb;
+    }
+  });
+}
+
+// The CTAs' bins to sums up to each bin, in the first CTA.
+__device__ __noinline__ void wide_tabulate(WideShared& s, bool finer, bool held) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int tid = threadIdx.x;
+  cluster.sync();
+  // a thread for each number of the bins that this CTA adds up: a warp's lanes read neighbours from one CTA after the other
+  constexpr int OWN = WIDE_BINS / WIDE_CTAS;
+  static_assert(OWN * (1 + WIDE_LIMBS) <= WIDE_THREADS, "a thread for each number");
+  const int b = cluster_rank() * OWN + tid % OWN, l = tid / OWN;
+  if (l <= WIDE_LIMBS) {
+    unsigned long long sum = 0;
+#pragma unroll
+    for (int r = 0; r < WIDE_CTAS; ++r) sum += *cluster.map_shared_rank(&s.bins.count[l * WIDE_BINS + b], r);
+    s.sums[l][tid % OWN] = sum;
+  }
+  __syncthreads();
+  if (tid < OWN) {
+    WideTable* table = cluster.map_shared_rank(finer ? &s.finer : &s.first, 0);
+    table->count[b] = static_cast<uint32_t>(s.sums[0][tid]);
+    double v = 0.0;
+#pragma unroll
+    for (int i = WIDE_LIMBS; i >= 1; --i) v = v * (held ? 0x1p18 : 0x1p14) + static_cast<double>(s.sums[i][tid]);
+    table->mass[b] = v * (held ? 0x1p-54 : 0x1p-56);
+  }
+  cluster.sync();
+  if (cluster_rank() != 0) return;
+  constexpr int PER = WIDE_BINS / WIDE_THREADS;
+  WideTable& t = finer ? s.finer : s.first;
+  uint32_t c[PER];
+  double v[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    c[j] = t.count[tid * PER + j] + (j ? c[j - 1] : 0u);
+    v[j] = t.mass[tid * PER + j] + (j ? v[j - 1] : 0.0);
+  }
+  uint32_t before_c = 0;
+  const double before = wide_before(s, v[PER - 1], c[PER - 1], &before_c);
+#pragma unroll
+  for (int j = 0; j < PER; ++j) { t.count[tid * PER + j] = before_c + c[j]; t.mass[tid * PER + j] = before + v[j]; }
+  __syncthreads();
+}
+
+// The first CTA looks for the bin with the place: the first one up to which more than `target` of the weight stands, or (by_count)
+// at least `rank_target` tokens; the last one with any, if there is none. Behind the barrier all CTAs know the bin.
+__device__ __noinline__ void wide_find(WideShared& s, bool finer, bool by_count, uint32_t rank_target, double target, uint32_t base_count,
+                                       double base_mass) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int tid = threadIdx.x;
+  if (cluster_rank() == 0) {
+    const WideTable& t = finer ? s.finer : s.first;
+    if (tid == 0) s.bin = -1;
+    __syncthreads();
+    for (int b = tid; b < WIDE_BINS; b += WIDE_THREADS) {
+      const bool here = by_count ? base_count + t.count[b] >= rank_target : base_mass + t.mass[b] > target;
+      const bool before = b > 0 && (by_count ? base_count + t.count[b - 1] >= rank_target : base_mass + t.mass[b - 1] > target);
+      if (here && !before) s.bin = b;
+    }
+    __syncthreads();
+    if (s.bin < 0) {  // all of it stands before the target, by a rounding or by more: the last bin that has any
       __syncthreads();
       for (int b = tid; b < WIDE_BINS; b += WIDE_THREADS) {
-        const bool here = by_count ? base_count + t.count[b] >= rank_target : base_mass + t.mass[b] > target;
-        const bool before = b > 0 && (by_count ? base_count + t.count[b - 1] >= rank_target : base_mass + t.mass[b - 1] > target);
-        if (here && !before) s.bin = b;
+        const bool any = by_count ? t.count[b] == t.count[WIDE_BINS - 1] && t.count[b] > (b ? t.count[b - 1] : 0u)
+                                  : t.mass[b] == t.mass[WIDE_BINS - 1] && t.mass[b] > (b ? t.mass[b - 1] : 0.0);
+        if (any) s.bin = b;
       }
       __syncthreads();
-      if (s.bin < 0) {  // all of it stands before the target, by a rounding or by more: the last bin that has any
-        __syncthreads();
-        for (int b = tid; b < WIDE_BINS; b += WIDE_THREADS) {
-          const bool any = by_count ? t.count[b] == t.count[WIDE_BINS - 1] && t.count[b] > (b ? t.count[b - 1] : 0u)
-                                    : t.mass[b] == t.mass[WIDE_BINS - 1] && t.mass[b] > (b ? t.mass[b - 1] : 0.0);
-          if (any) s.bin = b;
-        }
-        __syncthreads();
-      }
-      const int b = max(s.bin, 0);
-      if (tid < WIDE_CTAS) {
-        *cluster.map_shared_rank(&s.bin, tid) = b;
-        *cluster.map_shared_rank(&s.members, tid) = t.count[b] - (b ? t.count[b - 1] : 0u);
-      }
-      if (tid == 0) {
-        s.base_count = base_count + (b ? t.count[b - 1] : 0u);
-        s.base_mass = base_mass + (b ? t.mass[b - 1] : 0.0);
-      }
     }
-    cluster.sync();
+    const int b = max(s.bin, 0);
+    if (tid < WIDE_CTAS) {
+      *cluster.map_shared_rank(&s.bin, tid) = b;
+      *cluster.map_shared_rank(&s.members, tid) = t.count[b] - (b ? t.count[b - 1] : 0u);
+    }
+    if (tid == 0) {
+      s.base_count = base_count + (b ? t.count[b - 1] : 0u);
+      s.base_mass = base_mass + (b ? t.mass[b - 1] : 0.0);
+    }
   }
+  cluster.sync();
+}
 
-  // The place in the row's order: by count the token of rank `rank_target` (from 1), by weight the first one up to which more than
-  // `target` stands (target: the first CTA's). Leaves comp in s.cut of every CTA, the weight up to and with it in s.cut_mass of the first.
-  __device__ void search(bool by_count, uint32_t rank_target, double target) {
-    find_bin(s.first, by_count, rank_target, target, 0, 0.0);
-    const int bin = s.bin;
-    uint32_t members = s.members;
-    range_lo = 0; range_hi = ~0ull;
-    const auto member = [&](float x, uint64_t c) { return bin_of(x) == bin && c >= range_lo && c <= range_hi; };
-    if (members > WIDE_LIST) {  // bins within the bin, until the place's has few enough
-      uint64_t top = 0, low = ~0ull;
-      each([&](float x, uint64_t c) { if (bin_of(x) == bin) { top = max(top, c); low = min(low, c); } });
-      extremes(top, low);
-      range_lo = low; range_hi = top;
-      while (members > WIDE_LIST) {
-        const int bits = 64 - __clzll(range_hi - range_lo);
-        const int shift = max(0, bits - 11);
-        clear();
-        each([&](float x, uint64_t c) { if (member(x, c)) add(static_cast<int>((range_hi - c) >> shift), weight_of(x, m, inv_t)); });
-        tabulate(&WideShared::finer);
-        find_bin(s.finer, by_count, rank_target, target, s.base_count, s.base_mass);
-        members = s.members;
-        range_hi -= static_cast<uint64_t>(s.bin) << shift;
-        const uint64_t wide = (1ull << shift) - 1;
-        range_lo = range_hi - range_lo > wide ? range_hi - wide : range_lo;
-        cluster.sync();  // s.bin and s.members are read before the next find
-      }
-    }
-    if (rank == 0 && tid == 0) s.listed = 0;
+// The place in the row's order: by count the token of rank `rank_target` (from 1), by weight the first one up to which more than
+// `target` stands (target: the first CTA's). Leaves comp in s.cut of every CTA, the weight up to and with it in s.cut_mass of the first.
+template <typename T>
+__device__ __noinline__ void wide_search(WidePart<T> part, WideScale c, double power, bool by_count, uint32_t rank_target, double target) {
+  cg::cluster_group cluster = cg::this_cluster();
+  WideShared& s = part.s;
+  const int tid = threadIdx.x;
+  const bool first = cluster_rank() == 0;
+  wide_find(s, false, by_count, rank_target, target, 0, 0.0);
+  const int bin = s.bin;
+  float hi = c.m - bin / c.scale, lo = c.m - (bin + 1) / c.scale;
+  uint64_t range_lo = 0, range_hi = ~0ull;  // of the members
+  uint32_t* listed = cluster.map_shared_rank(&s.listed, 0);
+  for (;;) {
+    if (first && tid == 0) s.listed = 0;
     cluster.sync();  // (also: the bins have been read, the list takes their place)
-    uint32_t* listed = cluster.map_shared_rank(&s.listed, 0);
     uint64_t* item = cluster.map_shared_rank(s.list.item, 0);
-    each([&](float x, uint64_t c) { if (member(x, c)) { const uint32_t at = atomicAdd(listed, 1u); if (at < WIDE_LIST) item[at] = c; } });
+    part.each([&](float x, int i) {
+      if (x == -INFINITY || c.bin(x) != bin) return;
+      const uint64_t comp = comp_of(x, i);
+      if (comp < range_lo || comp > range_hi) return;
+      const uint32_t to = atomicAdd(listed, 1u);
+      if (to < LIST) item[to] = comp;
+    });
     cluster.sync();
-    if (rank == 0) {
-      const int n = min(static_cast<int>(s.listed), WIDE_LIST);
-      int size = 2;
-      while (size < n) size <<= 1;
-      for (int i = n + tid; i < size; i += WIDE_THREADS) s.list.item[i] = 0;
-      sort_down<WIDE_THREADS>(s.list.item, size);
-      constexpr int PER = WIDE_LIST / WIDE_THREADS;
-      double v[PER];
-      for (int j = 0; j < PER; ++j) {
-        const int i = tid * PER + j;
-        v[j] = (i < n ? weight_of(comp_value(s.list.item[i]), m, inv_t) : 0.0) + (j ? v[j - 1] : 0.0);
-      }
-      uint32_t none;
-      const double before = s.base_mass + scan_before(v[PER - 1], 0, &none);
-      for (int j = 0; j < PER; ++j) s.list.mass[tid * PER + j] = before + v[j];
-      if (tid == 0) s.bin = -1;
-      __syncthreads();
-      if (by_count) {
-        if (tid == 0) s.bin = min(n - 1, static_cast<int>(rank_target - 1 - s.base_count));
-      } else {
-        for (int i = tid; i < n; i += WIDE_THREADS)
-          if (s.list.mass[i] > target && !(i > 0 && s.list.mass[i - 1] > target)) s.bin = i;
-        __syncthreads();
-        if (s.bin < 0) {  // as above: the last one that adds anything
-          __syncthreads();
-          for (int i = tid; i < n; i += WIDE_THREADS)
-            if (s.list.mass[i] == s.list.mass[n - 1] && s.list.mass[i] > (i > 0 ? s.list.mass[i - 1] : s.base_mass)) s.bin = i;
-        }
-      }
-      __syncthreads();
-      const int at = max(0, s.bin);
-      if (tid < WIDE_CTAS) *cluster.map_shared_rank(&s.cut, tid) = s.list.item[at];
-      if (tid == 0) s.cut_mass = s.list.mass[at];
+    uint32_t members = *listed;
+    if (members <= LIST) break;
+    // bins within the bin, until the place's has few enough
+    uint64_t top = 0, low = ~0ull;
+    part.each([&](float x, int i) {
+      if (x == -INFINITY || c.bin(x) != bin) return;
+      top = max(top, comp_of(x, i)); low = min(low, comp_of(x, i));
+    });
+    wide_extremes(s, &top, &low);
+    range_lo = low; range_hi = top;
+    while (members > LIST) {
+      const int bits = 64 - __clzll(range_hi - range_lo), shift = max(0, bits - 11);
+      wide_tally(part, c, power, true, [&](float x, int i) {
+        const uint64_t comp = comp_of(x, i);
+        return c.bin(x) == bin && comp >= range_lo && comp <= range_hi ? static_cast<int>((range_hi - comp) >> shift) : -1;
+      });
+      wide_tabulate(s, true, part.held);
+      wide_find(s, true, by_count, rank_target, target, s.base_count, s.base_mass);
+      members = s.members;
+      range_hi -= static_cast<uint64_t>(s.bin) << shift;
+      const uint64_t wide = (1ull << shift) - 1;
+      range_lo = range_hi - range_lo > wide ? range_hi - wide : range_lo;
+      cluster.sync();  // s.bin and s.members are read before the next find
     }
-    cluster.sync();
+    hi = comp_value(range_hi); lo = comp_value(range_lo);
   }
-};
+  if (first) {
+    const int n = min(static_cast<int>(s.listed), LIST);
+    order_list<WIDE_THREADS>(s.list, n, hi, lo);
+    constexpr int PER = LIST / WIDE_THREADS, NONE = 1 << 30;
+    double v[PER];
+    bool adds[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int i = tid * PER + j;
+      const double w = i < n ? weight_of(comp_value(s.list.item[i]), c.m, c.inv_t) : 0.0;
+      adds[j] = w > 0.0;
+      v[j] = w + (j ? v[j - 1] : 0.0);
+    }
+    uint32_t none;
+    const double before = s.base_mass + wide_before(s, v[PER - 1], 0, &none);
+    if (tid == 0) { s.place = NONE; s.bin = 0; }
+    __syncthreads();
+    int last = -1;
+#pragma unroll
+    for (int j = PER - 1; j >= 0; --j) {
+      const int i = tid * PER + j;
+      if (by_count ? i + 1 + s.base_count == rank_target : before + v[j] > target && i < n) atomicMin(&s.place, i);
+      if (adds[j] && last < 0) last = i;
+    }
+    if (last >= 0) atomicMax(&s.bin, last);  // where the weight ends, should all of it stand before the target by a rounding
+    __syncthreads();
+    const int at = s.place < n ? s.place : by_count ? n - 1 : s.bin;
+    __syncthreads();
+    if (tid < WIDE_CTAS) *cluster.map_shared_rank(&s.cut, tid) = s.list.item[at];
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (tid * PER + j == at) s.cut_mass = before + v[j];
+  }
+  cluster.sync();
+}
 
 template <typename T>
-__device__ void sample_wide_row(const SampleArgs& a, int at, WideShared& s) {
-  const int tid = threadIdx.x;
-  const int per = (a.V + WIDE_CTAS * 8 - 1) / (WIDE_CTAS * 8) * 8;
-  WideRow<T> r(s, static_cast<const T*>(a.logits) + at * a.stride, a.V, per);
+__device__ __forceinline__ void sample_wide_row(const SampleArgs& a, const SampleWork& work, int at, WideShared& s) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int tid = threadIdx.x, rank = cluster_rank(), per = (a.V + WIDE_CTAS - 1) / WIDE_CTAS;
+  const WidePart<T> part{s, static_cast<const T*>(a.logits) + at * a.stride, min(a.V, rank * per), min(a.V, (rank + 1) * per), per <= WIDE_HELD};
   const float temperature = a.temperature[at];
   const int k = a.top_k[at];
-  const double p = a.top_p[at], least = a.min_p[at], u = a.u[at];
-  if (tid == 0) {
-    int found = 0;
-    for (int j = 0; j < a.n_exclude; ++j) {
-      const int id = a.exclude[static_cast<long long>(at) * a.n_exclude + j];
-      if (id >= r.begin && id < r.end) s.banned[found++] = id;
-    }
-    s.n_banned = found;
+  const double p = a.top_p[at], least = a.min_p[at], u = a.u[at], power = work.powers[tid & 31];
+  const SamplePlan& plan = work.plan[at];
+  if (tid == 0) s.n_banned = 0;
+  if (part.held) {
+#pragma unroll 8
+    for (int i = part.begin + tid; i < part.end; i += WIDE_THREADS) s.held[i - part.begin] = logit_value(part.row[i]);
   }
-  r.cluster.sync();  // (also: every CTA of the cluster is there, before anything is written into it)
-  uint64_t top = 0, low = ~0ull;
-  r.each([&](float, uint64_t c) { top = max(top, c); low = min(low, c); });
-  r.extremes(top, low);
-  const bool first = r.rank == 0 && tid == 0;
+  __syncthreads();
+  for (int j = tid; j < a.n_exclude; j += WIDE_THREADS) {
+    const int id = a.exclude[static_cast<long long>(at) * a.n_exclude + j];
+    if (id < part.begin || id >= part.end) continue;
+    if (part.held) s.held[id - part.begin] = -INFINITY;
+    else s.banned[atomicAdd(&s.n_banned, 1)] = id;
+  }
+  cluster.sync();  // (also: every CTA of the cluster is there, before anything is written into it)
+  uint64_t top = plan.top, low = comp_of(plan.low, 0);
+  if (top == 0) {
+    float hi = -INFINITY, lo = INFINITY;
+    int id = 0;
+    part.each([&](float x, int i) {
+      if (x > hi) { hi = x; id = i; }  // (the first of a thread's)
+      if (x != -INFINITY) lo = fminf(lo, x);
+    });
+    top = comp_of(hi, id);
+    low = top ? comp_of(lo, 0) : ~0ull;
+    wide_extremes(s, &top, &low);
+  }
+  const bool first = rank == 0 && tid == 0;
   if (top == 0 || !(temperature > 0.f)) {
     if (first) a.out[at] = top ? comp_id(top) : -1;
-    return;  // (nothing reaches into another CTA behind `extremes`)
+    return;  // (nothing reaches into another CTA behind `wide_extremes`)
   }
-  r.m = comp_value(top);
-  r.inv_t = 1.0 / static_cast<double>(temperature);
-  const float range = fminf(fminf(WIDE_RANGE * temperature, r.m - comp_value(low)), 1e38f);
-  r.scale = range > 0.f ? WIDE_BINS / range : 0.f;
-  if (!(r.scale < 1e38f)) r.scale = 1e38f;
-  r.clear();
-  r.each([&](float x, uint64_t c) { r.add(r.bin_of(x), weight_of(x, r.m, r.inv_t)); });
-  r.tabulate(&WideShared::first);
+  const bool cut_k = k > 0 && k < a.V;
+  WideScale c;
+  c.m = comp_value(top);
+  c.inv_t = 1.0 / static_cast<double>(temperature);
+  c.step = c.inv_t * STEPS;
+  c.floor = fmaxf(c.m - WIDE_RANGE * temperature, -FLT_MAX);
+  const float range = fminf(fminf(WIDE_RANGE * temperature, c.m - comp_value(low)), 1e38f);
+  c.scale = range > 0.f ? fminf(WIDE_BINS / range, 1e38f) : 0.f;
+  wide_tally(part, c, power, cut_k, [&](float x, int) { return c.bin(x); });
+  wide_tabulate(s, false, part.held);
 
   uint64_t cut = 0;
   double total = s.first.mass[WIDE_BINS - 1];  // (the first CTA's numbers; nobody else uses them)
-  if (k > 0 && k < a.V) {
-    r.search(true, static_cast<uint32_t>(k), 0.0);
+  if (cut_k) {
+    wide_search(part, c, power, true, static_cast<uint32_t>(k), 0.0);
     cut = s.cut;
     total = s.cut_mass;
   }
   if (p < 1.0) {
-    r.search(false, 0, p * total);
+    wide_search(part, c, power, false, 0, p * total);
     if (s.cut >= cut) { cut = s.cut; total = s.cut_mass; }
   }
   if (least > 0.0) {  // the weight of what min-p leaves, and its last token
     double mass = 0.0;
     uint64_t last = ~0ull, none = 0;
-    r.each([&](float x, uint64_t c) {
-      if (c < cut) return;
-      const double w = weight_of(x, r.m, r.inv_t);
-      if (w >= least || c == top) { mass += w; last = min(last, c); }
+    part.each([&](float x, int i) {
+      const uint64_t comp = comp_of(x, i);
+      if (comp == 0 || comp < cut) return;
+      const double w = weight_of(x, c.m, c.inv_t);
+      if (w >= least || comp == top) { mass += w; last = min(last, comp); }
     });
-    total = r.sum(mass);
-    r.extremes(none, last);
+    total = wide_sum(s, mass);
+    wide_extremes(s, &none, &last);
     cut = last;
-    r.cluster.sync();
+    cluster.sync();
   }
-  r.search(false, 0, u * total);
+  wide_search(part, c, power, false, 0, u * total);
   if (first) a.out[at] = comp_id(s.cut > cut ? s.cut : cut);
 }
 
 // The rows that the stream left to this kernel: a cluster takes one after the other.
 template <typename T>
-__global__ void __cluster_dims__(WIDE_CTAS, 1, 1) __launch_bounds__(WIDE_THREADS)
-sample_wide_kernel(SampleArgs a, SampleWork w) {
+__global__ void __launch_bounds__(WIDE_THREADS) sample_wide_kernel(SampleArgs a, SampleWork w) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   WideShared& s = *reinterpret_cast<WideShared*>(smem_raw);
   pdl_wait();
   pdl_launch();
   const int rows = *w.left;
+  if (static_cast<int>(blockIdx.x / WIDE_CTAS) >= rows) return;
   for (int i = blockIdx.x / WIDE_CTAS; i < rows; i += gridDim.x / WIDE_CTAS) {
-    sample_wide_row<T>(a, w.left_rows[i], s);
+    sample_wide_row<T>(a, w, w.left_rows[i], s);
     cg::this_cluster().sync();  // everyone has read what the next row writes over
   }
 }
@@ -458,9 +640,8 @@ sample_wide_kernel(SampleArgs a, SampleWork w) {
 //
 // Sums are added up in an order that goes by V alone: the weights of a lane's tokens of a task, the lanes of a warp, the tasks of a row.
 constexpr int PLAN_THREADS = 512, PLAN_PER = 32, PLAN_SAMPLE = PLAN_THREADS * PLAN_PER, PLAN_BLOCK = 256, PLAN_BINS = 1024;
-constexpr int STREAM_THREADS = 512, STREAM_WARPS = STREAM_THREADS / 32;
-constexpr int TASK = 512;           // tokens that a warp takes at a time
-constexpr int LIST = 2048;          // most tokens of a list
+constexpr int STREAM_THREADS = 256, STREAM_WARPS = STREAM_THREADS / 32;
+constexpr int TASK = 1024;          // tokens that a warp takes at a time
 constexpr int LIST_PER = LIST / STREAM_THREADS;
 constexpr int LIST_K = 1024;        // top-k up to which a list is expected to hold the k tokens
 
@@ -506,79 +687,21 @@ __device__ __forceinline__ double sum_before(double v, double* warp_sum) {
   return before + (lane ? mine : 0.0);
 }
 
-constexpr int LIST_BINS = 1024;
-constexpr int LIST_BIN_MOST = 96;  // tokens of a bin that are compared each with each
-
 struct ListShared {
-  uint64_t item[LIST], other[LIST];
-  uint32_t bins[LIST_BINS];
-  uint32_t warp_count[STREAM_WARPS];
+  Order list;
   double warp_sum[STREAM_WARPS];
   double total, cut;
   int place, last;
 };
-
-// Puts s.item[0 .. c) into descending order: bins by value, in a bin by comparing each with each. `hi` and `lo`: about where the values lie.
-// Rows of many equal values are sorted by exchanges instead. (1,400 tokens by exchanges alone: TODO us of a row's 22.)
-__device__ void order_list(ListShared& s, int c, float hi, float lo) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  static_assert(LIST_BINS == 2 * STREAM_THREADS, "two bins per thread");
-  const float scale = hi > lo ? fminf(LIST_BINS / (hi - lo), 1e30f) : 0.f;
-  s.bins[2 * tid] = s.bins[2 * tid + 1] = 0;
-  __syncthreads();
-  uint64_t mine[LIST_PER];
-  uint32_t bin[LIST_PER], at[LIST_PER];
-#pragma unroll
-  for (int j = 0; j < LIST_PER; ++j) {
-    const int i = tid + j * STREAM_THREADS;
-    if (i < c) {
-      mine[j] = s.item[i];
-      bin[j] = min(LIST_BINS - 1, max(0, static_cast<int>((hi - comp_value(mine[j])) * scale)));
-      at[j] = atomicAdd(&s.bins[bin[j]], 1u);
-    }
-  }
-  __syncthreads();
-  const uint32_t c0 = s.bins[2 * tid], c1 = s.bins[2 * tid + 1];
-  uint32_t up = c0 + c1;
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t v = __shfl_up_sync(0xffffffffu, up, o);
-    if (lane >= o) up += v;
-  }
-  if (lane == 31) s.warp_count[warp] = up;
-  if (__syncthreads_or(max(c0, c1) > LIST_BIN_MOST)) {
-    int size = 2;
-    while (size < c) size <<= 1;
-    for (int i = c + tid; i < size; i += STREAM_THREADS) s.item[i] = 0;
-    sort_down<STREAM_THREADS>(s.item, size);
-    return;
-  }
-  for (int w = 0; w < warp; ++w) up += s.warp_count[w];
-  s.bins[2 * tid] = up - c1 - c0;  // where a bin starts
-  s.bins[2 * tid + 1] = up - c1;
-  __syncthreads();
-#pragma unroll
-  for (int j = 0; j < LIST_PER; ++j)
-    if (tid + j * STREAM_THREADS < c) s.other[s.bins[bin[j]] + at[j]] = mine[j];
-  __syncthreads();
-#pragma unroll
-  for (int j = 0; j < LIST_PER; ++j)
-    if (tid + j * STREAM_THREADS < c) {
-      const uint32_t from = s.bins[bin[j]], to = bin[j] + 1 < LIST_BINS ? s.bins[bin[j] + 1] : static_cast<uint32_t>(c);
-      uint32_t above = from;
-      for (uint32_t i = from; i < to; ++i) above += s.other[i] > mine[j];
-      s.item[above] = mine[j];
-    }
-  __syncthreads();
-}
 
 // The pick of a row from its `c` largest tokens in s.item (unsorted) and the weight `tail` of all others, relative to `ref`; all: there
 // are no others of any weight. -2 where the tokens do not decide it. All threads of a CTA of STREAM_THREADS.
 __device__ int pick_from_list(ListShared& s, int c, const RowAsk& r, double tail, float ref, bool all, float hi, float lo) {
   const int tid = threadIdx.x;
   if (c == 0) return ref == -INFINITY && all ? -1 : -2;
-  order_list(s, c, hi, lo);
-  if (r.greedy) return comp_id(s.item[0]);
-  const float m = comp_value(s.item[0]);
+  order_list<STREAM_THREADS>(s.list, c, hi, lo);
+  if (r.greedy) return comp_id(s.list.item[0]);
+  const float m = comp_value(s.list.item[0]);
   // what weighs nothing beside `ref` weighs nothing beside m as well, unless m lies far below (an excluded token is the largest)
   if ((static_cast<double>(ref) - static_cast<double>(m)) * r.inv_t > WIDE_RANGE / 4) return -2;
   if (tail > 0.0) tail *= ref == m ? 1.0 : exp((static_cast<double>(ref) - static_cast<double>(m)) * r.inv_t);
@@ -593,7 +716,7 @@ __device__ int pick_from_list(ListShared& s, int c, const RowAsk& r, double tail
 #pragma unroll
   for (int j = 0; j < LIST_PER; ++j) {
     const int i = tid * LIST_PER + j;
-    const double w = i < nk ? weight_of(comp_value(s.item[i]), m, r.inv_t) : 0.0;
+    const double w = i < nk ? weight_of(comp_value(s.list.item[i]), m, r.inv_t) : 0.0;
     positive += w > 0.0;
     enough += w >= r.least && i < nk;
     cum[j] = w + (j ? cum[j - 1] : 0.0);
@@ -624,10 +747,14 @@ __device__ int pick_from_list(ListShared& s, int c, const RowAsk& r, double tail
     __syncthreads();
     return s.place;
   };
+  double rest = 0.0;  // where the nucleus ends in the tail, its weight is between p * sum and one token's more
   if (r.p < 1.0) {
     const int at = find(r.p * sum);
     if (at != OPEN) limit = at + 1;
-    else if (!closed) return -2;
+    else if (!closed) {
+      rest = weight_of(comp_value(s.list.item[c - 1]), m, r.inv_t);
+      if (!(rest > 0.0)) return -2;
+    }
   }
   if (r.least > 0.0) {
     if (enough < nk || closed) limit = min(limit, enough);
@@ -642,11 +769,14 @@ __device__ int pick_from_list(ListShared& s, int c, const RowAsk& r, double tail
       if (i == j) s.cut = cum[i];
     __syncthreads();
     total = s.cut;
+  } else if (rest > 0.0) {
+    total = r.p * sum;
   }
   const int at = find(r.u * total);
-  if (at < limit && at != OPEN) return comp_id(s.item[at]);
+  if (limit == OPEN && rest > 0.0 && at != find(r.u * (total + rest) * (1.0 + 0x1p-40))) return -2;
+  if (at < limit && at != OPEN) return comp_id(s.list.item[at]);
   if (limit == OPEN) return -2;
-  return comp_id(s.item[max(0, min(limit, positive) - 1)]);
+  return comp_id(s.list.item[max(0, min(limit, positive) - 1)]);
 }
 
 template <typename T>
@@ -661,6 +791,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) sample_plan_kernel(SampleArgs a,
   const T* row = static_cast<const T*>(a.logits) + at * a.stride;
   const RowAsk ask(a, at);
   if (at == 0 && tid == 0) *w.left = 0;
+  if (at == 0 && tid < 32) w.powers[tid] = exp2(tid / 32.0);
   for (int b = tid; b < PLAN_BINS; b += PLAN_THREADS) bins[b] = 0;
   if (tid == 0) found = -1;
   float x[PLAN_PER];
@@ -714,6 +845,10 @@ __global__ void __launch_bounds__(PLAN_THREADS) sample_plan_kernel(SampleArgs a,
     plan.reach = number ? reach : -FLT_MAX;
     plan.least = number ? least : -FLT_MAX;
     plan.ref = top;
+    plan.low = low;
+    plan.top = 0;
+    plan.step = ask.inv_t * STEPS;
+    plan.with_tail = !ask.greedy && !ask.cut_k && plan.reach > plan.least;
     plan.listed = 0;
     plan.done = 0;
     plan.skip = (ask.cut_k && ask.k > LIST_K && reach > least) || t > 1e30f;  // (at such a temperature even a token of `least` weighs something)
@@ -721,30 +856,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) sample_plan_kernel(SampleArgs a,
   }
 }
 
-// 2^(s / 32) for s in [-4000, 0] and a little more: the fraction's 32 values are held by a warp's lanes, and what is left of s, at most half either
-// way, goes through a polynomial: with f ln 2 / 32 = g, at most 0.011, the powers of g over their factorials up to the fifth (the sixth is one part
-// in 2^49). All lanes of the warp take part. Ten 64-bit operations for each token, the multiplication into the caller's sum included.
-struct ExpLanes {
-  int lo, hi;
-  __device__ __forceinline__ ExpLanes() {
-    const double t = exp2((threadIdx.x & 31) / 32.0);
-    lo = __double2loint(t);
-    hi = __double2hiint(t);
-  }
-  static constexpr double G = 0.69314718055994531 / 32;
-  __device__ __forceinline__ double add(double sum, double s) const {
-    const double z = s + 0x1.8p52;  // the nearest whole number stands in the low word
-    const int n = __double2loint(z);
-    const double f = s - (z - 0x1.8p52);
-    double q = fma(f, G * G * G * G * G / 120, G * G * G * G / 24);
-    q = fma(f, q, G * G * G / 6);
-    q = fma(f, q, G * G / 2);
-    q = fma(f, q, G);
-    const double t = __hiloint2double(__shfl_sync(0xffffffffu, hi, n) + ((n & ~31) << 15), __shfl_sync(0xffffffffu, lo, n));
-    return fma(t, fma(f, q, 1.0), sum);
-  }
-};
-// The sixteen logits of a lane in a task, from `row` on: piece i of 16 bytes holds tokens first + i * 32 * VE ..
+// The logits of a lane in a task, from `row` on: piece i of 16 bytes holds tokens first + i * 32 * VE ..
 template <typename T>
 struct TaskLogits {
   static constexpr int VE = 16 / sizeof(T), PIECES = TASK / (32 * VE);
@@ -786,19 +898,20 @@ struct TaskLogits {
 
 // CTA x of a row takes `tasks_per_warp` tasks for each warp, from task x * STREAM_WARPS * tasks_per_warp on.
 template <typename T>
-__global__ void __launch_bounds__(STREAM_THREADS, 2) sample_stream_kernel(SampleArgs a, SampleWork w, int tasks, int tasks_per_warp) {
+__global__ void __launch_bounds__(STREAM_THREADS, 3) sample_stream_kernel(SampleArgs a, SampleWork w, int tasks, int tasks_per_warp) {
   using Task = TaskLogits<T>;
   __shared__ ListShared s;
   __shared__ int banned[SAMPLE_MAX_EXCLUDE];
   __shared__ int n_banned;
   const int at = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.V;
-  const ExpLanes exps;
   if (tid == 0) n_banned = 0;
   __syncthreads();
   pdl_wait();
   pdl_launch();
-  const RowAsk ask(a, at);
   SamplePlan& plan = w.plan[at];
+  const ExpLanes exps(w.powers[lane]);
+  const double step = plan.step, from = plan.ref;
+  const bool with_tail = plan.with_tail;
   if (plan.skip) {
     if (blockIdx.x == 0 && tid == 0) w.left_rows[atomicAdd(w.left, 1)] = at;
     return;
@@ -813,8 +926,6 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) sample_stream_kernel(Sample
   }
   if (a.n_exclude) __syncthreads();
   const int bans = n_banned;
-  const bool with_tail = !ask.greedy && !ask.cut_k && reach > least;
-  const double step = ask.inv_t * 46.166241308446828, start = -static_cast<double>(ref) * step;  // 32 / ln 2
   uint64_t* list = w.list + static_cast<size_t>(at) * LIST;
 
   for (int i = 0; i < tasks_per_warp; ++i) {
@@ -826,15 +937,17 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) sample_stream_kernel(Sample
     if (bans) x.strike(first, banned, bans);
     uint32_t hits = 0;
     if (with_tail) {
-      double tail = 0.0;
+      double tail = 0.0, odd = 0.0;
 #pragma unroll
       for (int e = 0; e < TASK / 32; ++e) {
         const float v = x.value(e);
         const bool hit = v >= reach;  // (a NaN is in neither the list nor the tail)
         hits |= hit ? 1u << e : 0u;
         // tokens that are not the tail's add e^-80 each: nothing
-        tail = exps.add(tail, fma(static_cast<double>(hit ? least : fmaxf(v, least)), step, start));
+        double& sum = e & 1 ? odd : tail;
+        sum = exps.add(sum, (static_cast<double>(hit ? least : fmaxf(v, least)) - from) * step);
       }
+      tail += odd;
       for (int o = 16; o; o >>= 1) tail += __shfl_xor_sync(0xffffffffu, tail, o);
       if (lane == 0) w.tail[static_cast<size_t>(at) * tasks + task] = tail;
     } else {
@@ -873,13 +986,17 @@ __global__ void __launch_bounds__(STREAM_THREADS, 2) sample_stream_kernel(Sample
       __syncthreads();
       tail = s.total;
     }
-    for (int i = tid; i < static_cast<int>(listed); i += STREAM_THREADS) s.item[i] = __ldcg(list + i);
+    for (int i = tid; i < static_cast<int>(listed); i += STREAM_THREADS) s.list.item[i] = __ldcg(list + i);
     __syncthreads();
-    pick = pick_from_list(s, static_cast<int>(listed), ask, tail, ref, reach <= least, ref, reach);
+    pick = pick_from_list(s, static_cast<int>(listed), RowAsk(a, at), tail, ref, reach <= least, ref, reach);
   }
   if (tid == 0) {
-    if (pick == -2) w.left_rows[atomicAdd(w.left, 1)] = at;
-    else a.out[at] = pick;
+    if (pick == -2) {
+      if (listed > 0 && listed <= LIST) plan.top = s.list.item[0];
+      w.left_rows[atomicAdd(w.left, 1)] = at;
+    } else {
+      a.out[at] = pick;
+    }
   }
 }
 
@@ -900,7 +1017,7 @@ __global__ void __launch_bounds__(STREAM_THREADS) sample_short_kernel(SampleArgs
     bool out = c == 0;
     for (int j = 0; j < a.n_exclude; ++j) out |= a.exclude[static_cast<long long>(at) * a.n_exclude + j] == i;
     if (out) continue;
-    s.item[atomicAdd(&listed, 1)] = c;
+    s.list.item[atomicAdd(&listed, 1)] = c;
     atomicMax(&top, static_cast<uint32_t>(c >> 32));
     atomicMin(&low, static_cast<uint32_t>(c >> 32));
   }
@@ -924,6 +1041,7 @@ static size_t sample_work(int n, int V, void* base, SampleWork* w) {
   w->plan = reinterpret_cast<SamplePlan*>(take(static_cast<size_t>(n) * sizeof(SamplePlan)));
   w->list = reinterpret_cast<uint64_t*>(take(static_cast<size_t>(n) * LIST * 8));
   w->tail = reinterpret_cast<double*>(take(static_cast<size_t>(n) * task_count(V) * 8));
+  w->powers = reinterpret_cast<double*>(take(32 * 8));
   return at;
 }
 
@@ -936,6 +1054,7 @@ static int launch_sample(const SampleArgs& a, void* work, cudaStream_t st) {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= MAX_DEVICES) return -3;
   if (!sms[dev]) {
     if (cudaFuncSetAttribute(sample_wide_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(WideShared)) != cudaSuccess) return -3;
+    if (cudaFuncSetAttribute(sample_wide_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return -3;
     if (cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return -3;
   }
   SampleWork w;
@@ -948,7 +1067,7 @@ static int launch_sample(const SampleArgs& a, void* work, cudaStream_t st) {
   const int clusters = a.n < sms[dev] / WIDE_CTAS ? a.n : sms[dev] / WIDE_CTAS;
   if (launch_pdl(sample_plan_kernel<T>, dim3(a.n), dim3(PLAN_THREADS), 0, st, a, w) != cudaSuccess) return -4;
   if (launch_pdl(sample_stream_kernel<T>, dim3(ctas, a.n), dim3(STREAM_THREADS), 0, st, a, w, tasks, per) != cudaSuccess) return -4;
-  return launch_pdl(sample_wide_kernel<T>, dim3(clusters * WIDE_CTAS), dim3(WIDE_THREADS), sizeof(WideShared), st, a, w) == cudaSuccess ? 0 : -4;
+  return launch_clusters(WIDE_CTAS, sample_wide_kernel<T>, dim3(clusters * WIDE_CTAS), dim3(WIDE_THREADS), sizeof(WideShared), st, a, w) == cudaSuccess ? 0 : -4;
 }
 
 }  // namespace b200
@@ -957,6 +1076,7 @@ using namespace b200;
 
 extern "C" int b200_sample_max_exclude() { return SAMPLE_MAX_EXCLUDE; }
 extern "C" int b200_sample_max_rows() { return 65535; }
+extern "C" int b200_sample_max_vocab() { return SAMPLE_MAX_VOCAB; }
 
 extern "C" long long b200_sample_work_bytes(int n, int V) {
   SampleWork w;
@@ -967,7 +1087,7 @@ extern "C" int b200_sample(const void* logits, int type, long long stride, int n
                            const float* top_p, const float* min_p, const float* u, const int* exclude, int n_exclude, int64_t* out,
                            void* work, cudaStream_t st) {
   if (n <= 0) return 0;
-  if (V <= 0 || n_exclude < 0 || n_exclude > SAMPLE_MAX_EXCLUDE || V > (1 << 30) || n > b200_sample_max_rows()) return -7;
+  if (V <= 0 || n_exclude < 0 || n_exclude > SAMPLE_MAX_EXCLUDE || V > SAMPLE_MAX_VOCAB || n > b200_sample_max_rows()) return -7;
   const SampleArgs a{logits, stride, n, V, temperature, top_k, top_p, min_p, u, exclude, n_exclude, out};
   switch (type) {
     case LOGIT_F32: return launch_sample<float>(a, work, st);

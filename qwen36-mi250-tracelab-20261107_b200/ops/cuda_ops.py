@@ -1011,6 +1011,7 @@ def _kv8_attention(qkv, positions, seq_of_row, block_tables, layer, q_norm, k_no
 
 # --------------------------------------------------------------------------- sampling
 SAMPLE_ROWS = 4096  # of one launch
+SAMPLE_VOCAB = 1 << 22
 
 
 @functools.cache
@@ -1033,8 +1034,8 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor,
     kind = LOGIT_TYPES.get(logits.dtype)
     if not logits.is_cuda:
         raise ValueError(f"sample: the logits are on {logits.device}: torch_ops has the operator for them")
-    if len(shape) != 2 or kind is None or shape[1] < 1 or shape[1] > 1 << 30:
-        raise ValueError(f"sample: logits {tuple(shape)} {logits.dtype} are not fp32, bf16 or fp16 [rows, vocabulary]")
+    if len(shape) != 2 or kind is None or not 1 <= shape[1] <= SAMPLE_VOCAB:
+        raise ValueError(f"sample: logits {tuple(shape)} {logits.dtype} are not fp32, bf16 or fp16 [rows, 1 to {SAMPLE_VOCAB} tokens]")
     n, V = shape
     dev = logits.device
     for name, t, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
