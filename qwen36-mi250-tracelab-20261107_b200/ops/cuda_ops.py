@@ -23,6 +23,7 @@ from ..obs import buildlog
 from . import torch_ops
 from .build import lib_path
 from .kv8 import Kv8Layer, check_layer
+from .lora import LoraWeights, check_weights
 from .spans import span_tables
 
 _lib = None
@@ -94,6 +95,7 @@ class _Sig:
     b200_kv8_prefill_positions = [I]
     b200_kv8_prefill_cut = [I]
     b200_kv8_prefill = [P, P, P, P, P, P, I, I, I, I, I, L, P, I, I, I, I, I, I, P, P, P, P, P]
+    b200_lora_add = [P, L, P, P, P, P, P, P, I, I, I, I, I, I, I, P, P]
     b200_sample_max_exclude = []
     b200_sample_max_rows = []
     b200_sample_work_bytes = [I, I]
@@ -274,6 +276,41 @@ def linear(x: torch.Tensor, w: torch.Tensor, out_dtype: torch.dtype | None = Non
         None, None, _ptr(err_word(x.device)), split_k(N, K), is_packed(w), _stream(),
     )
     _check(rc, "gemm_dense")
+    return out
+
+
+def lora_linear(x: torch.Tensor, w: torch.Tensor, adapters: LoraWeights, rows: torch.Tensor, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``linear(x, w)`` with the low-rank adapter of each row's own request beside it (``ops/lora.py``): row ``t`` of ``x [T, K]`` uses adapter
+    ``rows[t]`` (int32 ``[T]``), none where that is negative. One rounding, to bf16 (default) or fp32. A row's bits depend on its own numbers and
+    adapter only, and are ``linear``'s for a row without one. An adapter number that is too large leaves the row without one, and is reported by
+    ``check_errors``. Only device tensors are touched, so the call can be captured in a CUDA graph."""
+    dev, f32 = x.device, out_dtype == torch.float32
+    if not x.is_cuda:
+        raise ValueError(f"lora_linear: the rows are on {dev}: torch_ops has the operator for them")
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1] or x.dtype != torch.bfloat16 or w.dtype != torch.bfloat16:
+        raise ValueError(f"lora_linear: rows {tuple(x.shape)} {x.dtype} and weights {tuple(w.shape)} {w.dtype} are not bf16 [T, K] and [N, K]")
+    if out_dtype not in (None, torch.bfloat16, torch.float32):
+        raise ValueError(f"lora_linear: {out_dtype} outputs, bf16 and fp32 are there")
+    (T, K), N = x.shape, w.shape[0]
+    if adapters.b.dim() != 3 or not (N - 128 * is_packed(w) < adapters.b.shape[1] <= N or adapters.b.shape[1] == N):
+        raise ValueError(f"lora_linear: adapters of {tuple(adapters.b.shape)} for {N} outputs")
+    n_own = adapters.b.shape[1]  # a packed weight has rows of zeros behind its own
+    L, R = check_weights(adapters, n_own, K, "lora_linear")
+    if adapters.a.dtype != torch.bfloat16:
+        raise ValueError(f"lora_linear: adapters of {adapters.a.dtype}, not bf16")
+    if rows.shape != (T,) or rows.dtype != torch.int32 or not rows.is_contiguous():
+        raise ValueError(f"lora_linear: adapter numbers {tuple(rows.shape)} {rows.dtype} are not a contiguous int32 [{T}]")
+    if w.device != dev or adapters.a.device != dev or rows.device != dev:
+        raise ValueError(f"lora_linear: rows on {dev}, weights on {w.device}, adapters on {adapters.a.device}, their numbers on {rows.device}")
+    if K % 8 or x.stride(1) != 1 or w.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
+        raise ValueError(f"lora_linear: rows of {K} numbers with strides {x.stride()} and weights with strides {w.stride()}: rows are whole 16-byte pieces")
+    out = torch.empty(T, N, dtype=torch.float32 if f32 else torch.bfloat16, device=dev)
+    if T == 0:
+        return out
+    base = linear(x, w, out_dtype=torch.float32)
+    _check(lib().b200_lora_add(
+        x.data_ptr(), x.stride(0), base.data_ptr(), adapters.a.data_ptr(), adapters.b.data_ptr(), adapters.scale.data_ptr(), rows.data_ptr(),
+        out.data_ptr(), f32, T, N, n_own, K, R, L, _err_ptr(dev), _raw_stream(dev)), "lora_add")
     return out
 
 

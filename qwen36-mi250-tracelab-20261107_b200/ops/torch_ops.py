@@ -18,6 +18,7 @@ import torch.nn.functional as F
 
 from ..config import GDN_CHUNK, PAGE_SIZE
 from .kv8 import Kv8Layer, check_layer, dequantise, quantise
+from .lora import LoraWeights, check_weights
 
 
 # --------------------------------------------------------------------------- norms
@@ -50,6 +51,16 @@ def linear(x: torch.Tensor, w: torch.Tensor, out_dtype: torch.dtype | None = Non
 
 
 # --------------------------------------------------------------------------- rope
+def lora_linear(x: torch.Tensor, w: torch.Tensor, adapters: LoraWeights, rows: torch.Tensor, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``x w^T`` and, for a row ``t`` with an adapter (``rows[t] >= 0``), ``scale (x a^T) b^T`` of it, rounded once."""
+    L, R = check_weights(adapters, w.shape[0], x.shape[1], "lora_linear")
+    y = x.float() @ w.float().t()
+    for i in rows[(rows >= 0) & (rows < L)].unique().tolist():
+        at = (rows == i).nonzero().view(-1)
+        y[at] += (x[at].float() @ adapters.a[i].float().t() * adapters.scale[i]) @ adapters.b[i].float().t()
+    return y.to(out_dtype or x.dtype)
+
+
 def rope_cos_sin(positions: torch.Tensor, rotary_dim: int, theta: float):
     """cos/sin ``[T, rotary_dim/2]`` in fp32 for integer positions."""
     inv = 1.0 / (
