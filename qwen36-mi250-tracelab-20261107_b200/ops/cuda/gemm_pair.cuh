@@ -47,9 +47,11 @@ __device__ __forceinline__ void group_sync(int id) { asm volatile("barrier.cta.s
 // EPI_BF16 (dense, or grouped with rows that are sorted already), EPI_F32 or EPI_ARGMAX (dense) or EPI_SILU_MUL (grouped, rows fetched by index,
 // tile-packed weights). In a SiLU tile a CTA's 128 accumulator rows are 64 gate rows and the 64 up rows
 // that go with them.
-template <int EPI, bool GROUPED, int PBT>
+// LORA: as in gemm_swapab_kernel.
+template <int EPI, bool GROUPED, int PBT, bool LORA = false>
 __global__ void __launch_bounds__(pair_threads(EPI), 1)
-gemm_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, GemmParams p) {
+gemm_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, GemmParams p,
+                 const __grid_constant__ LoraArg<LORA> lora) {
   constexpr bool SILU = EPI == EPI_SILU_MUL;
   constexpr int PAIR_ROWS = SILU ? BM : 2 * BM;  // output columns of a tile
   constexpr int CTA_ROWS = PAIR_ROWS / 2;
@@ -193,8 +195,8 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
           load_weights(smem + kb * STAGE_BYTES, dsmem_addr(smem_u32(&full[kb]), 0), nx, 0, kb);
         }
       }
-      pdl_wait();
-      if (!GROUPED) pdl_launch();
+      if (!LORA) pdl_wait();
+      if (!GROUPED && !LORA) pdl_launch();
       for (int tile = tile0; tile < total && live; tile += tstep) {
         int nx, expert, row0, nrows;
         tile_geom(tile, nx, expert, row0, nrows);
@@ -217,6 +219,22 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
               tma_load_2d_pair(st + PAIR_A_BYTES + b * (VAR_BOX * BK * 2), &tmX, bar, kb * BK, x0 + b * VAR_BOX);
           } else {
             tma_load_2d_pair(st + PAIR_A_BYTES, &tmX, bar, kb * BK, x0);
+          }
+        }
+        if constexpr (LORA) {
+          if (tile == tile0) { pdl_wait(); pdl_launch(); }
+          const int by = tile / tiles_n;
+          const LoraSteps steps(lora, by, 1);
+          for (int e0 = 0; e0 < steps.entries && live; e0 += steps.per_stage, ++it) {
+            const int s = it % STAGES, n = steps.of_stage(e0);
+            uint8_t* st = smem + s * STAGE_BYTES;
+            const uint32_t bar = dsmem_addr(smem_u32(&full[s]), 0);
+            if (!mbar_wait<true>(&empty[s], ((it / STAGES) & 1) ^ 1, p.err, ERR_WAIT_EMPTY, abort_flag)) { live = false; break; }
+            if (rank == 0) mbar_expect_tx(&full[s], n * (2 * BM + bt) * lora.width * 2);
+            for (int j = 0; j < n; ++j) {
+              tma_load_3d_pair(st + j * BM * lora.width * 2, &lora.b, bar, lora.column(e0 + j), (2 * nx + static_cast<int>(rank)) * BM, lora.adapter(by, e0 + j));
+              tma_load_2d_pair(st + PAIR_A_BYTES + j * (bt / 2) * lora.width * 2, &lora.h, bar, 0, lora.row(by, e0 + j) + static_cast<int>(rank) * half);
+            }
           }
         }
       }
@@ -245,6 +263,21 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
             umma_bf16_pair(tmem, umma_smem_desc(a_addr + k * UMMA_K * 2), umma_smem_desc(a_addr + PAIR_A_BYTES + k * UMMA_K * 2),
                            idesc, (kb | k) != 0);
           umma_commit_pair(&empty[s]);
+        }
+        if constexpr (LORA) {
+          if (tile == tile0) pdl_wait();
+          const LoraSteps steps(lora, tile / tiles_n, 1);
+          for (int e0 = 0; e0 < steps.entries && ok; e0 += steps.per_stage, ++it) {
+            const int s = it % STAGES, n = steps.of_stage(e0);
+            ok = mbar_wait<true>(&full[s], (it / STAGES) & 1, p.err, ERR_WAIT_FULL, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t a_addr = smem_u32(smem + s * STAGE_BYTES), b_addr = a_addr + PAIR_A_BYTES;
+            for (int j = 0; j < n; ++j)
+              for (int k = 0; k < lora.width; k += UMMA_K)
+                umma_bf16_pair(tmem, lora.desc(a_addr + (j * BM * lora.width + k) * 2), lora.desc(b_addr + (j * (bt / 2) * lora.width + k) * 2), idesc, 1);
+            umma_commit_pair(&empty[s]);
+          }
         }
         umma_commit_pair(&acc_full[acc]);  // always arrive so that the epilogues are released
       }

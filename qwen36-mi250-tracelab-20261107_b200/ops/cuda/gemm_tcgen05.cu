@@ -22,6 +22,7 @@
 // buffer (replaces the reference's Triton GEMV / grouped GEMM family: engine/fast/mfma.py:90-179,
 // engine/fast/moe_prefill.py:156-319, engine/fast/fused.py:581-692).
 #include "comm.cuh"
+#include "lora.cuh"
 
 namespace b200 {
 
@@ -177,9 +178,13 @@ __device__ __forceinline__ int argmax_column(int lane) {
   return ((lane >> 4) & 1) * 8 + ((lane >> 3) & 1) * 4 + ((lane >> 2) & 1) * 2 + ((lane >> 1) & 1);
 }
 
-template <int BT, int EPI, bool GROUPED, bool SPLIT = false, int RT = BM, int KPS = 1>
+// LORA (dense): behind the k-blocks of a tile come those of the low-rank adapters that its token rows use (lora.cuh), on the same accumulator.
+// The kernel in front is the one that makes their operand; it writes nothing that the other k-blocks read, and everything before it is complete when
+// this one starts, so the wait for it comes where the adapters do.
+template <int BT, int EPI, bool GROUPED, bool SPLIT = false, int RT = BM, int KPS = 1, bool LORA = false>
 __global__ void __launch_bounds__(GROUPED ? 160 + 32 * Cfg<BT, EPI, RT, KPS>::GATHER_WARPS : 192, Cfg<BT, EPI, RT, KPS>::CTAS_PER_SM)
-gemm_swapab_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, GemmParams p) {
+gemm_swapab_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, GemmParams p,
+                   const __grid_constant__ LoraArg<LORA> lora) {
   using C = Cfg<BT, EPI, RT, KPS>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -353,8 +358,8 @@ gemm_swapab_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
           load_weights(st, &full[kb], n0, 0, kb);
         }
       }
-      pdl_wait();
-      if (!GROUPED) pdl_launch();
+      if (!LORA) pdl_wait();
+      if (!GROUPED && !LORA) pdl_launch();
       for (int tile = tile0; tile < total && live; tile += tstep) {
       int n0, by, expert, row0, nrows;
       tile_geom(tile, n0, by, expert, row0, nrows);
@@ -374,6 +379,20 @@ gemm_swapab_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
             tma_load_2d(st + C::B_OFF + r * (BK * 2), &tmX, &full[s], (kb0 + kb) * BK, row0 + r);
         } else if constexpr (C::THIN) tma_load_3d(st + C::B_OFF, &tmX, &full[s], 0, row0, (kb0 + kb) * KPS);
         else tma_load_2d(st + C::B_OFF, &tmX, &full[s], (kb0 + kb) * BK, row0);
+      }
+      if constexpr (LORA) {
+        if (tile == tile0) { pdl_wait(); pdl_launch(); }
+        const LoraSteps steps(lora, by, KPS);
+        for (int e0 = 0; e0 < steps.entries && live; e0 += steps.per_stage, ++it) {
+          const int s = it % C::STAGES, n = steps.of_stage(e0);
+          uint8_t* st = smem + s * C::STAGE_BYTES;
+          if (!wait_free(it)) { live = false; break; }
+          mbar_expect_tx(&full[s], n * (RT + lora.tile_rows) * lora.width * 2);
+          for (int j = 0; j < n; ++j) {
+            tma_load_3d(st + j * RT * lora.width * 2, &lora.b, &full[s], lora.column(e0 + j), n0, lora.adapter(by, e0 + j));
+            tma_load_2d(st + C::B_OFF + j * lora.tile_rows * lora.width * 2, &lora.h, &full[s], 0, lora.row(by, e0 + j));
+          }
+        }
       }
       }
     }
@@ -423,6 +442,22 @@ gemm_swapab_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
         }
         // the group's stages are reusable once these MMAs have read them
         if (it % C::GROUP == C::GROUP - 1) umma_commit_if(LONE ? 1u : issue, &empty[it / C::GROUP % (C::STAGES / C::GROUP)]);
+      }
+      if constexpr (LORA) {
+        if (tile == tile0) pdl_wait();
+        const LoraSteps steps(lora, tile / tiles_n, KPS);
+        for (int e0 = 0; e0 < steps.entries && ok; e0 += steps.per_stage, ++it) {
+          const int s = it % C::STAGES, n = steps.of_stage(e0);
+          ok = wait(&full[s], (it / C::STAGES) & 1, ERR_WAIT_FULL);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t a_addr = smem_u32(smem + s * C::STAGE_BYTES), b_addr = a_addr + C::B_OFF;
+          for (int j = 0; j < n; ++j)
+            for (int k = 0; k < lora.width; k += UMMA_K)
+              umma_bf16_if(issue, tmem, lora.desc(a_addr + (j * RT * lora.width + k) * 2), lora.desc(b_addr + (j * lora.tile_rows * lora.width + k) * 2),
+                           idesc, 1);
+          if (it % C::GROUP == C::GROUP - 1) umma_commit_if(issue, &empty[it / C::GROUP % (C::STAGES / C::GROUP)]);
+        }
       }
       umma_commit_if(LONE ? 1u : issue, &acc_full[acc]);  // always arrive so that the epilogue is released
       }
@@ -793,6 +828,21 @@ static int make_map_gate_up(CUtensorMap* m, const void* base, uint64_t blocks, u
   return r == CUDA_SUCCESS ? 0 : -2;
 }
 
+// bf16 rows of `d0` numbers for boxes of `width` x `box_rows` (columns behind d0 read as zeros), swizzled over a box's row.
+static int make_map_lora(CUtensorMap* m, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, int width, uint32_t box_rows) {
+  EncodeFn fn = encode_fn();
+  if (!fn) return -1;
+  cuuint64_t dims[3] = {d0, d1, d2};
+  cuuint64_t strides[2] = {d0 * 2, d0 * d1 * 2};
+  cuuint32_t box[3] = {static_cast<cuuint32_t>(width), box_rows, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, d2 > 0 ? 3 : 2, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  width == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : width == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : -2;
+}
+
 // Weight map of a launch: `packed` selects the tile-packed layout (N padded to a multiple of 128 per expert, K a
 // multiple of 64; with the SiLU-mul epilogue the gate and up tiles of a k-block are stored back to back).
 static int weight_map(CUtensorMap* m, const void* W, int E, int N, int w_rows, int K, int ldw, bool silu, int packed,
@@ -831,16 +881,16 @@ static int launch_split(const CUtensorMap& tw, const CUtensorMap& tx, const Gemm
   cfg.numAttrs = 1;
   GemmParams q = p;
   q.grid_y = grid_y;
-  return cudaLaunchKernelEx(&cfg, kern, tw, tx, q) == cudaSuccess ? 0 : -4;
+  return cudaLaunchKernelEx(&cfg, kern, tw, tx, q, NoLora{}) == cudaSuccess ? 0 : -4;
 }
 
-template <int BT, int EPI, bool GROUPED, int RT = BM, int KPS = 1>
-static int launch(const CUtensorMap& tw, const CUtensorMap& tx, const GemmParams& p, int grid_y, cudaStream_t st) {
+template <int BT, int EPI, bool GROUPED, int RT = BM, int KPS = 1, bool LORA = false>
+static int launch(const CUtensorMap& tw, const CUtensorMap& tx, const GemmParams& p, int grid_y, cudaStream_t st, const LoraArg<LORA>& lora = {}) {
   using C = Cfg<BT, EPI, RT, KPS>;
-  if constexpr (!C::THIN && (EPI == EPI_BF16 || EPI == EPI_F32 || EPI == EPI_SILU_MUL)) {
+  if constexpr (!LORA && !C::THIN && (EPI == EPI_BF16 || EPI == EPI_F32 || EPI == EPI_SILU_MUL)) {
     if (p.splits > 1) return launch_split<BT, EPI, GROUPED>(tw, tx, p, grid_y, st);
   }
-  auto kern = gemm_swapab_kernel<BT, EPI, GROUPED, false, RT, KPS>;
+  auto kern = gemm_swapab_kernel<BT, EPI, GROUPED, false, RT, KPS, LORA>;
   // per device: the shared-memory attribute is set on the device that is current, and the persistent grid is sized
   // from that device's SM count (a process may drive several GPUs)
   static bool configured[MAX_DEVICES] = {};
@@ -860,18 +910,19 @@ static int launch(const CUtensorMap& tw, const CUtensorMap& tx, const GemmParams
   const long long tiles = static_cast<long long>((p.N + RT - 1) / RT) * grid_y;
   constexpr int threads = GROUPED ? 160 + 32 * C::GATHER_WARPS : 192;
   return launch_pdl(kern, dim3(static_cast<unsigned>(tiles < resident ? tiles : resident)), dim3(threads), C::SMEM, st, tw,
-                    tx, q) == cudaSuccess ? 0 : -4;
+                    tx, q, lora) == cudaSuccess ? 0 : -4;
 }
 
-template <int EPI, bool GROUPED>
-static int dispatch_bt(int bt, const CUtensorMap& tw, const CUtensorMap& tx, const GemmParams& p, int grid_y, cudaStream_t st) {
+template <int EPI, bool GROUPED, bool LORA = false>
+static int dispatch_bt(int bt, const CUtensorMap& tw, const CUtensorMap& tx, const GemmParams& p, int grid_y, cudaStream_t st,
+                       const LoraArg<LORA>& lora = {}) {
   switch (bt) {
-    case 16: return launch<16, EPI, GROUPED>(tw, tx, p, grid_y, st);
-    case 32: return launch<32, EPI, GROUPED>(tw, tx, p, grid_y, st);
-    case 64: return launch<64, EPI, GROUPED>(tw, tx, p, grid_y, st);
-    case 128: return launch<128, EPI, GROUPED>(tw, tx, p, grid_y, st);
+    case 16: return launch<16, EPI, GROUPED, BM, 1, LORA>(tw, tx, p, grid_y, st, lora);
+    case 32: return launch<32, EPI, GROUPED, BM, 1, LORA>(tw, tx, p, grid_y, st, lora);
+    case 64: return launch<64, EPI, GROUPED, BM, 1, LORA>(tw, tx, p, grid_y, st, lora);
+    case 128: return launch<128, EPI, GROUPED, BM, 1, LORA>(tw, tx, p, grid_y, st, lora);
     case 256:
-      if (EPI != EPI_SILU_MUL) return launch<(EPI != EPI_SILU_MUL ? 256 : 128), EPI, GROUPED>(tw, tx, p, grid_y, st);
+      if (EPI != EPI_SILU_MUL) return launch<(EPI != EPI_SILU_MUL ? 256 : 128), EPI, GROUPED, BM, 1, LORA>(tw, tx, p, grid_y, st, lora);
       return -5;  // the gate/up epilogue has no 256-row form
     default: return -5;
   }
@@ -941,9 +992,9 @@ constexpr int PAIR_FORM = -256;  // token tile of up to 256 rows on two SMs, in 
 constexpr int PAIR_FORM_128 = -128;  // of up to 128 rows
 
 // Two SMs per tile (gemm_pair.cuh). A cluster's CTAs sit on one SM each; the persistent grid is one cluster per pair of SMs.
-template <int EPI, bool GROUPED, int PBT>
-static int launch_pair(const CUtensorMap& tw, const CUtensorMap& tx, GemmParams p, int grid_y, cudaStream_t st) {
-  auto kern = gemm_pair_kernel<EPI, GROUPED, PBT>;
+template <int EPI, bool GROUPED, int PBT, bool LORA = false>
+static int launch_pair(const CUtensorMap& tw, const CUtensorMap& tx, GemmParams p, int grid_y, cudaStream_t st, const LoraArg<LORA>& lora = {}) {
+  auto kern = gemm_pair_kernel<EPI, GROUPED, PBT, LORA>;
   static bool configured[MAX_DEVICES] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= MAX_DEVICES) return -3;
@@ -955,7 +1006,7 @@ static int launch_pair(const CUtensorMap& tw, const CUtensorMap& tx, GemmParams 
   const int rows = EPI == EPI_SILU_MUL ? BM : 2 * BM;
   const long long tiles = static_cast<long long>((p.N + rows - 1) / rows) * grid_y, pairs = sm_count() / 2;
   return launch_clusters(2, kern, dim3(2 * static_cast<unsigned>(tiles < pairs ? tiles : pairs)), dim3(pair_threads(EPI)), PairCfg<PBT>::SMEM,
-                         st, tw, tx, p) == cudaSuccess ? 0 : -4;
+                         st, tw, tx, p, lora) == cudaSuccess ? 0 : -4;
 }
 
 // What the pair form asks of a launch: an epilogue that it has (gate/up grouped only), whole k-blocks, and bf16 output rows that
@@ -1015,14 +1066,14 @@ static bool pair_pays(int T, int N, int K, int epi) {
 }
 
 // Dense GEMM with two SMs per tile.
-template <int EPI>
-static int launch_pair_dense(const void* X, const void* W, GemmParams p, int ldx, int ldw, int packed, cudaStream_t st) {
+template <int EPI, bool LORA = false>
+static int launch_pair_dense(const void* X, const void* W, GemmParams p, int ldx, int ldw, int packed, cudaStream_t st, const LoraArg<LORA>& lora = {}) {
   CUtensorMap tw, tx;
   p.pair_bt = pair_rows(p.T, p.N);
   if (weight_map(&tw, W, 0, p.N, p.N, p.K, ldw, false, packed, &p)) return -1;
   if (make_map(&tx, X, p.K, p.T, 0, ldx, 0, p.pair_bt / 2)) return -1;
   const int gy = (p.T + p.pair_bt - 1) / p.pair_bt;
-  return p.pair_bt <= 128 ? launch_pair<EPI, false, 128>(tw, tx, p, gy, st) : launch_pair<EPI, false, PAIR_BT>(tw, tx, p, gy, st);
+  return p.pair_bt <= 128 ? launch_pair<EPI, false, 128, LORA>(tw, tx, p, gy, st, lora) : launch_pair<EPI, false, PAIR_BT, LORA>(tw, tx, p, gy, st, lora);
 }
 
 // Grouped GEMMs with two SMs per tile of up to PBT rows: gate/up with rows by index, or a bf16 projection of sorted rows.
@@ -1048,8 +1099,8 @@ static int launch_pair_grouped(const void* X, const void* W, GemmParams p, int E
 }
 
 // Launch of a thin dense form; -5 where there is no such form.
-template <int EPI>
-static int launch_thin_dense(const DenseForm& f, const void* X, const void* W, GemmParams p, int ldx, cudaStream_t st) {
+template <int EPI, bool LORA = false>
+static int launch_thin_dense(const DenseForm& f, const void* X, const void* W, GemmParams p, int ldx, cudaStream_t st, const LoraArg<LORA>& lora = {}) {
   CUtensorMap tw, tx;
   const uint64_t nk = p.K / BK;
   p.packed = 1;
@@ -1057,12 +1108,12 @@ static int launch_thin_dense(const DenseForm& f, const void* X, const void* W, G
   if (make_map_kblocks(&tw, W, BM, BK * 2, p.w_tiles * nk, BM * BK * 2, f.rt, f.kps)) return -1;
   if (make_map_kblocks(&tx, X, p.T, static_cast<uint64_t>(ldx) * 2, nk, BK * 2, f.bt, f.kps)) return -1;
   const int gy = (p.T + f.bt - 1) / f.bt;
-  if (f.bt == 16 && f.rt == 32 && f.kps == 4) return launch<16, EPI, false, 32, 4>(tw, tx, p, gy, st);
-  if (f.bt == 16 && f.rt == 64 && f.kps == 4) return launch<16, EPI, false, 64, 4>(tw, tx, p, gy, st);
-  if (f.bt == 16 && f.rt == 64 && f.kps == 2) return launch<16, EPI, false, 64, 2>(tw, tx, p, gy, st);
-  if (f.bt == 32 && f.rt == 64 && f.kps == 4) return launch<32, EPI, false, 64, 4>(tw, tx, p, gy, st);
-  if (f.bt == 32 && f.rt == 64 && f.kps == 2) return launch<32, EPI, false, 64, 2>(tw, tx, p, gy, st);
-  if (f.bt == 64 && f.rt == 64 && f.kps == 4) return launch<64, EPI, false, 64, 4>(tw, tx, p, gy, st);
+  if (f.bt == 16 && f.rt == 32 && f.kps == 4) return launch<16, EPI, false, 32, 4, LORA>(tw, tx, p, gy, st, lora);
+  if (f.bt == 16 && f.rt == 64 && f.kps == 4) return launch<16, EPI, false, 64, 4, LORA>(tw, tx, p, gy, st, lora);
+  if (f.bt == 16 && f.rt == 64 && f.kps == 2) return launch<16, EPI, false, 64, 2, LORA>(tw, tx, p, gy, st, lora);
+  if (f.bt == 32 && f.rt == 64 && f.kps == 4) return launch<32, EPI, false, 64, 4, LORA>(tw, tx, p, gy, st, lora);
+  if (f.bt == 32 && f.rt == 64 && f.kps == 2) return launch<32, EPI, false, 64, 2, LORA>(tw, tx, p, gy, st, lora);
+  if (f.bt == 64 && f.rt == 64 && f.kps == 4) return launch<64, EPI, false, 64, 4, LORA>(tw, tx, p, gy, st, lora);
   return -5;
 }
 
@@ -1153,6 +1204,68 @@ extern "C" int b200_gemm_dense(const void* X, const void* W, void* out, int T, i
     case EPI_ARGMAX: return dispatch_bt<EPI_ARGMAX, false>(bt, tw, tx, p, gy, st);
   }
   return -6;
+}
+
+// ------------------------------------------------------------------ a projection with low-rank adapters beside it
+// The form of the projection is the one that it takes without adapters, and with it the token rows that share a tile.
+struct LoraForm {
+  bool pair;
+  DenseForm f;
+  int rows;  // token rows per tile
+};
+static LoraForm lora_form(const GemmParams& p, int epi, bool packed) {
+  if (pair_takes(p, epi, false) && pair_pays(p.T, p.N, p.K, epi)) return {true, {}, pair_rows(p.T, p.N)};
+  const DenseForm f = dense_form(p.T, p.N, p.K, packed);
+  return {false, f, f.rt == BM && p.T <= f.bt ? (p.T + 15) / 16 * 16 : f.bt};
+}
+
+template <int EPI>
+static int launch_lora(const LoraForm& form, const void* X, const void* W, GemmParams p, int ldx, int ldw, int packed, const LoraExt& ext, cudaStream_t st) {
+  if (form.pair) return launch_pair_dense<EPI, true>(X, W, p, ldx, ldw, packed, st, ext);
+  if (form.f.rt < BM) return launch_thin_dense<EPI, true>(form.f, X, W, p, ldx, st, ext);
+  CUtensorMap tw, tx;
+  const int bt = form.f.bt, gy = (p.T + bt - 1) / bt;
+  if (weight_map(&tw, W, 0, p.N, p.N, p.K, ldw, false, packed, &p)) return -1;
+  if (gy == 1) p.x_rows = form.rows;
+  if (make_map(&tx, X, p.K, p.T, 0, ldx, 0, form.rows)) return -1;
+  return dispatch_bt<EPI, false, true>(bt, tw, tx, p, gy, st, ext);
+}
+
+// Bytes of b200_lora_linear's workspace.
+extern "C" long long b200_lora_work_bytes(int T, int N, int K, int R, int L, int out_f32, int packed) {
+  GemmParams p{};
+  p.T = T; p.N = N; p.K = K; p.ldo = N;
+  const LoraForm form = lora_form(p, out_f32 ? EPI_F32 : EPI_BF16, packed);
+  LoraTiles t;
+  return static_cast<long long>(lora_tiles(T, R, L, form.rows, out_f32, nullptr, &t));
+}
+
+// out[T, N] = X[T, K] W[N, K]^T, and for a row t with 0 <= rows[t] < L the adapter's part (lora.cuh). B has `nb` rows, at most N.
+extern "C" int b200_lora_linear(const void* X, int ldx, const void* W, int ldw, int packed, const void* A, const void* B, const float* scale,
+                                const int* rows, void* out, int out_f32, int T, int N, int nb, int K, int R, int L, void* work, int* err,
+                                cudaStream_t st) {
+  if (T <= 0) return 0;
+  if (R <= 0 || R % 8 || R > LORA_MAX_RANK || L <= 0 || L > LORA_MAX_ADAPTERS || nb > N) return -7;
+  const int epi = out_f32 ? EPI_F32 : EPI_BF16;
+  GemmParams p{N, K, T, N, out, nullptr, nullptr, 0, nullptr, nullptr, err, nullptr, CommCtx{}, 0, nullptr, nullptr, 1, nullptr, {}};
+  const LoraForm form = lora_form(p, epi, packed);
+  LoraTiles t;
+  lora_tiles(T, R, L, form.rows, out_f32, work, &t);
+  if (const int rc = lora_shrink(X, ldx, A, scale, rows, T, K, R, L, t, err, st)) return rc;
+  LoraExt ext;
+  ext.count = t.count;
+  ext.list = t.list;
+  ext.cap = t.cap;
+  ext.chunks = t.chunks;
+  ext.parts = t.parts;
+  ext.width = t.width;
+  ext.tile_rows = form.rows;
+  // rows of 2 * width bytes, in groups of 8, swizzled over as many bytes: layout type 2, 4 or 6 for 128, 64 or 32
+  ext.desc_base = static_cast<uint64_t>(1) << 16 | static_cast<uint64_t>(8 * t.width * 2 >> 4) << 32 | static_cast<uint64_t>(1) << 46 |
+                  static_cast<uint64_t>(t.width == 64 ? 2 : t.width == 32 ? 4 : 6) << 61;
+  if (make_map_lora(&ext.b, B, R, nb, L, t.width, form.pair ? BM : form.f.rt)) return -1;
+  if (make_map_lora(&ext.h, t.h, t.width, static_cast<uint64_t>(t.tiles) * t.cap * t.chunks * form.rows, 0, t.width, form.pair ? form.rows / 2 : form.rows)) return -1;
+  return out_f32 ? launch_lora<EPI_F32>(form, X, W, p, ldx, ldw, packed, ext, st) : launch_lora<EPI_BF16>(form, X, W, p, ldx, ldw, packed, ext, st);
 }
 
 // Grouped: X is the expert-sorted activation buffer [cap, K]; tile i covers rows

@@ -95,7 +95,8 @@ class _Sig:
     b200_kv8_prefill_positions = [I]
     b200_kv8_prefill_cut = [I]
     b200_kv8_prefill = [P, P, P, P, P, P, I, I, I, I, I, L, P, I, I, I, I, I, I, P, P, P, P, P]
-    b200_lora_add = [P, L, P, P, P, P, P, P, I, I, I, I, I, I, I, P, P]
+    b200_lora_work_bytes = [I, I, I, I, I, I, I]
+    b200_lora_linear = [P, I, P, I, I, P, P, P, P, P, I, I, I, I, I, I, I, P, P, P]
     b200_sample_max_exclude = []
     b200_sample_max_rows = []
     b200_sample_work_bytes = [I, I]
@@ -279,6 +280,33 @@ def linear(x: torch.Tensor, w: torch.Tensor, out_dtype: torch.dtype | None = Non
     return out
 
 
+LORA_WORK = 256 << 20  # bytes of workspace that one launch of lora_linear may take: h, once for every adapter of a token tile
+
+
+@functools.cache
+def _lora_work(device: int, T: int, N: int, K: int, R: int, L: int, f32: bool, packed: int) -> int:
+    """Bytes of workspace on a device, whose number of SMs the form goes by."""
+    fn = lib().b200_lora_work_bytes
+    fn.restype = ctypes.c_longlong
+    return fn(T, N, K, R, L, f32, packed)
+
+
+def _lora_part(x, w, adapters, rows, out, n_own: int) -> None:
+    a, b, scale = adapters
+    (T, K), N, (L, R, _) = x.shape, w.shape[0], a.shape
+    dev, f32, packed = x.device, out.dtype == torch.float32, is_packed(w)
+    size = _lora_work(dev.index, T, N, K, R, L, f32, packed)
+    if size > LORA_WORK and T > 256:  # hundreds of adapters in a long pass: by parts of its rows
+        half = (T // 2 + 255) // 256 * 256
+        for part in (slice(0, half), slice(half, T)):
+            _lora_part(x[part], w, adapters, rows[part], out[part], n_own)
+        return
+    work = torch.empty(size, dtype=torch.uint8, device=dev)
+    _check(lib().b200_lora_linear(
+        x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), packed, a.data_ptr(), b.data_ptr(), scale.data_ptr(), rows.data_ptr(), out.data_ptr(),
+        f32, T, N, n_own, K, R, L, work.data_ptr(), _err_ptr(dev), _raw_stream(dev)), "lora_linear")
+
+
 def lora_linear(x: torch.Tensor, w: torch.Tensor, adapters: LoraWeights, rows: torch.Tensor, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """``linear(x, w)`` with the low-rank adapter of each row's own request beside it (``ops/lora.py``): row ``t`` of ``x [T, K]`` uses adapter
     ``rows[t]`` (int32 ``[T]``), none where that is negative. One rounding, to bf16 (default) or fp32. A row's bits depend on its own numbers and
@@ -302,15 +330,14 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, adapters: LoraWeights, rows: t
         raise ValueError(f"lora_linear: adapter numbers {tuple(rows.shape)} {rows.dtype} are not a contiguous int32 [{T}]")
     if w.device != dev or adapters.a.device != dev or rows.device != dev:
         raise ValueError(f"lora_linear: rows on {dev}, weights on {w.device}, adapters on {adapters.a.device}, their numbers on {rows.device}")
-    if K % 8 or x.stride(1) != 1 or w.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
-        raise ValueError(f"lora_linear: rows of {K} numbers with strides {x.stride()} and weights with strides {w.stride()}: rows are whole 16-byte pieces")
+    if K % 8 or x.stride(1) != 1 or w.stride(1) != 1 or x.stride(0) % 8 or w.stride(0) % 8 \
+            or (x.data_ptr() | w.data_ptr() | adapters.a.data_ptr() | adapters.b.data_ptr()) % 16:
+        raise ValueError(f"lora_linear: rows of {K} numbers with strides {x.stride()}, weights with strides {w.stride()}: rows, weights and adapters are "
+                         "whole 16-byte pieces on 16-byte boundaries")
     out = torch.empty(T, N, dtype=torch.float32 if f32 else torch.bfloat16, device=dev)
     if T == 0:
         return out
-    base = linear(x, w, out_dtype=torch.float32)
-    _check(lib().b200_lora_add(
-        x.data_ptr(), x.stride(0), base.data_ptr(), adapters.a.data_ptr(), adapters.b.data_ptr(), adapters.scale.data_ptr(), rows.data_ptr(),
-        out.data_ptr(), f32, T, N, n_own, K, R, L, _err_ptr(dev), _raw_stream(dev)), "lora_add")
+    _lora_part(x, w, adapters, rows, out, n_own)
     return out
 
 
