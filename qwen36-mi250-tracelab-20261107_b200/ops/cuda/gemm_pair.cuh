@@ -225,15 +225,16 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
           if (tile == tile0) { pdl_wait(); pdl_launch(); }
           const int by = tile / tiles_n;
           const LoraSteps steps(lora, by, 1);
+          LoraEntry e(lora, by, steps.entries);
           for (int e0 = 0; e0 < steps.entries && live; e0 += steps.per_stage, ++it) {
             const int s = it % STAGES, n = steps.of_stage(e0);
             uint8_t* st = smem + s * STAGE_BYTES;
             const uint32_t bar = dsmem_addr(smem_u32(&full[s]), 0);
             if (!mbar_wait<true>(&empty[s], ((it / STAGES) & 1) ^ 1, p.err, ERR_WAIT_EMPTY, abort_flag)) { live = false; break; }
             if (rank == 0) mbar_expect_tx(&full[s], n * (2 * BM + bt) * lora.width * 2);
-            for (int j = 0; j < n; ++j) {
-              tma_load_3d_pair(st + j * BM * lora.width * 2, &lora.b, bar, lora.column(e0 + j), (2 * nx + static_cast<int>(rank)) * BM, lora.adapter(by, e0 + j));
-              tma_load_2d_pair(st + PAIR_A_BYTES + j * (bt / 2) * lora.width * 2, &lora.h, bar, 0, lora.row(by, e0 + j) + static_cast<int>(rank) * half);
+            for (int j = 0; j < n; ++j, e.step(lora, steps.entries - e0 - j)) {
+              tma_load_3d_pair(st + j * BM * lora.width * 2, &lora.b, bar, e.column, (2 * nx + static_cast<int>(rank)) * BM, e.adapter);
+              tma_load_2d_pair(st + PAIR_A_BYTES + j * (bt / 2) * lora.width * 2, &lora.h, bar, 0, e.row + static_cast<int>(rank) * half);
             }
           }
         }

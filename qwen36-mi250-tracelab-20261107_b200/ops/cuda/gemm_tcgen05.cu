@@ -383,14 +383,15 @@ gemm_swapab_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
       if constexpr (LORA) {
         if (tile == tile0) { pdl_wait(); pdl_launch(); }
         const LoraSteps steps(lora, by, KPS);
+        LoraEntry e(lora, by, steps.entries);
         for (int e0 = 0; e0 < steps.entries && live; e0 += steps.per_stage, ++it) {
           const int s = it % C::STAGES, n = steps.of_stage(e0);
           uint8_t* st = smem + s * C::STAGE_BYTES;
           if (!wait_free(it)) { live = false; break; }
           mbar_expect_tx(&full[s], n * (RT + lora.tile_rows) * lora.width * 2);
-          for (int j = 0; j < n; ++j) {
-            tma_load_3d(st + j * RT * lora.width * 2, &lora.b, &full[s], lora.column(e0 + j), n0, lora.adapter(by, e0 + j));
-            tma_load_2d(st + C::B_OFF + j * lora.tile_rows * lora.width * 2, &lora.h, &full[s], 0, lora.row(by, e0 + j));
+          for (int j = 0; j < n; ++j, e.step(lora, steps.entries - e0 - j)) {
+            tma_load_3d(st + j * RT * lora.width * 2, &lora.b, &full[s], e.column, n0, e.adapter);
+            tma_load_2d(st + C::B_OFF + j * lora.tile_rows * lora.width * 2, &lora.h, &full[s], 0, e.row);
           }
         }
       }

@@ -24,9 +24,6 @@ struct LoraExt {
   const int* count;    // adapters of each token tile
   const int* list;     // [tile][cap] which
   int cap, chunks, parts, width, tile_rows;  // most adapters of a tile; entries per adapter; parts of h; columns of an entry
-  __device__ __forceinline__ int adapter(int tile, int e) const { return list[tile * cap + e / chunks]; }
-  __device__ __forceinline__ int column(int e) const { return e % chunks / parts * width; }
-  __device__ __forceinline__ int row(int tile, int e) const { return (tile * cap * chunks + e) * tile_rows; }
   __device__ __forceinline__ uint64_t desc(uint32_t smem_addr) const { return desc_base | ((smem_addr & 0x3FFFF) >> 4); }
 };
 template <bool LORA>
@@ -41,6 +38,27 @@ struct LoraSteps {
   int entries, per_stage;
   __device__ __forceinline__ LoraSteps(const LoraExt& x, int tile, int k_blocks) : entries(x.count[tile] * x.chunks), per_stage(k_blocks * 64 / x.width) {}
   __device__ __forceinline__ int of_stage(int e0) const { return min(per_stage, entries - e0); }
+};
+
+// The entries of a token tile one after the other: adapter, first rank, row of h. (Counted on, as each entry of a batch of many adapters would cost the
+// producer three divisions and a look-up.)
+struct LoraEntry {
+  const int* next;
+  int adapter, column = 0, row, then, sub = 0, part = 0;
+  __device__ __forceinline__ LoraEntry(const LoraExt& x, int tile, int entries)
+      : next(x.list + tile * x.cap), row(tile * x.cap * x.chunks * x.tile_rows) {
+    adapter = entries > 0 ? *next : 0;
+    then = entries > x.chunks ? *++next : 0;
+  }
+  __device__ __forceinline__ void step(const LoraExt& x, int left) {  // left: entries behind the one left
+    row += x.tile_rows;
+    if (++part == x.parts) { part = 0; column += x.width; }
+    if (++sub == x.chunks) {
+      sub = column = 0;
+      adapter = then;
+      if (left > x.chunks) then = *++next;
+    }
+  }
 };
 
 // A call's tables and h in its workspace.
