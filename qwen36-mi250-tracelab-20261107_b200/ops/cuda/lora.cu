@@ -189,6 +189,14 @@ static int launch_shrink(const void* x, int ldx, const void* a, const float* sca
   const int blocks = (T + 16 * MT - 1) / (16 * MT), columns = t.width * (t.chunks / t.parts);
   // CTAs for the adapters of 16 rows: as many as there may be while the rows are few, one when they fill the SMs
   const int side = blocks >= 64 ? 1 : min(min(16 * MT, T), L);
+  // An SM that runs this kernel gives its memory to shared memory as the GEMM needs it: otherwise no CTA of that one can join before the SM is empty
+  // (128 rows of 9216 x 2048, one adapter: TODO us).
+  static bool configured[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -3;
+  if (!configured[dev] && cudaFuncSetAttribute(lora_shrink_kernel<NT, MT>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                               cudaSharedmemCarveoutMaxShared) != cudaSuccess) return -3;
+  configured[dev] = true;
   return launch_pdl(lora_shrink_kernel<NT, MT>, dim3(blocks, side, (columns + 8 * NT - 1) / (8 * NT)), dim3(SHRINK_THREADS), 0, st,
                     static_cast<const bf16*>(x), ldx, static_cast<const bf16*>(a), scale, rows, T, K, R, L, t, err) == cudaSuccess ? 0 : -4;
 }
