@@ -112,6 +112,7 @@ def _sampling(body: dict, default_max: int | None, max_keys: tuple[str, ...]) ->
         stop=_stops(body),
         ignore_eos=bool(body.get("ignore_eos", False)),
         min_tokens=_int(body, "min_tokens", 0, 0) or 0,
+        min_p=_num(body, "min_p", 0.0, 0.0, 1.0),
     )
 
 
@@ -249,6 +250,7 @@ def error_body(message: str, status: int) -> dict:
     return {"error": {"message": message, "type": kinds.get(status, "BadRequestError"), "code": status}}
 
 
-def models_body(model: str, max_model_len: int) -> dict:
-    return {"object": "list", "data": [{"id": model, "object": "model", "owned_by": "b200serve",
-                                        "max_model_len": max_model_len}]}
+def models_body(model: str, max_model_len: int, adapters=()) -> dict:
+    """The served model, and its adapters, which requests name in its place."""
+    own = {"object": "model", "owned_by": "b200serve", "max_model_len": max_model_len}
+    return {"object": "list", "data": [{"id": model, **own}, *({"id": a, **own, "parent": model} for a in adapters)]}

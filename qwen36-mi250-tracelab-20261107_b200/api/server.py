@@ -138,7 +138,7 @@ class RequestState:
     def __init__(self, service, request: CompletionRequest | ChatRequest, prompt_len: int, gen: Generation) -> None:
         self.service, self.request, self.gen = service, request, gen
         self.chat = isinstance(request, ChatRequest)
-        self.env = Envelope(service.model_name, "chat.completion" if self.chat else "text_completion")
+        self.env = Envelope(request.model or service.model_name, "chat.completion" if self.chat else "text_completion")
         self.text = _TextStream(service.codec, request.sampling.stop, self.chat and request.thinking)
         self.usage = Usage(prompt_len)
         self.ids: list[int] = []
@@ -210,7 +210,7 @@ class Stream:
         self.q: "queue.SimpleQueue[TokenEvent]" = queue.SimpleQueue()
         self.lock = threading.Lock()
         self.to_writer = False
-        self.gen = Generation(prompt, request.sampling, on_event=self._sink)
+        self.gen = Generation(prompt, request.sampling, on_event=self._sink, adapter=service.adapter_of(request))
         self.state = RequestState(service, request, len(prompt), self.gen)
         self.sock: socket.socket | None = None  # set for SSE responses: the writer sends on it
         self.backlog = bytearray()  # bytes the socket did not take yet
@@ -357,6 +357,8 @@ class Service:
         self.engine = engine
         self.codec = codec
         self.model_name = model_name
+        if model_name in getattr(engine, "adapters", ()):
+            raise ValueError(f"an adapter is called {model_name!r}, as the served model is")
         self.worker = EngineWorker(engine)
         self.worker.start()
         self.writer: StreamWriter | None = None
@@ -364,10 +366,14 @@ class Service:
             self.writer = StreamWriter()
             self.writer.start()
 
+    def adapter_of(self, request: CompletionRequest | ChatRequest) -> str | None:
+        """The adapter that the request names as its model; None for the served model itself."""
+        return request.model if request.model is not None and request.model != self.model_name else None
+
     # ------------------------------------------------------------------ request -> events
-    def _events(self, prompt: list[int], sampling) -> tuple[Generation, "queue.Queue[TokenEvent]"]:
+    def _events(self, prompt: list[int], sampling, adapter: str | None = None) -> tuple[Generation, "queue.Queue[TokenEvent]"]:
         q: "queue.Queue[TokenEvent]" = queue.Queue()
-        gen = Generation(prompt, sampling, on_event=lambda g, e: q.put(e))
+        gen = Generation(prompt, sampling, on_event=lambda g, e: q.put(e), adapter=adapter)
         self.worker.submit(gen)
         return gen, q
 
@@ -376,7 +382,7 @@ class Service:
 
         Raises ``RequestError`` before the first yield when the engine refuses the request.
         """
-        gen, q = self._events(prompt, request.sampling)
+        gen, q = self._events(prompt, request.sampling, self.adapter_of(request))
         state = RequestState(self, request, len(prompt), gen)
         try:
             while True:
@@ -472,7 +478,7 @@ class Handler(BaseHTTPRequestHandler):
             body = svc.health()
             self._json(503 if body["status"] == "unavailable" else 200, body)
         elif self.path == "/v1/models":
-            self._json(200, protocol.models_body(svc.model_name, svc.engine.max_model_len))
+            self._json(200, protocol.models_body(svc.model_name, svc.engine.max_model_len, getattr(svc.engine, "adapters", ())))
         elif self.path == "/metrics":
             data = metrics_text(svc.health()).encode()
             self.send_response(200)
@@ -499,7 +505,7 @@ class Handler(BaseHTTPRequestHandler):
                 request = protocol.parse_chat(body)
             else:
                 raise RequestError(f"no route {self.path}", 404)
-            if request.model is not None and request.model != svc.model_name:
+            if request.model is not None and request.model != svc.model_name and request.model not in getattr(svc.engine, "adapters", ()):
                 raise RequestError(f"model {request.model!r} is not served here (serving {svc.model_name!r})", 404)
             reqstamps.mark(stamp, "parsed")
             prompt = svc.tokenize(request)
@@ -636,6 +642,8 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--replica-devices", default=env("ENGINE_REPLICA_DEVICES"))
     ap.add_argument("--device", default=env("ENGINE_DEVICE", "auto"), choices=["auto", "cpu", "cuda"])
     ap.add_argument("--max-seqs", type=int, default=int(env("ENGINE_SLOTS", "128")))
+    ap.add_argument("--adapter", action="append", default=None, metavar="NAME=DIR",
+                    help="a low-rank adapter (PEFT directory) that requests may name as their model; may be given several times")
     ap.add_argument("--replica-split", default=env("ENGINE_REPLICA_SPLIT", "tensor"), choices=["tensor", "layers"],
                     help="how a replica of several GPUs (--gpus-per-replica) divides the model: every layer sharded "
                          "across them, or a run of whole layers on each (a capacity measure: one GPU computes at a time)")
@@ -657,7 +665,7 @@ def load_service(args: argparse.Namespace) -> Service:
     cfg = EngineConfig.from_env(
         model=args.model, max_model_len=args.max_model_len, prefill_chunk_tokens=args.prefill_chunk_tokens,
         prefix_cache_tokens=args.prefix_cache_tokens, prefix_cache_entries=args.prefix_cache_entries,
-        prefix_cache_gib=args.prefix_cache_gib, max_seqs=args.max_seqs,
+        prefix_cache_gib=args.prefix_cache_gib, max_seqs=args.max_seqs, adapters=",".join(args.adapter) if args.adapter else None,
     )
     if os.environ.get("ENGINE_PACK_WEIGHTS") is None:
         cfg.pack_weights = True  # the server owns the weights it loads: stream them tile-packed

@@ -30,6 +30,9 @@ from ..config import PAGE_SIZE
 from .pools import PagePool, SlotPool
 
 
+NO_SALT = b"\0" * 16
+
+
 def _block_hash(prev: bytes, tokens) -> bytes:
     return hashlib.blake2b(array("q", tokens).tobytes(), key=prev, digest_size=16).digest()
 
@@ -80,9 +83,10 @@ class PrefixCache:
         self.bytes = 0
 
     # ------------------------------------------------------------------ keys
-    def _chain(self, tokens, upto_blocks: int) -> list[bytes]:
-        """Chain hashes after 0, 1, ..., ``upto_blocks`` full blocks."""
-        out = [b"\0" * 16]
+    def _chain(self, tokens, upto_blocks: int, salt: bytes = NO_SALT) -> list[bytes]:
+        """Chain hashes after 0, 1, ..., ``upto_blocks`` full blocks. ``salt`` (16 bytes) keeps apart the entries of sequences whose states differ
+        although their tokens do not: those of another adapter."""
+        out = [salt]
         if upto_blocks <= 0:
             return out
         # one conversion of the covered tokens to bytes, then a digest per block over slices of it (the per-block
@@ -110,12 +114,12 @@ class PrefixCache:
         self.stats.stored += 1
         self._enforce()
 
-    def store_snapshot(self, tokens, length: int, pages: list[int], slot: int) -> bool:
+    def store_snapshot(self, tokens, length: int, pages: list[int], slot: int, salt: bytes = NO_SALT) -> bool:
         """Keep the state at ``length`` (a block multiple). ``pages`` are shared (ref count raised);
         ``slot`` must already hold a private copy of the GDN state and is owned by the cache."""
         assert length % self.block == 0 and length > 0
         nb = length // self.block
-        chain = self._chain(tokens, nb)
+        chain = self._chain(tokens, nb, salt)
         key = (nb, chain[nb], "s")
         if key in self._lru:
             self._lru.move_to_end(key)
@@ -126,22 +130,22 @@ class PrefixCache:
         self._insert(e)
         return True
 
-    def has_snapshot(self, tokens, length: int) -> bool:
+    def has_snapshot(self, tokens, length: int, salt: bytes = NO_SALT) -> bool:
         nb = length // self.block
-        return (nb, self._chain(tokens, nb)[nb], "s") in self._lru
+        return (nb, self._chain(tokens, nb, salt)[nb], "s") in self._lru
 
-    def store_tail(self, tokens, pages: list[int], slot: int) -> None:
+    def store_tail(self, tokens, pages: list[int], slot: int, salt: bytes = NO_SALT) -> None:
         """Park a finished sequence: ``tokens`` are what its KV and state cover; ownership moves here."""
         n = len(tokens)
         nb = n // self.block
-        chain = self._chain(tokens, nb)
+        chain = self._chain(tokens, nb, salt)
         key = (nb, chain[nb], "t", bytes(array("q", tokens[nb * self.block :]).tobytes()))
         e = Entry("tail", array("q", tokens), list(pages), slot, key,
                   nbytes=self.slot_bytes + len(pages) * self.page_bytes)
         self._insert(e)
 
     # ------------------------------------------------------------------ lookup
-    def lookup(self, prompt) -> Entry | None:
+    def lookup(self, prompt, salt: bytes = NO_SALT) -> Entry | None:
         """Longest entry that covers a proper prefix of ``prompt`` (at most ``len(prompt) - 1`` tokens,
         so that at least one row is left to produce logits). A tail is removed from the cache and
         handed to the caller; a snapshot stays and the caller copies its state."""
@@ -149,7 +153,7 @@ class PrefixCache:
         if limit <= 0 or not self._lru:
             return None
         nb_max = limit // self.block
-        chain = self._chain(prompt, nb_max)
+        chain = self._chain(prompt, nb_max, salt)
         best: Entry | None = None
         for nb in range(nb_max, -1, -1):
             for e in self._tails_at.get((nb, chain[nb]), ()):

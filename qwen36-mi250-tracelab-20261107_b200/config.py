@@ -270,6 +270,7 @@ class EngineConfig:
     # clusters of the index built at load; draft_ivf_probes clusters are scored exactly per draft
     draft_ivf: int = 0
     draft_ivf_probes: int = 64
+    adapters: str = ""  # low-rank adapters that requests may name as their model: NAME=DIR[,NAME=DIR...] (models/lora.py)
     # observability
     loop_timers: bool = False
     req_stamps: bool = False
@@ -301,6 +302,7 @@ class EngineConfig:
             "kv_pages": "ENGINE_KV_PAGES",
             "kv_dtype": "ENGINE_KV_DTYPE",
             "state_slots": "ENGINE_STATE_SLOTS",
+            "adapters": "ENGINE_ADAPTERS",
         }
         for attr, env in env_map.items():
             setattr(cfg, attr, _env(env, getattr(cfg, attr)))

@@ -25,6 +25,7 @@ from typing import Any, Callable
 import torch
 
 from ..config import ModelConfig
+from ..ops.lora import LoraWeights
 
 INDEX = "model.safetensors.index.json"
 
@@ -52,6 +53,9 @@ class LayerWeights:
     shared_down: torch.Tensor | None = None
     shared_gate: torch.Tensor | None = None
     expert_map: torch.Tensor | None = None  # expert parallelism: global expert id -> local slot or -1
+    # low-rank adapters of the mixer's projections (models/lora.py)
+    in_lora: LoraWeights | None = None
+    out_lora: LoraWeights | None = None
 
     def tensors(self):
         for k, v in self.__dict__.items():

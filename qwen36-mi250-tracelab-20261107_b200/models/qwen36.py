@@ -114,6 +114,13 @@ class Model:
         self.tp = tp
         self.ep = ep
         self.pp = pp
+        # adapter of the sequence in each state slot, -1: none (``models/lora.py``); None: the weights have no adapters
+        self.slot_adapter = None
+        if any(lw.in_lora is not None or lw.out_lora is not None for lw in weights.layers):
+            if tp is not None or ep is not None or pp is not None:
+                raise ValueError("adapters are served by replicas of one GPU")
+            self.slot_adapter = torch.full((state_slots,), -1, dtype=torch.int32, device=weights.device)
+        self._rows = None  # adapter of each row of the pass that runs
         self.draft_index = None  # spec.ivf.IvfIndex: draft picks from a vocabulary shortlist instead of the full head
         self.w = weights
         self.cfg: ModelConfig = weights.config
@@ -247,17 +254,17 @@ class Model:
 
     def _attention(self, lw, kv_layer, h, batch: PackedBatch) -> torch.Tensor:
         cfg, ops = self.cfg, self.ops
-        qkv = ops.linear(h, lw.in_proj)
+        qkv = self._project(h, lw.in_proj, lw.in_lora)
         core = ops.attention(
             qkv, batch.positions, batch.seq_of_row, batch.block_tables, kv_layer, lw.q_norm, lw.k_norm,
             cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim, cfg.rotary_dim, cfg.rope_theta,
             cfg.rms_norm_eps, batch.G, **self._attention_spans(batch),
         )
-        return self._out_proj(core, lw.out_proj)
+        return self._out_proj(core, lw)
 
     def _gdn(self, lw, gi: int, h: torch.Tensor, batch: PackedBatch, ring) -> torch.Tensor:
         cfg, ops = self.cfg, self.ops
-        mixed = ops.linear(h, lw.in_proj)
+        mixed = self._project(h, lw.in_proj, lw.in_lora)
         args = (
             lw.conv_w, lw.A_log, lw.dt_bias, lw.gnorm_w, cfg.linear_num_key_heads, cfg.linear_num_value_heads,
             cfg.linear_key_head_dim, cfg.linear_value_head_dim, cfg.rms_norm_eps,
@@ -269,13 +276,17 @@ class Model:
             r = None if ring is None else (ring[0][gi], ring[1][gi])
             behind = {"behind_projection": True} if getattr(ops, "GDN_BEHIND_PROJECTION", False) else {}
             core = ops.gdn_decode(mixed, batch.slots, conv, rec, *args, G=batch.G, ring=r, **behind)
-        return self._out_proj(core, lw.out_proj)
+        return self._out_proj(core, lw)
 
-    def _out_proj(self, core: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
+    def _project(self, x: torch.Tensor, w: torch.Tensor, lora) -> torch.Tensor:
+        """A projection of the pass's rows, with the adapter of each row's own request beside it where the layer has adapters."""
+        return self.ops.linear(x, w) if lora is None else self.ops.lora_linear(x, w, lora, self._rows)
+
+    def _out_proj(self, core: torch.Tensor, lw: LayerWeights) -> torch.Tensor:
         """Mixer output projection; under tensor parallelism the GEMM's epilogue is the all-reduce."""
         if self.tp is None:
-            return self.ops.linear(core, w)
-        return self.tp.comm.gemm_allreduce(self.ops, core, w)
+            return self._project(core, lw.out_proj, lw.out_lora)
+        return self.tp.comm.gemm_allreduce(self.ops, core, lw.out_proj)
 
     def _moe_norm(self, lw: LayerWeights, h: torch.Tensor, res: torch.Tensor, norm_w: torch.Tensor):
         """MoE block, residual add and the RMSNorm that follows it (the next layer's input norm or the final norm);
@@ -386,6 +397,8 @@ class Model:
             if sp is not None:
                 return self._forward_sp(batch, sp)
         ops.DECODE_MODE = batch.G > 0  # decode / verify passes may split K across clusters; prefill never does
+        if self.slot_adapter is not None:
+            self._rows = self.slot_adapter[batch.slots.long()][batch.seq_of_row.long()]
         layers = self.w.layers
         pp = self.pp
         if pp is not None and not pp.is_first:

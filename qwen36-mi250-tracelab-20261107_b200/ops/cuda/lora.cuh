@@ -13,7 +13,7 @@
 
 namespace b200 {
 
-constexpr int LORA_MAX_RANK = 128;
+constexpr int LORA_MAX_RANK = 256;
 constexpr int LORA_MAX_ADAPTERS = 1024;
 
 struct NoLora {};

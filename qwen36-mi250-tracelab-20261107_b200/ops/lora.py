@@ -13,7 +13,7 @@ from typing import NamedTuple
 import torch
 
 RANK_STEP = 8  # ranks are multiples of it: rows of b are then whole 16-byte pieces
-MAX_RANK = 128
+MAX_RANK = 256
 MAX_ADAPTERS = 1024
 
 

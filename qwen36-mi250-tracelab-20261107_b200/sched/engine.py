@@ -17,6 +17,7 @@ greedy tokens identical to the same request served alone.
 
 from __future__ import annotations
 
+import hashlib
 import queue
 import time
 from typing import Iterable
@@ -24,7 +25,7 @@ from typing import Iterable
 import torch
 
 from ..cache.pools import OutOfCapacity, PagePool, SlotPool
-from ..cache.prefix import PrefixCache
+from ..cache.prefix import NO_SALT, PrefixCache
 from ..config import PAGE_SIZE, EngineConfig, ModelConfig
 from ..models.checkpoint import Weights
 from ..models.qwen36 import Model, PackedBatch
@@ -70,6 +71,14 @@ class Engine:
         c = self.cfg
         if c.kv_dtype not in KV_DTYPES:
             raise ValueError(f"kv_dtype {c.kv_dtype!r} is none of {', '.join(KV_DTYPES)}")
+        # Low-rank adapters: name -> number. They lie in the layers' weights, which ``attach_adapters`` may have done ahead of the engine.
+        self.adapters: dict[str, int] = {}
+        if c.adapters:
+            from ..models.lora import attach_adapters, parse_adapters
+
+            if tp is not None or ep is not None or pp is not None:
+                raise ValueError("adapters are served by replicas of one GPU")
+            self.adapters = {name: i for i, name in enumerate(attach_adapters(weights, parse_adapters(c.adapters)))}
         self.chunk = max(PAGE_SIZE, (c.prefill_chunk_tokens + PAGE_SIZE - 1) // PAGE_SIZE * PAGE_SIZE)
         self.max_model_len = c.max_model_len
         self.max_pages_per_seq = (self.max_model_len + PAGE_SIZE - 1) // PAGE_SIZE + 1
@@ -190,11 +199,12 @@ class Engine:
     def has_work(self) -> bool:
         return bool(self.waiting or self.prefilling or self.running or self._pending) or not self._inbox.empty()
 
-    def generate(self, prompts: Iterable[list[int]], sampling: Sampling | list[Sampling]) -> list[Generation]:
-        """Offline convenience: run the given prompts to completion and return their generations."""
+    def generate(self, prompts: Iterable[list[int]], sampling: Sampling | list[Sampling], adapters: list[str | None] | None = None) -> list[Generation]:
+        """Offline convenience: run the given prompts (with the adapters of these names, if any) to completion and return their generations."""
         prompts = list(prompts)
         samplings = sampling if isinstance(sampling, list) else [sampling] * len(prompts)
-        gens = [self.submit(Generation(p, s)) for p, s in zip(prompts, samplings)]
+        adapters = adapters or [None] * len(prompts)
+        gens = [self.submit(Generation(p, s, adapter=a)) for p, s, a in zip(prompts, samplings, adapters)]
         while any(not g.done for g in gens):
             self.step()
         return gens
@@ -227,7 +237,7 @@ class Engine:
 
     def _claim(self, gen: Generation) -> None:
         """Give the request a state slot and any cached prefix (reference: ``_claim``, generator.py:932-973)."""
-        entry = self.cache.lookup(gen.prompt)
+        entry = self.cache.lookup(gen.prompt, self._salt(gen))
         if entry is not None and entry.kind == "tail":
             gen.slot, gen.pages, gen.computed = entry.slot, list(entry.pages), entry.length
         elif entry is not None:
@@ -245,6 +255,8 @@ class Engine:
                 raise EngineError("all sequence slots are busy", 503, "service_unavailable") from None
             self.model.reset_slot(gen.slot)
             gen.pages, gen.computed = [], 0
+        if self.model.slot_adapter is not None:
+            self.model.slot_adapter[gen.slot] = -1 if gen.adapter is None else self.adapters[gen.adapter]
         gen.cached_tokens = gen.computed
         gen.mtp_computed = 0
         L = len(gen.prompt)
@@ -264,6 +276,10 @@ class Engine:
         if gen.sampling.seed is not None or not gen.sampling.greedy:
             gen.rng = torch.Generator(device="cpu")
             gen.rng.manual_seed(gen.sampling.seed if gen.sampling.seed is not None else gen.id * 7919)
+
+    def _salt(self, gen: Generation) -> bytes:
+        """What keeps the cached states of this request's adapter apart from the others'."""
+        return NO_SALT if gen.adapter is None else hashlib.blake2b(gen.adapter.encode(), digest_size=16, person=b"adapter").digest()
 
     def _poll_local(self) -> None:
         """Single-process mode: take new submissions and latch cancellations at the iteration boundary."""
@@ -291,6 +307,8 @@ class Engine:
                 continue
             try:
                 self.validate(gen.prompt, gen.sampling)
+                if gen.adapter is not None and gen.adapter not in self.adapters:
+                    raise EngineError(f"no adapter {gen.adapter!r} is served here", 404)
                 if gen.sampling.max_tokens == 0:
                     self._finish(gen, "length", retire=False)
                     continue
@@ -401,14 +419,14 @@ class Engine:
         return True
 
     def _snapshot(self, gen: Generation) -> None:
-        if self.cache.has_snapshot(gen.prompt, gen.computed):
+        if self.cache.has_snapshot(gen.prompt, gen.computed, self._salt(gen)):
             return
         try:
             slot = self.slots.alloc()
         except OutOfCapacity:
             return
         self.model.copy_slot(gen.slot, slot)
-        if not self.cache.store_snapshot(gen.prompt, gen.computed, gen.pages, slot):
+        if not self.cache.store_snapshot(gen.prompt, gen.computed, gen.pages, slot, self._salt(gen)):
             self.slots.release(slot)
 
     def _empty_pass(self) -> bool:
@@ -608,7 +626,7 @@ class Engine:
                 if len(g.pages) > keep:
                     self.pages.release(g.pages[keep:])
                     g.pages = g.pages[:keep]
-                self.cache.store_tail(covered, g.pages, g.slot)
+                self.cache.store_tail(covered, g.pages, g.slot, self._salt(g))
             else:
                 self.pages.release(g.pages)
                 self.slots.release(g.slot)

@@ -23,6 +23,7 @@ class Sampling:
     stop: list[str] = field(default_factory=list)
     ignore_eos: bool = False
     min_tokens: int = 0
+    min_p: float = 0.0  # least weight of a token, as a share of the likeliest one's
 
     @property
     def greedy(self) -> bool:
@@ -50,8 +51,10 @@ class TokenEvent:
 class Generation:
     """One request inside the engine."""
 
-    def __init__(self, prompt: list[int], sampling: Sampling, on_event: Callable[["Generation", TokenEvent], None] | None = None) -> None:
+    def __init__(self, prompt: list[int], sampling: Sampling, on_event: Callable[["Generation", TokenEvent], None] | None = None,
+                 adapter: str | None = None) -> None:
         self.id = next(_ids)
+        self.adapter = adapter  # name of the low-rank adapter that it runs with
         self.prompt = list(prompt)
         self.sampling = sampling
         self.on_event = on_event
