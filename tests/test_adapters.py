@@ -1,0 +1,215 @@
+"""Low-rank adapters: loading, serving several beside the shared weights, and what is refused."""
+
+import json
+
+import pytest
+import torch
+
+from adapter_util import merged, write_adapter
+from b200serve.config import EngineConfig, ModelConfig
+from b200serve.models.checkpoint import random_weights
+from b200serve.models.lora import attach_adapters, parse_adapters, read_adapter
+from b200serve.ops import torch_ops
+from b200serve.ops.lora import LoraWeights
+from b200serve.sched.engine import Engine
+from b200serve.sched.request import Sampling
+
+
+def _weights():
+    return random_weights(ModelConfig.tiny(), seed=0, dtype=torch.float32, std=0.05, lm_head_std=0.5)
+
+
+def _engine(weights, adapters="", **kw):
+    return Engine(weights, EngineConfig(max_model_len=1024, prefill_chunk_tokens=64, max_seqs=8, mtp=False, adapters=adapters, **kw))
+
+
+def _prompts(n, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randint(3, 1024, (int(torch.randint(16, 150, (1,), generator=g)),), generator=g).tolist() for _ in range(n)]
+
+
+@pytest.fixture(scope="module")
+def dirs(tmp_path_factory):
+    root, cfg = tmp_path_factory.mktemp("adapters"), ModelConfig.tiny()
+    parts = {"all": write_adapter(root / "all", cfg, 1), "narrow": write_adapter(root / "narrow", cfg, 2, r=3, alpha=3.0, only=("q_proj", "out_proj", "in_proj_z")),
+             "root": write_adapter(root / "root", cfg, 3, r=16, alpha=4.0, only=("v_proj", "o_proj", "in_proj_qkv"), use_rslora=True)}
+    return {n: str(root / n) for n in parts}, parts, {"all": 2.0, "narrow": 1.0, "root": 1.0}
+
+
+def test_the_operator_is_the_formula():
+    g = torch.Generator().manual_seed(0)
+    x, w = torch.randn(9, 24, generator=g), torch.randn(17, 24, generator=g)
+    ad = LoraWeights(torch.randn(3, 8, 24, generator=g), torch.randn(3, 17, 8, generator=g), torch.tensor([1.0, -2.0, 0.5]))
+    rows = torch.tensor([0, 1, 2, -1, 0, -5, 2, 1, 3], dtype=torch.int32)
+    got = torch_ops.lora_linear(x, w, ad, rows)
+    for t, i in enumerate(rows.tolist()):
+        want = w.double() @ x[t].double()
+        if 0 <= i < 3:
+            want = want + ad.scale[i].double() * ad.b[i].double() @ (ad.a[i].double() @ x[t].double())
+        # fp32 sums of 24 and 8 products: 40 roundings of 2^-24 of their magnitudes at most
+        assert (got[t].double() - want).abs().max() <= 40 * 2.0 ** -24 * (w.abs().sum(1).max() * x.abs().max() * (1 + 20))
+
+
+def test_adapters_together_are_their_merged_weights_alone(dirs):
+    """A batch of requests with different adapters and none: each gets the tokens of an engine whose weights have its adapter merged in."""
+    paths, parts, scale = dirs
+    eng = _engine(_weights(), ",".join(f"{n}={p}" for n, p in paths.items()))
+    assert eng.adapters == {"all": 0, "narrow": 1, "root": 2}
+    prompts, s = _prompts(8), Sampling(max_tokens=12, ignore_eos=True)
+    names = ["all", None, "narrow", "root", "all", None, "root", "narrow"]
+    together = eng.generate(prompts, s, adapters=names)
+    plain = _engine(_weights())
+    for name in (None, "all", "narrow", "root"):
+        alone = plain if name is None else _engine(merged(_weights(), parts[name], scale[name]))
+        mine = [i for i, n in enumerate(names) if n == name]
+        assert [together[i].output for i in mine] == [g.output for g in alone.generate([prompts[i] for i in mine], s)]
+    assert together[0].output != plain.generate([prompts[0]], s)[0].output  # (the adapter shows)
+
+
+def test_cached_prefixes_belong_to_their_adapter(dirs):
+    paths, _, _ = dirs
+    spec = ",".join(f"{n}={p}" for n, p in paths.items())
+    eng, s = _engine(_weights(), spec), Sampling(max_tokens=6, ignore_eos=True)
+    prompt = _prompts(1, 5)[0] + _prompts(1, 6)[0]
+    first = eng.generate([prompt], s, adapters=["all"])[0]
+    follow = prompt + first.output + [7, 8]
+    for name in (None, "narrow"):
+        other = eng.generate([follow], s, adapters=[name])[0]
+        assert other.cached_tokens == 0
+        assert other.output == _engine(_weights(), spec).generate([follow], s, adapters=[name])[0].output
+    again = eng.generate([follow], s, adapters=["all"])[0]
+    assert again.cached_tokens >= len(prompt)
+    cold = _engine(_weights(), spec).generate([follow], s, adapters=["all"])[0]
+    assert cold.cached_tokens == 0 and cold.output == again.output
+    assert eng.generate([follow + again.output], s)[0].output == _engine(_weights()).generate([follow + again.output], s)[0].output
+
+
+def test_a_slot_forgets_its_adapter(dirs):
+    """More requests than state slots: a slot's next sequence runs with its own adapter, or none."""
+    paths, _, _ = dirs
+    eng = _engine(_weights(), f"all={paths['all']}", prefix_cache_entries=0)
+    prompts, s = _prompts(12, 9), Sampling(max_tokens=5, ignore_eos=True)
+    names = [None if i % 3 else "all" for i in range(12)]
+    got = [g.output for g in eng.generate(prompts, s, adapters=names)]
+    plain = _engine(_weights())
+    for i in (1, 2, 10, 11):
+        assert got[i] == plain.generate([prompts[i]], s)[0].output
+
+
+def test_captured_pass_scheduling_with_adapters(dirs):
+    """The decode-graph scheduling (buckets, run-ahead), run without a CUDA device."""
+    paths, _, _ = dirs
+    spec = ",".join(f"{n}={p}" for n, p in paths.items())
+    prompts, s, names = _prompts(6, 3), Sampling(max_tokens=10, ignore_eos=True), ["all", None, "root", "narrow", None, "all"]
+    graphs = _engine(_weights(), spec, graphs_on_cpu=True, decode_buckets=(1, 4, 8))
+    got = [g.output for g in graphs.generate(prompts, s, adapters=names)]
+    assert graphs._graphs is not None and graphs._graphs.buckets and graphs.stats["ahead_steps"] > 0
+    assert got == [g.output for g in _engine(_weights(), spec, cuda_graphs=False).generate(prompts, s, adapters=names)]
+
+
+def test_speculation_with_adapters(dirs):
+    paths, _, _ = dirs
+    prompts, s, names = _prompts(4, 4), Sampling(max_tokens=10, ignore_eos=True), ["all", None, "all", None]
+    spec = Engine(_weights(), EngineConfig(max_model_len=1024, prefill_chunk_tokens=64, max_seqs=8, mtp=True, spec_k=2, adapters=f"all={paths['all']}"))
+    assert spec.spec is not None
+    assert [g.output for g in spec.generate(prompts, s, adapters=names)] == [
+        g.output for g in _engine(_weights(), f"all={paths['all']}").generate(prompts, s, adapters=names)]
+
+
+def test_refused_adapters(tmp_path, dirs):
+    cfg = ModelConfig.tiny()
+    ok = write_adapter(tmp_path / "ok", cfg, 0)
+    assert len(read_adapter(tmp_path / "ok", cfg).parts) == len(ok) > 0
+    with pytest.raises(ValueError, match="No such file"):
+        read_adapter(tmp_path / "nowhere", cfg)
+    for conf in ({"use_dora": True}, {"bias": "all"}, {"modules_to_save": ["lm_head"]}, {"rank_pattern": {"q_proj": 2}}, {"peft_type": "IA3"}, {"r": 5}):
+        write_adapter(tmp_path / "bad", cfg, 0, **{k: v for k, v in conf.items() if k != "r"})
+        if "r" in conf:
+            c = json.loads((tmp_path / "bad/adapter_config.json").read_text())
+            (tmp_path / "bad/adapter_config.json").write_text(json.dumps({**c, **conf}))
+        with pytest.raises(ValueError, match="adapter"):
+            read_adapter(tmp_path / "bad", cfg)
+    from safetensors.torch import load_file, save_file
+
+    good = load_file(str(tmp_path / "ok/adapter_model.safetensors"))
+    some = next(k for k in good if "lora_A" in k)
+    nan = good[some].clone()
+    nan[0, 0] = float("nan")
+    write_adapter(tmp_path / "odd", cfg, 0)
+    for state in ({}, {k: v for k, v in good.items() if k != some}, {**good, "base_model.model.lm_head.lora_A.weight": torch.zeros(4, 128)},
+                  {**good, some: nan}, {**good, some: good[some][:, 1:].contiguous()}, {some.replace("layers.0", "layers.9"): good[some]}):
+        save_file(state, str(tmp_path / "odd/adapter_model.safetensors"))
+        with pytest.raises(ValueError, match="adapter"):
+            read_adapter(tmp_path / "odd", cfg)
+    write_adapter(tmp_path / "big", cfg, 0, r=100)
+    with pytest.raises(ValueError, match="rank"):
+        attach_adapters(_weights(), {"big": tmp_path / "big"})
+    for spec in ("a", "=x", "a=", "a=x,a=y"):
+        with pytest.raises(ValueError, match="adapter"):
+            parse_adapters(spec)
+    assert parse_adapters(" a=x , b=/y=z,") == {"a": "x", "b": "/y=z"}
+
+
+def test_refused_requests_and_engines(dirs):
+    paths, _, _ = dirs
+    eng = _engine(_weights(), f"all={paths['all']}")
+    g = eng.generate([[5, 6, 7]], Sampling(max_tokens=3), adapters=["none"])[0]
+    assert g.finish_reason == "error" and g.output == []
+    assert eng.generate([[5, 6, 7]], Sampling(max_tokens=3, ignore_eos=True), adapters=["all"])[0].finish_reason == "length"
+    plain = _engine(_weights()).generate([[5, 6, 7]], Sampling(max_tokens=3), adapters=["all"])[0]
+    assert plain.finish_reason == "error"
+    with pytest.raises(ValueError, match="one GPU"):
+        Engine(_weights(), EngineConfig(max_model_len=256, max_seqs=2, mtp=False, adapters=f"all={paths['all']}"), tp=object())
+    ad = LoraWeights(torch.zeros(2, 8, 16), torch.zeros(2, 5, 8), torch.ones(2))
+    x, w, rows = torch.zeros(3, 16), torch.zeros(5, 16), torch.zeros(3, dtype=torch.int32)
+    for bad in (LoraWeights(ad.a[:1], ad.b, ad.scale), LoraWeights(ad.a[:, :7], ad.b[..., :7], ad.scale), LoraWeights(ad.a, ad.b, ad.scale.double()),
+                LoraWeights(ad.a, ad.b[:, :4], ad.scale), LoraWeights(ad.a, ad.b.bfloat16(), ad.scale), LoraWeights(ad.a[0], ad.b, ad.scale)):
+        with pytest.raises(ValueError, match="lora_linear"):
+            torch_ops.lora_linear(x, w, bad, rows)
+    from b200serve.ops import cuda_ops
+
+    with pytest.raises(ValueError, match="torch_ops"):
+        cuda_ops.lora_linear(x, w, ad, rows)
+
+
+def test_the_server_serves_adapters_as_models(dirs):
+    import threading
+
+    import requests
+
+    from b200serve.api.server import Server, Service
+
+    paths, _, _ = dirs
+    eng = _engine(_weights(), f"all={paths['all']}")
+    with pytest.raises(ValueError, match="adapter"):
+        Service(eng, None, "all")
+    from b200serve.api.tokenizer import TextCodec
+    from b200serve.models.tiny import build_tokenizer
+    import tempfile
+
+    with tempfile.TemporaryDirectory() as d:
+        build_tokenizer(512).save_pretrained(d)
+        service = Service(eng, TextCodec(d), "tiny")
+    server = Server(("127.0.0.1", 0), service)
+    threading.Thread(target=server.serve_forever, daemon=True).start()
+    url = f"http://127.0.0.1:{server.server_address[1]}"
+    try:
+        models = requests.get(url + "/v1/models", timeout=20).json()["data"]
+        assert [m["id"] for m in models] == ["tiny", "all"] and models[1]["parent"] == "tiny"
+        body = {"prompt": [9, 8, 7, 6], "max_tokens": 6, "temperature": 0, "ignore_eos": True, "return_token_ids": True}
+
+        def ask(model, **more):
+            return requests.post(url + "/v1/completions", json={**body, "model": model, **more}, timeout=60)
+
+        base, tuned = ask("tiny").json(), ask("all").json()
+        s = Sampling(max_tokens=6, ignore_eos=True)
+        assert tuned["model"] == "all" and base["model"] == "tiny"
+        assert base["choices"][0]["token_ids"] == _engine(_weights()).generate([[9, 8, 7, 6]], s)[0].output
+        assert tuned["choices"][0]["token_ids"] == _engine(_weights(), f"all={paths['all']}").generate([[9, 8, 7, 6]], s, adapters=["all"])[0].output
+        assert ask("other").status_code == 404
+        assert ask("all", temperature=0.8, min_p=0.2, seed=3).status_code == 200
+        for bad in (-0.1, 1.5, "x", True):
+            assert ask("tiny", min_p=bad).status_code == 400
+    finally:
+        server.shutdown()
+        service.worker.stop()

@@ -77,7 +77,7 @@ def test_shapes(C, T, N, K, dt):
     C.check_errors(x.device)
 
 
-@pytest.mark.parametrize("R", list(range(8, 129, 8)))
+@pytest.mark.parametrize("R", [*range(8, 129, 8), 136, 192, 200, 256])
 def test_ranks(C, R):
     N, K, L = 520, 256, 5
     w, ad = _bf(N, K, by=K ** -0.5, seed=1), _adapters(L, R, N, K, seed=R)
@@ -222,7 +222,7 @@ def test_refusals(C):
     wrong = [(x.float(), w, ad, rows), (x[:, :56], w, ad, rows), (x, w.float(), ad, rows), (x, w, ad, rows.long()), (x, w, ad, rows[:3]), (x, w, ad, rows.cpu()),
              (x, w, LoraWeights(a[:2], b, s), rows), (x, w, LoraWeights(a, b[:, :120], s), rows), (x, w, LoraWeights(a.float(), b.float(), s), rows),
              (x, w, LoraWeights(a[:, :12], b[..., :12], s), rows), (x, w, LoraWeights(a, b, s.double()), rows), (x, w, LoraWeights(a, b, s.cpu()), rows),
-             (x, w, LoraWeights(a.repeat(1, 9, 1), b.repeat(1, 1, 9), s), rows), (x, w, LoraWeights(a, b.transpose(1, 2).contiguous().transpose(1, 2), s), rows),
+             (x, w, LoraWeights(a.repeat(1, 17, 1), b.repeat(1, 1, 17), s), rows), (x, w, LoraWeights(a, b.transpose(1, 2).contiguous().transpose(1, 2), s), rows),
              (x.cpu(), w, ad, rows), (_bf(4, 65)[:, 1:], w, ad, rows), (_bf(4, 128)[:, ::2], w, ad, rows), (x, w, ad, _rows(8, 3)[::2])]
     for args in wrong:
         with pytest.raises(ValueError, match="lora_linear"):

@@ -54,3 +54,20 @@ def test_the_kernels_refuse_logits_of_the_host():
     f = torch.zeros(2)
     with pytest.raises(ValueError, match="torch_ops"):
         cuda_ops.sample(torch.zeros(2, 5), f, f.int(), f, f, f)
+
+
+def test_pick_tokens_takes_every_setting():
+    from b200serve.sched.request import Sampling
+    from b200serve.sched.sampling import pick_tokens
+
+    torch.manual_seed(0)
+    logits = torch.randn(1, 400) * 2
+    w = torch.softmax(logits[0].double() / 0.9, -1)
+    allowed = set((w >= 0.3 * w.max()).nonzero().view(-1).tolist())
+    g = torch.Generator().manual_seed(1)
+    got = {pick_tokens(logits, [Sampling(temperature=0.9, min_p=0.3, seed=0)], [g], [None])[0] for _ in range(200)}
+    assert got <= allowed and len(got) == len(allowed) > 1
+    # more ids to leave out than the operator takes by itself
+    order = logits[0].argsort(descending=True).tolist()
+    assert pick_tokens(logits, [Sampling()], [None], [set(order[:80])]) == [order[80]]
+    assert pick_tokens(logits[:, :3], [Sampling()], [None], [{0, 1, 2}]) == [0]
