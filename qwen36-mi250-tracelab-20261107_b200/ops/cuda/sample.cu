@@ -1074,10 +1074,6 @@ static int launch_sample(const SampleArgs& a, void* work, cudaStream_t st) {
 
 using namespace b200;
 
-extern "C" int b200_sample_max_exclude() { return SAMPLE_MAX_EXCLUDE; }
-extern "C" int b200_sample_max_rows() { return 65535; }
-extern "C" int b200_sample_max_vocab() { return SAMPLE_MAX_VOCAB; }
-
 extern "C" long long b200_sample_work_bytes(int n, int V) {
   SampleWork w;
   return V <= LIST ? 0 : static_cast<long long>(sample_work(n, V, nullptr, &w));
@@ -1087,7 +1083,7 @@ extern "C" int b200_sample(const void* logits, int type, long long stride, int n
                            const float* top_p, const float* min_p, const float* u, const int* exclude, int n_exclude, int64_t* out,
                            void* work, cudaStream_t st) {
   if (n <= 0) return 0;
-  if (V <= 0 || n_exclude < 0 || n_exclude > SAMPLE_MAX_EXCLUDE || V > SAMPLE_MAX_VOCAB || n > b200_sample_max_rows()) return -7;
+  if (V <= 0 || n_exclude < 0 || n_exclude > SAMPLE_MAX_EXCLUDE || V > SAMPLE_MAX_VOCAB || n > 65535) return -7;
   const SampleArgs a{logits, stride, n, V, temperature, top_k, top_p, min_p, u, exclude, n_exclude, out};
   switch (type) {
     case LOGIT_F32: return launch_sample<float>(a, work, st);

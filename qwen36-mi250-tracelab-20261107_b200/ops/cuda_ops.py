@@ -23,7 +23,7 @@ from ..obs import buildlog
 from . import torch_ops
 from .build import lib_path
 from .kv8 import Kv8Layer, check_layer
-from .lora import LoraWeights, check_weights
+from .lora import MAX_ADAPTERS, MAX_RANK, RANK_STEP, LoraWeights, check_weights
 from .spans import span_tables
 
 _lib = None
@@ -97,8 +97,6 @@ class _Sig:
     b200_kv8_prefill = [P, P, P, P, P, P, I, I, I, I, I, L, P, I, I, I, I, I, I, P, P, P, P, P]
     b200_lora_work_bytes = [I, I, I, I, I, I, I]
     b200_lora_linear = [P, I, P, I, I, P, P, P, P, P, I, I, I, I, I, I, I, P, P, P]
-    b200_sample_max_exclude = []
-    b200_sample_max_rows = []
     b200_sample_work_bytes = [I, I]
     b200_sample = [P, I, L, I, I, P, P, P, P, P, P, I, P, P, P]
     b200_kv8_decode = [P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, P, P, P, P, P]
@@ -291,53 +289,66 @@ def _lora_work(device: int, T: int, N: int, K: int, R: int, L: int, f32: bool, p
     return fn(T, N, K, R, L, f32, packed)
 
 
-def _lora_part(x, w, adapters, rows, out, n_own: int) -> None:
+def _lora_part(x, w, adapters, rows, out, T: int, N: int, K: int, R: int, L: int, n_own: int, packed: int, dev: torch.device) -> None:
     a, b, scale = adapters
-    (T, K), N, (L, R, _) = x.shape, w.shape[0], a.shape
-    dev, f32, packed = x.device, out.dtype == torch.float32, is_packed(w)
+    f32 = out.dtype is torch.float32
     size = _lora_work(dev.index, T, N, K, R, L, f32, packed)
     if size > LORA_WORK and T > 256:  # hundreds of adapters in a long pass: by parts of its rows
         half = (T // 2 + 255) // 256 * 256
-        for part in (slice(0, half), slice(half, T)):
-            _lora_part(x[part], w, adapters, rows[part], out[part], n_own)
+        for i, j in ((0, half), (half, T)):
+            _lora_part(x[i:j], w, adapters, rows[i:j], out[i:j], j - i, N, K, R, L, n_own, packed, dev)
         return
-    work = torch.empty(size, dtype=torch.uint8, device=dev)
+    work = rows.new_empty(size // 4)  # (an allocation like another's takes half the time of one that names type and device)
     _check(lib().b200_lora_linear(
         x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), packed, a.data_ptr(), b.data_ptr(), scale.data_ptr(), rows.data_ptr(), out.data_ptr(),
         f32, T, N, n_own, K, R, L, work.data_ptr(), _err_ptr(dev), _raw_stream(dev)), "lora_linear")
 
 
-def lora_linear(x: torch.Tensor, w: torch.Tensor, adapters: LoraWeights, rows: torch.Tensor, out_dtype: torch.dtype | None = None) -> torch.Tensor:
-    """``linear(x, w)`` with the low-rank adapter of each row's own request beside it (``ops/lora.py``): row ``t`` of ``x [T, K]`` uses adapter
-    ``rows[t]`` (int32 ``[T]``), none where that is negative. One rounding, to bf16 (default) or fp32. A row's bits depend on its own numbers and
-    adapter only, and are ``linear``'s for a row without one. An adapter number that is too large leaves the row without one, and is reported by
-    ``check_errors``. Only device tensors are touched, so the call can be captured in a CUDA graph."""
-    dev, f32 = x.device, out_dtype == torch.float32
+def _lora_refuse(x, w, adapters, rows, out_dtype) -> None:
+    """Say what is wrong with the arguments of ``lora_linear``."""
+    dev = x.device
     if not x.is_cuda:
         raise ValueError(f"lora_linear: the rows are on {dev}: torch_ops has the operator for them")
     if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1] or x.dtype != torch.bfloat16 or w.dtype != torch.bfloat16:
         raise ValueError(f"lora_linear: rows {tuple(x.shape)} {x.dtype} and weights {tuple(w.shape)} {w.dtype} are not bf16 [T, K] and [N, K]")
     if out_dtype not in (None, torch.bfloat16, torch.float32):
         raise ValueError(f"lora_linear: {out_dtype} outputs, bf16 and fp32 are there")
-    (T, K), N = x.shape, w.shape[0]
-    if adapters.b.dim() != 3 or not (N - 128 * is_packed(w) < adapters.b.shape[1] <= N or adapters.b.shape[1] == N):
+    N = w.shape[0]
+    if adapters.b.dim() != 3 or not N - 128 * is_packed(w) < adapters.b.shape[1] <= N and adapters.b.shape[1] != N:
         raise ValueError(f"lora_linear: adapters of {tuple(adapters.b.shape)} for {N} outputs")
-    n_own = adapters.b.shape[1]  # a packed weight has rows of zeros behind its own
-    L, R = check_weights(adapters, n_own, K, "lora_linear")
+    check_weights(adapters, adapters.b.shape[1], x.shape[1], "lora_linear")
     if adapters.a.dtype != torch.bfloat16:
         raise ValueError(f"lora_linear: adapters of {adapters.a.dtype}, not bf16")
-    if rows.shape != (T,) or rows.dtype != torch.int32 or not rows.is_contiguous():
-        raise ValueError(f"lora_linear: adapter numbers {tuple(rows.shape)} {rows.dtype} are not a contiguous int32 [{T}]")
+    if rows.shape != x.shape[:1] or rows.dtype != torch.int32 or not rows.is_contiguous():
+        raise ValueError(f"lora_linear: adapter numbers {tuple(rows.shape)} {rows.dtype} are not a contiguous int32 [{x.shape[0]}]")
     if w.device != dev or adapters.a.device != dev or rows.device != dev:
         raise ValueError(f"lora_linear: rows on {dev}, weights on {w.device}, adapters on {adapters.a.device}, their numbers on {rows.device}")
-    if K % 8 or x.stride(1) != 1 or w.stride(1) != 1 or x.stride(0) % 8 or w.stride(0) % 8 \
-            or (x.data_ptr() | w.data_ptr() | adapters.a.data_ptr() | adapters.b.data_ptr()) % 16:
-        raise ValueError(f"lora_linear: rows of {K} numbers with strides {x.stride()}, weights with strides {w.stride()}: rows, weights and adapters are "
-                         "whole 16-byte pieces on 16-byte boundaries")
-    out = torch.empty(T, N, dtype=torch.float32 if f32 else torch.bfloat16, device=dev)
-    if T == 0:
-        return out
-    _lora_part(x, w, adapters, rows, out, n_own)
+    raise ValueError(f"lora_linear: rows of {x.shape[1]} numbers with strides {x.stride()}, weights with strides {w.stride()}: rows, weights and adapters "
+                     "are whole 16-byte pieces on 16-byte boundaries")
+
+
+def lora_linear(x: torch.Tensor, w: torch.Tensor, adapters: LoraWeights, rows: torch.Tensor, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``linear(x, w)`` with the low-rank adapter of each row's own request beside it (``ops/lora.py``): row ``t`` of ``x [T, K]`` uses adapter
+    ``rows[t]`` (int32 ``[T]``), none where that is negative. One rounding, to bf16 (default) or fp32. A row's bits depend on its own numbers and
+    adapter only, and are ``linear``'s (without a split K) for a row without one. An adapter number that is too large leaves the row without one, and is
+    reported by ``check_errors``. Only device tensors are touched, so the call can be captured in a CUDA graph."""
+    a, b, scale = adapters
+    (xs, ws, sa, sb), d, packed = (x.shape, w.shape, a.shape, b.shape), x.get_device(), is_packed(w)
+    bf = torch.bfloat16
+    # (one condition: a call at decode size takes less time on the GPU than its arguments' attributes here)
+    if not (d >= 0 and len(xs) == 2 and len(ws) == 2 and len(sa) == 3 and len(sb) == 3 and x.dtype is bf and w.dtype is bf and a.dtype is bf and b.dtype is bf
+            and scale.dtype is torch.float32 and rows.dtype is torch.int32 and ws[1] == xs[1] == sa[2] and sa[0] == sb[0] and sa[1] == sb[2]
+            and scale.shape == sa[:1] and rows.shape == xs[:1] and (sb[1] == ws[0] or packed and ws[0] - 128 < sb[1] < ws[0])
+            and 1 <= sa[0] <= MAX_ADAPTERS and RANK_STEP <= sa[1] <= MAX_RANK and sa[1] % RANK_STEP == 0
+            and w.get_device() == d and a.get_device() == d and b.get_device() == d and scale.get_device() == d and rows.get_device() == d
+            and a.is_contiguous() and b.is_contiguous() and scale.is_contiguous() and rows.is_contiguous()
+            and (out_dtype is None or out_dtype is bf or out_dtype is torch.float32) and xs[1] % 8 == 0 and x.stride(1) == 1 and w.stride(1) == 1
+            and x.stride(0) % 8 == 0 and w.stride(0) % 8 == 0 and (x.data_ptr() | w.data_ptr() | a.data_ptr() | b.data_ptr()) % 16 == 0):
+        _lora_refuse(x, w, adapters, rows, out_dtype)
+    T, N = xs[0], ws[0]
+    out = (scale if out_dtype is torch.float32 else x).new_empty(T, N)
+    if T:
+        _lora_part(x, w, adapters, rows, out, T, N, xs[1], sa[1], sa[0], sb[1], packed, x.device)
     return out
 
 
@@ -1076,6 +1087,7 @@ def _kv8_attention(qkv, positions, seq_of_row, block_tables, layer, q_norm, k_no
 # --------------------------------------------------------------------------- sampling
 SAMPLE_ROWS = 4096  # of one launch
 SAMPLE_VOCAB = 1 << 22
+SAMPLE_EXCLUDED = 64  # most excluded ids of a row
 
 
 @functools.cache
@@ -1094,32 +1106,25 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor,
     rules. A row's own settings: ``temperature``, ``top_p``, ``min_p``, ``u`` fp32 ``[n]`` and ``top_k`` int32 ``[n]``; ``exclude [n, m]`` int32, at
     most 64 ids per row. A row's pick depends on its own logits and settings only. ``out`` (int64 ``[n]``, contiguous) receives the picks in place of
     a new tensor. Only device tensors are touched, so the call can be captured in a CUDA graph."""
-    shape = logits.shape
+    shape, d = logits.shape, logits.get_device()
+    n, m = shape[0] if len(shape) else -1, 0 if exclude is None else exclude.shape[-1]
+    f32 = torch.float32
     kind = LOGIT_TYPES.get(logits.dtype)
-    if not logits.is_cuda:
-        raise ValueError(f"sample: the logits are on {logits.device}: torch_ops has the operator for them")
-    if len(shape) != 2 or kind is None or not 1 <= shape[1] <= SAMPLE_VOCAB:
-        raise ValueError(f"sample: logits {tuple(shape)} {logits.dtype} are not fp32, bf16 or fp16 [rows, 1 to {SAMPLE_VOCAB} tokens]")
-    n, V = shape
+    # (one condition: a row takes less time on the GPU than its arguments' attributes here)
+    if not (d >= 0 and len(shape) == 2 and kind is not None and 1 <= shape[1] <= SAMPLE_VOCAB
+            and temperature.dtype is f32 and top_p.dtype is f32 and min_p.dtype is f32 and u.dtype is f32 and top_k.dtype is torch.int32
+            and temperature.shape == top_p.shape == min_p.shape == u.shape == top_k.shape == shape[:1]
+            and temperature.get_device() == d and top_p.get_device() == d and min_p.get_device() == d and u.get_device() == d and top_k.get_device() == d
+            and temperature.is_contiguous() and top_p.is_contiguous() and min_p.is_contiguous() and u.is_contiguous() and top_k.is_contiguous()
+            and (exclude is None or exclude.dtype is torch.int32 and exclude.shape == (n, m) and m <= SAMPLE_EXCLUDED and exclude.get_device() == d
+                 and exclude.is_contiguous())
+            and (out is None or out.dtype is torch.int64 and out.shape == shape[:1] and out.get_device() == d and out.is_contiguous())):
+        _sample_refuse(logits, temperature, top_k, top_p, min_p, u, exclude, out)
     dev = logits.device
-    for name, t, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
-                           ("min_p", min_p, torch.float32), ("u", u, torch.float32)):
-        if t.shape != (n,) or t.dtype is not dtype or t.device != dev or not t.is_contiguous():
-            raise ValueError(f"sample: {name} {tuple(t.shape)} {t.dtype} with strides {t.stride()} on {t.device} is not a contiguous {dtype} [{n}] on {dev}")
-    m = 0
-    if exclude is not None:
-        m = exclude.shape[1] if exclude.dim() == 2 else -1
-        if exclude.shape != (n, m) or exclude.dtype is not torch.int32 or exclude.device != dev or not exclude.is_contiguous():
-            raise ValueError(f"sample: exclude {tuple(exclude.shape)} {exclude.dtype} on {exclude.device} is not a contiguous int32 [{n}, ids] on {dev}")
-        if m > lib().b200_sample_max_exclude():
-            raise ValueError(f"sample: {m} excluded ids per row, at most {lib().b200_sample_max_exclude()}")
     if out is None:
         out = torch.empty(n, dtype=torch.int64, device=dev)
-    elif out.shape != (n,) or out.dtype is not torch.int64 or out.device != dev or not out.is_contiguous():
-        raise ValueError(f"sample: out {tuple(out.shape)} {out.dtype} on {out.device} is not a contiguous int64 [{n}] on {dev}")
     if n == 0:
         return out
-    _err_ptr(dev)  # refuses tensors of another device than the current one
     if logits.stride(1) != 1:
         logits = logits.contiguous()
     if n > SAMPLE_ROWS:  # parts of the rows, each with a workspace of its own
@@ -1127,12 +1132,32 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor,
             j = slice(i, i + SAMPLE_ROWS)
             sample(logits[j], temperature[j], top_k[j], top_p[j], min_p[j], u[j], None if exclude is None else exclude[j], out[j])
         return out
-    size = _sample_work(n, V)
-    work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    _err_ptr(dev)  # refuses tensors of another device than the current one
+    size = _sample_work(n, shape[1])
+    work = top_k.new_empty(size // 4) if size else None  # (an allocation like another's takes half the time of one that names type and device)
     _check(lib().b200_sample(
-        logits.data_ptr(), kind, logits.stride(0), n, V, temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(), min_p.data_ptr(),
+        logits.data_ptr(), kind, logits.stride(0), n, shape[1], temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(), min_p.data_ptr(),
         u.data_ptr(), exclude.data_ptr() if m else None, m, out.data_ptr(), _ptr(work), _raw_stream(dev)), "sample")
     return out
+
+
+def _sample_refuse(logits, temperature, top_k, top_p, min_p, u, exclude, out) -> None:
+    """Say what is wrong with the arguments of ``sample``."""
+    shape, dev = logits.shape, logits.device
+    if not logits.is_cuda:
+        raise ValueError(f"sample: the logits are on {dev}: torch_ops has the operator for them")
+    if len(shape) != 2 or logits.dtype not in LOGIT_TYPES or not 1 <= shape[1] <= SAMPLE_VOCAB:
+        raise ValueError(f"sample: logits {tuple(shape)} {logits.dtype} are not fp32, bf16 or fp16 [rows, 1 to {SAMPLE_VOCAB} tokens]")
+    n = shape[0]
+    for name, t, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
+                           ("min_p", min_p, torch.float32), ("u", u, torch.float32)):
+        if t.shape != (n,) or t.dtype is not dtype or t.device != dev or not t.is_contiguous():
+            raise ValueError(f"sample: {name} {tuple(t.shape)} {t.dtype} with strides {t.stride()} on {t.device} is not a contiguous {dtype} [{n}] on {dev}")
+    if exclude is not None and (exclude.dim() != 2 or exclude.shape[0] != n or exclude.dtype is not torch.int32 or exclude.device != dev
+                                or not exclude.is_contiguous() or exclude.shape[1] > SAMPLE_EXCLUDED):
+        raise ValueError(f"sample: exclude {tuple(exclude.shape)} {exclude.dtype} on {exclude.device} is not a contiguous int32 [{n}, up to "
+                         f"{SAMPLE_EXCLUDED} ids] on {dev}")
+    raise ValueError(f"sample: out {tuple(out.shape)} {out.dtype} on {out.device} is not a contiguous int64 [{n}] on {dev}")
 
 
 def argmax_rows(logits: torch.Tensor) -> torch.Tensor:
