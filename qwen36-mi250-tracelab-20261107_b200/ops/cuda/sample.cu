@@ -35,7 +35,8 @@ struct SampleArgs {
 
 // What a row's launches tell each other.
 struct SamplePlan {
-  double step;              // 32 log2 of a logit's weight beside `ref` is (logit - ref) * step
+  double tail_by;           // the tail's sum in fp32 times this is its weight beside `ref`
+  float slope, zero;        // log2 of a logit's weight: logit * slope - zero
   float reach, least, ref;  // threshold of the list; below `least` a token has no weight; what the tail's weights are relative to
   float low;                // the sample's smallest
   int skip, with_tail;      // the list cannot decide this row; the others' weights are summed up
@@ -104,31 +105,28 @@ constexpr int LIST_BINS = 1024;
 constexpr int LIST_BIN_MOST = 96;  // tokens of a bin that are compared each with each
 
 struct Order {
-  uint64_t item[LIST], other[LIST];
+  uint64_t item[LIST];
+  union {
+    uint64_t other[LIST];
+    double sum[LIST];  // of the weights of the ordered list, up to and with each
+  };
+  uint16_t at[LIST];
   uint32_t bins[LIST_BINS], warp_count[32];
 };
 
 // Puts s.item[0 .. c) into descending order: bins by value, in a bin each is compared with each. `hi` and `lo`: about where the values lie.
-// Many equal values are sorted by exchanges instead, which take 66 rounds for a full list. All threads of the CTA.
+// Many equal values are sorted by exchanges instead, which take 66 rounds for a full list. All threads of the CTA. A row's list is put in order once, so
+// this and what follows is short code and not unrolled: 166 tokens took 11,000 cycles unrolled eight times, nearly all of them for instructions.
 template <int THREADS>
 __device__ void order_list(Order& s, int c, float hi, float lo) {
-  constexpr int PER = LIST / THREADS, BINS = LIST_BINS / THREADS;
+  constexpr int BINS = LIST_BINS / THREADS;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const float scale = hi > lo ? fminf(LIST_BINS / (hi - lo), 1e30f) : 0.f;
-#pragma unroll
-  for (int j = 0; j < BINS; ++j) s.bins[tid * BINS + j] = 0;
+  const auto bin_of = [&](uint64_t comp) { return min(LIST_BINS - 1, max(0, static_cast<int>((hi - comp_value(comp)) * scale))); };
+  for (int b = tid; b < LIST_BINS; b += THREADS) s.bins[b] = 0;
   __syncthreads();
-  uint64_t mine[PER];
-  uint32_t bin[PER], at[PER];
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const int i = tid + j * THREADS;
-    if (i < c) {
-      mine[j] = s.item[i];
-      bin[j] = min(LIST_BINS - 1, max(0, static_cast<int>((hi - comp_value(mine[j])) * scale)));
-      at[j] = atomicAdd(&s.bins[bin[j]], 1u);
-    }
-  }
+#pragma unroll 1
+  for (int i = tid; i < c; i += THREADS) s.at[i] = static_cast<uint16_t>(atomicAdd(&s.bins[bin_of(s.item[i])], 1u));
   __syncthreads();
   uint32_t own[BINS], most = 0, up = 0;
 #pragma unroll
@@ -146,23 +144,24 @@ __device__ void order_list(Order& s, int c, float hi, float lo) {
     sort_down<THREADS>(s.item, size);
     return;
   }
+#pragma unroll 1
   for (int w = 0; w < warp; ++w) up += s.warp_count[w];
   up -= sum;
 #pragma unroll
   for (int j = 0; j < BINS; ++j) { s.bins[tid * BINS + j] = up; up += own[j]; }  // where a bin starts
   __syncthreads();
-#pragma unroll
-  for (int j = 0; j < PER; ++j)
-    if (tid + j * THREADS < c) s.other[s.bins[bin[j]] + at[j]] = mine[j];
+#pragma unroll 1
+  for (int i = tid; i < c; i += THREADS) s.other[s.bins[bin_of(s.item[i])] + s.at[i]] = s.item[i];
   __syncthreads();
-#pragma unroll
-  for (int j = 0; j < PER; ++j)
-    if (tid + j * THREADS < c) {
-      const uint32_t from = s.bins[bin[j]], to = bin[j] + 1 < LIST_BINS ? s.bins[bin[j] + 1] : static_cast<uint32_t>(c);
-      uint32_t above = from;
-      for (uint32_t i = from; i < to; ++i) above += s.other[i] > mine[j];
-      s.item[above] = mine[j];
-    }
+#pragma unroll 1
+  for (int i = tid; i < c; i += THREADS) {
+    const uint64_t mine = s.other[i];
+    const int b = bin_of(mine);
+    const uint32_t from = s.bins[b], to = b + 1 < LIST_BINS ? s.bins[b + 1] : static_cast<uint32_t>(c);
+    uint32_t above = from;
+    for (uint32_t k = from; k < to; ++k) above += s.other[k] > mine;
+    s.item[above] = mine;
+  }
   __syncthreads();
 }
 
@@ -641,8 +640,7 @@ __global__ void __launch_bounds__(WIDE_THREADS) sample_wide_kernel(SampleArgs a,
 // Sums are added up in an order that goes by V alone: the weights of a lane's tokens of a task, the lanes of a warp, the tasks of a row.
 constexpr int PLAN_THREADS = 512, PLAN_PER = 32, PLAN_SAMPLE = PLAN_THREADS * PLAN_PER, PLAN_BLOCK = 256, PLAN_BINS = 1024;
 constexpr int STREAM_THREADS = 256, STREAM_WARPS = STREAM_THREADS / 32;
-constexpr int TASK = 1024;          // tokens that a warp takes at a time
-constexpr int LIST_PER = LIST / STREAM_THREADS;
+constexpr int TASK = 1024;          // tokens that a warp adds up by itself, in two halves
 constexpr int LIST_K = 1024;        // top-k up to which a list is expected to hold the k tokens
 
 // What a list is made to hold: all of the k, with room for the guess's error (one part in sqrt(want * 16384 / V)), or as many as leave room above.
@@ -690,13 +688,18 @@ __device__ __forceinline__ double sum_before(double v, double* warp_sum) {
 struct ListShared {
   Order list;
   double warp_sum[STREAM_WARPS];
-  double total, cut;
+  double total;
   int place, last;
 };
 
-// The pick of a row from its `c` largest tokens in s.item (unsorted) and the weight `tail` of all others, relative to `ref`; all: there
-// are no others of any weight. -2 where the tokens do not decide it. All threads of a CTA of STREAM_THREADS.
-__device__ int pick_from_list(ListShared& s, int c, const RowAsk& r, double tail, float ref, bool all, float hi, float lo) {
+// By how much a tail's sum in fp32 may be off, as a share of it. A token's weight is 2^y, y = logit * slope - zero: slope and y are rounded (2^-24 of y
+// each, times ln 2 in the weight), 2^y is off by 2^-21 of itself, eight additions by 2^-24 each: (1.4 |y| + 8 + 8) 2^-24. Tokens with y below -40 add up to
+// less than 2^22 2^-40, so what they are off by is within the 2^-30 that is added; |y| of 40 gives 72 2^-24, 75 is taken for the sums that follow.
+constexpr double TAIL_OFF = 75 * 0x1p-24;
+
+// The pick of a row from its `c` largest tokens in s.list (unsorted) and the weight of all others, within `off` of `tail`, relative to `ref`; all: there
+// are no others of any weight. -2 where that does not decide it. All threads of a CTA of STREAM_THREADS.
+__device__ int pick_from_list(ListShared& s, int c, const RowAsk& r, double tail, double off, float ref, bool all, float hi, float lo) {
   const int tid = threadIdx.x;
   if (c == 0) return ref == -INFINITY && all ? -1 : -2;
   order_list<STREAM_THREADS>(s.list, c, hi, lo);
@@ -704,34 +707,43 @@ __device__ int pick_from_list(ListShared& s, int c, const RowAsk& r, double tail
   const float m = comp_value(s.list.item[0]);
   // what weighs nothing beside `ref` weighs nothing beside m as well, unless m lies far below (an excluded token is the largest)
   if ((static_cast<double>(ref) - static_cast<double>(m)) * r.inv_t > WIDE_RANGE / 4) return -2;
-  if (tail > 0.0) tail *= ref == m ? 1.0 : exp((static_cast<double>(ref) - static_cast<double>(m)) * r.inv_t);
-  else all = all || !r.cut_k;  // (a row with a top-k has no tail summed up)
+  if (tail > 0.0 && ref != m) {
+    const double by = exp((static_cast<double>(ref) - static_cast<double>(m)) * r.inv_t);
+    tail *= by;
+    off *= by;
+  }
   if (!(tail < 1e300)) return -2;
   if (r.cut_k && c < r.k && !all) return -2;
   const int nk = r.cut_k ? min(r.k, c) : c;
   const bool closed = r.cut_k || all;  // no token outside the list is in play
 
-  double cum[LIST_PER];
   int positive = 0, enough = 0;
-#pragma unroll
-  for (int j = 0; j < LIST_PER; ++j) {
-    const int i = tid * LIST_PER + j;
-    const double w = i < nk ? weight_of(comp_value(s.list.item[i]), m, r.inv_t) : 0.0;
+#pragma unroll 1
+  for (int i = tid; i < nk; i += STREAM_THREADS) {
+    const double w = weight_of(comp_value(s.list.item[i]), m, r.inv_t);
     positive += w > 0.0;
-    enough += w >= r.least && i < nk;
-    cum[j] = w + (j ? cum[j - 1] : 0.0);
+    enough += w >= r.least;
+    s.list.sum[i] = w;
   }
-  const double before = sum_before<STREAM_THREADS>(cum[LIST_PER - 1], s.warp_sum);
-#pragma unroll
-  for (int j = 0; j < LIST_PER; ++j) cum[j] += before;
   if (tid == 0) { s.place = s.last = 0; }
-  if (tid == STREAM_THREADS - 1) s.total = cum[LIST_PER - 1] + (closed ? 0.0 : tail);
   __syncthreads();
+  const int per = (nk + STREAM_THREADS - 1) / STREAM_THREADS, from = min(nk, tid * per), to = min(nk, from + per);
+  double sum = 0.0;
+#pragma unroll 1
+  for (int i = from; i < to; ++i) { sum += s.list.sum[i]; s.list.sum[i] = sum; }
+  const double before = sum_before<STREAM_THREADS>(sum, s.warp_sum);
+#pragma unroll 1
+  for (int i = from; i < to; ++i) s.list.sum[i] += before;
   for (int o = 16; o; o >>= 1) { positive += __shfl_xor_sync(0xffffffffu, positive, o); enough += __shfl_xor_sync(0xffffffffu, enough, o); }
   if ((tid & 31) == 0) { atomicAdd(&s.place, positive); atomicAdd(&s.last, enough); }
   __syncthreads();
   positive = s.place; enough = max(1, s.last);
-  const double sum = s.total;
+  // the weight that top-p goes by, and then that of the kept, lies between these
+  double least_sum = s.list.sum[nk - 1], most_sum = least_sum;
+  if (!closed) {
+    least_sum += fmax(tail - off, 0.0);
+    most_sum += tail + off;
+  }
   constexpr int OPEN = 1 << 30;
   int limit = closed ? nk : OPEN;
   // the first place with more than `target` up to it, OPEN if there is none
@@ -739,44 +751,30 @@ __device__ int pick_from_list(ListShared& s, int c, const RowAsk& r, double tail
     __syncthreads();
     if (tid == 0) s.place = OPEN;
     __syncthreads();
-    int at = OPEN;
-#pragma unroll
-    for (int j = LIST_PER - 1; j >= 0; --j)
-      if (cum[j] > target && tid * LIST_PER + j < nk) at = tid * LIST_PER + j;
-    if (at != OPEN) atomicMin(&s.place, at);
+#pragma unroll 1
+    for (int i = tid; i < nk; i += STREAM_THREADS)
+      if (s.list.sum[i] > target && !(i > 0 && s.list.sum[i - 1] > target)) atomicMin(&s.place, i);
     __syncthreads();
     return s.place;
   };
-  double rest = 0.0;  // where the nucleus ends in the tail, its weight is between p * sum and one token's more
   if (r.p < 1.0) {
-    const int at = find(r.p * sum);
-    if (at != OPEN) limit = at + 1;
-    else if (!closed) {
-      rest = weight_of(comp_value(s.list.item[c - 1]), m, r.inv_t);
-      if (!(rest > 0.0)) return -2;
+    const int at = find(r.p * least_sum);
+    if (!closed && at != find(r.p * most_sum)) return -2;
+    if (at != OPEN) {
+      limit = at + 1;
+    } else if (!closed) {  // the nucleus ends in the tail: its weight is p of the sum and up to one token's more
+      least_sum *= r.p;
+      most_sum = r.p * most_sum + weight_of(comp_value(s.list.item[c - 1]), m, r.inv_t);
     }
   }
   if (r.least > 0.0) {
     if (enough < nk || closed) limit = min(limit, enough);
     else if (limit == OPEN) return -2;
   }
-  double total = sum;
-  if (limit != OPEN) {
-    __syncthreads();
-    const int j = limit - 1 - tid * LIST_PER;
-#pragma unroll
-    for (int i = 0; i < LIST_PER; ++i)
-      if (i == j) s.cut = cum[i];
-    __syncthreads();
-    total = s.cut;
-  } else if (rest > 0.0) {
-    total = r.p * sum;
-  }
-  const int at = find(r.u * total);
-  if (limit == OPEN && rest > 0.0 && at != find(r.u * (total + rest) * (1.0 + 0x1p-40))) return -2;
-  if (at < limit && at != OPEN) return comp_id(s.list.item[at]);
-  if (limit == OPEN) return -2;
-  return comp_id(s.list.item[max(0, min(limit, positive) - 1)]);
+  if (limit != OPEN) least_sum = most_sum = s.list.sum[limit - 1];
+  const int at = find(r.u * least_sum);
+  if (limit == OPEN) return at != OPEN && at == find(r.u * most_sum * (1.0 + 0x1p-40)) ? comp_id(s.list.item[at]) : -2;
+  return comp_id(s.list.item[at < limit ? at : max(0, min(limit, positive) - 1)]);
 }
 
 template <typename T>
@@ -826,6 +824,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) sample_plan_kernel(SampleArgs a,
   // the bin in which the sample has its share of `want`
   const int want = list_want(ask.greedy, ask.cut_k ? ask.k : 0);
   const uint32_t share = max(1u, static_cast<uint32_t>(static_cast<long long>(want) * min(V, PLAN_SAMPLE) / V));
+  static_assert(PLAN_BINS == 2 * PLAN_THREADS, "two bins for each thread");
   const uint32_t c0 = bins[2 * tid], c1 = bins[2 * tid + 1];
   uint32_t up = c0 + c1;
   for (int o = 1; o < 32; o <<= 1) {
@@ -847,19 +846,31 @@ __global__ void __launch_bounds__(PLAN_THREADS) sample_plan_kernel(SampleArgs a,
     plan.ref = top;
     plan.low = low;
     plan.top = 0;
-    plan.step = ask.inv_t * STEPS;
+    const double slope = ask.inv_t * 1.4426950408889634;  // 1 / ln 2
+    plan.slope = static_cast<float>(slope);
+    plan.zero = top * plan.slope;
+    plan.tail_by = exp2(static_cast<double>(plan.zero) - static_cast<double>(top) * plan.slope);
     plan.with_tail = !ask.greedy && !ask.cut_k && plan.reach > plan.least;
     plan.listed = 0;
     plan.done = 0;
-    plan.skip = (ask.cut_k && ask.k > LIST_K && reach > least) || t > 1e30f;  // (at such a temperature even a token of `least` weighs something)
+    // (at a huge temperature even a token of `least` weighs something; at |zero| of 2^20 fp32 does not tell weights apart)
+    plan.skip = (ask.cut_k && ask.k > LIST_K && reach > least) || t > 1e30f || (plan.with_tail && !(fabsf(plan.zero) < 0x1p20f));
     w.plan[at] = plan;
   }
 }
 
-// The logits of a lane in a task, from `row` on: piece i of 16 bytes holds tokens first + i * 32 * VE ..
+__device__ __forceinline__ float exp2_fast(float y) {  // off by 2^-21 of the result at most
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y));
+  return r;
+}
+
+constexpr int HALF = TASK / 2;
+
+// The logits of a lane in half a task, from `row` on: piece i of 16 bytes holds tokens first + i * 32 * VE ..
 template <typename T>
-struct TaskLogits {
-  static constexpr int VE = 16 / sizeof(T), PIECES = TASK / (32 * VE);
+struct HalfLogits {
+  static constexpr int VE = 16 / sizeof(T), PIECES = HALF / (32 * VE);
   static __device__ __forceinline__ int id(int first, int e) { return first + e / VE * (32 * VE) + e % VE; }
   uint4 raw[PIECES];
   __device__ __forceinline__ void load(const T* row, int first, int V, bool aligned) {
@@ -898,8 +909,8 @@ struct TaskLogits {
 
 // CTA x of a row takes `tasks_per_warp` tasks for each warp, from task x * STREAM_WARPS * tasks_per_warp on.
 template <typename T>
-__global__ void __launch_bounds__(STREAM_THREADS, 3) sample_stream_kernel(SampleArgs a, SampleWork w, int tasks, int tasks_per_warp) {
-  using Task = TaskLogits<T>;
+__global__ void __launch_bounds__(STREAM_THREADS, 4) sample_stream_kernel(SampleArgs a, SampleWork w, int tasks, int tasks_per_warp) {
+  using Half = HalfLogits<T>;
   __shared__ ListShared s;
   __shared__ int banned[SAMPLE_MAX_EXCLUDE];
   __shared__ int n_banned;
@@ -909,8 +920,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, 3) sample_stream_kernel(Sample
   pdl_wait();
   pdl_launch();
   SamplePlan& plan = w.plan[at];
-  const ExpLanes exps(w.powers[lane]);
-  const double step = plan.step, from = plan.ref;
+  const float slope = plan.slope, zero = plan.zero;
   const bool with_tail = plan.with_tail;
   if (plan.skip) {
     if (blockIdx.x == 0 && tid == 0) w.left_rows[atomicAdd(w.left, 1)] = at;
@@ -920,57 +930,61 @@ __global__ void __launch_bounds__(STREAM_THREADS, 3) sample_stream_kernel(Sample
   const T* row = static_cast<const T*>(a.logits) + at * a.stride;
   const bool aligned = (reinterpret_cast<uintptr_t>(row) & 15) == 0;
   const int task0 = blockIdx.x * STREAM_WARPS * tasks_per_warp;
+  if (tid == 0) s.place = 0;  // tokens of this CTA's list
   for (int j = tid; j < a.n_exclude; j += STREAM_THREADS) {
     const int id = a.exclude[static_cast<long long>(at) * a.n_exclude + j];
     if (id >= task0 * TASK && id < min(V, (task0 + STREAM_WARPS * tasks_per_warp) * TASK)) banned[atomicAdd(&n_banned, 1)] = id;
   }
-  if (a.n_exclude) __syncthreads();
+  __syncthreads();
   const int bans = n_banned;
   uint64_t* list = w.list + static_cast<size_t>(at) * LIST;
 
-  for (int i = 0; i < tasks_per_warp; ++i) {
-    const int task = task0 + i * STREAM_WARPS + warp;
-    if (task >= tasks) break;
-    const int first = task * TASK + lane * Task::VE;
-    Task x;
-    x.load(row, first, V, aligned);
+  // the next half is on its way while this one is looked at
+  const int mine = max(0, min(tasks_per_warp, (tasks - task0 - warp + STREAM_WARPS - 1) / STREAM_WARPS));  // tasks of this warp
+  const auto first_of = [&](int half) { return (task0 + (half >> 1) * STREAM_WARPS + warp) * TASK + (half & 1) * HALF + lane * Half::VE; };
+  int* ids = reinterpret_cast<int*>(s.list.item);  // of the tokens for the list
+  Half next;
+  if (mine > 0) next.load(row, first_of(0), V, aligned);
+  float part[4] = {};
+  for (int half = 0; half < 2 * mine; ++half) {
+    const int first = first_of(half);
+    Half x = next;
+    if (half + 1 < 2 * mine) next.load(row, first_of(half + 1), V, aligned);
     if (bans) x.strike(first, banned, bans);
     uint32_t hits = 0;
     if (with_tail) {
-      double tail = 0.0, odd = 0.0;
 #pragma unroll
-      for (int e = 0; e < TASK / 32; ++e) {
-        const float v = x.value(e);
-        const bool hit = v >= reach;  // (a NaN is in neither the list nor the tail)
-        hits |= hit ? 1u << e : 0u;
-        // tokens that are not the tail's add e^-80 each: nothing
-        double& sum = e & 1 ? odd : tail;
-        sum = exps.add(sum, (static_cast<double>(hit ? least : fmaxf(v, least)) - from) * step);
+      for (int e = 0; e < HALF / 32; ++e) {
+        const float v = x.value(e), weight = exp2_fast(fmaf(v, slope, -zero));
+        if (v < reach) part[e & 3] += weight;
+        if (v >= reach) hits |= 1u << e;  // (a NaN is in neither the list nor the tail)
       }
-      tail += odd;
-      for (int o = 16; o; o >>= 1) tail += __shfl_xor_sync(0xffffffffu, tail, o);
-      if (lane == 0) w.tail[static_cast<size_t>(at) * tasks + task] = tail;
+      if (half & 1) {
+        double tail = static_cast<double>((part[0] + part[1]) + (part[2] + part[3]));
+        part[0] = part[1] = part[2] = part[3] = 0.f;
+        for (int o = 16; o; o >>= 1) tail += __shfl_xor_sync(0xffffffffu, tail, o);
+        if (lane == 0) w.tail[static_cast<size_t>(at) * tasks + task0 + (half >> 1) * STREAM_WARPS + warp] = tail;
+      }
     } else {
 #pragma unroll
-      for (int e = 0; e < TASK / 32; ++e) hits |= x.value(e) >= reach ? 1u << e : 0u;
+      for (int e = 0; e < HALF / 32; ++e) hits |= x.value(e) >= reach ? 1u << e : 0u;
     }
-    if (__any_sync(0xffffffffu, hits)) {
-      const uint32_t mine = __popc(hits);
-      uint32_t up = mine;
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t v = __shfl_up_sync(0xffffffffu, up, o);
-        if (lane >= o) up += v;
-      }
-      uint32_t to = lane == 31 ? atomicAdd(&plan.listed, up) : 0;
-      to = __shfl_sync(0xffffffffu, to, 31) + up - mine;
-      for (; hits; hits &= hits - 1, ++to) {
-        const int id = Task::id(first, __ffs(hits) - 1);
-        if (to < LIST) list[to] = comp_of(logit_value(row[id]), id);
-      }
+    for (; hits; hits &= hits - 1) {
+      const int to = atomicAdd(&s.place, 1);
+      if (to < LIST) ids[to] = Half::id(first, __ffs(hits) - 1);
     }
   }
-  __threadfence();
+  // this CTA's tokens into the row's list
   __syncthreads();
+  const int found = s.place;
+  if (found > 0) {
+    if (tid == 0) s.last = atomicAdd(&plan.listed, found);
+    __syncthreads();
+    for (int i = tid; i < min(found, LIST); i += STREAM_THREADS)  // (their logits are asked for together, not one by one in the loop above)
+      if (s.last + i < LIST) list[s.last + i] = comp_of(logit_value(row[ids[i]]), ids[i]);
+  }
+  __threadfence();
+  __syncthreads();  // (also: s.last has been read)
   if (tid == 0) s.last = atomicAdd(&plan.done, 1u) == gridDim.x - 1;
   __syncthreads();
   if (!s.last) return;
@@ -984,11 +998,11 @@ __global__ void __launch_bounds__(STREAM_THREADS, 3) sample_stream_kernel(Sample
       const double before = sum_before<STREAM_THREADS>(tail, s.warp_sum);
       if (tid == STREAM_THREADS - 1) s.total = before + tail;
       __syncthreads();
-      tail = s.total;
+      tail = s.total * plan.tail_by;
     }
     for (int i = tid; i < static_cast<int>(listed); i += STREAM_THREADS) s.list.item[i] = __ldcg(list + i);
     __syncthreads();
-    pick = pick_from_list(s, static_cast<int>(listed), RowAsk(a, at), tail, ref, reach <= least, ref, reach);
+    pick = pick_from_list(s, static_cast<int>(listed), RowAsk(a, at), tail, tail * TAIL_OFF + 0x1p-30, ref, reach <= least, ref, reach);
   }
   if (tid == 0) {
     if (pick == -2) {
@@ -1022,7 +1036,7 @@ __global__ void __launch_bounds__(STREAM_THREADS) sample_short_kernel(SampleArgs
     atomicMin(&low, static_cast<uint32_t>(c >> 32));
   }
   __syncthreads();
-  const int pick = pick_from_list(s, listed, RowAsk(a, at), 0.0, -INFINITY, true, key_value(top), key_value(low));
+  const int pick = pick_from_list(s, listed, RowAsk(a, at), 0.0, 0.0, -INFINITY, true, key_value(top), key_value(low));
   if (tid == 0) a.out[at] = pick;
 }
 
@@ -1061,7 +1075,7 @@ static int launch_sample(const SampleArgs& a, void* work, cudaStream_t st) {
   sample_work(a.n, a.V, work, &w);
   const int tasks = task_count(a.V);
   // tasks for a warp: as many as leave every SM a few CTAs
-  const long long all = static_cast<long long>(tasks) * a.n / STREAM_WARPS, most = 16LL * sms[dev];
+  const long long all = static_cast<long long>(tasks) * a.n / STREAM_WARPS, most = 8LL * sms[dev];
   const int per = static_cast<int>(all / most < 1 ? 1 : all / most > 16 ? 16 : all / most);
   const int ctas = (tasks + STREAM_WARPS * per - 1) / (STREAM_WARPS * per);
   const int clusters = a.n < sms[dev] / WIDE_CTAS ? a.n : sms[dev] / WIDE_CTAS;
