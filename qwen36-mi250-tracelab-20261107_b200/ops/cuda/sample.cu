@@ -639,7 +639,7 @@ __global__ void __launch_bounds__(WIDE_THREADS) sample_wide_kernel(SampleArgs a,
 //
 // Sums are added up in an order that goes by V alone: the weights of a lane's tokens of a task, the lanes of a warp, the tasks of a row.
 constexpr int PLAN_THREADS = 512, PLAN_PER = 32, PLAN_SAMPLE = PLAN_THREADS * PLAN_PER, PLAN_BLOCK = 256, PLAN_BINS = 1024;
-constexpr int STREAM_THREADS = 256, STREAM_WARPS = STREAM_THREADS / 32;
+constexpr int STREAM_THREADS = 256, STREAM_WARPS = STREAM_THREADS / 32, STREAM_PER_SM = 4;
 constexpr int TASK = 1024;          // tokens that a warp adds up by itself, in two halves
 constexpr int LIST_K = 1024;        // top-k up to which a list is expected to hold the k tokens
 
@@ -866,6 +866,7 @@ __device__ __forceinline__ float exp2_fast(float y) {  // off by 2^-21 of the re
 }
 
 constexpr int HALF = TASK / 2;
+constexpr int SEEN = LIST / STREAM_WARPS;  // entries that a warp has room for
 
 // The logits of a lane in half a task, from `row` on: piece i of 16 bytes holds tokens first + i * 32 * VE ..
 template <typename T>
@@ -873,18 +874,18 @@ struct HalfLogits {
   static constexpr int VE = 16 / sizeof(T), PIECES = HALF / (32 * VE);
   static __device__ __forceinline__ int id(int first, int e) { return first + e / VE * (32 * VE) + e % VE; }
   uint4 raw[PIECES];
-  __device__ __forceinline__ void load(const T* row, int first, int V, bool aligned) {
+  __device__ __forceinline__ void load(const T* row, int first, int V, bool whole) {  // whole: all of it is there, in pieces of 16 bytes
+    if (whole) {
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) raw[i] = __ldg(reinterpret_cast<const uint4*>(row + first) + i * 32);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
-      const int at = id(first, i * VE);
-      if (aligned && at + VE <= V) {
-        raw[i] = __ldg(reinterpret_cast<const uint4*>(row + at));
-      } else {
-        T one[VE];
+      T one[VE];
 #pragma unroll
-        for (int j = 0; j < VE; ++j) one[j] = at + j < V ? row[at + j] : static_cast<T>(-INFINITY);
-        memcpy(&raw[i], one, 16);
-      }
+      for (int j = 0; j < VE; ++j) one[j] = id(first, i * VE + j) < V ? row[id(first, i * VE + j)] : static_cast<T>(-INFINITY);
+      memcpy(&raw[i], one, 16);
     }
   }
   __device__ __forceinline__ float value(int e) const {
@@ -909,7 +910,7 @@ struct HalfLogits {
 
 // CTA x of a row takes `tasks_per_warp` tasks for each warp, from task x * STREAM_WARPS * tasks_per_warp on.
 template <typename T>
-__global__ void __launch_bounds__(STREAM_THREADS, 4) sample_stream_kernel(SampleArgs a, SampleWork w, int tasks, int tasks_per_warp) {
+__global__ void __launch_bounds__(STREAM_THREADS, STREAM_PER_SM) sample_stream_kernel(SampleArgs a, SampleWork w, int tasks, int tasks_per_warp) {
   using Half = HalfLogits<T>;
   __shared__ ListShared s;
   __shared__ int banned[SAMPLE_MAX_EXCLUDE];
@@ -930,7 +931,6 @@ __global__ void __launch_bounds__(STREAM_THREADS, 4) sample_stream_kernel(Sample
   const T* row = static_cast<const T*>(a.logits) + at * a.stride;
   const bool aligned = (reinterpret_cast<uintptr_t>(row) & 15) == 0;
   const int task0 = blockIdx.x * STREAM_WARPS * tasks_per_warp;
-  if (tid == 0) s.place = 0;  // tokens of this CTA's list
   for (int j = tid; j < a.n_exclude; j += STREAM_THREADS) {
     const int id = a.exclude[static_cast<long long>(at) * a.n_exclude + j];
     if (id >= task0 * TASK && id < min(V, (task0 + STREAM_WARPS * tasks_per_warp) * TASK)) banned[atomicAdd(&n_banned, 1)] = id;
@@ -939,17 +939,12 @@ __global__ void __launch_bounds__(STREAM_THREADS, 4) sample_stream_kernel(Sample
   const int bans = n_banned;
   uint64_t* list = w.list + static_cast<size_t>(at) * LIST;
 
-  // the next half is on its way while this one is looked at
-  const int mine = max(0, min(tasks_per_warp, (tasks - task0 - warp + STREAM_WARPS - 1) / STREAM_WARPS));  // tasks of this warp
-  const auto first_of = [&](int half) { return (task0 + (half >> 1) * STREAM_WARPS + warp) * TASK + (half & 1) * HALF + lane * Half::VE; };
-  int* ids = reinterpret_cast<int*>(s.list.item);  // of the tokens for the list
-  Half next;
-  if (mine > 0) next.load(row, first_of(0), V, aligned);
+  // The lanes that have seen tokens for the list, in the order of this warp's halves: first token << 16 | which of the lane's. (One entry for each token, by a
+  // counter of the CTA's, took as long as all the rest: 256 open rows 111 -> 76 us.)
+  uint64_t* seen = s.list.item + warp * SEEN;
+  int n_seen = 0;
   float part[4] = {};
-  for (int half = 0; half < 2 * mine; ++half) {
-    const int first = first_of(half);
-    Half x = next;
-    if (half + 1 < 2 * mine) next.load(row, first_of(half + 1), V, aligned);
+  const auto look = [&](Half& x, int first) {
     if (bans) x.strike(first, banned, bans);
     uint32_t hits = 0;
     if (with_tail) {
@@ -959,32 +954,66 @@ __global__ void __launch_bounds__(STREAM_THREADS, 4) sample_stream_kernel(Sample
         if (v < reach) part[e & 3] += weight;
         if (v >= reach) hits |= 1u << e;  // (a NaN is in neither the list nor the tail)
       }
-      if (half & 1) {
-        double tail = static_cast<double>((part[0] + part[1]) + (part[2] + part[3]));
-        part[0] = part[1] = part[2] = part[3] = 0.f;
-        for (int o = 16; o; o >>= 1) tail += __shfl_xor_sync(0xffffffffu, tail, o);
-        if (lane == 0) w.tail[static_cast<size_t>(at) * tasks + task0 + (half >> 1) * STREAM_WARPS + warp] = tail;
-      }
     } else {
 #pragma unroll
       for (int e = 0; e < HALF / 32; ++e) hits |= x.value(e) >= reach ? 1u << e : 0u;
     }
-    for (; hits; hits &= hits - 1) {
-      const int to = atomicAdd(&s.place, 1);
-      if (to < LIST) ids[to] = Half::id(first, __ffs(hits) - 1);
+    const uint32_t lanes = __ballot_sync(0xffffffffu, hits != 0);
+    const int to = n_seen + __popc(lanes & ((1u << lane) - 1));
+    if (hits && to < SEEN) seen[to] = static_cast<uint64_t>(first) << 16 | hits;
+    n_seen += __popc(lanes);
+  };
+  // a half is on its way while the other is looked at
+  const int stop = min(tasks, task0 + tasks_per_warp * STREAM_WARPS);
+  const auto whole = [&](int task) { return aligned && (task + 1) * TASK <= V; };
+  Half a0, a1;
+  if (task0 + warp < stop) a0.load(row, (task0 + warp) * TASK + lane * Half::VE, V, whole(task0 + warp));
+  for (int task = task0 + warp; task < stop; task += STREAM_WARPS) {
+    const int first = task * TASK + lane * Half::VE;
+    a1.load(row, first + HALF, V, whole(task));
+    look(a0, first);
+    if (task + STREAM_WARPS < stop) a0.load(row, first + STREAM_WARPS * TASK, V, whole(task + STREAM_WARPS));
+    look(a1, first + HALF);
+    if (with_tail) {
+      double tail = static_cast<double>((part[0] + part[1]) + (part[2] + part[3]));
+      part[0] = part[1] = part[2] = part[3] = 0.f;
+      for (int o = 16; o; o >>= 1) tail += __shfl_xor_sync(0xffffffffu, tail, o);
+      if (lane == 0) w.tail[static_cast<size_t>(at) * tasks + task] = tail;
     }
   }
   // this CTA's tokens into the row's list
+  __syncwarp();
+  int count = 0;
+  for (int e = lane; e < min(n_seen, SEEN); e += 32) count += __popc(static_cast<uint32_t>(seen[e]) & 0xffffu);
+  for (int o = 16; o; o >>= 1) count += __shfl_xor_sync(0xffffffffu, count, o);
+  if (n_seen > SEEN) count = LIST + 1;  // more than there is room for: the row is left to the search over bins
+  if (lane == 0) s.list.warp_count[warp] = count;
   __syncthreads();
-  const int found = s.place;
-  if (found > 0) {
-    if (tid == 0) s.last = atomicAdd(&plan.listed, found);
-    __syncthreads();
-    for (int i = tid; i < min(found, LIST); i += STREAM_THREADS)  // (their logits are asked for together, not one by one in the loop above)
-      if (s.last + i < LIST) list[s.last + i] = comp_of(logit_value(row[ids[i]]), ids[i]);
+  if (tid == 0) {
+    uint32_t sum = 0;
+    for (int i = 0; i < STREAM_WARPS; ++i) sum += s.list.warp_count[i];
+    s.place = sum ? atomicAdd(&plan.listed, sum) : 0;
+  }
+  __syncthreads();
+  int at_list = s.place;
+  for (int i = 0; i < warp; ++i) at_list += s.list.warp_count[i];
+  for (int e0 = 0; e0 < min(n_seen, SEEN); e0 += 32) {
+    const uint64_t entry = e0 + lane < min(n_seen, SEEN) ? seen[e0 + lane] : 0;
+    uint32_t which = static_cast<uint32_t>(entry) & 0xffffu;
+    const int mine = __popc(which);
+    int up = mine;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, up, o);
+      if (lane >= o) up += v;
+    }
+    for (int to = at_list + up - mine; which; which &= which - 1, ++to) {
+      const int id = Half::id(static_cast<int>(entry >> 16), __ffs(which) - 1);
+      if (to < LIST) list[to] = comp_of(logit_value(row[id]), id);
+    }
+    at_list += __shfl_sync(0xffffffffu, up, 31);
   }
   __threadfence();
-  __syncthreads();  // (also: s.last has been read)
+  __syncthreads();
   if (tid == 0) s.last = atomicAdd(&plan.done, 1u) == gridDim.x - 1;
   __syncthreads();
   if (!s.last) return;
@@ -1074,10 +1103,15 @@ static int launch_sample(const SampleArgs& a, void* work, cudaStream_t st) {
   SampleWork w;
   sample_work(a.n, a.V, work, &w);
   const int tasks = task_count(a.V);
-  // tasks for a warp: as many as leave every SM a few CTAs
-  const long long all = static_cast<long long>(tasks) * a.n / STREAM_WARPS, most = 8LL * sms[dev];
-  const int per = static_cast<int>(all / most < 1 ? 1 : all / most > 16 ? 16 : all / most);
-  const int ctas = (tasks + STREAM_WARPS * per - 1) / (STREAM_WARPS * per);
+  // CTAs of a row: those that take the least time in waves of what the SMs hold at once, where a CTA's own start and end count as four tasks
+  const int units = (tasks + STREAM_WARPS - 1) / STREAM_WARPS;
+  int ctas = 1, per = units;
+  long long least = -1;
+  for (int c = 1; c <= min(units, 64); ++c) {
+    const int p = (units + c - 1) / c;
+    const long long cost = (static_cast<long long>(c) * a.n + STREAM_PER_SM * sms[dev] - 1) / (STREAM_PER_SM * sms[dev]) * (p + 4);
+    if (least < 0 || cost < least) { least = cost; per = p; ctas = (units + p - 1) / p; }
+  }
   const int clusters = a.n < sms[dev] / WIDE_CTAS ? a.n : sms[dev] / WIDE_CTAS;
   if (launch_pdl(sample_plan_kernel<T>, dim3(a.n), dim3(PLAN_THREADS), 0, st, a, w) != cudaSuccess) return -4;
   if (launch_pdl(sample_stream_kernel<T>, dim3(ctas, a.n), dim3(STREAM_THREADS), 0, st, a, w, tasks, per) != cudaSuccess) return -4;
