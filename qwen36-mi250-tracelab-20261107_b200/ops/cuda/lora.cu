@@ -4,14 +4,16 @@
 //
 // This file makes h; the GEMM goes on over it (lora.cuh).
 //
-// A CTA takes 16 token rows (32 where there are more CTAs of 16 than the SMs hold) and the adapters among them one after the other, or every
+// A CTA takes 16 token rows (64 where the CTAs of 16 would be more than two for each SM) and the adapters among them one after the other, or every
 // gridDim.y-th one: in a decode step each row may have its own. Its eight warps share K in pieces of 32, join their sums in a fixed order, and round h to
-// bf16. Rows of other adapters take part in the product and are not stored. All of it goes by the row alone, so its bits do not depend on the batch.
+// bf16, as x itself is rounded: 2^-9 of each h, a part of y's own rounding. Rows of other adapters take part in the product and are not stored. All of
+// it goes by the row alone, so its bits do not depend on the batch.
 //
-// The products are 16 x 8 x 16 instructions fed from global memory: A and x are read once, at 2 R flops for each number of x, far below what tensor
-// memory would be needed for. Bound by the latency of those reads in a decode step, so a warp asks for a whole batch of pieces at a time (64 ranks, K of
-// 4096: 78 us piece by piece, 22 in batches), and by nothing that shows in a long pass: with 256 threads and less than 13 KB of shared memory a CTA
-// runs beside the GEMM's, which needs h behind its first 32 k-blocks.
+// The products are 16 x 8 x 16 instructions fed from global memory, in an order that is the same for one row and for 8,192. In a decode step the latency
+// of those reads bounds it, so a warp asks for a whole batch of pieces at a time (64 ranks, K of 4096: 78 us piece by piece, 22 in batches); with 256
+// threads and less than 13 KB of shared memory a CTA runs beside the GEMM's, which needs h behind its own k-blocks: the whole call takes 12.3 us for one row
+// of 9216 x 2048 where the projection alone takes 11.0, 22.4 and 11.6 for 128 rows of 32 adapters. In a long pass the rate of these instructions bounds
+// it (about 144 TFLOP/s; 8,192 rows, 64 ranks, K of 2048: 35 us, of which 26 show beside the GEMM's 197).
 #include "lora.cuh"
 
 namespace b200 {
@@ -173,11 +175,14 @@ __global__ void __launch_bounds__(SHRINK_THREADS) lora_shrink_kernel(const bf16*
             if (mine[row] != id || col >= tiles.width * (tiles.chunks / tiles.parts)) continue;
             // (R is even; columns behind it are 0)
             const float h0 = col < R ? acc[m][n][2 * half] * s : 0.f, h1 = col < R ? acc[m][n][2 * half + 1] * s : 0.f;
-            const __nv_bfloat162 hi = __floats2bfloat162_rn(h0, h1);
             const int e = e0 + col / 64 * tiles.parts;
-            *reinterpret_cast<__nv_bfloat162*>(place(e, row) + col % 64) = hi;
-            if (tiles.parts == 2)
-              *reinterpret_cast<__nv_bfloat162*>(place(e + 1, row) + col % 64) = __floats2bfloat162_rn(h0 - __low2float(hi), h1 - __high2float(hi));
+            float l0 = h0, l1 = h1;  // what is left
+            for (int p = 0; p < tiles.parts; ++p) {
+              const __nv_bfloat162 v = __floats2bfloat162_rn(l0, l1);
+              *reinterpret_cast<__nv_bfloat162*>(place(e + p, row) + col % 64) = v;
+              l0 -= __low2float(v);
+              l1 -= __high2float(v);
+            }
           }
       }
   }

@@ -42,7 +42,7 @@ def _rows(T, L, seed=0, bare=0.2, run=1):
 def _check(got, x, w, ad, rows, what=""):
     """Within what the roundings leave. A sum of K products is added up sixteen at a time: K / 16 additions to a running sum, which is at most the sum of
     the products' magnitudes, each cut to 24 bits: off by 2^-23 of that at most, so K / 16 * 2^-23 of the magnitudes in all (so is h's). h is
-    rounded to bf16 (half a step: 2^-9 of each h, 2^-8 taken), or to two bf16 parts for fp32 outputs (2^-17); the result to bf16 by 2^-9 of itself
+    rounded to bf16 (half a step: 2^-9 of each h, 2^-8 taken), or to three bf16 parts for fp32 outputs (2^-24 of it, 2^-23 taken); the result to bf16 by 2^-9 of itself
     (2^-8 taken), or to fp32 (2^-24, 2^-23 taken)."""
     acc = (x.shape[1] / 16 + 1) * 2.0 ** -23
     x64, w64 = x.double(), w.double()
@@ -55,7 +55,7 @@ def _check(got, x, w, ad, rows, what=""):
             h, hm = x64[at] @ ad.a[i].double().t() * s, x64[at].abs() @ ad.a[i].double().abs().t() * s.abs()
             y[at] += h @ b.t()
             mag[at] += h.abs() @ b.abs().t()
-            off[at] += (h.abs() * (2.0 ** -17 if f32 else 2.0 ** -8) + hm * acc) @ b.abs().t()
+            off[at] += (h.abs() * (2.0 ** -23 if f32 else 2.0 ** -8) + hm * acc) @ b.abs().t()
     tol = mag * (acc + ad.a.shape[1] / 16 * 2.0 ** -23) + off + y.abs() * (2.0 ** -23 if f32 else 2.0 ** -8) + 1e-30
     assert got.isfinite().all(), what
     worst = ((got.double() - y).abs() / tol).max().item()
