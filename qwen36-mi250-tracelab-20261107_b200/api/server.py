@@ -671,6 +671,8 @@ def load_service(args: argparse.Namespace) -> Service:
         cfg.pack_weights = True  # the server owns the weights it loads: stream them tile-packed
     tp = int(args.gpus_per_replica or os.environ.get("ENGINE_TP", "1") or 1)
     followers = []
+    if tp > 1 and cfg.adapters:  # (before the other ranks are started)
+        raise ValueError("adapters are served by replicas of one GPU")
     from ..parallel import dpep
 
     if dpep.env_group() is not None:

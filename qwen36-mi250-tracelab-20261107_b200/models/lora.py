@@ -88,17 +88,18 @@ def read_adapter(path: str | Path, cfg: ModelConfig) -> _Adapter:
         if set(ab) != {"A", "B"}:
             raise ValueError(f"adapter {path}: layer {layer} {module} has no lora_{'B' if 'A' in ab else 'A'}")
         a, b = ab["A"].float(), ab["B"].float()
+        low, high = torch.finfo(torch.bfloat16).min, torch.finfo(torch.bfloat16).max  # (what rounds to infinity in bf16 is as bad)
         ins, outs = modules(cfg, cfg.layer_types[layer])
         n = dict(ins + outs)[module]
         k = cfg.hidden_size if module in dict(ins) else mixer_width(cfg, cfg.layer_types[layer])
         if a.shape != (r, k) or b.shape != (n, r):
             raise ValueError(f"adapter {path}: layer {layer} {module} has {tuple(a.shape)} and {tuple(b.shape)}, not {(r, k)} and {(n, r)}")
-        if not (a.isfinite().all() and b.isfinite().all()):
-            raise ValueError(f"adapter {path}: layer {layer} {module} holds numbers that are not finite")
+        if not all(((t >= low) & (t <= high)).all() for t in (a, b)):
+            raise ValueError(f"adapter {path}: layer {layer} {module} holds numbers that are not finite, or not in bf16")
         parts[layer, module] = (a, b)
     alpha = float(conf.get("lora_alpha", r))
     scale = alpha / math.sqrt(r) if conf.get("use_rslora") else alpha / r
-    if not math.isfinite(scale):
+    if not abs(scale) <= torch.finfo(torch.float32).max:
         raise ValueError(f"adapter {path}: alpha {alpha}")
     return _Adapter(scale, parts)
 

@@ -8,8 +8,9 @@
 // None needs the whole order. Token and logit are one 64-bit number (`comp`: the logit's bits made monotone, then the id reversed),
 // all different, so that ties need no rule of their own.
 //
-// Weights and their sums are held in 64 bits: with 248,320 tokens kept, sums that were off by one part in 1e8 would move one draw in
-// 400 to a neighbouring token, and a request's tokens would depend on how the sums were cut.
+// What decides a pick is held in 64 bits: with 248,320 tokens kept, sums that were off by one part in 1e8 would move one draw in
+// 400 to a neighbouring token, and a request's tokens would depend on how the sums were cut. The weights of the tokens outside a row's list are added up in
+// fp32, with a bound on what that is off by: a row that the bound leaves undecided goes to the wide kernel, which works in 64 bits throughout.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 #include <float.h>
@@ -227,8 +228,9 @@ struct WideShared {
   double base_mass, cut_mass;
 };
 
-// One row, one cluster. This is one-off code: what it takes is the latency of its steps and of fetching their instructions, so what is used
-// twice is there once. Arguments go by value, into registers.
+// One row, one cluster: 16 SMs hold the row's logits in shared memory and look for its places with bins of the whole row (2,048 by value), then within the
+// place's bin. This is one-off code: what it takes is the latency of its steps and of fetching their instructions, so what is used
+// twice is there once. Arguments go by value, into registers. 36 us for up to nine rows of 248,320, 70 for ten to eighteen.
 template <typename T>
 struct WidePart {  // a CTA's part of the row
   WideShared& s;
@@ -636,6 +638,9 @@ __global__ void __launch_bounds__(WIDE_THREADS) sample_wide_kernel(SampleArgs a,
 //          list has run over) is left to
 //  wide    the kernel above.
 // A guess that is off costs time, never a result: what the list and the tail say is exact.
+//
+// Rows of 248,320 fp32 logits, device time: one row 16 us (three launches, each a chain of latencies), 16 rows 41, 128 of mixed settings 105, 256 open ones
+// 141: plan 10, stream 76 (254 MB: 3.3 TB/s; a number takes about ten instructions, which bound it before the memory does), wide 36 to 70.
 //
 // Sums are added up in an order that goes by V alone: the weights of a lane's tokens of a task, the lanes of a warp, the tasks of a row.
 constexpr int PLAN_THREADS = 512, PLAN_PER = 32, PLAN_SAMPLE = PLAN_THREADS * PLAN_PER, PLAN_BLOCK = 256, PLAN_BINS = 1024;

@@ -43,7 +43,7 @@ class Coordinator:
             if g.sampling.seed is None and not g.sampling.greedy:
                 g.sampling.seed = (g.id * 7919 + int(time.time() * 1e3)) % (2**31)
             self.live[g.id] = g
-            new.append((g.id, g.prompt, dataclasses.asdict(g.sampling)))
+            new.append((g.id, g.prompt, dataclasses.asdict(g.sampling), g.adapter))
             engine.waiting.append(g)
         cancel = [i for i, g in self.live.items() if g.cancelled.is_set() and i not in self._cancel_sent and not g.done]
         self._cancel_sent.update(cancel)
@@ -67,8 +67,8 @@ class Coordinator:
         self.dist.broadcast_object_list(msg, src=self.leader, group=self.group)
         m = msg[0]
         if not self.is_leader:
-            for gid, prompt, sampling in m["new"]:
-                g = Generation(prompt, Sampling(**sampling))
+            for gid, prompt, sampling, adapter in m["new"]:
+                g = Generation(prompt, Sampling(**sampling), adapter=adapter)  # (every rank refuses the same requests)
                 g.id = gid
                 self.live[gid] = g
                 engine.waiting.append(g)

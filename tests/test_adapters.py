@@ -135,15 +135,23 @@ def test_refused_adapters(tmp_path, dirs):
     some = next(k for k in good if "lora_A" in k)
     nan = good[some].clone()
     nan[0, 0] = float("nan")
+    huge = good[some].float()
+    huge[0, 0] = 3.4e38  # finite, and infinite as bf16
     write_adapter(tmp_path / "odd", cfg, 0)
     for state in ({}, {k: v for k, v in good.items() if k != some}, {**good, "base_model.model.lm_head.lora_A.weight": torch.zeros(4, 128)},
-                  {**good, some: nan}, {**good, some: good[some][:, 1:].contiguous()}, {some.replace("layers.0", "layers.9"): good[some]}):
+                  {**good, some: nan}, {**good, some: huge}, {**good, some: good[some][:, 1:].contiguous()}, {some.replace("layers.0", "layers.9"): good[some]}):
         save_file(state, str(tmp_path / "odd/adapter_model.safetensors"))
         with pytest.raises(ValueError, match="adapter"):
             read_adapter(tmp_path / "odd", cfg)
     write_adapter(tmp_path / "big", cfg, 0, r=100)
     with pytest.raises(ValueError, match="rank"):
         attach_adapters(_weights(), {"big": tmp_path / "big"})
+    for alpha in (1e300, float("inf"), float("nan")):  # out of fp32's range
+        write_adapter(tmp_path / "loud", cfg, 0)
+        c = json.loads((tmp_path / "loud/adapter_config.json").read_text())
+        (tmp_path / "loud/adapter_config.json").write_text(json.dumps({**c, "lora_alpha": alpha}))
+        with pytest.raises(ValueError, match="alpha"):
+            read_adapter(tmp_path / "loud", cfg)
     for spec in ("a", "=x", "a=", "a=x,a=y"):
         with pytest.raises(ValueError, match="adapter"):
             parse_adapters(spec)
@@ -170,6 +178,37 @@ def test_refused_requests_and_engines(dirs):
 
     with pytest.raises(ValueError, match="torch_ops"):
         cuda_ops.lora_linear(x, w, ad, rows)
+
+
+def test_ranks_of_a_replica_refuse_the_same_requests():
+    """A request for an adapter reaches the other ranks with the adapter's name: were it refused by the first rank alone, they would wait for it."""
+    import torch.distributed as dist
+
+    from b200serve.parallel.lockstep import Coordinator
+    from b200serve.sched.request import Generation
+
+    sent = []
+
+    class Wire:
+        ReduceOp = dist.ReduceOp
+
+        def all_reduce(self, t, op=None, group=None):
+            pass
+
+        def broadcast_object_list(self, msg, src, group):
+            if msg[0] is not None:
+                sent.append(msg[0])
+            msg[0] = sent[-1]
+
+    engines = [_engine(_weights()) for _ in range(2)]
+    for rank, eng in enumerate(engines):
+        eng.coordinator = Coordinator(None, rank)
+        eng.coordinator.dist = Wire()
+    gens = [engines[0].submit(Generation([5, 6, 7], Sampling(max_tokens=3, ignore_eos=True), adapter=a)) for a in ("all", None)]
+    for eng in engines:
+        eng.coordinator.sync(eng)
+        eng.step(synced=True)
+    assert gens[0].finish_reason == "error" and [len(e.prefilling) + len(e.running) for e in engines] == [1, 1]
 
 
 def test_the_server_serves_adapters_as_models(dirs):
