@@ -160,6 +160,7 @@ __device__ void order_list(Order& s, int c, float hi, float lo) {
     const int b = bin_of(mine);
     const uint32_t from = s.bins[b], to = b + 1 < LIST_BINS ? s.bins[b + 1] : static_cast<uint32_t>(c);
     uint32_t above = from;
+#pragma unroll 4
     for (uint32_t k = from; k < to; ++k) above += s.other[k] > mine;
     s.item[above] = mine;
   }
@@ -742,7 +743,7 @@ __device__ int pick_from_list(ListShared& s, int c, const RowAsk& r, double tail
   for (int o = 16; o; o >>= 1) { positive += __shfl_xor_sync(0xffffffffu, positive, o); enough += __shfl_xor_sync(0xffffffffu, enough, o); }
   if ((tid & 31) == 0) { atomicAdd(&s.place, positive); atomicAdd(&s.last, enough); }
   __syncthreads();
-  positive = s.place; enough = max(1, s.last);
+  positive = s.place; enough = max(1, s.last);  // (neither is written again)
   // the weight that top-p goes by, and then that of the kept, lies between these
   double least_sum = s.list.sum[nk - 1], most_sum = least_sum;
   if (!closed) {
@@ -751,16 +752,16 @@ __device__ int pick_from_list(ListShared& s, int c, const RowAsk& r, double tail
   }
   constexpr int OPEN = 1 << 30;
   int limit = closed ? nk : OPEN;
-  // the first place with more than `target` up to it, OPEN if there is none
+  // A place with more than `target` up to it and no more before it, OPEN if there is none: each warp looks for it by itself, at 32 places and then between two.
+  const int lane = tid & 31, stride = (nk + 31) / 32;
   const auto find = [&](double target) {
-    __syncthreads();
-    if (tid == 0) s.place = OPEN;
-    __syncthreads();
-#pragma unroll 1
-    for (int i = tid; i < nk; i += STREAM_THREADS)
-      if (s.list.sum[i] > target && !(i > 0 && s.list.sum[i - 1] > target)) atomicMin(&s.place, i);
-    __syncthreads();
-    return s.place;
+    const uint32_t ends = __ballot_sync(0xffffffffu, s.list.sum[min(nk, (lane + 1) * stride) - 1] > target);
+    if (ends == 0) return OPEN;
+    const int first = (__ffs(ends) - 1) * stride;
+    static_assert(LIST <= 32 * 64, "two places for each lane");
+    const uint32_t low = __ballot_sync(0xffffffffu, s.list.sum[min(nk - 1, first + lane)] > target);
+    const uint32_t high = __ballot_sync(0xffffffffu, s.list.sum[min(nk - 1, first + 32 + lane)] > target);
+    return first + (low ? __ffs(low) - 1 : 31 + __ffs(high));
   };
   if (r.p < 1.0) {
     const int at = find(r.p * least_sum);
@@ -1019,22 +1020,30 @@ __global__ void __launch_bounds__(STREAM_THREADS, STREAM_PER_SM) sample_stream_k
   }
   __threadfence();
   __syncthreads();
-  if (tid == 0) s.last = atomicAdd(&plan.done, 1u) == gridDim.x - 1;
+  if (tid == 0) {
+    s.last = atomicAdd(&plan.done, 1u) == gridDim.x - 1;
+    __threadfence();
+  }
   __syncthreads();
   if (!s.last) return;
-  __threadfence();
+  // all of it is asked for at a time, the list without knowing how much of it there is
   const uint32_t listed = __ldcg(&plan.listed);
+  uint64_t item[LIST / STREAM_THREADS];
+#pragma unroll
+  for (int j = 0; j < LIST / STREAM_THREADS; ++j) item[j] = __ldcg(list + j * STREAM_THREADS + tid);
   int pick = -2;
   if (listed <= LIST) {
     double tail = 0.0;
-    if (with_tail) {
+    if (with_tail)
       for (int i = tid; i < tasks; i += STREAM_THREADS) tail += __ldcg(w.tail + static_cast<size_t>(at) * tasks + i);
+#pragma unroll
+    for (int j = 0; j < LIST / STREAM_THREADS; ++j) s.list.item[j * STREAM_THREADS + tid] = item[j];
+    if (with_tail) {
       const double before = sum_before<STREAM_THREADS>(tail, s.warp_sum);
       if (tid == STREAM_THREADS - 1) s.total = before + tail;
       __syncthreads();
       tail = s.total * plan.tail_by;
     }
-    for (int i = tid; i < static_cast<int>(listed); i += STREAM_THREADS) s.list.item[i] = __ldcg(list + i);
     __syncthreads();
     pick = pick_from_list(s, static_cast<int>(listed), RowAsk(a, at), tail, tail * TAIL_OFF + 0x1p-30, ref, reach <= least, ref, reach);
   }
