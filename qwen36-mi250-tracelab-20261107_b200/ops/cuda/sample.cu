@@ -126,7 +126,7 @@ __device__ void order_list(Order& s, int c, float hi, float lo) {
   const auto bin_of = [&](uint64_t comp) { return min(LIST_BINS - 1, max(0, static_cast<int>((hi - comp_value(comp)) * scale))); };
   for (int b = tid; b < LIST_BINS; b += THREADS) s.bins[b] = 0;
   __syncthreads();
-#pragma unroll 1
+#pragma unroll 2
   for (int i = tid; i < c; i += THREADS) s.at[i] = static_cast<uint16_t>(atomicAdd(&s.bins[bin_of(s.item[i])], 1u));
   __syncthreads();
   uint32_t own[BINS], most = 0, up = 0;
@@ -151,7 +151,7 @@ __device__ void order_list(Order& s, int c, float hi, float lo) {
 #pragma unroll
   for (int j = 0; j < BINS; ++j) { s.bins[tid * BINS + j] = up; up += own[j]; }  // where a bin starts
   __syncthreads();
-#pragma unroll 1
+#pragma unroll 2
   for (int i = tid; i < c; i += THREADS) s.other[s.bins[bin_of(s.item[i])] + s.at[i]] = s.item[i];
   __syncthreads();
 #pragma unroll 1
@@ -786,14 +786,13 @@ __device__ int pick_from_list(ListShared& s, int c, const RowAsk& r, double tail
 template <typename T>
 __global__ void __launch_bounds__(PLAN_THREADS) sample_plan_kernel(SampleArgs a, SampleWork w) {
   __shared__ uint32_t bins[PLAN_BINS];
-  __shared__ float warp_top[PLAN_THREADS / 32], warp_low[PLAN_THREADS / 32];
+  __shared__ float warp_top[PLAN_THREADS / 32], warp_low[PLAN_THREADS / 32], warp_over[PLAN_THREADS / 32];
   __shared__ uint32_t warp_count[PLAN_THREADS / 32];
   __shared__ int found;
   pdl_wait();
   pdl_launch();
   const int at = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.V;
   const T* row = static_cast<const T*>(a.logits) + at * a.stride;
-  const RowAsk ask(a, at);
   if (at == 0 && tid == 0) *w.left = 0;
   if (at == 0 && tid < 32) w.powers[tid] = exp2(tid / 32.0);
   for (int b = tid; b < PLAN_BINS; b += PLAN_THREADS) bins[b] = 0;
@@ -812,24 +811,34 @@ __global__ void __launch_bounds__(PLAN_THREADS) sample_plan_kernel(SampleArgs a,
     top = fmaxf(top, x[i]);
     if (x[i] != -INFINITY) low = fminf(low, x[i]);
   }
-  for (int o = 16; o; o >>= 1) {
+  const RowAsk ask(a, at);  // (behind the logits' loads: its division waits for the temperature)
+  const int want = list_want(ask.greedy, ask.cut_k ? ask.k : 0);
+  const uint32_t share = max(1u, static_cast<uint32_t>(static_cast<long long>(want) * min(V, PLAN_SAMPLE) / V));
+  // `share` tokens of the sample lie at `over` or above, if as many groups of lanes each have one: of the others none need be counted
+  float over = INFINITY;
+  int lanes = 32;  // of a group
+  while (lanes > 1 && PLAN_THREADS / lanes < static_cast<int>(share)) lanes >>= 1;
+  for (int o = 1; o < 32; o <<= 1) {
+    if (o == lanes) over = top;
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
   }
-  if (lane == 0) { warp_top[warp] = top; warp_low[warp] = low; }
+  if (lanes == 32) over = top;
+  for (int o = 16; o; o >>= 1) over = fminf(over, __shfl_xor_sync(0xffffffffu, over, o));
+  if (lane == 0) { warp_top[warp] = top; warp_low[warp] = low; warp_over[warp] = over; }
   __syncthreads();
-  for (int i = 0; i < PLAN_THREADS / 32; ++i) { top = fmaxf(top, warp_top[i]); low = fminf(low, warp_low[i]); }
+  for (int i = 0; i < PLAN_THREADS / 32; ++i) { top = fmaxf(top, warp_top[i]); low = fminf(low, warp_low[i]); over = fminf(over, warp_over[i]); }
+  if (PLAN_THREADS / lanes < static_cast<int>(share)) over = low;
   const float t = ask.greedy ? 1.f : a.temperature[at];
   const float least = fmaxf(top - WIDE_RANGE * t, -FLT_MAX);  // below it nothing has any weight
-  const float range = fminf(fminf(WIDE_RANGE * t, top - low), 1e38f);
+  const float range = fminf(fminf(WIDE_RANGE * t, top - fmaxf(low, over)), 1e38f);
   const float scale = range > 0.f ? fminf(PLAN_BINS / range, 1e38f) : 0.f;
+  const float count_from = fmaxf(least, over);
 #pragma unroll
   for (int i = 0; i < PLAN_PER; ++i)
-    if (x[i] >= least) atomicAdd(&bins[min(PLAN_BINS - 1, static_cast<int>((top - x[i]) * scale))], 1u);
+    if (x[i] >= count_from) atomicAdd(&bins[min(PLAN_BINS - 1, static_cast<int>((top - x[i]) * scale))], 1u);
   __syncthreads();
   // the bin in which the sample has its share of `want`
-  const int want = list_want(ask.greedy, ask.cut_k ? ask.k : 0);
-  const uint32_t share = max(1u, static_cast<uint32_t>(static_cast<long long>(want) * min(V, PLAN_SAMPLE) / V));
   static_assert(PLAN_BINS == 2 * PLAN_THREADS, "two bins for each thread");
   const uint32_t c0 = bins[2 * tid], c1 = bins[2 * tid + 1];
   uint32_t up = c0 + c1;
@@ -1018,9 +1027,9 @@ __global__ void __launch_bounds__(STREAM_THREADS, STREAM_PER_SM) sample_stream_k
     }
     at_list += __shfl_sync(0xffffffffu, up, 31);
   }
-  __threadfence();
   __syncthreads();
-  if (tid == 0) {
+  if (tid == 0) {  // (one fence for the CTA, behind the barrier: a fence of every warp waited for the others')
+    __threadfence();
     s.last = atomicAdd(&plan.done, 1u) == gridDim.x - 1;
     __threadfence();
   }
