@@ -103,7 +103,7 @@ __device__ __forceinline__ void sort_down(uint64_t* a, int n) {
 
 constexpr int LIST = 2048;         // most tokens that are put in order one by one
 constexpr int LIST_BINS = 1024;
-constexpr int LIST_BIN_MOST = 96;  // tokens of a bin that are compared each with each
+constexpr uint32_t LIST_COMPARES = 1536;  // comparisons of a thread, up to which the tokens of a bin are compared each with each
 
 struct Order {
   uint64_t item[LIST];
@@ -115,8 +115,9 @@ struct Order {
   uint32_t bins[LIST_BINS], warp_count[32];
 };
 
-// Puts s.item[0 .. c) into descending order: bins by value, in a bin each is compared with each. `hi` and `lo`: about where the values lie.
-// Many equal values are sorted by exchanges instead, which take 66 rounds for a full list. All threads of the CTA. A row's list is put in order once, so
+// Puts s.item[0 .. c) into descending order: bins by value, in a bin each is compared with each. `hi` and `lo`: between which most of the values lie.
+// Many equal values are sorted by exchanges instead, which take 66 rounds for a full list (256 open rows of fp32 logits 128 us with 1,000 to 2,560 comparisons
+// to a thread before that, 136 with 512; 61 rows of bf16 logits 74 and 84, and 126 with 6,000). All threads of the CTA. A row's list is put in order once, so
 // this and what follows is short code and not unrolled: 166 tokens took 11,000 cycles unrolled eight times, nearly all of them for instructions.
 template <int THREADS>
 __device__ void order_list(Order& s, int c, float hi, float lo) {
@@ -138,7 +139,7 @@ __device__ void order_list(Order& s, int c, float hi, float lo) {
     if (lane >= o) up += v;
   }
   if (lane == 31) s.warp_count[warp] = up;
-  if (__syncthreads_or(most > LIST_BIN_MOST)) {
+  if (__syncthreads_or(most * ((c + THREADS - 1) / THREADS) > LIST_COMPARES)) {
     int size = 2;
     while (size < c) size <<= 1;
     for (int i = c + tid; i < size; i += THREADS) s.item[i] = 0;
@@ -195,7 +196,7 @@ constexpr int WIDE_CTAS = 16;       // of a row: one cluster
 constexpr int WIDE_THREADS = 1024;
 constexpr int WIDE_HELD = 16384;    // logits that a CTA holds; its part of a larger vocabulary is read again in every pass
 constexpr int WIDE_BINS = 2048;
-constexpr int WIDE_LIMBS = 4;
+constexpr int WIDE_WORDS = 2;
 constexpr float WIDE_RANGE = 80.f;  // e^-80 of the largest weight, 2^22 times, is nothing in 64 bits
 constexpr int SAMPLE_MAX_VOCAB = 1 << 22;
 
@@ -206,13 +207,13 @@ struct WideTable {  // sums up to and with each bin, of the whole row
 struct WideShared {
   float held[WIDE_HELD];
   union {
-    struct { uint32_t count[WIDE_BINS], mass[WIDE_LIMBS][WIDE_BINS]; } bins;  // this CTA's part
+    struct { uint32_t count[WIDE_BINS], mass[WIDE_WORDS][WIDE_BINS]; } bins;  // this CTA's part
     Order list;                                                             // (of the first CTA)
   };
   WideTable first, finer;  // of the first CTA
   uint64_t top[WIDE_CTAS], low[WIDE_CTAS];  // every CTA's
   double part[WIDE_CTAS];
-  unsigned long long sums[1 + WIDE_LIMBS][WIDE_BINS / WIDE_CTAS];
+  unsigned long long sums[1 + WIDE_WORDS][WIDE_BINS / WIDE_CTAS];
   double warp_sum[WIDE_THREADS / 32];
   uint64_t warp_top[WIDE_THREADS / 32], warp_low[WIDE_THREADS / 32];
   uint32_t warp_count[WIDE_THREADS / 32];
@@ -231,7 +232,7 @@ struct WideShared {
 
 // One row, one cluster: 16 SMs hold the row's logits in shared memory and look for its places with bins of the whole row (2,048 by value), then within the
 // place's bin. This is one-off code: what it takes is the latency of its steps and of fetching their instructions, so what is used
-// twice is there once. Arguments go by value, into registers. 36 us for up to nine rows of 248,320, 70 for ten to eighteen.
+// twice is there once. Arguments go by value, into registers. 30 us for up to nine rows of 248,320, 60 for ten to eighteen.
 template <typename T>
 struct WidePart {  // a CTA's part of the row
   WideShared& s;
@@ -342,17 +343,17 @@ __device__ __forceinline__ double wide_before(WideShared& s, double v, uint32_t 
   return (warp ? before : 0.0) + (lane ? mine : 0.0);
 }
 
-// The tokens that `place` gives a bin (none: -1) into this CTA's bins. A weight goes in as a whole number, in limbs of as many bits as no sum of this
-// CTA's tokens runs over with: whole numbers add up to the same sum in any order.
+// The tokens that `place` gives a bin (none: -1) into this CTA's bins. A weight goes in as a whole number of 64 bits, of which as many are left free as the
+// sum of this CTA's tokens needs: whole numbers add up to the same sum in any order. (2^14 tokens in multiples of 2^-50 of the largest weight, 2^18 in
+// multiples of 2^-46. Two words, the first one's carry goes with the second: three words of 18 bits each took 15.5 thousand tokens 18,000 cycles.)
 template <typename T, typename F>
 __device__ __forceinline__ void wide_tally(const WidePart<T>& part, const WideScale& c, double power, bool counts, F place) {
   WideShared& s = part.s;
-  for (int b = threadIdx.x; b < WIDE_BINS * (1 + WIDE_LIMBS); b += WIDE_THREADS) s.bins.count[b] = 0;  // (and the masses behind the counts)
+  for (int b = threadIdx.x; b < WIDE_BINS * (1 + WIDE_WORDS); b += WIDE_THREADS) s.bins.count[b] = 0;  // (and the masses behind the counts)
   __syncthreads();
   const ExpLanes exps(power);
-  const double one = part.held ? 0x1p54 : 0x1p56, m = c.m;
-  const int limb = part.held ? 18 : 14;
-  const uint32_t mask = (1u << limb) - 1;
+  const double one = part.held ? 0x1p50 : 0x1p46, m = c.m;
+  static_assert(WIDE_HELD <= 1 << 14 && SAMPLE_MAX_VOCAB / WIDE_CTAS <= 1 << 18, "no sum runs over");
   part.each([&](float x, int i) {
     double w = exps.add(0.0, (static_cast<double>(x) - m) * c.step);
     if (x < c.floor) w = 0.0;
@@ -360,13 +361,11 @@ __device__ __forceinline__ void wide_tally(const WidePart<T>& part, const WideSc
     const int b = x == -INFINITY ? -1 : place(x, i);
     if (b < 0) return;
     if (counts) atomicAdd(&s.bins.count[b], 1u);
-    unsigned long long f = __double2ull_rn(w * one);
-#pragma unroll
-    for (int l = 0; l < WIDE_LIMBS; ++l) {
-      const uint32_t v = static_cast<uint32_t>(f) & (l == WIDE_LIMBS - 1 ? ~0u : mask);
-      if (v) atomicAdd(&s.bins.mass[l][b], v);
-      f >>= limb;
-    }
+    const unsigned long long f = __double2ull_rn(w * one);
+    const uint32_t low = static_cast<uint32_t>(f);
+    uint32_t high = static_cast<uint32_t>(f >> 32);
+    if (low) high += atomicAdd(&s.bins.mass[0][b], low) > ~low;
+    if (high) atomicAdd(&s.bins.mass[1][b], high);
   });
 }
 
@@ -377,9 +376,9 @@ __device__ __noinline__ void wide_tabulate(WideShared& s, bool finer, bool held)
   cluster.sync();
   // a thread for each number of the bins that this CTA adds up: a warp's lanes read neighbours from one CTA after the other
   constexpr int OWN = WIDE_BINS / WIDE_CTAS;
-  static_assert(OWN * (1 + WIDE_LIMBS) <= WIDE_THREADS, "a thread for each number");
+  static_assert(OWN * (1 + WIDE_WORDS) <= WIDE_THREADS, "a thread for each number");
   const int b = cluster_rank() * OWN + tid % OWN, l = tid / OWN;
-  if (l <= WIDE_LIMBS) {
+  if (l <= WIDE_WORDS) {
     unsigned long long sum = 0;
 #pragma unroll
     for (int r = 0; r < WIDE_CTAS; ++r) sum += *cluster.map_shared_rank(&s.bins.count[l * WIDE_BINS + b], r);
@@ -389,10 +388,7 @@ __device__ __noinline__ void wide_tabulate(WideShared& s, bool finer, bool held)
   if (tid < OWN) {
     WideTable* table = cluster.map_shared_rank(finer ? &s.finer : &s.first, 0);
     table->count[b] = static_cast<uint32_t>(s.sums[0][tid]);
-    double v = 0.0;
-#pragma unroll
-    for (int i = WIDE_LIMBS; i >= 1; --i) v = v * (held ? 0x1p18 : 0x1p14) + static_cast<double>(s.sums[i][tid]);
-    table->mass[b] = v * (held ? 0x1p-54 : 0x1p-56);
+    table->mass[b] = (static_cast<double>(s.sums[2][tid]) * 0x1p32 + static_cast<double>(s.sums[1][tid])) * (held ? 0x1p-50 : 0x1p-46);
   }
   cluster.sync();
   if (cluster_rank() != 0) return;
@@ -640,8 +636,9 @@ __global__ void __launch_bounds__(WIDE_THREADS) sample_wide_kernel(SampleArgs a,
 //  wide    the kernel above.
 // A guess that is off costs time, never a result: what the list and the tail say is exact.
 //
-// Rows of 248,320 fp32 logits, device time: one row 16 us (three launches, each a chain of latencies), 16 rows 41, 128 of mixed settings 105, 256 open ones
-// 141: plan 10, stream 76 (254 MB: 3.3 TB/s; a number takes about ten instructions, which bound it before the memory does), wide 36 to 70.
+// Rows of 248,320 fp32 logits, device time: one row 15 us (three launches, each a chain of latencies), 16 rows 36, 128 of mixed settings 98, 256 open ones
+// 128: plan 10, stream 70 (254 MB: 3.6 TB/s; a number takes about ten instructions, which bound it before the memory does, and a row's end 13 us), wide 30
+// to 60.
 //
 // Sums are added up in an order that goes by V alone: the weights of a lane's tokens of a task, the lanes of a warp, the tasks of a row.
 constexpr int PLAN_THREADS = 512, PLAN_PER = 32, PLAN_SAMPLE = PLAN_THREADS * PLAN_PER, PLAN_BLOCK = 256, PLAN_BINS = 1024;
