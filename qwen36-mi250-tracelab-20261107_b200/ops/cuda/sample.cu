@@ -636,7 +636,7 @@ __global__ void __launch_bounds__(WIDE_THREADS) sample_wide_kernel(SampleArgs a,
 //  wide    the kernel above.
 // A guess that is off costs time, never a result: what the list and the tail say is exact.
 //
-// Rows of 248,320 fp32 logits, device time: one row 15 us (three launches, each a chain of latencies), 16 rows 36, 128 of mixed settings 98, 256 open ones
+// Rows of 248,320 fp32 logits, device time: one row 15 us (three launches, each a chain of latencies), 16 rows 36, 128 of mixed settings 93, 256 open ones
 // 128: plan 10, stream 70 (254 MB: 3.6 TB/s; a number takes about ten instructions, which bound it before the memory does, and a row's end 13 us), wide 30
 // to 60.
 //
@@ -646,11 +646,12 @@ constexpr int STREAM_THREADS = 256, STREAM_WARPS = STREAM_THREADS / 32, STREAM_P
 constexpr int TASK = 1024;          // tokens that a warp adds up by itself, in two halves
 constexpr int LIST_K = 1024;        // top-k up to which a list is expected to hold the k tokens
 
-// What a list is made to hold: all of the k, with room for the guess's error (one part in sqrt(want * 16384 / V)), or as many as leave room above.
+// What a list is made to hold: all of the k, with room for the guess's error (one part in sqrt(want * 16384 / V): of 248,320 tokens the sample has 11 for a k
+// of 20, and less than two of them stand among the k), or as many as leave room above. (2 k + 64: one row of 128 had too few, and took 25 us more.)
 __device__ __forceinline__ int list_want(bool greedy, int k) {
   if (greedy) return 48;
   if (k <= 0) return 1400;
-  return k <= 700 ? 2 * k + 64 : 1500;
+  return min(2 * k + 128, 1500);
 }
 
 // The settings of a row in a form that all CTAs agree on.
