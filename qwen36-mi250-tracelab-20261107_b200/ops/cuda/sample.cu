@@ -263,8 +263,11 @@ struct WidePart {  // a CTA's part of the row
 };
 struct WideScale {
   float m, floor, scale;  // maximum; below it no weight; bins per unit of m - x
+  float fall;             // powers of two by which weights fall from bin to bin
   double inv_t, step;
   __device__ __forceinline__ int bin(float x) const { return min(WIDE_BINS - 1, static_cast<int>((m - x) * scale)); }
+  // A bin's weights are at most 2^-lift, but for a rounding.
+  __device__ __forceinline__ int lift(int bin) const { return min(127, static_cast<int>(bin * fall)); }
 };
 
 // Largest and smallest over the cluster, in every CTA.
@@ -344,16 +347,17 @@ __device__ __forceinline__ double wide_before(WideShared& s, double v, uint32_t 
 }
 
 // The tokens that `place` gives a bin (none: -1) into this CTA's bins. A weight goes in as a whole number of 64 bits, of which as many are left free as the
-// sum of this CTA's tokens needs: whole numbers add up to the same sum in any order. (2^14 tokens in multiples of 2^-50 of the largest weight, 2^18 in
-// multiples of 2^-46. Two words, the first one's carry goes with the second: three words of 18 bits each took 15.5 thousand tokens 18,000 cycles.)
+// sum of this CTA's tokens needs: whole numbers add up to the same sum in any order. (2^14 tokens in multiples of 2^-49 of a bin's largest weight, 2^18 in
+// multiples of 2^-45, so that as many of the largest weight add up to 2^63. `whole`: the bin that all of these are parts of, -1: they are the row's. Multiples of
+// the row's largest weight instead of the bin's moved draws that lie among tokens of 1e-11 of it. Two words, the first one's carry goes with the second: three words of 18 bits each took 15.5 thousand tokens 18,000 cycles.)
 template <typename T, typename F>
-__device__ __forceinline__ void wide_tally(const WidePart<T>& part, const WideScale& c, double power, bool counts, F place) {
+__device__ __forceinline__ void wide_tally(const WidePart<T>& part, const WideScale& c, double power, bool counts, int whole, F place) {
   WideShared& s = part.s;
   for (int b = threadIdx.x; b < WIDE_BINS * (1 + WIDE_WORDS); b += WIDE_THREADS) s.bins.count[b] = 0;  // (and the masses behind the counts)
   __syncthreads();
   const ExpLanes exps(power);
-  const double one = part.held ? 0x1p50 : 0x1p46, m = c.m;
-  static_assert(WIDE_HELD <= 1 << 14 && SAMPLE_MAX_VOCAB / WIDE_CTAS <= 1 << 18, "no sum runs over");
+  const double one = part.held ? 0x1p49 : 0x1p45, m = c.m;
+  static_assert(WIDE_HELD <= 1 << 14 && SAMPLE_MAX_VOCAB / WIDE_CTAS <= 1 << 18, "no sum runs over: it stays below 2^64");
   part.each([&](float x, int i) {
     double w = exps.add(0.0, (static_cast<double>(x) - m) * c.step);
     if (x < c.floor) w = 0.0;
@@ -361,7 +365,8 @@ __device__ __forceinline__ void wide_tally(const WidePart<T>& part, const WideSc
     const int b = x == -INFINITY ? -1 : place(x, i);
     if (b < 0) return;
     if (counts) atomicAdd(&s.bins.count[b], 1u);
-    const unsigned long long f = __double2ull_rn(w * one);
+    const int lift = c.lift(whole < 0 ? b : whole);
+    const unsigned long long f = __double2ull_rn(w * one * __hiloint2double((1023 + lift) << 20, 0));
     const uint32_t low = static_cast<uint32_t>(f);
     uint32_t high = static_cast<uint32_t>(f >> 32);
     if (low) high += atomicAdd(&s.bins.mass[0][b], low) > ~low;
@@ -370,7 +375,7 @@ __device__ __forceinline__ void wide_tally(const WidePart<T>& part, const WideSc
 }
 
 // The CTAs' bins to sums up to each bin, in the first CTA.
-__device__ __noinline__ void wide_tabulate(WideShared& s, bool finer, bool held) {
+__device__ __noinline__ void wide_tabulate(WideShared& s, WideScale c, bool finer, int whole, bool held) {
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x;
   cluster.sync();
@@ -388,23 +393,24 @@ __device__ __noinline__ void wide_tabulate(WideShared& s, bool finer, bool held)
   if (tid < OWN) {
     WideTable* table = cluster.map_shared_rank(finer ? &s.finer : &s.first, 0);
     table->count[b] = static_cast<uint32_t>(s.sums[0][tid]);
-    table->mass[b] = (static_cast<double>(s.sums[2][tid]) * 0x1p32 + static_cast<double>(s.sums[1][tid])) * (held ? 0x1p-50 : 0x1p-46);
+    const double unit = (held ? 0x1p-49 : 0x1p-45) * __hiloint2double((1023 - c.lift(whole < 0 ? b : whole)) << 20, 0);
+    table->mass[b] = (static_cast<double>(s.sums[2][tid]) * 0x1p32 + static_cast<double>(s.sums[1][tid])) * unit;
   }
   cluster.sync();
   if (cluster_rank() != 0) return;
   constexpr int PER = WIDE_BINS / WIDE_THREADS;
   WideTable& t = finer ? s.finer : s.first;
-  uint32_t c[PER];
+  uint32_t n[PER];
   double v[PER];
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
-    c[j] = t.count[tid * PER + j] + (j ? c[j - 1] : 0u);
+    n[j] = t.count[tid * PER + j] + (j ? n[j - 1] : 0u);
     v[j] = t.mass[tid * PER + j] + (j ? v[j - 1] : 0.0);
   }
   uint32_t before_c = 0;
-  const double before = wide_before(s, v[PER - 1], c[PER - 1], &before_c);
+  const double before = wide_before(s, v[PER - 1], n[PER - 1], &before_c);
 #pragma unroll
-  for (int j = 0; j < PER; ++j) { t.count[tid * PER + j] = before_c + c[j]; t.mass[tid * PER + j] = before + v[j]; }
+  for (int j = 0; j < PER; ++j) { t.count[tid * PER + j] = before_c + n[j]; t.mass[tid * PER + j] = before + v[j]; }
   __syncthreads();
 }
 
@@ -483,11 +489,11 @@ __device__ __noinline__ void wide_search(WidePart<T> part, WideScale c, double p
     range_lo = low; range_hi = top;
     while (members > LIST) {
       const int bits = 64 - __clzll(range_hi - range_lo), shift = max(0, bits - 11);
-      wide_tally(part, c, power, true, [&](float x, int i) {
+      wide_tally(part, c, power, true, bin, [&](float x, int i) {
         const uint64_t comp = comp_of(x, i);
         return c.bin(x) == bin && comp >= range_lo && comp <= range_hi ? static_cast<int>((range_hi - comp) >> shift) : -1;
       });
-      wide_tabulate(s, true, part.held);
+      wide_tabulate(s, c, true, bin, part.held);
       wide_find(s, true, by_count, rank_target, target, s.base_count, s.base_mass);
       members = s.members;
       range_hi -= static_cast<uint64_t>(s.bin) << shift;
@@ -580,8 +586,9 @@ __device__ __forceinline__ void sample_wide_row(const SampleArgs& a, const Sampl
   c.floor = fmaxf(c.m - WIDE_RANGE * temperature, -FLT_MAX);
   const float range = fminf(fminf(WIDE_RANGE * temperature, c.m - comp_value(low)), 1e38f);
   c.scale = range > 0.f ? fminf(WIDE_BINS / range, 1e38f) : 0.f;
-  wide_tally(part, c, power, cut_k, [&](float x, int) { return c.bin(x); });
-  wide_tabulate(s, false, part.held);
+  c.fall = c.scale > 0.f ? static_cast<float>(c.inv_t / c.scale * 1.4426950408889634) : 0.f;
+  wide_tally(part, c, power, cut_k, -1, [&](float x, int) { return c.bin(x); });
+  wide_tabulate(s, c, false, -1, part.held);
 
   uint64_t cut = 0;
   double total = s.first.mass[WIDE_BINS - 1];  // (the first CTA's numbers; nobody else uses them)

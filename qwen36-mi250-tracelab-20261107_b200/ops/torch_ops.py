@@ -593,7 +593,7 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor,
     do NaNs; a row with nothing but those gives -1. All in 64 bits: with a large vocabulary a draw decides between numbers 1e-9 apart."""
     n, V = logits.shape
     dev = logits.device
-    x = logits.double()
+    x = logits.double() + 0.0  # (-0 becomes 0, which a sort may tell apart)
     x = torch.where(x.isnan(), float("-inf"), x)
     if exclude is not None and exclude.shape[1]:
         ids = exclude.long()

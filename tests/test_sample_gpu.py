@@ -74,6 +74,30 @@ def test_a_row_of_equal_logits(C):
         _same(C, (torch.randint(0, 4, (n, V), device=DEV, generator=_gen(V)) * 0.5), _settings(ASKS, n, V + 1))
 
 
+@pytest.mark.parametrize("V", [1 << 18, (1 << 18) + 1, 1 << 22])
+def test_equal_logits_that_fill_every_part_of_the_search(C, V):
+    """2^14 and 2^18 tokens of the largest weight in each of 16 parts: their sums take all the bits that there are."""
+    asks = [(1.0, 0, 1.0, 0.0), (0.7, 0, 0.5, 0.0), (1.0, V - 1, 0.9, 0.0), (1.0, 0, 1.0, 0.5)]
+    _same(C, torch.full((len(asks), V), -7.0, device=DEV), _settings(asks, len(asks), V))
+    x = torch.full((len(asks), V), 1.0, device=DEV)
+    x[:, V // 16 : V // 8] = 2.0
+    _same(C, x, _settings(asks, len(asks), V + 1))
+
+
+@pytest.mark.parametrize("V", [100003, 248320, 262145, 300001])
+def test_draws_among_tokens_of_little_weight(C, V):
+    """The last of the weight lies in thousands of equal tokens of 1e-11 of the largest one's: sums need their bits there as well."""
+    n = 40
+    asks = [(1.0, 0, 1.0, 0.0), (0.7, 0, 1.0, 0.0), (1.0, V - 1, 1.0, 0.0), (0.9, 0, 1.0, 1e-13)]
+    t, k, p, m, u = _settings(asks, n, V)
+    u = 1 - torch.arange(1, n + 1, device=DEV) * 2.0**-24
+    x = (torch.randn(n, V, device=DEV, generator=_gen(V)) * 2).round()
+    x[:, 17] = 30.0
+    for dtype in (torch.float32, torch.float16):
+        _same(C, x.to(dtype), (t, k, p, m, u))
+    _same(C, x + torch.rand(n, V, device=DEV, generator=_gen(V + 1)), (t, k, p, m, u))
+
+
 def test_few_distinct_values_in_a_large_vocabulary(C):
     n, V = 2 * len(ASKS), 120001
     g = _gen(3)
