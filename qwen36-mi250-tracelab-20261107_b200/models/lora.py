@@ -132,14 +132,24 @@ def _merge(adapters: list[_Adapter], layer: int, mods: list[tuple[str, int]], K:
     return LoraWeights(a.to(device, dtype), b.to(device, dtype), scale.to(device))
 
 
-def attach_adapters(weights: Weights, paths: dict[str, str]) -> list[str]:
-    """Load the adapters into ``weights``' layers (``LayerWeights.in_lora``, ``out_lora``); their names, in the order of their numbers."""
+def load_adapters(weights: Weights, paths: dict[str, str]) -> list[tuple[LoraWeights | None, LoraWeights | None]]:
+    """The adapters of every layer's input and output projection, numbered in the order of ``paths``. ``weights`` stay as they are: engines that
+    share them have adapters of their own."""
     if len(paths) > MAX_ADAPTERS:
         raise ValueError(f"{len(paths)} adapters, at most {MAX_ADAPTERS}")
     cfg = weights.config
     adapters = [read_adapter(p, cfg) for p in paths.values()]
+    layers = []
     for i, lw in enumerate(weights.layers):
         ins, outs = modules(cfg, lw.kind)
-        lw.in_lora = _merge(adapters, i, ins, cfg.hidden_size, "input", weights.device, weights.dtype)
-        lw.out_lora = _merge(adapters, i, outs, mixer_width(cfg, lw.kind), "output", weights.device, weights.dtype)
+        layers.append((_merge(adapters, i, ins, cfg.hidden_size, "input", weights.device, weights.dtype),
+                       _merge(adapters, i, outs, mixer_width(cfg, lw.kind), "output", weights.device, weights.dtype)))
+    return layers
+
+
+def attach_adapters(weights: Weights, paths: dict[str, str]) -> list[str]:
+    """Load the adapters into ``weights``' layers (``LayerWeights.in_lora``, ``out_lora``), for every ``Model`` that is made of them from then on;
+    their names, in the order of their numbers."""
+    for lw, pair in zip(weights.layers, load_adapters(weights, paths)):
+        lw.in_lora, lw.out_lora = pair
     return list(paths)

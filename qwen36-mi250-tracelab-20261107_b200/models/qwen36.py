@@ -102,7 +102,7 @@ class PackedBatch:
 
 class Model:
     def __init__(self, weights: Weights, num_pages: int, state_slots: int, ops=None,
-                 kv_dtype: torch.dtype | None = None, tp=None, ep=None, pp=None) -> None:
+                 kv_dtype: torch.dtype | None = None, tp=None, ep=None, pp=None, lora: list | None = None) -> None:
         """``weights`` may be one rank's shard (``parallel.tp.shard_weights``); then ``tp`` names the rank
         group and every mixer / MoE output is summed across it. ``ep`` (a ``parallel.ep.EpMoE``) selects data-parallel
         attention with expert-parallel MoE instead: this rank serves its own rows with full dense weights, holds only
@@ -110,13 +110,16 @@ class Model:
         every MoE block, so all ranks must run their forward passes in step. ``pp`` (a ``parallel.pp.PPContext``) marks
         ``weights`` as one rank's run of layers (``parallel.pp.split_layers``): the pass receives its input rows from the
         rank before and hands its output to the rank after. ``kv_dtype``: the type of the paged KV pool, the activations' by default;
-        ``torch.float8_e4m3fn`` selects the 8-bit pool (``ops/kv8.py``), whose pages take half the memory and half the time to read."""
+        ``torch.float8_e4m3fn`` selects the 8-bit pool (``ops/kv8.py``), whose pages take half the memory and half the time to read.
+        ``lora``: the low-rank adapters of every layer's input and output projection (``models.lora.load_adapters``), by default those that the layers
+        carry at this moment; the model holds them itself, so that others over the same weights may have others or none."""
         self.tp = tp
         self.ep = ep
         self.pp = pp
-        # adapter of the sequence in each state slot, -1: none (``models/lora.py``); None: the weights have no adapters
+        # adapter of the sequence in each state slot, -1: none (``models/lora.py``); None: the model has no adapters
         self.slot_adapter = None
-        if any(lw.in_lora is not None or lw.out_lora is not None for lw in weights.layers):
+        self.lora = list(lora) if lora is not None else [(lw.in_lora, lw.out_lora) for lw in weights.layers]
+        if any(ad is not None for pair in self.lora for ad in pair):
             if tp is not None or ep is not None or pp is not None:
                 raise ValueError("adapters are served by replicas of one GPU")
             self.slot_adapter = torch.full((state_slots,), -1, dtype=torch.int32, device=weights.device)
@@ -252,19 +255,19 @@ class Model:
             return {"seg_starts": None, "seg_pos0": None, "meta": batch.meta.spans}
         return {"seg_starts": batch.seg_starts, "seg_pos0": batch.seg_pos0, "meta": batch.tables.spans}
 
-    def _attention(self, lw, kv_layer, h, batch: PackedBatch) -> torch.Tensor:
+    def _attention(self, lw, kv_layer, h, batch: PackedBatch, lora=(None, None)) -> torch.Tensor:
         cfg, ops = self.cfg, self.ops
-        qkv = self._project(h, lw.in_proj, lw.in_lora)
+        qkv = self._project(h, lw.in_proj, lora[0])
         core = ops.attention(
             qkv, batch.positions, batch.seq_of_row, batch.block_tables, kv_layer, lw.q_norm, lw.k_norm,
             cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim, cfg.rotary_dim, cfg.rope_theta,
             cfg.rms_norm_eps, batch.G, **self._attention_spans(batch),
         )
-        return self._out_proj(core, lw)
+        return self._out_proj(core, lw, lora[1])
 
-    def _gdn(self, lw, gi: int, h: torch.Tensor, batch: PackedBatch, ring) -> torch.Tensor:
+    def _gdn(self, lw, gi: int, h: torch.Tensor, batch: PackedBatch, ring, lora=(None, None)) -> torch.Tensor:
         cfg, ops = self.cfg, self.ops
-        mixed = self._project(h, lw.in_proj, lw.in_lora)
+        mixed = self._project(h, lw.in_proj, lora[0])
         args = (
             lw.conv_w, lw.A_log, lw.dt_bias, lw.gnorm_w, cfg.linear_num_key_heads, cfg.linear_num_value_heads,
             cfg.linear_key_head_dim, cfg.linear_value_head_dim, cfg.rms_norm_eps,
@@ -276,16 +279,16 @@ class Model:
             r = None if ring is None else (ring[0][gi], ring[1][gi])
             behind = {"behind_projection": True} if getattr(ops, "GDN_BEHIND_PROJECTION", False) else {}
             core = ops.gdn_decode(mixed, batch.slots, conv, rec, *args, G=batch.G, ring=r, **behind)
-        return self._out_proj(core, lw)
+        return self._out_proj(core, lw, lora[1])
 
     def _project(self, x: torch.Tensor, w: torch.Tensor, lora) -> torch.Tensor:
         """A projection of the pass's rows, with the adapter of each row's own request beside it where the layer has adapters."""
         return self.ops.linear(x, w) if lora is None else self.ops.lora_linear(x, w, lora, self._rows)
 
-    def _out_proj(self, core: torch.Tensor, lw: LayerWeights) -> torch.Tensor:
+    def _out_proj(self, core: torch.Tensor, lw: LayerWeights, lora) -> torch.Tensor:
         """Mixer output projection; under tensor parallelism the GEMM's epilogue is the all-reduce."""
         if self.tp is None:
-            return self._project(core, lw.out_proj, lw.out_lora)
+            return self._project(core, lw.out_proj, lora)
         return self.tp.comm.gemm_allreduce(self.ops, core, lw.out_proj)
 
     def _moe_norm(self, lw: LayerWeights, h: torch.Tensor, res: torch.Tensor, norm_w: torch.Tensor):
@@ -311,14 +314,14 @@ class Model:
                                  residual=res, norm_w=norm_w, eps=cfg.rms_norm_eps)
         return ops.add_rmsnorm(self._moe(lw, h), res, norm_w, cfg.rms_norm_eps)
 
-    def _layer(self, lw, h, res, batch, next_norm, kv_layer=None, gi=None, ring=None):
+    def _layer(self, lw, h, res, batch, next_norm, kv_layer=None, gi=None, ring=None, lora=(None, None)):
         """One decoder layer from its normed input ``h`` and the residual stream ``res``; returns the new residual
         and the input of the next layer, already normed with ``next_norm``."""
         cfg, ops = self.cfg, self.ops
         if lw.kind == "linear_attention":
-            mix = self._gdn(lw, gi, h, batch, ring)
+            mix = self._gdn(lw, gi, h, batch, ring, lora)
         else:
-            mix = self._attention(lw, kv_layer, h, batch)
+            mix = self._attention(lw, kv_layer, h, batch, lora)
         res, h = ops.add_rmsnorm(mix, res, lw.post_norm, cfg.rms_norm_eps)
         return self._moe_norm(lw, h, res, next_norm)
 
@@ -410,10 +413,11 @@ class Model:
                 res, h = ops.add_rmsnorm(ops.embed(batch.tokens, self.w.embed), None, layers[0].input_norm, cfg.rms_norm_eps)
         for i, lw in enumerate(layers):
             nxt = layers[i + 1].input_norm if i + 1 < len(layers) else self.w.final_norm
+            lora = self.lora[i] if self.slot_adapter is not None else (None, None)
             if lw.kind == "linear_attention":
-                res, h = self._layer(lw, h, res, batch, nxt, gi=self._gdn_index[i], ring=ring)
+                res, h = self._layer(lw, h, res, batch, nxt, gi=self._gdn_index[i], ring=ring, lora=lora)
             else:
-                res, h = self._layer(lw, h, res, batch, nxt, kv_layer=self.kv[self._kv_index[i]])
+                res, h = self._layer(lw, h, res, batch, nxt, kv_layer=self.kv[self._kv_index[i]], lora=lora)
         if pp is not None and not pp.is_last:
             pp.send(res, h)  # normed with the next rank's first input norm (carried in final_norm)
         return h

@@ -71,14 +71,17 @@ class Engine:
         c = self.cfg
         if c.kv_dtype not in KV_DTYPES:
             raise ValueError(f"kv_dtype {c.kv_dtype!r} is none of {', '.join(KV_DTYPES)}")
-        # Low-rank adapters: name -> number. They lie in the layers' weights, which ``attach_adapters`` may have done ahead of the engine.
+        # Low-rank adapters: name -> number. The model holds them, not the weights, which other engines may share.
         self.adapters: dict[str, int] = {}
+        lora: list = []
         if c.adapters:
-            from ..models.lora import attach_adapters, parse_adapters
+            from ..models.lora import load_adapters, parse_adapters
 
             if tp is not None or ep is not None or pp is not None:
                 raise ValueError("adapters are served by replicas of one GPU")
-            self.adapters = {name: i for i, name in enumerate(attach_adapters(weights, parse_adapters(c.adapters)))}
+            paths = parse_adapters(c.adapters)
+            lora = load_adapters(weights, paths)
+            self.adapters = {name: i for i, name in enumerate(paths)}
         self.chunk = max(PAGE_SIZE, (c.prefill_chunk_tokens + PAGE_SIZE - 1) // PAGE_SIZE * PAGE_SIZE)
         self.max_model_len = c.max_model_len
         self.max_pages_per_seq = (self.max_model_len + PAGE_SIZE - 1) // PAGE_SIZE + 1
@@ -94,7 +97,7 @@ class Engine:
             self.ops.pack_weights(weights)  # before the KV pool is sized: padded copies replace a few tensors
         n_slots = c.state_slots or (c.max_seqs * 2 + 2)
         n_pages = c.kv_pages or self._agree_min(self._auto_pages(weights, n_slots), tp if tp is not None else pp)
-        self.model = Model(weights, n_pages, n_slots, ops=self.ops, tp=tp, ep=ep, pp=pp, kv_dtype=KV_DTYPES[c.kv_dtype])
+        self.model = Model(weights, n_pages, n_slots, ops=self.ops, tp=tp, ep=ep, pp=pp, kv_dtype=KV_DTYPES[c.kv_dtype], lora=lora)
         self.model.draft_index = draft_index
         self.pages = PagePool(n_pages)
         self.slots = SlotPool(n_slots)

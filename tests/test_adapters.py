@@ -252,3 +252,29 @@ def test_the_server_serves_adapters_as_models(dirs):
     finally:
         server.shutdown()
         service.worker.stop()
+
+
+@pytest.mark.parametrize("graphs", [False, True])
+def test_engines_over_one_set_of_weights_keep_apart(dirs, graphs):
+    """Adapters belong to the engine that was given them: others over the same weights, made before or after, run with their own or with none."""
+    paths, _, _ = dirs
+    kw = dict(graphs_on_cpu=True, decode_buckets=(1, 4)) if graphs else dict(cuda_graphs=False)
+    prompts, s = _prompts(2, 11), Sampling(max_tokens=6, ignore_eos=True)
+
+    def ask(eng, name):
+        eng.cache.clear()
+        return [g.output for g in eng.generate(prompts, s, adapters=[name] * 2)]
+
+    want = {n: ask(_engine(_weights(), f"x={paths[n]}" if n else "", **kw), "x" if n else None) for n in ("all", "root", None)}
+    w = _weights()
+    made = []
+    for name in (None, "all", "root", None):
+        made.append((_engine(w, f"x={paths[name]}" if name else "", **kw), name))
+        for eng, own in made:  # (every engine that is there, after each new one)
+            assert ask(eng, "x" if own else None) == want[own]
+            assert ask(eng, None) == want[None]
+    assert all(lw.in_lora is None and lw.out_lora is None for lw in w.layers)
+    # adapters attached to the weights are those of the models made from then on, and of no engine
+    model = made[1][0].model
+    attach_adapters(w, {"narrow": paths["narrow"]})
+    assert made[1][0].model is model and ask(made[1][0], "x") == want["all"] and ask(_engine(w, **kw), None) == want[None]
