@@ -22,6 +22,13 @@ from .checkpoint import Weights
 
 _NAME = re.compile(r"^(?:.*\.)?layers\.(\d+)\.((?:self_attn|linear_attn)\.\w+)\.lora_([AB])(?:\.default)?\.weight$")
 
+# The keys of a configuration that may be set: those read here, and those that change neither the formula nor which weights it is added to. Any
+# other one that is set, of this format's later versions too, stands for something else than a plain low-rank product.
+_PLAIN = frozenset(("peft_type", "r", "lora_alpha", "use_rslora", "bias", "init_lora_weights", "auto_mapping", "base_model_name_or_path", "revision",
+                    "inference_mode", "task_type", "lora_dropout", "target_modules", "exclude_modules", "layers_to_transform", "layers_pattern", "eva_config",
+                    "megatron_core", "qalora_group_size", "runtime_config", "peft_version"))
+_PLAIN_INIT = frozenset(("gaussian", "eva", "orthogonal"))  # starting points that leave the base weights alone
+
 
 def modules(cfg: ModelConfig, kind: str) -> tuple[list[tuple[str, int]], list[tuple[str, int]]]:
     """``(name, outputs)`` of the modules in a layer's input projection, in its order, and in its output projection."""
@@ -64,9 +71,12 @@ def read_adapter(path: str | Path, cfg: ModelConfig) -> _Adapter:
         state = load_file(str(path / "adapter_model.safetensors"))
     except OSError as e:
         raise ValueError(f"adapter {path}: {e}") from None
-    for key in ("use_dora", "modules_to_save", "rank_pattern", "alpha_pattern", "trainable_token_indices"):
-        if conf.get(key):
+    for key, value in conf.items():
+        if value and key not in _PLAIN:
             raise ValueError(f"adapter {path}: {key} is not supported")
+    init = conf.get("init_lora_weights")
+    if not (init is None or isinstance(init, bool) or isinstance(init, str) and init in _PLAIN_INIT):
+        raise ValueError(f"adapter {path}: init_lora_weights {init!r}, which may belong to other base weights, is not supported")
     if conf.get("peft_type", "LORA") != "LORA" or conf.get("bias", "none") != "none":
         raise ValueError(f"adapter {path}: a {conf.get('peft_type')} adapter with bias {conf.get('bias')!r} is not supported")
     found: dict[tuple[int, str], dict[str, torch.Tensor]] = {}

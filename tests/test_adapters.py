@@ -278,3 +278,32 @@ def test_engines_over_one_set_of_weights_keep_apart(dirs, graphs):
     model = made[1][0].model
     attach_adapters(w, {"narrow": paths["narrow"]})
     assert made[1][0].model is model and ask(made[1][0], "x") == want["all"] and ask(_engine(w, **kw), None) == want[None]
+
+
+# (what PEFT writes for an ordinary adapter, defaults of its newer versions among them)
+_USUAL = dict(alpha_pattern={}, arrow_config=None, auto_mapping=None, base_model_name_or_path="some/model", corda_config=None, ensure_weight_tying=False,
+              eva_config=None, exclude_modules=None, fan_in_fan_out=False, inference_mode=True, init_lora_weights=True, layer_replication=None, layers_pattern=None,
+              layers_to_transform=None, loftq_config={}, lora_bias=False, lora_dropout=0.05, megatron_config=None, megatron_core="megatron.core",
+              modules_to_save=None, peft_version="0.18.0", qalora_group_size=16, rank_pattern={}, revision=None, target_modules=["q_proj"],
+              target_parameters=None, task_type="CAUSAL_LM", trainable_token_indices=None, use_dora=False, use_qalora=False, use_rslora=False,
+              alora_invocation_tokens=None, a_later_switch=None)
+
+
+@pytest.mark.parametrize("conf", [
+    {"alora_invocation_tokens": [5, 6]}, {"use_qalora": True}, {"layer_replication": [[0, 2], [1, 3]]}, {"target_parameters": ["experts.w"]}, {"lora_bias": True},
+    {"fan_in_fan_out": True}, {"arrow_config": {"top_k": 3}}, {"megatron_config": {"x": 1}}, {"loftq_config": {"loftq_bits": 4}}, {"a_later_switch": True},
+    {"corda_config": {"x": 1}}, *({"init_lora_weights": v} for v in ("pissa", "pissa_niter_16", "olora", "corda", "loftq", "something", 1, ["gaussian"]))])
+def test_adapters_of_another_kind_are_refused(tmp_path, conf):
+    """What is not known to leave the formula and the base weights as they are is refused, not read as a plain adapter."""
+    cfg = ModelConfig.tiny()
+    write_adapter(tmp_path / "a", cfg, 0, **{**_USUAL, **conf})
+    with pytest.raises(ValueError, match=f"adapter .*{next(iter(conf))}"):
+        read_adapter(tmp_path / "a", cfg)
+
+
+@pytest.mark.parametrize("init", [True, False, None, "gaussian", "eva", "orthogonal"])
+def test_usual_configurations_are_read(tmp_path, init):
+    cfg = ModelConfig.tiny()
+    parts = write_adapter(tmp_path / "a", cfg, 0, **{**_USUAL, "init_lora_weights": init, "eva_config": {"rho": 2.0} if init == "eva" else None})
+    got = read_adapter(tmp_path / "a", cfg)
+    assert got.scale == 2.0 and got.parts.keys() == parts.keys()
