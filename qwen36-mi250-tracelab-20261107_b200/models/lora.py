@@ -20,7 +20,8 @@ from ..config import ModelConfig
 from ..ops.lora import MAX_ADAPTERS, MAX_RANK, RANK_STEP, LoraWeights
 from .checkpoint import Weights
 
-_NAME = re.compile(r"^(?:.*\.)?layers\.(\d+)\.((?:self_attn|linear_attn)\.\w+)\.lora_([AB])(?:\.default)?\.weight$")
+# (a draft block, or an encoder beside the text model, has layers of its own, under other names)
+_NAME = re.compile(r"^(?:(?:base_model|model|language_model)\.)*layers\.(\d+)\.((?:self_attn|linear_attn)\.\w+)\.lora_([AB])(?:\.default)?\.weight$")
 
 # The keys of a configuration that may be set: those read here, and those that change neither the formula nor which weights it is added to. Any
 # other one that is set, of this format's later versions too, stands for something else than a plain low-rank product.
@@ -89,7 +90,10 @@ def read_adapter(path: str | Path, cfg: ModelConfig) -> _Adapter:
             known = module in dict(ins + outs)
         if not known:
             raise ValueError(f"adapter {path}: {name} is of no module that can have one")
-        found.setdefault((layer, module), {})[m.group(3)] = t
+        part = found.setdefault((layer, module), {})
+        if m.group(3) in part:
+            raise ValueError(f"adapter {path}: {name} gives layer {layer} {module} lora_{m.group(3)} twice")
+        part[m.group(3)] = t
     if not found:
         raise ValueError(f"adapter {path}: it holds nothing")
     r = int(conf.get("r", 0))

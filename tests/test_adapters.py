@@ -307,3 +307,46 @@ def test_usual_configurations_are_read(tmp_path, init):
     parts = write_adapter(tmp_path / "a", cfg, 0, **{**_USUAL, "init_lora_weights": init, "eva_config": {"rho": 2.0} if init == "eva" else None})
     got = read_adapter(tmp_path / "a", cfg)
     assert got.scale == 2.0 and got.parts.keys() == parts.keys()
+
+
+def _with_state(path, edit):
+    from safetensors.torch import load_file, save_file
+
+    f = str(path / "adapter_model.safetensors")
+    state = load_file(f)
+    edit(state)
+    save_file(state, f)
+
+
+@pytest.mark.parametrize("prefix", ["mtp", "base_model.model.mtp", "base_model.model.model.visual", "base_model.model.model.layers.1.sub"])
+def test_other_stacks_of_layers_are_not_the_models(tmp_path, prefix):
+    """The draft block has a layer 0 as well: its adapter is not one of the model's first layer."""
+    cfg = ModelConfig.tiny()
+    write_adapter(tmp_path / "a", cfg, 0)
+    _with_state(tmp_path / "a", lambda s: s.update({f"{prefix}.layers.0.linear_attn.out_proj.lora_A.weight": torch.ones(4, cfg.gdn_value_dim),
+                                                    f"{prefix}.layers.0.linear_attn.out_proj.lora_B.weight": torch.ones(cfg.hidden_size, 4)}))
+    with pytest.raises(ValueError, match="no module"):
+        read_adapter(tmp_path / "a", cfg)
+
+
+@pytest.mark.parametrize("prefix", ["", "model.", "model.language_model.", "base_model.model.", "base_model.model.model.", "base_model.model.model.language_model.",
+                                    "base_model.model.language_model.model."])
+def test_names_of_the_models_layers(tmp_path, prefix):
+    cfg = ModelConfig.tiny()
+    parts = write_adapter(tmp_path / "a", cfg, 0)
+
+    def rename(s):
+        for k in list(s):
+            s[prefix + k[k.index("layers."):].replace("lora_A.weight", "lora_A.default.weight" if "model.l" in prefix else "lora_A.weight")] = s.pop(k)
+
+    _with_state(tmp_path / "a", rename)
+    got = read_adapter(tmp_path / "a", cfg).parts
+    assert got.keys() == parts.keys() and all(torch.equal(got[k][i], parts[k][i]) for k in parts for i in (0, 1))
+
+
+def test_a_module_is_given_once(tmp_path):
+    cfg = ModelConfig.tiny()
+    write_adapter(tmp_path / "a", cfg, 0)
+    _with_state(tmp_path / "a", lambda s: s.update({"layers." + k.split(".layers.")[1]: v + 1 for k, v in list(s.items())[:1]}))
+    with pytest.raises(ValueError, match="twice"):
+        read_adapter(tmp_path / "a", cfg)
