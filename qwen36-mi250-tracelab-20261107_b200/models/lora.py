@@ -64,14 +64,17 @@ class _Adapter:
 
 def read_adapter(path: str | Path, cfg: ModelConfig) -> _Adapter:
     """One adapter directory, refused where it asks for what this engine does not do."""
+    from safetensors import SafetensorError
     from safetensors.torch import load_file
 
     path = Path(path)
     try:
         conf = json.loads((path / "adapter_config.json").read_text())
         state = load_file(str(path / "adapter_model.safetensors"))
-    except OSError as e:
+    except (OSError, ValueError, SafetensorError) as e:
         raise ValueError(f"adapter {path}: {e}") from None
+    if not isinstance(conf, dict):
+        raise ValueError(f"adapter {path}: its configuration is no object")
     for key, value in conf.items():
         if value and key not in _PLAIN:
             raise ValueError(f"adapter {path}: {key} is not supported")
@@ -80,6 +83,10 @@ def read_adapter(path: str | Path, cfg: ModelConfig) -> _Adapter:
         raise ValueError(f"adapter {path}: init_lora_weights {init!r}, which may belong to other base weights, is not supported")
     if conf.get("peft_type", "LORA") != "LORA" or conf.get("bias", "none") != "none":
         raise ValueError(f"adapter {path}: a {conf.get('peft_type')} adapter with bias {conf.get('bias')!r} is not supported")
+    r = conf.get("r")
+    alpha = conf.get("lora_alpha", r)
+    if type(r) is not int or r < 1 or type(alpha) not in (int, float):
+        raise ValueError(f"adapter {path}: rank {r!r} and alpha {alpha!r} are not a whole number from 1 on and a number")
     found: dict[tuple[int, str], dict[str, torch.Tensor]] = {}
     for name, t in state.items():
         m = _NAME.match(name)
@@ -96,7 +103,6 @@ def read_adapter(path: str | Path, cfg: ModelConfig) -> _Adapter:
         part[m.group(3)] = t
     if not found:
         raise ValueError(f"adapter {path}: it holds nothing")
-    r = int(conf.get("r", 0))
     parts = {}
     for (layer, module), ab in found.items():
         if set(ab) != {"A", "B"}:
@@ -111,7 +117,6 @@ def read_adapter(path: str | Path, cfg: ModelConfig) -> _Adapter:
         if not all(((t >= low) & (t <= high)).all() for t in (a, b)):
             raise ValueError(f"adapter {path}: layer {layer} {module} holds numbers that are not finite, or not in bf16")
         parts[layer, module] = (a, b)
-    alpha = float(conf.get("lora_alpha", r))
     scale = alpha / math.sqrt(r) if conf.get("use_rslora") else alpha / r
     if not abs(scale) <= torch.finfo(torch.float32).max:
         raise ValueError(f"adapter {path}: alpha {alpha}")

@@ -350,3 +350,28 @@ def test_a_module_is_given_once(tmp_path):
     _with_state(tmp_path / "a", lambda s: s.update({"layers." + k.split(".layers.")[1]: v + 1 for k, v in list(s.items())[:1]}))
     with pytest.raises(ValueError, match="twice"):
         read_adapter(tmp_path / "a", cfg)
+
+
+@pytest.mark.parametrize("conf", [{"r": 0}, {"r": -4}, {"r": None}, {"r": "four"}, {"r": 4.5}, {"r": True}, {"lora_alpha": None}, {"lora_alpha": "x"}, {"lora_alpha": [1]}])
+def test_numbers_of_a_configuration(tmp_path, conf):
+    cfg = ModelConfig.tiny()
+    write_adapter(tmp_path / "a", cfg, 0)
+    f = tmp_path / "a" / "adapter_config.json"
+    f.write_text(json.dumps({**json.loads(f.read_text()), **conf}))
+    if conf.get("r") == 0:
+        _with_state(tmp_path / "a", lambda s: s.update({k: v[:0].contiguous() if "lora_A" in k else v[:, :0].contiguous() for k, v in s.items()}))
+    with pytest.raises(ValueError, match="adapter"):
+        read_adapter(tmp_path / "a", cfg)
+
+
+@pytest.mark.parametrize("text", ["{", "[]", "3", "null", "\xff"])
+def test_broken_files(tmp_path, text):
+    cfg = ModelConfig.tiny()
+    write_adapter(tmp_path / "a", cfg, 0)
+    (tmp_path / "a" / "adapter_config.json").write_bytes(text.encode("latin-1"))
+    with pytest.raises(ValueError, match="adapter .*a"):
+        read_adapter(tmp_path / "a", cfg)
+    write_adapter(tmp_path / "b", cfg, 0)
+    (tmp_path / "b" / "adapter_model.safetensors").write_bytes(text.encode("latin-1") * 20)
+    with pytest.raises(ValueError, match="adapter .*b"):
+        read_adapter(tmp_path / "b", cfg)
