@@ -206,7 +206,9 @@ class Engine:
         """Offline convenience: run the given prompts (with the adapters of these names, if any) to completion and return their generations."""
         prompts = list(prompts)
         samplings = sampling if isinstance(sampling, list) else [sampling] * len(prompts)
-        adapters = adapters or [None] * len(prompts)
+        adapters = [None] * len(prompts) if adapters is None else adapters
+        if len(adapters) != len(prompts):
+            raise ValueError(f"{len(adapters)} adapters for {len(prompts)} prompts")
         gens = [self.submit(Generation(p, s, adapter=a)) for p, s, a in zip(prompts, samplings, adapters)]
         while any(not g.done for g in gens):
             self.step()

@@ -375,3 +375,16 @@ def test_broken_files(tmp_path, text):
     (tmp_path / "b" / "adapter_model.safetensors").write_bytes(text.encode("latin-1") * 20)
     with pytest.raises(ValueError, match="adapter .*b"):
         read_adapter(tmp_path / "b", cfg)
+
+
+def test_every_prompt_has_its_adapter(dirs):
+    """A list that is too short would leave requests out without a word."""
+    paths, _, _ = dirs
+    eng, s = _engine(_weights(), f"all={paths['all']}"), Sampling(max_tokens=2, ignore_eos=True)
+    prompts = [[5, 6], [7, 8], [9, 10]]
+    for adapters in (["all"], ["all", None], [None] * 4, []):
+        with pytest.raises(ValueError, match="adapters"):
+            eng.generate(prompts, s, adapters=adapters)
+    assert not eng.has_work()
+    assert [len(g.output) for g in eng.generate(iter(prompts), s, adapters=["all", None, "all"])] == [2, 2, 2]
+    assert eng.generate([], s, adapters=[]) == []
