@@ -590,7 +590,7 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor,
     first ``top_k`` (0: all), of those the ones before which at most ``top_p`` of their weight stands, of those the ones of weight ``min_p``
     at least; the pick is the first kept token up to which more than ``u`` (in ``[0, 1)``) of the kept weight stands. A row of temperature 0 picks
     the first token of the order. ``exclude [n, m]`` int32 names tokens that count as minus infinity (entries outside ``[0, V)`` name none), as
-    do NaNs; a row with nothing but those gives -1. All in 64 bits: with a large vocabulary a draw decides between numbers 1e-9 apart."""
+    do NaNs; a row with nothing but those gives -1. A NaN as ``top_p`` or ``min_p`` filters nothing. All in 64 bits: with a large vocabulary a draw decides between numbers 1e-9 apart."""
     n, V = logits.shape
     dev = logits.device
     x = logits.double() + 0.0  # (-0 becomes 0, which a sort may tell apart)
@@ -607,7 +607,7 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor,
     w.masked_fill_((k > 0) & (rank >= k), 0.0)
     cum = torch.cumsum(w, -1)
     p = top_p.double()[:, None]
-    keep = ((cum - w <= p * cum[:, -1:]) | (p >= 1)) & (w >= min_p.double()[:, None]) & (w > 0)
+    keep = ~((cum - w > p * cum[:, -1:]) & (p < 1)) & ~(w < min_p.double()[:, None]) & (w > 0)
     last = (keep.sum(-1, keepdim=True) - 1).clamp_(min=0)  # the kept tokens are the first ones
     at = (cum <= u.double()[:, None] * cum.gather(1, last)).sum(-1, keepdim=True)
     at = torch.minimum(at, last).masked_fill_(greedy[:, None], 0)

@@ -71,3 +71,16 @@ def test_pick_tokens_takes_every_setting():
     order = logits[0].argsort(descending=True).tolist()
     assert pick_tokens(logits, [Sampling()], [None], [set(order[:80])]) == [order[80]]
     assert pick_tokens(logits[:, :3], [Sampling()], [None], [{0, 1, 2}]) == [0]
+
+
+def test_settings_that_are_no_numbers_filter_nothing():
+    """A NaN as top-p or min-p, which no comparison holds for, leaves every token in."""
+    g = torch.Generator().manual_seed(3)
+    x, n = torch.randn(64, 50, generator=g), 64
+    u = torch.rand(n, generator=g)
+    one, zero, nan, k = torch.ones(n), torch.zeros(n), torch.full((n,), math.nan), torch.zeros(n, dtype=torch.int32)
+    want = torch_ops.sample(x, one, k, one, zero, u)
+    assert len(set(want.tolist())) > 20
+    for p, m in ((nan, zero), (one, nan), (nan, nan)):
+        assert torch.equal(torch_ops.sample(x, one, k, p, m, u), want)
+    assert torch.equal(torch_ops.sample(x, one, k + 7, nan, nan, u), torch_ops.sample(x, one, k + 7, one, zero, u))

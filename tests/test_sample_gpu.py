@@ -272,3 +272,11 @@ def test_refusals(C):
     for o in (torch.zeros(3, device=DEV), torch.zeros(2, dtype=torch.int64, device=DEV), torch.zeros(6, dtype=torch.int64, device=DEV)[::2]):
         with pytest.raises(ValueError, match="out"):
             C.sample(x, *s, out=o)
+
+
+@pytest.mark.parametrize("V", [900, 60000])
+def test_settings_that_are_no_numbers(C, V):
+    asks = [(1.0, 0, math.nan, 0.0), (1.0, 0, 1.0, math.nan), (0.7, 30, math.nan, math.nan), (math.nan, 0, 1.0, 0.0), (1.5, 0, 0.9, math.nan), (1.0, 0, math.nan, 0.1)]
+    got = _same(C, _logits(60, V, V), _settings(asks, 60, V))
+    filters_off = [(t, k, 1.0 if math.isnan(p) else p, 0.0 if math.isnan(m) else m) for t, k, p, m in asks]
+    assert torch.equal(got, C.sample(_logits(60, V, V), *_settings(filters_off, 60, V)))
