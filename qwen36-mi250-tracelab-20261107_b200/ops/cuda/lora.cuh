@@ -10,7 +10,11 @@
 // K of 520; from K of 2,000 on those are off by more, 2e-6, and 4e-6 at 4,096.)
 #pragma once
 
+#ifdef B200_EMU  // host build of the walk over entries for tests/emu
+#include "emu_shim.h"
+#else
 #include "common.cuh"
+#endif
 
 namespace b200 {
 
@@ -51,7 +55,7 @@ struct LoraEntry {
     adapter = entries > 0 ? *next : 0;
     then = entries > x.chunks ? *++next : 0;
   }
-  __device__ __forceinline__ void step(const LoraExt& x, int left) {  // left: entries behind the one left
+  __device__ __forceinline__ void step(const LoraExt& x, int left) {  // left: entries behind the one that is left
     row += x.tile_rows;
     if (++part == x.parts) { part = 0; column += x.width; }
     if (++sub == x.chunks) {

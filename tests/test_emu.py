@@ -92,3 +92,13 @@ def test_expert_plan_of_more_pairs_and_wider_tiles_on_the_host(tmp_path, tsan):
     assert build.returncode == 0, build.stderr[-3000:]
     run = subprocess.run([str(exe)], capture_output=True, text=True, timeout=600)
     assert run.returncode == 0 and run.stdout.startswith("OK") and "ThreadSanitizer" not in run.stderr, run.stdout + run.stderr[-3000:]
+
+
+def test_adapter_entries_of_a_tile_on_the_host(tmp_path):
+    """``ops/cuda/lora.cuh``: the walk over a token tile's adapter entries, and that it ends with the tile's list."""
+    exe = tmp_path / "lora_entries_emu"
+    build = subprocess.run(["g++", "-std=c++20", "-O1", "-pthread", "-DB200_EMU", "-I", str(ROOT / "tests/emu"), "-x", "c++",
+                            str(ROOT / "tests/emu/lora_entries_emu.cpp"), "-o", str(exe)], capture_output=True, text=True, timeout=300)
+    assert build.returncode == 0, build.stderr[-3000:]
+    run = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and run.stdout.startswith("OK"), run.stdout[-3000:] + run.stderr
