@@ -592,26 +592,78 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor,
     the first token of the order. ``exclude [n, m]`` int32 names tokens that count as minus infinity (entries outside ``[0, V)`` name none), as
     do NaNs; a row with nothing but those gives -1. A NaN as ``top_p`` or ``min_p`` filters nothing. All in 64 bits: with a large vocabulary a draw decides between numbers 1e-9 apart."""
     n, V = logits.shape
-    dev = logits.device
-    x = logits.double() + 0.0  # (-0 becomes 0, which a sort may tell apart)
-    x = torch.where(x.isnan(), float("-inf"), x)
+    inf = float("inf")
+    x = torch.nan_to_num(logits if logits.dtype == torch.float64 else logits.float(), nan=-inf, posinf=inf, neginf=-inf)
+    x.add_(0.0)  # (-0 becomes 0, which a sort may tell apart)
     if exclude is not None and exclude.shape[1]:
         ids = exclude.long()
-        x = torch.cat([x, x.new_zeros(n, 1)], 1).scatter_(1, ids.where((ids >= 0) & (ids < V), V), float("-inf"))[:, :V]
-    x, ids = torch.sort(x, dim=-1, descending=True, stable=True)
-    top, greedy = x[:, :1], ~(temperature > 0)
-    y = (x - top) / torch.where(greedy, 1.0, temperature.double())[:, None]
-    w = torch.where(x == top, 1.0, torch.where(y <= 0, torch.exp(y), 0.0)).masked_fill_(x == float("-inf"), 0.0)
-    rank = torch.arange(V, device=dev)[None, :]
-    k = top_k.long()[:, None]
-    w.masked_fill_((k > 0) & (rank >= k), 0.0)
+        row, at = ((ids >= 0) & (ids < V)).nonzero(as_tuple=True)
+        x[row, ids[row, at]] = -inf
+    top, out = x.max(-1)  # (the first of equals)
+    out = out.masked_fill(top == -inf, -1)
+    k = torch.where((top_k <= 0) | (top_k > V), V, top_k.long())
+    asks = (temperature.double()[:, None], k[:, None], top_p.double()[:, None], min_p.double()[:, None], u.double()[:, None])
+    left = (temperature > 0) & (top > -inf)
+    # a row of a large vocabulary is mostly decided by its largest tokens: a short part of its order first, all of it for the rows that this leaves open
+    for width in (64, 2048) if V > 4096 else ():
+        now = (left & ((k < width) | (k == V) & (width > 64))).nonzero().view(-1)
+        if len(now):
+            picks = _draw_front(x[now], *(a[now] for a in asks), width)
+            sure = picks >= 0
+            out[now[sure]] = picks[sure]
+            left[now[sure]] = False
+    now = left.nonzero().view(-1)
+    if len(now) == n:
+        return _draw(x, *asks)
+    if len(now):
+        out[now] = _draw(x[now], *(a[now] for a in asks))
+    return out
+
+
+def _draw_weights(x: torch.Tensor, top: torch.Tensor, t: torch.Tensor) -> torch.Tensor:
+    """``exp((x - top) / t)`` in 64 bits for logits up to ``top``: 1 at it, 0 where the quotient is none (infinite numbers) and at minus infinity."""
+    y = (x.double() - top).div_(t)
+    return y.nan_to_num_(nan=float("-inf"), neginf=float("-inf")).exp_().masked_fill_(x == top, 1.0).masked_fill_(x == float("-inf"), 0.0)
+
+
+def _draw_kept(w, cum, total, p, m) -> torch.Tensor:
+    """Which tokens of an order top-p and min-p leave (the first ones), by their weights and these summed up."""
+    return ~((cum - w > p * total) & (p < 1)) & ~(w < m) & (w > 0)
+
+
+def _draw(x, t, k, p, m, u) -> torch.Tensor:
+    """The picks of rows that have tokens, by all of their order."""
+    v, ids = torch.sort(x, dim=-1, descending=True, stable=True)
+    v = v[:, : int(k.max())]
+    w = _draw_weights(v, v[:, :1], t).masked_fill_(torch.arange(v.shape[1], device=x.device) >= k, 0.0)
     cum = torch.cumsum(w, -1)
-    p = top_p.double()[:, None]
-    keep = ~((cum - w > p * cum[:, -1:]) & (p < 1)) & ~(w < min_p.double()[:, None]) & (w > 0)
-    last = (keep.sum(-1, keepdim=True) - 1).clamp_(min=0)  # the kept tokens are the first ones
-    at = (cum <= u.double()[:, None] * cum.gather(1, last)).sum(-1, keepdim=True)
-    at = torch.minimum(at, last).masked_fill_(greedy[:, None], 0)
-    return ids.gather(1, at)[:, 0].masked_fill_(top[:, 0] == float("-inf"), -1)
+    last = (_draw_kept(w, cum, cum[:, -1:], p, m).sum(-1, keepdim=True) - 1).clamp_(min=0)
+    at = (cum <= u * cum.gather(1, last)).sum(-1, keepdim=True)
+    return ids.gather(1, torch.minimum(at, last))[:, 0]
+
+
+def _draw_front(x, t, k, p, m, u, width: int) -> torch.Tensor:
+    """``_draw`` by the first ``width`` tokens of the order alone; -1 where they do not decide."""
+    V, inf = x.shape[1], float("inf")
+    v, ids = torch.topk(x, width, dim=-1, sorted=False)
+    ids, at = torch.sort(ids, dim=-1)
+    v, at = torch.sort(v.gather(1, at), dim=-1, descending=True, stable=True)
+    ids = ids.gather(1, at)
+    known = (v > v[:, -1:]) | (v[:, -1:] == -inf)  # (equals of the last one may be missing; behind minus infinity there is nothing)
+    n_known = known.sum(-1, keepdim=True)
+    w = _draw_weights(v, v[:, :1], t).masked_fill_(~known | (torch.arange(width, device=x.device) >= k), 0.0)
+    cum = torch.cumsum(w, -1)
+    total = cum[:, -1:].clone()
+    closed = (k <= n_known) | (v[:, -1:] == -inf)  # no other token is in play
+    for i in (~closed & (k == V)).view(-1).nonzero().view(-1).split(16):  # all tokens are: summed in the order of their ids, alike in any batch
+        total[i] = _draw_weights(x[i], v[i, :1], t[i]).cumsum_(-1)[:, -1:]
+    keep = _draw_kept(w, cum, total, p, m)
+    last = (keep.sum(-1, keepdim=True) - 1).clamp_(min=0)
+    ends = closed | (known & ~keep).any(-1, keepdim=True)  # the last kept one is among them
+    at = (known & (cum <= u * torch.where(ends, cum.gather(1, last), total))).sum(-1, keepdim=True)
+    sure = closed | (k == V) & (ends | ~(p < 1) & ~(m > 0) & (at < n_known))
+    at = torch.where(ends, torch.minimum(at, last), at.clamp(max=width - 1))
+    return ids.gather(1, at).masked_fill_(~sure, -1)[:, 0]
 
 
 def argmax_rows(logits: torch.Tensor) -> torch.Tensor:

@@ -84,3 +84,83 @@ def test_settings_that_are_no_numbers_filter_nothing():
     for p, m in ((nan, zero), (one, nan), (nan, nan)):
         assert torch.equal(torch_ops.sample(x, one, k, p, m, u), want)
     assert torch.equal(torch_ops.sample(x, one, k + 7, nan, nan, u), torch_ops.sample(x, one, k + 7, one, zero, u))
+
+
+def _pick64(row, t, k, p, m, u, exclude=()):
+    """The rules for a row of thousands, by the tokens that it has and sums in 64 bits."""
+    x = row.double().clone()
+    x[x.isnan()] = -math.inf
+    x[[i for i in exclude if 0 <= i < len(x)]] = -math.inf
+    ids = (x > -math.inf).nonzero().view(-1)
+    if not len(ids):
+        return -1
+    v, at = x[ids].sort(descending=True, stable=True)
+    ids = ids[at]
+    if not t > 0:
+        return int(ids[0])
+    w = torch.where(v == v[0], 1.0, torch.exp((v - v[0]) / t).nan_to_num(0.0))[: k if k > 0 else None]
+    cum = w.cumsum(0)
+    if p < 1:
+        w = w[cum - w <= p * cum[-1]]
+    w = w[(w >= m) & (w > 0)]
+    w = w if len(w) else torch.ones(1, dtype=torch.float64)
+    cum = w.cumsum(0)
+    return int(ids[min(int((cum <= u * cum[-1]).sum()), len(w) - 1)])
+
+
+def _random_asks(rng, n, V):
+    ask = [(rng.choice([0.0, 0.3, 1.0, 1.0, 2.5, 50.0, math.inf]), rng.choice([0, 0, 0, 1, 20, 63, 64, 65, 1000, 2047, 2048, V - 1, V, V + 1]),
+            rng.choice([1.0, 0.999, 0.9, 0.5, 1e-6, 0.0]), rng.choice([0.0, 0.0, 1e-4, 0.05, 1.0]), rng.random()) for _ in range(n)]
+    f = lambda v: torch.tensor(v, dtype=torch.float32)  # noqa: E731
+    t, k, p, m, u = (list(c) for c in zip(*ask))
+    return f(t), torch.tensor(k, dtype=torch.int32), f(p), f(m), f(u)
+
+
+@pytest.mark.parametrize("V", [63, 2049, 4096, 4097, 6001])
+def test_large_rows_are_the_rules(V):
+    """Rows longer than what is put in order at first: steep and flat ones, ties, whole blocks of minus infinity, excluded ids."""
+    rng, g = random.Random(V), torch.Generator().manual_seed(V)
+    n = 120
+    x = 12 - (torch.rand(n, 1, generator=g) * 3) * torch.log(torch.rand(n, V, generator=g) * V + 1)
+    x[::4] = x[::4].round()
+    x[1::8] = 0.0
+    x[2::16, 40:] = -math.inf
+    x[3::16, rng.randrange(V)] = math.inf
+    x[5::16, : V // 2] = math.nan
+    args = _random_asks(rng, n, V)
+    ban = torch.cat([x.nan_to_num(-1e9).argmax(-1, keepdim=True), torch.randint(-2, V + 2, (n, 3), generator=g)], 1).int()
+    as32 = list(zip(*(a.tolist() for a in args)))
+    for dtype in (torch.float32, torch.bfloat16, torch.float16, torch.float64):
+        y = x.to(dtype)
+        for exclude in (None, ban):
+            got = torch_ops.sample(y, *args, exclude=exclude).tolist()
+            want = [_pick64(y[i], *as32[i], () if exclude is None else ban[i].tolist()) for i in range(n)]
+            assert got == want, dtype
+        assert torch.equal(y.nan_to_num(7.5), x.to(dtype).nan_to_num(7.5))  # (the logits stay as they are)
+        alone = [int(torch_ops.sample(y[i : i + 1], *(a[i : i + 1] for a in args))[0]) for i in range(0, n, 7)]
+        assert alone == torch_ops.sample(y, *args)[::7].tolist()
+
+
+@pytest.mark.parametrize("ask", [(0.0, 0, 1.0, 0.0), (0.7, 20, 0.8, 0.0), (0.8, 50, 1.0, 0.05), (1.0, 1000, 0.95, 0.0), (0.7, 0, 0.9, 0.0), (1.0, 0, 1.0, 0.05)])
+def test_rows_that_need_no_order_of_the_vocabulary_do_without(ask, monkeypatch):
+    """The plain form puts as much of a row in order as decides it: a sort of every row's whole vocabulary took ten times as long."""
+    n, V = 4, 100000
+    g = torch.Generator().manual_seed(1)
+    x = 15 - 2 * torch.log(torch.rand(n, V, generator=g) * V + 1)
+    f = lambda v: torch.full((n,), v)  # noqa: E731
+    sorted_at_all, sort = [0], torch.sort
+
+    def counted(t, *args, **kw):
+        sorted_at_all[0] += t.numel()
+        return sort(t, *args, **kw)
+
+    args = (f(ask[0]), f(ask[1]).int(), f(ask[2]), f(ask[3]), torch.rand(n, generator=g) * 0.8)
+    ban = x.argmax(-1, keepdim=True).int()
+    for exclude in (None, ban):
+        monkeypatch.setattr(torch, "sort", counted)
+        got = torch_ops.sample(x, *args, exclude=exclude).tolist()
+        monkeypatch.setattr(torch, "sort", sort)
+        as32 = list(zip(*(a.tolist() for a in args)))
+        for i in range(n):
+            assert got[i] == _pick64(x[i], *as32[i], () if exclude is None else ban[i].tolist())
+    assert sorted_at_all[0] <= 2 * 2 * n * 2200
