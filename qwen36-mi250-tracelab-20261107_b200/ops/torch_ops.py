@@ -613,10 +613,8 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor,
             out[now[sure]] = picks[sure]
             left[now[sure]] = False
     now = left.nonzero().view(-1)
-    if len(now) == n:
-        return _draw(x, *asks)
     if len(now):
-        out[now] = _draw(x[now], *(a[now] for a in asks))
+        out[now] = _draw(x, *asks) if len(now) == n else _draw(x[now], *(a[now] for a in asks))
     return out
 
 

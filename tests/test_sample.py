@@ -164,3 +164,13 @@ def test_rows_that_need_no_order_of_the_vocabulary_do_without(ask, monkeypatch):
         for i in range(n):
             assert got[i] == _pick64(x[i], *as32[i], () if exclude is None else ban[i].tolist())
     assert sorted_at_all[0] <= 2 * 2 * n * 2200
+
+
+def test_no_rows():
+    from b200serve.sched.sampling import pick_tokens
+
+    for V in (1, 50, 5000):
+        e = torch.empty(0)
+        got = torch_ops.sample(torch.empty(0, V), e, e.int(), e, e, e, exclude=torch.empty(0, 2, dtype=torch.int32))
+        assert got.shape == (0,) and got.dtype == torch.int64
+        assert pick_tokens(torch.empty(0, V), [], [], []) == []
