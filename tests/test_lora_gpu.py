@@ -229,3 +229,35 @@ def test_refusals(C):
             C.lora_linear(*args)
     with pytest.raises(ValueError, match="outputs"):
         C.lora_linear(x, w, ad, rows, out_dtype=torch.float16)
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T", [257, 513, 1531])
+def test_a_call_cut_into_parts(C, monkeypatch, T, dt):
+    """A call whose workspace would be too large goes out by parts of its rows, with the bits of the whole; captured as well."""
+    L, R, cuts = 24, 40, []
+    part = C._lora_part
+    monkeypatch.setattr(C, "_lora_part", lambda *args: (cuts.append(args[5]), part(*args))[1])
+    for N, K in ((1003, 520), (2048, 1024), (12352, 512)):
+        w, ad = _bf(N, K, by=K ** -0.5, seed=N), _adapters(L, R, N, K, seed=T)
+        x = _bf(T, K + 24, seed=T)[:, 8 : 8 + K]
+        rows = _rows(T, L, T, run=2)
+        for weights in (w, C.pack_weight(w.clone())) if K % 64 == 0 else (w,):
+            monkeypatch.setattr(C, "LORA_WORK", 256 << 20)
+            del cuts[:]
+            whole = C.lora_linear(x, weights, ad, rows, out_dtype=dt)
+            assert cuts == [T]
+            monkeypatch.setattr(C, "LORA_WORK", 200 << 10)
+            cut = C.lora_linear(x, weights, ad, rows, out_dtype=dt)
+            ends = [n for n in cuts[1:] if n <= 256]  # (parts of up to 256 rows are not cut)
+            assert len(ends) == -(-T // 256) and sum(ends) == T
+            assert torch.equal(cut, whole)
+            _check(cut[:, :N], x, w, ad, rows, f"{T} rows in parts")
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                y = C.lora_linear(x, weights, ad, rows, out_dtype=dt)
+            y.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, whole)
+    C.check_errors(x.device)
