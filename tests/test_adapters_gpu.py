@@ -99,3 +99,24 @@ def test_adapters_against_the_cpu_path(spec):
     a, b = hidden
     # one layer: a dozen bf16 roundings (2^-9 each) between the adapters and the normed output, whose numbers are about 1
     assert (a - b).norm() / b.norm() < 12 * 2.0 ** -9
+
+
+@pytest.mark.parametrize("pack", [False, True])
+def test_engines_over_one_set_of_weights(spec, pack):
+    """Two engines with other adapters under one name, and one without, over the same weights: captured and eager passes of each go by its own."""
+    own = [f"x={part.split('=')[1]}" for part in spec.split(",")[:2]] + [""]
+    kw = dict(max_model_len=1024, prefill_chunk_tokens=64, max_seqs=8, mtp=False, kv_pages=256, decode_buckets=(1, 4, 8), pack_weights=pack)
+    prompts, s = _prompts(4, 7), Sampling(max_tokens=10, ignore_eos=True)
+
+    def ask(eng, name):
+        eng.cache.clear()
+        return [g.output for g in eng.generate(prompts, s, adapters=[name, None, name, name])]
+
+    want = [ask(_engine(a, pack_weights=pack), "x" if a else None) for a in own]
+    assert want[0] != want[1] != want[2]
+    w = random_weights(ModelConfig.tiny(), seed=0, device="cuda", dtype=torch.bfloat16, std=0.05, lm_head_std=0.5)
+    engines = []
+    for a in own:
+        engines.append(Engine(w, EngineConfig(**kw, adapters=a)))
+        for _ in range(2):
+            assert [ask(e, "x" if b else None) for e, b in zip(engines, own)] == want[: len(engines)]
