@@ -45,10 +45,13 @@ def pick_tokens(logits: torch.Tensor, samplings: list[Sampling], rngs: list, mas
     block = host.to(dev)
     t, p, m, u = block[: 4 * n].view(4, n)
     ints = block[4 * n :].view(torch.int32)
-    ops = torch_ops
+    args, exclude = (logits, t, ints[:n], p, m, u), ints[n:].view(n, most) if most else None
     if dev.type == "cuda":
-        from ..ops import cuda_ops as ops
-    picks = ops.sample(logits, t, ints[:n], p, m, u, exclude=ints[n:].view(n, most) if most else None)
+        from ..ops import cuda_ops
+
+        with torch.cuda.device(dev):  # (the kernels run on the current device)
+            return [max(0, i) for i in cuda_ops.sample(*args, exclude=exclude).tolist()]
+    picks = torch_ops.sample(*args, exclude=exclude)
     return [max(0, i) for i in picks.tolist()]
 
 

@@ -280,3 +280,21 @@ def test_settings_that_are_no_numbers(C, V):
     got = _same(C, _logits(60, V, V), _settings(asks, 60, V))
     filters_off = [(t, k, 1.0 if math.isnan(p) else p, 0.0 if math.isnan(m) else m) for t, k, p, m in asks]
     assert torch.equal(got, C.sample(_logits(60, V, V), *_settings(filters_off, 60, V)))
+
+
+def test_pick_tokens_goes_to_the_device_of_the_logits(C, monkeypatch):
+    """Logits of another device than the current one: the kernels run on theirs."""
+    from b200serve.sched import sampling
+    from b200serve.sched.request import Sampling
+
+    entered = []
+
+    class Device(torch.cuda.device):
+        def __enter__(self):
+            entered.append(self.idx)
+            super().__enter__()
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    x = _logits(3, 5000, 1)
+    assert sampling.pick_tokens(x, [Sampling()] * 3, [None] * 3, [None] * 3) == x.argmax(-1).tolist()
+    assert entered == [x.device.index]
