@@ -49,8 +49,9 @@ def pick_tokens(logits: torch.Tensor, samplings: list[Sampling], rngs: list, mas
     if dev.type == "cuda":
         from ..ops import cuda_ops
 
-        with torch.cuda.device(dev):  # (the kernels run on the current device)
-            return [max(0, i) for i in cuda_ops.sample(*args, exclude=exclude).tolist()]
+        if V <= cuda_ops.SAMPLE_VOCAB:  # (a larger vocabulary by the plain form)
+            with torch.cuda.device(dev):  # (the kernels run on the current device)
+                return [max(0, i) for i in cuda_ops.sample(*args, exclude=exclude).tolist()]
     picks = torch_ops.sample(*args, exclude=exclude)
     return [max(0, i) for i in picks.tolist()]
 

@@ -298,3 +298,19 @@ def test_pick_tokens_goes_to_the_device_of_the_logits(C, monkeypatch):
     x = _logits(3, 5000, 1)
     assert sampling.pick_tokens(x, [Sampling()] * 3, [None] * 3, [None] * 3) == x.argmax(-1).tolist()
     assert entered == [x.device.index]
+
+
+def test_pick_tokens_of_a_vocabulary_beyond_the_kernels(C):
+    from b200serve.sched.request import Sampling
+    from b200serve.sched.sampling import pick_tokens
+
+    V = C.SAMPLE_VOCAB + 3
+    x = _logits(3, V, 1)
+    asks = [Sampling(), Sampling(temperature=0.7, top_k=20, top_p=0.9, seed=1), Sampling(temperature=1.0, seed=2)]
+
+    def picks(x):
+        return pick_tokens(x, asks, [None, *(torch.Generator().manual_seed(s) for s in (1, 2))], [{int(x[0].argmax())}, None, None])
+
+    assert picks(x) == picks(x.cpu())
+    with pytest.raises(ValueError, match="sample"):
+        _same(C, x, _settings(ASKS, 3))
