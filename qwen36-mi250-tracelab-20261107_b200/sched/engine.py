@@ -760,12 +760,17 @@ class Engine:
         return did
 
     def warmup(self) -> None:
-        """Run one short request and capture every decode graph before serving, so that no request pays for
-        first-use work (the reference warms its kernels and captures its graphs before ``/health`` answers,
+        """Run a short greedy and a sampled request, draw tokens at every step size and capture every decode graph before serving, so that no request
+        pays for first-use work (the reference warms its kernels and captures its graphs before ``/health`` answers,
         ``engine/generator.py:706-728``). Counters and caches are reset afterwards."""
         n = min(self.chunk + 8, self.max_model_len - 8)
         g = self.generate([[1 + (i % 7) for i in range(n)]], Sampling(max_tokens=3, ignore_eos=True))[0]
         assert g.done
+        s = Sampling(max_tokens=3, temperature=1.0, seed=0, ignore_eos=True)
+        assert self.generate([[1] * 8], s)[0].done
+        for rows in sorted({min(b, self.cfg.max_seqs) for b in self.cfg.decode_buckets} | {self.cfg.max_seqs}):  # (the LM head's form goes by the rows)
+            logits = self.model.logits(torch.zeros(rows, self.mcfg.hidden_size, dtype=self.model.dtype, device=self.device))
+            pick_tokens(logits, [s] * rows, [torch.Generator().manual_seed(0)] * rows, [self.eos or None] * rows)
         if self._pgraphs is not None:
             self._pgraphs.warm()
         if self._graphs is not None:

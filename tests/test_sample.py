@@ -174,3 +174,21 @@ def test_no_rows():
         got = torch_ops.sample(torch.empty(0, V), e, e.int(), e, e, e, exclude=torch.empty(0, 2, dtype=torch.int32))
         assert got.shape == (0,) and got.dtype == torch.int64
         assert pick_tokens(torch.empty(0, V), [], [], []) == []
+
+
+@pytest.mark.parametrize("graphs", [False, True])
+def test_warmup_draws_tokens_of_every_step_size(graphs, monkeypatch):
+    """No request pays for the first use of what draws tokens: the LM head's logits and the draw, at every size that a step may have."""
+    from b200serve.config import EngineConfig, ModelConfig
+    from b200serve.models.checkpoint import random_weights
+    from b200serve.sched import engine as module
+
+    drawn, pick = [], module.pick_tokens
+    monkeypatch.setattr(module, "pick_tokens", lambda logits, *a: (drawn.append(logits.shape[0]), pick(logits, *a))[1])
+    w = random_weights(ModelConfig.tiny(), seed=0, dtype=torch.float32, std=0.05, lm_head_std=0.5)
+    eng = module.Engine(w, EngineConfig(max_model_len=256, prefill_chunk_tokens=64, max_seqs=6, mtp=False, decode_buckets=(1, 4, 8), graphs_on_cpu=graphs,
+                                        cuda_graphs=graphs))
+    eng.warmup()
+    assert set(drawn) == {1, 4, 6}
+    assert not any(eng.stats.values()) and len(eng.cache) == 0 and not eng.has_work() and not eng.running
+    assert eng.slots.free == eng.slots.num_slots - 1
