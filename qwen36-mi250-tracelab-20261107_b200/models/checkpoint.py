@@ -96,6 +96,9 @@ class Weights:
             kw = dict(lw.__dict__)
             for k, v in lw.tensors():
                 kw[k] = fn(k, v)
+            for k in ("in_lora", "out_lora"):
+                if kw[k] is not None:
+                    kw[k] = LoraWeights(fn(k, kw[k].a), fn(k, kw[k].b), fn("lora_scale", kw[k].scale))
             return LayerWeights(**kw)
 
         mtp = None
@@ -120,12 +123,12 @@ class Weights:
         )
 
     def to(self, device: torch.device | str | None = None, dtype: torch.dtype | None = None) -> "Weights":
-        """Move/cast. ``A_log`` and ``dt_bias`` stay fp32 whatever ``dtype`` is."""
+        """Move/cast. ``A_log``, ``dt_bias`` and adapters' factors stay fp32 whatever ``dtype`` is."""
 
         def fn(name: str, t: torch.Tensor) -> torch.Tensor:
             if not t.is_floating_point():
                 return t.to(device=device)
-            dt = torch.float32 if name in ("A_log", "dt_bias") else dtype
+            dt = torch.float32 if name in ("A_log", "dt_bias", "lora_scale") else dtype
             return t.to(device=device, dtype=dt)
 
         return self._map(fn)

@@ -388,3 +388,18 @@ def test_every_prompt_has_its_adapter(dirs):
     assert not eng.has_work()
     assert [len(g.output) for g in eng.generate(iter(prompts), s, adapters=["all", None, "all"])] == [2, 2, 2]
     assert eng.generate([], s, adapters=[]) == []
+
+
+def test_adapters_move_with_their_weights(dirs):
+    paths, _, _ = dirs
+    w = _weights()
+    bare = w.nbytes()
+    attach_adapters(w, {"all": paths["all"]})
+    pairs = [ad for lw in w.layers for ad in (lw.in_lora, lw.out_lora)]
+    assert w.nbytes() - bare == sum(t.numel() * t.element_size() for ad in pairs for t in ad)
+    moved = w.to(dtype=torch.bfloat16)
+    for lw, old in zip(moved.layers, w.layers):
+        for ad, was in ((lw.in_lora, old.in_lora), (lw.out_lora, old.out_lora)):
+            assert isinstance(ad, LoraWeights) and [t.dtype for t in ad] == [torch.bfloat16, torch.bfloat16, torch.float32]
+            assert torch.equal(ad.a, was.a.bfloat16()) and torch.equal(ad.b, was.b.bfloat16()) and torch.equal(ad.scale, was.scale)
+    assert {t.device.type for lw in w.to("meta").layers for t in (*lw.in_lora, *lw.out_lora)} == {"meta"}
