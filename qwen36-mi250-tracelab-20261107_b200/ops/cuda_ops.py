@@ -330,7 +330,9 @@ def _lora_refuse(x, w, adapters, rows, out_dtype) -> None:
 def lora_linear(x: torch.Tensor, w: torch.Tensor, adapters: LoraWeights, rows: torch.Tensor, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """``linear(x, w)`` with the low-rank adapter of each row's own request beside it (``ops/lora.py``): row ``t`` of ``x [T, K]`` uses adapter
     ``rows[t]`` (int32 ``[T]``), none where that is negative. One rounding, to bf16 (default) or fp32. A row's bits depend on its own numbers and
-    adapter only, and are ``linear``'s (without a split K) for a row without one. An adapter number that is too large leaves the row without one, and is
+    adapter only, and are ``linear``'s (without a split K) for a row without one. That asks for finite numbers in every adapter's ``b``, which the call does not look
+    at: the rows of a tile meet the ``b`` of the others' adapters with a factor of 0, and 0 times an infinity or a NaN is a NaN in all of them (an
+    adapter's ``a`` and ``scale``, and what stands in ``x``, reach their own rows alone). An adapter number that is too large leaves the row without one, and is
     reported by ``check_errors``. Only device tensors are touched, so the call can be captured in a CUDA graph."""
     a, b, scale = adapters
     (xs, ws, sa, sb), d, packed = (x.shape, w.shape, a.shape, b.shape), x.get_device(), is_packed(w)

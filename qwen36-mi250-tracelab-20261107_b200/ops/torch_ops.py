@@ -50,7 +50,6 @@ def linear(x: torch.Tensor, w: torch.Tensor, out_dtype: torch.dtype | None = Non
     return F.linear(x, w)
 
 
-# --------------------------------------------------------------------------- rope
 def lora_linear(x: torch.Tensor, w: torch.Tensor, adapters: LoraWeights, rows: torch.Tensor, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """``x w^T`` and, for a row ``t`` with an adapter (``rows[t] >= 0``), ``scale (x a^T) b^T`` of it, rounded once."""
     L, R = check_weights(adapters, w.shape[0], x.shape[1], "lora_linear")
@@ -61,6 +60,7 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, adapters: LoraWeights, rows: t
     return y.to(out_dtype or x.dtype)
 
 
+# --------------------------------------------------------------------------- rope
 def rope_cos_sin(positions: torch.Tensor, rotary_dim: int, theta: float):
     """cos/sin ``[T, rotary_dim/2]`` in fp32 for integer positions."""
     inv = 1.0 / (
