@@ -206,7 +206,7 @@ class Engine:
         """Offline convenience: run the given prompts (with the adapters of these names, if any) to completion and return their generations."""
         prompts = list(prompts)
         samplings = sampling if isinstance(sampling, list) else [sampling] * len(prompts)
-        adapters = [None] * len(prompts) if adapters is None else adapters
+        adapters = adapters or [None] * len(prompts)
         if len(adapters) != len(prompts):
             raise ValueError(f"{len(adapters)} adapters for {len(prompts)} prompts")
         gens = [self.submit(Generation(p, s, adapter=a)) for p, s, a in zip(prompts, samplings, adapters)]
@@ -768,7 +768,8 @@ class Engine:
         assert g.done
         s = Sampling(max_tokens=3, temperature=1.0, seed=0, ignore_eos=True)
         assert self.generate([[1] * 8], s)[0].done
-        for rows in sorted({min(b, self.cfg.max_seqs) for b in self.cfg.decode_buckets} | {self.cfg.max_seqs}):  # (the LM head's form goes by the rows)
+        most = min(self.cfg.max_seqs, 256)  # (the LM head's form goes by the rows, up to 256)
+        for rows in sorted({min(b, most) for b in self.cfg.decode_buckets} | {most}):
             logits = self.model.logits(torch.zeros(rows, self.mcfg.hidden_size, dtype=self.model.dtype, device=self.device))
             pick_tokens(logits, [s] * rows, [torch.Generator().manual_seed(0)] * rows, [self.eos or None] * rows)
         if self._pgraphs is not None:

@@ -382,12 +382,12 @@ def test_every_prompt_has_its_adapter(dirs):
     paths, _, _ = dirs
     eng, s = _engine(_weights(), f"all={paths['all']}"), Sampling(max_tokens=2, ignore_eos=True)
     prompts = [[5, 6], [7, 8], [9, 10]]
-    for adapters in (["all"], ["all", None], [None] * 4, []):
+    for adapters in (["all"], ["all", None], [None] * 4):
         with pytest.raises(ValueError, match="adapters"):
             eng.generate(prompts, s, adapters=adapters)
     assert not eng.has_work()
     assert [len(g.output) for g in eng.generate(iter(prompts), s, adapters=["all", None, "all"])] == [2, 2, 2]
-    assert eng.generate([], s, adapters=[]) == []
+    assert eng.generate([], s, adapters=[]) == [] and len(eng.generate(prompts, s, adapters=[])) == 3
 
 
 def test_adapters_move_with_their_weights(dirs):

@@ -192,3 +192,7 @@ def test_warmup_draws_tokens_of_every_step_size(graphs, monkeypatch):
     assert set(drawn) == {1, 4, 6}
     assert not any(eng.stats.values()) and len(eng.cache) == 0 and not eng.has_work() and not eng.running
     assert eng.slots.free == eng.slots.num_slots - 1
+    del drawn[:]
+    eng.cfg.max_seqs, eng.cfg.decode_buckets = 1000, (1, 512)  # (as many rows as its forms tell apart, not all that there may be)
+    eng.warmup()
+    assert set(drawn) == {1, 256}
