@@ -11,8 +11,8 @@
 //
 // The products are 16 x 8 x 16 instructions fed from global memory, in an order that is the same for one row and for 8,192. In a decode step the latency
 // of those reads bounds it, so a warp asks for a whole batch of pieces at a time (64 ranks, K of 4096: 78 us piece by piece, 22 in batches); with 256
-// threads and less than 13 KB of shared memory a CTA runs beside the GEMM's, which needs h behind its own k-blocks: the whole call takes 12.3 us for one row
-// of 9216 x 2048 where the projection alone takes 11.0, 22.4 and 11.6 for 128 rows of 32 adapters. In a long pass the rate of these instructions bounds
+// threads and less than 13 KB of shared memory a CTA runs beside the GEMM's, which needs h behind its own k-blocks: the whole call takes 12.7 us for one row
+// of 9216 x 2048 where the projection alone takes 11.0, 22.2 and 11.6 for 128 rows of 32 adapters. In a long pass the rate of these instructions bounds
 // it (about 144 TFLOP/s for its share of the tiles; 8,192 rows, K of 2048: 28 us at 16 ranks, 35 at 64; of the 28, 23 show beside the GEMM's 197).
 #include "lora.cuh"
 

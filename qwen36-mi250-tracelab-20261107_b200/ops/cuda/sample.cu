@@ -643,8 +643,8 @@ __global__ void __launch_bounds__(WIDE_THREADS) sample_wide_kernel(SampleArgs a,
 //  wide    the kernel above.
 // A guess that is off costs time, never a result: what the list and the tail say is exact.
 //
-// Rows of 248,320 fp32 logits, device time: one row 15 us (three launches, each a chain of latencies), 16 rows 36, 128 of mixed settings 93, 256 open ones
-// 128: plan 10, stream 70 (254 MB: 3.6 TB/s; a number takes about ten instructions, which bound it before the memory does, and a row's end 13 us), wide 30
+// Rows of 248,320 fp32 logits, device time: one row 15 us (three launches, each a chain of latencies), 16 rows 28, 128 of mixed settings 86, 256 open ones
+// 137: plan 10, stream 70 (254 MB: 3.6 TB/s; a number takes about ten instructions, which bound it before the memory does, and a row's end 13 us), wide 30
 // to 60.
 //
 // Sums are added up in an order that goes by V alone: the weights of a lane's tokens of a task, the lanes of a warp, the tasks of a row.
